@@ -8,9 +8,10 @@ LIB_PATH = os.environ.get("HIPSTER_B200_LIB") or os.path.join(HERE, "libhipster_
 HEADER = os.path.join(HERE, "..", "include", "hipster_b200.h")
 
 _lib = _hot = None
-# the calls whose latency counts, with their argument types (p pointer, i int, f float), so that integers pass without a wrapper object
-_TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float}
-_HOT = {"hp_quantize_x_q8": "piiippp", "hp_gemv_q4k_q8": "ppppiiiip", "hp_argmax": "piiipppp", "hp_accept_greedy": "ppipp", "hp_attn_decode": "piiiiiipppppipppfpp"}
+# the calls whose latency counts, with their argument types (p pointer, i int, l long long, f float), so that integers pass without a wrapper object
+_TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+_HOT = {"hp_quantize_x_q8": "piiippp", "hp_gemv_q4k_q8": "ppppiiiip", "hp_argmax": "piiipppp", "hp_accept_greedy": "ppipp", "hp_attn_decode": "piiiiiipppppipppfpp",
+        "hp_kv_append": "pllpllipllpllpppiiipippiipfp", "hp_kv_read": "pippiipppllp", "hp_attn_paged": "pllpllipippiiiipfiippppp"}
 
 
 class HipsterError(RuntimeError):
@@ -35,7 +36,7 @@ def lib():
             raise HipsterError(-1, f"{LIB_PATH} is missing: build it with `python -m hipster_b200.build` (needs nvcc); no fallback path exists")
         _lib = ctypes.CDLL(LIB_PATH)
         _lib.hp_last_error.restype = ctypes.c_char_p
-        for name in ("hp_xq8_q_bytes", "hp_xq8_sc_bytes", "hp_argmax_scratch_bytes", "hp_attn_workspace_bytes"):
+        for name in ("hp_xq8_q_bytes", "hp_xq8_sc_bytes", "hp_argmax_scratch_bytes", "hp_attn_workspace_bytes", "hp_attn_paged_workspace_bytes"):
             getattr(_lib, name).restype = ctypes.c_size_t
     return _lib
 

@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <string>
+#include <algorithm>
 #include <exception>
 
 namespace hp {
@@ -20,13 +21,23 @@ int cuda_fail(cudaError_t e, const char* what, const char* file, int line) {
     set_error("CUDA error %d (%s) in %s @%s:%d", (int)e, cudaGetErrorString(e), what, file, line);
     return HP_ECUDA;
 }
-// one status word per device, set by kernels whose bounded waits gave up
+// two status words per device: set by kernels whose bounded waits gave up (kernels that wait look at it), and by kernels that met lengths or indexes that do not fit
 static int* g_dev_err[MAX_DEVICES] = {};
 int* device_err_flag() {
     const int dev = current_device(); if (dev < 0) return nullptr;
-    if (!g_dev_err[dev]) { if (cudaMalloc(&g_dev_err[dev], sizeof(int)) != cudaSuccess) return nullptr; cudaMemset(g_dev_err[dev], 0, sizeof(int)); }
+    if (!g_dev_err[dev]) {   // on a stream of its own, and allowed while some stream is capturing: the first call on a device may be a captured one
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+        int* p = nullptr; cudaStream_t s = nullptr;
+        const bool ok = cudaMalloc(&p, 2 * sizeof(int)) == cudaSuccess && cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking) == cudaSuccess &&
+                        cudaMemsetAsync(p, 0, 2 * sizeof(int), s) == cudaSuccess && cudaStreamSynchronize(s) == cudaSuccess;
+        if (s) cudaStreamDestroy(s);
+        if (ok) g_dev_err[dev] = p; else if (p) cudaFree(p);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+    }
     return g_dev_err[dev];
 }
+int* device_arg_flag() { int* p = device_err_flag(); return p ? p + 1 : nullptr; }
 // workspace of the kernel-level GEMV entry point (per device, allocated on first use; the engine owns its own)
 static GemvWorkspace g_ws[MAX_DEVICES] = {};
 int default_gemv_workspace(GemvWorkspace* out, size_t need) {
@@ -56,10 +67,12 @@ int hp_device_status(void* stream) {
     HP_GUARD_BEGIN
     int* f = hp::device_err_flag();
     if (!f) { hp::set_error("cannot allocate the device status word"); return HP_ENOMEM; }
-    int h = 0;
-    HP_CUDA(cudaMemcpyAsync(&h, f, sizeof(int), cudaMemcpyDeviceToHost, (cudaStream_t)stream));
+    int h[2] = {0, 0};
+    HP_CUDA(cudaMemcpyAsync(h, f, sizeof h, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
     HP_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
-    if (h != 0) { HP_CUDA(cudaMemsetAsync(f, 0, sizeof(int), (cudaStream_t)stream)); hp::set_error("a kernel gave up a bounded wait (device status %d)", h); return h; }
+    if (h[0] || h[1]) HP_CUDA(cudaMemsetAsync(f, 0, sizeof h, (cudaStream_t)stream));
+    if (h[0]) { hp::set_error("a kernel gave up a bounded wait (device status %d)", h[0]); return h[0]; }
+    if (h[1]) { hp::set_error("a kernel met a length or an index in device memory that does not fit (device status %d)", h[1]); return h[1]; }
     return HP_OK;
     HP_GUARD_END
 }
@@ -217,6 +230,92 @@ int hp_moe_layer(const float* xn_dev, const void* xq_q_dev, const void* xq_sc_de
     g.segs = ws + w.segs; g.ctl = (int*)(ws + w.ctl); g.err = hp::device_err_flag();
     { const int rc = hp::moe_experts_grouped(g, s); if (rc) return rc; }
     return hp::moe_combine(v, weights_dev, y_dev, T, ns, E, s);
+    HP_GUARD_END
+}
+
+// ------------------------------------------------------------------ paged 8-bit cache
+namespace {
+int paged_args(const char* who, const hp_kv_pages* c, const int* table, int table_ld, const int* row_start, const int* kv_len, int S, int R, long long max_rows, long long max_kv, hp::PagedPool* p, hp::PagedBatch* b) {
+    HP_REQUIRE(c, "%s: null cache", who);
+    HP_REQUIRE(c->type == HP_KV_I8 || c->type == HP_KV_E4M3, "%s: unknown cache type %d", who, c->type);
+    HP_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "%s: head_dim must be 64, 128 or 256, not %d", who, c->head_dim);
+    HP_REQUIRE(c->page_size >= 16 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0, "%s: page_size must be a power of two from 16 to 1024, not %d", who, c->page_size);
+    HP_REQUIRE(c->n_pages >= 1 && c->n_kv >= 1 && table_ld >= 1 && (long long)c->n_pages * c->n_kv < (0xffffffffll / c->page_size) && (long long)table_ld * c->page_size < (1ll << 30),
+               "%s: bad cache n_pages=%d n_kv=%d table_ld=%d", who, c->n_pages, c->n_kv, table_ld);
+    HP_REQUIRE(S >= 1 && R >= 1 && max_rows >= 1 && max_kv >= 1, "%s: bad batch S=%d R=%d max_rows=%lld max_kv=%lld", who, S, R, max_rows, max_kv);
+    p->k = (uint8_t*)c->k; p->v = (uint8_t*)c->v; p->k_scale = c->k_scale; p->v_scale = c->v_scale; p->table = table; p->table_ld = table_ld;
+    p->kind = c->type; p->n_pages = c->n_pages; p->n_kv = c->n_kv; p->head_dim = c->head_dim; p->lg_page = 0;
+    while ((1 << p->lg_page) < c->page_size) ++p->lg_page;
+    b->row_start = row_start; b->kv_len = kv_len; b->S = S; b->R = R;
+    b->max_rows = (int)(max_rows < R ? max_rows : R); b->max_kv = (int)std::min<long long>(max_kv, (long long)table_ld * c->page_size);
+    return HP_OK;
+}
+int paged_ptrs(const char* who, const hp_kv_pages* c, const int* table, const int* row_start, const int* kv_len) {
+    HP_REQUIRE(c->k && c->v && c->k_scale && c->v_scale && table && row_start && kv_len, "%s: null pointer", who);
+    HP_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0 && (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale | (uintptr_t)table | (uintptr_t)row_start | (uintptr_t)kv_len) & 3) == 0, "%s: misaligned cache or batch", who);
+    return HP_OK;
+}
+bool rows_ok(const void* p, long long ld, long long hs) { return ((uintptr_t)p & 15) == 0 && ld % 4 == 0 && hs % 4 == 0 && ld >= 0 && hs >= 0; }
+}
+int hp_rope_table(float* table_dev, int n_pos, int n_rot, double base, int scaling, double factor, int orig_ctx, double beta_fast, double beta_slow, double attn_factor, void* stream) {
+    HP_GUARD_BEGIN
+    HP_REQUIRE(table_dev && ((uintptr_t)table_dev & 7) == 0, "hp_rope_table: null or misaligned table");
+    HP_REQUIRE(n_pos >= 1 && n_rot >= 2 && n_rot % 2 == 0 && n_rot <= 256 && base > 0, "hp_rope_table: bad shape n_pos=%d n_rot=%d base=%g", n_pos, n_rot, base);
+    HP_REQUIRE(scaling == HP_ROPE_NONE || scaling == HP_ROPE_LINEAR || scaling == HP_ROPE_YARN, "hp_rope_table: unknown scaling %d", scaling);
+    HP_REQUIRE(scaling == HP_ROPE_NONE || (factor >= 1 && factor < 1e9), "hp_rope_table: factor must be at least 1");
+    HP_REQUIRE(scaling != HP_ROPE_YARN || (orig_ctx >= 1 && beta_fast > beta_slow), "hp_rope_table: bad original context or betas");
+    HP_REQUIRE(attn_factor >= 0, "hp_rope_table: bad attention factor");
+    return hp::rope_table(table_dev, n_pos, n_rot, base, scaling, factor, orig_ctx, beta_fast, beta_slow, attn_factor, (cudaStream_t)stream);
+    HP_GUARD_END
+}
+int hp_kv_append(const float* q_dev, long long q_ld, long long q_hs, float* q_out_dev, long long qo_ld, long long qo_hs, int n_head, const float* k_dev, long long k_ld, long long k_hs,
+                 const float* v_dev, long long v_ld, long long v_hs, const void* q_norm_bf16_dev, const void* k_norm_bf16_dev, const float* rope_dev, int n_pos, int n_rot, int interleaved,
+                 const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, float eps, void* stream) {
+    HP_GUARD_BEGIN
+    hp::PagedPool pool; hp::PagedBatch b;
+    { int rc = paged_args("hp_kv_append", pages, table_dev, table_ld, row_start_dev, kv_len_dev, S, R, R, 1 << 30, &pool, &b); if (!rc) rc = paged_ptrs("hp_kv_append", pages, table_dev, row_start_dev, kv_len_dev); if (rc) return rc; }
+    HP_REQUIRE(k_dev && v_dev && n_head >= 0 && (n_head == 0 || (q_dev && q_out_dev)) && (n_rot == 0 || rope_dev), "hp_kv_append: null pointer");
+    HP_REQUIRE(n_rot >= 0 && n_rot % 2 == 0 && n_rot <= pool.head_dim && (n_rot == 0 || n_pos >= 1) && ((uintptr_t)rope_dev & 7) == 0, "hp_kv_append: bad n_rot=%d n_pos=%d or rope table", n_rot, n_pos);
+    HP_REQUIRE(rows_ok(k_dev, k_ld, k_hs) && rows_ok(v_dev, v_ld, v_hs) && (n_head == 0 || (rows_ok(q_dev, q_ld, q_hs) && rows_ok(q_out_dev, qo_ld, qo_hs))), "hp_kv_append: rows must be 16-byte aligned, with strides that are multiples of 4");
+    HP_REQUIRE((long long)R * (n_head + 2 * pool.n_kv) < (1ll << 33), "hp_kv_append: too many rows");
+    hp::KvAppendParams p; p.q = q_dev; p.q_ld = q_ld; p.q_hs = q_hs; p.q_out = q_out_dev; p.qo_ld = qo_ld; p.qo_hs = qo_hs; p.n_head = n_head; p.k = k_dev; p.k_ld = k_ld; p.k_hs = k_hs;
+    p.v = v_dev; p.v_ld = v_ld; p.v_hs = v_hs; p.q_norm = q_norm_bf16_dev; p.k_norm = k_norm_bf16_dev; p.rope = rope_dev; p.n_pos = n_rot ? n_pos : 1 << 30; p.n_rot = n_rot; p.interleaved = interleaved; p.eps = eps;
+    return hp::kv_append(pool, b, p, (cudaStream_t)stream);
+    HP_GUARD_END
+}
+int hp_kv_read(const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, void* k_out_f16_dev, void* v_out_f16_dev, long long row_stride, long long head_stride, void* stream) {
+    HP_GUARD_BEGIN
+    hp::PagedPool pool; hp::PagedBatch b;
+    { int rc = paged_args("hp_kv_read", pages, table_dev, table_ld, row_start_dev, kv_len_dev, S, R, R, 1 << 30, &pool, &b); if (!rc) rc = paged_ptrs("hp_kv_read", pages, table_dev, row_start_dev, kv_len_dev); if (rc) return rc; }
+    HP_REQUIRE(k_out_f16_dev && v_out_f16_dev, "hp_kv_read: null pointer");
+    HP_REQUIRE((((uintptr_t)k_out_f16_dev | (uintptr_t)v_out_f16_dev) & 15) == 0 && row_stride >= 0 && head_stride >= 0 && row_stride % 8 == 0 && head_stride % 8 == 0, "hp_kv_read: outputs must be 16-byte aligned, with strides that are multiples of 8");
+    return hp::kv_read(pool, b, k_out_f16_dev, v_out_f16_dev, (size_t)row_stride, (size_t)head_stride, (cudaStream_t)stream);
+    HP_GUARD_END
+}
+static int attn_paged_check(const char* who, int n_head, int window, int n_sink, const hp::PagedPool& pool) {
+    HP_REQUIRE(n_head >= 1 && n_head % pool.n_kv == 0, "%s: n_head=%d must be a multiple of n_kv=%d", who, n_head, pool.n_kv);
+    HP_REQUIRE(window >= 0 && n_sink >= 0 && (window > 0 || n_sink == 0), "%s: bad window=%d n_sink=%d (first tokens go with a window)", who, window, n_sink);
+    return HP_OK;
+}
+size_t hp_attn_paged_workspace_bytes(int table_ld, int S, int R, int max_rows, int max_kv, int n_head, int window, int n_sink, const hp_kv_pages* pages) {
+    hp::PagedPool pool; hp::PagedBatch b;
+    if (paged_args("hp_attn_paged_workspace_bytes", pages, nullptr, table_ld, nullptr, nullptr, S, R, max_rows, max_kv, &pool, &b) || attn_paged_check("hp_attn_paged_workspace_bytes", n_head, window, n_sink, pool)) return 0;
+    return hp::attn_paged_workspace_bytes(pool, b, n_head, window, n_sink);
+}
+int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const float* gate_dev, long long g_ld, long long g_hs, int n_head, const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev,
+                  int S, int R, int max_rows, int max_kv, const hp_kv_pages* pages, float scale, int window, int n_sink, float* out_dev, void* xq_q_dev, void* xq_sc_dev, void* workspace_dev, void* stream) {
+    HP_GUARD_BEGIN
+    hp::PagedPool pool; hp::PagedBatch b;
+    { int rc = paged_args("hp_attn_paged", pages, table_dev, table_ld, row_start_dev, kv_len_dev, S, R, max_rows, max_kv, &pool, &b); if (!rc) rc = paged_ptrs("hp_attn_paged", pages, table_dev, row_start_dev, kv_len_dev);
+      if (!rc) rc = attn_paged_check("hp_attn_paged", n_head, window, n_sink, pool); if (rc) return rc; }
+    HP_REQUIRE(q_dev && workspace_dev && (out_dev || xq_q_dev), "hp_attn_paged: null pointer");
+    HP_REQUIRE((xq_q_dev == nullptr) == (xq_sc_dev == nullptr), "hp_attn_paged: give both quantised-output buffers or neither");
+    HP_REQUIRE(rows_ok(q_dev, q_ld, q_hs) && (!gate_dev || (((uintptr_t)gate_dev & 3) == 0 && g_ld >= 0 && g_hs >= 0)) && ((uintptr_t)workspace_dev & 15) == 0 && ((uintptr_t)out_dev & 3) == 0,
+               "hp_attn_paged: rows and workspace must be 16-byte aligned, with strides that are multiples of 4");
+    HP_REQUIRE(scale > 0 && scale < 1e30f, "hp_attn_paged: bad scale");
+    hp::AttnPagedParams p; p.q = q_dev; p.q_ld = q_ld; p.q_hs = q_hs; p.gate = gate_dev; p.g_ld = g_ld; p.g_hs = g_hs; p.n_head = n_head; p.scale = scale; p.window = window; p.n_sink = n_sink;
+    p.out = out_dev; p.xq = hp::XQ8F{xq_q_dev, xq_sc_dev}; p.workspace = workspace_dev;
+    return hp::attn_paged(pool, b, p, (cudaStream_t)stream);
     HP_GUARD_END
 }
 

@@ -15,6 +15,8 @@ constexpr int MAX_DEVICES = 64;
 inline int current_device() { int d = -1; return (cudaGetDevice(&d) == cudaSuccess && d >= 0 && d < MAX_DEVICES) ? d : -1; }
 // device status word of the current device (set by kernels whose bounded waits gave up); nullptr if it cannot be allocated
 int* device_err_flag();
+// its neighbour, set by kernels that met lengths or indexes in device memory that do not fit
+int* device_arg_flag();
 
 // ---- gemv_q4k.cu ----
 // Work partition of the tensor-core GEMV. It is part of the numerics contract (it fixes the fp32 summation order)
@@ -178,5 +180,28 @@ int argmax_static_max_rows();
 int argmax_static_max_n();
 // greedy prefix acceptance on device: out[0] = accepted drafts mm, out[1] = bonus id ids[mm]
 int accept_greedy(const int* ids, const int* drafts, int n_draft, int* out, cudaStream_t s);
+
+// ---- kv_pages.cu, attn_paged.cu: a cache of 8-bit pages for ragged batches (no counterpart in the reference) ----
+enum : int { KV_I8 = 0, KV_E4M3 = 1 };
+struct PagedPool {
+    uint8_t* k; uint8_t* v; float* k_scale; float* v_scale;   // codes [n_pages][n_kv][page][head_dim], scales [n_pages][n_kv][page]
+    const int* table; int table_ld;                           // [S][table_ld]
+    int kind, n_pages, n_kv, lg_page, head_dim;
+};
+struct PagedBatch { const int* row_start; const int* kv_len; int S, R, max_rows, max_kv; };   // max_rows, max_kv: bounds that the host knows
+int rope_table(float* table, int n_pos, int n_rot, double base, int scaling, double factor, int orig_ctx, double beta_fast, double beta_slow, double attn_factor, cudaStream_t s);
+struct KvAppendParams {
+    const float* q; size_t q_ld, q_hs; float* q_out; size_t qo_ld, qo_hs; int n_head;   // n_head = 0: keys and values alone
+    const float* k; size_t k_ld, k_hs; const float* v; size_t v_ld, v_hs;
+    const void* q_norm; const void* k_norm; const float* rope; int n_pos, n_rot, interleaved; float eps;
+};
+int kv_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, cudaStream_t s);
+int kv_read(const PagedPool& pool, const PagedBatch& b, void* k_out, void* v_out, size_t row_stride, size_t head_stride, cudaStream_t s);
+struct AttnPagedParams {
+    const float* q; const float* gate; size_t q_ld, q_hs, g_ld, g_hs; int n_head; float scale; int window, n_sink;
+    float* out; XQ8F xq; void* workspace;
+};
+size_t attn_paged_workspace_bytes(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink);
+int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams& p, cudaStream_t s);
 
 }  // namespace hp

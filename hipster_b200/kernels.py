@@ -5,7 +5,7 @@ import functools
 
 import torch
 
-from ._lib import lib, hot, check, ptr
+from ._lib import HipsterError, lib, hot, check, ptr
 
 # The calls below are a few microseconds of device work, so what they spend in Python counts: the handle of the current stream
 # comes without a Stream object around it, the short calls go through native entry points that take addresses as integers (_lib.hot; to
@@ -162,3 +162,130 @@ def moe_layer(xn, router, exp_gate_up, exp_down, sh_gate_up, sh_down, F, n_exper
     check(L.hp_moe_layer(ptr(xn), ptr(xq.q), ptr(xq.sc), ptr(router), ptr(egu), ptr(edn), ptr(sgu), ptr(sdn), T, E, F, n_expert, k,
                          ptr(ids), ptr(w), ptr(y), ptr(ws), _stream()))
     return ids, w, y
+
+
+# ---- a paged cache in 8 bits (no counterpart in the reference)
+class _Pages(ctypes.Structure):   # hp_kv_pages
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)] + [(n, ctypes.c_int) for n in ("type", "n_pages", "n_kv", "page_size", "head_dim")]
+
+
+def _refuse(ok, what):
+    if not ok:
+        raise HipsterError(1, what)
+
+
+class KVPages:
+    """A pool of pages: k, v [n_pages][n_kv][page_size][head_dim] in int8 or float8_e4m3fn, k_scale, v_scale f32 [n_pages][n_kv][page_size] (one scale per
+    token and head). The tensors are kept, not copied; KVPages.empty() allocates them."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        _refuse(k.dim() == 4 and k.dtype in (torch.int8, torch.float8_e4m3fn), "KVPages: k must be [n_pages][n_kv][page_size][head_dim] in int8 or float8_e4m3fn")
+        _refuse(v.dtype == k.dtype and v.shape == k.shape, "KVPages: k and v must be alike")
+        _refuse(all(t.dtype == torch.float32 and t.shape == k.shape[:3] for t in (k_scale, v_scale)), "KVPages: scales must be f32 [n_pages][n_kv][page_size]")
+        _refuse(all(t.is_contiguous() and t.device == k.device for t in (k, v, k_scale, v_scale)), "KVPages: contiguous tensors of one device")
+        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
+        self.n_pages, self.n_kv, self.page_size, self.head_dim = k.shape
+        self._c = _Pages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), int(k.dtype != torch.int8), *k.shape)
+        self._at = ctypes.addressof(self._c)
+
+    @classmethod
+    def empty(cls, n_pages, n_kv, page_size, head_dim, dtype=torch.int8, device="cuda"):
+        codes = [torch.zeros((n_pages, n_kv, page_size, head_dim), dtype=torch.uint8, device=device).view(dtype) for _ in range(2)]
+        return cls(*codes, *(torch.zeros((n_pages, n_kv, page_size), dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _batch(pages, table, row_start, kv_len):
+    """Checks what describes a ragged batch; -> its arguments from the table on, up to S."""
+    dev, cur = pages.device.index, _device()
+    _refuse(dev == cur, f"the pages are on device {dev}, and device {cur} is current")
+    _refuse(table.dtype == row_start.dtype == kv_len.dtype == torch.int32, "table, row_start and kv_len must be int32")
+    S = kv_len.shape[0]
+    _refuse(table.dim() == 2 and table.shape[0] == S and table.stride(1) == 1 and table.stride(0) >= table.shape[1] and row_start.shape == (S + 1,) and kv_len.dim() == 1, "table [S][columns], row_start [S + 1], kv_len [S]")
+    _refuse(row_start.is_contiguous() and kv_len.is_contiguous() and table.device == row_start.device == kv_len.device == pages.device, "table, row_start and kv_len must be contiguous and on the device of the pages")
+    return S
+
+
+def _rows(t, pages, R, what):
+    """f32 rows [R][heads][head_dim] -> address, row stride, head stride."""
+    _refuse(t.dtype == torch.float32 and t.dim() == 3 and t.shape[0] == R and t.shape[2] == pages.head_dim and t.stride(2) == 1 and t.device == pages.device, f"{what} must be f32 [R][heads][head_dim] on the device of the pages")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+_SCALING = {None: 0, "none": 0, "linear": 1, "yarn": 2}
+
+
+def rope_table(n_pos, n_rot, base, scaling=None, factor=1.0, orig_ctx=0, beta_fast=32.0, beta_slow=1.0, attn_factor=0.0, device="cuda"):
+    """(cos, sin) of pos * base^(-2 i / n_rot), f32 [n_pos][n_rot / 2][2], computed in 64 bits; scaling "linear" divides the frequencies by factor, "yarn"
+    by parts: those that turn less than beta_slow times over orig_ctx positions wholly, those over beta_fast times not."""
+    _refuse(scaling in _SCALING, f"rope_table: unknown scaling {scaling!r}")
+    out = torch.empty((n_pos, n_rot // 2, 2), dtype=torch.float32, device=device)
+    _refuse(out.device.index == _device(), "rope_table: the device must be the current one")
+    d = ctypes.c_double
+    check(lib().hp_rope_table(ptr(out), n_pos, n_rot, d(base), _SCALING[scaling], d(factor), orig_ctx, d(beta_fast), d(beta_slow), d(attn_factor), _stream()))
+    return out
+
+
+def kv_append(pages, k, v, table, row_start, kv_len, rope=None, q=None, q_out=None, interleaved=False, q_norm=None, k_norm=None, eps=1e-6):
+    """Appends rows k, v f32 [R][n_kv][head_dim] of a ragged batch to their sequences' pages, k normalised (k_norm bf16 [head_dim]) and rotated by rope
+    f32 [n_pos][n_rot / 2][2]. q [R][n_head][head_dim] is normalised and rotated alike. -> q_out (f32 [R][n_head][head_dim]; None without q).
+    Rows row_start[s] .. row_start[s + 1] - 1 are the newest of the kv_len[s] tokens of sequence s."""
+    S, R = _batch(pages, table, row_start, kv_len), k.shape[0]
+    kr, vr = _rows(k, pages, R, "k"), _rows(v, pages, R, "v")
+    _refuse(k.shape[1] == v.shape[1] == pages.n_kv, "kv_append: k and v have the heads of the pages")
+    qr = qo = (None, 0, 0)
+    n_head = 0
+    if q is not None:
+        n_head, qr = q.shape[1], _rows(q, pages, R, "q")
+        if q_out is None:
+            q_out = torch.empty((R, n_head, pages.head_dim), dtype=torch.float32, device=pages.device)
+        qo = _rows(q_out, pages, R, "q_out")
+        _refuse(q_out.shape[1] == n_head, "kv_append: q_out has the heads of q")
+    n_pos = n_rot = 0
+    if rope is not None:
+        _refuse(rope.dtype == torch.float32 and rope.dim() == 3 and rope.shape[2] == 2 and rope.is_contiguous() and rope.device == pages.device, "kv_append: rope must be f32 [n_pos][n_rot / 2][2]")
+        n_pos, n_rot = rope.shape[0], 2 * rope.shape[1]
+    for w in (q_norm, k_norm):
+        _refuse(w is None or (w.element_size() == 2 and w.dtype != torch.float16 and w.shape == (pages.head_dim,) and w.is_contiguous() and w.device == pages.device), "kv_append: norm weights are bf16 [head_dim]")
+    check(hot().hp_kv_append(*qr, *qo, n_head, *kr, *vr, None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), None if rope is None else rope.data_ptr(), n_pos, n_rot,
+                             int(interleaved), table.data_ptr(), table.stride(0), row_start.data_ptr(), kv_len.data_ptr(), S, R, pages._at, eps, _raw_stream(_device())))
+    return q_out
+
+
+def kv_read(pages, table, row_start, kv_len, R=None, k_out=None, v_out=None):
+    """The tokens of the rows back as f16 -> k, v [R][n_kv][head_dim]. With kv_len[s] rows for each sequence whole caches; k_out, v_out may be views with other
+    strides, as cache.transpose(0, 1) of an f16 [n_kv][max_ctx][256] cache for attn_decode."""
+    S = _batch(pages, table, row_start, kv_len)
+    if k_out is None:
+        _refuse(v_out is None and R is not None and R >= 1, "kv_read: give R, or both outputs")
+        k_out, v_out = torch.empty((2, R, pages.n_kv, pages.head_dim), dtype=torch.float16, device=pages.device)
+    R = k_out.shape[0]
+    for t in (k_out, v_out):
+        _refuse(t is not None and t.dtype == torch.float16 and t.dim() == 3 and t.shape == (R, pages.n_kv, pages.head_dim) and t.stride() == k_out.stride() and t.stride(2) == 1 and t.device == pages.device,
+                "kv_read: outputs are f16 [R][n_kv][head_dim] with the same strides")
+    check(hot().hp_kv_read(table.data_ptr(), table.stride(0), row_start.data_ptr(), kv_len.data_ptr(), S, R, pages._at, k_out.data_ptr(), v_out.data_ptr(), k_out.stride(0), k_out.stride(1), _raw_stream(_device())))
+    return k_out, v_out
+
+
+@functools.lru_cache(maxsize=256, typed=True)
+def _attn_paged_workspace_bytes(cols, S, R, max_rows, max_kv, n_head, window, n_sink, kind, n_pages, n_kv, page_size, head_dim):
+    return lib().hp_attn_paged_workspace_bytes(cols, S, R, max_rows, max_kv, n_head, window, n_sink, ctypes.byref(_Pages(None, None, None, None, kind, n_pages, n_kv, page_size, head_dim)))
+
+
+def attn_paged(q, pages, table, row_start, kv_len, max_rows, max_kv, scale=None, window=0, n_sink=0, gate=None, want_f32=True, want_q8=False):
+    """Attention of rows q f32 [R][n_head][head_dim] over their sequences' pages (causal; window > 0: the last `window` tokens and the first n_sink), times sigmoid(gate)
+    where a gate [R][n_head][head_dim] is given. scale: 1 / sqrt(head_dim). max_rows, max_kv bound the rows and tokens of a sequence.
+    -> (out f32 [R][n_head][head_dim] or None, XQ8 of its rows or None)."""
+    S, (R, n_head, D) = _batch(pages, table, row_start, kv_len), q.shape
+    qr = _rows(q, pages, R, "q")
+    gr = (None, 0, 0)
+    if gate is not None:
+        gr = _rows(gate, pages, R, "gate")
+        _refuse(gate.shape[1] == n_head, "attn_paged: gate has the heads of q")
+    c = pages._c
+    nb = _attn_paged_workspace_bytes(table.stride(0), S, R, max_rows, -(-max_kv // 1024) * 1024, n_head, window, n_sink, c.type, c.n_pages, c.n_kv, c.page_size, c.head_dim)   # grows with max_kv
+    ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=pages.device)
+    out = torch.empty((R, n_head, D), dtype=torch.float32, device=pages.device) if want_f32 else None
+    xq = XQ8(R, n_head * D, pages.device) if want_q8 else None
+    check(hot().hp_attn_paged(*qr, *gr, n_head, table.data_ptr(), table.stride(0), row_start.data_ptr(), kv_len.data_ptr(), S, R, max_rows, max_kv, pages._at, D ** -0.5 if scale is None else scale, window, n_sink,
+                              None if out is None else out.data_ptr(), xq.q.data_ptr() if xq else None, xq.sc.data_ptr() if xq else None, ws.data_ptr(), _raw_stream(_device())))
+    return out, xq

@@ -25,7 +25,8 @@ enum { HP_OK = 0, HP_EINVAL = 1, HP_ECUDA = 2, HP_ENOMEM = 3, HP_ETIMEOUT = 4, H
 
 const char* hp_last_error(void);
 int hp_version(void);
-/* Reads (and clears) the device-side status word that kernels set when a bounded wait gave up. */
+/* Reads (and clears) the device-side status word that kernels set when a bounded wait gave up (HP_ETIMEOUT), or when lengths or page numbers in
+ * device memory did not fit (HP_EINVAL). */
 int hp_device_status(void* stream);
 
 /* ------------------------------------------------------------------ kernel level (engine/kernels/gemv.h, ops.h) */
@@ -120,6 +121,54 @@ size_t hp_moe_workspace_bytes(int T, int E, int F, int n_expert, int k);
 int hp_moe_layer(const float* xn_dev, const void* xq_q_dev, const void* xq_sc_dev, const float* router_dev, const void* exp_gate_up_tiled_dev, const void* exp_down_tiled_dev,
                  const void* sh_gate_up_tiled_dev, const void* sh_down_tiled_dev, int T, int E, int F, int n_expert, int k, int* ids_dev, float* weights_dev, float* y_dev,
                  void* workspace_dev, void* stream);
+
+/* ------------------------------------------------------------------ a paged cache in 8 bits, for ragged batches
+ * No counterpart in the reference, whose caches are f16 and contiguous. Tokens of many sequences share a pool of pages; k and v are held as
+ * int8 or e4m3 codes with one f32 scale per token and head (int8: largest magnitude / 127, e4m3: / 448), so that a token that a verify pass wrote
+ * and that is overwritten later leaves no trace in its neighbours. A token with an infinite or NaN element gets a NaN scale over codes of
+ * zero: rows that see it become NaN, others do not. e4m3 codes 0x7f and 0xff are never written and read as 480 and -480.
+ *
+ * hp_kv_pages describes a cache (host struct, read during the call). k, v: [n_pages][n_kv][page_size][head_dim] bytes, 16-byte aligned; k_scale, v_scale: f32
+ * [n_pages][n_kv][page_size]. page_size: a power of two, 16 to 1024; head_dim: 64, 128 or 256.
+ * A batch: table_dev, int [S][table_ld], holds the page of positions [i * page_size, (i + 1) * page_size) of each sequence, which has at most table_ld * page_size
+ * tokens. Sequences may share pages to read; the slots that one call appends to must be distinct. Rows [row_start[s], row_start[s + 1]) are the newest tokens of sequence s, which has kv_len[s] tokens with them, so that its row t is at
+ * position kv_len[s] - T + t. row_start (S + 1 ints) and kv_len (S ints) are device memory like the table, read when the kernels run: a captured call can be
+ * replayed with other lengths. R is the number of rows that the buffers hold: rows behind row_start[S] are neither read nor written. Entries that do
+ * not fit (rows outside of [0, R), a sequence with more rows than max_rows or more tokens than max_kv, table_ld * page_size or the rotary table, a
+ * page number outside of [0, n_pages) of a token that is used) fault nothing: what does not fit is left out (append, read) or makes the outputs of its
+ * sequence meaningless (attention), and hp_device_status returns HP_EINVAL. Rows of negative position are not appended, read back or
+ * normalised (HP_EINVAL), and attend to nothing. Row strides (ld) and head strides (hs) are in elements. */
+enum { HP_KV_I8 = 0, HP_KV_E4M3 = 1 };
+typedef struct hp_kv_pages {
+    void* k; void* v; float* k_scale; float* v_scale;
+    int type, n_pages, n_kv, page_size, head_dim;
+} hp_kv_pages;
+/* table_dev f32 [n_pos][n_rot / 2][2] = (cos, sin) of pos * f_i, f_i = base^(-2 i / n_rot): the rope_dev of hp_attn_decode and hp_kv_append. Scaled for
+ * contexts beyond the trained one: HP_ROPE_LINEAR f_i / factor; HP_ROPE_YARN (by parts; Peng et al. 2023) with r_i = orig_ctx * f_i / (2 pi) and
+ * g_i = clamp((r_i - beta_slow) / (beta_fast - beta_slow), 0, 1): f_i * (g_i + (1 - g_i) / factor). attn_factor multiplies cos and sin; 0 takes
+ * 0.1 ln(factor) + 1 with HP_ROPE_YARN and 1 otherwise. Computed in 64 bits. n_rot even, 2 to 256; factor >= 1. */
+enum { HP_ROPE_NONE = 0, HP_ROPE_LINEAR = 1, HP_ROPE_YARN = 2 };
+int hp_rope_table(float* table_dev, int n_pos, int n_rot, double base, int scaling, double factor, int orig_ctx, double beta_fast, double beta_slow, double attn_factor, void* stream);
+/* Appends the rows of a batch: per head RMSNorm (q_norm / k_norm: bf16 [head_dim], NULL: none; eps), rotation of the first n_rot dims (rope_dev
+ * [n_pos][n_rot / 2][2]; pairs (i, i + n_rot / 2), or neighbours (2 i, 2 i + 1) with interleaved != 0; n_rot = 0: none), then q to q_out and k, and v as it is, into
+ * the pages. n_head = 0: no queries (q_dev, q_out_dev NULL). q_out_dev may be q_dev with the same strides. Pointers 16-byte aligned, strides
+ * multiples of 4. */
+int hp_kv_append(const float* q_dev, long long q_ld, long long q_hs, float* q_out_dev, long long qo_ld, long long qo_hs, int n_head, const float* k_dev, long long k_ld, long long k_hs,
+                 const float* v_dev, long long v_ld, long long v_hs, const void* q_norm_bf16_dev, const void* k_norm_bf16_dev, const float* rope_dev, int n_pos, int n_rot, int interleaved,
+                 const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, float eps, void* stream);
+/* The tokens of the rows back as f16 (code * scale, rounded once): k_out / v_out + r * row_stride + head * head_stride hold head_dim values each. With kv_len[s] rows a
+ * whole sequence; row_stride = head_dim and head_stride = max_ctx * head_dim give the cache of hp_attn_decode. Strides multiples of 8. */
+int hp_kv_read(const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, void* k_out_f16_dev, void* v_out_f16_dev, long long row_stride, long long head_stride, void* stream);
+/* Attention of the rows over their sequences' pages: softmax(scale * q k^T) v in fp32 over the keys j <= pos, with window > 0 only those with
+ * j > pos - window or j < n_sink (first tokens that stay visible; pages without a visible token are not looked up). n_head a multiple of n_kv; head h reads kv head
+ * h / (n_head / n_kv). gate_dev (nullable): the output is multiplied by sigmoid(gate). out_dev f32 [R][n_head * head_dim] and / or its int8 quantisation (K = n_head * head_dim),
+ * either may be NULL. max_rows, max_kv: bounds of a sequence's rows and tokens; they size the launch. Up to max_rows = 8 a row's result depends neither
+ * on the other rows of its sequence nor on the other sequences, bit for bit (for one table_ld, window and n_sink); calls of more rows per sequence sum a row's keys in
+ * another order. Not for rows of both kinds at once: a short row beside a prompt takes as long as all of its keys on one SM.
+ * workspace_dev: hp_attn_paged_workspace_bytes of the same arguments, 16-byte aligned, of this call alone until it is done (captured calls that may run at once need one each). */
+size_t hp_attn_paged_workspace_bytes(int table_ld, int S, int R, int max_rows, int max_kv, int n_head, int window, int n_sink, const hp_kv_pages* pages);
+int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const float* gate_dev, long long g_ld, long long g_hs, int n_head, const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev,
+                  int S, int R, int max_rows, int max_kv, const hp_kv_pages* pages, float scale, int window, int n_sink, float* out_dev, void* xq_q_dev, void* xq_sc_dev, void* workspace_dev, void* stream);
 
 /* ------------------------------------------------------------------ engine level (engine/src/qwen35.h, qwen4exp.h) */
 
