@@ -6,11 +6,11 @@
 // fp32 results from the f16 tensor pipe: codes of int8 and of e4m3 (times 2^-8) are exact in f16, a token's scale multiplies its score or its weight in
 // fp32, and q and the weights (times the scale of v) go in as two f16 each, the value and what is left of it: 22 bits. q is brought to [2^14, 2^15) by a
 // power of two per row, the weights by the reference mu: whole, at least the largest of s_j + log2(scale of v_j) - 14, so that a weight times
-// its scale stays below 2^15 and every rescaling is by a power of two, exact. The tensor pipe adds 32 keys (or head_dim products) at a time; these sums
+// its scale stays below 2^15 and every rescaling is by a power of two, exact. The tensor pipe adds 16 keys (or head_dim products) at a time; these sums
 // are added to the running ones in fp32.
 //
-// The pairs (row, head) of a sequence and kv head, row by row, are cut into blocks of up to 64; a CTA holds one block and the keys of one split, in tiles of
-// 64 keys through a ring of asynchronous copies. Two warps share 16 pairs, one half of each tile each, scores, weights and outputs in
+// The pairs (row, head) of a sequence and kv head, row by row, are cut into blocks of up to 32; a CTA holds one block and the keys of one split, in tiles of
+// 64 keys through a ring of asynchronous copies. Four warps share 16 pairs, a quarter of each tile each, scores, weights and outputs in
 // registers from end to end. Splits lie at fixed positions and a warp's sums at fixed keys: a row's bits depend neither on the other rows of the call
 // nor on the other sequences.
 #include "paged.cuh"
@@ -19,9 +19,10 @@
 namespace hp {
 namespace {
 
-constexpr int TK = 64, KPW = 32, KPAD = 32, VPAD = 16;   // keys of a tile and of a warp in it; bytes behind a row of k / v in shared memory: 64-bit reads of 4 rows x 4 lanes from distinct banks
-constexpr int MAX_TILES_M = 4;                           // 16-pair tiles of a CTA
+constexpr int TK = 64, KW = 4, KPW = TK / KW, KPAD = 32, VPAD = 16;   // keys of a tile, warps that share it, keys of a warp in it; bytes behind a row of k / v in shared memory: 64-bit reads of 4 rows x 4 lanes from distinct banks
+constexpr int MAX_TILES_M = 2;                           // 16-pair tiles of a CTA
 
+__host__ __device__ constexpr int out_stride(int D) { return D + 4; }
 struct PagedArgs {
     PagedPool pool; PagedBatch b;
     const float* q; size_t q_ld, q_hs; int n_head, G; float scale2;   // scale2 = scale * log2 e (times 256 for e4m3)
@@ -67,9 +68,7 @@ __device__ __forceinline__ void cp_wait(int left) {
         default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
     }
 }
-__device__ __forceinline__ uint2 lds64(uint32_t a) { uint2 v; asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a)); return v; }
-__device__ __forceinline__ float2 lds64f(uint32_t a) { float2 v; asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a)); return v; }
-__device__ __forceinline__ uint4 lds128(uint32_t a) { uint4 v; asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a)); return v; }
+template <typename T> __device__ __forceinline__ T at_smem(const uint8_t* p) { return *reinterpret_cast<const T*>(p); }
 
 // The block of pairs that blockIdx.z stands for: sequences in order, each with ceil(T * G / MB) blocks.
 struct Block { PagedSeq q; int p0, np; };
@@ -96,13 +95,14 @@ __device__ __forceinline__ Block find_block(const PagedBatch& b, int G, int MB, 
     return o;
 }
 
-// grid (splits, n_kv, blocks), 64 threads per 16 pairs
+// grid (splits, n_kv, blocks), 128 threads per 16 pairs
 template <int D, int KIND>
-__global__ void __launch_bounds__(256, 1) k_paged_split(PagedArgs a) {
-    constexpr int KS = D + KPAD, VS = D + VPAD, CPR = D / 16;   // row strides in shared memory, 16-byte pieces of a row
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_paged_split(PagedArgs a) {
+    constexpr int KS = D + KPAD, VS = D + VPAD, CPR = D / 16, NT = KPW / 8, XS = out_stride(D);   // row strides in shared memory, 16-byte pieces of a row, 8-key tiles of a warp
+    static_assert(NT == 2, "the weights of a warp are one fragment");
     extern __shared__ __align__(16) uint8_t sm[];
     const int tid = threadIdx.x, nthr = blockDim.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
-    const int MT = nthr >> 6, MB = MT * 16, mw = warp >> 1, kw = warp & 1;
+    const int MT = nthr / (32 * KW), MB = MT * 16, mw = warp / KW, kw = warp % KW;
     uint8_t* const sQ = sm;
     float* const sC = reinterpret_cast<float*>(sm + q_bytes(D, MT));        // [MB] factor of a pair's scores
     int* const sPos = reinterpret_cast<int*>(sC + MB);                      // [MB] position of a pair's row, -1: no pair
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_split(PagedArgs a) {
     // tiles between these positions are visible to all 16 (an absent pair counts as nothing)
     const int all_hi = (int)__reduce_min_sync(0xffffffffu, (unsigned)min(p0 < 0 ? 0x7fffffff : p0, p1 < 0 ? 0x7fffffff : p1));
     const int all_lo = a.window ? mpos - a.window : -1;
-    const uint32_t qf = smem_u32(sQ) + mw * D * 64 + lane * 16;
+    const uint8_t* const qf = sQ + mw * D * 64 + lane * 16;
 
     float O[D / 8][4];
 #pragma unroll
@@ -219,46 +219,49 @@ __global__ void __launch_bounds__(256, 1) k_paged_split(PagedArgs a) {
         fetch(slot == 0 ? a.stages - 1 : slot - 1);
         const int kb = ct * TK + kw * KPW;
         if (kb > mpos) continue;   // nothing of this half is visible to these pairs
-        const uint32_t st = ring_u + slot * stage_bytes(D);
-        // ---- scores of 16 pairs x 32 keys
-        float s[4][4], sl[4][4];
+        const uint8_t* const st = ring + slot * stage_bytes(D);
+        // ---- scores of 16 pairs x 16 keys
+        float s[NT][4], sl[NT][4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 4; ++c) s[n][c] = sl[n][c] = 0.f;
         {
-            const uint32_t kr = st + (kw * KPW + g) * KS + q4 * 8;
+            const uint8_t* kr = st + (kw * KPW + g) * KS + q4 * 8;
 #pragma unroll
             for (int x = 0; x < D / 32; ++x) {
-                const uint4 h0 = lds128(qf + x * 2048), r0 = lds128(qf + x * 2048 + 512), h1 = lds128(qf + x * 2048 + 1024), r1 = lds128(qf + x * 2048 + 1536);
+                const uint4 h0 = at_smem<uint4>(qf + x * 2048), r0 = at_smem<uint4>(qf + x * 2048 + 512), h1 = at_smem<uint4>(qf + x * 2048 + 1024), r1 = at_smem<uint4>(qf + x * 2048 + 1536);
+                uint32_t b[NT][4];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const uint2 kk = lds64(kr + n * 8 * KS + x * 32);
-                    uint32_t w = prepare4<KIND>(kk.x), b0 = pair<KIND, 0>(w), b1 = pair<KIND, 2>(w);
-                    mma_f16(s[n], h0, b0, b1); mma_f16(sl[n], r0, b0, b1);
-                    w = prepare4<KIND>(kk.y); b0 = pair<KIND, 0>(w); b1 = pair<KIND, 2>(w);
-                    mma_f16(s[n], h1, b0, b1); mma_f16(sl[n], r1, b0, b1);
+                for (int n = 0; n < NT; ++n) {
+                    const uint2 kk = at_smem<uint2>(kr + n * 8 * KS + x * 32);
+                    const uint32_t w0 = prepare4<KIND>(kk.x), w1 = prepare4<KIND>(kk.y);
+                    b[n][0] = pair<KIND, 0>(w0); b[n][1] = pair<KIND, 2>(w0); b[n][2] = pair<KIND, 0>(w1); b[n][3] = pair<KIND, 2>(w1);
                 }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) { mma_f16(s[n], h0, b[n][0], b[n][1]); mma_f16(sl[n], r0, b[n][0], b[n][1]); }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) { mma_f16(s[n], h1, b[n][2], b[n][3]); mma_f16(sl[n], r1, b[n][2], b[n][3]); }
             }
         }
         // ---- weights
-        const uint32_t sc = st + TK * (KS + VS) + (kw * KPW + 2 * q4) * 4;
-        float2 vs[4];
+        const uint8_t* sc = st + TK * (KS + VS) + (kw * KPW + 2 * q4) * 4;
+        float2 vs[NT];
         float t0 = -INFINITY, t1 = -INFINITY;
         const bool whole = kb + KPW - 1 <= all_hi && (kb > all_lo || kb + KPW <= sink);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const float2 ks = lds64f(sc + n * 32);
-            vs[n] = lds64f(sc + TK * 4 + n * 32);
+        for (int n = 0; n < NT; ++n) {
+            const float2 ks = at_smem<float2>(sc + n * 32);
+            vs[n] = at_smem<float2>(sc + TK * 4 + n * 32);
             s[n][0] = (s[n][0] + sl[n][0]) * (ks.x * c0); s[n][1] = (s[n][1] + sl[n][1]) * (ks.y * c0);
             s[n][2] = (s[n][2] + sl[n][2]) * (ks.x * c1); s[n][3] = (s[n][3] + sl[n][3]) * (ks.y * c1);
         }
-        float wv[4][4];   // the scale of v that a weight takes
+        float wv[NT][4];   // the scale of v that a weight takes
 #pragma unroll
-        for (int n = 0; n < 4; ++n) { wv[n][0] = wv[n][2] = vs[n].x; wv[n][1] = wv[n][3] = vs[n].y; }
+        for (int n = 0; n < NT; ++n) { wv[n][0] = wv[n][2] = vs[n].x; wv[n][1] = wv[n][3] = vs[n].y; }
         if (!whole) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int key = kb + n * 8 + 2 * q4 + (c & 1);
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_split(PagedArgs a) {
                 }
         }
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < NT; ++n) {
             const float lx = lg2(fmaxf(vs[n].x, 8.0779357e-28f)), ly = lg2(fmaxf(vs[n].y, 8.0779357e-28f));   // 2^-90: the weights' sum cannot overflow
             t0 = fmaxf(t0, fmaxf(s[n][0] + lx, s[n][1] + ly));
             t1 = fmaxf(t1, fmaxf(s[n][2] + lx, s[n][3] + ly));
@@ -277,11 +280,11 @@ __global__ void __launch_bounds__(256, 1) k_paged_split(PagedArgs a) {
         const float n0 = fmaxf(mu0, ceilf(t0) - 14.f), n1 = fmaxf(mu1, ceilf(t1) - 14.f);
         const float al0 = pow2i(mu0 - n0), al1 = pow2i(mu1 - n1);
         mu0 = n0; mu1 = n1; l0 = l0 * al0; l1 = l1 * al1;
-        uint4 ph[2], pr[2];   // A fragments of 16 keys: weights times scales, values and rests
+        uint4 ph, pr;   // A fragment of the 16 keys: weights times scales, values and rests
         {
-            uint32_t h[4][2], r[4][2];
+            uint32_t h[NT][2], r[NT][2];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int c = 0; c < 4; c += 2) {
                     const float m = c ? mu1 : mu0, e0 = ex2(s[n][c] - m), e1 = ex2(s[n][c + 1] - m);
@@ -292,40 +295,24 @@ __global__ void __launch_bounds__(256, 1) k_paged_split(PagedArgs a) {
                     h[n][c / 2] = h2_bits(hh); r[n][c / 2] = h2_bits(__floats2half2_rn(y0 - f.x, y1 - f.y));
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                ph[i] = make_uint4(h[2 * i][0], h[2 * i][1], h[2 * i + 1][0], h[2 * i + 1][1]);
-                pr[i] = make_uint4(r[2 * i][0], r[2 * i][1], r[2 * i + 1][0], r[2 * i + 1][1]);
-            }
+            ph = make_uint4(h[0][0], h[0][1], h[1][0], h[1][1]); pr = make_uint4(r[0][0], r[0][1], r[1][0], r[1][1]);
         }
         // ---- outputs: 64 dims at a time, lane group g holds 8 neighbouring ones of the rows of its keys
-        const uint32_t vr = st + TK * KS + (kw * KPW + 2 * q4) * VS + g * 8;
+        const uint8_t* vr = st + TK * KS + (kw * KPW + 2 * q4) * VS + g * 8;
 #pragma unroll
         for (int y = 0; y < D / 64; ++y) {
-            uint2 v[2][4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                v[i][0] = lds64(vr + (16 * i) * VS + y * 64); v[i][1] = lds64(vr + (16 * i + 1) * VS + y * 64);
-                v[i][2] = lds64(vr + (16 * i + 8) * VS + y * 64); v[i][3] = lds64(vr + (16 * i + 9) * VS + y * 64);
-            }
+            const uint2 v0 = at_smem<uint2>(vr + y * 64), v1 = at_smem<uint2>(vr + VS + y * 64), v2 = at_smem<uint2>(vr + 8 * VS + y * 64), v3 = at_smem<uint2>(vr + 9 * VS + y * 64);
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
+                const uint32_t a0 = prepare4<KIND>(w ? v0.y : v0.x), a1 = prepare4<KIND>(w ? v1.y : v1.x), a2 = prepare4<KIND>(w ? v2.y : v2.x), a3 = prepare4<KIND>(w ? v3.y : v3.x);
+                const uint32_t u0 = prmt(a0, a1, 0x5140), u1 = prmt(a0, a1, 0x7362), u2 = prmt(a2, a3, 0x5140), u3 = prmt(a2, a3, 0x7362);
+                const uint32_t b0[4] = {pair<KIND, 0>(u0), pair<KIND, 2>(u0), pair<KIND, 0>(u1), pair<KIND, 2>(u1)};
+                const uint32_t b1[4] = {pair<KIND, 0>(u2), pair<KIND, 2>(u2), pair<KIND, 0>(u3), pair<KIND, 2>(u3)};
                 float f[4][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) f[j][0] = f[j][1] = f[j][2] = f[j][3] = 0.f;
+                for (int j = 0; j < 4; ++j) { f[j][0] = f[j][1] = f[j][2] = f[j][3] = 0.f; mma_f16(f[j], pr, b0[j], b1[j]); }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t a0 = prepare4<KIND>(w ? v[i][0].y : v[i][0].x), a1 = prepare4<KIND>(w ? v[i][1].y : v[i][1].x);
-                    const uint32_t a2 = prepare4<KIND>(w ? v[i][2].y : v[i][2].x), a3 = prepare4<KIND>(w ? v[i][3].y : v[i][3].x);
-                    const uint32_t u0 = prmt(a0, a1, 0x5140), u1 = prmt(a0, a1, 0x7362), u2 = prmt(a2, a3, 0x5140), u3 = prmt(a2, a3, 0x7362);
-                    uint32_t b0[4], b1[4];
-                    b0[0] = pair<KIND, 0>(u0); b0[1] = pair<KIND, 2>(u0); b0[2] = pair<KIND, 0>(u1); b0[3] = pair<KIND, 2>(u1);
-                    b1[0] = pair<KIND, 0>(u2); b1[1] = pair<KIND, 2>(u2); b1[2] = pair<KIND, 0>(u3); b1[3] = pair<KIND, 2>(u3);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f16(f[j], pr[i], b0[j], b1[j]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f16(f[j], ph[i], b0[j], b1[j]);
-                }
+                for (int j = 0; j < 4; ++j) mma_f16(f[j], ph, b0[j], b1[j]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     float (&o)[4] = O[y * 8 + w * 4 + j];
@@ -337,47 +324,43 @@ __global__ void __launch_bounds__(256, 1) k_paged_split(PagedArgs a) {
     l0 = l0 + __shfl_xor_sync(0xffffffffu, l0, 1); l1 = l1 + __shfl_xor_sync(0xffffffffu, l1, 1);
     l0 = l0 + __shfl_xor_sync(0xffffffffu, l0, 2); l1 = l1 + __shfl_xor_sync(0xffffffffu, l1, 2);
 
-    // ---- the halves of the tiles meet: each warp of the two finishes eight of the pairs. Thread (g, q4) holds dims 64 y + 16 q4 + 0..15 of a row
+    // ---- the warps that share the tiles meet, in order. Thread (g, q4) holds dims 64 y + 16 q4 + 0..15 of rows g and g + 8
     cp_wait(0);
     __syncthreads();   // the ring and q are free
-    float* const xo = reinterpret_cast<float*>(sm) + (size_t)warp * (8 * D + 16);   // rows [8][D], then (mu, l)
+    float* const xo = reinterpret_cast<float*>(sm);   // [warp][16][XS]: D sums, mu, sum of weights
     {
-        float* dst = xo + g * D + 16 * q4;
-        // warp 0 keeps rows 0..7 (values 0, 1), hands on rows 8..15
-        auto other = [&](int i, int c) { return kw ? O[i][c] : O[i][c + 2]; };
+        float* dst = xo + (size_t)(warp * 16 + g) * XS + 16 * q4;
 #pragma unroll
         for (int y = 0; y < D / 64; ++y)
 #pragma unroll
-            for (int j = 0; j < 8; j += 4) {
-                *reinterpret_cast<float4*>(dst + 64 * y + j) = make_float4(other(y * 8 + j, 0), other(y * 8 + j + 1, 0), other(y * 8 + j + 2, 0), other(y * 8 + j + 3, 0));
-                *reinterpret_cast<float4*>(dst + 64 * y + 8 + j) = make_float4(other(y * 8 + j, 1), other(y * 8 + j + 1, 1), other(y * 8 + j + 2, 1), other(y * 8 + j + 3, 1));
-            }
-        if (q4 == 0) { xo[8 * D + 2 * g] = kw ? mu0 : mu1; xo[8 * D + 2 * g + 1] = kw ? l0 : l1; }
+            for (int j = 0; j < 8; j += 4)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    *reinterpret_cast<float4*>(dst + (c >> 1) * 8 * XS + 64 * y + 8 * (c & 1) + j) = make_float4(O[y * 8 + j][c], O[y * 8 + j + 1][c], O[y * 8 + j + 2][c], O[y * 8 + j + 3][c]);
+        if (q4 == 0) {
+            float* e = xo + (size_t)(warp * 16 + g) * XS + D;
+            e[0] = mu0; e[1] = l0; e[8 * XS] = mu1; e[8 * XS + 1] = l1;
+        }
     }
     __syncthreads();
-    const int i = kw ? i1 : i0;
-    if ((kw ? p1 : p0) < 0) return;
-    const float* src = reinterpret_cast<const float*>(sm) + (size_t)(warp ^ 1) * (8 * D + 16);
-    const float muo = src[8 * D + 2 * g], lo_ = src[8 * D + 2 * g + 1], mum = kw ? mu1 : mu0, lm = kw ? l1 : l0;
-    const float mu = fmaxf(mum, muo), am = pow2i(mum - mu), ao = pow2i(muo - mu);
-    const int p = blk.p0 + i, t = p / a.G;
-    const size_t at = ((size_t)(sq.row0 + t) * a.n_head + kh * a.G + p - t * a.G) * (a.ns + a.nwin) + blockIdx.x;
-    float* po = a.pO + at * D + 16 * q4;
-    src += g * D + 16 * q4;
-    auto own = [&](int i, int c) { return kw ? O[i][c + 2] : O[i][c]; };
+    for (int i = warp; i < blk.np; i += nthr >> 5) {   // a warp per pair
+        const int p = blk.p0 + i, t = p / a.G;
+        if (sq.len - sq.T + t < 0) continue;
+        const float* src = xo + (size_t)((i >> 4) * KW * 16 + (i & 15)) * XS;
+        float m[KW], w[KW], mu = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int y = 0; y < D / 64; ++y)
+        for (int k = 0; k < KW; ++k) { m[k] = src[k * 16 * XS + D]; mu = fmaxf(mu, m[k]); }
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int k = 0; k < KW; ++k) { w[k] = pow2i(m[k] - mu); l = fmaf(src[k * 16 * XS + D + 1], w[k], l); }
+        const size_t at = ((size_t)(sq.row0 + t) * a.n_head + kh * a.G + p - t * a.G) * (a.ns + a.nwin) + blockIdx.x;
+        for (int d = 2 * lane; d < D; d += 64) {
+            float2 o = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < 8; j += 4) {
-                const float4 o = *reinterpret_cast<const float4*>(src + 64 * y + 8 * c + j);
-                float4 v;
-                v.x = own(y * 8 + j, c) * am + o.x * ao; v.y = own(y * 8 + j + 1, c) * am + o.y * ao;
-                v.z = own(y * 8 + j + 2, c) * am + o.z * ao; v.w = own(y * 8 + j + 3, c) * am + o.w * ao;
-                *reinterpret_cast<float4*>(po + 64 * y + 8 * c + j) = v;
-            }
-    if (q4 == 0) a.pml[at] = make_float2(mu, lm * am + lo_ * ao);
+            for (int k = 0; k < KW; ++k) { const float2 v = *reinterpret_cast<const float2*>(src + k * 16 * XS + d); o.x = fmaf(v.x, w[k], o.x); o.y = fmaf(v.y, w[k], o.y); }
+            *reinterpret_cast<float2*>(a.pO + at * D + d) = o;
+        }
+        if (lane == 0) a.pml[at] = make_float2(mu, l);
+    }
 }
 
 // Splits of a row in order, gate, f32 and q8 outputs. One block of head_dim threads per row and head.
@@ -425,7 +408,7 @@ Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window,
     Plan p;
     const int G = n_head / pool.n_kv, cap = pool.table_ld << pool.lg_page;
     const long long eff = window ? std::min<long long>(cap, (long long)window + n_sink) : cap;
-    const long long pairs = (long long)b.max_rows * G, nb = (pairs + 63) / 64;
+    const long long pairs = (long long)b.max_rows * G, nb = (pairs + 16 * MAX_TILES_M - 1) / (16 * MAX_TILES_M);
     p.MT = (int)std::min<long long>(MAX_TILES_M, ((pairs + nb - 1) / nb + 15) / 16);
     const int MB = p.MT * 16;
     p.blocks = std::min<long long>((long long)b.S * ((pairs + MB - 1) / MB), (long long)b.R * G / MB + b.S);
@@ -447,8 +430,8 @@ template <int D, int KIND> int launch_split(const PagedArgs& a, dim3 grid, int M
     const int dev = current_device(); if (dev < 0) return HP_ECUDA;
     if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_split<D, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024)); attr[dev] = true; }
     // the outputs of the tiles' halves pass through the same memory at the end
-    const size_t smem = std::max<size_t>(q_bytes(D, MT) + MT * 16 * 8 + (size_t)a.stages * stage_bytes(D), (size_t)2 * MT * (8 * D + 16) * 4);
-    HP_CUDA(launch_pdl<4>(k_paged_split<D, KIND>, grid, dim3(64 * MT), smem, s, a));
+    const size_t smem = std::max<size_t>(q_bytes(D, MT) + MT * 16 * 8 + (size_t)a.stages * stage_bytes(D), (size_t)KW * MT * 16 * out_stride(D) * 4);
+    HP_CUDA(launch_pdl<4>(k_paged_split<D, KIND>, grid, dim3(32 * KW * MT), smem, s, a));
     return HP_OK;
 }
 
@@ -464,7 +447,7 @@ int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams
     HP_REQUIRE(pl.blocks <= 65535 && (long long)b.R * p.n_head < (1ll << 31), "attn_paged: too many rows (%d) for one call", b.R);
     PagedArgs a; a.pool = pool; a.b = b; a.q = p.q; a.q_ld = p.q_ld; a.q_hs = p.q_hs; a.n_head = p.n_head; a.G = p.n_head / pool.n_kv;
     a.scale2 = (float)((double)p.scale * 1.4426950408889634074 * (pool.kind == KV_E4M3 ? 256.0 : 1.0)); a.window = p.window; a.n_sink = p.n_sink;
-    a.U = pl.U; a.ns = pl.ns; a.nwin = pl.nwin; a.stages = pl.MT > 2 ? 4 : pool.head_dim == 256 ? 2 : 3;
+    a.U = pl.U; a.ns = pl.ns; a.nwin = pl.nwin; a.stages = pool.head_dim == 256 ? (pl.MT == 1 ? 2 : 4) : 3;
     a.pO = (float*)p.workspace; a.pml = (float2*)(a.pO + partials(pl, b, p.n_head) * pool.head_dim); a.err = device_arg_flag();
     const dim3 grid(pl.ns + pl.nwin, pool.n_kv, (unsigned)pl.blocks);
     int rc;

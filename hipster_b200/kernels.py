@@ -194,21 +194,29 @@ class KVPages:
         return cls(*codes, *(torch.zeros((n_pages, n_kv, page_size), dtype=torch.float32, device=device) for _ in range(2)))
 
 
+# The checks below run on every call of a few microseconds: a test that fails builds its message, one that holds costs its attribute reads alone.
 def _batch(pages, table, row_start, kv_len):
-    """Checks what describes a ragged batch; -> its arguments from the table on, up to S."""
-    dev, cur = pages.device.index, _device()
-    _refuse(dev == cur, f"the pages are on device {dev}, and device {cur} is current")
-    _refuse(table.dtype == row_start.dtype == kv_len.dtype == torch.int32, "table, row_start and kv_len must be int32")
-    S = kv_len.shape[0]
-    _refuse(table.dim() == 2 and table.shape[0] == S and table.stride(1) == 1 and table.stride(0) >= table.shape[1] and row_start.shape == (S + 1,) and kv_len.dim() == 1, "table [S][columns], row_start [S + 1], kv_len [S]")
-    _refuse(row_start.is_contiguous() and kv_len.is_contiguous() and table.device == row_start.device == kv_len.device == pages.device, "table, row_start and kv_len must be contiguous and on the device of the pages")
+    """Checks what describes a ragged batch; -> the number of sequences."""
+    dev = pages.device
+    if dev.index != _device():
+        raise HipsterError(1, f"the pages are on device {dev.index}, and device {_device()} is current")
+    S, = kv_len.shape
+    rows, cols = table.shape
+    if not (table.dtype is torch.int32 and row_start.dtype is torch.int32 and kv_len.dtype is torch.int32):
+        raise HipsterError(1, "table, row_start and kv_len must be int32")
+    if not (rows == S and row_start.numel() == S + 1 and table.stride(1) == 1 and (S == 1 or table.stride(0) >= cols) and row_start.is_contiguous() and kv_len.is_contiguous()):
+        raise HipsterError(1, "table [S][columns], row_start [S + 1] and kv_len [S] must be contiguous")
+    if not (table.device == dev and row_start.device == dev and kv_len.device == dev):
+        raise HipsterError(1, "table, row_start and kv_len must be on the device of the pages")
     return S
 
 
 def _rows(t, pages, R, what):
     """f32 rows [R][heads][head_dim] -> address, row stride, head stride."""
-    _refuse(t.dtype == torch.float32 and t.dim() == 3 and t.shape[0] == R and t.shape[2] == pages.head_dim and t.stride(2) == 1 and t.device == pages.device, f"{what} must be f32 [R][heads][head_dim] on the device of the pages")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    shape, (ld, hs, one) = t.shape, t.stride()
+    if not (t.dtype is torch.float32 and shape[0] == R and shape[2] == pages.head_dim and one == 1 and t.device == pages.device):
+        raise HipsterError(1, f"{what} must be f32 [R][heads][head_dim] on the device of the pages")
+    return t.data_ptr(), ld, hs
 
 
 _SCALING = {None: 0, "none": 0, "linear": 1, "yarn": 2}
@@ -223,6 +231,14 @@ def rope_table(n_pos, n_rot, base, scaling=None, factor=1.0, orig_ctx=0, beta_fa
     d = ctypes.c_double
     check(lib().hp_rope_table(ptr(out), n_pos, n_rot, d(base), _SCALING[scaling], d(factor), orig_ctx, d(beta_fast), d(beta_slow), d(attn_factor), _stream()))
     return out
+
+
+def _norm_weight(w, pages):
+    if w is None:
+        return None
+    if not (w.dtype in (torch.bfloat16, torch.int16) and w.shape == (pages.head_dim,) and w.is_contiguous() and w.device == pages.device):
+        raise HipsterError(1, "norm weights are bf16 [head_dim]")
+    return w.data_ptr()
 
 
 def kv_append(pages, k, v, table, row_start, kv_len, rope=None, q=None, q_out=None, interleaved=False, q_norm=None, k_norm=None, eps=1e-6):
@@ -242,12 +258,10 @@ def kv_append(pages, k, v, table, row_start, kv_len, rope=None, q=None, q_out=No
         _refuse(q_out.shape[1] == n_head, "kv_append: q_out has the heads of q")
     n_pos = n_rot = 0
     if rope is not None:
-        _refuse(rope.dtype == torch.float32 and rope.dim() == 3 and rope.shape[2] == 2 and rope.is_contiguous() and rope.device == pages.device, "kv_append: rope must be f32 [n_pos][n_rot / 2][2]")
-        n_pos, n_rot = rope.shape[0], 2 * rope.shape[1]
-    for w in (q_norm, k_norm):
-        _refuse(w is None or (w.element_size() == 2 and w.dtype != torch.float16 and w.shape == (pages.head_dim,) and w.is_contiguous() and w.device == pages.device), "kv_append: norm weights are bf16 [head_dim]")
-    check(hot().hp_kv_append(*qr, *qo, n_head, *kr, *vr, None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), None if rope is None else rope.data_ptr(), n_pos, n_rot,
-                             int(interleaved), table.data_ptr(), table.stride(0), row_start.data_ptr(), kv_len.data_ptr(), S, R, pages._at, eps, _raw_stream(_device())))
+        n_pos, n_rot, two = rope.shape
+        n_rot *= 2
+        _refuse(rope.dtype is torch.float32 and two == 2 and rope.is_contiguous() and rope.device == pages.device, "kv_append: rope must be f32 [n_pos][n_rot / 2][2]")
+    check(hot().hp_kv_append(*qr, *qo, n_head, *kr, *vr, _norm_weight(q_norm, pages), _norm_weight(k_norm, pages), None if rope is None else rope.data_ptr(), n_pos, n_rot, int(interleaved), table.data_ptr(), table.stride(0), row_start.data_ptr(), kv_len.data_ptr(), S, R, pages._at, eps, _raw_stream(_device())))
     return q_out
 
 
@@ -257,12 +271,12 @@ def kv_read(pages, table, row_start, kv_len, R=None, k_out=None, v_out=None):
     S = _batch(pages, table, row_start, kv_len)
     if k_out is None:
         _refuse(v_out is None and R is not None and R >= 1, "kv_read: give R, or both outputs")
-        k_out, v_out = torch.empty((2, R, pages.n_kv, pages.head_dim), dtype=torch.float16, device=pages.device)
-    R = k_out.shape[0]
-    for t in (k_out, v_out):
-        _refuse(t is not None and t.dtype == torch.float16 and t.dim() == 3 and t.shape == (R, pages.n_kv, pages.head_dim) and t.stride() == k_out.stride() and t.stride(2) == 1 and t.device == pages.device,
-                "kv_read: outputs are f16 [R][n_kv][head_dim] with the same strides")
-    check(hot().hp_kv_read(table.data_ptr(), table.stride(0), row_start.data_ptr(), kv_len.data_ptr(), S, R, pages._at, k_out.data_ptr(), v_out.data_ptr(), k_out.stride(0), k_out.stride(1), _raw_stream(_device())))
+        k_out, v_out = torch.empty((2, R, pages.n_kv, pages.head_dim), dtype=torch.float16, device=pages.device).unbind(0)
+    R, (ld, hs, one) = k_out.shape[0], k_out.stride()
+    if not (v_out is not None and k_out.shape == (R, pages.n_kv, pages.head_dim) and v_out.shape == k_out.shape and v_out.stride() == (ld, hs, 1) and one == 1 and k_out.dtype is torch.float16 and
+            v_out.dtype is torch.float16 and k_out.device == pages.device and v_out.device == pages.device):
+        raise HipsterError(1, "kv_read: outputs are f16 [R][n_kv][head_dim] with the same strides")
+    check(hot().hp_kv_read(table.data_ptr(), table.stride(0), row_start.data_ptr(), kv_len.data_ptr(), S, R, pages._at, k_out.data_ptr(), v_out.data_ptr(), ld, hs, _raw_stream(_device())))
     return k_out, v_out
 
 
