@@ -1,4 +1,5 @@
-// Attention of a ragged batch of rows over a cache of 8-bit pages (kv_pages.cu), with a window and first tokens that stay visible.
+// Attention of a ragged batch of rows over a cache of 8-bit pages (kv_pages.cu), with a window and first tokens that stay visible: calls of up to
+// 8 rows per sequence (decode steps, drafts, verify passes), the merge of the splits, and the plan. Prompts: attn_paged_tc.cu.
 //
 // Row r at position p of its sequence: o = sum_j w_j v_j / sum_j w_j over the keys j <= p with j > p - window or j < n_sink (no window: all), w_j =
 // 2^(s_j - mu), s_j = (q . k_j) * scale * log2 e, times sigmoid(gate). No key: zeros.
@@ -6,360 +7,297 @@
 // fp32 results from the f16 tensor pipe: codes of int8 and of e4m3 (times 2^-8) are exact in f16, a token's scale multiplies its score or its weight in
 // fp32, and q and the weights (times the scale of v) go in as two f16 each, the value and what is left of it: 22 bits. q is brought to [2^14, 2^15) by a
 // power of two per row, the weights by the reference mu: whole, at least the largest of s_j + log2(scale of v_j) - 14, so that a weight times
-// its scale stays below 2^15 and every rescaling is by a power of two, exact. The tensor pipe adds 16 keys (or head_dim products) at a time; these sums
-// are added to the running ones in fp32.
+// its scale stays below 2^15 and every rescaling is by a power of two, exact. The tensor pipe adds up head_dim / 2 products for a score, in three sums, and 16
+// keys for an output; these are added to the running sums in fp32.
 //
-// The pairs (row, head) of a sequence and kv head, row by row, are cut into blocks of up to 32; a CTA holds one block and the keys of one split, in tiles of
-// 64 keys through a ring of asynchronous copies. Four warps share 16 pairs, a quarter of each tile each, scores, weights and outputs in
-// registers from end to end. Splits lie at fixed positions and a warp's sums at fixed keys: a row's bits depend neither on the other rows of the call
-// nor on the other sequences.
+// Keys, and dims, are the 16 rows of mma.sync, the pairs (row of the batch, query head) of a kv head its 8 columns: few pairs waste nothing. A warp has 16 keys at a
+// time, every fourth such slice of its CTA's split, in a ring of three slots of its own (k, v, k, ...), so that no warp waits for another; 16 keys of a head
+// lie in one page, one run of memory. The weights change from rows of keys to columns of pairs by movmatrix. Splits lie at fixed positions and a
+// slice's keys at fixed lanes and warps: a row's bits depend neither on the other rows of the call nor on the other sequences.
 #include "paged.cuh"
 #include <algorithm>
 
 namespace hp {
 namespace {
 
-constexpr int TK = 64, KW = 4, KPW = TK / KW, KPAD = 32, VPAD = 16;   // keys of a tile, warps that share it, keys of a warp in it; bytes behind a row of k / v in shared memory: 64-bit reads of 4 rows x 4 lanes from distinct banks
-constexpr int MAX_TILES_M = 2;                           // 16-pair tiles of a CTA
-
+constexpr int KW = 4, KS = 16, SLOTS = 3;   // warps that share a split, keys of a slice, slots of a warp's ring
 __host__ __device__ constexpr int out_stride(int D) { return D + 4; }
-struct PagedArgs {
-    PagedPool pool; PagedBatch b;
-    const float* q; size_t q_ld, q_hs; int n_head, G; float scale2;   // scale2 = scale * log2 e (times 256 for e4m3)
-    int window, n_sink;
-    int U, ns, nwin, stages;    // keys of a split, splits of the first tokens, splits behind them, stages of the ring
-    float* pO; float2* pml;     // partials [row][head][ns + nwin] (x head_dim): sums, (mu, sum of weights)
-    int* err;
-};
+__host__ __device__ constexpr int smem_bytes(int D, int NT) {   // fragments of q | rings; the outputs of the warps pass through the same memory at the end
+    const int run = NT * D * 32 + KW * SLOTS * KS * D, end = KW * NT * 8 * out_stride(D) * 4;
+    return run > end ? run : end;
+}
 
-__host__ __device__ constexpr int stage_bytes(int D) { return TK * (2 * D + KPAD + VPAD) + 2 * TK * 4; }
-__host__ __device__ constexpr int q_bytes(int D, int m) { return m * D * 64; }   // per 16 pairs and 16 dims: two fragments (value, rest) of 32 lanes x 16 bytes
-
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ float pow2i(float d) { return d < -126.f ? 0.f : __uint_as_float((uint32_t)((int)d + 127) << 23); }   // 2^d, d whole and <= 0
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// Four codes as they are loaded -> what `pair` takes; bytes LO and LO + 1 of it as two f16. int8: the code plus 128 becomes the low bits of 1024 + code + 128,
-// and 1152 is subtracted, exactly. e4m3: its bits are those of the f16 2^-8 times as large, subnormals included (so 0x7f, which the quantiser does
-// not write, reads as 480 and not as NaN: bytes of absent tokens are harmless).
-template <int KIND> __device__ __forceinline__ uint32_t prepare4(uint32_t w) { return KIND == KV_I8 ? w ^ 0x80808080u : w; }
-template <int KIND, int LO> __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    if constexpr (KIND == KV_I8) {
-        const uint32_t h = prmt(w, 0x64646464u, LO == 0 ? 0x4140 : 0x4342);
-        return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&h), __floats2half2_rn(1152.f, 1152.f)));
-    } else {
-        const uint32_t h = prmt(w, 0u, LO == 0 ? 0x1404 : 0x3424);
-        return (h & 0x80008000u) | ((h >> 1) & 0x3f803f80u);
-    }
-}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) { uint32_t r; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v)); return r; }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void cp_async4_u(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_wait(int left) {
-    switch (left) {
-        case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-        case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-        case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-        default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    }
-}
 template <typename T> __device__ __forceinline__ T at_smem(const uint8_t* p) { return *reinterpret_cast<const T*>(p); }
-
-// The block of pairs that blockIdx.z stands for: sequences in order, each with ceil(T * G / MB) blocks.
-struct Block { PagedSeq q; int p0, np; };
-__device__ __forceinline__ Block find_block(const PagedBatch& b, int G, int MB, int blk, int lane, int* err) {
-    Block o; o.q.s = -1; o.p0 = o.np = 0;
-    int acc = 0;
-    for (int s0 = 0; s0 < b.S; s0 += 32) {
-        PagedSeq q{-1, 0, 0, 0};
-        if (s0 + lane < b.S) q = paged_seq(b, s0 + lane, err);
-        const int n = (q.T * G + MB - 1) / MB;
-        int incl = n;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) { const int t = __shfl_up_sync(0xffffffffu, incl, off); if (lane >= off) incl += t; }
-        const unsigned hit = __ballot_sync(0xffffffffu, acc + incl > blk);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            o.q.s = s0 + l; o.q.row0 = __shfl_sync(0xffffffffu, q.row0, l); o.q.T = __shfl_sync(0xffffffffu, q.T, l); o.q.len = __shfl_sync(0xffffffffu, q.len, l);
-            o.p0 = (blk - acc - __shfl_sync(0xffffffffu, incl - n, l)) * MB;
-            o.np = min(MB, o.q.T * G - o.p0);
-            return o;
-        }
-        acc += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    return o;
+// Where 16-byte piece c of row r of a slot lies. k is read as 8 bytes of four neighbouring rows and four neighbouring places, v of every second row: each
+// of these has to hit 16 different pairs of banks, so neighbours (v: every second) shift by two pieces. 64 dims: two rows share 128 bytes, and
+// rows 4 to 7 swap halves.
+template <int D, bool V> __device__ __forceinline__ int place(int r, int c) {
+    if constexpr (D == 64) return (r >> 1) * 128 + (((r & 1) ^ ((r >> 2) & 1)) << 6) + ((c ^ (((r >> 1) & 1) << 1)) << 4);
+    else return r * D + ((c ^ (((V ? r >> 1 : r) & 3) << 1)) << 4);
 }
 
-// grid (splits, n_kv, blocks), 128 threads per 16 pairs
-template <int D, int KIND>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_paged_split(PagedArgs a) {
-    constexpr int KS = D + KPAD, VS = D + VPAD, CPR = D / 16, NT = KPW / 8, XS = out_stride(D);   // row strides in shared memory, 16-byte pieces of a row, 8-key tiles of a warp
-    static_assert(NT == 2, "the weights of a warp are one fragment");
-    extern __shared__ __align__(16) uint8_t sm[];
-    const int tid = threadIdx.x, nthr = blockDim.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
-    const int MT = nthr / (32 * KW), MB = MT * 16, mw = warp / KW, kw = warp % KW;
-    uint8_t* const sQ = sm;
-    float* const sC = reinterpret_cast<float*>(sm + q_bytes(D, MT));        // [MB] factor of a pair's scores
-    int* const sPos = reinterpret_cast<int*>(sC + MB);                      // [MB] position of a pair's row, -1: no pair
-    uint8_t* const ring = reinterpret_cast<uint8_t*>(sPos + MB);
-    const uint32_t ring_u = smem_u32(ring);
+// grid (splits, n_kv, blocks), four warps; NT sets of 8 pairs
+template <int D, int KIND, int NT>
+__global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : (D == 256 ? 3 : 4)) k_paged_split(const PagedArgs a) {
+    constexpr int CPR = D / 16, MB = 8 * NT, XS = out_stride(D);   // 16-byte pieces of a row
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ float s_c[MB];   // factor of a pair's scores
+    __shared__ int s_pos[MB];   // position of a pair's row, -1: none
+    __shared__ float s_mu[KW][MB], s_l[KW][MB];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
     pdl_launch_dependents();
     pdl_wait();
-    const Block blk = find_block(a.b, a.G, MB, blockIdx.z, lane, a.err);
+    const Block blk = find_block(a.b, a.G, MB, blockIdx.z, lane, a.arg_err);
     if (blk.q.s < 0) return;
     const PagedSeq& sq = blk.q;
+    const Span sp = span_of(a, blk);
     const int kh = blockIdx.y;
-    const int pos_lo = sq.len - sq.T + blk.p0 / a.G, pos_hi = sq.len - sq.T + (blk.p0 + blk.np - 1) / a.G;
-    const int kend = pos_hi + 1, lo = a.window ? max(0, pos_lo - a.window + 1) : 0, sink = a.window ? a.n_sink : 0;   // keys [0, sink) and [lo, kend)
-    int split = blockIdx.x;
-    if (split >= a.ns) {   // the split of the window whose number leaves this remainder
-        const int w0 = max(a.ns, lo / a.U), m = (w0 - a.ns) % a.nwin, j = split - a.ns - m;
-        split = w0 + (j < 0 ? j + a.nwin : j);
+    if (sp.u0 >= sp.kend) return;
+    // slices of 16 keys [i * 16, i * 16 + 16): those of this warp leave remainder `warp`; first visible one at or behind i
+    const int i_end = (int)((sp.u1 + KS - 1) / KS), i_lo = sp.lo / KS;
+    auto first_from = [&](int i) {
+        if (i * KS >= sp.sink && i < i_lo) i += (i_lo - i + KW - 1) / KW * KW;
+        return i;
+    };
+    {   // is any slice of the split visible?
+        const int i0 = (int)(sp.u0 / KS);
+        if ((i0 * KS >= sp.sink && i0 < i_lo ? i_lo : i0) >= i_end) return;
     }
-    const long long u0 = (long long)split * a.U;
-    if (u0 >= kend) return;
-    const int t_end = (int)((min(u0 + a.U, (long long)kend) + TK - 1) / TK);
-    auto first_from = [&](int t) { return t * TK >= sink && t * TK + TK <= lo ? lo / TK : t; };   // first visible tile at or behind t
-    int lt = first_from((int)(u0 / TK));   // next tile to fetch
-    if (lt >= t_end) return;
-
-    // ---- fetching: a lane holds the page of 16-token pieces of the tile; key rows go round the threads
-    const int lg = a.pool.lg_page, pmask = (1 << lg) - 1, row_step = nthr / CPR, row_of = tid / CPR, col = (tid % CPR) * 16;
-    auto page_of = [&](int t) -> uint32_t {   // of the tile's page number `lane`
-        const int c = ((t * TK) >> lg) + lane;
-        uint32_t p = 0;
-        const long long k = (long long)c << lg;   // a page without a visible key is not looked up: page 0 stands for it, and for a number out of range
-        if (t < t_end && lane < max(1, TK >> lg) && k < kend && (k < sink || k + pmask >= lo)) p = paged_row(a.pool, sq.s, c, kh, a.err);
-        return p == 0xffffffffu ? 0u : p;
+    const int lg = a.pool.lg_page, pmask = (1 << lg) - 1;
+    auto row_of = [&](int i) -> uint32_t {   // the pool's row of the slice's first key; 0 behind the end, and for a page number out of range (told by the status word)
+        uint32_t r = 0;
+        if (i < i_end) { r = paged_row(a.pool, sq.s, (i * KS) >> lg, kh, a.arg_err); r = r == 0xffffffffu ? 0u : r + (uint32_t)((i * KS) & pmask); }
+        return r;
     };
-    uint32_t pages = page_of(lt);
-    auto fetch = [&](int slot) {
-        if (lt < t_end) {
-            const int k0 = lt * TK, c0 = k0 >> lg;
-            const uint32_t st = ring_u + slot * stage_bytes(D);
-#pragma unroll 4
-            for (int r0 = 0; r0 < TK; r0 += row_step) {   // the same number of steps for every lane
-                const int r = r0 + row_of, key = k0 + r;
-                const size_t at = (size_t)__shfl_sync(0xffffffffu, pages, (key >> lg) - c0) + (key & pmask);
-                if (r < TK && key < kend) {
-                    cp_async16(st + r * KS + col, a.pool.k + at * D + col);
-                    cp_async16(st + TK * KS + r * VS + col, a.pool.v + at * D + col);
-                }
+    uint8_t* const ring = sm + NT * D * 32 + warp * (SLOTS * KS * D);
+    const uint32_t ring_u = smem_u32(ring);
+    auto fetch = [&](int slot, const uint8_t* src, bool v, bool live) {   // 16 rows, one run of memory
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < KS * CPR / 32; ++i) {
+                const int e = i * 32 + lane, r = e / CPR, c = e % CPR;
+                cp_async16(ring_u + slot * (KS * D) + (v ? place<D, true>(r, c) : place<D, false>(r, c)), src + e * 16);
             }
-            for (int i = warp * 32; i < 2 * TK; i += nthr) {
-                const int r = (i + lane) & (TK - 1), key = k0 + r;
-                const size_t at = (size_t)__shfl_sync(0xffffffffu, pages, (key >> lg) - c0) + (key & pmask);
-                if (key < kend) cp_async4_u(st + TK * (KS + VS) + (i + lane) * 4, (i < TK ? a.pool.k_scale : a.pool.v_scale) + at);
-            }
-            lt = first_from(lt + 1);
-            pages = page_of(lt);
         }
-        cp_commit();
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    int ct = lt;   // tile to compute
-    for (int i = 0; i + 1 < a.stages; ++i) fetch(i);
+    int i0 = first_from((int)(sp.u0 / KS) + ((warp - (int)(sp.u0 / KS)) & (KW - 1)));   // this slice, the next ones and where they lie
+    int i1 = first_from(i0 + KW), i2 = first_from(i1 + KW);
+    uint32_t r0 = row_of(i0), r1 = row_of(i1);
+    fetch(0, a.pool.k + (size_t)r0 * D, false, i0 < i_end);
+    fetch(1, a.pool.v + (size_t)r0 * D, true, i0 < i_end);
+    fetch(2, a.pool.k + (size_t)r1 * D, false, i1 < i_end);
+    auto scales = [&](uint32_t r) { return (lane < 16 ? a.pool.k_scale : a.pool.v_scale)[(size_t)r + (lane & 15)]; };   // of k in lanes 0 to 15, of v in the others
+    float sc = i0 < i_end ? scales(r0) : 0.f;
+    uint32_t r2 = row_of(i2);
 
-    // ---- q: a warp per pair; its 8 dims of a lane are one fragment word of two steps of 16 dims each, for the values and for the rests
-    for (int i = warp; i < MB; i += nthr >> 5) {
-        float x[8];
+    // ---- q: a warp per pair; the 8 dims of a lane are its words of two steps of 16 dims, values and rests
+    for (int i = warp; i < MB; i += KW) {
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         uint32_t m = 0;
         const bool live = i < blk.np;
         const int p = blk.p0 + i, t = live ? p / a.G : 0;
-        if (lane < D / 8) {
-            float4 x0 = make_float4(0.f, 0.f, 0.f, 0.f), x1 = x0;
-            if (live) {
-                const float4* src = reinterpret_cast<const float4*>(a.q + (size_t)(sq.row0 + t) * a.q_ld + (size_t)(kh * a.G + p - t * a.G) * a.q_hs) + 2 * lane;
-                x0 = src[0]; x1 = src[1];
-            }
+        if (live && lane < D / 8) {
+            const float4* src = reinterpret_cast<const float4*>(a.q + (size_t)(sq.row0 + t) * a.q_ld + (size_t)(kh * a.G + p - t * a.G) * a.q_hs) + 2 * lane;
+            const float4 x0 = src[0], x1 = src[1];
             x[0] = x0.x; x[1] = x0.y; x[2] = x0.z; x[3] = x0.w; x[4] = x1.x; x[5] = x1.y; x[6] = x1.z; x[7] = x1.w;
 #pragma unroll
             for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
         }
         m = __reduce_max_sync(0xffffffffu, m);
-        const int e = m == 0 || m >= 0x7f800000u ? 0 : min(100, 14 - ((int)(m >> 23) - 127));
+        const int e = q_exponent(m);
         const float up = __uint_as_float((uint32_t)(e + 127) << 23);
         if (lane < D / 8) {
-            uint32_t* dst = reinterpret_cast<uint32_t*>(sQ + (size_t)(i >> 4) * D * 64 + (lane >> 2) * 2048) + ((i & 7) * 4 + (lane & 3)) * 4 + ((i >> 3) & 1);
+            uint32_t h[4], r[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {   // dims 2 j, 2 j + 1: step j / 2, words 0 and 2 (rows 8 and more: 1 and 3)
+            for (int j = 0; j < 4; ++j) {
                 const float y0 = x[2 * j] * up, y1 = x[2 * j + 1] * up;
-                const __half2 h = __floats2half2_rn(y0, y1);
-                const float2 f = __half22float2(h);
-                const __half2 l = __floats2half2_rn(y0 - f.x, y1 - f.y);
-                dst[(j >> 1) * 256 + (j & 1) * 2] = h2_bits(h);
-                dst[(j >> 1) * 256 + 128 + (j & 1) * 2] = h2_bits(l);
+                const __half2 hh = __floats2half2_rn(y0, y1);
+                const float2 f = __half22float2(hh);
+                h[j] = h2_bits(hh); r[j] = h2_bits(__floats2half2_rn(y0 - f.x, y1 - f.y));
             }
+            uint4* dst = reinterpret_cast<uint4*>(sm + (i >> 3) * D * 32 + (lane >> 2) * 1024) + (i & 7) * 4 + (lane & 3);
+            dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            dst[32] = make_uint4(r[0], r[1], r[2], r[3]);
         }
-        if (lane == 0) { sC[i] = a.scale2 * __uint_as_float((uint32_t)(127 - e) << 23); sPos[i] = live ? max(-1, sq.len - sq.T + t) : -1; }
+        if (lane == 0) { s_c[i] = a.scale2 * __uint_as_float((uint32_t)(127 - e) << 23); s_pos[i] = live ? max(-1, sq.len - sq.T + t) : -1; }
     }
     __syncthreads();
-    const int i0 = mw * 16 + g, i1 = i0 + 8;   // this lane's pairs
-    const float c0 = sC[i0], c1 = sC[i1];
-    const int p0 = sPos[i0], p1 = sPos[i1];
-    const int w0 = a.window ? p0 - a.window : -1, w1 = a.window ? p1 - a.window : -1;   // keys behind these, or in front of `sink`
-    const int mpos = (int)__reduce_max_sync(0xffffffffu, (unsigned)(max(p0, p1) + 1)) - 1;   // last position of the 16 pairs
-    // tiles between these positions are visible to all 16 (an absent pair counts as nothing)
-    const int all_hi = (int)__reduce_min_sync(0xffffffffu, (unsigned)min(p0 < 0 ? 0x7fffffff : p0, p1 < 0 ? 0x7fffffff : p1));
-    const int all_lo = a.window ? mpos - a.window : -1;
-    const uint8_t* const qf = sQ + mw * D * 64 + lane * 16;
-
-    float O[D / 8][4];
+    float cf[NT][2], mu[NT][2], l[NT][2];
+    int pos[NT][2];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) { O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.f; }
-    float mu0 = -1e30f, mu1 = -1e30f, l0 = 0.f, l1 = 0.f;
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) { cf[n][c] = s_c[8 * n + 2 * q4 + c]; pos[n][c] = s_pos[8 * n + 2 * q4 + c]; mu[n][c] = -1e30f; l[n][c] = 0.f; }
+    const int win = a.window ? a.window : 1 << 30;
+    // slices between these positions are visible to all pairs
+    const int all_hi = sp.pos_lo, all_lo = a.window ? sp.pos_hi - a.window : -1;
+    const uint8_t* const qf = sm + lane * 16;
 
-    for (int slot = 0; ct < t_end; ct = first_from(ct + 1), slot = slot + 1 == a.stages ? 0 : slot + 1) {
-        cp_wait(a.stages - 2);
-        __syncthreads();
-        fetch(slot == 0 ? a.stages - 1 : slot - 1);
-        const int kb = ct * TK + kw * KPW;
-        if (kb > mpos) continue;   // nothing of this half is visible to these pairs
-        const uint8_t* const st = ring + slot * stage_bytes(D);
-        // ---- scores of 16 pairs x 16 keys
-        float s[NT][4], sl[NT][4];
+    float O[D / 16][NT][4];   // dims (tile m of 64 y: 64 y + 8 g + 2 m, and the next one) x pairs (2 q4, 2 q4 + 1)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) { O[i][n][0] = O[i][n][1] = O[i][n][2] = O[i][n][3] = 0.f; }
+
+    int slot = 0;
+    for (; i0 < i_end; ) {
+        const float sc1 = i1 < i_end ? scales(r1) : 0.f;
+        const int i3 = first_from(i2 + KW);
+        const uint32_t r3 = row_of(i3);
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        __syncwarp();
+        // ---- scores of 16 keys
+        float s[NT][4];
+        {
+            float sh[NT][2][4], sl[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sh[n][0][c] = sh[n][1][c] = sl[n][c] = 0.f;
+            const uint8_t* kr = ring + slot * (KS * D);
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+                const uint2 ka = at_smem<uint2>(kr + place<D, false>(g, 2 * x + (q4 >> 1)) + (q4 & 1) * 8), kb = at_smem<uint2>(kr + place<D, false>(g + 8, 2 * x + (q4 >> 1)) + (q4 & 1) * 8);
+                const uint32_t a0[4] = {code_pair<KIND, 0>(ka.x), code_pair<KIND, 0>(kb.x), code_pair<KIND, 2>(ka.x), code_pair<KIND, 2>(kb.x)};
+                const uint32_t a1[4] = {code_pair<KIND, 0>(ka.y), code_pair<KIND, 0>(kb.y), code_pair<KIND, 2>(ka.y), code_pair<KIND, 2>(kb.y)};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint4 h = at_smem<uint4>(qf + n * D * 32 + x * 1024), r = at_smem<uint4>(qf + n * D * 32 + x * 1024 + 512);
+                    mma_f16(sh[n][0], a0, h.x, h.y); mma_f16(sl[n], a0, r.x, r.y);
+                    mma_f16(sh[n][1], a1, h.z, h.w); mma_f16(sl[n], a1, r.z, r.w);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[n][c] = (sh[n][0][c] + sh[n][1][c]) + sl[n][c];
+        }
+        __syncwarp();
+        fetch(slot, a.pool.v + (size_t)r1 * D, true, i1 < i_end);
+        slot = slot + 1 == SLOTS ? 0 : slot + 1;
+        // ---- weights
+        const float k0 = __shfl_sync(0xffffffffu, sc, g), k1 = __shfl_sync(0xffffffffu, sc, g + 8), v0 = __shfl_sync(0xffffffffu, sc, g + 16), v1 = __shfl_sync(0xffffffffu, sc, g + 24);
+        const float lv0 = lg2(fmaxf(v0, 8.0779357e-28f)), lv1 = lg2(fmaxf(v1, 8.0779357e-28f));   // 2^-90: the weights' sum cannot overflow
+        const int j = i0 * KS + g;
+        const bool whole = i0 * KS + KS - 1 <= all_hi && (i0 * KS > all_lo || i0 * KS + KS <= sp.sink);
+        bool hide[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) s[n][c] = sl[n][c] = 0.f;
-        {
-            const uint8_t* kr = st + (kw * KPW + g) * KS + q4 * 8;
-#pragma unroll
-            for (int x = 0; x < D / 32; ++x) {
-                const uint4 h0 = at_smem<uint4>(qf + x * 2048), r0 = at_smem<uint4>(qf + x * 2048 + 512), h1 = at_smem<uint4>(qf + x * 2048 + 1024), r1 = at_smem<uint4>(qf + x * 2048 + 1536);
-                uint32_t b[NT][4];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const uint2 kk = at_smem<uint2>(kr + n * 8 * KS + x * 32);
-                    const uint32_t w0 = prepare4<KIND>(kk.x), w1 = prepare4<KIND>(kk.y);
-                    b[n][0] = pair<KIND, 0>(w0); b[n][1] = pair<KIND, 2>(w0); b[n][2] = pair<KIND, 0>(w1); b[n][3] = pair<KIND, 2>(w1);
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) { mma_f16(s[n], h0, b[n][0], b[n][1]); mma_f16(sl[n], r0, b[n][0], b[n][1]); }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) { mma_f16(s[n], h1, b[n][2], b[n][3]); mma_f16(sl[n], r1, b[n][2], b[n][3]); }
-            }
-        }
-        // ---- weights
-        const uint8_t* sc = st + TK * (KS + VS) + (kw * KPW + 2 * q4) * 4;
-        float2 vs[NT];
-        float t0 = -INFINITY, t1 = -INFINITY;
-        const bool whole = kb + KPW - 1 <= all_hi && (kb > all_lo || kb + KPW <= sink);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float2 ks = at_smem<float2>(sc + n * 32);
-            vs[n] = at_smem<float2>(sc + TK * 4 + n * 32);
-            s[n][0] = (s[n][0] + sl[n][0]) * (ks.x * c0); s[n][1] = (s[n][1] + sl[n][1]) * (ks.y * c0);
-            s[n][2] = (s[n][2] + sl[n][2]) * (ks.x * c1); s[n][3] = (s[n][3] + sl[n][3]) * (ks.y * c1);
-        }
-        float wv[NT][4];   // the scale of v that a weight takes
-#pragma unroll
-        for (int n = 0; n < NT; ++n) { wv[n][0] = wv[n][2] = vs[n].x; wv[n][1] = wv[n][3] = vs[n].y; }
+            for (int c = 0; c < 4; ++c) { s[n][c] = s[n][c] * ((c < 2 ? k0 : k1) * cf[n][c & 1]); hide[n][c] = false; }
         if (!whole) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const int key = kb + n * 8 + 2 * q4 + (c & 1);
-                    const bool see = key <= (c < 2 ? p0 : p1) && (key > (c < 2 ? w0 : w1) || key < sink);
-                    if (!see) { s[n][c] = -INFINITY; wv[n][c] = 0.f; }
+                    const int key = c < 2 ? j : j + 8, p = pos[n][c & 1];
+                    hide[n][c] = !(key <= p && (key > p - win || key < sp.sink));
+                    if (hide[n][c]) s[n][c] = -INFINITY;
                 }
         }
+        uint32_t bh[NT][2], br[NT][2];   // weights times scales of v as columns of pairs: values and rests
+        float al[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float lx = lg2(fmaxf(vs[n].x, 8.0779357e-28f)), ly = lg2(fmaxf(vs[n].y, 8.0779357e-28f));   // 2^-90: the weights' sum cannot overflow
-            t0 = fmaxf(t0, fmaxf(s[n][0] + lx, s[n][1] + ly));
-            t1 = fmaxf(t1, fmaxf(s[n][2] + lx, s[n][3] + ly));
+            float y[4];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float t = fmaxf(s[n][c] + lv0, s[n][c + 2] + lv1);
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                const float next = fmaxf(mu[n][c], ceilf(t) - 14.f);
+                al[n][c] = pow2i(mu[n][c] - next); mu[n][c] = next;
+                const float e0 = ex2(s[n][c] - next), e1 = ex2(s[n][c + 2] - next);
+                l[n][c] = fmaf(l[n][c], al[n][c], e0 + e1);
+                y[c] = hide[n][c] ? 0.f : e0 * v0; y[c + 2] = hide[n][c + 2] ? 0.f : e1 * v1;   // a masked key's scale may be anything
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const __half2 hh = __floats2half2_rn(y[2 * c], y[2 * c + 1]);
+                const float2 f = __half22float2(hh);
+                bh[n][c] = transpose8(h2_bits(hh)); br[n][c] = transpose8(h2_bits(__floats2half2_rn(y[2 * c] - f.x, y[2 * c + 1] - f.y)));
+            }
         }
-        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1)); t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
-        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2)); t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
-        const float n0 = fmaxf(mu0, ceilf(t0) - 14.f), n1 = fmaxf(mu1, ceilf(t1) - 14.f);
-        const float al0 = pow2i(mu0 - n0), al1 = pow2i(mu1 - n1);
-        mu0 = n0; mu1 = n1; l0 = l0 * al0; l1 = l1 * al1;
-        uint4 ph, pr;   // A fragment of the 16 keys: weights times scales, values and rests
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        __syncwarp();
+        // ---- outputs: 64 dims at a time; the 8 dims of a lane group are four tiles of 16 rows
         {
-            uint32_t h[NT][2], r[NT][2];
+            const uint8_t* vr = ring + slot * (KS * D);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int y = 0; y < D / 64; ++y) {
+                uint2 v[4];   // keys 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
 #pragma unroll
-                for (int c = 0; c < 4; c += 2) {
-                    const float m = c ? mu1 : mu0, e0 = ex2(s[n][c] - m), e1 = ex2(s[n][c + 1] - m);
-                    if (c) l1 = (l1 + e0) + e1; else l0 = (l0 + e0) + e1;
-                    const float y0 = e0 * wv[n][c], y1 = e1 * wv[n][c + 1];
-                    const __half2 hh = __floats2half2_rn(y0, y1);
-                    const float2 f = __half22float2(hh);
-                    h[n][c / 2] = h2_bits(hh); r[n][c / 2] = h2_bits(__floats2half2_rn(y0 - f.x, y1 - f.y));
-                }
-            }
-            ph = make_uint4(h[0][0], h[0][1], h[1][0], h[1][1]); pr = make_uint4(r[0][0], r[0][1], r[1][0], r[1][1]);
-        }
-        // ---- outputs: 64 dims at a time, lane group g holds 8 neighbouring ones of the rows of its keys
-        const uint8_t* vr = st + TK * KS + (kw * KPW + 2 * q4) * VS + g * 8;
+                for (int i = 0; i < 4; ++i) v[i] = at_smem<uint2>(vr + place<D, true>(2 * q4 + (i & 1) + (i >> 1) * 8, 4 * y + (g >> 1)) + (g & 1) * 8);
 #pragma unroll
-        for (int y = 0; y < D / 64; ++y) {
-            const uint2 v0 = at_smem<uint2>(vr + y * 64), v1 = at_smem<uint2>(vr + VS + y * 64), v2 = at_smem<uint2>(vr + 8 * VS + y * 64), v3 = at_smem<uint2>(vr + 9 * VS + y * 64);
+                for (int w = 0; w < 2; ++w) {
+                    const uint32_t x0 = w ? v[0].y : v[0].x, x1 = w ? v[1].y : v[1].x, x2 = w ? v[2].y : v[2].x, x3 = w ? v[3].y : v[3].x;
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const uint32_t a0 = prepare4<KIND>(w ? v0.y : v0.x), a1 = prepare4<KIND>(w ? v1.y : v1.x), a2 = prepare4<KIND>(w ? v2.y : v2.x), a3 = prepare4<KIND>(w ? v3.y : v3.x);
-                const uint32_t u0 = prmt(a0, a1, 0x5140), u1 = prmt(a0, a1, 0x7362), u2 = prmt(a2, a3, 0x5140), u3 = prmt(a2, a3, 0x7362);
-                const uint32_t b0[4] = {pair<KIND, 0>(u0), pair<KIND, 2>(u0), pair<KIND, 0>(u1), pair<KIND, 2>(u1)};
-                const uint32_t b1[4] = {pair<KIND, 0>(u2), pair<KIND, 2>(u2), pair<KIND, 0>(u3), pair<KIND, 2>(u3)};
-                float f[4][4];
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t lo2 = __byte_perm(x0, x1, h ? 0x7362 : 0x5140), hi2 = __byte_perm(x2, x3, h ? 0x7362 : 0x5140);
+                        const uint32_t af[4] = {code_pair<KIND, 0>(lo2), code_pair<KIND, 2>(lo2), code_pair<KIND, 0>(hi2), code_pair<KIND, 2>(hi2)};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { f[j][0] = f[j][1] = f[j][2] = f[j][3] = 0.f; mma_f16(f[j], pr, b0[j], b1[j]); }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mma_f16(f[j], ph, b0[j], b1[j]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float (&o)[4] = O[y * 8 + w * 4 + j];
-                    o[0] = fmaf(o[0], al0, f[j][0]); o[1] = fmaf(o[1], al0, f[j][1]); o[2] = fmaf(o[2], al1, f[j][2]); o[3] = fmaf(o[3], al1, f[j][3]);
+                        for (int n = 0; n < NT; ++n) {
+                            float f[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_f16(f, af, br[n][0], br[n][1]);
+                            mma_f16(f, af, bh[n][0], bh[n][1]);
+                            float (&o)[4] = O[y * 4 + w * 2 + h][n];
+                            o[0] = fmaf(o[0], al[n][0], f[0]); o[1] = fmaf(o[1], al[n][1], f[1]); o[2] = fmaf(o[2], al[n][0], f[2]); o[3] = fmaf(o[3], al[n][1], f[3]);
+                        }
+                    }
                 }
             }
         }
+        __syncwarp();
+        fetch(slot, a.pool.k + (size_t)r2 * D, false, i2 < i_end);
+        slot = slot + 1 == SLOTS ? 0 : slot + 1;
+        i0 = i1; i1 = i2; i2 = i3; r1 = r2; r2 = r3; sc = sc1;
     }
-    l0 = l0 + __shfl_xor_sync(0xffffffffu, l0, 1); l1 = l1 + __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 = l0 + __shfl_xor_sync(0xffffffffu, l0, 2); l1 = l1 + __shfl_xor_sync(0xffffffffu, l1, 2);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) l[n][c] = l[n][c] + __shfl_xor_sync(0xffffffffu, l[n][c], off);
 
-    // ---- the warps that share the tiles meet, in order. Thread (g, q4) holds dims 64 y + 16 q4 + 0..15 of rows g and g + 8
-    cp_wait(0);
-    __syncthreads();   // the ring and q are free
-    float* const xo = reinterpret_cast<float*>(sm);   // [warp][16][XS]: D sums, mu, sum of weights
-    {
-        float* dst = xo + (size_t)(warp * 16 + g) * XS + 16 * q4;
+    // ---- the warps meet, in order
+    cp_async_wait_all();
+    __syncthreads();   // rings and q are free
+    float* const xo = reinterpret_cast<float*>(sm);   // [warp][pair][XS]
 #pragma unroll
-        for (int y = 0; y < D / 64; ++y)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 8; j += 4)
+        for (int c = 0; c < 2; ++c) {
+            float* dst = xo + (size_t)(warp * MB + 8 * n + 2 * q4 + c) * XS + 8 * g;
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    *reinterpret_cast<float4*>(dst + (c >> 1) * 8 * XS + 64 * y + 8 * (c & 1) + j) = make_float4(O[y * 8 + j][c], O[y * 8 + j + 1][c], O[y * 8 + j + 2][c], O[y * 8 + j + 3][c]);
-        if (q4 == 0) {
-            float* e = xo + (size_t)(warp * 16 + g) * XS + D;
-            e[0] = mu0; e[1] = l0; e[8 * XS] = mu1; e[8 * XS + 1] = l1;
+            for (int y = 0; y < D / 64; ++y)
+#pragma unroll
+                for (int m = 0; m < 4; m += 2)
+                    *reinterpret_cast<float4*>(dst + 64 * y + 2 * m) = make_float4(O[y * 4 + m][n][c], O[y * 4 + m][n][c + 2], O[y * 4 + m + 1][n][c], O[y * 4 + m + 1][n][c + 2]);
+            if (g == 0) { s_mu[warp][8 * n + 2 * q4 + c] = mu[n][c]; s_l[warp][8 * n + 2 * q4 + c] = l[n][c]; }
         }
-    }
     __syncthreads();
-    for (int i = warp; i < blk.np; i += nthr >> 5) {   // a warp per pair
+    for (int i = warp; i < blk.np; i += KW) {   // a warp per pair
         const int p = blk.p0 + i, t = p / a.G;
-        if (sq.len - sq.T + t < 0) continue;
-        const float* src = xo + (size_t)((i >> 4) * KW * 16 + (i & 15)) * XS;
-        float m[KW], w[KW], mu = -INFINITY, l = 0.f;
+        if (s_pos[i] < 0) continue;
+        float w[KW], m = -INFINITY, ls = 0.f;
 #pragma unroll
-        for (int k = 0; k < KW; ++k) { m[k] = src[k * 16 * XS + D]; mu = fmaxf(mu, m[k]); }
+        for (int k = 0; k < KW; ++k) m = fmaxf(m, s_mu[k][i]);
 #pragma unroll
-        for (int k = 0; k < KW; ++k) { w[k] = pow2i(m[k] - mu); l = fmaf(src[k * 16 * XS + D + 1], w[k], l); }
+        for (int k = 0; k < KW; ++k) { w[k] = pow2i(s_mu[k][i] - m); ls = fmaf(s_l[k][i], w[k], ls); }
         const size_t at = ((size_t)(sq.row0 + t) * a.n_head + kh * a.G + p - t * a.G) * (a.ns + a.nwin) + blockIdx.x;
         for (int d = 2 * lane; d < D; d += 64) {
             float2 o = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < KW; ++k) { const float2 v = *reinterpret_cast<const float2*>(src + k * 16 * XS + d); o.x = fmaf(v.x, w[k], o.x); o.y = fmaf(v.y, w[k], o.y); }
+            for (int k = 0; k < KW; ++k) { const float2 v = *reinterpret_cast<const float2*>(xo + (size_t)(k * MB + i) * XS + d); o.x = fmaf(v.x, w[k], o.x); o.y = fmaf(v.y, w[k], o.y); }
             *reinterpret_cast<float2*>(a.pO + at * D + d) = o;
         }
-        if (lane == 0) a.pml[at] = make_float2(mu, l);
+        if (lane == 0) a.pml[at] = make_float2(m, ls);
     }
 }
 
@@ -401,38 +339,40 @@ __global__ void __launch_bounds__(256) k_paged_merge(MergeArgs a) {
     if (a.oq) warp_quant32_store(v, r, (head * a.D + d) >> 5, a.n_head * a.D, a.oq, a.osc, lane);
 }
 
-struct Plan { int U, ns, nwin, MT; long long blocks; };
+struct Plan { int U, ns, nwin, MB; long long blocks; };
 // Splits lie at multiples of U, a number that the cache's capacity and the window alone decide, so that a row's sums do not hang on what else is in the
 // call. Calls of more than 8 rows per sequence (prompts) have blocks enough and take a row's keys as one split.
 Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink) {
     Plan p;
     const int G = n_head / pool.n_kv, cap = pool.table_ld << pool.lg_page;
     const long long eff = window ? std::min<long long>(cap, (long long)window + n_sink) : cap;
-    const long long pairs = (long long)b.max_rows * G, nb = (pairs + 16 * MAX_TILES_M - 1) / (16 * MAX_TILES_M);
-    p.MT = (int)std::min<long long>(MAX_TILES_M, ((pairs + nb - 1) / nb + 15) / 16);
-    const int MB = p.MT * 16;
-    p.blocks = std::min<long long>((long long)b.S * ((pairs + MB - 1) / MB), (long long)b.R * G / MB + b.S);
+    const long long pairs = (long long)b.max_rows * G;
+    p.MB = b.max_rows > 8 ? PAGED_TC_PAIRS : pairs <= 8 ? 8 : 16;
+    p.blocks = std::min<long long>((long long)b.S * ((pairs + p.MB - 1) / p.MB), (long long)b.R * G / p.MB + b.S);
     if (b.max_rows > 8) { p.U = 1 << 30; p.ns = 0; p.nwin = 1; return p; }
-    p.U = eff <= 8192 ? 256 : eff <= 32768 ? 512 : 1024;
+    p.U = eff <= 8192 ? 512 : 1024;
     const int total = (b.max_kv + p.U - 1) / p.U;   // splits of the longest sequence
     p.ns = window ? std::min((n_sink + p.U - 1) / p.U, total) : 0;
     p.nwin = std::max(1, total);
     if (window) {   // a block's rows see at most this many keys in a run
-        const long long rows = std::min<long long>(b.max_rows, (MB - 1) / G + 2), run = (long long)window + rows - 1;
+        const long long rows = std::min<long long>(b.max_rows, (p.MB - 1) / G + 2), run = (long long)window + rows - 1;
         p.nwin = (int)std::min<long long>(p.nwin, run < 2 ? 1 : (run - 2) / p.U + 2);
     }
     return p;
 }
 size_t partials(const Plan& p, const PagedBatch& b, int n_head) { return (size_t)b.R * n_head * (p.ns + p.nwin); }
 
-template <int D, int KIND> int launch_split(const PagedArgs& a, dim3 grid, int MT, cudaStream_t s) {
+template <int D, int KIND, int NT> int launch_split(const PagedArgs& a, dim3 grid, cudaStream_t s) {
+    constexpr int smem = smem_bytes(D, NT);
     static bool attr[MAX_DEVICES] = {};   // per device: the opt-in belongs to the device's copy of the kernel
     const int dev = current_device(); if (dev < 0) return HP_ECUDA;
-    if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_split<D, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024)); attr[dev] = true; }
-    // the outputs of the tiles' halves pass through the same memory at the end
-    const size_t smem = std::max<size_t>(q_bytes(D, MT) + MT * 16 * 8 + (size_t)a.stages * stage_bytes(D), (size_t)KW * MT * 16 * out_stride(D) * 4);
-    HP_CUDA(launch_pdl<4>(k_paged_split<D, KIND>, grid, dim3(32 * KW * MT), smem, s, a));
+    if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_split<D, KIND, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); attr[dev] = true; }
+    HP_CUDA(launch_pdl<4>(k_paged_split<D, KIND, NT>, grid, dim3(32 * KW), smem, s, a));
     return HP_OK;
+}
+template <int D, int KIND> int launch_split(const PagedArgs& a, dim3 grid, int MB, cudaStream_t s) { return MB == 8 ? launch_split<D, KIND, 1>(a, grid, s) : launch_split<D, KIND, 2>(a, grid, s); }
+template <int KIND> int launch_split(const PagedArgs& a, dim3 grid, int MB, cudaStream_t s) {
+    return a.pool.head_dim == 256 ? launch_split<256, KIND>(a, grid, MB, s) : a.pool.head_dim == 128 ? launch_split<128, KIND>(a, grid, MB, s) : launch_split<64, KIND>(a, grid, MB, s);
 }
 
 }  // namespace
@@ -447,15 +387,13 @@ int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams
     HP_REQUIRE(pl.blocks <= 65535 && (long long)b.R * p.n_head < (1ll << 31), "attn_paged: too many rows (%d) for one call", b.R);
     PagedArgs a; a.pool = pool; a.b = b; a.q = p.q; a.q_ld = p.q_ld; a.q_hs = p.q_hs; a.n_head = p.n_head; a.G = p.n_head / pool.n_kv;
     a.scale2 = (float)((double)p.scale * 1.4426950408889634074 * (pool.kind == KV_E4M3 ? 256.0 : 1.0)); a.window = p.window; a.n_sink = p.n_sink;
-    a.U = pl.U; a.ns = pl.ns; a.nwin = pl.nwin; a.stages = pool.head_dim == 256 ? (pl.MT == 1 ? 2 : 4) : 3;
-    a.pO = (float*)p.workspace; a.pml = (float2*)(a.pO + partials(pl, b, p.n_head) * pool.head_dim); a.err = device_arg_flag();
+    a.U = pl.U; a.ns = pl.ns; a.nwin = pl.nwin;
+    a.pO = (float*)p.workspace; a.pml = (float2*)(a.pO + partials(pl, b, p.n_head) * pool.head_dim); a.err = device_err_flag(); a.arg_err = device_arg_flag();
     const dim3 grid(pl.ns + pl.nwin, pool.n_kv, (unsigned)pl.blocks);
-    int rc;
-    if (pool.kind == KV_I8) rc = pool.head_dim == 256 ? launch_split<256, KV_I8>(a, grid, pl.MT, s) : pool.head_dim == 128 ? launch_split<128, KV_I8>(a, grid, pl.MT, s) : launch_split<64, KV_I8>(a, grid, pl.MT, s);
-    else rc = pool.head_dim == 256 ? launch_split<256, KV_E4M3>(a, grid, pl.MT, s) : pool.head_dim == 128 ? launch_split<128, KV_E4M3>(a, grid, pl.MT, s) : launch_split<64, KV_E4M3>(a, grid, pl.MT, s);
+    const int rc = b.max_rows > 8 ? attn_paged_tc(a, grid, s) : pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, pl.MB, s) : launch_split<KV_E4M3>(a, grid, pl.MB, s);
     if (rc != HP_OK) return rc;
     MergeArgs m; m.b = b; m.pO = a.pO; m.pml = a.pml; m.gate = p.gate; m.g_ld = p.g_ld; m.g_hs = p.g_hs; m.n_head = p.n_head; m.D = pool.head_dim; m.window = p.window; m.n_sink = p.n_sink;
-    m.U = pl.U; m.ns = pl.ns; m.nwin = pl.nwin; m.mul = pool.kind == KV_E4M3 ? 256.f : 1.f; m.out = p.out; m.oq = (int8_t*)p.xq.q; m.osc = (float*)p.xq.sc; m.err = a.err;
+    m.U = pl.U; m.ns = pl.ns; m.nwin = pl.nwin; m.mul = pool.kind == KV_E4M3 ? 256.f : 1.f; m.out = p.out; m.oq = (int8_t*)p.xq.q; m.osc = (float*)p.xq.sc; m.err = a.arg_err;
     HP_CUDA(launch_pdl<4>(k_paged_merge, dim3((unsigned)(b.R * p.n_head)), dim3(pool.head_dim), 0, s, m));
     return HP_OK;
 }

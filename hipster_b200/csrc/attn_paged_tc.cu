@@ -1,0 +1,426 @@
+// Attention of a ragged batch of rows over a cache of 8-bit pages (kv_pages.cu), with a window and first tokens that stay visible.
+//
+// Row r at position p of its sequence: o = sum_j w_j v_j / sum_j w_j over the keys j <= p with j > p - window or j < n_sink (no window: all), w_j =
+// 2^(s_j - mu), s_j = (q . k_j) * scale * log2 e, times sigmoid(gate). No key: zeros.
+//
+// fp32 results from the f16 tensor pipe: codes of int8 and of e4m3 (times 2^-8) are exact in f16, a token's scale multiplies its score or its weight in
+// fp32, and q and the weights (times the scale of v) go in as two f16 each, the value and what is left of it: 22 bits. q is brought to [2^14, 2^15) by a
+// power of two per row, the weights by the reference mu: whole, at least the largest of s_j + log2(scale of v_j) - 14, so that a weight times
+// its scale stays below 2^15 and every rescaling is by a power of two, exact. The tensor pipe adds up head_dim products for a score and the 128 keys of a tile
+// for an output; tiles are added in fp32 registers.
+//
+// Both products stand on their heads: keys, then dims, are the 128 rows of tcgen05.mma, and its columns are the pairs (row of the batch, query head) of a
+// kv head, each twice: column i its values, column n + i what is left of them. So the tensor pipe's time goes with the number of pairs (16 pairs: 32 columns),
+// a thread that reads a row of the accumulator has value and rest of every pair at hand, needs one scale of k and of v, and adds up its own keys' weights without
+// another thread until the end. The pairs of a sequence and kv head, row by row, are cut into blocks of up to 32; a CTA holds one block and the keys of one
+// split, in tiles of 128 keys:
+//   producer (one warp): bulk copies of pieces of pages into a ring of 8 KB slots (32, 64 or 128 tokens of 256, 128 or 64 dims)
+//   conversion (four warps): codes -> f16, 128-byte swizzle: a row of 64 dims per key, read as the K-major operand of the scores and as the other's M-major one
+//   MMA (one thread): S[128 keys][pairs] = K q^T, and O[128 dims][pairs] = V^T w, one tile of scores ahead
+//   weights (two groups of four warps, a thread per key, a group takes every second set of eight pairs): S -> w in shared memory (N-major operand)
+//   sums (a thread per dim): O of the tile into registers
+// Splits lie at fixed positions and a tile's keys at fixed threads: a row's bits depend neither on the other rows of the call nor on the other sequences.
+#include "paged.cuh"
+#include "tc.cuh"
+#include <algorithm>
+
+namespace hp {
+namespace {
+
+constexpr int TK = 128, SLOT = 8192;   // keys of a tile, bytes of a slot of the ring
+
+// Shared memory of a CTA, operands on 1024-byte boundaries. 64 dims of a key (or of a pair of q, 64 columns of the weights of a key) are a row of 128 bytes.
+template <int D, int MB> struct PagedGeo {
+    static constexpr int N = 2 * MB, NB = D > 128 ? 2 : 1, ACC = 4 * NB;                 // columns, blocks of 128 dims, warps that sum
+    static constexpr int WARPS = 8 + ACC + 4 + 2, W_ACC = 8, W_CNV = W_ACC + ACC, W_MMA = W_CNV + 4;   // the last one copies
+    static constexpr int OFF_Q = 0, OFF_K = N * D * 2, OFF_V = OFF_K + TK * D * 2, OFF_P = OFF_V + TK * D * 2, OFF_X = OFF_P + TK * 128;
+    static constexpr int X_BYTES = 4096, OFF_RING = OFF_X + X_BYTES, FIXED = OFF_RING + 1024;   // 1024 for the alignment
+    static constexpr int TMEM = NB * N + 2 * N <= 128 ? 128 : 256;
+    static constexpr int ST = SLOT / D;                                                    // tokens of a slot
+    static_assert(OFF_K % 1024 == 0 && NB * N + 2 * N <= 256, "");
+};
+constexpr int MAX_SLOTS = 16, SMEM_LIMIT = 227 * 1024;
+
+__device__ __forceinline__ float warp_max(float x) { float y; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x)); return y; }
+// 128-byte swizzle, groups of 8 rows 1024 bytes apart. K-major: a row holds 64 elements along K. M- or N-major: a row is one step along K and holds 64 elements
+// along M or N, the next 64 lie `next` bytes behind.
+__device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t next) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(next >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int add) {   // D = A * B (+ D)
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+// eight columns from col0 and from col1 of this warp's 32 lanes, added: values and rests
+__device__ __forceinline__ void ld_sum8(float (&v)[8], uint32_t col0, uint32_t col1) {
+    float a[8], b[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n"
+                 "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]), "=f"(a[4]), "=f"(a[5]), "=f"(a[6]), "=f"(a[7]), "=f"(b[0]), "=f"(b[1]), "=f"(b[2]), "=f"(b[3]), "=f"(b[4]), "=f"(b[5]), "=f"(b[6]), "=f"(b[7])
+                 : "r"(col0), "r"(col1) : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = a[i] + b[i];
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) { return __all_sync(0xffffffffu, tc_wait(bar, parity, err)); }
+__device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) { __syncwarp(); if (lane == 0) mbar_arrive(bar); }
+
+// grid (splits, n_kv, blocks)
+template <int D, int KIND, int MB>
+__global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt(const PagedArgs a) {
+    using Geo = PagedGeo<D, MB>;
+    constexpr int N = Geo::N, NB = Geo::NB, ST = Geo::ST, NC = MB / 16;
+    extern __shared__ uint8_t sm_raw[];
+    __shared__ uint32_t tmem_ptr;
+    uint8_t* const sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    struct Shared {
+        uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], k_full, k_empty, v_full, s_full[2], s_empty[2], p_full, pv_done, o_empty, red[2], fin;
+        alignas(16) float c[MB]; float alpha[2][MB], top[2][2][4][8 * NC], l[2][4][8 * NC];   // factor of a pair's scores; rescaling by tile; largest scores by tile, group, warp
+        int2 see[MB]; int at[MB];                                            // a pair's position and the last key in front of its window; row * n_head + head, -1: nothing to write
+    };
+    static_assert(sizeof(Shared) <= Geo::X_BYTES, "");
+    Shared& x = *reinterpret_cast<Shared*>(sm + Geo::OFF_X);
+    pdl_launch_dependents();
+    pdl_wait();
+    const Block blk = find_block(a.b, a.G, MB, blockIdx.z, lane, a.arg_err);
+    if (blk.q.s < 0) return;
+    const PagedSeq& sq = blk.q;
+    const int kh = blockIdx.y, np = blk.np;
+    const Span sp = span_of(a, blk);
+    const int pos_lo = sp.pos_lo, pos_hi = sp.pos_hi, kend = sp.kend, lo = sp.lo, sink = sp.sink;
+    if (sp.u0 >= kend) return;
+    const int t_end = (int)((sp.u1 + TK - 1) / TK);
+    auto first_from = [&](int t) { return t * TK >= sink && t * TK + TK <= lo ? lo / TK : t; };   // first visible tile at or behind t
+    const int t_first = first_from((int)(sp.u0 / TK));
+    if (t_first >= t_end) return;
+    // first row of the pool's of the page of key j, 0xffffffff where no token of it is visible or its number is out of range
+    const int lg = a.pool.lg_page, pmask = (1 << lg) - 1;
+    auto page_of = [&](int j) -> uint32_t {
+        const int k = j & ~pmask;
+        return j < kend && (k < sink || k + pmask >= lo) ? paged_row(a.pool, sq.s, j >> lg, kh, a.arg_err) : 0xffffffffu;
+    };
+
+    if (tid == 0) {
+        for (int i = 0; i < a.slots; ++i) { mbar_init(smem_u32(&x.full[i]), 1); mbar_init(smem_u32(&x.empty[i]), 4); }
+        mbar_init(smem_u32(&x.k_full), 4); mbar_init(smem_u32(&x.k_empty), 1); mbar_init(smem_u32(&x.v_full), 4);
+        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); mbar_init(smem_u32(&x.s_empty[i]), 8); mbar_init(smem_u32(&x.red[i]), 4); }
+        mbar_init(smem_u32(&x.p_full), 8); mbar_init(smem_u32(&x.pv_done), 1); mbar_init(smem_u32(&x.o_empty), Geo::ACC); mbar_init(smem_u32(&x.fin), 1);
+        fence_barrier_init();
+    }
+    if (warp == Geo::W_MMA) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_ptr)), "n"(Geo::TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // q: a warp per pair, 8 dims per lane, as values (row i) and rests (row MB + i)
+    for (int i = warp; i < MB; i += Geo::WARPS) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        uint32_t m = 0;
+        const bool live = i < np;
+        const int p = blk.p0 + i, t = live ? p / a.G : 0;
+        if (live && lane < D / 8) {
+            const float4* src = reinterpret_cast<const float4*>(a.q + (size_t)(sq.row0 + t) * a.q_ld + (size_t)(kh * a.G + p - t * a.G) * a.q_hs) + 2 * lane;
+            const float4 v0 = src[0], v1 = src[1];
+            v[0] = v0.x; v[1] = v0.y; v[2] = v0.z; v[3] = v0.w; v[4] = v1.x; v[5] = v1.y; v[6] = v1.z; v[7] = v1.w;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+        }
+        m = __reduce_max_sync(0xffffffffu, m);
+        const int e = q_exponent(m);
+        const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+        if (lane < D / 8) {
+            uint32_t h[4], r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float y0 = v[2 * j] * up, y1 = v[2 * j + 1] * up;
+                const __half2 hh = __floats2half2_rn(y0, y1);
+                const float2 f = __half22float2(hh);
+                h[j] = h2_bits(hh); r[j] = h2_bits(__floats2half2_rn(y0 - f.x, y1 - f.y));
+            }
+            uint8_t* dst = sm + Geo::OFF_Q + (lane >> 3) * (N * 128);
+            const int ch = lane & 7;
+            *reinterpret_cast<uint4*>(dst + i * 128 + ((ch ^ (i & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(dst + (MB + i) * 128 + ((ch ^ (i & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+        }
+        if (lane == 0) {
+            const int pos = live ? max(-1, sq.len - sq.T + t) : -1;
+            x.c[i] = a.scale2 * __uint_as_float((uint32_t)(127 - e) << 23);
+            x.see[i] = make_int2(pos, a.window ? pos - a.window : -1);
+            x.at[i] = pos >= 0 ? (sq.row0 + t) * a.n_head + kh * a.G + p - t * a.G : -1;
+        }
+    }
+    fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_ptr;
+    bool ok = true;
+
+    if (warp < 8) {   // ---- weights
+        const int grp = warp >> 2, qt = warp & 3, key = qt * 32 + lane;
+        const uint32_t tlane = tmem + ((uint32_t)qt << 21);
+        uint8_t* const pw = sm + Geo::OFF_P + key * 128;
+        float l[NC][8], mu = -1e30f;   // mu of pair 8 (2 (lane / 8) + grp) + lane % 8
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) l[i][e] = 0.f;
+        // positions between which a tile is visible to all pairs
+        const int all_hi = pos_lo, all_lo = a.window ? pos_hi - a.window : -1;
+        // scales of this thread's key, a tile ahead, and its page, two tiles ahead
+        float ks = 0.f, vs = 0.f;
+        uint32_t page = page_of(t_first * TK + key);
+        auto scales = [&](int t, float& k, float& v) {
+            k = v = 0.f;
+            if (t < t_end && page != 0xffffffffu) { const size_t at = (size_t)page + ((t * TK + key) & pmask); k = a.pool.k_scale[at]; v = a.pool.v_scale[at]; }
+        };
+        scales(t_first, ks, vs);
+        int t1 = first_from(t_first + 1);
+        page = t1 < t_end ? page_of(t1 * TK + key) : 0xffffffffu;
+        int n = 0;
+        for (int t = t_first; t < t_end && ok; t = t1, ++n) {
+            float ks1, vs1;
+            t1 = first_from(t + 1);
+            scales(t1, ks1, vs1);
+            const int t2 = first_from(t1 + 1);
+            page = t2 < t_end ? page_of(t2 * TK + key) : 0xffffffffu;
+            const uint32_t sb = tlane + (n & 1) * N;
+            ok = warp_wait(smem_u32(&x.s_full[n & 1]), (n >> 1) & 1, a.err);
+            if (!ok) break;
+            tc_fence_after();
+            float s[NC][8];
+#pragma unroll
+            for (int i = 0; i < NC; ++i) { const int c8 = 8 * (2 * i + grp); if (c8 < np) ld_sum8(s[i], sb + c8, sb + MB + c8); }
+            tc_fence_before();
+            warp_arrive(smem_u32(&x.s_empty[n & 1]), lane);
+            const float lv = lg2(fmaxf(vs, 8.0779357e-28f));   // 2^-90: the weights' sum cannot overflow
+            const int j = t * TK + key;
+            const bool whole = t * TK + TK - 1 <= all_hi && (t * TK > all_lo || t * TK + TK <= sink);
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const int c8 = 8 * (2 * i + grp);
+                if (c8 < np) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) {
+                        const float4 c = *reinterpret_cast<const float4*>(&x.c[c8 + e]);
+                        s[i][e] = s[i][e] * (ks * c.x); s[i][e + 1] = s[i][e + 1] * (ks * c.y); s[i][e + 2] = s[i][e + 2] * (ks * c.z); s[i][e + 3] = s[i][e + 3] * (ks * c.w);
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int2 v = x.see[c8 + e];
+                            if (!(j <= v.x && (j > v.y || j < sink))) s[i][e] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) { const float m = warp_max(s[i][e] + lv); if (lane == 8 * i + e) top = m; }
+                }
+            }
+            if (lane < 8 * NC) x.top[n & 1][grp][qt][lane] = top;
+            warp_arrive(smem_u32(&x.red[grp]), lane);
+            ok = warp_wait(smem_u32(&x.red[grp]), n & 1, a.err);
+            if (!ok) break;
+            float al = 1.f;
+            if (lane < 8 * NC) {
+                const float m = fmaxf(fmaxf(x.top[n & 1][grp][0][lane], x.top[n & 1][grp][1][lane]), fmaxf(x.top[n & 1][grp][2][lane], x.top[n & 1][grp][3][lane]));
+                const float next = fmaxf(mu, ceilf(m) - 14.f);
+                al = pow2i(mu - next); mu = next;
+                if (qt == 0) x.alpha[n & 1][8 * (2 * (lane >> 3) + grp) + (lane & 7)] = al;
+            }
+            ok = warp_wait(smem_u32(&x.pv_done), (n & 1) ^ 1, a.err);   // the weights of the tile before are read
+            if (!ok) break;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const int c8 = 8 * (2 * i + grp);
+                if (c8 < np) {
+                    uint32_t h[4], r[4];
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        float y[2];
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            const float m = __shfl_sync(0xffffffffu, mu, 8 * i + e + d), f = __shfl_sync(0xffffffffu, al, 8 * i + e + d);
+                            const float p = ex2(s[i][e + d] - m);
+                            l[i][e + d] = fmaf(l[i][e + d], f, p);
+                            y[d] = s[i][e + d] == -INFINITY ? 0.f : p * vs;   // a masked key's scale may be anything
+                        }
+                        const __half2 hh = __floats2half2_rn(y[0], y[1]);
+                        const float2 f = __half22float2(hh);
+                        h[e / 2] = h2_bits(hh); r[e / 2] = h2_bits(__floats2half2_rn(y[0] - f.x, y[1] - f.y));
+                    }
+                    *reinterpret_cast<uint4*>(pw + (((c8 / 8) ^ (key & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(pw + (((MB / 8 + c8 / 8) ^ (key & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+                }
+            }
+            fence_proxy_async();
+            warp_arrive(smem_u32(&x.p_full), lane);
+            ks = ks1; vs = vs1;
+        }
+        // weights' sums: the 32 keys of a warp in a tree, then the warps in order
+        float mine = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float v = l[i][e];
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) v = v + __shfl_xor_sync(0xffffffffu, v, off);
+                if (lane == 8 * i + e) mine = v;
+            }
+        if (lane < 8 * NC) x.l[grp][qt][lane] = mine;
+        warp_arrive(smem_u32(&x.red[grp]), lane);
+        if (ok) ok = warp_wait(smem_u32(&x.red[grp]), n & 1, a.err);
+        if (ok && qt == 0 && lane < 8 * NC) {
+            const int pair = 8 * (2 * (lane >> 3) + grp) + (lane & 7);
+            if (pair < np && x.at[pair] >= 0)
+                a.pml[(size_t)x.at[pair] * (a.ns + a.nwin) + blockIdx.x] = make_float2(mu, ((x.l[grp][0][lane] + x.l[grp][1][lane]) + x.l[grp][2][lane]) + x.l[grp][3][lane]);
+        }
+    } else if (warp < Geo::W_CNV) {   // ---- sums
+        const int b = (warp - Geo::W_ACC) >> 2, qt = warp & 3, dim = 128 * b + 32 * qt + lane;
+        const uint32_t ob = tmem + ((uint32_t)qt << 21) + 2 * N + b * N;
+        float O[MB];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) O[i] = 0.f;
+        int n = 0;
+        for (int t = t_first; t < t_end && ok; t = first_from(t + 1), ++n) {
+            ok = warp_wait(smem_u32(&x.pv_done), n & 1, a.err);
+            if (!ok) break;
+            tc_fence_after();
+            float f[MB / 8][8];
+#pragma unroll
+            for (int c = 0; c < MB / 8; ++c) if (8 * c < np) ld_sum8(f[c], ob + 8 * c, ob + MB + 8 * c);
+            float4 al[MB / 4];
+#pragma unroll
+            for (int c = 0; c < MB / 4; ++c) al[c] = *reinterpret_cast<const float4*>(&x.alpha[n & 1][4 * c]);
+            tc_fence_before();
+            warp_arrive(smem_u32(&x.o_empty), lane);
+#pragma unroll
+            for (int c = 0; c < MB / 4; ++c)
+                if (4 * c < np) {
+                    O[4 * c] = fmaf(O[4 * c], al[c].x, f[c / 2][4 * (c & 1)]); O[4 * c + 1] = fmaf(O[4 * c + 1], al[c].y, f[c / 2][4 * (c & 1) + 1]);
+                    O[4 * c + 2] = fmaf(O[4 * c + 2], al[c].z, f[c / 2][4 * (c & 1) + 2]); O[4 * c + 3] = fmaf(O[4 * c + 3], al[c].w, f[c / 2][4 * (c & 1) + 3]);
+                }
+        }
+        if (ok && dim < D) {
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+                if (i < np && x.at[i] >= 0) a.pO[((size_t)x.at[i] * (a.ns + a.nwin) + blockIdx.x) * D + dim] = O[i];
+        }
+    } else if (warp < Geo::W_MMA) {   // ---- conversion: a warp takes a quarter of each slot, 16 codes per lane and step
+        const int cw = warp - Geo::W_CNV;
+        int k = 0, n = 0;
+        for (int t = t_first; t < t_end && ok; t = first_from(t + 1), ++n) {
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                ok = ok && warp_wait(kv ? smem_u32(&x.pv_done) : smem_u32(&x.k_empty), (n & 1) ^ 1, a.err);   // the operand of the tile before is read
+                uint8_t* const dst = sm + (kv ? Geo::OFF_V : Geo::OFF_K);
+                for (int sl = 0; sl < TK / ST && ok; ++sl, ++k) {
+                    const int slot = k % a.slots;
+                    ok = warp_wait(smem_u32(&x.full[slot]), (k / a.slots) & 1, a.err);
+                    if (!ok) break;
+                    const uint4* src = reinterpret_cast<const uint4*>(sm + Geo::OFF_RING + slot * SLOT + cw * (SLOT / 4));
+                    uint4 w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = src[i * 32 + lane];
+                    warp_arrive(smem_u32(&x.empty[slot]), lane);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = i * 32 + lane, row = sl * ST + cw * (ST / 4) + e / (D / 16), part = e % (D / 16);
+                        const uint4 h0 = make_uint4(code_pair<KIND, 0>(w[i].x), code_pair<KIND, 2>(w[i].x), code_pair<KIND, 0>(w[i].y), code_pair<KIND, 2>(w[i].y));
+                        const uint4 h1 = make_uint4(code_pair<KIND, 0>(w[i].z), code_pair<KIND, 2>(w[i].z), code_pair<KIND, 0>(w[i].w), code_pair<KIND, 2>(w[i].w));
+                        uint8_t* o = dst + (part >> 2) * (TK * 128) + row * 128;
+                        const int ch = (part & 3) * 2, odd = (part >> 2) & 1;   // lanes of neighbouring blocks of 64 dims store the halves the other way round: other banks
+                        *reinterpret_cast<uint4*>(o + (((ch + odd) ^ (row & 7)) << 4)) = odd ? h1 : h0;
+                        *reinterpret_cast<uint4*>(o + (((ch + 1 - odd) ^ (row & 7)) << 4)) = odd ? h0 : h1;
+                    }
+                }
+                fence_proxy_async();
+                if (ok) warp_arrive(kv ? smem_u32(&x.v_full) : smem_u32(&x.k_full), lane);
+            }
+        }
+    } else if (warp == Geo::W_MMA) {   // ---- products
+        const uint32_t base = smem_u32(sm);
+        constexpr uint32_t ID_S = (1u << 4) | ((uint32_t)(N >> 3) << 17) | (8u << 24), ID_O = ID_S | (1u << 15) | (1u << 16);   // f32 = f16 x f16, M = 128; O: both operands M- / N-major
+        auto outputs = [&](int n) {
+            ok = ok && warp_wait(smem_u32(&x.p_full), n & 1, a.err) && warp_wait(smem_u32(&x.v_full), n & 1, a.err) && warp_wait(smem_u32(&x.o_empty), (n & 1) ^ 1, a.err);
+            if (!ok) return;
+            tc_fence_after();
+            if (tc_elect()) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < TK / 16; ++i)   // 16 keys
+                        mma_f16(tmem + 2 * N + b * N, desc128(base + Geo::OFF_V + b * 2 * (TK * 128) + i * 2048, TK * 128), desc128(base + Geo::OFF_P + i * 2048, 16), ID_O, i != 0);
+                tc_commit(smem_u32(&x.pv_done));
+            }
+            __syncwarp();
+        };
+        int n = 0;
+        for (int t = t_first; t < t_end && ok; t = first_from(t + 1), ++n) {
+            ok = warp_wait(smem_u32(&x.k_full), n & 1, a.err) && warp_wait(smem_u32(&x.s_empty[n & 1]), ((n >> 1) & 1) ^ 1, a.err);
+            if (!ok) break;
+            tc_fence_after();
+            if (tc_elect()) {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)   // 16 dims
+                    mma_f16(tmem + (n & 1) * N, desc128(base + Geo::OFF_K + (i >> 2) * (TK * 128) + (i & 3) * 32, 16), desc128(base + Geo::OFF_Q + (i >> 2) * (N * 128) + (i & 3) * 32, 16), ID_S, i != 0);
+                tc_commit(smem_u32(&x.s_full[n & 1]));
+                tc_commit(smem_u32(&x.k_empty));
+            }
+            __syncwarp();
+            if (n) outputs(n - 1);
+        }
+        if (ok) outputs(n - 1);
+        if (tc_elect()) tc_commit(smem_u32(&x.fin));
+        __syncwarp();
+        tc_wait(smem_u32(&x.fin), 0, a.err);   // nothing in flight when the accumulator memory is given back
+    } else {   // ---- copies: lane i holds the page of the tile's i-th piece of up to 16 .. 128 tokens
+        const int pt = min(1 << lg, ST);   // tokens of a copy: within a page and a slot
+        uint32_t page = page_of(t_first * TK + lane * pt < t_first * TK + TK ? t_first * TK + lane * pt : 0x7fffffff);
+        int k = 0;
+        for (int t = t_first; t < t_end && ok; ) {
+            const int t1 = first_from(t + 1);
+            const uint32_t next = t1 < t_end && lane * pt < TK ? page_of(t1 * TK + lane * pt) : 0xffffffffu;
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv)
+                for (int sl = 0; sl < TK / ST && ok; ++sl, ++k) {
+                    const int slot = k % a.slots;
+                    ok = warp_wait(smem_u32(&x.empty[slot]), ((k / a.slots) & 1) ^ 1, a.err);
+                    if (!ok) break;
+                    const int i0 = sl * ST / pt, cnt = ST / pt;
+                    const bool mine = lane >= i0 && lane < i0 + cnt && page != 0xffffffffu;
+                    const int live = __popc(__ballot_sync(0xffffffffu, mine));
+                    const uint32_t bar = smem_u32(&x.full[slot]);
+                    if (lane == 0) { if (live) mbar_expect_tx(bar, (uint32_t)(live * pt * D)); else mbar_arrive(bar); }
+                    __syncwarp();
+                    if (mine)
+                        bulk_g2s(smem_u32(sm + Geo::OFF_RING + slot * SLOT + (lane - i0) * pt * D), (kv ? a.pool.v : a.pool.k) + ((size_t)page + ((t * TK + lane * pt) & pmask)) * D, (uint32_t)(pt * D), bar);
+                }
+            page = next; t = t1;
+        }
+        for (int i = k > a.slots ? k - a.slots : 0; i < k; ++i) tc_wait(smem_u32(&x.full[i % a.slots]), (i / a.slots) & 1, a.err);   // no copy outlives the CTA
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == Geo::W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Geo::TMEM) : "memory");
+}
+
+template <int D, int KIND, int MB> int launch_split(PagedArgs& a, dim3 grid, cudaStream_t s) {
+    using Geo = PagedGeo<D, MB>;
+    static bool attr[MAX_DEVICES] = {};   // per device: the opt-in belongs to the device's copy of the kernel
+    const int dev = current_device(); if (dev < 0) return HP_ECUDA;
+    a.slots = std::min(MAX_SLOTS, (SMEM_LIMIT - 1024 - Geo::FIXED) / SLOT);   // 1024: what the kernel declares besides
+    const int smem = Geo::FIXED + a.slots * SLOT;
+    if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_prompt<D, KIND, MB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); attr[dev] = true; }
+    HP_CUDA(launch_pdl<4>(k_paged_prompt<D, KIND, MB>, grid, dim3(Geo::WARPS * 32), smem, s, a));
+    return HP_OK;
+}
+template <int KIND> int launch_split(PagedArgs& a, dim3 grid, cudaStream_t s) {
+    return a.pool.head_dim == 256 ? launch_split<256, KIND, PAGED_TC_PAIRS>(a, grid, s) : a.pool.head_dim == 128 ? launch_split<128, KIND, PAGED_TC_PAIRS>(a, grid, s) : launch_split<64, KIND, PAGED_TC_PAIRS>(a, grid, s);
+}
+
+}  // namespace
+
+int attn_paged_tc(PagedArgs& a, dim3 grid, cudaStream_t s) { return a.pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, s) : launch_split<KV_E4M3>(a, grid, s); }
+
+}  // namespace hp

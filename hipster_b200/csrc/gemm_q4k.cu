@@ -35,6 +35,7 @@
 // last four warps (56): 63488 in all.
 // Every wait is bounded and reports through the device status word.
 #include "hp_common.cuh"
+#include "tc.cuh"
 #include "kernels.h"
 #include <cuda_fp8.h>
 
@@ -54,33 +55,12 @@ template <int NTC> struct TcGeom {
 };
 static_assert(TcGeom<16>::SMEM <= GEMV_SMEM_LIMIT && TcGeom<12>::SMEM <= GEMV_SMEM_LIMIT && TcGeom<8>::SMEM <= GEMV_SMEM_LIMIT, "shared memory of the widest tiles");
 
-// Bounded wait that lets the hardware park the warp: up to 2^20 attempts of up to a microsecond
-__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, int* err) {
-    for (uint32_t it = 0; it < (1u << 20); ++it) {
-        uint32_t ok;
-        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
-        if (ok) return true;
-    }
-    if (err) atomicExch(err, HP_ETIMEOUT);
-    return false;
-}
-// one lane of a converged warp; unlike lane == 0 the compiler knows that a single thread issues what follows
-__device__ __forceinline__ bool tc_elect() {
-    uint32_t p;
-    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(p));
-    return p != 0;
-}
 __device__ __forceinline__ uint64_t tc_desc(uint32_t addr) {   // K-major operand, 64-byte swizzle: 8-row groups 512 bytes apart
     return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | (32ull << 32) | (1ull << 46) | (4ull << 61);
 }
 __device__ __forceinline__ void tc_mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int add) {   // D = A * B (+ D)
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void tc_reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void tc_reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;"); }

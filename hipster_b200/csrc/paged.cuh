@@ -39,4 +39,76 @@ __device__ __forceinline__ uint32_t paged_row(const PagedPool& p, int s, int col
     return ((uint32_t)id * (uint32_t)p.n_kv + (uint32_t)head) << p.lg_page;
 }
 
+// ---- attention: what its two kernels (attn_paged.cu, attn_paged_tc.cu) share
+struct PagedArgs {
+    PagedPool pool; PagedBatch b;
+    const float* q; size_t q_ld, q_hs; int n_head, G; float scale2;   // scale2 = scale * log2 e (times 256 for e4m3)
+    int window, n_sink;
+    int U, ns, nwin, slots;     // keys of a split, splits of the first tokens, splits behind them; slots of the prompt kernel's ring
+    float* pO; float2* pml;     // partials [row][head][ns + nwin] (x head_dim): sums, (mu, sum of weights)
+    int* err; int* arg_err;
+};
+
+// the prompt kernel: MB pairs per CTA
+constexpr int PAGED_TC_PAIRS = 32;
+int attn_paged_tc(PagedArgs& a, dim3 grid, cudaStream_t s);
+
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float pow2i(float d) { return d < -126.f ? 0.f : __uint_as_float((uint32_t)((int)d + 127) << 23); }   // 2^d, d whole and <= 0
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// Two of four codes as two f16. int8: the code plus 128 becomes the low bits of 1024 + code + 128, and 1152 is subtracted, exactly. e4m3: its bits
+// are those of the f16 2^-8 times as large, subnormals included (so 0x7f, which the quantiser does not write, reads as 480 and not as NaN: what lies in
+// slots of absent tokens is harmless).
+template <int KIND, int LO> __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+    if constexpr (KIND == KV_I8) {
+        const uint32_t h = __byte_perm(w ^ 0x80808080u, 0x64646464u, LO == 0 ? 0x4140 : 0x4342);
+        return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&h), __floats2half2_rn(1152.f, 1152.f)));
+    } else {
+        const uint32_t h = __byte_perm(w, 0u, LO == 0 ? 0x1404 : 0x3424);
+        return (h & 0x80008000u) | ((h >> 1) & 0x3f803f80u);
+    }
+}
+// The block of pairs that blockIdx.z stands for: sequences in order, each with ceil(T * G / MB) blocks.
+struct Block { PagedSeq q; int p0, np; };
+__device__ __forceinline__ Block find_block(const PagedBatch& b, int G, int MB, int blk, int lane, int* err) {
+    Block o; o.q.s = -1; o.p0 = o.np = 0;
+    int acc = 0;
+    for (int s0 = 0; s0 < b.S; s0 += 32) {
+        PagedSeq q{-1, 0, 0, 0};
+        if (s0 + lane < b.S) q = paged_seq(b, s0 + lane, err);
+        const int n = (q.T * G + MB - 1) / MB;
+        int incl = n;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) { const int t = __shfl_up_sync(0xffffffffu, incl, off); if (lane >= off) incl += t; }
+        const unsigned hit = __ballot_sync(0xffffffffu, acc + incl > blk);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            o.q.s = s0 + l; o.q.row0 = __shfl_sync(0xffffffffu, q.row0, l); o.q.T = __shfl_sync(0xffffffffu, q.T, l); o.q.len = __shfl_sync(0xffffffffu, q.len, l);
+            o.p0 = (blk - acc - __shfl_sync(0xffffffffu, incl - n, l)) * MB;
+            o.np = min(MB, o.q.T * G - o.p0);
+            return o;
+        }
+        acc += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return o;
+}
+
+// What a CTA of a block has to look at: keys [0, sink) and [lo, kend), of these its split's.
+struct Span { int kend, lo, sink, pos_lo, pos_hi; long long u0, u1; };
+__device__ __forceinline__ Span span_of(const PagedArgs& a, const Block& blk) {
+    Span v;
+    v.pos_lo = blk.q.len - blk.q.T + blk.p0 / a.G; v.pos_hi = blk.q.len - blk.q.T + (blk.p0 + blk.np - 1) / a.G;
+    v.kend = v.pos_hi + 1; v.lo = a.window ? max(0, v.pos_lo - a.window + 1) : 0; v.sink = a.window ? a.n_sink : 0;
+    int split = blockIdx.x;
+    if (split >= a.ns) {   // the split of the window whose number leaves this remainder
+        const int w0 = max(a.ns, v.lo / a.U), m = (w0 - a.ns) % a.nwin, j = split - a.ns - m;
+        split = w0 + (j < 0 ? j + a.nwin : j);
+    }
+    v.u0 = (long long)split * a.U; v.u1 = min(v.u0 + a.U, (long long)v.kend);
+    return v;
+}
+// power of two that brings the largest magnitude (its bits) to [2^14, 2^15)
+__device__ __forceinline__ int q_exponent(uint32_t m) { return m == 0 || m >= 0x7f800000u ? 0 : min(100, 14 - ((int)(m >> 23) - 127)); }
+
 }  // namespace hp
