@@ -31,6 +31,16 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   // c = a * b: no zeros to be put into registers
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void fma_pair(float& x, float& y, float fx, float fy, float ax, float ay) {   // x = x * fx + ax, y = y * fy + ay
+    float2 o = make_float2(x, y);
+    asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(reinterpret_cast<unsigned long long&>(o))
+        : "l"(reinterpret_cast<const unsigned long long&>(static_cast<const float2&>(make_float2(fx, fy)))), "l"(reinterpret_cast<const unsigned long long&>(static_cast<const float2&>(make_float2(ax, ay)))));
+    x = o.x; y = o.y;
+}
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) { uint32_t r; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v)); return r; }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 template <typename T> __device__ __forceinline__ T at_smem(const uint8_t* p) { return *reinterpret_cast<const T*>(p); }
@@ -51,8 +61,8 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     __shared__ int s_pos[MB];   // position of a pair's row, -1: none
     __shared__ float s_mu[KW][MB], s_l[KW][MB];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();   // behind the wait: what was enqueued in front of this kernel is complete when the merge starts
     const Block blk = find_block(a.b, a.G, MB, blockIdx.z, lane, a.arg_err);
     if (blk.q.s < 0) return;
     const PagedSeq& sq = blk.q;
@@ -146,6 +156,12 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
 #pragma unroll
         for (int n = 0; n < NT; ++n) { O[i][n][0] = O[i][n][1] = O[i][n][2] = O[i][n][3] = 0.f; }
 
+    // where a lane's 8 bytes lie: rows g and g + 8 of k (these shift alike), the 32 dims x; rows 2 q4 and 2 q4 + 1 (+ 8) of v, the 64 dims y
+    int kofs[4], vofs[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kofs[i] = i < D / 32 ? place<D, false>(g, 2 * i + (q4 >> 1)) + (q4 & 1) * 8 : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vofs[i >> 1][i & 1] = (i & 1) < D / 64 ? place<D, true>(2 * q4 + (i >> 1), 4 * (i & 1) + (g >> 1)) + (g & 1) * 8 : 0;
     int slot = 0;
     for (; i0 < i_end; ) {
         const float sc1 = i1 < i_end ? scales(r1) : 0.f;
@@ -157,21 +173,19 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         float s[NT][4];
         {
             float sh[NT][2][4], sl[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) sh[n][0][c] = sh[n][1][c] = sl[n][c] = 0.f;
             const uint8_t* kr = ring + slot * (KS * D);
 #pragma unroll
             for (int x = 0; x < D / 32; ++x) {
-                const uint2 ka = at_smem<uint2>(kr + place<D, false>(g, 2 * x + (q4 >> 1)) + (q4 & 1) * 8), kb = at_smem<uint2>(kr + place<D, false>(g + 8, 2 * x + (q4 >> 1)) + (q4 & 1) * 8);
+                const uint8_t* kx = kr + kofs[x & 3] + (x >> 2) * 128;
+                const uint2 ka = at_smem<uint2>(kx), kb = at_smem<uint2>(kx + 8 * D);
                 const uint32_t a0[4] = {code_pair<KIND, 0>(ka.x), code_pair<KIND, 0>(kb.x), code_pair<KIND, 2>(ka.x), code_pair<KIND, 2>(kb.x)};
                 const uint32_t a1[4] = {code_pair<KIND, 0>(ka.y), code_pair<KIND, 0>(kb.y), code_pair<KIND, 2>(ka.y), code_pair<KIND, 2>(kb.y)};
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const uint4 h = at_smem<uint4>(qf + n * D * 32 + x * 1024), r = at_smem<uint4>(qf + n * D * 32 + x * 1024 + 512);
-                    mma_f16(sh[n][0], a0, h.x, h.y); mma_f16(sl[n], a0, r.x, r.y);
-                    mma_f16(sh[n][1], a1, h.z, h.w); mma_f16(sl[n], a1, r.z, r.w);
+                    if (x == 0) { mma_f16_first(sh[n][0], a0, h.x, h.y); mma_f16_first(sl[n], a0, r.x, r.y); mma_f16_first(sh[n][1], a1, h.z, h.w); }
+                    else { mma_f16(sh[n][0], a0, h.x, h.y); mma_f16(sl[n], a0, r.x, r.y); mma_f16(sh[n][1], a1, h.z, h.w); }
+                    mma_f16(sl[n], a1, r.z, r.w);
                 }
             }
 #pragma unroll
@@ -233,7 +247,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             for (int y = 0; y < D / 64; ++y) {
                 uint2 v[4];   // keys 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = at_smem<uint2>(vr + place<D, true>(2 * q4 + (i & 1) + (i >> 1) * 8, 4 * y + (g >> 1)) + (g & 1) * 8);
+                for (int i = 0; i < 4; ++i) v[i] = at_smem<uint2>(vr + vofs[i & 1][y & 1] + (y >> 1) * 128 + (i >> 1) * 8 * D);
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
                     const uint32_t x0 = w ? v[0].y : v[0].x, x1 = w ? v[1].y : v[1].x, x2 = w ? v[2].y : v[2].x, x3 = w ? v[3].y : v[3].x;
@@ -243,11 +257,11 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
                         const uint32_t af[4] = {code_pair<KIND, 0>(lo2), code_pair<KIND, 2>(lo2), code_pair<KIND, 0>(hi2), code_pair<KIND, 2>(hi2)};
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            float f[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_f16(f, af, br[n][0], br[n][1]);
+                            float f[4];
+                            mma_f16_first(f, af, br[n][0], br[n][1]);
                             mma_f16(f, af, bh[n][0], bh[n][1]);
                             float (&o)[4] = O[y * 4 + w * 2 + h][n];
-                            o[0] = fmaf(o[0], al[n][0], f[0]); o[1] = fmaf(o[1], al[n][1], f[1]); o[2] = fmaf(o[2], al[n][0], f[2]); o[3] = fmaf(o[3], al[n][1], f[3]);
+                            fma_pair(o[0], o[1], al[n][0], al[n][1], f[0], f[1]); fma_pair(o[2], o[3], al[n][0], al[n][1], f[2], f[3]);
                         }
                     }
                 }
@@ -301,42 +315,61 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     }
 }
 
-// Splits of a row in order, gate, f32 and q8 outputs. One block of head_dim threads per row and head.
+// Splits of a row, gate, f32 and q8 outputs. A block per row and head: D / 4 threads hold four dims each, and 1024 / D sets of them take every such
+// split in order; the sets are added in order. Bound by latency: the row, its place and gate are read ahead of the dependency wait (the kernel of the splits
+// releases this one once its predecessors are complete), the partials of up to four splits of each set are in flight.
 struct MergeArgs {
-    PagedBatch b; const float* pO; const float2* pml; const float* gate; size_t g_ld, g_hs; int n_head, D, window, n_sink, U, ns, nwin; float mul;
+    PagedBatch b; const float* pO; const float2* pml; const float* gate; size_t g_ld, g_hs; int n_head, window, n_sink, U, ns, nwin; float mul;
     float* out; int8_t* oq; float* osc; int* err;
 };
-__global__ void __launch_bounds__(256) k_paged_merge(MergeArgs a) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const int r = blockIdx.x / a.n_head, head = blockIdx.x % a.n_head, d = threadIdx.x, lane = d & 31;
+template <int D>
+__global__ void __launch_bounds__(256) k_paged_merge(const MergeArgs a) {
+    constexpr int TD = D / 4, SETS = 256 / TD, PF = 4;
+    __shared__ float4 s_o[SETS][TD]; __shared__ float s_l[SETS];
+    const int r = blockIdx.x / a.n_head, head = blockIdx.x % a.n_head, set = threadIdx.x / TD, d4 = threadIdx.x % TD, lane = threadIdx.x & 31;
     const PagedSeq q = paged_find(a.b, r, lane, a.err);
-    if (q.s < 0) return;
     const int pos = q.len - q.T + r - q.row0;
-    float v = 0.f;
-    if (pos >= 0) {
-        const int lo = a.window ? max(0, pos - a.window + 1) : 0, w0 = max(a.ns, lo / a.U), w1 = pos / a.U;
-        const int s1 = a.ns ? (min(a.n_sink, pos + 1) + a.U - 1) / a.U : 0;   // splits [0, s1) and [w0, w1]
-        const int n = s1 + max(0, w1 - w0 + 1);
-        const size_t base = ((size_t)r * a.n_head + head) * (a.ns + a.nwin);
-        auto slot = [&](int i) { return base + (i < s1 ? i : a.ns + (w0 + i - s1 - a.ns) % a.nwin); };
-        float mu = -INFINITY;
-        for (int i = lane; i < n; i += 32) mu = fmaxf(mu, a.pml[slot(i)].x);
+    float gate = 0.f;
+    if (a.gate && q.s >= 0 && threadIdx.x < D) gate = a.gate[(size_t)r * a.g_ld + (size_t)head * a.g_hs + threadIdx.x];
+    pdl_wait();
+    pdl_launch_dependents();
+    if (q.s < 0) return;
+    const int lo = a.window ? max(0, pos - a.window + 1) : 0, w0 = max(a.ns, lo / a.U), w1 = max(pos, 0) / a.U;
+    const int s1 = a.ns ? (min(a.n_sink, pos + 1) + a.U - 1) / a.U : 0;   // splits [0, s1) and [w0, w1]
+    const int n = pos < 0 ? 0 : s1 + max(0, w1 - w0 + 1);
+    const size_t base = ((size_t)r * a.n_head + head) * (a.ns + a.nwin);
+    auto slot = [&](int i) { return base + (i < s1 ? i : a.ns + (w0 + i - s1 - a.ns) % a.nwin); };
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f); float l = 0.f, mu = -INFINITY;
+    float4 v[PF];
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, off));
-        float o = 0.f, l = 0.f;
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-            const size_t at = slot(i);
-            const float2 ml = a.pml[at];
-            const float w = pow2i(ml.x - mu);
-            o = fmaf(w, a.pO[at * a.D + d], o); l = fmaf(w, ml.y, l);
+    for (int i = 0; i < PF; ++i) if (set + i * SETS < n) v[i] = reinterpret_cast<const float4*>(a.pO + slot(set + i * SETS) * D)[d4];
+    for (int i = lane; i < n; i += 32) mu = fmaxf(mu, a.pml[slot(i)].x);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, off));
+    for (int i0 = set; i0 < n; i0 += PF * SETS) {
+#pragma unroll
+        for (int j = 0; j < PF; ++j) {
+            const int i = i0 + j * SETS;
+            if (i < n) {
+                const float2 ml = a.pml[slot(i)];
+                const float w = pow2i(ml.x - mu);
+                o.x = fmaf(w, v[j].x, o.x); o.y = fmaf(w, v[j].y, o.y); o.z = fmaf(w, v[j].z, o.z); o.w = fmaf(w, v[j].w, o.w); l = fmaf(w, ml.y, l);
+                if (i + PF * SETS < n) v[j] = reinterpret_cast<const float4*>(a.pO + slot(i + PF * SETS) * D)[d4];
+            }
         }
-        v = l == 0.f ? 0.f : o * a.mul / l;
-        if (a.gate) v = v * sigmoid_det(a.gate[(size_t)r * a.g_ld + (size_t)head * a.g_hs + d]);
     }
-    if (a.out) a.out[((size_t)r * a.n_head + head) * a.D + d] = v;
-    if (a.oq) warp_quant32_store(v, r, (head * a.D + d) >> 5, a.n_head * a.D, a.oq, a.osc, lane);
+    s_o[set][d4] = o;
+    if (d4 == 0) s_l[set] = l;
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= D) return;
+    float x = 0.f; l = 0.f;
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) { x = x + reinterpret_cast<const float*>(&s_o[i][0])[d]; l = l + s_l[i]; }
+    x = l == 0.f ? 0.f : x * a.mul / l;
+    if (a.gate) x = x * sigmoid_det(gate);
+    if (a.out) a.out[((size_t)r * a.n_head + head) * D + d] = x;
+    if (a.oq) warp_quant32_store(x, r, (head * D + d) >> 5, a.n_head * D, a.oq, a.osc, lane);
 }
 
 struct Plan { int U, ns, nwin, MB; long long blocks; };
@@ -392,9 +425,11 @@ int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams
     const dim3 grid(pl.ns + pl.nwin, pool.n_kv, (unsigned)pl.blocks);
     const int rc = b.max_rows > 8 ? attn_paged_tc(a, grid, s) : pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, pl.MB, s) : launch_split<KV_E4M3>(a, grid, pl.MB, s);
     if (rc != HP_OK) return rc;
-    MergeArgs m; m.b = b; m.pO = a.pO; m.pml = a.pml; m.gate = p.gate; m.g_ld = p.g_ld; m.g_hs = p.g_hs; m.n_head = p.n_head; m.D = pool.head_dim; m.window = p.window; m.n_sink = p.n_sink;
+    MergeArgs m; m.b = b; m.pO = a.pO; m.pml = a.pml; m.gate = p.gate; m.g_ld = p.g_ld; m.g_hs = p.g_hs; m.n_head = p.n_head; m.window = p.window; m.n_sink = p.n_sink;
     m.U = pl.U; m.ns = pl.ns; m.nwin = pl.nwin; m.mul = pool.kind == KV_E4M3 ? 256.f : 1.f; m.out = p.out; m.oq = (int8_t*)p.xq.q; m.osc = (float*)p.xq.sc; m.err = a.arg_err;
-    HP_CUDA(launch_pdl<4>(k_paged_merge, dim3((unsigned)(b.R * p.n_head)), dim3(pool.head_dim), 0, s, m));
+    const dim3 mg((unsigned)(b.R * p.n_head));
+    HP_CUDA(pool.head_dim == 256 ? launch_pdl<4>(k_paged_merge<256>, mg, dim3(256), 0, s, m) : pool.head_dim == 128 ? launch_pdl<4>(k_paged_merge<128>, mg, dim3(256), 0, s, m)
+                                                                                                   : launch_pdl<4>(k_paged_merge<64>, mg, dim3(256), 0, s, m));
     return HP_OK;
 }
 

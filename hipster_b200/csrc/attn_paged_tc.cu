@@ -80,8 +80,8 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
     };
     static_assert(sizeof(Shared) <= Geo::X_BYTES, "");
     Shared& x = *reinterpret_cast<Shared*>(sm + Geo::OFF_X);
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();   // behind the wait: what was enqueued in front of this kernel is complete when the merge starts
     const Block blk = find_block(a.b, a.G, MB, blockIdx.z, lane, a.arg_err);
     if (blk.q.s < 0) return;
     const PagedSeq& sq = blk.q;
