@@ -8,10 +8,11 @@ LIB_PATH = os.environ.get("HIPSTER_B200_LIB") or os.path.join(HERE, "libhipster_
 HEADER = os.path.join(HERE, "..", "include", "hipster_b200.h")
 
 _lib = _hot = None
-# the calls whose latency counts, with their argument types (p pointer, i int, l long long, f float), so that integers pass without a wrapper object
-_TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+# the calls whose latency counts, with their argument types (p pointer, i int, l long long, f float, d double), so that integers pass without a wrapper object
+_TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float, "d": ctypes.c_double}
 _HOT = {"hp_quantize_x_q8": "piiippp", "hp_gemv_q4k_q8": "ppppiiiip", "hp_argmax": "piiipppp", "hp_accept_greedy": "ppipp", "hp_attn_decode": "piiiiiipppppipppfpp",
-        "hp_kv_append": "pllpllipllpllpppiiipippiipfp", "hp_kv_read": "pippiipppllp", "hp_attn_paged": "pllpllipippiiiipfiippppp"}
+        "hp_kv_append": "pllpllipllpllpppiiipippiipfp", "hp_kv_read": "pippiipppllp", "hp_attn_paged": "pllpllipippiiiipfiippppp",
+        "hp_rope_table": "piidididddp"}
 
 
 class HipsterError(RuntimeError):

@@ -7,9 +7,9 @@
 #include <stdint.h>
 
 typedef struct { const char* name; void* fn; } Bound;
-enum { QUANTIZE, GEMV, ARGMAX, ACCEPT, ATTN, KV_APPEND, KV_READ, ATTN_PAGED, N_BOUND };
+enum { QUANTIZE, GEMV, ARGMAX, ACCEPT, ATTN, KV_APPEND, KV_READ, ATTN_PAGED, ROPE_TABLE, N_BOUND };
 static Bound bound[N_BOUND] = {{"hp_quantize_x_q8", NULL}, {"hp_gemv_q4k_q8", NULL}, {"hp_argmax", NULL}, {"hp_accept_greedy", NULL}, {"hp_attn_decode", NULL},
-    {"hp_kv_append", NULL}, {"hp_kv_read", NULL}, {"hp_attn_paged", NULL}};
+    {"hp_kv_append", NULL}, {"hp_kv_read", NULL}, {"hp_attn_paged", NULL}, {"hp_rope_table", NULL}};
 
 static void* as_ptr(PyObject* o) { return o == Py_None ? NULL : (void*)(uintptr_t)PyLong_AsUnsignedLongLongMask(o); }
 static long long as_long(PyObject* o) { return (long long)PyLong_AsUnsignedLongLongMask(o); }
@@ -83,6 +83,13 @@ static PyObject* py_attn_paged(PyObject* self, PyObject* const* a, Py_ssize_t n)
     CALL(((int (*)(const float*, long long, long long, const float*, long long, long long, int, const int*, int, const int*, const int*, int, int, int, int, const void*, float, int, int, float*, void*, void*, void*, void*))
               bound[ATTN_PAGED].fn)(q, ql, qh, g, gl, gh, nh, table, tl, rs, kl, S, R, mr, mk, pages, scale, win, sink, out, xq, sc, ws, s));
 }
+static PyObject* py_rope_table(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    if (!usable(ROPE_TABLE, n, 11)) return NULL;
+    void *t = as_ptr(a[0]), *s = as_ptr(a[10]);
+    const int np = as_int(a[1]), nr = as_int(a[2]), kind = as_int(a[4]), orig = as_int(a[6]);
+    const double base = PyFloat_AsDouble(a[3]), factor = PyFloat_AsDouble(a[5]), fast = PyFloat_AsDouble(a[7]), slow = PyFloat_AsDouble(a[8]), mul = PyFloat_AsDouble(a[9]);
+    CALL(((int (*)(float*, int, int, double, int, double, int, double, double, double, void*))bound[ROPE_TABLE].fn)(t, np, nr, base, kind, factor, orig, fast, slow, mul, s));
+}
 /* bind(name, address) */
 static PyObject* py_bind(PyObject* self, PyObject* args) {
     const char* name; PyObject* addr;
@@ -102,6 +109,6 @@ static PyMethodDef methods[] = {
     {"hp_quantize_x_q8", (PyCFunction)(void*)py_quantize, METH_FASTCALL, NULL}, {"hp_gemv_q4k_q8", (PyCFunction)(void*)py_gemv, METH_FASTCALL, NULL},
     {"hp_argmax", (PyCFunction)(void*)py_argmax, METH_FASTCALL, NULL}, {"hp_accept_greedy", (PyCFunction)(void*)py_accept, METH_FASTCALL, NULL},
     {"hp_attn_decode", (PyCFunction)(void*)py_attn, METH_FASTCALL, NULL}, {"hp_kv_append", (PyCFunction)(void*)py_kv_append, METH_FASTCALL, NULL},
-    {"hp_kv_read", (PyCFunction)(void*)py_kv_read, METH_FASTCALL, NULL}, {"hp_attn_paged", (PyCFunction)(void*)py_attn_paged, METH_FASTCALL, NULL}, {NULL, NULL, 0, NULL}};
+    {"hp_kv_read", (PyCFunction)(void*)py_kv_read, METH_FASTCALL, NULL}, {"hp_attn_paged", (PyCFunction)(void*)py_attn_paged, METH_FASTCALL, NULL}, {"hp_rope_table", (PyCFunction)(void*)py_rope_table, METH_FASTCALL, NULL}, {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__calls(void) { return PyModule_Create(&module); }

@@ -165,6 +165,9 @@ def moe_layer(xn, router, exp_gate_up, exp_down, sh_gate_up, sh_down, F, n_exper
 
 
 # ---- a paged cache in 8 bits (no counterpart in the reference)
+_F32, _I32, _F16 = torch.float32, torch.int32, torch.float16
+
+
 class _Pages(ctypes.Structure):   # hp_kv_pages
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)] + [(n, ctypes.c_int) for n in ("type", "n_pages", "n_kv", "page_size", "head_dim")]
 
@@ -186,7 +189,7 @@ class KVPages:
         self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
         self.n_pages, self.n_kv, self.page_size, self.head_dim = k.shape
         self._c = _Pages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), int(k.dtype != torch.int8), *k.shape)
-        self._at = ctypes.addressof(self._c)
+        self._at, self._dev, self._f16 = ctypes.addressof(self._c), k.get_device(), torch.empty(0, dtype=_F16, device=k.device)
 
     @classmethod
     def empty(cls, n_pages, n_kv, page_size, head_dim, dtype=torch.int8, device="cuda"):
@@ -194,28 +197,27 @@ class KVPages:
         return cls(*codes, *(torch.zeros((n_pages, n_kv, page_size), dtype=torch.float32, device=device) for _ in range(2)))
 
 
-# The checks below run on every call of a few microseconds: a test that fails builds its message, one that holds costs its attribute reads alone.
+# The checks below run on every call of a few microseconds, hence one reading of each attribute and no message before a test fails.
 def _batch(pages, table, row_start, kv_len):
-    """Checks what describes a ragged batch; -> the number of sequences."""
-    dev = pages.device
-    if dev.index != _device():
-        raise HipsterError(1, f"the pages are on device {dev.index}, and device {_device()} is current")
-    S, = kv_len.shape
-    rows, cols = table.shape
-    if not (table.dtype is torch.int32 and row_start.dtype is torch.int32 and kv_len.dtype is torch.int32):
+    """Checks what describes a ragged batch; -> number of sequences, and its addresses as the calls take them."""
+    dev, S = pages._dev, kv_len.numel()
+    (rows, cols), (ld, one) = table.shape, table.stride()
+    if dev != _device():
+        raise HipsterError(1, f"the pages are on device {dev}, and device {_device()} is current")
+    if not (table.dtype is _I32 and row_start.dtype is _I32 and kv_len.dtype is _I32):
         raise HipsterError(1, "table, row_start and kv_len must be int32")
-    if not (rows == S and row_start.numel() == S + 1 and table.stride(1) == 1 and (S == 1 or table.stride(0) >= cols) and row_start.is_contiguous() and kv_len.is_contiguous()):
+    if not (rows == S and row_start.numel() == S + 1 and one == 1 and (ld >= cols or S == 1) and row_start.is_contiguous() and kv_len.is_contiguous()):
         raise HipsterError(1, "table [S][columns], row_start [S + 1] and kv_len [S] must be contiguous")
-    if not (table.device == dev and row_start.device == dev and kv_len.device == dev):
+    if not (table.get_device() == dev and row_start.get_device() == dev and kv_len.get_device() == dev):
         raise HipsterError(1, "table, row_start and kv_len must be on the device of the pages")
-    return S
+    return S, table.data_ptr(), ld if S > 1 else max(cols, 1), row_start.data_ptr(), kv_len.data_ptr()
 
 
-def _rows(t, pages, R, what):
+def _rows(t, pages, R, heads, what):
     """f32 rows [R][heads][head_dim] -> address, row stride, head stride."""
-    shape, (ld, hs, one) = t.shape, t.stride()
-    if not (t.dtype is torch.float32 and shape[0] == R and shape[2] == pages.head_dim and one == 1 and t.device == pages.device):
-        raise HipsterError(1, f"{what} must be f32 [R][heads][head_dim] on the device of the pages")
+    ld, hs, one = t.stride()
+    if not (t.dtype is _F32 and t.shape == (R, heads, pages.head_dim) and one == 1 and t.get_device() == pages._dev):
+        raise HipsterError(1, f"{what} must be f32 [{R}][{heads}][{pages.head_dim}] on the device of the pages")
     return t.data_ptr(), ld, hs
 
 
@@ -225,18 +227,19 @@ _SCALING = {None: 0, "none": 0, "linear": 1, "yarn": 2}
 def rope_table(n_pos, n_rot, base, scaling=None, factor=1.0, orig_ctx=0, beta_fast=32.0, beta_slow=1.0, attn_factor=0.0, device="cuda"):
     """(cos, sin) of pos * base^(-2 i / n_rot), f32 [n_pos][n_rot / 2][2], computed in 64 bits; scaling "linear" divides the frequencies by factor, "yarn"
     by parts: those that turn less than beta_slow times over orig_ctx positions wholly, those over beta_fast times not."""
-    _refuse(scaling in _SCALING, f"rope_table: unknown scaling {scaling!r}")
-    out = torch.empty((n_pos, n_rot // 2, 2), dtype=torch.float32, device=device)
-    _refuse(out.device.index == _device(), "rope_table: the device must be the current one")
-    d = ctypes.c_double
-    check(lib().hp_rope_table(ptr(out), n_pos, n_rot, d(base), _SCALING[scaling], d(factor), orig_ctx, d(beta_fast), d(beta_slow), d(attn_factor), _stream()))
+    if scaling not in _SCALING:
+        raise HipsterError(1, f"rope_table: unknown scaling {scaling!r}")
+    out = torch.empty((n_pos, n_rot // 2, 2), dtype=_F32, device=device)
+    if out.get_device() != _device():
+        raise HipsterError(1, "rope_table: the device must be the current one")
+    check(hot().hp_rope_table(out.data_ptr(), n_pos, n_rot, base, _SCALING[scaling], factor, orig_ctx, beta_fast, beta_slow, attn_factor, _raw_stream(_device())))
     return out
 
 
 def _norm_weight(w, pages):
     if w is None:
         return None
-    if not (w.dtype in (torch.bfloat16, torch.int16) and w.shape == (pages.head_dim,) and w.is_contiguous() and w.device == pages.device):
+    if not (w.dtype in (torch.bfloat16, torch.int16) and w.shape == (pages.head_dim,) and w.is_contiguous() and w.get_device() == pages._dev):
         raise HipsterError(1, "norm weights are bf16 [head_dim]")
     return w.data_ptr()
 
@@ -245,38 +248,43 @@ def kv_append(pages, k, v, table, row_start, kv_len, rope=None, q=None, q_out=No
     """Appends rows k, v f32 [R][n_kv][head_dim] of a ragged batch to their sequences' pages, k normalised (k_norm bf16 [head_dim]) and rotated by rope
     f32 [n_pos][n_rot / 2][2]. q [R][n_head][head_dim] is normalised and rotated alike. -> q_out (f32 [R][n_head][head_dim]; None without q).
     Rows row_start[s] .. row_start[s + 1] - 1 are the newest of the kv_len[s] tokens of sequence s."""
-    S, R = _batch(pages, table, row_start, kv_len), k.shape[0]
-    kr, vr = _rows(k, pages, R, "k"), _rows(v, pages, R, "v")
-    _refuse(k.shape[1] == v.shape[1] == pages.n_kv, "kv_append: k and v have the heads of the pages")
+    S, *at = _batch(pages, table, row_start, kv_len)
+    R, n_kv = k.shape[0], pages.n_kv
     qr = qo = (None, 0, 0)
-    n_head = 0
+    n_head = n_pos = n_rot = 0
     if q is not None:
-        n_head, qr = q.shape[1], _rows(q, pages, R, "q")
+        n_head = q.shape[1]
+        qr = _rows(q, pages, R, n_head, "q")
         if q_out is None:
-            q_out = torch.empty((R, n_head, pages.head_dim), dtype=torch.float32, device=pages.device)
-        qo = _rows(q_out, pages, R, "q_out")
-        _refuse(q_out.shape[1] == n_head, "kv_append: q_out has the heads of q")
-    n_pos = n_rot = 0
+            q_out = q.new_empty((R, n_head, pages.head_dim))
+        qo = _rows(q_out, pages, R, n_head, "q_out")
     if rope is not None:
         n_pos, n_rot, two = rope.shape
         n_rot *= 2
-        _refuse(rope.dtype is torch.float32 and two == 2 and rope.is_contiguous() and rope.device == pages.device, "kv_append: rope must be f32 [n_pos][n_rot / 2][2]")
-    check(hot().hp_kv_append(*qr, *qo, n_head, *kr, *vr, _norm_weight(q_norm, pages), _norm_weight(k_norm, pages), None if rope is None else rope.data_ptr(), n_pos, n_rot, int(interleaved), table.data_ptr(), table.stride(0), row_start.data_ptr(), kv_len.data_ptr(), S, R, pages._at, eps, _raw_stream(_device())))
+        if not (rope.dtype is _F32 and two == 2 and rope.is_contiguous() and rope.get_device() == pages._dev):
+            raise HipsterError(1, "kv_append: rope must be f32 [n_pos][n_rot / 2][2]")
+        rope = rope.data_ptr()
+    check(hot().hp_kv_append(*qr, *qo, n_head, *_rows(k, pages, R, n_kv, "k"), *_rows(v, pages, R, n_kv, "v"), _norm_weight(q_norm, pages), _norm_weight(k_norm, pages), rope, n_pos, n_rot, int(interleaved),
+                             *at, S, R, pages._at, eps, _raw_stream(pages._dev)))
     return q_out
 
 
 def kv_read(pages, table, row_start, kv_len, R=None, k_out=None, v_out=None):
     """The tokens of the rows back as f16 -> k, v [R][n_kv][head_dim]. With kv_len[s] rows for each sequence whole caches; k_out, v_out may be views with other
     strides, as cache.transpose(0, 1) of an f16 [n_kv][max_ctx][256] cache for attn_decode."""
-    S = _batch(pages, table, row_start, kv_len)
-    if k_out is None:
-        _refuse(v_out is None and R is not None and R >= 1, "kv_read: give R, or both outputs")
-        k_out, v_out = torch.empty((2, R, pages.n_kv, pages.head_dim), dtype=torch.float16, device=pages.device).unbind(0)
-    R, (ld, hs, one) = k_out.shape[0], k_out.stride()
-    if not (v_out is not None and k_out.shape == (R, pages.n_kv, pages.head_dim) and v_out.shape == k_out.shape and v_out.stride() == (ld, hs, 1) and one == 1 and k_out.dtype is torch.float16 and
-            v_out.dtype is torch.float16 and k_out.device == pages.device and v_out.device == pages.device):
-        raise HipsterError(1, "kv_read: outputs are f16 [R][n_kv][head_dim] with the same strides")
-    check(hot().hp_kv_read(table.data_ptr(), table.stride(0), row_start.data_ptr(), kv_len.data_ptr(), S, R, pages._at, k_out.data_ptr(), v_out.data_ptr(), ld, hs, _raw_stream(_device())))
+    S, *at = _batch(pages, table, row_start, kv_len)
+    n_kv, D = pages.n_kv, pages.head_dim
+    if k_out is None and v_out is None and R is not None:
+        k_out, v_out = pages._f16.new_empty((R, n_kv, D)), pages._f16.new_empty((R, n_kv, D))
+        ld, hs = n_kv * D, D
+    else:
+        if k_out is None or v_out is None:
+            raise HipsterError(1, "kv_read: give R, or both outputs")
+        R, (ld, hs, one) = k_out.shape[0], k_out.stride()
+        if not (k_out.shape == (R, n_kv, D) and v_out.shape == k_out.shape and v_out.stride() == (ld, hs, 1) and one == 1 and k_out.dtype is _F16 and v_out.dtype is _F16 and
+                k_out.get_device() == pages._dev and v_out.get_device() == pages._dev):
+            raise HipsterError(1, "kv_read: outputs are f16 [R][n_kv][head_dim] with the same strides")
+    check(hot().hp_kv_read(*at, S, R, pages._at, k_out.data_ptr(), v_out.data_ptr(), ld, hs, _raw_stream(pages._dev)))
     return k_out, v_out
 
 
@@ -289,17 +297,14 @@ def attn_paged(q, pages, table, row_start, kv_len, max_rows, max_kv, scale=None,
     """Attention of rows q f32 [R][n_head][head_dim] over their sequences' pages (causal; window > 0: the last `window` tokens and the first n_sink), times sigmoid(gate)
     where a gate [R][n_head][head_dim] is given. scale: 1 / sqrt(head_dim). max_rows, max_kv bound the rows and tokens of a sequence.
     -> (out f32 [R][n_head][head_dim] or None, XQ8 of its rows or None)."""
-    S, (R, n_head, D) = _batch(pages, table, row_start, kv_len), q.shape
-    qr = _rows(q, pages, R, "q")
-    gr = (None, 0, 0)
-    if gate is not None:
-        gr = _rows(gate, pages, R, "gate")
-        _refuse(gate.shape[1] == n_head, "attn_paged: gate has the heads of q")
+    (S, *at), (R, n_head, D) = _batch(pages, table, row_start, kv_len), q.shape
+    qr = _rows(q, pages, R, n_head, "q")
+    gr = (None, 0, 0) if gate is None else _rows(gate, pages, R, n_head, "gate")
     c = pages._c
-    nb = _attn_paged_workspace_bytes(table.stride(0), S, R, max_rows, -(-max_kv // 1024) * 1024, n_head, window, n_sink, c.type, c.n_pages, c.n_kv, c.page_size, c.head_dim)   # grows with max_kv
-    ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=pages.device)
-    out = torch.empty((R, n_head, D), dtype=torch.float32, device=pages.device) if want_f32 else None
+    nb = _attn_paged_workspace_bytes(at[1], S, R, max_rows, -(-max_kv // 1024) * 1024, n_head, window, n_sink, c.type, c.n_pages, c.n_kv, c.page_size, c.head_dim)   # grows with max_kv
+    ws = q.new_empty(nb // 4 + 4)
+    out = q.new_empty((R, n_head, D)) if want_f32 else None
     xq = XQ8(R, n_head * D, pages.device) if want_q8 else None
-    check(hot().hp_attn_paged(*qr, *gr, n_head, table.data_ptr(), table.stride(0), row_start.data_ptr(), kv_len.data_ptr(), S, R, max_rows, max_kv, pages._at, D ** -0.5 if scale is None else scale, window, n_sink,
-                              None if out is None else out.data_ptr(), xq.q.data_ptr() if xq else None, xq.sc.data_ptr() if xq else None, ws.data_ptr(), _raw_stream(_device())))
+    check(hot().hp_attn_paged(*qr, *gr, n_head, *at, S, R, max_rows, max_kv, pages._at, D ** -0.5 if scale is None else scale, window, n_sink, None if out is None else out.data_ptr(),
+                              xq.q.data_ptr() if xq else None, xq.sc.data_ptr() if xq else None, ws.data_ptr(), _raw_stream(pages._dev)))
     return out, xq
