@@ -373,17 +373,28 @@ __global__ void __launch_bounds__(256) k_paged_merge(const MergeArgs a) {
 }
 
 struct Plan { int U, ns, nwin, MB; long long blocks; };
-// Splits lie at multiples of U, a number that the cache's capacity and the window alone decide, so that a row's sums do not hang on what else is in the
-// call. Calls of more than 8 rows per sequence (prompts) have blocks enough and take a row's keys as one split.
+// Splits lie at multiples of U, which the cache's capacity and the window alone decide (16 to 32 splits and more of a full sequence), so that a row's sums do not hang on what
+// else is in the call. Captured, us: 1 token of 24 heads at 4097, U = 128 13.3, 256 13.3, 512 17.4, 1024 27.7; 48 sequences of up to 8192, 197, 146, 124, 124.
+// Prompts have blocks of rows: their keys are split as the launch fills the GPU best, a split costing the start of a CTA, some two tiles.
 Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink) {
     Plan p;
     const int G = n_head / pool.n_kv, cap = pool.table_ld << pool.lg_page;
     const long long eff = window ? std::min<long long>(cap, (long long)window + n_sink) : cap;
     const long long pairs = (long long)b.max_rows * G;
-    p.MB = b.max_rows > 8 ? PAGED_TC_PAIRS : pairs <= 8 ? 8 : 16;
+    const bool prompt = b.max_rows > PAGED_DECODE_ROWS;
+    p.MB = prompt ? PAGED_TC_PAIRS : pairs <= 8 ? 8 : 16;
     p.blocks = std::min<long long>((long long)b.S * ((pairs + p.MB - 1) / p.MB), (long long)b.R * G / p.MB + b.S);
-    if (b.max_rows > 8) { p.U = 1 << 30; p.ns = 0; p.nwin = 1; return p; }
-    p.U = eff <= 8192 ? 512 : 1024;
+    p.U = eff < 8192 ? 256 : eff < 32768 ? 512 : 1024;
+    if (prompt) {
+        const long long ctas = p.blocks * pool.n_kv, tiles = (b.max_kv + 1023) / 1024 * 8;   // the same splits for all max_kv up to the next 1024: the workspace grows with max_kv
+        long long best = 0; int n = 1;
+        for (int i = 1; i <= 8; ++i) {
+            const long long cost = (ctas * i + 147) / 148 * ((tiles + i - 1) / i + 2);
+            if (i == 1 || cost < best) { best = cost; n = i; }
+        }
+        p.U = n == 1 || window ? 1 << 30 : (int)((tiles + n - 1) / n * 128);
+        if (p.U == 1 << 30) { p.ns = 0; p.nwin = 1; return p; }
+    }
     const int total = (b.max_kv + p.U - 1) / p.U;   // splits of the longest sequence
     p.ns = window ? std::min((n_sink + p.U - 1) / p.U, total) : 0;
     p.nwin = std::max(1, total);
@@ -412,7 +423,7 @@ template <int KIND> int launch_split(const PagedArgs& a, dim3 grid, int MB, cuda
 
 size_t attn_paged_workspace_bytes(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink) {
     const Plan p = plan_of(pool, b, n_head, window, n_sink);
-    return partials(p, b, n_head) * (pool.head_dim + 2) * sizeof(float);
+    return (partials(p, b, n_head) * (pool.head_dim + 2) * sizeof(float) + 127) / 128 * 128 + (b.max_rows > PAGED_DECODE_ROWS ? attn_paged_tc_bytes(pool, b) : 0);
 }
 
 int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams& p, cudaStream_t s) {
@@ -422,8 +433,9 @@ int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams
     a.scale2 = (float)((double)p.scale * 1.4426950408889634074 * (pool.kind == KV_E4M3 ? 256.0 : 1.0)); a.window = p.window; a.n_sink = p.n_sink;
     a.U = pl.U; a.ns = pl.ns; a.nwin = pl.nwin;
     a.pO = (float*)p.workspace; a.pml = (float2*)(a.pO + partials(pl, b, p.n_head) * pool.head_dim); a.err = device_err_flag(); a.arg_err = device_arg_flag();
+    a.f16 = (uint8_t*)p.workspace + (partials(pl, b, p.n_head) * (pool.head_dim + 2) * sizeof(float) + 127) / 128 * 128; a.tiles = 0;
     const dim3 grid(pl.ns + pl.nwin, pool.n_kv, (unsigned)pl.blocks);
-    const int rc = b.max_rows > 8 ? attn_paged_tc(a, grid, s) : pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, pl.MB, s) : launch_split<KV_E4M3>(a, grid, pl.MB, s);
+    const int rc = b.max_rows > PAGED_DECODE_ROWS ? attn_paged_tc(a, grid, s) : pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, pl.MB, s) : launch_split<KV_E4M3>(a, grid, pl.MB, s);
     if (rc != HP_OK) return rc;
     MergeArgs m; m.b = b; m.pO = a.pO; m.pml = a.pml; m.gate = p.gate; m.g_ld = p.g_ld; m.g_hs = p.g_hs; m.n_head = p.n_head; m.window = p.window; m.n_sink = p.n_sink;
     m.U = pl.U; m.ns = pl.ns; m.nwin = pl.nwin; m.mul = pool.kind == KV_E4M3 ? 256.f : 1.f; m.out = p.out; m.oq = (int8_t*)p.xq.q; m.osc = (float*)p.xq.sc; m.err = a.arg_err;

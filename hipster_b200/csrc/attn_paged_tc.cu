@@ -1,25 +1,20 @@
-// Attention of a ragged batch of rows over a cache of 8-bit pages (kv_pages.cu), with a window and first tokens that stay visible.
+// Attention over 8-bit pages for prompts: calls of many rows per sequence. The formulas, the exact splits of q and of the weights, and the merge are those of
+// attn_paged.cu; here the products run on tcgen05, and the codes are turned into f16 once per call instead of once per block of rows.
 //
-// Row r at position p of its sequence: o = sum_j w_j v_j / sum_j w_j over the keys j <= p with j > p - window or j < n_sink (no window: all), w_j =
-// 2^(s_j - mu), s_j = (q . k_j) * scale * log2 e, times sigmoid(gate). No key: zeros.
-//
-// fp32 results from the f16 tensor pipe: codes of int8 and of e4m3 (times 2^-8) are exact in f16, a token's scale multiplies its score or its weight in
-// fp32, and q and the weights (times the scale of v) go in as two f16 each, the value and what is left of it: 22 bits. q is brought to [2^14, 2^15) by a
-// power of two per row, the weights by the reference mu: whole, at least the largest of s_j + log2(scale of v_j) - 14, so that a weight times
-// its scale stays below 2^15 and every rescaling is by a power of two, exact. The tensor pipe adds up head_dim products for a score and the 128 keys of a tile
-// for an output; tiles are added in fp32 registers.
+// k_paged_f16 writes each visible tile of 128 tokens of a kv head as the picture that shared memory holds: rows of 64 dims (128 bytes) per token, 128-byte
+// swizzle, one group of 64 dims behind the other. A row of it is read as the K-major operand of the scores and as the M-major one of the outputs. Converting in the
+// attention kernel itself (from a ring of codes, four warps) took 11000 clocks per tile of 32 pairs: the conversion's instructions, and
+// 3600 clocks of shared memory for codes in, codes out, f16 in and operands out.
 //
 // Both products stand on their heads: keys, then dims, are the 128 rows of tcgen05.mma, and its columns are the pairs (row of the batch, query head) of a
-// kv head, each twice: column i its values, column n + i what is left of them. So the tensor pipe's time goes with the number of pairs (16 pairs: 32 columns),
-// a thread that reads a row of the accumulator has value and rest of every pair at hand, needs one scale of k and of v, and adds up its own keys' weights without
-// another thread until the end. The pairs of a sequence and kv head, row by row, are cut into blocks of up to 32; a CTA holds one block and the keys of one
-// split, in tiles of 128 keys:
-//   producer (one warp): bulk copies of pieces of pages into a ring of 8 KB slots (32, 64 or 128 tokens of 256, 128 or 64 dims)
-//   conversion (four warps): codes -> f16, 128-byte swizzle: a row of 64 dims per key, read as the K-major operand of the scores and as the other's M-major one
-//   MMA (one thread): S[128 keys][pairs] = K q^T, and O[128 dims][pairs] = V^T w, one tile of scores ahead
+// kv head, each twice: column i its values, column MB + i what is left of them. So a thread that reads a row of the accumulator has value and rest of every pair
+// at hand, needs one scale of k and of v, and adds up its own keys' weights without another thread until the end. A CTA holds a block of 48 pairs
+// and the keys of one split, in tiles of 128 keys:
+//   copies (one warp): pictures of k and v into shared memory
+//   products (one thread): S[128 keys][pairs] = K q^T, and O[128 dims][pairs] = V^T w, one tile of scores ahead
 //   weights (two groups of four warps, a thread per key, a group takes every second set of eight pairs): S -> w in shared memory (N-major operand)
 //   sums (a thread per dim): O of the tile into registers
-// Splits lie at fixed positions and a tile's keys at fixed threads: a row's bits depend neither on the other rows of the call nor on the other sequences.
+// Bound by shared memory: a tile's pictures go in (1024 clocks at 256 dims) and, as operands with q and the weights, out again (1800), against 1536 clocks of products.
 #include "paged.cuh"
 #include "tc.cuh"
 #include <algorithm>
@@ -27,19 +22,18 @@
 namespace hp {
 namespace {
 
-constexpr int TK = 128, SLOT = 8192;   // keys of a tile, bytes of a slot of the ring
+constexpr int TK = 128;   // keys of a tile
 
 // Shared memory of a CTA, operands on 1024-byte boundaries. 64 dims of a key (or of a pair of q, 64 columns of the weights of a key) are a row of 128 bytes.
 template <int D, int MB> struct PagedGeo {
     static constexpr int N = 2 * MB, NB = D > 128 ? 2 : 1, ACC = 4 * NB;                 // columns, blocks of 128 dims, warps that sum
-    static constexpr int WARPS = 8 + ACC + 4 + 2, W_ACC = 8, W_CNV = W_ACC + ACC, W_MMA = W_CNV + 4;   // the last one copies
-    static constexpr int OFF_Q = 0, OFF_K = N * D * 2, OFF_V = OFF_K + TK * D * 2, OFF_P = OFF_V + TK * D * 2, OFF_X = OFF_P + TK * 128;
-    static constexpr int X_BYTES = 4096, OFF_RING = OFF_X + X_BYTES, FIXED = OFF_RING + 1024;   // 1024 for the alignment
-    static constexpr int TMEM = NB * N + 2 * N <= 128 ? 128 : 256;
-    static constexpr int ST = SLOT / D;                                                    // tokens of a slot
-    static_assert(OFF_K % 1024 == 0 && NB * N + 2 * N <= 256, "");
+    static constexpr int WARPS = 8 + ACC + 2, W_ACC = 8, W_MMA = W_ACC + ACC;            // the last one copies
+    static constexpr int PICTURE = TK * D * 2;                                            // bytes of a tile of k or v
+    static constexpr int OFF_Q = 0, OFF_K = N * D * 2, OFF_V = OFF_K + PICTURE, OFF_P = OFF_V + PICTURE, OFF_X = OFF_P + (N + 63) / 64 * TK * 128;
+    static constexpr int X_BYTES = 4096, SMEM = OFF_X + X_BYTES + 1024;                   // 1024 for the alignment
+    static constexpr int TMEM = 512;
+    static_assert(OFF_K % 1024 == 0 && NB * N + 2 * N <= TMEM && SMEM <= 226 * 1024, "");
 };
-constexpr int MAX_SLOTS = 16, SMEM_LIMIT = 227 * 1024;
 
 __device__ __forceinline__ float warp_max(float x) { float y; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x)); return y; }
 // 128-byte swizzle, groups of 8 rows 1024 bytes apart. K-major: a row holds 64 elements along K. M- or N-major: a row is one step along K and holds 64 elements
@@ -68,13 +62,13 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) { __syncwarp
 template <int D, int KIND, int MB>
 __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt(const PagedArgs a) {
     using Geo = PagedGeo<D, MB>;
-    constexpr int N = Geo::N, NB = Geo::NB, ST = Geo::ST, NC = MB / 16;
+    constexpr int N = Geo::N, NB = Geo::NB, NC = MB / 16;
     extern __shared__ uint8_t sm_raw[];
     __shared__ uint32_t tmem_ptr;
     uint8_t* const sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     struct Shared {
-        uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], k_full, k_empty, v_full, s_full[2], s_empty[2], p_full, pv_done, o_empty, red[2], fin;
+        uint64_t k_full, k_empty, v_full, s_full[2], s_empty[2], p_full, pv_done, o_empty, red[2], fin;
         alignas(16) float c[MB]; float alpha[2][MB], top[2][2][4][8 * NC], l[2][4][8 * NC];   // factor of a pair's scores; rescaling by tile; largest scores by tile, group, warp
         int2 see[MB]; int at[MB];                                            // a pair's position and the last key in front of its window; row * n_head + head, -1: nothing to write
     };
@@ -101,8 +95,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
     };
 
     if (tid == 0) {
-        for (int i = 0; i < a.slots; ++i) { mbar_init(smem_u32(&x.full[i]), 1); mbar_init(smem_u32(&x.empty[i]), 4); }
-        mbar_init(smem_u32(&x.k_full), 4); mbar_init(smem_u32(&x.k_empty), 1); mbar_init(smem_u32(&x.v_full), 4);
+        mbar_init(smem_u32(&x.k_full), 1); mbar_init(smem_u32(&x.k_empty), 1); mbar_init(smem_u32(&x.v_full), 1);
         for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); mbar_init(smem_u32(&x.s_empty[i]), 8); mbar_init(smem_u32(&x.red[i]), 4); }
         mbar_init(smem_u32(&x.p_full), 8); mbar_init(smem_u32(&x.pv_done), 1); mbar_init(smem_u32(&x.o_empty), Geo::ACC); mbar_init(smem_u32(&x.fin), 1);
         fence_barrier_init();
@@ -154,6 +147,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
     tc_fence_after();
     const uint32_t tmem = tmem_ptr;
     bool ok = true;
+    int sent[2] = {0, 0};   // pictures under way (copies)
 
     if (warp < 8) {   // ---- weights
         const int grp = warp >> 2, qt = warp & 3, key = qt * 32 + lane;
@@ -248,8 +242,9 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
                         const float2 f = __half22float2(hh);
                         h[e / 2] = h2_bits(hh); r[e / 2] = h2_bits(__floats2half2_rn(y[0] - f.x, y[1] - f.y));
                     }
-                    *reinterpret_cast<uint4*>(pw + (((c8 / 8) ^ (key & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(pw + (((MB / 8 + c8 / 8) ^ (key & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+                    const int ch = c8 / 8, cr = MB / 8 + ch;   // eights of columns; 64 columns of all keys lie one behind the other
+                    *reinterpret_cast<uint4*>(pw + (ch >> 3) * (TK * 128) + (((ch & 7) ^ (key & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(pw + (cr >> 3) * (TK * 128) + (((cr & 7) ^ (key & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
                 }
             }
             fence_proxy_async();
@@ -275,7 +270,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
             if (pair < np && x.at[pair] >= 0)
                 a.pml[(size_t)x.at[pair] * (a.ns + a.nwin) + blockIdx.x] = make_float2(mu, ((x.l[grp][0][lane] + x.l[grp][1][lane]) + x.l[grp][2][lane]) + x.l[grp][3][lane]);
         }
-    } else if (warp < Geo::W_CNV) {   // ---- sums
+    } else if (warp < Geo::W_MMA) {   // ---- sums
         const int b = (warp - Geo::W_ACC) >> 2, qt = warp & 3, dim = 128 * b + 32 * qt + lane;
         const uint32_t ob = tmem + ((uint32_t)qt << 21) + 2 * N + b * N;
         float O[MB];
@@ -286,57 +281,24 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
             ok = warp_wait(smem_u32(&x.pv_done), n & 1, a.err);
             if (!ok) break;
             tc_fence_after();
-            float f[MB / 8][8];
 #pragma unroll
-            for (int c = 0; c < MB / 8; ++c) if (8 * c < np) ld_sum8(f[c], ob + 8 * c, ob + MB + 8 * c);
-            float4 al[MB / 4];
-#pragma unroll
-            for (int c = 0; c < MB / 4; ++c) al[c] = *reinterpret_cast<const float4*>(&x.alpha[n & 1][4 * c]);
+            for (int c = 0; c < MB / 8; ++c) {
+                if (8 * c < np) {
+                    float f[8];
+                    ld_sum8(f, ob + 8 * c, ob + MB + 8 * c);
+                    const float4 u = *reinterpret_cast<const float4*>(&x.alpha[n & 1][8 * c]), v = *reinterpret_cast<const float4*>(&x.alpha[n & 1][8 * c + 4]);
+                    float* o = O + 8 * c;
+                    o[0] = fmaf(o[0], u.x, f[0]); o[1] = fmaf(o[1], u.y, f[1]); o[2] = fmaf(o[2], u.z, f[2]); o[3] = fmaf(o[3], u.w, f[3]);
+                    o[4] = fmaf(o[4], v.x, f[4]); o[5] = fmaf(o[5], v.y, f[5]); o[6] = fmaf(o[6], v.z, f[6]); o[7] = fmaf(o[7], v.w, f[7]);
+                }
+            }
             tc_fence_before();
             warp_arrive(smem_u32(&x.o_empty), lane);
-#pragma unroll
-            for (int c = 0; c < MB / 4; ++c)
-                if (4 * c < np) {
-                    O[4 * c] = fmaf(O[4 * c], al[c].x, f[c / 2][4 * (c & 1)]); O[4 * c + 1] = fmaf(O[4 * c + 1], al[c].y, f[c / 2][4 * (c & 1) + 1]);
-                    O[4 * c + 2] = fmaf(O[4 * c + 2], al[c].z, f[c / 2][4 * (c & 1) + 2]); O[4 * c + 3] = fmaf(O[4 * c + 3], al[c].w, f[c / 2][4 * (c & 1) + 3]);
-                }
         }
         if (ok && dim < D) {
 #pragma unroll
             for (int i = 0; i < MB; ++i)
                 if (i < np && x.at[i] >= 0) a.pO[((size_t)x.at[i] * (a.ns + a.nwin) + blockIdx.x) * D + dim] = O[i];
-        }
-    } else if (warp < Geo::W_MMA) {   // ---- conversion: a warp takes a quarter of each slot, 16 codes per lane and step
-        const int cw = warp - Geo::W_CNV;
-        int k = 0, n = 0;
-        for (int t = t_first; t < t_end && ok; t = first_from(t + 1), ++n) {
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-                ok = ok && warp_wait(kv ? smem_u32(&x.pv_done) : smem_u32(&x.k_empty), (n & 1) ^ 1, a.err);   // the operand of the tile before is read
-                uint8_t* const dst = sm + (kv ? Geo::OFF_V : Geo::OFF_K);
-                for (int sl = 0; sl < TK / ST && ok; ++sl, ++k) {
-                    const int slot = k % a.slots;
-                    ok = warp_wait(smem_u32(&x.full[slot]), (k / a.slots) & 1, a.err);
-                    if (!ok) break;
-                    const uint4* src = reinterpret_cast<const uint4*>(sm + Geo::OFF_RING + slot * SLOT + cw * (SLOT / 4));
-                    uint4 w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = src[i * 32 + lane];
-                    warp_arrive(smem_u32(&x.empty[slot]), lane);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int e = i * 32 + lane, row = sl * ST + cw * (ST / 4) + e / (D / 16), part = e % (D / 16);
-                        const uint4 h0 = make_uint4(code_pair<KIND, 0>(w[i].x), code_pair<KIND, 2>(w[i].x), code_pair<KIND, 0>(w[i].y), code_pair<KIND, 2>(w[i].y));
-                        const uint4 h1 = make_uint4(code_pair<KIND, 0>(w[i].z), code_pair<KIND, 2>(w[i].z), code_pair<KIND, 0>(w[i].w), code_pair<KIND, 2>(w[i].w));
-                        uint8_t* o = dst + (part >> 2) * (TK * 128) + row * 128;
-                        const int ch = (part & 3) * 2, odd = (part >> 2) & 1;   // lanes of neighbouring blocks of 64 dims store the halves the other way round: other banks
-                        *reinterpret_cast<uint4*>(o + (((ch + odd) ^ (row & 7)) << 4)) = odd ? h1 : h0;
-                        *reinterpret_cast<uint4*>(o + (((ch + 1 - odd) ^ (row & 7)) << 4)) = odd ? h0 : h1;
-                    }
-                }
-                fence_proxy_async();
-                if (ok) warp_arrive(kv ? smem_u32(&x.v_full) : smem_u32(&x.k_full), lane);
-            }
         }
     } else if (warp == Geo::W_MMA) {   // ---- products
         const uint32_t base = smem_u32(sm);
@@ -350,7 +312,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int i = 0; i < TK / 16; ++i)   // 16 keys
-                        mma_f16(tmem + 2 * N + b * N, desc128(base + Geo::OFF_V + b * 2 * (TK * 128) + i * 2048, TK * 128), desc128(base + Geo::OFF_P + i * 2048, 16), ID_O, i != 0);
+                        mma_f16(tmem + 2 * N + b * N, desc128(base + Geo::OFF_V + b * 2 * (TK * 128) + i * 2048, TK * 128), desc128(base + Geo::OFF_P + i * 2048, TK * 128), ID_O, i != 0);
                 tc_commit(smem_u32(&x.pv_done));
             }
             __syncwarp();
@@ -374,53 +336,93 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
         if (tc_elect()) tc_commit(smem_u32(&x.fin));
         __syncwarp();
         tc_wait(smem_u32(&x.fin), 0, a.err);   // nothing in flight when the accumulator memory is given back
-    } else {   // ---- copies: lane i holds the page of the tile's i-th piece of up to 16 .. 128 tokens
-        const int pt = min(1 << lg, ST);   // tokens of a copy: within a page and a slot
-        uint32_t page = page_of(t_first * TK + lane * pt < t_first * TK + TK ? t_first * TK + lane * pt : 0x7fffffff);
-        int k = 0;
-        for (int t = t_first; t < t_end && ok; ) {
-            const int t1 = first_from(t + 1);
-            const uint32_t next = t1 < t_end && lane * pt < TK ? page_of(t1 * TK + lane * pt) : 0xffffffffu;
+    } else {   // ---- copies
+        const uint8_t* src = a.f16 + ((size_t)sq.s * a.pool.n_kv + kh) * a.tiles * (2 * Geo::PICTURE);
+        int n = 0;
+        for (int t = t_first; t < t_end && ok; t = first_from(t + 1), ++n) {
 #pragma unroll
-            for (int kv = 0; kv < 2; ++kv)
-                for (int sl = 0; sl < TK / ST && ok; ++sl, ++k) {
-                    const int slot = k % a.slots;
-                    ok = warp_wait(smem_u32(&x.empty[slot]), ((k / a.slots) & 1) ^ 1, a.err);
-                    if (!ok) break;
-                    const int i0 = sl * ST / pt, cnt = ST / pt;
-                    const bool mine = lane >= i0 && lane < i0 + cnt && page != 0xffffffffu;
-                    const int live = __popc(__ballot_sync(0xffffffffu, mine));
-                    const uint32_t bar = smem_u32(&x.full[slot]);
-                    if (lane == 0) { if (live) mbar_expect_tx(bar, (uint32_t)(live * pt * D)); else mbar_arrive(bar); }
-                    __syncwarp();
-                    if (mine)
-                        bulk_g2s(smem_u32(sm + Geo::OFF_RING + slot * SLOT + (lane - i0) * pt * D), (kv ? a.pool.v : a.pool.k) + ((size_t)page + ((t * TK + lane * pt) & pmask)) * D, (uint32_t)(pt * D), bar);
+            for (int kv = 0; kv < 2; ++kv) {
+                ok = ok && warp_wait(kv ? smem_u32(&x.pv_done) : smem_u32(&x.k_empty), (n & 1) ^ 1, a.err);   // the operand of the tile before is read
+                if (!ok) break;
+                const uint32_t bar = smem_u32(kv ? &x.v_full : &x.k_full), dst = smem_u32(sm + (kv ? Geo::OFF_V : Geo::OFF_K));
+                if (tc_elect()) {
+                    mbar_expect_tx(bar, Geo::PICTURE);
+#pragma unroll
+                    for (int i = 0; i < D / 64; ++i) bulk_g2s(dst + i * (TK * 128), src + ((size_t)t * 2 + kv) * Geo::PICTURE + i * (TK * 128), TK * 128, bar);
                 }
-            page = next; t = t1;
+                __syncwarp();
+                sent[kv] = n + 1;
+            }
         }
-        for (int i = k > a.slots ? k - a.slots : 0; i < k; ++i) tc_wait(smem_u32(&x.full[i % a.slots]), (i / a.slots) & 1, a.err);   // no copy outlives the CTA
+        // no copy outlives the CTA
+        if (sent[0]) tc_wait(smem_u32(&x.k_full), (sent[0] - 1) & 1, a.err);
+        if (sent[1]) tc_wait(smem_u32(&x.v_full), (sent[1] - 1) & 1, a.err);
     }
     tc_fence_before();
     __syncthreads();
     if (warp == Geo::W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Geo::TMEM) : "memory");
 }
 
-template <int D, int KIND, int MB> int launch_split(PagedArgs& a, dim3 grid, cudaStream_t s) {
+// The pictures: grid (tiles, 2 n_kv, sequences); a thread turns 16 codes into two pieces of 16 bytes. Tokens that no row sees are zeros in a tile of which others are seen;
+// tiles without a visible token are not written, nor read.
+template <int KIND>
+__global__ void __launch_bounds__(256) k_paged_f16(const PagedArgs a) {
+    const int lane = threadIdx.x & 31, t = blockIdx.x, h = blockIdx.y >> 1, kv = blockIdx.y & 1, D = a.pool.head_dim, cpr = D / 16, lg = a.pool.lg_page, pmask = (1 << lg) - 1;
+    __shared__ uint32_t rows[TK / 16];   // the pool's rows of the tile's runs of 16 tokens
+    pdl_wait();
+    pdl_launch_dependents();   // behind the wait: what was enqueued in front of this kernel is complete when the attention starts
+    const PagedSeq q = paged_seq(a.b, blockIdx.z, a.arg_err);
+    const int pos_lo = max(q.len - q.T, 0), lo = a.window ? max(0, pos_lo - a.window + 1) : 0, sink = a.window ? a.n_sink : 0;
+    if (q.T == 0 || t * TK >= q.len || (t * TK >= sink && t * TK + TK <= lo)) return;
+    if (threadIdx.x < TK / 16) {
+        const int j = t * TK + 16 * lane, k = j & ~pmask;
+        uint32_t r = 0xffffffffu;
+        if (j < q.len && (k < sink || k + pmask >= lo)) { r = paged_row(a.pool, q.s, j >> lg, h, a.arg_err); if (r != 0xffffffffu) r += j & pmask; }
+        rows[lane] = r;
+    }
+    __syncthreads();
+    uint8_t* const dst = a.f16 + ((((size_t)blockIdx.z * a.pool.n_kv + h) * a.tiles + t) * 2 + kv) * ((size_t)TK * D * 2);
+    const uint8_t* src = kv ? a.pool.v : a.pool.k;
+    for (int e0 = threadIdx.x; e0 < TK * cpr; e0 += 4 * 256) {
+        uint4 w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int e = e0 + u * 256, row = e / cpr, part = e % cpr;
+            w[u] = make_uint4(0, 0, 0, 0);   // codes of zero
+            if (e < TK * cpr && rows[row >> 4] != 0xffffffffu && t * TK + row < q.len) w[u] = *reinterpret_cast<const uint4*>(src + ((size_t)rows[row >> 4] + (row & 15)) * D + part * 16);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int e = e0 + u * 256, row = e / cpr, part = e % cpr;
+            if (e >= TK * cpr) break;
+            uint8_t* o = dst + (part >> 2) * (TK * 128) + row * 128;
+            const int ch = (part & 3) * 2;
+            *reinterpret_cast<uint4*>(o + ((ch ^ (row & 7)) << 4)) = make_uint4(code_pair<KIND, 0>(w[u].x), code_pair<KIND, 2>(w[u].x), code_pair<KIND, 0>(w[u].y), code_pair<KIND, 2>(w[u].y));
+            *reinterpret_cast<uint4*>(o + (((ch + 1) ^ (row & 7)) << 4)) = make_uint4(code_pair<KIND, 0>(w[u].z), code_pair<KIND, 2>(w[u].z), code_pair<KIND, 0>(w[u].w), code_pair<KIND, 2>(w[u].w));
+        }
+    }
+}
+
+template <int D, int KIND, int MB> int launch_split(const PagedArgs& a, dim3 grid, cudaStream_t s) {
     using Geo = PagedGeo<D, MB>;
     static bool attr[MAX_DEVICES] = {};   // per device: the opt-in belongs to the device's copy of the kernel
     const int dev = current_device(); if (dev < 0) return HP_ECUDA;
-    a.slots = std::min(MAX_SLOTS, (SMEM_LIMIT - 1024 - Geo::FIXED) / SLOT);   // 1024: what the kernel declares besides
-    const int smem = Geo::FIXED + a.slots * SLOT;
-    if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_prompt<D, KIND, MB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); attr[dev] = true; }
-    HP_CUDA(launch_pdl<4>(k_paged_prompt<D, KIND, MB>, grid, dim3(Geo::WARPS * 32), smem, s, a));
+    if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_prompt<D, KIND, MB>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo::SMEM)); attr[dev] = true; }
+    HP_CUDA(launch_pdl<4>(k_paged_f16<KIND>, dim3(a.tiles, 2 * a.pool.n_kv, a.b.S), dim3(256), 0, s, a));
+    HP_CUDA(launch_pdl<4>(k_paged_prompt<D, KIND, MB>, grid, dim3(Geo::WARPS * 32), Geo::SMEM, s, a));
     return HP_OK;
 }
-template <int KIND> int launch_split(PagedArgs& a, dim3 grid, cudaStream_t s) {
+template <int KIND> int launch_split(const PagedArgs& a, dim3 grid, cudaStream_t s) {
     return a.pool.head_dim == 256 ? launch_split<256, KIND, PAGED_TC_PAIRS>(a, grid, s) : a.pool.head_dim == 128 ? launch_split<128, KIND, PAGED_TC_PAIRS>(a, grid, s) : launch_split<64, KIND, PAGED_TC_PAIRS>(a, grid, s);
 }
 
 }  // namespace
 
-int attn_paged_tc(PagedArgs& a, dim3 grid, cudaStream_t s) { return a.pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, s) : launch_split<KV_E4M3>(a, grid, s); }
+size_t attn_paged_tc_bytes(const PagedPool& pool, const PagedBatch& b) { return (size_t)b.S * pool.n_kv * ((b.max_kv + TK - 1) / TK) * (2 * TK * 2) * pool.head_dim; }
+int attn_paged_tc(PagedArgs& a, dim3 grid, cudaStream_t s) {
+    a.tiles = (a.b.max_kv + TK - 1) / TK;
+    HP_REQUIRE(a.b.S <= 65535 && 2 * a.pool.n_kv <= 65535, "attn_paged: too many sequences (%d) or heads for a prompt", a.b.S);
+    return a.pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, s) : launch_split<KV_E4M3>(a, grid, s);
+}
 
 }  // namespace hp

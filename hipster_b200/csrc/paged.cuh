@@ -44,13 +44,15 @@ struct PagedArgs {
     PagedPool pool; PagedBatch b;
     const float* q; size_t q_ld, q_hs; int n_head, G; float scale2;   // scale2 = scale * log2 e (times 256 for e4m3)
     int window, n_sink;
-    int U, ns, nwin, slots;     // keys of a split, splits of the first tokens, splits behind them; slots of the prompt kernel's ring
+    int U, ns, nwin;            // keys of a split, splits of the first tokens, splits behind them
     float* pO; float2* pml;     // partials [row][head][ns + nwin] (x head_dim): sums, (mu, sum of weights)
+    uint8_t* f16; int tiles;    // prompts: tiles of 128 tokens in f16, [sequence][kv head][tiles][k, v]
     int* err; int* arg_err;
 };
 
-// the prompt kernel: MB pairs per CTA
-constexpr int PAGED_TC_PAIRS = 32;
+// Prompts, calls of more than PAGED_DECODE_ROWS rows per sequence: blocks of PAGED_TC_PAIRS pairs, and the bytes of their f16 tiles
+constexpr int PAGED_DECODE_ROWS = 16, PAGED_TC_PAIRS = 48;
+size_t attn_paged_tc_bytes(const PagedPool& pool, const PagedBatch& b);
 int attn_paged_tc(PagedArgs& a, dim3 grid, cudaStream_t s);
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }

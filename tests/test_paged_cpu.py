@@ -102,10 +102,15 @@ def test_workspace_sizes():
     L = hb.lib()
     L.hp_attn_paged_workspace_bytes.restype = ctypes.c_size_t
     f = lambda p=None, ld=64, S=4, R=8, mr=2, mk=1000, nh=4, w=0, k=0: L.hp_attn_paged_workspace_bytes(ld, S, R, mr, mk, nh, w, k, ctypes.byref(p or pages()))  # noqa: E731
-    assert f() == 8 * 4 * 4 * (64 + 2) * 4                       # four splits of 256 keys
-    assert f(R=16, mr=9) == f(R=16, mr=9, mk=2000) == 16 * 4 * (64 + 2) * 4   # prompts: one
-    assert f(w=200) == 8 * 4 * 2 * (64 + 2) * 4                  # a run of up to 201 keys lies in two splits
-    assert f(w=200, k=3) == 8 * 4 * 3 * (64 + 2) * 4             # and the first tokens in one more
+    part = (64 + 2) * 4
+    up = lambda n: (n + 127) // 128 * 128  # noqa: E731
+    assert f() == up(8 * 4 * 4 * part)                       # four splits of 256 keys
+    assert f(ld=1024, mk=1000) == up(8 * 4 * 2 * part)       # two of 512
+    assert f(w=200) == up(8 * 4 * 2 * part)                  # a run of up to 201 keys lies in two splits
+    assert f(w=200, k=3) == up(8 * 4 * 3 * part)             # and the first tokens in one more
+    tiles = lambda mk: 4 * 2 * -(-mk // 128) * 2 * 128 * 64 * 2  # noqa: E731
+    assert f(R=4000, mr=1000, w=100) == up(4000 * 4 * part) + tiles(1000)   # prompts: keys and values in f16; a window in one split
+    assert all(f(R=600, mr=300, mk=m) <= f(R=600, mr=300, mk=(m + 1023) // 1024 * 1024) for m in range(1, 5000, 37))
     assert all(f(mk=m) <= f(mk=m + 1) and f(mk=m, w=300, k=5) <= f(mk=m + 1, w=300, k=5) for m in range(1, 1500, 7))
     assert f(p=pages(type=9)) == 0 and f(nh=3) == 0 and f(k=1) == 0
 

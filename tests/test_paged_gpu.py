@@ -330,9 +330,15 @@ def test_attention_window(D, kind, window, n_sink):
 
 
 @pytest.mark.parametrize("D,kind,H,n_kv", [(256, "i8", 24, 4), (128, "e4m3", 7, 1), (64, "i8", 4, 4)])
-@pytest.mark.parametrize("window,n_sink", [(0, 0), (50, 3), (200, 0)])
+@pytest.mark.parametrize("window,n_sink", [(0, 0), (50, 3), (200, 0), (129, 300)])
 def test_attention_prompts(D, kind, H, n_kv, window, n_sink):
-    check_attn([33, 9, 100], [33, 400, 217], H, n_kv, D, 32, kind, window=window, n_sink=n_sink, gate=True)
+    check_attn([33, 9, 0, 100], [33, 400, 70, 217], H, n_kv, D, 32, kind, window=window, n_sink=n_sink, gate=True)
+
+
+@pytest.mark.parametrize("D,kind,H,n_kv,page", [(256, "e4m3", 12, 2, 16), (128, "i8", 2, 1, 1024), (64, "e4m3", 49, 1, 64)])
+def test_attention_long_prompts(D, kind, H, n_kv, page):
+    check_attn([17], [3001], H, n_kv, D, page, kind)                    # few blocks: the keys in several splits
+    check_attn([301, 1], [2301, 2000], H, n_kv, D, page, kind, window=1000, n_sink=130)
 
 
 def test_attention_long_context():
@@ -342,12 +348,12 @@ def test_attention_long_context():
 
 def test_rows_without_a_key_and_rows_behind_the_last():
     st = Setup([3, 1, 2], [1, 0, 40], 1, 64, 16, "i8", cols=3)
-    q = torch.randn((9, 4, 64), generator=gen(2), device="cuda")
-    for mr in (3, 16):   # both forms
-        ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
-        out = torch.full((9, 4, 64), 3.0, device="cuda")
+    q = torch.randn((20, 4, 64), generator=gen(2), device="cuda")
+    for mr in (3, 17):   # both forms
+        ws = torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda")
+        out = torch.full((20, 4, 64), 3.0, device="cuda")
         v, z = ctypes.c_void_p, ctypes.c_longlong
-        hb.check(hb.lib().hp_attn_paged(hb.ptr(q), z(256), z(64), None, z(0), z(0), 4, hb.ptr(st.table), 3, hb.ptr(st.row_start), hb.ptr(st.kv_len), 3, 9, mr, 40, v(st.pool._at), ctypes.c_float(0.125), 0, 0,
+        hb.check(hb.lib().hp_attn_paged(hb.ptr(q), z(256), z(64), None, z(0), z(0), 4, hb.ptr(st.table), 3, hb.ptr(st.row_start), hb.ptr(st.kv_len), 3, 20, mr, 40, v(st.pool._at), ctypes.c_float(0.125), 0, 0,
                                         hb.ptr(out), None, None, hb.ptr(ws), K_._stream()))
         assert status() == 0
         want, tol = attn64(st, q[:6], 0.125, 0, 0, None)
@@ -358,11 +364,11 @@ def test_what_no_row_sees_does_not_count():
     """Codes and scales of masked, unused and foreign slots: NaN, infinity, huge; pages in front of the window are not even in the table."""
     for kind in ("i8", "e4m3"):
         for window, n_sink in ((0, 0), (70, 3)):
-            rows, lens = [2, 1, 12], [300, 201, 250]
+            rows, lens = [2, 1, 20], [300, 201, 250]
             a = Setup(rows, lens, 2, 128, 16, kind, seed=4)
-            q = torch.randn((15, 4, 128), generator=gen(1), device="cuda")
+            q = torch.randn((23, 4, 128), generator=gen(1), device="cuda")
             want = [K_.attn_paged(q[i:j], a.pool, a.table[s:s + 1], torch.tensor([0, j - i], dtype=torch.int32, device="cuda"), a.kv_len[s:s + 1], max_rows=j - i, max_kv=300, window=window, n_sink=n_sink)[0]
-                    for s, (i, j) in enumerate(((0, 2), (2, 3), (3, 15)))]
+                    for s, (i, j) in enumerate(((0, 2), (2, 3), (3, 23)))]
             seen = torch.zeros(a.pool.k.shape[:3], dtype=torch.bool, device="cuda")
             for s, (t, n) in enumerate(zip(rows, lens)):
                 for pos in range(n):
@@ -377,7 +383,7 @@ def test_what_no_row_sees_does_not_count():
                 codes.view(torch.uint8)[~seen] = 0x7f
             a.pool.k_scale[~seen] = math.nan
             a.pool.v_scale[~seen] = math.inf
-            for s, (i, j) in enumerate(((0, 2), (2, 3), (3, 15))):
+            for s, (i, j) in enumerate(((0, 2), (2, 3), (3, 23))):
                 got, _ = K_.attn_paged(q[i:j], a.pool, a.table[s:s + 1], torch.tensor([0, j - i], dtype=torch.int32, device="cuda"), a.kv_len[s:s + 1], max_rows=j - i, max_kv=300, window=window, n_sink=n_sink)
                 assert status() == 0 and torch.isfinite(got).all() and torch.equal(got, want[s])
 
@@ -414,8 +420,8 @@ def test_magnitudes(k_up, v_up):
 
 @pytest.mark.parametrize("D,kind,G,window,n_sink", [(256, "i8", 6, 0, 0), (128, "e4m3", 12, 0, 0), (64, "i8", 5, 300, 4), (256, "e4m3", 12, 100, 1)])
 def test_a_rows_bits_depend_on_nothing_else(D, kind, G, window, n_sink):
-    """Up to 8 rows per sequence: the same bits alone, in a verify pass, and among other sequences."""
-    rows, lens, H = [8, 1, 5, 3], [1300, 600, 271, 1025], 2 * G
+    """Up to 16 rows per sequence: the same bits alone, in a verify pass, and among other sequences."""
+    rows, lens, H = [16, 1, 5, 8], [1300, 600, 271, 1025], 2 * G
     st, q, got = check_attn(rows, lens, H, 2, D, 32, kind, window=window, n_sink=n_sink)
     one = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
     r = 0
@@ -424,7 +430,7 @@ def test_a_rows_bits_depend_on_nothing_else(D, kind, G, window, n_sink):
             alone, _ = K_.attn_paged(q[r:r + 1], st.pool, st.table[s:s + 1], one, torch.tensor([n - t + i + 1], dtype=torch.int32, device="cuda"), max_rows=1, max_kv=n, window=window, n_sink=n_sink)
             assert torch.equal(alone[0], got[r]), (s, i)
             r += 1
-    again, _ = K_.attn_paged(q, st.pool, *st.batch, max_rows=8, max_kv=4000, window=window, n_sink=n_sink)
+    again, _ = K_.attn_paged(q, st.pool, *st.batch, max_rows=16, max_kv=4000, window=window, n_sink=n_sink)
     assert torch.equal(again, got)
 
 
