@@ -6,8 +6,7 @@
 //
 // fp32 results from the f16 tensor pipe: codes of int8 and of e4m3 (times 2^-8) are exact in f16, a token's scale multiplies its score or its weight in
 // fp32, and q and the weights (times the scale of v) go in as two f16 each, the value and what is left of it: 22 bits. q is brought to [2^14, 2^15) by a
-// power of two per row, the weights by the reference mu: whole, at least the largest of s_j + log2(scale of v_j) - 14, so that a weight times
-// its scale stays below 2^15 and every rescaling is by a power of two, exact. The tensor pipe adds up head_dim / 2 products for a score, in three sums, and 16
+// power of two per row, the weights by the reference mu, which is whole: every rescaling is by a power of two, exact (MU_TOP in paged.cuh). The tensor pipe adds up head_dim / 2 products for a score, in three sums, and 16
 // keys for an output; these are added to the running sums in fp32.
 //
 // Keys, and dims, are the 16 rows of mma.sync, the pairs (row of the batch, query head) of a kv head its 8 columns: few pairs waste nothing. A warp has 16 keys at a
@@ -34,12 +33,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   // c = a * b: no zeros to be put into registers
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ void fma_pair(float& x, float& y, float fx, float fy, float ax, float ay) {   // x = x * fx + ax, y = y * fy + ay
-    float2 o = make_float2(x, y);
-    asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(reinterpret_cast<unsigned long long&>(o))
-        : "l"(reinterpret_cast<const unsigned long long&>(static_cast<const float2&>(make_float2(fx, fy)))), "l"(reinterpret_cast<const unsigned long long&>(static_cast<const float2&>(make_float2(ax, ay)))));
-    x = o.x; y = o.y;
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) { uint32_t r; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v)); return r; }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
@@ -144,7 +137,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) { cf[n][c] = s_c[8 * n + 2 * q4 + c]; pos[n][c] = s_pos[8 * n + 2 * q4 + c]; mu[n][c] = -1e30f; l[n][c] = 0.f; }
+        for (int c = 0; c < 2; ++c) { cf[n][c] = s_c[8 * n + 2 * q4 + c]; pos[n][c] = s_pos[8 * n + 2 * q4 + c]; mu[n][c] = MU_NONE; l[n][c] = 0.f; }
     const int win = a.window ? a.window : 1 << 30;
     // slices between these positions are visible to all pairs
     const int all_hi = sp.pos_lo, all_lo = a.window ? sp.pos_hi - a.window : -1;
@@ -202,33 +195,50 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         const int j = i0 * KS + g;
         const bool whole = i0 * KS + KS - 1 <= all_hi && (i0 * KS > all_lo || i0 * KS + KS <= sp.sink);
         bool hide[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) { s[n][c] = s[n][c] * ((c < 2 ? k0 : k1) * cf[n][c & 1]); hide[n][c] = false; }
-        if (!whole) {
+        float d[NT][4], top = -INFINITY;
+        if (whole) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int key = c < 2 ? j : j + 8, p = pos[n][c & 1];
-                    hide[n][c] = !(key <= p && (key > p - win || key < sp.sink));
-                    if (hide[n][c]) s[n][c] = -INFINITY;
+                for (int c = 0; c < 4; ++c) hide[n][c] = false;
+        } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) { const int key = c < 2 ? j : j + 8, p = pos[n][c & 1]; hide[n][c] = !(key <= p && (key > p - win || key < sp.sink)); }
+        }
+        auto distance = [&](int n, int c) { return hide[n][c] ? -INFINITY : fmaf(s[n][c], (c < 2 ? k0 : k1) * cf[n][c & 1], -mu[n][c & 1]); };
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) { d[n][c] = distance(n, c); top = fmaxf(top, d[n][c] + (c < 2 ? lv0 : lv1)); }
+        if (__any_sync(0xffffffffu, top > MU_LIMIT)) {   // rare behind the first slices. A pair moves by its own keys alone
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float t = fmaxf(hide[n][c] ? -INFINITY : s[n][c] * (k0 * cf[n][c]) + lv0, hide[n][c + 2] ? -INFINITY : s[n][c + 2] * (k1 * cf[n][c]) + lv1);
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                    if (t - mu[n][c] > MU_LIMIT) {
+                        const float next = ceilf(t) - MU_TOP, al = pow2i(mu[n][c] - next);
+                        mu[n][c] = next; l[n][c] = l[n][c] * al;
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) { O[i][n][c] = O[i][n][c] * al; O[i][n][c + 2] = O[i][n][c + 2] * al; }
+                    }
                 }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) d[n][c] = distance(n, c);
         }
         uint32_t bh[NT][2], br[NT][2];   // weights times scales of v as columns of pairs: values and rests
-        float al[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float y[4];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float t = fmaxf(s[n][c] + lv0, s[n][c + 2] + lv1);
-                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-                const float next = fmaxf(mu[n][c], ceilf(t) - 14.f);
-                al[n][c] = pow2i(mu[n][c] - next); mu[n][c] = next;
-                const float e0 = ex2(s[n][c] - next), e1 = ex2(s[n][c + 2] - next);
-                l[n][c] = fmaf(l[n][c], al[n][c], e0 + e1);
+                const float e0 = ex2(d[n][c]), e1 = ex2(d[n][c + 2]);
+                l[n][c] = l[n][c] + (e0 + e1);
                 y[c] = hide[n][c] ? 0.f : e0 * v0; y[c + 2] = hide[n][c + 2] ? 0.f : e1 * v1;   // a masked key's scale may be anything
             }
 #pragma unroll
@@ -261,7 +271,8 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
                             mma_f16_first(f, af, br[n][0], br[n][1]);
                             mma_f16(f, af, bh[n][0], bh[n][1]);
                             float (&o)[4] = O[y * 4 + w * 2 + h][n];
-                            fma_pair(o[0], o[1], al[n][0], al[n][1], f[0], f[1]); fma_pair(o[2], o[3], al[n][0], al[n][1], f[2], f[3]);
+                            const float2 u = add2(make_float2(o[0], o[1]), make_float2(f[0], f[1])), t = add2(make_float2(o[2], o[3]), make_float2(f[2], f[3]));
+                            o[0] = u.x; o[1] = u.y; o[2] = t.x; o[3] = t.y;
                         }
                     }
                 }

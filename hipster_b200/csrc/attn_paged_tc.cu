@@ -44,16 +44,17 @@ __device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t next) {
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int add) {   // D = A * B (+ D)
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
-// eight columns from col0 and from col1 of this warp's 32 lanes, added: values and rests
-__device__ __forceinline__ void ld_sum8(float (&v)[8], uint32_t col0, uint32_t col1) {
-    float a[8], b[8];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n"
-                 "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n"
-                 "tcgen05.wait::ld.sync.aligned;"
-                 : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]), "=f"(a[4]), "=f"(a[5]), "=f"(a[6]), "=f"(a[7]), "=f"(b[0]), "=f"(b[1]), "=f"(b[2]), "=f"(b[3]), "=f"(b[4]), "=f"(b[5]), "=f"(b[6]), "=f"(b[7])
-                 : "r"(col0), "r"(col1) : "memory");
+// eight columns from col0 and from col1 of this warp's 32 lanes: values and rests. They are there behind ld_wait
+__device__ __forceinline__ void ld8(float (&a)[8], uint32_t col) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]), "=f"(a[4]), "=f"(a[5]), "=f"(a[6]), "=f"(a[7]) : "r"(col) : "memory");
+}
+template <int C> __device__ __forceinline__ void ld_wait(float (&a)[C][8], float (&b)[C][8]) {   // the empty statements order the use of the registers behind the wait
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = a[i] + b[i];
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { asm volatile("" : "+f"(a[c][i])); asm volatile("" : "+f"(b[c][i])); }
 }
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) { return __all_sync(0xffffffffu, tc_wait(bar, parity, err)); }
 __device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) { __syncwarp(); if (lane == 0) mbar_arrive(bar); }
@@ -69,8 +70,9 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     struct Shared {
         uint64_t k_full, k_empty, v_full, s_full[2], s_empty[2], p_full, pv_done, o_empty, red[2], fin;
-        alignas(16) float c[MB]; float alpha[2][MB], top[2][2][4][8 * NC], l[2][4][8 * NC];   // factor of a pair's scores; rescaling by tile; largest scores by tile, group, warp
-        int2 see[MB]; int at[MB];                                            // a pair's position and the last key in front of its window; row * n_head + head, -1: nothing to write
+        alignas(16) float c[MB]; float mu[MB], alpha[4][MB], top[2][4][8 * NC], l[2][4][8 * NC];   // factor of a pair's scores, reference; rescaling by tile; largest logarithms by group, warp
+        int2 see[MB]; int at[MB];   // a pair's position and the last key in front of its window; row * n_head + head, -1: nothing to write
+        int moved[4][2];            // by tile and group: the tile's number + 1 where references move, and alpha holds
     };
     static_assert(sizeof(Shared) <= Geo::X_BYTES, "");
     Shared& x = *reinterpret_cast<Shared*>(sm + Geo::OFF_X);
@@ -100,6 +102,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
         mbar_init(smem_u32(&x.p_full), 8); mbar_init(smem_u32(&x.pv_done), 1); mbar_init(smem_u32(&x.o_empty), Geo::ACC); mbar_init(smem_u32(&x.fin), 1);
         fence_barrier_init();
     }
+    if (tid < 8) x.moved[tid >> 1][tid & 1] = 0;
     if (warp == Geo::W_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_ptr)), "n"(Geo::TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -137,6 +140,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
         if (lane == 0) {
             const int pos = live ? max(-1, sq.len - sq.T + t) : -1;
             x.c[i] = a.scale2 * __uint_as_float((uint32_t)(127 - e) << 23);
+            x.mu[i] = MU_NONE;
             x.see[i] = make_int2(pos, a.window ? pos - a.window : -1);
             x.at[i] = pos >= 0 ? (sq.row0 + t) * a.n_head + kh * a.G + p - t * a.G : -1;
         }
@@ -153,7 +157,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
         const int grp = warp >> 2, qt = warp & 3, key = qt * 32 + lane;
         const uint32_t tlane = tmem + ((uint32_t)qt << 21);
         uint8_t* const pw = sm + Geo::OFF_P + key * 128;
-        float l[NC][8], mu = -1e30f;   // mu of pair 8 (2 (lane / 8) + grp) + lane % 8
+        float l[NC][8];
 #pragma unroll
         for (int i = 0; i < NC; ++i)
 #pragma unroll
@@ -170,7 +174,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
         scales(t_first, ks, vs);
         int t1 = first_from(t_first + 1);
         page = t1 < t_end ? page_of(t1 * TK + key) : 0xffffffffu;
-        int n = 0;
+        int n = 0, ph = 0;   // tile, phase of the group's barrier
         for (int t = t_first; t < t_end && ok; t = t1, ++n) {
             float ks1, vs1;
             t1 = first_from(t + 1);
@@ -182,44 +186,90 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
             if (!ok) break;
             tc_fence_after();
             float s[NC][8];
+            {
+                float b[NC][8];
 #pragma unroll
-            for (int i = 0; i < NC; ++i) { const int c8 = 8 * (2 * i + grp); if (c8 < np) ld_sum8(s[i], sb + c8, sb + MB + c8); }
-            tc_fence_before();
-            warp_arrive(smem_u32(&x.s_empty[n & 1]), lane);
+                for (int i = 0; i < NC; ++i) { const int c8 = 8 * (2 * i + grp); if (c8 < np) { ld8(s[i], sb + c8); ld8(b[i], sb + MB + c8); } }
+                ld_wait(s, b);
+                tc_fence_before();
+                warp_arrive(smem_u32(&x.s_empty[n & 1]), lane);
+#pragma unroll
+                for (int i = 0; i < NC; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[i][e] = s[i][e] + b[i][e];
+            }
             const float lv = lg2(fmaxf(vs, 8.0779357e-28f));   // 2^-90: the weights' sum cannot overflow
             const int j = t * TK + key;
             const bool whole = t * TK + TK - 1 <= all_hi && (t * TK > all_lo || t * TK + TK <= sink);
+            uint32_t hide = 0;   // a bit per pair
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < NC; ++i)
+                    if (8 * (2 * i + grp) < np) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) { const int2 v = x.see[8 * (2 * i + grp) + e]; if (!(j <= v.x && (j > v.y || j < sink))) hide |= 1u << (8 * i + e); }
+                    }
+            }
+            // distance of a logarithm from its reference; computed again for the weight, which costs less than 24 registers
+            auto distance4 = [&](float (&d)[4], int i, int e) {
+                const int c8 = 8 * (2 * i + grp);
+                const float4 c = *reinterpret_cast<const float4*>(&x.c[c8 + e]), m = *reinterpret_cast<const float4*>(&x.mu[c8 + e]);
+                d[0] = fmaf(s[i][e], ks * c.x, -m.x); d[1] = fmaf(s[i][e + 1], ks * c.y, -m.y); d[2] = fmaf(s[i][e + 2], ks * c.z, -m.z); d[3] = fmaf(s[i][e + 3], ks * c.w, -m.w);
+                if (hide) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) if (hide >> (8 * i + e + u) & 1) d[u] = -INFINITY;
+                }
+            };
             float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < NC; ++i) {
-                const int c8 = 8 * (2 * i + grp);
-                if (c8 < np) {
+            for (int i = 0; i < NC; ++i)
+                if (8 * (2 * i + grp) < np) {
 #pragma unroll
-                    for (int e = 0; e < 8; e += 4) {
-                        const float4 c = *reinterpret_cast<const float4*>(&x.c[c8 + e]);
-                        s[i][e] = s[i][e] * (ks * c.x); s[i][e + 1] = s[i][e + 1] * (ks * c.y); s[i][e + 2] = s[i][e + 2] * (ks * c.z); s[i][e + 3] = s[i][e + 3] * (ks * c.w);
-                    }
-                    if (!whole) {
+                    for (int e = 0; e < 8; e += 4) { float d[4]; distance4(d, i, e); top = fmaxf(top, fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3]))); }
+                }
+            if (__any_sync(0xffffffffu, top + lv > MU_LIMIT) && lane == 0) x.moved[n & 3][grp] = n + 1;
+            warp_arrive(smem_u32(&x.red[grp]), lane);
+            ok = warp_wait(smem_u32(&x.red[grp]), ph & 1, a.err);
+            ++ph;
+            if (!ok) break;
+            if (x.moved[n & 3][grp] == n + 1) {   // rare behind the first tiles. A pair moves by its own keys alone
+                float mine = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NC; ++i) {
+                    const int c8 = 8 * (2 * i + grp);
+                    if (c8 < np) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const int2 v = x.see[c8 + e];
-                            if (!(j <= v.x && (j > v.y || j < sink))) s[i][e] = -INFINITY;
+                            const float m = warp_max(hide >> (8 * i + e) & 1 ? -INFINITY : s[i][e] * (ks * x.c[c8 + e]) + lv);
+                            if (lane == 8 * i + e) mine = m;
                         }
                     }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) { const float m = warp_max(s[i][e] + lv); if (lane == 8 * i + e) top = m; }
                 }
-            }
-            if (lane < 8 * NC) x.top[n & 1][grp][qt][lane] = top;
-            warp_arrive(smem_u32(&x.red[grp]), lane);
-            ok = warp_wait(smem_u32(&x.red[grp]), n & 1, a.err);
-            if (!ok) break;
-            float al = 1.f;
-            if (lane < 8 * NC) {
-                const float m = fmaxf(fmaxf(x.top[n & 1][grp][0][lane], x.top[n & 1][grp][1][lane]), fmaxf(x.top[n & 1][grp][2][lane], x.top[n & 1][grp][3][lane]));
-                const float next = fmaxf(mu, ceilf(m) - 14.f);
-                al = pow2i(mu - next); mu = next;
-                if (qt == 0) x.alpha[n & 1][8 * (2 * (lane >> 3) + grp) + (lane & 7)] = al;
+                if (lane < 8 * NC) x.top[grp][qt][lane] = mine;
+                warp_arrive(smem_u32(&x.red[grp]), lane);
+                ok = warp_wait(smem_u32(&x.red[grp]), ph & 1, a.err);
+                ++ph;
+                if (!ok) break;
+                const int pair = 8 * (2 * (lane >> 3) + grp) + (lane & 7);
+                float al = 1.f, next = MU_NONE;
+                if (lane < 8 * NC) {
+                    const float m = fmaxf(fmaxf(x.top[grp][0][lane], x.top[grp][1][lane]), fmaxf(x.top[grp][2][lane], x.top[grp][3][lane]));
+                    next = x.mu[pair];
+                    if (m - next > MU_LIMIT) { al = pow2i(next - (ceilf(m) - MU_TOP)); next = ceilf(m) - MU_TOP; }
+                }
+#pragma unroll
+                for (int i = 0; i < NC; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) l[i][e] = l[i][e] * __shfl_sync(0xffffffffu, al, 8 * i + e);
+                warp_arrive(smem_u32(&x.red[grp]), lane);   // everybody has read the references
+                ok = warp_wait(smem_u32(&x.red[grp]), ph & 1, a.err);
+                ++ph;
+                if (!ok) break;
+                if (qt == 0 && lane < 8 * NC) { x.mu[pair] = next; x.alpha[n & 3][pair] = al; }
+                warp_arrive(smem_u32(&x.red[grp]), lane);
+                ok = warp_wait(smem_u32(&x.red[grp]), ph & 1, a.err);
+                ++ph;
+                if (!ok) break;
             }
             ok = warp_wait(smem_u32(&x.pv_done), (n & 1) ^ 1, a.err);   // the weights of the tile before are read
             if (!ok) break;
@@ -229,18 +279,25 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
                 if (c8 < np) {
                     uint32_t h[4], r[4];
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        float y[2];
+                    for (int e = 0; e < 8; e += 4) {
+                        float d[4], y[4];
+                        distance4(d, i, e);
 #pragma unroll
-                        for (int d = 0; d < 2; ++d) {
-                            const float m = __shfl_sync(0xffffffffu, mu, 8 * i + e + d), f = __shfl_sync(0xffffffffu, al, 8 * i + e + d);
-                            const float p = ex2(s[i][e + d] - m);
-                            l[i][e + d] = fmaf(l[i][e + d], f, p);
-                            y[d] = s[i][e + d] == -INFINITY ? 0.f : p * vs;   // a masked key's scale may be anything
+                        for (int u = 0; u < 4; ++u) {
+                            const float p = ex2(d[u]);
+                            l[i][e + u] = l[i][e + u] + p;
+                            y[u] = p * vs;
                         }
-                        const __half2 hh = __floats2half2_rn(y[0], y[1]);
-                        const float2 f = __half22float2(hh);
-                        h[e / 2] = h2_bits(hh); r[e / 2] = h2_bits(__floats2half2_rn(y[0] - f.x, y[1] - f.y));
+                        if (hide) {   // a masked key's scale may be anything
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) if (hide >> (8 * i + e + u) & 1) y[u] = 0.f;
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; u += 2) {
+                            const __half2 hh = __floats2half2_rn(y[u], y[u + 1]);
+                            const float2 f = __half22float2(hh);
+                            h[(e + u) / 2] = h2_bits(hh); r[(e + u) / 2] = h2_bits(__floats2half2_rn(y[u] - f.x, y[u + 1] - f.y));
+                        }
                     }
                     const int ch = c8 / 8, cr = MB / 8 + ch;   // eights of columns; 64 columns of all keys lie one behind the other
                     *reinterpret_cast<uint4*>(pw + (ch >> 3) * (TK * 128) + (((ch & 7) ^ (key & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
@@ -264,11 +321,11 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
             }
         if (lane < 8 * NC) x.l[grp][qt][lane] = mine;
         warp_arrive(smem_u32(&x.red[grp]), lane);
-        if (ok) ok = warp_wait(smem_u32(&x.red[grp]), n & 1, a.err);
+        if (ok) ok = warp_wait(smem_u32(&x.red[grp]), ph & 1, a.err);
         if (ok && qt == 0 && lane < 8 * NC) {
             const int pair = 8 * (2 * (lane >> 3) + grp) + (lane & 7);
             if (pair < np && x.at[pair] >= 0)
-                a.pml[(size_t)x.at[pair] * (a.ns + a.nwin) + blockIdx.x] = make_float2(mu, ((x.l[grp][0][lane] + x.l[grp][1][lane]) + x.l[grp][2][lane]) + x.l[grp][3][lane]);
+                a.pml[(size_t)x.at[pair] * (a.ns + a.nwin) + blockIdx.x] = make_float2(x.mu[pair], ((x.l[grp][0][lane] + x.l[grp][1][lane]) + x.l[grp][2][lane]) + x.l[grp][3][lane]);
         }
     } else if (warp < Geo::W_MMA) {   // ---- sums
         const int b = (warp - Geo::W_ACC) >> 2, qt = warp & 3, dim = 128 * b + 32 * qt + lane;
@@ -281,16 +338,24 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
             ok = warp_wait(smem_u32(&x.pv_done), n & 1, a.err);
             if (!ok) break;
             tc_fence_after();
+            const int moved[2] = {x.moved[n & 3][0], x.moved[n & 3][1]};
 #pragma unroll
-            for (int c = 0; c < MB / 8; ++c) {
-                if (8 * c < np) {
-                    float f[8];
-                    ld_sum8(f, ob + 8 * c, ob + MB + 8 * c);
-                    const float4 u = *reinterpret_cast<const float4*>(&x.alpha[n & 1][8 * c]), v = *reinterpret_cast<const float4*>(&x.alpha[n & 1][8 * c + 4]);
-                    float* o = O + 8 * c;
-                    o[0] = fmaf(o[0], u.x, f[0]); o[1] = fmaf(o[1], u.y, f[1]); o[2] = fmaf(o[2], u.z, f[2]); o[3] = fmaf(o[3], u.w, f[3]);
-                    o[4] = fmaf(o[4], v.x, f[4]); o[5] = fmaf(o[5], v.y, f[5]); o[6] = fmaf(o[6], v.z, f[6]); o[7] = fmaf(o[7], v.w, f[7]);
-                }
+            for (int c0 = 0; c0 < MB / 8; c0 += 2) {
+                float f[2][8], g[2][8];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) if (8 * (c0 + c) < np) { ld8(f[c], ob + 8 * (c0 + c)); ld8(g[c], ob + MB + 8 * (c0 + c)); }
+                ld_wait(f, g);
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    if (8 * (c0 + c) < np) {
+                        float* o = O + 8 * (c0 + c);
+                        if (moved[c] == n + 1) {
+                            const float4 u = *reinterpret_cast<const float4*>(&x.alpha[n & 3][8 * (c0 + c)]), v = *reinterpret_cast<const float4*>(&x.alpha[n & 3][8 * (c0 + c) + 4]);
+                            o[0] = o[0] * u.x; o[1] = o[1] * u.y; o[2] = o[2] * u.z; o[3] = o[3] * u.w; o[4] = o[4] * v.x; o[5] = o[5] * v.y; o[6] = o[6] * v.z; o[7] = o[7] * v.w;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[e] = o[e] + (f[c][e] + g[c][e]);
+                    }
             }
             tc_fence_before();
             warp_arrive(smem_u32(&x.o_empty), lane);

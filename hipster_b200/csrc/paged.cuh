@@ -55,6 +55,9 @@ constexpr int PAGED_DECODE_ROWS = 16, PAGED_TC_PAIRS = 48;
 size_t attn_paged_tc_bytes(const PagedPool& pool, const PagedBatch& b);
 int attn_paged_tc(PagedArgs& a, dim3 grid, cudaStream_t s);
 
+// The reference mu of a pair's weights is whole. It moves when a logarithm passes mu + MU_LIMIT, to MU_TOP below the largest of the keys at hand: weights times scales stay
+// below 2^15 (f16 ends at 65504), the largest is above 2^7 (f16 ends in steps of 2^-24), and almost all keys take no maximum at all.
+constexpr float MU_TOP = 8.f, MU_LIMIT = 15.f, MU_NONE = -1e30f;
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float pow2i(float d) { return d < -126.f ? 0.f : __uint_as_float((uint32_t)((int)d + 127) << 23); }   // 2^d, d whole and <= 0

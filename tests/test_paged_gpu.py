@@ -260,10 +260,10 @@ def attn64(st, q, scale, window, n_sink, gate):
     by at most 2 ds sum p |v|. The weights (2^-22 of ex2, 2^-22 of their rests, two roundings) and the sums (a step per 32 keys and per split of 256,
     counted on both sides of the quotient), gate and quotient (8 roundings) come on top.
 
-    Weights far below the largest: w_j = p_j times the scale of v goes in as two f16 on a common scale on which the largest is at least 2^13 (the reference is whole
-    and at most 14 + 1 below the largest logarithm, and it only grows: what was added earlier is scaled down with its error), and f16 ends in steps
-    of 2^-24. So each weight may be off by half such a step, 2^-25 / 2^13 = 2^-38 of the largest, and an output by 2^-38 max_j w_j sum_j |code_jd|: this is
-    what is left where the code of a key that takes nearly all of the weight is zero."""
+    Weights far below the largest: w_j = p_j times the scale of v goes in as two f16 each on a common scale on which the largest is above 2^7 (the reference is whole and
+    moves to 8 below the largest logarithm; it only grows, and what was added earlier is scaled down with its error), and f16 ends in steps of 2^-24. So each weight
+    may be off by half such a step, 2^-25 / 2^7 = 2^-32 of the largest, and an output by 2^-32 max_j w_j sum_j |code_jd|: this is what is left where the
+    code of a key that takes nearly all of the weight is zero."""
     H, n_kv, D = q.shape[1], st.pool.n_kv, st.D
     G = H // n_kv
     out, tol = torch.zeros((st.R, H, D), dtype=torch.float64, device="cuda"), torch.zeros((st.R, H, D), dtype=torch.float64, device="cuda")
@@ -284,7 +284,7 @@ def attn64(st, q, scale, window, n_sink, gate):
             mag = torch.einsum("hj,hjd->hd", p, v.abs())
             steps = (2 * (D / 16 + 8) * A[:, None] + 2 * (len(j) / 32 + len(j) / 256 + 8) + 12)
             vs = st.scales(s)[:, j].repeat_interleave(G, 0)
-            small = 2.0 ** -38 * (p * vs).amax(-1)[:, None] * (v.abs() / vs.clamp(min=1e-300)[..., None]).sum(1)
+            small = 2.0 ** -32 * (p * vs).amax(-1)[:, None] * (v.abs() / vs.clamp(min=1e-300)[..., None]).sum(1)
             tol[r0 + t] = steps * 2.0 ** -23 * mag + small
         r0 += T
     if gate is not None:
