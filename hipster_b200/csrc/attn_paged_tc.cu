@@ -10,10 +10,11 @@
 // kv head, each twice: column i its values, column MB + i what is left of them. So a thread that reads a row of the accumulator has value and rest of every pair
 // at hand, needs one scale of k and of v, and adds up its own keys' weights without another thread until the end. A CTA holds a block of 48 pairs
 // and the keys of one split, in tiles of 128 keys:
-//   copies (one warp): pictures of k and v into shared memory
-//   products (one thread): S[128 keys][pairs] = K q^T, and O[128 dims][pairs] = V^T w, one tile of scores ahead
+//   copies (a warp for k, one for v: in one warp a copy of k waits behind the outputs that a copy of v waits for, 6600 clocks per tile): pictures into shared memory
+//   products (one thread; its warp does nothing else, since issuing them takes as long as they take): S[128 keys][pairs] = K q^T, and O[128 dims][pairs] = V^T w, one tile
+//     of scores ahead
 //   weights (two groups of four warps, a thread per key, a group takes every second set of eight pairs): S -> w in shared memory (N-major operand)
-//   sums (a thread per dim): O of the tile into registers
+//   sums (four warps per 128 dims, a thread per dim): O of the tile into registers
 // Bound by shared memory: a tile's pictures go in (1024 clocks at 256 dims) and, as operands with q and the weights, out again (1800), against 1536 clocks of products.
 #include "paged.cuh"
 #include "tc.cuh"
@@ -27,12 +28,12 @@ constexpr int TK = 128;   // keys of a tile
 // Shared memory of a CTA, operands on 1024-byte boundaries. 64 dims of a key (or of a pair of q, 64 columns of the weights of a key) are a row of 128 bytes.
 template <int D, int MB> struct PagedGeo {
     static constexpr int N = 2 * MB, NB = D > 128 ? 2 : 1, ACC = 4 * NB;                 // columns, blocks of 128 dims, warps that sum
-    static constexpr int WARPS = 8 + ACC + 2, W_ACC = 8, W_MMA = W_ACC + ACC;            // the last one copies
+    static constexpr int W_ACC = 8, W_MMA = W_ACC + ACC, W_K = W_MMA + 1, W_V = W_K + 1, WARPS = W_V + 1;
     static constexpr int PICTURE = TK * D * 2;                                            // bytes of a tile of k or v
     static constexpr int OFF_Q = 0, OFF_K = N * D * 2, OFF_V = OFF_K + PICTURE, OFF_P = OFF_V + PICTURE, OFF_X = OFF_P + (N + 63) / 64 * TK * 128;
     static constexpr int X_BYTES = 4096, SMEM = OFF_X + X_BYTES + 1024;                   // 1024 for the alignment
     static constexpr int TMEM = 512;
-    static_assert(OFF_K % 1024 == 0 && NB * N + 2 * N <= TMEM && SMEM <= 226 * 1024, "");
+    static_assert(OFF_K % 1024 == 0 && NB * N + 2 * N + MB <= TMEM && SMEM <= 226 * 1024, "");
 };
 
 __device__ __forceinline__ float warp_max(float x) { float y; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x)); return y; }
@@ -44,18 +45,21 @@ __device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t next) {
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int add) {   // D = A * B (+ D)
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
-// eight columns from col0 and from col1 of this warp's 32 lanes: values and rests. They are there behind ld_wait
+// eight columns of this warp's 32 lanes; there behind ld_wait
 __device__ __forceinline__ void ld8(float (&a)[8], uint32_t col) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]), "=f"(a[4]), "=f"(a[5]), "=f"(a[6]), "=f"(a[7]) : "r"(col) : "memory");
 }
-template <int C> __device__ __forceinline__ void ld_wait(float (&a)[C][8], float (&b)[C][8]) {   // the empty statements order the use of the registers behind the wait
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { asm volatile("" : "+f"(a[c][i])); asm volatile("" : "+f"(b[c][i])); }
+__device__ __forceinline__ void st8(uint32_t col, const float (&a)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\ntcgen05.wait::st.sync.aligned;"
+                 :: "r"(col), "f"(a[0]), "f"(a[1]), "f"(a[2]), "f"(a[3]), "f"(a[4]), "f"(a[5]), "f"(a[6]), "f"(a[7]) : "memory");
 }
+__device__ __forceinline__ void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ld_there(float (&a)[8]) {   // orders the use of the registers behind the wait
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+f"(a[i]));
+}
+__device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory"); }
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) { return __all_sync(0xffffffffu, tc_wait(bar, parity, err)); }
 __device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) { __syncwarp(); if (lane == 0) mbar_arrive(bar); }
 
@@ -69,8 +73,8 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
     uint8_t* const sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     struct Shared {
-        uint64_t k_full, k_empty, v_full, s_full[2], s_empty[2], p_full, pv_done, o_empty, red[2], fin;
-        alignas(16) float c[MB]; float mu[MB], alpha[4][MB], top[2][4][8 * NC], l[2][4][8 * NC];   // factor of a pair's scores, reference; rescaling by tile; largest logarithms by group, warp
+        uint64_t k_full, k_empty, v_full, s_full[2], s_empty[2], p_full, pv_done, o_empty, fin;
+        alignas(16) float c[MB]; float mu[8][8 * NC], alpha[4][MB], top[2][4][8 * NC], l[2][4][8 * NC];   // factor of a pair's scores, references (a copy of each warp's own); rescaling by tile; largest logarithms by group, warp
         int2 see[MB]; int at[MB];   // a pair's position and the last key in front of its window; row * n_head + head, -1: nothing to write
         int moved[4][2];            // by tile and group: the tile's number + 1 where references move, and alpha holds
     };
@@ -98,11 +102,12 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
 
     if (tid == 0) {
         mbar_init(smem_u32(&x.k_full), 1); mbar_init(smem_u32(&x.k_empty), 1); mbar_init(smem_u32(&x.v_full), 1);
-        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); mbar_init(smem_u32(&x.s_empty[i]), 8); mbar_init(smem_u32(&x.red[i]), 4); }
+        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); mbar_init(smem_u32(&x.s_empty[i]), 8); }
         mbar_init(smem_u32(&x.p_full), 8); mbar_init(smem_u32(&x.pv_done), 1); mbar_init(smem_u32(&x.o_empty), Geo::ACC); mbar_init(smem_u32(&x.fin), 1);
         fence_barrier_init();
     }
     if (tid < 8) x.moved[tid >> 1][tid & 1] = 0;
+    if (warp < 8 && lane < 8 * NC) x.mu[warp][lane] = MU_NONE;
     if (warp == Geo::W_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_ptr)), "n"(Geo::TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -140,7 +145,6 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
         if (lane == 0) {
             const int pos = live ? max(-1, sq.len - sq.T + t) : -1;
             x.c[i] = a.scale2 * __uint_as_float((uint32_t)(127 - e) << 23);
-            x.mu[i] = MU_NONE;
             x.see[i] = make_int2(pos, a.window ? pos - a.window : -1);
             x.at[i] = pos >= 0 ? (sq.row0 + t) * a.n_head + kh * a.G + p - t * a.G : -1;
         }
@@ -151,17 +155,19 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
     tc_fence_after();
     const uint32_t tmem = tmem_ptr;
     bool ok = true;
-    int sent[2] = {0, 0};   // pictures under way (copies)
 
     if (warp < 8) {   // ---- weights
-        const int grp = warp >> 2, qt = warp & 3, key = qt * 32 + lane;
-        const uint32_t tlane = tmem + ((uint32_t)qt << 21);
+        // The loops over the sets of eight pairs are not unrolled, and the sums of the weights wait in accumulator memory: with everything in registers and unrolled the
+        // roles' loops did not fit the instruction cache (some 10 clocks per instruction; 8400 clocks per tile). A wait that gave up does not end the loop, which is as long for
+        // all warps of a group: their barrier is not bounded, so all of them have to come to it.
+        const int grp = warp >> 2, qt = warp & 3, key = qt * 32 + lane, nc = (np - 8 * grp + 15) / 16;   // sets of this group: pairs 8 (2 i + grp) ..
+        const uint32_t tlane = tmem + ((uint32_t)qt << 21), lcol = tlane + 2 * N + NB * N + 8 * grp;
         uint8_t* const pw = sm + Geo::OFF_P + key * 128;
-        float l[NC][8];
-#pragma unroll
-        for (int i = 0; i < NC; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) l[i][e] = 0.f;
+        {
+            const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int i = 0; i < nc; ++i) st8(lcol + 16 * i, zero);
+        }
         // positions between which a tile is visible to all pairs
         const int all_hi = pos_lo, all_lo = a.window ? pos_hi - a.window : -1;
         // scales of this thread's key, a tile ahead, and its page, two tiles ahead
@@ -174,158 +180,133 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
         scales(t_first, ks, vs);
         int t1 = first_from(t_first + 1);
         page = t1 < t_end ? page_of(t1 * TK + key) : 0xffffffffu;
-        int n = 0, ph = 0;   // tile, phase of the group's barrier
-        for (int t = t_first; t < t_end && ok; t = t1, ++n) {
+        int n = 0;
+        for (int t = t_first; t < t_end; t = t1, ++n) {
             float ks1, vs1;
             t1 = first_from(t + 1);
             scales(t1, ks1, vs1);
             const int t2 = first_from(t1 + 1);
             page = t2 < t_end ? page_of(t2 * TK + key) : 0xffffffffu;
-            const uint32_t sb = tlane + (n & 1) * N;
-            ok = warp_wait(smem_u32(&x.s_full[n & 1]), (n >> 1) & 1, a.err);
-            if (!ok) break;
+            const uint32_t sb = tlane + (n & 1) * N + 8 * grp;
+            ok = ok && warp_wait(smem_u32(&x.s_full[n & 1]), (n >> 1) & 1, a.err);
             tc_fence_after();
-            float s[NC][8];
-            {
-                float b[NC][8];
-#pragma unroll
-                for (int i = 0; i < NC; ++i) { const int c8 = 8 * (2 * i + grp); if (c8 < np) { ld8(s[i], sb + c8); ld8(b[i], sb + MB + c8); } }
-                ld_wait(s, b);
-                tc_fence_before();
-                warp_arrive(smem_u32(&x.s_empty[n & 1]), lane);
-#pragma unroll
-                for (int i = 0; i < NC; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s[i][e] = s[i][e] + b[i][e];
-            }
             const float lv = lg2(fmaxf(vs, 8.0779357e-28f));   // 2^-90: the weights' sum cannot overflow
             const int j = t * TK + key;
             const bool whole = t * TK + TK - 1 <= all_hi && (t * TK > all_lo || t * TK + TK <= sink);
             uint32_t hide = 0;   // a bit per pair
             if (!whole) {
+#pragma unroll 1
+                for (int i = 0; i < nc; ++i)
 #pragma unroll
-                for (int i = 0; i < NC; ++i)
-                    if (8 * (2 * i + grp) < np) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) { const int2 v = x.see[8 * (2 * i + grp) + e]; if (!(j <= v.x && (j > v.y || j < sink))) hide |= 1u << (8 * i + e); }
-                    }
+                    for (int e = 0; e < 8; ++e) { const int2 v = x.see[8 * (2 * i + grp) + e]; if (!(j <= v.x && (j > v.y || j < sink))) hide |= 1u << (8 * i + e); }
             }
-            // distance of a logarithm from its reference; computed again for the weight, which costs less than 24 registers
-            auto distance4 = [&](float (&d)[4], int i, int e) {
-                const int c8 = 8 * (2 * i + grp);
-                const float4 c = *reinterpret_cast<const float4*>(&x.c[c8 + e]), m = *reinterpret_cast<const float4*>(&x.mu[c8 + e]);
-                d[0] = fmaf(s[i][e], ks * c.x, -m.x); d[1] = fmaf(s[i][e + 1], ks * c.y, -m.y); d[2] = fmaf(s[i][e + 2], ks * c.z, -m.z); d[3] = fmaf(s[i][e + 3], ks * c.w, -m.w);
+            auto scores = [&](float (&s)[8], int i) {
+                float r[8];
+                ld8(s, sb + 16 * i); ld8(r, sb + MB + 16 * i);
+                ld_wait(); ld_there(s); ld_there(r);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[e] = s[e] + r[e];
+            };
+            // distances of the logarithms from their references
+            auto distances = [&](float (&d)[8], int i) {
+                scores(d, i);
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    const float4 c = *reinterpret_cast<const float4*>(&x.c[8 * (2 * i + grp) + e]), m = *reinterpret_cast<const float4*>(&x.mu[warp][8 * i + e]);
+                    d[e] = fmaf(d[e], ks * c.x, -m.x); d[e + 1] = fmaf(d[e + 1], ks * c.y, -m.y); d[e + 2] = fmaf(d[e + 2], ks * c.z, -m.z); d[e + 3] = fmaf(d[e + 3], ks * c.w, -m.w);
+                }
                 if (hide) {
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) if (hide >> (8 * i + e + u) & 1) d[u] = -INFINITY;
+                    for (int e = 0; e < 8; ++e) if (hide >> (8 * i + e) & 1) d[e] = -INFINITY;
                 }
             };
             float top = -INFINITY;
+#pragma unroll 1
+            for (int i = 0; i < nc; ++i) {
+                float d[8];
+                distances(d, i);
 #pragma unroll
-            for (int i = 0; i < NC; ++i)
-                if (8 * (2 * i + grp) < np) {
-#pragma unroll
-                    for (int e = 0; e < 8; e += 4) { float d[4]; distance4(d, i, e); top = fmaxf(top, fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3]))); }
-                }
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, d[e]);
+            }
             if (__any_sync(0xffffffffu, top + lv > MU_LIMIT) && lane == 0) x.moved[n & 3][grp] = n + 1;
-            warp_arrive(smem_u32(&x.red[grp]), lane);
-            ok = warp_wait(smem_u32(&x.red[grp]), ph & 1, a.err);
-            ++ph;
-            if (!ok) break;
+            group_sync(grp);
             if (x.moved[n & 3][grp] == n + 1) {   // rare behind the first tiles. A pair moves by its own keys alone
                 float mine = -INFINITY;
+#pragma unroll 1
+                for (int i = 0; i < nc; ++i) {
+                    float d[8];
+                    scores(d, i);
 #pragma unroll
-                for (int i = 0; i < NC; ++i) {
-                    const int c8 = 8 * (2 * i + grp);
-                    if (c8 < np) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float m = warp_max(hide >> (8 * i + e) & 1 ? -INFINITY : s[i][e] * (ks * x.c[c8 + e]) + lv);
-                            if (lane == 8 * i + e) mine = m;
-                        }
+                    for (int e = 0; e < 8; ++e) {
+                        const float m = warp_max(hide >> (8 * i + e) & 1 ? -INFINITY : d[e] * (ks * x.c[8 * (2 * i + grp) + e]) + lv);
+                        if (lane == 8 * i + e) mine = m;
                     }
                 }
                 if (lane < 8 * NC) x.top[grp][qt][lane] = mine;
-                warp_arrive(smem_u32(&x.red[grp]), lane);
-                ok = warp_wait(smem_u32(&x.red[grp]), ph & 1, a.err);
-                ++ph;
-                if (!ok) break;
-                const int pair = 8 * (2 * (lane >> 3) + grp) + (lane & 7);
-                float al = 1.f, next = MU_NONE;
+                group_sync(grp);
+                float al = 1.f;
                 if (lane < 8 * NC) {
-                    const float m = fmaxf(fmaxf(x.top[grp][0][lane], x.top[grp][1][lane]), fmaxf(x.top[grp][2][lane], x.top[grp][3][lane]));
-                    next = x.mu[pair];
-                    if (m - next > MU_LIMIT) { al = pow2i(next - (ceilf(m) - MU_TOP)); next = ceilf(m) - MU_TOP; }
+                    const float m = fmaxf(fmaxf(x.top[grp][0][lane], x.top[grp][1][lane]), fmaxf(x.top[grp][2][lane], x.top[grp][3][lane])), mu = x.mu[warp][lane], next = ceilf(m) - MU_TOP;
+                    if (m - mu > MU_LIMIT) { al = pow2i(mu - next); x.mu[warp][lane] = next; }
+                    if (qt == 0) x.alpha[n & 3][8 * (2 * (lane >> 3) + grp) + (lane & 7)] = al;
                 }
+#pragma unroll 1
+                for (int i = 0; i < nc; ++i) {
+                    float l[8];
+                    ld8(l, lcol + 16 * i); ld_wait(); ld_there(l);
 #pragma unroll
-                for (int i = 0; i < NC; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) l[i][e] = l[i][e] * __shfl_sync(0xffffffffu, al, 8 * i + e);
-                warp_arrive(smem_u32(&x.red[grp]), lane);   // everybody has read the references
-                ok = warp_wait(smem_u32(&x.red[grp]), ph & 1, a.err);
-                ++ph;
-                if (!ok) break;
-                if (qt == 0 && lane < 8 * NC) { x.mu[pair] = next; x.alpha[n & 3][pair] = al; }
-                warp_arrive(smem_u32(&x.red[grp]), lane);
-                ok = warp_wait(smem_u32(&x.red[grp]), ph & 1, a.err);
-                ++ph;
-                if (!ok) break;
-            }
-            ok = warp_wait(smem_u32(&x.pv_done), (n & 1) ^ 1, a.err);   // the weights of the tile before are read
-            if (!ok) break;
-#pragma unroll
-            for (int i = 0; i < NC; ++i) {
-                const int c8 = 8 * (2 * i + grp);
-                if (c8 < np) {
-                    uint32_t h[4], r[4];
-#pragma unroll
-                    for (int e = 0; e < 8; e += 4) {
-                        float d[4], y[4];
-                        distance4(d, i, e);
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const float p = ex2(d[u]);
-                            l[i][e + u] = l[i][e + u] + p;
-                            y[u] = p * vs;
-                        }
-                        if (hide) {   // a masked key's scale may be anything
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) if (hide >> (8 * i + e + u) & 1) y[u] = 0.f;
-                        }
-#pragma unroll
-                        for (int u = 0; u < 4; u += 2) {
-                            const __half2 hh = __floats2half2_rn(y[u], y[u + 1]);
-                            const float2 f = __half22float2(hh);
-                            h[(e + u) / 2] = h2_bits(hh); r[(e + u) / 2] = h2_bits(__floats2half2_rn(y[u] - f.x, y[u + 1] - f.y));
-                        }
-                    }
-                    const int ch = c8 / 8, cr = MB / 8 + ch;   // eights of columns; 64 columns of all keys lie one behind the other
-                    *reinterpret_cast<uint4*>(pw + (ch >> 3) * (TK * 128) + (((ch & 7) ^ (key & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(pw + (cr >> 3) * (TK * 128) + (((cr & 7) ^ (key & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+                    for (int e = 0; e < 8; ++e) l[e] = l[e] * __shfl_sync(0xffffffffu, al, 8 * i + e);
+                    st8(lcol + 16 * i, l);
                 }
+                __syncwarp();
             }
+            ok = ok && warp_wait(smem_u32(&x.pv_done), (n & 1) ^ 1, a.err);   // the weights of the tile before are read
+#pragma unroll 1
+            for (int i = 0; i < nc; ++i) {
+                float d[8], l[8];
+                ld8(l, lcol + 16 * i);
+                distances(d, i);
+                ld_there(l);
+                uint32_t h[4], r[4];
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float p0 = ex2(d[e]), p1 = ex2(d[e + 1]);
+                    l[e] = l[e] + p0; l[e + 1] = l[e + 1] + p1;
+                    float y0 = p0 * vs, y1 = p1 * vs;
+                    if (hide) { y0 = hide >> (8 * i + e) & 1 ? 0.f : y0; y1 = hide >> (8 * i + e + 1) & 1 ? 0.f : y1; }   // a masked key's scale may be anything
+                    const __half2 hh = __floats2half2_rn(y0, y1);
+                    const float2 f = __half22float2(hh);
+                    h[e / 2] = h2_bits(hh); r[e / 2] = h2_bits(__floats2half2_rn(y0 - f.x, y1 - f.y));
+                }
+                st8(lcol + 16 * i, l);
+                const int ch = 2 * i + grp, cr = MB / 8 + ch;   // eights of columns; 64 columns of all keys lie one behind the other
+                *reinterpret_cast<uint4*>(pw + (ch >> 3) * (TK * 128) + (((ch & 7) ^ (key & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4*>(pw + (cr >> 3) * (TK * 128) + (((cr & 7) ^ (key & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+            }
+            tc_fence_before();
             fence_proxy_async();
-            warp_arrive(smem_u32(&x.p_full), lane);
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(smem_u32(&x.s_empty[n & 1])); mbar_arrive(smem_u32(&x.p_full)); }
             ks = ks1; vs = vs1;
         }
         // weights' sums: the 32 keys of a warp in a tree, then the warps in order
-        float mine = 0.f;
-#pragma unroll
-        for (int i = 0; i < NC; ++i)
+#pragma unroll 1
+        for (int i = 0; i < nc; ++i) {
+            float l[8];
+            ld8(l, lcol + 16 * i); ld_wait(); ld_there(l);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                float v = l[i][e];
+                float v = l[e];
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) v = v + __shfl_xor_sync(0xffffffffu, v, off);
-                if (lane == 8 * i + e) mine = v;
+                if (lane == 0) x.l[grp][qt][8 * i + e] = v;
             }
-        if (lane < 8 * NC) x.l[grp][qt][lane] = mine;
-        warp_arrive(smem_u32(&x.red[grp]), lane);
-        if (ok) ok = warp_wait(smem_u32(&x.red[grp]), ph & 1, a.err);
+        }
+        group_sync(grp);
         if (ok && qt == 0 && lane < 8 * NC) {
             const int pair = 8 * (2 * (lane >> 3) + grp) + (lane & 7);
             if (pair < np && x.at[pair] >= 0)
-                a.pml[(size_t)x.at[pair] * (a.ns + a.nwin) + blockIdx.x] = make_float2(x.mu[pair], ((x.l[grp][0][lane] + x.l[grp][1][lane]) + x.l[grp][2][lane]) + x.l[grp][3][lane]);
+                a.pml[(size_t)x.at[pair] * (a.ns + a.nwin) + blockIdx.x] = make_float2(x.mu[warp][lane], ((x.l[grp][0][lane] + x.l[grp][1][lane]) + x.l[grp][2][lane]) + x.l[grp][3][lane]);
         }
     } else if (warp < Geo::W_MMA) {   // ---- sums
         const int b = (warp - Geo::W_ACC) >> 2, qt = warp & 3, dim = 128 * b + 32 * qt + lane;
@@ -334,6 +315,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
 #pragma unroll
         for (int i = 0; i < MB; ++i) O[i] = 0.f;
         int n = 0;
+#pragma unroll 1
         for (int t = t_first; t < t_end && ok; t = first_from(t + 1), ++n) {
             ok = warp_wait(smem_u32(&x.pv_done), n & 1, a.err);
             if (!ok) break;
@@ -341,21 +323,23 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
             const int moved[2] = {x.moved[n & 3][0], x.moved[n & 3][1]};
 #pragma unroll
             for (int c0 = 0; c0 < MB / 8; c0 += 2) {
-                float f[2][8], g[2][8];
+                if (8 * c0 < np) {
+                    float f[2][8], g[2][8];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) if (8 * (c0 + c) < np) { ld8(f[c], ob + 8 * (c0 + c)); ld8(g[c], ob + MB + 8 * (c0 + c)); }
-                ld_wait(f, g);
+                    for (int c = 0; c < 2; ++c) { ld8(f[c], ob + 8 * (c0 + c)); ld8(g[c], ob + MB + 8 * (c0 + c)); }
+                    ld_wait();
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    if (8 * (c0 + c) < np) {
+                    for (int c = 0; c < 2; ++c) {
+                        ld_there(f[c]); ld_there(g[c]);
                         float* o = O + 8 * (c0 + c);
                         if (moved[c] == n + 1) {
-                            const float4 u = *reinterpret_cast<const float4*>(&x.alpha[n & 3][8 * (c0 + c)]), v = *reinterpret_cast<const float4*>(&x.alpha[n & 3][8 * (c0 + c) + 4]);
-                            o[0] = o[0] * u.x; o[1] = o[1] * u.y; o[2] = o[2] * u.z; o[3] = o[3] * u.w; o[4] = o[4] * v.x; o[5] = o[5] * v.y; o[6] = o[6] * v.z; o[7] = o[7] * v.w;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) o[e] = o[e] * x.alpha[n & 3][8 * (c0 + c) + e];
                         }
 #pragma unroll
                         for (int e = 0; e < 8; ++e) o[e] = o[e] + (f[c][e] + g[c][e]);
                     }
+                }
             }
             tc_fence_before();
             warp_arrive(smem_u32(&x.o_empty), lane);
@@ -368,60 +352,61 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
     } else if (warp == Geo::W_MMA) {   // ---- products
         const uint32_t base = smem_u32(sm);
         constexpr uint32_t ID_S = (1u << 4) | ((uint32_t)(N >> 3) << 17) | (8u << 24), ID_O = ID_S | (1u << 15) | (1u << 16);   // f32 = f16 x f16, M = 128; O: both operands M- / N-major
-        auto outputs = [&](int n) {
-            ok = ok && warp_wait(smem_u32(&x.p_full), n & 1, a.err) && warp_wait(smem_u32(&x.v_full), n & 1, a.err) && warp_wait(smem_u32(&x.o_empty), (n & 1) ^ 1, a.err);
-            if (!ok) return;
-            tc_fence_after();
-            if (tc_elect()) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int i = 0; i < TK / 16; ++i)   // 16 keys
-                        mma_f16(tmem + 2 * N + b * N, desc128(base + Geo::OFF_V + b * 2 * (TK * 128) + i * 2048, TK * 128), desc128(base + Geo::OFF_P + i * 2048, TK * 128), ID_O, i != 0);
-                tc_commit(smem_u32(&x.pv_done));
-            }
-            __syncwarp();
-        };
         int n = 0;
-        for (int t = t_first; t < t_end && ok; t = first_from(t + 1), ++n) {
-            ok = warp_wait(smem_u32(&x.k_full), n & 1, a.err) && warp_wait(smem_u32(&x.s_empty[n & 1]), ((n >> 1) & 1) ^ 1, a.err);
-            if (!ok) break;
-            tc_fence_after();
-            if (tc_elect()) {
+#pragma unroll 1
+        for (int t = t_first; ok; ++n) {   // scores of tile n, outputs of tile n - 1
+            const bool more = t < t_end;
+            if (more) {
+                ok = warp_wait(smem_u32(&x.k_full), n & 1, a.err) && warp_wait(smem_u32(&x.s_empty[n & 1]), ((n >> 1) & 1) ^ 1, a.err);
+                if (!ok) break;
+                tc_fence_after();
+                if (tc_elect()) {
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)   // 16 dims
-                    mma_f16(tmem + (n & 1) * N, desc128(base + Geo::OFF_K + (i >> 2) * (TK * 128) + (i & 3) * 32, 16), desc128(base + Geo::OFF_Q + (i >> 2) * (N * 128) + (i & 3) * 32, 16), ID_S, i != 0);
-                tc_commit(smem_u32(&x.s_full[n & 1]));
-                tc_commit(smem_u32(&x.k_empty));
+                    for (int i = 0; i < D / 16; ++i)   // 16 dims
+                        mma_f16(tmem + (n & 1) * N, desc128(base + Geo::OFF_K + (i >> 2) * (TK * 128) + (i & 3) * 32, 16), desc128(base + Geo::OFF_Q + (i >> 2) * (N * 128) + (i & 3) * 32, 16), ID_S, i != 0);
+                    tc_commit(smem_u32(&x.s_full[n & 1]));
+                    tc_commit(smem_u32(&x.k_empty));
+                }
+                __syncwarp();
+                t = first_from(t + 1);
             }
-            __syncwarp();
-            if (n) outputs(n - 1);
+            if (n) {
+                const int m = n - 1;
+                ok = warp_wait(smem_u32(&x.p_full), m & 1, a.err) && warp_wait(smem_u32(&x.v_full), m & 1, a.err) && warp_wait(smem_u32(&x.o_empty), (m & 1) ^ 1, a.err);
+                if (!ok) break;
+                tc_fence_after();
+                if (tc_elect()) {
+#pragma unroll
+                    for (int d = 0; d < NB; ++d)
+#pragma unroll
+                        for (int i = 0; i < TK / 16; ++i)   // 16 keys
+                            mma_f16(tmem + 2 * N + d * N, desc128(base + Geo::OFF_V + d * 2 * (TK * 128) + i * 2048, TK * 128), desc128(base + Geo::OFF_P + i * 2048, TK * 128), ID_O, i != 0);
+                    tc_commit(smem_u32(&x.pv_done));
+                }
+                __syncwarp();
+            }
+            if (!more) break;
         }
-        if (ok) outputs(n - 1);
         if (tc_elect()) tc_commit(smem_u32(&x.fin));
         __syncwarp();
         tc_wait(smem_u32(&x.fin), 0, a.err);   // nothing in flight when the accumulator memory is given back
-    } else {   // ---- copies
-        const uint8_t* src = a.f16 + ((size_t)sq.s * a.pool.n_kv + kh) * a.tiles * (2 * Geo::PICTURE);
+    } else {   // ---- copies: k of tile n when the scores of tile n - 1 are there, v when the outputs are
+        const int kv = warp == Geo::W_V;
+        const uint8_t* src = a.f16 + (((size_t)sq.s * a.pool.n_kv + kh) * a.tiles * 2 + kv) * Geo::PICTURE;
+        const uint32_t full = smem_u32(kv ? &x.v_full : &x.k_full), empty = smem_u32(kv ? &x.pv_done : &x.k_empty), dst = smem_u32(sm) + (kv ? Geo::OFF_V : Geo::OFF_K);
         int n = 0;
-        for (int t = t_first; t < t_end && ok; t = first_from(t + 1), ++n) {
+        for (int t = t_first; t < t_end && ok; t = first_from(t + 1)) {
+            ok = warp_wait(empty, (n & 1) ^ 1, a.err);
+            if (!ok) break;
+            if (tc_elect()) {
+                mbar_expect_tx(full, Geo::PICTURE);
 #pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-                ok = ok && warp_wait(kv ? smem_u32(&x.pv_done) : smem_u32(&x.k_empty), (n & 1) ^ 1, a.err);   // the operand of the tile before is read
-                if (!ok) break;
-                const uint32_t bar = smem_u32(kv ? &x.v_full : &x.k_full), dst = smem_u32(sm + (kv ? Geo::OFF_V : Geo::OFF_K));
-                if (tc_elect()) {
-                    mbar_expect_tx(bar, Geo::PICTURE);
-#pragma unroll
-                    for (int i = 0; i < D / 64; ++i) bulk_g2s(dst + i * (TK * 128), src + ((size_t)t * 2 + kv) * Geo::PICTURE + i * (TK * 128), TK * 128, bar);
-                }
-                __syncwarp();
-                sent[kv] = n + 1;
+                for (int i = 0; i < D / 64; ++i) bulk_g2s(dst + i * (TK * 128), src + (size_t)t * (2 * Geo::PICTURE) + i * (TK * 128), TK * 128, full);
             }
+            __syncwarp();
+            ++n;
         }
-        // no copy outlives the CTA
-        if (sent[0]) tc_wait(smem_u32(&x.k_full), (sent[0] - 1) & 1, a.err);
-        if (sent[1]) tc_wait(smem_u32(&x.v_full), (sent[1] - 1) & 1, a.err);
+        if (n) tc_wait(full, (n - 1) & 1, a.err);   // no copy outlives the CTA
     }
     tc_fence_before();
     __syncthreads();
