@@ -73,10 +73,12 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         if ((i0 * KS >= sp.sink && i0 < i_lo ? i_lo : i0) >= i_end) return;
     }
     const int lg = a.pool.lg_page, pmask = (1 << lg) - 1;
-    auto row_of = [&](int i) -> uint32_t {   // the pool's row of the slice's first key; 0 behind the end, and for a page number out of range (told by the status word)
-        uint32_t r = 0;
-        if (i < i_end) { r = paged_row(a.pool, sq.s, (i * KS) >> lg, kh, a.arg_err); r = r == 0xffffffffu ? 0u : r + (uint32_t)((i * KS) & pmask); }
-        return r;
+    // the pool's row of a slice's first key; 0 behind the end, and for a page number out of range (told by the status word). The number is fetched a slice ahead
+    auto id_of = [&](int i) -> int { return i < i_end ? paged_id(a.pool, sq.s, (i * KS) >> lg) : 0; };
+    auto row_of = [&](int i, int id) -> uint32_t {
+        if (i >= i_end) return 0u;
+        const uint32_t r = paged_row_of(a.pool, id, kh, a.arg_err);
+        return r == 0xffffffffu ? 0u : r + (uint32_t)((i * KS) & pmask);
     };
     uint8_t* const ring = sm + NT * D * 32 + warp * (SLOTS * KS * D);
     const uint32_t ring_u = smem_u32(ring);
@@ -92,13 +94,14 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     };
     int i0 = first_from((int)(sp.u0 / KS) + ((warp - (int)(sp.u0 / KS)) & (KW - 1)));   // this slice, the next ones and where they lie
     int i1 = first_from(i0 + KW), i2 = first_from(i1 + KW);
-    uint32_t r0 = row_of(i0), r1 = row_of(i1);
+    const int id0 = id_of(i0), id1 = id_of(i1);
+    int id2 = id_of(i2);
+    uint32_t r0 = row_of(i0, id0), r1 = row_of(i1, id1);
     fetch(0, a.pool.k + (size_t)r0 * D, false, i0 < i_end);
     fetch(1, a.pool.v + (size_t)r0 * D, true, i0 < i_end);
     fetch(2, a.pool.k + (size_t)r1 * D, false, i1 < i_end);
     auto scales = [&](uint32_t r) { return (lane < 16 ? a.pool.k_scale : a.pool.v_scale)[(size_t)r + (lane & 15)]; };   // of k in lanes 0 to 15, of v in the others
     float sc = i0 < i_end ? scales(r0) : 0.f;
-    uint32_t r2 = row_of(i2);
 
     // ---- q: a warp per pair; the 8 dims of a lane are its words of two steps of 16 dims, values and rests
     for (int i = warp; i < MB; i += KW) {
@@ -158,8 +161,9 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     int slot = 0;
     for (; i0 < i_end; ) {
         const float sc1 = i1 < i_end ? scales(r1) : 0.f;
+        const uint32_t r2 = row_of(i2, id2);
         const int i3 = first_from(i2 + KW);
-        const uint32_t r3 = row_of(i3);
+        id2 = id_of(i3);
         asm volatile("cp.async.wait_group 2;" ::: "memory");
         __syncwarp();
         // ---- scores of 16 keys
@@ -281,7 +285,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         __syncwarp();
         fetch(slot, a.pool.k + (size_t)r2 * D, false, i2 < i_end);
         slot = slot + 1 == SLOTS ? 0 : slot + 1;
-        i0 = i1; i1 = i2; i2 = i3; r1 = r2; r2 = r3; sc = sc1;
+        i0 = i1; i1 = i2; i2 = i3; r1 = r2; sc = sc1;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)

@@ -60,7 +60,8 @@ __device__ __forceinline__ void ld_there(float (&a)[8]) {   // orders the use of
     for (int i = 0; i < 8; ++i) asm volatile("" : "+f"(a[i]));
 }
 __device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory"); }
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) { return __all_sync(0xffffffffu, tc_wait(bar, parity, err)); }
+// a wait that is over already takes a test, not the 250 clocks of an attempt that may suspend
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) { return __all_sync(0xffffffffu, mbar_test(bar, parity) || tc_wait(bar, parity, err)); }
 __device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) { __syncwarp(); if (lane == 0) mbar_arrive(bar); }
 
 // grid (splits, n_kv, blocks)
@@ -93,12 +94,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
     auto first_from = [&](int t) { return t * TK >= sink && t * TK + TK <= lo ? lo / TK : t; };   // first visible tile at or behind t
     const int t_first = first_from((int)(sp.u0 / TK));
     if (t_first >= t_end) return;
-    // first row of the pool's of the page of key j, 0xffffffff where no token of it is visible or its number is out of range
     const int lg = a.pool.lg_page, pmask = (1 << lg) - 1;
-    auto page_of = [&](int j) -> uint32_t {
-        const int k = j & ~pmask;
-        return j < kend && (k < sink || k + pmask >= lo) ? paged_row(a.pool, sq.s, j >> lg, kh, a.arg_err) : 0xffffffffu;
-    };
 
     if (tid == 0) {
         mbar_init(smem_u32(&x.k_full), 1); mbar_init(smem_u32(&x.k_empty), 1); mbar_init(smem_u32(&x.v_full), 1);
@@ -172,21 +168,28 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
         const int all_hi = pos_lo, all_lo = a.window ? pos_hi - a.window : -1;
         // scales of this thread's key, a tile ahead, and its page, two tiles ahead
         float ks = 0.f, vs = 0.f;
-        uint32_t page = page_of(t_first * TK + key);
+        auto id_of = [&](int t) -> int {   // its check waits for it: a tile ahead of its use
+            const int j = t * TK + key, k = j & ~pmask;
+            return t < t_end && j < kend && (k < sink || k + pmask >= lo) ? paged_id(a.pool, sq.s, j >> lg) : -1;
+        };
+        auto row_of = [&](int t, int id) -> uint32_t {
+            const int j = t * TK + key, k = j & ~pmask;
+            return t < t_end && j < kend && (k < sink || k + pmask >= lo) ? paged_row_of(a.pool, id, kh, a.arg_err) : 0xffffffffu;
+        };
+        uint32_t page = row_of(t_first, id_of(t_first));
         auto scales = [&](int t, float& k, float& v) {
             k = v = 0.f;
             if (t < t_end && page != 0xffffffffu) { const size_t at = (size_t)page + ((t * TK + key) & pmask); k = a.pool.k_scale[at]; v = a.pool.v_scale[at]; }
         };
         scales(t_first, ks, vs);
-        int t1 = first_from(t_first + 1);
-        page = t1 < t_end ? page_of(t1 * TK + key) : 0xffffffffu;
+        int t1 = first_from(t_first + 1), id = id_of(t1);
         int n = 0;
         for (int t = t_first; t < t_end; t = t1, ++n) {
             float ks1, vs1;
             t1 = first_from(t + 1);
+            page = row_of(t1, id);
             scales(t1, ks1, vs1);
-            const int t2 = first_from(t1 + 1);
-            page = t2 < t_end ? page_of(t2 * TK + key) : 0xffffffffu;
+            id = id_of(first_from(t1 + 1));
             const uint32_t sb = tlane + (n & 1) * N + 8 * grp;
             ok = ok && warp_wait(smem_u32(&x.s_full[n & 1]), (n >> 1) & 1, a.err);
             tc_fence_after();

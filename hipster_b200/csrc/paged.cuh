@@ -32,12 +32,14 @@ __device__ __forceinline__ PagedSeq paged_find(const PagedBatch& b, int r, int l
     if (r < q.row0 || r >= q.row0 + q.T) q.s = -1;
     return q;
 }
-// first row of the page of position pos, counted over the pool's rows of head_dim codes for one head: ((page * n_kv + head) << log2 page_size)
-__device__ __forceinline__ uint32_t paged_row(const PagedPool& p, int s, int column, int head, int* err) {
-    int id = p.table[(size_t)s * p.table_ld + column];
+// First row of a page for one head, counted over the pool's rows of head_dim codes: ((page * n_kv + head) << log2 page_size); 0xffffffff for a number out of
+// range. The number is fetched apart: its check waits for it, so a loop fetches the next page's number while it works on this one's.
+__device__ __forceinline__ int paged_id(const PagedPool& p, int s, int column) { return p.table[(size_t)s * p.table_ld + column]; }
+__device__ __forceinline__ uint32_t paged_row_of(const PagedPool& p, int id, int head, int* err) {
     if ((unsigned)id >= (unsigned)p.n_pages) { paged_bad(err); return 0xffffffffu; }
     return ((uint32_t)id * (uint32_t)p.n_kv + (uint32_t)head) << p.lg_page;
 }
+__device__ __forceinline__ uint32_t paged_row(const PagedPool& p, int s, int column, int head, int* err) { return paged_row_of(p, paged_id(p, s, column), head, err); }
 
 // ---- attention: what its two kernels (attn_paged.cu, attn_paged_tc.cu) share
 struct PagedArgs {
