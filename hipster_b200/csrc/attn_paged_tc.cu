@@ -51,9 +51,10 @@ __device__ __forceinline__ void ld8(float (&a)[8], uint32_t col) {
                  : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]), "=f"(a[4]), "=f"(a[5]), "=f"(a[6]), "=f"(a[7]) : "r"(col) : "memory");
 }
 __device__ __forceinline__ void st8(uint32_t col, const float (&a)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\ntcgen05.wait::st.sync.aligned;"
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                  :: "r"(col), "f"(a[0]), "f"(a[1]), "f"(a[2]), "f"(a[3]), "f"(a[4]), "f"(a[5]), "f"(a[6]), "f"(a[7]) : "memory");
 }
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void ld_there(float (&a)[8]) {   // orders the use of the registers behind the wait
 #pragma unroll
@@ -163,6 +164,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
             const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
             for (int i = 0; i < nc; ++i) st8(lcol + 16 * i, zero);
+            st_wait();
         }
         // positions between which a tile is visible to all pairs
         const int all_hi = pos_lo, all_lo = a.window ? pos_hi - a.window : -1;
@@ -211,8 +213,7 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
                 for (int e = 0; e < 8; ++e) s[e] = s[e] + r[e];
             };
             // distances of the logarithms from their references
-            auto distances = [&](float (&d)[8], int i) {
-                scores(d, i);
+            auto measure = [&](float (&d)[8], int i) {
 #pragma unroll
                 for (int e = 0; e < 8; e += 4) {
                     const float4 c = *reinterpret_cast<const float4*>(&x.c[8 * (2 * i + grp) + e]), m = *reinterpret_cast<const float4*>(&x.mu[warp][8 * i + e]);
@@ -223,13 +224,38 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
                     for (int e = 0; e < 8; ++e) if (hide >> (8 * i + e) & 1) d[e] = -INFINITY;
                 }
             };
-            float top = -INFINITY;
-#pragma unroll 1
-            for (int i = 0; i < nc; ++i) {
-                float d[8];
-                distances(d, i);
+            // a full block: the distances of all sets stay in registers, their loads in flight together
+            const bool full = nc == NC;
+            float da[NC][8];
+            auto measure_all = [&] {
+                float r[NC][8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, d[e]);
+                for (int i = 0; i < NC; ++i) { ld8(da[i], sb + 16 * i); ld8(r[i], sb + MB + 16 * i); }
+                ld_wait();
+#pragma unroll
+                for (int i = 0; i < NC; ++i) {
+                    ld_there(da[i]); ld_there(r[i]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) da[i][e] = da[i][e] + r[i][e];
+                }
+#pragma unroll
+                for (int i = 0; i < NC; ++i) measure(da[i], i);
+            };
+            float top = -INFINITY;
+            if (full) {
+                measure_all();
+#pragma unroll
+                for (int i = 0; i < NC; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, da[i][e]);
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < nc; ++i) {
+                    float d[8];
+                    scores(d, i); measure(d, i);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, d[e]);
+                }
             }
             if (__any_sync(0xffffffffu, top + lv > MU_LIMIT) && lane == 0) x.moved[n & 3][grp] = n + 1;
             group_sync(grp);
@@ -259,17 +285,13 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
                     ld8(l, lcol + 16 * i); ld_wait(); ld_there(l);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) l[e] = l[e] * __shfl_sync(0xffffffffu, al, 8 * i + e);
-                    st8(lcol + 16 * i, l);
+                    st8(lcol + 16 * i, l); st_wait();
                 }
                 __syncwarp();
+                if (full) measure_all();
             }
             ok = ok && warp_wait(smem_u32(&x.pv_done), (n & 1) ^ 1, a.err);   // the weights of the tile before are read
-#pragma unroll 1
-            for (int i = 0; i < nc; ++i) {
-                float d[8], l[8];
-                ld8(l, lcol + 16 * i);
-                distances(d, i);
-                ld_there(l);
+            auto weigh = [&](float (&d)[8], float (&l)[8], int i) {
                 uint32_t h[4], r[4];
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
@@ -285,7 +307,28 @@ __global__ void __launch_bounds__(PagedGeo<D, MB>::WARPS * 32, 1) k_paged_prompt
                 const int ch = 2 * i + grp, cr = MB / 8 + ch;   // eights of columns; 64 columns of all keys lie one behind the other
                 *reinterpret_cast<uint4*>(pw + (ch >> 3) * (TK * 128) + (((ch & 7) ^ (key & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
                 *reinterpret_cast<uint4*>(pw + (cr >> 3) * (TK * 128) + (((cr & 7) ^ (key & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+            };
+            if (full) {
+                float l[NC][8];
+#pragma unroll
+                for (int i = 0; i < NC; ++i) ld8(l[i], lcol + 16 * i);
+                ld_wait();
+#pragma unroll
+                for (int i = 0; i < NC; ++i) ld_there(l[i]);
+#pragma unroll
+                for (int i = 0; i < NC; ++i) weigh(da[i], l[i], i);
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < nc; ++i) {
+                    float d[8], l[8];
+                    ld8(l, lcol + 16 * i);
+                    scores(d, i);
+                    ld_there(l);
+                    measure(d, i);
+                    weigh(d, l, i);
+                }
             }
+            st_wait();
             tc_fence_before();
             fence_proxy_async();
             __syncwarp();
