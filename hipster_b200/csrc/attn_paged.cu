@@ -82,13 +82,30 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     };
     uint8_t* const ring = sm + NT * D * 32 + warp * (SLOTS * KS * D);
     const uint32_t ring_u = smem_u32(ring);
-    auto fetch = [&](int slot, const uint8_t* src, bool v, bool live) {   // 16 rows, one run of memory
-        if (live) {
+    // A slot's 16 rows are one run of memory; piece e = 32 i + lane of it goes to place(e / CPR, e % CPR), which is 512 i and a part that repeats after two (k) or four (v) i
+    int kput[2], vput[4];
 #pragma unroll
-            for (int i = 0; i < KS * CPR / 32; ++i) {
-                const int e = i * 32 + lane, r = e / CPR, c = e % CPR;
-                cp_async16(ring_u + slot * (KS * D) + (v ? place<D, true>(r, c) : place<D, false>(r, c)), src + e * 16);
-            }
+    for (int i = 0; i < 4; ++i) {
+        const int e = 32 * i + lane;
+        if (i < 2) kput[i] = place<D, false>(e / CPR, e % CPR) - 512 * i;
+        vput[i] = place<D, true>(e / CPR, e % CPR) - 512 * i;
+    }
+    const uint8_t* const kbase = a.pool.k + lane * 16; const uint8_t* const vbase = a.pool.v + lane * 16;
+    auto fetch_k = [&](int slot, uint32_t row, bool live) {
+        if (live) {
+            const uint8_t* src = kbase + (size_t)row * D;
+            const uint32_t d0 = ring_u + slot * (KS * D) + kput[0], d1 = ring_u + slot * (KS * D) + kput[1];
+#pragma unroll
+            for (int i = 0; i < KS * CPR / 32; ++i) cp_async16((i & 1 ? d1 : d0) + 512 * i, src + 512 * i);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto fetch_v = [&](int slot, uint32_t row, bool live) {
+        if (live) {
+            const uint8_t* src = vbase + (size_t)row * D;
+            const uint32_t at = ring_u + slot * (KS * D), d[4] = {at + vput[0], at + vput[1], at + vput[2], at + vput[3]};
+#pragma unroll
+            for (int i = 0; i < KS * CPR / 32; ++i) cp_async16(d[i & 3] + 512 * i, src + 512 * i);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -97,10 +114,9 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     const int id0 = id_of(i0), id1 = id_of(i1);
     int id2 = id_of(i2);
     uint32_t r0 = row_of(i0, id0), r1 = row_of(i1, id1);
-    fetch(0, a.pool.k + (size_t)r0 * D, false, i0 < i_end);
-    fetch(1, a.pool.v + (size_t)r0 * D, true, i0 < i_end);
-    fetch(2, a.pool.k + (size_t)r1 * D, false, i1 < i_end);
-    auto scales = [&](uint32_t r) { return (lane < 16 ? a.pool.k_scale : a.pool.v_scale)[(size_t)r + (lane & 15)]; };   // of k in lanes 0 to 15, of v in the others
+    fetch_k(0, r0, i0 < i_end); fetch_v(1, r0, i0 < i_end); fetch_k(2, r1, i1 < i_end);
+    const float* const sbase = (lane < 16 ? a.pool.k_scale : a.pool.v_scale) + (lane & 15);   // scales of k in lanes 0 to 15, of v in the others
+    auto scales = [&](uint32_t r) { return sbase[r]; };
     float sc = i0 < i_end ? scales(r0) : 0.f;
 
     // ---- q: a warp per pair; the 8 dims of a lane are its words of two steps of 16 dims, values and rests
@@ -191,7 +207,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
                 for (int c = 0; c < 4; ++c) s[n][c] = (sh[n][0][c] + sh[n][1][c]) + sl[n][c];
         }
         __syncwarp();
-        fetch(slot, a.pool.v + (size_t)r1 * D, true, i1 < i_end);
+        fetch_v(slot, r1, i1 < i_end);
         slot = slot + 1 == SLOTS ? 0 : slot + 1;
         // ---- weights
         const float k0 = __shfl_sync(0xffffffffu, sc, g), k1 = __shfl_sync(0xffffffffu, sc, g + 8), v0 = __shfl_sync(0xffffffffu, sc, g + 16), v1 = __shfl_sync(0xffffffffu, sc, g + 24);
@@ -283,7 +299,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             }
         }
         __syncwarp();
-        fetch(slot, a.pool.k + (size_t)r2 * D, false, i2 < i_end);
+        fetch_k(slot, r2, i2 < i_end);
         slot = slot + 1 == SLOTS ? 0 : slot + 1;
         i0 = i1; i1 = i2; i2 = i3; r1 = r2; sc = sc1;
     }
