@@ -7,6 +7,7 @@
 #include "paged.cuh"
 #include <algorithm>
 #include <cuda_fp8.h>
+#include <type_traits>
 
 namespace hp {
 namespace {
@@ -58,18 +59,16 @@ __global__ void __launch_bounds__(256) k_rope_table_sums(const RopeArgs a, int g
         rope_sm[e] = k < ROPE_GROUP ? make_double2(c, s) : make_double2(c * a.mul, s * a.mul);
     }
     __syncthreads();
+    // a thread keeps k and i, and goes through the values of h: one read of shared memory per entry
     const int n = ROPE_GROUP * a.half;
-    for (int h = 0; h < groups; ++h) {
-        const size_t p0 = (size_t)(h0 + h) * ROPE_GROUP;
-        if (p0 >= (size_t)a.n_pos) break;
-        const int live = min(n, (int)min((size_t)n, ((size_t)a.n_pos - p0) * a.half));
-        int i = threadIdx.x % a.half;
-        const int step = 256 % a.half;
-        for (int e = threadIdx.x; e < live; e += 256) {
-            const double2 u = far[h * a.half + i], v = near[e];
-            a.table[p0 * a.half + e] = make_float2((float)(u.x * v.x - u.y * v.y), (float)(u.y * v.x + u.x * v.y));
-            i += step; if (i >= a.half) i -= a.half;
-        }
+    const size_t end = (size_t)a.n_pos * a.half;
+    for (int e = threadIdx.x; e < n; e += 256) {
+        const double2 v = near[e];
+        const double2* u = far + e % a.half;
+        size_t at = (size_t)h0 * n + e;
+#pragma unroll 4
+        for (int h = 0; h < groups; ++h, at += n, u += a.half)
+            if (at < end) a.table[at] = make_float2((float)(u->x * v.x - u->y * v.y), (float)(u->y * v.x + u->x * v.y));
     }
 }
 
@@ -78,181 +77,175 @@ template <int KIND> __device__ __forceinline__ uint32_t kv_code(float x) {
     if constexpr (KIND == KV_I8) return (uint32_t)min(127, max(-127, __float2int_rn(x))) & 0xffu;
     else return (uint32_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
 }
-// A warp takes HPW neighbouring heads of a row (n_head query heads, then n_kv key heads, then n_kv value heads), whose loads are all in flight before the row's
-// place is known. A lane holds D / 32 elements of a head, in groups of four neighbours; a head goes through shared memory once, where each element finds the
-// other one of its pair in either layout; the angles are the row's, read once.
-template <int D, int KIND, int HPW>
-__global__ void __launch_bounds__(256) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, int* err) {
-    constexpr int NV = D >= 128 ? 4 : 2, NG = D / 32 / NV;   // neighbours of a group, groups of a lane
-    __shared__ __align__(16) float buf[8][D];
+// D / 8 lanes take a head of a row, eight neighbouring elements each, so that a warp has 1, 2 or 4 heads side by side; it takes hpw such sets of neighbouring
+// heads (n_head query heads, then n_kv key heads, then n_kv value heads) in a loop that fetches a set ahead. The row's place and angles are found once. Instructions
+// bound it beyond a few thousand heads: 220 per head of 128 with a warp per head and the loop unrolled four times (which did not fit the
+// instruction cache), 171 in a loop.
+template <int D, int KIND>
+__global__ void __launch_bounds__(256) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, int hpw, int* err) {
+    constexpr int LPH = D / 8, HPS = 32 / LPH;   // lanes of a head, heads of a set
+    __shared__ __align__(16) float buf[8][32 * 8];
     pdl_launch_dependents();
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = p.n_head + 2 * pool.n_kv, parts = (heads + HPW - 1) / HPW;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPH, d0 = (lane % LPH) * 8, heads = p.n_head + 2 * pool.n_kv, parts = (heads + hpw * HPS - 1) / (hpw * HPS);
+    const unsigned mask = LPH == 32 ? 0xffffffffu : ((1u << (LPH & 31)) - 1u) << (sub * LPH);
     const long long item = (long long)blockIdx.x * 8 + warp;
-    const int r = (int)(item / parts), h0 = (int)(item % parts) * HPW;
+    const int r = (int)(item / parts), h0 = (int)(item % parts) * hpw * HPS + sub, h1 = min(heads, h0 - sub + hpw * HPS);
     if (r >= b.R) return;
-    float y[HPW][NG][NV];
-#pragma unroll
-    for (int i = 0; i < HPW; ++i) {
-        const int h = h0 + i;
-        if (h < heads) {
-            const float* x = h < p.n_head ? p.q + (size_t)r * p.q_ld + h * p.q_hs : h < p.n_head + pool.n_kv ? p.k + (size_t)r * p.k_ld + (h - p.n_head) * p.k_hs : p.v + (size_t)r * p.v_ld + (h - p.n_head - pool.n_kv) * p.v_hs;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const float* s = x + (g * 32 + lane) * NV;
-                if constexpr (NV == 4) { const float4 t = *reinterpret_cast<const float4*>(s); y[i][g][0] = t.x; y[i][g][1] = t.y; y[i][g][2] = t.z; y[i][g][3] = t.w; }
-                else { const float2 t = *reinterpret_cast<const float2*>(s); y[i][g][0] = t.x; y[i][g][1] = t.y; }
-            }
-        }
-    }
+    float4 next[2];
+    auto fetch = [&](int h) {
+        const float* from = h < p.n_head ? p.q + (size_t)r * p.q_ld + (size_t)h * p.q_hs : h < p.n_head + pool.n_kv ? p.k + (size_t)r * p.k_ld + (size_t)(h - p.n_head) * p.k_hs
+                                                                                            : p.v + (size_t)r * p.v_ld + (size_t)(h - p.n_head - pool.n_kv) * p.v_hs;
+        next[0] = reinterpret_cast<const float4*>(from + d0)[0]; next[1] = reinterpret_cast<const float4*>(from + d0)[1];
+    };
+    if (h0 < h1) fetch(h0);
     const PagedSeq q = paged_find(b, r, lane, err);
     if (q.s < 0) return;
     const int pos = q.len - q.T + r - q.row0;
     if (pos < 0 || pos >= p.n_pos) { paged_bad(err); return; }
-    const uint32_t page = h0 + HPW > p.n_head ? paged_row(pool, q.s, pos >> pool.lg_page, 0, err) : 0u;
+    const uint32_t page = h1 > p.n_head ? paged_row(pool, q.s, pos >> pool.lg_page, 0, err) : 0u;
     const int half = p.n_rot / 2;
-    float2 cs[NG][NV];
-    if (p.n_rot && h0 < p.n_head + pool.n_kv) {
+    // angles of the lane's elements; interleaved: of its four pairs
+    float2 cs[8];
+    const bool turns = d0 < p.n_rot;
+    if (turns) {
         const float2* t = reinterpret_cast<const float2*>(p.rope) + (size_t)pos * half;
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int d = (g * 32 + lane) * NV + j;
-                if (d < p.n_rot) cs[g][j] = t[p.interleaved ? d >> 1 : d < half ? d : d - half];
-            }
+        for (int j = 0; j < 8; ++j) {
+            const int d = d0 + j;
+            if (d < p.n_rot && (!p.interleaved || !(j & 1))) cs[j] = t[p.interleaved ? d >> 1 : d < half ? d : d - half];
+        }
     }
-#pragma unroll
-    for (int i = 0; i < HPW; ++i) {
-        const int h = h0 + i;
-        if (h >= heads) return;
+#pragma unroll 1
+    for (int h = h0; h < h1; h += HPS) {
+        float x[8] = {next[0].x, next[0].y, next[0].z, next[0].w, next[1].x, next[1].y, next[1].z, next[1].w};
+        if (h + HPS < h1) fetch(h + HPS);
         const int kind = h < p.n_head ? 0 : h < p.n_head + pool.n_kv ? 1 : 2, hh = kind == 0 ? h : kind == 1 ? h - p.n_head : h - p.n_head - pool.n_kv;
-        float (&x)[NG][NV] = y[i];
         const uint16_t* nw = (const uint16_t*)(kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr);
         if (nw) {
             float ss = 0.f;
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
+            for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
 #pragma unroll
-                for (int j = 0; j < NV; ++j) ss = fmaf(x[g][j], x[g][j], ss);
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) ss = ss + __shfl_xor_sync(0xffffffffu, ss, off);
+            for (int off = LPH / 2; off > 0; off >>= 1) ss = ss + __shfl_xor_sync(mask, ss, off);
             const float inv = 1.0f / sqrtf(ss / (float)D + p.eps);
+            const uint16_t* w = nw + d0;
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-                for (int j = 0; j < NV; ++j) x[g][j] = (x[g][j] * inv) * bf2f(nw[(g * 32 + lane) * NV + j]);
+            for (int j = 0; j < 8; ++j) x[j] = (x[j] * inv) * bf2f(w[j]);
         }
         if (kind < 2 && p.n_rot) {
-            float* row = buf[warp];
-            if (HPW > 1) __syncwarp();
+            if (p.interleaved) {   // the other one of a pair is the lane's own
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                float* t = row + (g * 32 + lane) * NV;
-                if constexpr (NV == 4) *reinterpret_cast<float4*>(t) = make_float4(x[g][0], x[g][1], x[g][2], x[g][3]);
-                else *reinterpret_cast<float2*>(t) = make_float2(x[g][0], x[g][1]);
-            }
-            __syncwarp();
+                for (int j = 0; j < 8; j += 2)
+                    if (d0 + j < p.n_rot) {
+                        const float x0 = x[j], x1 = x[j + 1];
+                        x[j] = fmaf(-x1, cs[j].y, x0 * cs[j].x); x[j + 1] = fmaf(x1, cs[j].x, x0 * cs[j].y);
+                    }
+            } else {
+                float* row = buf[warp] + sub * D;
+                __syncwarp(mask);
+                reinterpret_cast<float4*>(row + d0)[0] = make_float4(x[0], x[1], x[2], x[3]); reinterpret_cast<float4*>(row + d0)[1] = make_float4(x[4], x[5], x[6], x[7]);
+                __syncwarp(mask);
+                if (turns) {
+                    if (half % 8 == 0) {   // the lane's elements are all first or all second ones
+                        const float* t = row + (d0 < half ? d0 + half : d0 - half);
+                        const float4 u = reinterpret_cast<const float4*>(t)[0], v = reinterpret_cast<const float4*>(t)[1];
+                        const float o[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w}, sign = d0 < half ? -1.f : 1.f;
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
+                        for (int j = 0; j < 8; ++j) x[j] = d0 < half ? fmaf(sign * o[j], cs[j].y, x[j] * cs[j].x) : fmaf(x[j], cs[j].x, o[j] * cs[j].y);
+                    } else {
 #pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int d = (g * 32 + lane) * NV + j;
-                    if (d < p.n_rot) {
-                        const bool first = p.interleaved ? !(d & 1) : d < half;
-                        const float other = row[p.interleaved ? d ^ 1 : first ? d + half : d - half];
-                        const float2 t = cs[g][j];
-                        x[g][j] = first ? fmaf(-other, t.y, x[g][j] * t.x) : fmaf(x[g][j], t.x, other * t.y);
+                        for (int j = 0; j < 8; ++j) {
+                            const int d = d0 + j;
+                            if (d < half) x[j] = fmaf(-row[d + half], cs[j].y, x[j] * cs[j].x); else if (d < p.n_rot) x[j] = fmaf(x[j], cs[j].x, row[d - half] * cs[j].y);
+                        }
                     }
                 }
+            }
         }
         if (kind == 0) {
-            float* o = p.q_out + (size_t)r * p.qo_ld + hh * p.qo_hs;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                float* t = o + (g * 32 + lane) * NV;
-                if constexpr (NV == 4) *reinterpret_cast<float4*>(t) = make_float4(x[g][0], x[g][1], x[g][2], x[g][3]);
-                else *reinterpret_cast<float2*>(t) = make_float2(x[g][0], x[g][1]);
-            }
+            float4* o = reinterpret_cast<float4*>(p.q_out + (size_t)r * p.qo_ld + (size_t)hh * p.qo_hs + d0);
+            o[0] = make_float4(x[0], x[1], x[2], x[3]); o[1] = make_float4(x[4], x[5], x[6], x[7]);
             continue;
         }
-        if (page == 0xffffffffu) continue;
         // largest magnitude, over the bit patterns: an infinity or a NaN wins, and the token is then marked by a NaN scale over codes of zero
         uint32_t m = 0;
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
 #pragma unroll
-            for (int j = 0; j < NV; ++j) m = max(m, __float_as_uint(x[g][j]) & 0x7fffffffu);
-        m = __reduce_max_sync(0xffffffffu, m);
+        for (int off = LPH / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(mask, m, off));
+        if (page == 0xffffffffu) continue;
         const bool finite = m < 0x7f800000u;
         const float scale = finite ? __fdiv_rn(__uint_as_float(m), KIND == KV_I8 ? 127.f : 448.f) : __uint_as_float(0x7fc00000u);
         const bool live = finite && scale > 0.f;
+        const float inv = live ? __fdiv_rn(1.f, scale) : 0.f;
         const size_t at = (size_t)page + ((size_t)hh << pool.lg_page) + (pos & ((1 << pool.lg_page) - 1));
-        uint8_t* o = (kind == 1 ? pool.k : pool.v) + at * D;
+        uint32_t w[2] = {0u, 0u};
+        if (live) {
+            if (inv < INFINITY) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            uint32_t w = 0;
-#pragma unroll
-            for (int j = 0; j < NV; ++j) w |= (live ? kv_code<KIND>(__fdiv_rn(x[g][j], scale)) : 0u) << (8 * j);
-            if constexpr (NV == 4) reinterpret_cast<uint32_t*>(o)[g * 32 + lane] = w;
-            else reinterpret_cast<uint16_t*>(o)[g * 32 + lane] = (uint16_t)w;
+                for (int j = 0; j < 8; ++j) w[j >> 2] |= kv_code<KIND>(x[j] * inv) << (8 * (j & 3));
+            } else {   // a scale below 2^-128 has no reciprocal in 32 bits
+                for (int j = 0; j < 8; ++j) w[j >> 2] |= kv_code<KIND>(__fdiv_rn(x[j], scale)) << (8 * (j & 3));
+            }
         }
-        if (lane == 0) (kind == 1 ? pool.k_scale : pool.v_scale)[at] = scale;
+        *reinterpret_cast<uint2*>((kind == 1 ? pool.k : pool.v) + at * D + d0) = make_uint2(w[0], w[1]);
+        if (d0 == 0) (kind == 1 ? pool.k_scale : pool.v_scale)[at] = scale;
     }
 }
 
-// code times scale, rounded to f16 once; the e4m3 patterns 0x7f and 0xff, which the quantiser does not write, read as 480 and -480
-template <int KIND> __device__ __forceinline__ float kv_value(uint32_t code) {
-    if constexpr (KIND == KV_I8) return (float)(int8_t)code;
-    else { const uint32_t h = ((code & 0x80u) << 8) | ((code & 0x7fu) << 7); return h2f((uint16_t)h) * 256.f; }
-}
-// 8 rows per block; thread = 16 neighbouring codes of a row, a head and k or v
-template <int KIND>
+// RB rows per block, RB / 8 of them found by each warp; thread = 16 neighbouring codes of a row, a head and k or v, times the scale, rounded to f16 once. The e4m3
+// patterns 0x7f and 0xff, which the quantiser does not write, read as 480 and -480.
+template <int D, int KIND, int RB>
 __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, __half* __restrict__ ko, __half* __restrict__ vo, size_t row_stride, size_t head_stride, int* err) {
-    __shared__ uint32_t base[8];   // of head 0
+    constexpr int CPR = D / 16, PER = RB / 8;
+    __shared__ uint32_t base[RB];   // of head 0
     pdl_launch_dependents();
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.x * 8, D = pool.head_dim, cpr = D / 16;
-    const int page = 1 << pool.lg_page;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.x * RB;
     {
-        const int r = r0 + warp;
-        uint32_t at = 0xffffffffu;
-        if (r < b.R) {
-            const PagedSeq q = paged_find(b, r, lane, err);
-            const int pos = q.len - q.T + r - q.row0;
-            if (q.s >= 0 && pos < 0) paged_bad(err);
-            if (q.s >= 0 && pos >= 0) { at = paged_row(pool, q.s, pos >> pool.lg_page, 0, err); if (at != 0xffffffffu) at += pos & (page - 1); }
+        int s = -1, pos = -1;   // of row `lane` of the warp's
+        PagedSeq q{-1, 0, 0, 0};
+#pragma unroll 1
+        for (int i = 0; i < PER; ++i) {
+            const int r = r0 + warp * PER + i;
+            if (r >= b.R) break;
+            if (q.s < 0 || r >= q.row0 + q.T) q = paged_find(b, r, lane, err);   // neighbours mostly belong to one sequence
+            if (q.s >= 0 && lane == i) { s = q.s; pos = q.len - q.T + r - q.row0; }
         }
-        if (lane == 0) base[warp] = at;
+        uint32_t at = 0xffffffffu;
+        if (s >= 0 && pos < 0) paged_bad(err);
+        if (s >= 0 && pos >= 0) { at = paged_row(pool, s, pos >> pool.lg_page, 0, err); if (at != 0xffffffffu) at += pos & ((1 << pool.lg_page) - 1); }
+        if (lane < PER) base[warp * PER + lane] = at;
     }
     __syncthreads();
-    const int n = 2 * pool.n_kv * 8 * cpr;
+    const int n = 2 * pool.n_kv * RB * CPR;
     for (int i0 = threadIdx.x; i0 < n; i0 += 4 * 256) {   // four pieces of a thread in flight
-        uint4 w[4]; float sc[4]; size_t to[4]; bool live[4];
+        uint4 w[4]; float sc[4]; uint32_t row[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * 256, c = i % cpr, t = i / cpr % 8, hv = i / (8 * cpr), h = hv >> 1;
-            live[u] = i < n && base[t] != 0xffffffffu;
-            if (live[u]) {
-                const size_t at = (size_t)base[t] + ((size_t)h << pool.lg_page);
+            const int i = i0 + u * 256, hv = i / (RB * CPR), c = i % CPR;
+            row[u] = i < n ? base[i / CPR % RB] : 0xffffffffu;
+            if (row[u] != 0xffffffffu) {
+                const size_t at = (size_t)row[u] + ((size_t)(hv >> 1) << pool.lg_page);
                 w[u] = *reinterpret_cast<const uint4*>((hv & 1 ? pool.v : pool.k) + at * D + c * 16);
                 sc[u] = (hv & 1 ? pool.v_scale : pool.k_scale)[at];
-                to[u] = (size_t)(r0 + t) * row_stride + (size_t)h * head_stride + c * 16;
             }
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            if (!live[u]) continue;
-            const int hv = (i0 + u * 256) / (8 * cpr);
+            if (row[u] == 0xffffffffu) continue;
+            const int i = i0 + u * 256, hv = i / (RB * CPR), c = i % CPR;
+            const float s = KIND == KV_I8 ? sc[u] : sc[u] * 256.f;   // code_pair gives e4m3 codes times 2^-8
             const uint32_t ws[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
             uint32_t o[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint32_t v = ws[j / 2] >> (16 * (j & 1));
-                const __half2 x = __floats2half2_rn(kv_value<KIND>(v & 0xffu) * sc[u], kv_value<KIND>((v >> 8) & 0xffu) * sc[u]);
-                o[j] = *reinterpret_cast<const uint32_t*>(&x);
+                const uint32_t pr = j & 1 ? code_pair<KIND, 2>(ws[j / 2]) : code_pair<KIND, 0>(ws[j / 2]);
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pr));
+                o[j] = h2_bits(__floats2half2_rn(f.x * s, f.y * s));
             }
-            uint4* dst = reinterpret_cast<uint4*>((hv & 1 ? vo : ko) + to[u]);
+            uint4* dst = reinterpret_cast<uint4*>((hv & 1 ? vo : ko) + (size_t)(r0 + i / CPR % RB) * row_stride + (size_t)(hv >> 1) * head_stride + c * 16);
             dst[0] = make_uint4(o[0], o[1], o[2], o[3]); dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
         }
     }
@@ -261,11 +254,11 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
 template <int D, int KIND> int launch_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, cudaStream_t s) {
     const int heads = p.n_head + 2 * pool.n_kv;
     int* err = device_arg_flag();
-    // one head per warp while all of them fit on the GPU at once; four beyond
-    const bool few = (long long)b.R * heads <= 148 * 64;
-    const long long items = (long long)b.R * (few ? heads : (heads + 3) / 4);
-    const dim3 grid((unsigned)((items + 7) / 8));
-    HP_CUDA(few ? launch_pdl<4>(k_kv_append<D, KIND, 1>, grid, dim3(256), 0, s, pool, b, p, err) : launch_pdl<4>(k_kv_append<D, KIND, 4>, grid, dim3(256), 0, s, pool, b, p, err));
+    // one set of heads per warp while all of them fit on the GPU at once; several beyond
+    constexpr int HPS = 32 / (D / 8);
+    const int hpw = (long long)b.R * heads <= 148 * 64 * HPS ? 1 : 6;
+    const long long items = (long long)b.R * ((heads + hpw * HPS - 1) / (hpw * HPS));
+    HP_CUDA(launch_pdl<4>(k_kv_append<D, KIND>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, s, pool, b, p, hpw, err));
     return HP_OK;
 }
 template <int KIND> int launch_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, cudaStream_t s) {
@@ -295,10 +288,16 @@ int kv_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& 
     return pool.kind == KV_I8 ? launch_append<KV_I8>(pool, b, p, s) : launch_append<KV_E4M3>(pool, b, p, s);
 }
 int kv_read(const PagedPool& pool, const PagedBatch& b, void* k_out, void* v_out, size_t row_stride, size_t head_stride, cudaStream_t s) {
-    const dim3 grid((b.R + 7) / 8);
+    // 8 rows per block until there are several blocks for every SM; 32 beyond, where finding the rows bounds a block of 8
+    const bool many = b.R > 148 * 32;
     int* err = device_arg_flag();
-    HP_CUDA(pool.kind == KV_I8 ? launch_pdl<4>(k_kv_read<KV_I8>, grid, dim3(256), 0, s, pool, b, (__half*)k_out, (__half*)v_out, row_stride, head_stride, err)
-                               : launch_pdl<4>(k_kv_read<KV_E4M3>, grid, dim3(256), 0, s, pool, b, (__half*)k_out, (__half*)v_out, row_stride, head_stride, err));
+    auto go = [&](auto kernel, int rb) { return launch_pdl<4>(kernel, dim3((b.R + rb - 1) / rb), dim3(256), 0, s, pool, b, (__half*)k_out, (__half*)v_out, row_stride, head_stride, err); };
+    auto type = [&](auto kind) {
+        constexpr int KIND = decltype(kind)::value;
+        return pool.head_dim == 256 ? (many ? go(k_kv_read<256, KIND, 32>, 32) : go(k_kv_read<256, KIND, 8>, 8)) : pool.head_dim == 128 ? (many ? go(k_kv_read<128, KIND, 32>, 32) : go(k_kv_read<128, KIND, 8>, 8))
+                                                                                                                          : (many ? go(k_kv_read<64, KIND, 32>, 32) : go(k_kv_read<64, KIND, 8>, 8));
+    };
+    HP_CUDA(pool.kind == KV_I8 ? type(std::integral_constant<int, KV_I8>()) : type(std::integral_constant<int, KV_E4M3>()));
     return HP_OK;
 }
 
