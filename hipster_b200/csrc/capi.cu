@@ -300,7 +300,7 @@ static int attn_paged_check(const char* who, int n_head, int window, int n_sink,
 size_t hp_attn_paged_workspace_bytes(int table_ld, int S, int R, int max_rows, int max_kv, int n_head, int window, int n_sink, const hp_kv_pages* pages) {
     hp::PagedPool pool; hp::PagedBatch b;
     if (paged_args("hp_attn_paged_workspace_bytes", pages, nullptr, table_ld, nullptr, nullptr, S, R, max_rows, max_kv, &pool, &b) || attn_paged_check("hp_attn_paged_workspace_bytes", n_head, window, n_sink, pool)) return 0;
-    return hp::attn_paged_workspace_bytes(pool, b, n_head, window, n_sink);
+    return hp::attn_paged_workspace_bytes(pool, b, n_head, window > 1 << 30 ? 1 << 30 : window, n_sink > 1 << 30 ? 1 << 30 : n_sink);
 }
 int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const float* gate_dev, long long g_ld, long long g_hs, int n_head, const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev,
                   int S, int R, int max_rows, int max_kv, const hp_kv_pages* pages, float scale, int window, int n_sink, float* out_dev, void* xq_q_dev, void* xq_sc_dev, void* workspace_dev, void* stream) {
@@ -313,6 +313,8 @@ int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const floa
     HP_REQUIRE(rows_ok(q_dev, q_ld, q_hs) && (!gate_dev || (((uintptr_t)gate_dev & 3) == 0 && g_ld >= 0 && g_hs >= 0)) && ((uintptr_t)workspace_dev & 15) == 0 && ((uintptr_t)out_dev & 3) == 0,
                "hp_attn_paged: rows and workspace must be 16-byte aligned, with strides that are multiples of 4");
     HP_REQUIRE(scale > 0 && scale < 1e30f, "hp_attn_paged: bad scale");
+    if (window > 1 << 30) window = 1 << 30;   // longer than any sequence
+    if (n_sink > 1 << 30) n_sink = 1 << 30;
     hp::AttnPagedParams p; p.q = q_dev; p.q_ld = q_ld; p.q_hs = q_hs; p.gate = gate_dev; p.g_ld = g_ld; p.g_hs = g_hs; p.n_head = n_head; p.scale = scale; p.window = window; p.n_sink = n_sink;
     p.out = out_dev; p.xq = hp::XQ8F{xq_q_dev, xq_sc_dev}; p.workspace = workspace_dev;
     return hp::attn_paged(pool, b, p, (cudaStream_t)stream);

@@ -271,7 +271,7 @@ int rope_table(float* table, int n_pos, int n_rot, double base, int scaling, dou
     const double mul = scaling == 2 ? (attn_factor > 0 ? attn_factor : 0.1 * log(factor) + 1.0) : (attn_factor > 0 ? attn_factor : 1.0);
     RopeArgs a; a.table = (float2*)table; a.n_pos = n_pos; a.half = n_rot / 2; a.base = base; a.scaling = scaling; a.factor = factor; a.orig_ctx = orig_ctx; a.fast = beta_fast; a.slow = beta_slow; a.mul = mul;
     const size_t n = (size_t)n_pos * a.half;
-    const int total = (n_pos + ROPE_GROUP - 1) / ROPE_GROUP;
+    const int total = (int)(((long long)n_pos + ROPE_GROUP - 1) / ROPE_GROUP);
     int groups = (total + 2 * 148 - 1) / (2 * 148);   // two blocks per SM
     if (groups > ROPE_GROUP) groups = ROPE_GROUP;
     if (groups < 4) {   // fewer groups share too little: see k_rope_table_sums

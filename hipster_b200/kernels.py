@@ -229,6 +229,8 @@ def rope_table(n_pos, n_rot, base, scaling=None, factor=1.0, orig_ctx=0, beta_fa
     by parts: those that turn less than beta_slow times over orig_ctx positions wholly, those over beta_fast times not."""
     if scaling not in _SCALING:
         raise HipsterError(1, f"rope_table: unknown scaling {scaling!r}")
+    if n_pos < 1 or n_rot < 2:
+        raise HipsterError(1, f"rope_table: bad shape n_pos={n_pos} n_rot={n_rot}")
     out = torch.empty((n_pos, n_rot // 2, 2), dtype=_F32, device=device)
     if out.get_device() != _device():
         raise HipsterError(1, "rope_table: the device must be the current one")

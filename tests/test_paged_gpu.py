@@ -1,6 +1,9 @@
 """The paged 8-bit cache on the GPU (hp_rope_table, hp_kv_append, hp_kv_read, hp_attn_paged) against plain implementations in 64 bits."""
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -346,6 +349,33 @@ def test_attention_long_context():
     check_attn([1], [40000], 2, 2, 64, 256, "e4m3", window=33000, n_sink=600)
 
 
+@pytest.mark.parametrize("H,n_kv,most", [(6, 2, 3), (2, 2, 16), (3, 1, 40)])
+def test_attention_many_sequences(H, n_kv, most):
+    rows = [1 + (7 * i) % most for i in range(75)]
+    check_attn(rows, [r + (37 * i) % 300 for i, r in enumerate(rows)], H, n_kv, 64, 16, "i8")
+
+
+def test_sequences_that_share_pages():
+    st = Setup([2, 2, 1], [140, 140, 100], 2, 128, 16, "e4m3")
+    st.table[1], st.table[2, :6] = st.table[0], st.table[0, :6]
+    q = torch.randn((5, 4, 128), generator=gen(1), device="cuda")
+    q[2:4] = q[:2]
+    got, _ = K_.attn_paged(q, st.pool, *st.batch, max_rows=2, max_kv=140)
+    want, tol = attn64(st, q, 128 ** -0.5, 0, 0, None)
+    assert torch.equal(got[:2], got[2:4]) and ((got.double() - want).abs() <= tol).all() and status() == 0
+
+
+def test_largest_window_and_first_tokens():
+    big = 2 ** 31 - 1
+    st = Setup([2, 20], [3, 300], 1, 64, 16, "i8")
+    q = torch.randn((22, 2, 64), generator=gen(1), device="cuda")
+    for mr, rs in ((20, st.row_start), (2, torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda"))):
+        a, b, c = (K_.attn_paged(q, st.pool, st.table, rs, st.kv_len, max_rows=mr, max_kv=300, window=w, n_sink=k)[0] for w, k in ((0, 0), (big, big), (big, 0)))
+        n = int(rs[-1])
+        assert status() == 0 and torch.equal(b[:n], c[:n])
+        assert ((a[:n] - b[:n]).abs() <= 1e-5 * a[:n].abs().amax()).all()   # other splits: the same but for rounding
+
+
 def test_rows_without_a_key_and_rows_behind_the_last():
     st = Setup([3, 1, 2], [1, 0, 40], 1, 64, 16, "i8", cols=3)
     q = torch.randn((20, 4, 64), generator=gen(2), device="cuda")
@@ -495,6 +525,74 @@ def test_captured_steps_replay_with_other_lengths():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, step())
+    assert status() == 0
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    code = ("import torch\n"
+            "from hipster_b200 import kernels as K\n"
+            "pool = K.KVPages.empty(4, 1, 16, 64)\n"
+            "i = lambda x: torch.tensor(x, dtype=torch.int32, device='cuda')\n"
+            "t, rs, kl = i([[0, 1]]), i([0, 1]), i([20])\n"
+            "x = torch.randn((1, 1, 64), device='cuda')\n"
+            "torch.cuda.synchronize()\n"
+            "g = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(g):\n"
+            "    rope = K.rope_table(32, 64, 1e4)\n"
+            "    q = K.kv_append(pool, x, x, t, rs, kl, rope, q=x)\n"
+            "    y, _ = K.attn_paged(q, pool, t, rs, kl, max_rows=1, max_kv=20)\n"
+            "    k, v = K.kv_read(pool, t, rs, kl, R=1)\n"
+            "g.replay()\n"
+            "torch.cuda.synchronize()\n"
+            "K.device_status()\n"
+            "z, _ = K.attn_paged(q, pool, t, rs, kl, max_rows=1, max_kv=20)\n"
+            "assert torch.equal(y, z) and (v.float() - x).abs().max() < 0.02 * x.abs().max()\n"
+            "print('fine')\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+def test_captured_prompts():
+    st = Setup([40, 3], [90, 40], 2, 64, 16, "i8", cols=7, spare=6)
+    for s in range(2):
+        for c in range(7):
+            if st.table[s, c] < 0:
+                st.table[s, c] = st.spare.pop()
+    q = torch.randn((43, 4, 64), generator=gen(1), device="cuda")
+    step = lambda: K_.attn_paged(q, st.pool, *st.batch, max_rows=40, max_kv=112)[0]  # noqa: E731
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = step()
+    for i in range(5):
+        st.kv_len += 4
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, step())
+    assert status() == 0
+
+
+def test_refusals_of_the_python_calls():
+    st = Setup([2], [20], 2, 64, 16, "i8")
+    q = torch.randn((2, 4, 64), device="cuda")
+    kv = q[:, :2]
+    rope = K_.rope_table(32, 64, 1e4)
+    t, rs, kl = st.batch
+    cpu = K_.KVPages.empty(2, 2, 16, 64, device="cpu")
+    bad = [lambda: K_.attn_paged(q, cpu, t, rs, kl, 2, 20), lambda: K_.attn_paged(q, st.pool, t.cpu(), rs, kl, 2, 20), lambda: K_.attn_paged(q, st.pool, t, rs.long(), kl, 2, 20),
+           lambda: K_.attn_paged(q, st.pool, t, rs[:1], kl, 2, 20), lambda: K_.attn_paged(q, st.pool, t.expand(2, -1), rs, kl, 2, 20), lambda: K_.attn_paged(q.half(), st.pool, t, rs, kl, 2, 20),
+           lambda: K_.attn_paged(q[..., :32], st.pool, t, rs, kl, 2, 20), lambda: K_.attn_paged(q.transpose(1, 2).contiguous().transpose(1, 2), st.pool, t, rs, kl, 2, 20), lambda: K_.attn_paged(q.cpu(), st.pool, t, rs, kl, 2, 20),
+           lambda: K_.attn_paged(q[:, :3], st.pool, t, rs, kl, 2, 20), lambda: K_.attn_paged(q, st.pool, t, rs, kl, 2, 20, gate=q[:, :2]), lambda: K_.attn_paged(q, st.pool, t, rs, kl, 0, 20),
+           lambda: K_.attn_paged(q, st.pool, t, rs, kl, 2, 20, n_sink=3), lambda: K_.attn_paged(q, st.pool, t, rs, kl, 2, 20, want_f32=False),
+           lambda: K_.kv_append(st.pool, q, q, t, rs, kl), lambda: K_.kv_append(st.pool, kv, kv[:1], t, rs, kl), lambda: K_.kv_append(st.pool, kv, kv, t, rs, kl, rope.half()), lambda: K_.kv_append(st.pool, kv, kv, t, rs, kl, rope[:, ::2]),
+           lambda: K_.kv_append(st.pool, kv, kv, t, rs, kl, K_.rope_table(32, 128, 1e4)), lambda: K_.kv_append(st.pool, kv, kv, t, rs, kl, rope, q=q, q_out=q[:, :2]), lambda: K_.kv_append(st.pool, kv, kv, t, rs, kl, q_norm=q[0, 0]),
+           lambda: K_.kv_append(st.pool, kv, kv, t, rs, kl, k_norm=torch.ones(64, dtype=torch.float16, device="cuda")), lambda: K_.kv_read(st.pool, t, rs, kl), lambda: K_.kv_read(st.pool, t, rs, kl, R=0),
+           lambda: K_.kv_read(st.pool, t, rs, kl, k_out=kv.half()), lambda: K_.kv_read(st.pool, t, rs, kl, k_out=kv, v_out=kv), lambda: K_.rope_table(0, 64, 1e4), lambda: K_.rope_table(8, 64, -1.0), lambda: K_.rope_table(8, 64, 1e4, device="cpu")]
+    for i, f in enumerate(bad):
+        with pytest.raises(hb.HipsterError):
+            f()
+            pytest.fail(f"call {i} was not refused")
     assert status() == 0
 
 
