@@ -7,7 +7,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("HIPSTER_B200_LIB") or os.path.join(HERE, "libhipster_b200.so")
 HEADER = os.path.join(HERE, "..", "include", "hipster_b200.h")
 
-_lib = _hot = None
+_lib = _hot = _tensor_calls = None
 # the calls whose latency counts, with their argument types (p pointer, i int, l long long, f float, d double), so that integers pass without a wrapper object
 _TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float, "d": ctypes.c_double}
 _HOT = {"hp_quantize_x_q8": "piiippp", "hp_gemv_q4k_q8": "ppppiiiip", "hp_argmax": "piiipppp", "hp_accept_greedy": "ppipp", "hp_attn_decode": "piiiiiipppppipppfpp",
@@ -60,6 +60,25 @@ def hot():
                 calls.bind(name, ctypes.cast(getattr(L, name), ctypes.c_void_p).value)
         _hot = calls
     return _hot
+
+
+def tensors():
+    """The paged-cache calls on torch tensors (csrc/pytensors.cpp), bound to the library that is loaded here; None where the module was not built, or for another torch."""
+    global _tensor_calls
+    if _tensor_calls is None:
+        import torch
+        L = lib()
+        try:
+            from . import _tensors as calls
+        except ImportError:
+            calls = None
+        if calls is not None and torch.__version__.split("+")[0] == calls.torch:
+            for name in ("hp_kv_append", "hp_kv_read", "hp_attn_paged", "hp_attn_paged_workspace_bytes", "hp_rope_table"):
+                calls.bind(name, ctypes.cast(getattr(L, name), ctypes.c_void_p).value)
+            _tensor_calls = calls
+        else:
+            _tensor_calls = False
+    return _tensor_calls or None
 
 
 def check(code):

@@ -63,6 +63,7 @@ def build(verbose=False, force=False):
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
     build_calls(force)
+    build_tensors(force)
     build_driver(force)
     return LIB
 
@@ -87,6 +88,33 @@ def build_calls(force=False):
                 os.remove(CALLS)
             return None
     return CALLS
+
+
+TENSORS_SRC = os.path.join(CSRC, "pytensors.cpp")
+TENSORS = os.path.join(HERE, "_tensors" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_tensors(force=False):
+    """The paged-cache calls on torch tensors in C++: linked with torch, not with the library. Without a compiler or torch's headers there are none (None), and the
+    package takes these calls in Python."""
+    if force or _stale(TENSORS, [TENSORS_SRC, os.path.join(HERE, "..", "include", "hipster_b200.h")]):
+        try:
+            import torch
+            home = os.path.dirname(torch.__file__)
+            inc, lib = os.path.join(home, "include"), os.path.join(home, "lib")
+            cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", inc,
+                   "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"), "-isystem", "/usr/local/cuda/include", "-I", sysconfig.get_paths()["include"], TENSORS_SRC, "-o", TENSORS,
+                   "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+            r = subprocess.run(cmd, capture_output=True, text=True)
+            failed = r.returncode != 0 and r.stdout + r.stderr
+        except (ImportError, AttributeError, OSError) as e:
+            failed = f"{e}\n"
+        if failed:
+            sys.stderr.write(failed + "the calls on torch tensors were not built: they go through Python\n")
+            if os.path.exists(TENSORS):
+                os.remove(TENSORS)
+            return None
+    return TENSORS
 
 
 DRIVER_SRC = os.path.join(HERE, "driver", "spec_driver.cpp")

@@ -5,7 +5,7 @@ import functools
 
 import torch
 
-from ._lib import HipsterError, lib, hot, check, ptr
+from ._lib import HipsterError, lib, hot, tensors, check, ptr
 
 # The calls below are a few microseconds of device work, so what they spend in Python counts: the handle of the current stream
 # comes without a Stream object around it, the short calls go through native entry points that take addresses as integers (_lib.hot; to
@@ -197,7 +197,8 @@ class KVPages:
         return cls(*codes, *(torch.zeros((n_pages, n_kv, page_size), dtype=torch.float32, device=device) for _ in range(2)))
 
 
-# The checks below run on every call of a few microseconds, hence one reading of each attribute and no message before a test fails.
+# Calls whose arguments are in order are taken by _lib.tensors(), in C++ (None: not taken). What follows takes the others, says what is wrong with them, and takes all calls
+# where that module was not built: it, too, reads each attribute once and makes no message before a test fails.
 def _batch(pages, table, row_start, kv_len):
     """Checks what describes a ragged batch; -> number of sequences, and its addresses as the calls take them."""
     dev, S = pages._dev, kv_len.numel()
@@ -229,6 +230,11 @@ def rope_table(n_pos, n_rot, base, scaling=None, factor=1.0, orig_ctx=0, beta_fa
     by parts: those that turn less than beta_slow times over orig_ctx positions wholly, those over beta_fast times not."""
     if scaling not in _SCALING:
         raise HipsterError(1, f"rope_table: unknown scaling {scaling!r}")
+    fast = device == "cuda" and tensors()
+    if fast:
+        out = fast.rope_table(n_pos, n_rot, base, _SCALING[scaling], factor, orig_ctx, beta_fast, beta_slow, attn_factor)
+        if out is not None:
+            return out
     if n_pos < 1 or n_rot < 2:
         raise HipsterError(1, f"rope_table: bad shape n_pos={n_pos} n_rot={n_rot}")
     out = torch.empty((n_pos, n_rot // 2, 2), dtype=_F32, device=device)
@@ -250,6 +256,11 @@ def kv_append(pages, k, v, table, row_start, kv_len, rope=None, q=None, q_out=No
     """Appends rows k, v f32 [R][n_kv][head_dim] of a ragged batch to their sequences' pages, k normalised (k_norm bf16 [head_dim]) and rotated by rope
     f32 [n_pos][n_rot / 2][2]. q [R][n_head][head_dim] is normalised and rotated alike. -> q_out (f32 [R][n_head][head_dim]; None without q).
     Rows row_start[s] .. row_start[s + 1] - 1 are the newest of the kv_len[s] tokens of sequence s."""
+    fast = tensors()
+    if fast:
+        out = fast.kv_append(pages._at, pages._dev, k, v, table, row_start, kv_len, rope, q, q_out, interleaved, q_norm, k_norm, eps)
+        if out is not None:
+            return None if out is True else out
     S, *at = _batch(pages, table, row_start, kv_len)
     R, n_kv = k.shape[0], pages.n_kv
     qr = qo = (None, 0, 0)
@@ -274,6 +285,11 @@ def kv_append(pages, k, v, table, row_start, kv_len, rope=None, q=None, q_out=No
 def kv_read(pages, table, row_start, kv_len, R=None, k_out=None, v_out=None):
     """The tokens of the rows back as f16 -> k, v [R][n_kv][head_dim]. With kv_len[s] rows for each sequence whole caches; k_out, v_out may be views with other
     strides, as cache.transpose(0, 1) of an f16 [n_kv][max_ctx][256] cache for attn_decode."""
+    fast = k_out is None and v_out is None and tensors()
+    if fast:
+        out = fast.kv_read(pages._at, pages._dev, table, row_start, kv_len, R)
+        if out is not None:
+            return out
     S, *at = _batch(pages, table, row_start, kv_len)
     n_kv, D = pages.n_kv, pages.head_dim
     if k_out is None and v_out is None and R is not None:
@@ -299,6 +315,11 @@ def attn_paged(q, pages, table, row_start, kv_len, max_rows, max_kv, scale=None,
     """Attention of rows q f32 [R][n_head][head_dim] over their sequences' pages (causal; window > 0: the last `window` tokens and the first n_sink), times sigmoid(gate)
     where a gate [R][n_head][head_dim] is given. scale: 1 / sqrt(head_dim). max_rows, max_kv bound the rows and tokens of a sequence.
     -> (out f32 [R][n_head][head_dim] or None, XQ8 of its rows or None)."""
+    fast = want_f32 and not want_q8 and tensors()
+    if fast:
+        out = fast.attn_paged(pages._at, pages._dev, q, gate, table, row_start, kv_len, max_rows, max_kv, scale, window, n_sink)
+        if out is not None:
+            return out, None
     (S, *at), (R, n_head, D) = _batch(pages, table, row_start, kv_len), q.shape
     qr = _rows(q, pages, R, n_head, "q")
     gr = (None, 0, 0) if gate is None else _rows(gate, pages, R, n_head, "gate")

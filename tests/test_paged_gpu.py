@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import hipster_b200 as hb
-from hipster_b200 import kernels as K_
+from hipster_b200 import _lib, kernels as K_
 
 pytestmark = pytest.mark.gpu
 
@@ -573,7 +573,39 @@ def test_captured_prompts():
     assert status() == 0
 
 
-def test_refusals_of_the_python_calls():
+@pytest.fixture(params=["native", "python"])
+def form(request, monkeypatch):
+    """The calls in C++ where they were built (they are, here), and without them."""
+    assert _lib.tensors() is not None
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_tensor_calls", False)
+    return request.param
+
+
+def test_both_forms_of_the_calls(form):
+    st = Setup([3, 0, 18], [50, 7, 200], 2, 128, 16, "e4m3")
+    g = gen(2)
+    x = torch.randn((23, 8, 128), generator=g, device="cuda")   # two rows behind the last
+    rope = K_.rope_table(300, 64, 1e4, "yarn", factor=4, orig_ctx=64)
+    assert torch.equal(rope, K_.rope_table(300, 64, 1e4, "yarn", factor=4.0, orig_ctx=64, beta_fast=32, beta_slow=1.0, attn_factor=0))
+    w = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    into = torch.full((23, 4, 256), 2.0, device="cuda")[..., :128]
+    q = K_.kv_append(st.pool, x[:, 4:6], x[:, 6:], *st.batch, rope, q=x[:, :4], q_out=into, interleaved=True, q_norm=w, k_norm=w.view(torch.int16))
+    assert q.data_ptr() == into.data_ptr() and (q[21:] == 2).all()
+    assert torch.equal(K_.kv_append(st.pool, x[:, 4:6], x[:, 6:], *st.batch, rope, q=x[:, :4], interleaved=1, q_norm=w, k_norm=w)[:21], q[:21])
+    assert K_.kv_append(st.pool, x[:, 4:6], x[:, 6:], *st.batch, rope, interleaved=True, k_norm=w) is None
+    k, v = K_.kv_read(st.pool, *st.batch, R=21)
+    a, xq = K_.attn_paged(q, st.pool, *st.batch, max_rows=18, max_kv=200, window=60, n_sink=2, gate=x[:, :4])
+    b, xr = K_.attn_paged(q, st.pool, *st.batch, max_rows=18, max_kv=200, scale=128 ** -0.5, window=60, n_sink=2, gate=x[:, :4], want_q8=True)
+    assert xq is None and torch.equal(a[:21], b[:21]) and k.shape == v.shape == (21, 2, 128) and status() == 0
+    have = torch.cat([q[:21].flatten(), k.float().flatten(), v.float().flatten(), a[:21].flatten()])
+    if form == "native":
+        test_both_forms_of_the_calls.seen = have
+    else:
+        assert torch.equal(have, test_both_forms_of_the_calls.seen)
+
+
+def test_refusals_of_the_python_calls(form):
     st = Setup([2], [20], 2, 64, 16, "i8")
     q = torch.randn((2, 4, 64), device="cuda")
     kv = q[:, :2]
