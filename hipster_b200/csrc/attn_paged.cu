@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     __shared__ float s_c[MB];   // factor of a pair's scores
     __shared__ int s_pos[MB];   // position of a pair's row, -1: none
     __shared__ float s_mu[KW][MB], s_l[KW][MB];
+    __shared__ float* s_out[MB];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
     pdl_wait();
     pdl_launch_dependents();   // behind the wait: what was enqueued in front of this kernel is complete when the merge starts
@@ -71,6 +72,18 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     {   // is any slice of the split visible?
         const int i0 = (int)(sp.u0 / KS);
         if ((i0 * KS >= sp.sink && i0 < i_lo ? i_lo : i0) >= i_end) return;
+    }
+    // q: a warp per pair, 8 dims per lane; under way while the pages are looked up
+    constexpr int QP = MB / KW;
+    float4 qv[QP][2];
+#pragma unroll
+    for (int u = 0; u < QP; ++u) {
+        const int i = warp + KW * u, p = blk.p0 + i, t = p / a.G;
+        qv[u][0] = qv[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < blk.np && lane < D / 8) {
+            const float4* src = reinterpret_cast<const float4*>(a.q + (size_t)(sq.row0 + t) * a.q_ld + (size_t)(kh * a.G + p - t * a.G) * a.q_hs) + 2 * lane;
+            qv[u][0] = src[0]; qv[u][1] = src[1];
+        }
     }
     const int lg = a.pool.lg_page, pmask = (1 << lg) - 1;
     // the pool's row of a slice's first key; 0 behind the end, and for a page number out of range (told by the status word). The number is fetched a slice ahead
@@ -119,19 +132,15 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     auto scales = [&](uint32_t r) { return sbase[r]; };
     float sc = i0 < i_end ? scales(r0) : 0.f;
 
-    // ---- q: a warp per pair; the 8 dims of a lane are its words of two steps of 16 dims, values and rests
-    for (int i = warp; i < MB; i += KW) {
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        uint32_t m = 0;
-        const bool live = i < blk.np;
-        const int p = blk.p0 + i, t = live ? p / a.G : 0;
-        if (live && lane < D / 8) {
-            const float4* src = reinterpret_cast<const float4*>(a.q + (size_t)(sq.row0 + t) * a.q_ld + (size_t)(kh * a.G + p - t * a.G) * a.q_hs) + 2 * lane;
-            const float4 x0 = src[0], x1 = src[1];
-            x[0] = x0.x; x[1] = x0.y; x[2] = x0.z; x[3] = x0.w; x[4] = x1.x; x[5] = x1.y; x[6] = x1.z; x[7] = x1.w;
+    // the 8 dims of a lane are its words of two steps of 16 dims, values and rests
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
-        }
+    for (int u = 0; u < QP; ++u) {
+        const int i = warp + KW * u, t = (blk.p0 + i) / a.G;
+        const float x[8] = {qv[u][0].x, qv[u][0].y, qv[u][0].z, qv[u][0].w, qv[u][1].x, qv[u][1].y, qv[u][1].z, qv[u][1].w};
+        const bool live = i < blk.np;
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
         m = __reduce_max_sync(0xffffffffu, m);
         const int e = q_exponent(m);
         const float up = __uint_as_float((uint32_t)(e + 127) << 23);
@@ -327,22 +336,29 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             if (g == 0) { s_mu[warp][8 * n + 2 * q4 + c] = mu[n][c]; s_l[warp][8 * n + 2 * q4 + c] = l[n][c]; }
         }
     __syncthreads();
-    for (int i = warp; i < blk.np; i += KW) {   // a warp per pair
-        const int p = blk.p0 + i, t = p / a.G;
-        if (s_pos[i] < 0) continue;
-        float w[KW], m = -INFINITY, ls = 0.f;
+    if (tid < blk.np) {   // a thread per pair: the warps' factors, the weights' sum, and where the sums go
+        const int p = blk.p0 + tid, t = p / a.G;
+        float m = -INFINITY, ls = 0.f;
 #pragma unroll
-        for (int k = 0; k < KW; ++k) m = fmaxf(m, s_mu[k][i]);
+        for (int k = 0; k < KW; ++k) m = fmaxf(m, s_mu[k][tid]);
 #pragma unroll
-        for (int k = 0; k < KW; ++k) { w[k] = pow2i(s_mu[k][i] - m); ls = fmaf(s_l[k][i], w[k], ls); }
+        for (int k = 0; k < KW; ++k) { const float w = pow2i(s_mu[k][tid] - m); s_mu[k][tid] = w; ls = fmaf(s_l[k][tid], w, ls); }
+        const bool live = s_pos[tid] >= 0;
         const size_t at = ((size_t)(sq.row0 + t) * a.n_head + kh * a.G + p - t * a.G) * (a.ns + a.nwin) + blockIdx.x;
-        for (int d = 2 * lane; d < D; d += 64) {
-            float2 o = make_float2(0.f, 0.f);
+        s_out[tid] = live ? a.pO + at * D : nullptr;
+        if (live) a.pml[at] = make_float2(m, ls);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int e = tid; e < blk.np * (D / 4); e += 32 * KW) {
+        const int i = e / (D / 4), d = e % (D / 4) * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < KW; ++k) { const float2 v = *reinterpret_cast<const float2*>(xo + (size_t)(k * MB + i) * XS + d); o.x = fmaf(v.x, w[k], o.x); o.y = fmaf(v.y, w[k], o.y); }
-            *reinterpret_cast<float2*>(a.pO + at * D + d) = o;
+        for (int k = 0; k < KW; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(xo + (size_t)(k * MB + i) * XS + d); const float w = s_mu[k][i];
+            o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
         }
-        if (lane == 0) a.pml[at] = make_float2(m, ls);
+        if (s_out[i]) *reinterpret_cast<float4*>(s_out[i] + d) = o;
     }
 }
 
