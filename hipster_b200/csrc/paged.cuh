@@ -48,12 +48,12 @@ struct PagedArgs {
     int window, n_sink;
     int U, ns, nwin;            // keys of a split, splits of the first tokens, splits behind them
     float* pO; float2* pml;     // partials [row][head][ns + nwin] (x head_dim): sums, (mu, sum of weights)
-    uint8_t* f16; int tiles;    // prompts: tiles of 128 tokens in f16, [sequence][kv head][tiles][k, v]
+    uint8_t* f16; int tiles;    // prompts: tiles of 64 tokens in f16, [sequence][kv head][tiles][k, v, scales]
     int* err; int* arg_err;
 };
 
 // Prompts, calls of more than PAGED_DECODE_ROWS rows per sequence: blocks of PAGED_TC_PAIRS pairs, and the bytes of their f16 tiles
-constexpr int PAGED_DECODE_ROWS = 16, PAGED_TC_PAIRS = 48;
+constexpr int PAGED_DECODE_ROWS = 16, PAGED_TC_PAIRS = 128;
 size_t attn_paged_tc_bytes(const PagedPool& pool, const PagedBatch& b);
 int attn_paged_tc(PagedArgs& a, dim3 grid, cudaStream_t s);
 

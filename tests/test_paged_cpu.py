@@ -108,8 +108,8 @@ def test_workspace_sizes():
     assert f(ld=1024, mk=1000) == up(8 * 4 * 2 * part)       # two of 512
     assert f(w=200) == up(8 * 4 * 2 * part)                  # a run of up to 201 keys lies in two splits
     assert f(w=200, k=3) == up(8 * 4 * 3 * part)             # and the first tokens in one more
-    tiles = lambda mk: 4 * 2 * -(-mk // 128) * 2 * 128 * 64 * 2  # noqa: E731
-    assert f(R=4000, mr=1000, w=100) == up(4000 * 4 * part) + tiles(1000)   # prompts: keys and values in f16; a window in one split
+    tiles = lambda mk: 4 * 2 * -(-mk // 64) * 2 * 64 * (64 * 2 + 4)  # noqa: E731
+    assert f(R=4000, mr=1000, w=100) == up(4000 * 4 * part) + tiles(1000)   # prompts: keys and values in f16 with their scales; a window in one split
     assert all(f(R=600, mr=300, mk=m) <= f(R=600, mr=300, mk=(m + 1023) // 1024 * 1024) for m in range(1, 5000, 37))
     assert all(f(mk=m) <= f(mk=m + 1) and f(mk=m, w=300, k=5) <= f(mk=m + 1, w=300, k=5) for m in range(1, 1500, 7))
     assert f(p=pages(type=9)) == 0 and f(nh=3) == 0 and f(k=1) == 0
