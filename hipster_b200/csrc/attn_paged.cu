@@ -15,6 +15,7 @@
 // slice's keys at fixed lanes and warps: a row's bits depend neither on the other rows of the call nor on the other sequences.
 #include "paged.cuh"
 #include <algorithm>
+#include <type_traits>
 
 namespace hp {
 namespace {
@@ -419,6 +420,68 @@ __global__ void __launch_bounds__(256) k_paged_merge(const MergeArgs a) {
     if (a.oq) warp_quant32_store(x, r, (head * D + d) >> 5, a.n_head * D, a.oq, a.osc, lane);
 }
 
+// The same sums, bit for bit, where a row has at most eight splits: a thread for four dims over all splits, 1024 dims of a row's heads per block. k_paged_merge's blocks, a head each,
+// are bound by their instructions and start-up once there are thousands of them. 509 rows of 24 heads in three splits (cold, us): 51 there, 27 here.
+constexpr int FEW = 8;
+template <int D>
+__global__ void __launch_bounds__(256) k_paged_merge_few(const MergeArgs a) {
+    constexpr int HEADS = 1024 / D, SETS = 1024 / D < FEW ? 1024 / D : FEW;   // sums of k_paged_merge's sets
+    const int per = (a.n_head + HEADS - 1) / HEADS, r = blockIdx.x / per, h = (blockIdx.x - r * per) * HEADS + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4, lane = threadIdx.x & 31;
+    const PagedSeq q = paged_find(a.b, r, lane, a.err);
+    const bool live = q.s >= 0 && h < a.n_head;
+    float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.gate && live) gate = *reinterpret_cast<const float4*>(a.gate + (size_t)r * a.g_ld + (size_t)h * a.g_hs + d);
+    pdl_wait();
+    pdl_launch_dependents();
+    if (!__any_sync(0xffffffffu, live)) return;   // 64 dims: a warp has two heads
+    const int pos = live ? q.len - q.T + r - q.row0 : -1;
+    const int lo = a.window ? max(0, pos - a.window + 1) : 0, w0 = max(a.ns, lo / a.U), w1 = max(pos, 0) / a.U;
+    const int s1 = a.ns ? (min(a.n_sink, pos + 1) + a.U - 1) / a.U : 0;   // splits [0, s1) and [w0, w1]
+    const int n = pos < 0 ? 0 : s1 + max(0, w1 - w0 + 1), first = (w0 - a.ns) % a.nwin;
+    const size_t base = ((size_t)r * a.n_head + h) * (a.ns + a.nwin);
+    auto slot = [&](int i) { const int k = first + i - s1; return base + (i < s1 ? i : a.ns + (k < a.nwin ? k : k - a.nwin)); };
+    float2 ml[FEW];
+    float mu = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < FEW; ++i) if (i < n) { ml[i] = a.pml[slot(i)]; mu = fmaxf(mu, ml[i].x); }
+    float4 o[SETS]; float l[SETS];
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) { o[i] = make_float4(0.f, 0.f, 0.f, 0.f); l[i] = 0.f; }
+#pragma unroll
+    for (int i0 = 0; i0 < FEW; i0 += 4) {
+        if (i0 >= n) break;
+        float4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (i0 + j < n) v[j] = *reinterpret_cast<const float4*>(a.pO + slot(i0 + j) * D + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i0 + j < n) {
+                const float w = pow2i(ml[i0 + j].x - mu);
+                float4& t = o[(i0 + j) % SETS];
+                t.x = fmaf(w, v[j].x, t.x); t.y = fmaf(w, v[j].y, t.y); t.z = fmaf(w, v[j].z, t.z); t.w = fmaf(w, v[j].w, t.w); l[(i0 + j) % SETS] = fmaf(w, ml[i0 + j].y, l[(i0 + j) % SETS]);
+            }
+    }
+    float x[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) { x[0] = x[0] + o[i].x; x[1] = x[1] + o[i].y; x[2] = x[2] + o[i].z; x[3] = x[3] + o[i].w; ls = ls + l[i]; }
+    const float g[4] = {gate.x, gate.y, gate.z, gate.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[e] = ls == 0.f ? 0.f : x[e] * a.mul / ls;
+        if (a.gate) x[e] = x[e] * sigmoid_det(g[e]);
+    }
+    if (a.out && live) *reinterpret_cast<float4*>(a.out + ((size_t)r * a.n_head + h) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+    if (a.oq) {   // runs of 32 dims lie in eight lanes: a run at a time to all lanes
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int from = 8 * b + (lane >> 2), at = __shfl_sync(0xffffffffu, live ? h * D + d : -1, 8 * b);
+            if (at < 0) continue;
+            const float y0 = __shfl_sync(0xffffffffu, x[0], from), y1 = __shfl_sync(0xffffffffu, x[1], from), y2 = __shfl_sync(0xffffffffu, x[2], from), y3 = __shfl_sync(0xffffffffu, x[3], from);
+            warp_quant32_store((lane & 2) ? (lane & 1 ? y3 : y2) : (lane & 1 ? y1 : y0), r, at >> 5, a.n_head * D, a.oq, a.osc, lane);
+        }
+    }
+}
+
 struct Plan { int U, ns, nwin, MB; long long blocks; };
 // Splits lie at multiples of U, which the cache's capacity and the window alone decide (16 to 32 splits and more of a full sequence), so that a row's sums do not hang on what
 // else is in the call. Captured, us: 1 token of 24 heads at 4097, U = 128 13.3, 256 13.3, 512 17.4, 1024 27.7; 48 sequences of up to 8192, 197, 146, 124, 124.
@@ -487,9 +550,13 @@ int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams
     if (rc != HP_OK) return rc;
     MergeArgs m; m.b = b; m.pO = a.pO; m.pml = a.pml; m.gate = p.gate; m.g_ld = p.g_ld; m.g_hs = p.g_hs; m.n_head = p.n_head; m.window = p.window; m.n_sink = p.n_sink;
     m.U = pl.U; m.ns = pl.ns; m.nwin = pl.nwin; m.mul = pool.kind == KV_E4M3 ? 256.f : 1.f; m.out = p.out; m.oq = (int8_t*)p.xq.q; m.osc = (float*)p.xq.sc; m.err = a.arg_err;
-    const dim3 mg((unsigned)(b.R * p.n_head));
-    HP_CUDA(pool.head_dim == 256 ? launch_pdl<4>(k_paged_merge<256>, mg, dim3(256), 0, s, m) : pool.head_dim == 128 ? launch_pdl<4>(k_paged_merge<128>, mg, dim3(256), 0, s, m)
-                                                                                                   : launch_pdl<4>(k_paged_merge<64>, mg, dim3(256), 0, s, m));
+    const bool wide = (((uintptr_t)p.gate | (uintptr_t)p.out) & 15) == 0 && (!p.gate || ((p.g_ld | p.g_hs) & 3) == 0);   // four dims of gate and output at a time
+    auto merge = [&](auto dims) {
+        constexpr int D = decltype(dims)::value, HPB = 1024 / D;
+        if (pl.ns + pl.nwin <= FEW && wide) return launch_pdl<4>(k_paged_merge_few<D>, dim3((unsigned)(b.R * ((p.n_head + HPB - 1) / HPB))), dim3(256), 0, s, m);
+        return launch_pdl<4>(k_paged_merge<D>, dim3((unsigned)(b.R * p.n_head)), dim3(256), 0, s, m);
+    };
+    HP_CUDA(pool.head_dim == 256 ? merge(std::integral_constant<int, 256>()) : pool.head_dim == 128 ? merge(std::integral_constant<int, 128>()) : merge(std::integral_constant<int, 64>()));
     return HP_OK;
 }
 

@@ -83,7 +83,8 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
         float c[MB], alpha[4][MB];   // factor of a pair's scores; rescaling by tile
         float top[2][MB];            // by half of the keys: a pair's largest logarithm where a reference may move
         float end[MB];               // sums of the weights of the second halves
-        int pos[MB], at[MB];         // a pair's position, -1: none; row * n_head + head, -1: nothing to write
+        long long from[MB];          // a pair's row of q, -1: none
+        int pos[MB], at[MB];         // its position, -1: none; row * n_head + head, -1: nothing to write
         int moved[4][4];             // by tile and warp: the tile's number + 1 where a reference moves, and alpha holds
     };
     static_assert(sizeof(Shared) <= Geo::X_BYTES, "");
@@ -114,21 +115,27 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_ptr)), "n"(Geo::TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (tid < MB) {
+        const int p = blk.p0 + tid, t = p / a.G, head = kh * a.G + p - t * a.G, pos = tid < np ? max(-1, sq.len - sq.T + t) : -1;
+        x.from[tid] = tid < np ? (long long)((size_t)(sq.row0 + t) * a.q_ld + (size_t)head * a.q_hs) : -1;
+        x.pos[tid] = pos; x.at[tid] = pos >= 0 ? (sq.row0 + t) * a.n_head + head : -1;
+    }
+    __syncthreads();
     // q: a warp per pair, 8 dims per lane, a warp's pairs all in flight; rests to their place, values to that of k, on their way to accumulator memory
     if (warp < 16) {
         float4 v[MB / 16][2];
 #pragma unroll
         for (int u = 0; u < MB / 16; ++u) {
-            const int i = warp + u * 16, p = blk.p0 + i, t = p / a.G;
+            const long long from = x.from[warp + u * 16];
             v[u][0] = v[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (i < np && lane < D / 8) {
-                const float4* src = reinterpret_cast<const float4*>(a.q + (size_t)(sq.row0 + t) * a.q_ld + (size_t)(kh * a.G + p - t * a.G) * a.q_hs) + 2 * lane;
+            if (from >= 0 && lane < D / 8) {
+                const float4* src = reinterpret_cast<const float4*>(a.q + from) + 2 * lane;
                 v[u][0] = src[0]; v[u][1] = src[1];
             }
         }
 #pragma unroll
         for (int u = 0; u < MB / 16; ++u) {
-            const int i = warp + u * 16, p = blk.p0 + i, t = p / a.G;
+            const int i = warp + u * 16;
             const float y[8] = {v[u][0].x, v[u][0].y, v[u][0].z, v[u][0].w, v[u][1].x, v[u][1].y, v[u][1].z, v[u][1].w};
             uint32_t m = 0;
 #pragma unroll
@@ -149,12 +156,7 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
                 *reinterpret_cast<uint4*>(sm + Geo::OFF_K + at) = make_uint4(h[0], h[1], h[2], h[3]);
                 *reinterpret_cast<uint4*>(sm + Geo::OFF_Q + at) = make_uint4(r[0], r[1], r[2], r[3]);
             }
-            if (lane == 0) {
-                const int pos = i < np ? max(-1, sq.len - sq.T + t) : -1;
-                x.c[i] = a.scale2 * __uint_as_float((uint32_t)(127 - e) << 23);
-                x.pos[i] = pos;
-                x.at[i] = pos >= 0 ? (sq.row0 + t) * a.n_head + kh * a.G + p - t * a.G : -1;
-            }
+            if (lane == 0) x.c[i] = a.scale2 * __uint_as_float((uint32_t)(127 - e) << 23);
         }
     }
     tc_fence_before();

@@ -689,3 +689,22 @@ def test_a_sequence_from_prompt_to_rejected_drafts():
     exact, tol = attn64(st, q, 1 / 16, 0, 0, gate)
     assert ((got.double() - exact).abs() <= tol).all() and k8.isfinite().all() and v8.isfinite().all()
     assert float((want.view(1, H, D).double() - exact).norm() / exact.norm()) < 0.05
+
+
+@pytest.mark.parametrize("D,H,n_kv", [(64, 5, 1), (128, 3, 3), (256, 6, 2)])
+@pytest.mark.parametrize("rows,lens,window,n_sink", [([3, 0, 1, 2], [700, 10, 1, 300], 0, 0), ([3, 1, 2], [900, 40, 513], 300, 20), ([40, 3, 0], [600, 3, 9], 0, 0), ([40, 19], [600, 777], 200, 5)])
+def test_gates_and_outputs_at_odd_places(D, H, n_kv, rows, lens, window, n_sink):
+    # the merge reads gates four at a time where they lie so, and one at a time elsewhere: the same bits, quantised rows too. The last row has no key.
+    lens = [*lens, 0]
+    rows = [*rows, 1]
+    st = Setup(rows, lens, n_kv, D, 16, "e4m3", 3)
+    g = gen(7)
+    q = torch.randn((st.R, H, D), generator=g, device="cuda")
+    gate = torch.randn((st.R, H, D), generator=g, device="cuda")
+    odd = torch.zeros(st.R * (H * (D + 1) + 2) + 1, device="cuda")[1:].as_strided((st.R, H, D), (H * (D + 1) + 2, D + 1, 1))
+    odd.copy_(gate)
+    run = lambda x: K_.attn_paged(q, st.pool, *st.batch, max_rows=max(rows), max_kv=max(lens), window=window, n_sink=n_sink, gate=x, want_q8=True)  # noqa: E731
+    (a, xa), (b, xb) = run(gate), run(odd)
+    assert torch.equal(a, b) and torch.equal(xa.q, xb.q) and torch.equal(xa.sc, xb.sc)
+    exact, tol = attn64(st, q, D ** -0.5, window, n_sink, gate)
+    assert ((a.double() - exact).abs() <= tol).all() and (a[-1] == 0).all()
