@@ -62,7 +62,7 @@ __device__ __forceinline__ void ld_there(float* a) {   // orders the use of the 
 #pragma unroll
     for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(a[i]));
 }
-// Registers: 640 threads start with 96 each, 61440; eight warps with 160, eight with 64 and four with 32 take all of them
+// Registers: 640 threads start with 96 each, 61440; eight warps with 152, eight with 72 and four with 32 take all of them (160 and 64: 157 us where this takes 151)
 template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void pair_sync(int qt) { asm volatile("bar.sync %0, 64;" ::"r"(qt + 1) : "memory"); }
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
     bool ok = true;
 
     if (warp < 8) {   // ---- weights: two warps share 32 pairs, a thread has half of the keys of one
-        regs_less<64>();
+        regs_less<72>();
         const int half = warp >> 2, qt = warp & 3, row = tid & (MB - 1);
         const uint32_t sw = tmem + ((uint32_t)qt << 21) + Geo::T_S + half * 32;
         const bool idle = 32 * qt >= np;   // rows of the products hang on nothing but themselves
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
             if (ok && half == 0 && x.at[row] >= 0) a.pml[(size_t)x.at[row] * (a.ns + a.nwin) + blockIdx.x] = make_float2(mu, l + x.end[row]);
         }
     } else if (warp < Geo::W_MMA) {   // ---- sums
-        regs_more<160>();
+        regs_more<152>();
         constexpr int DW = Geo::DW;
         const int qt = warp & 3, d0 = (warp - Geo::W_ACC) / 4 * DW;
         const uint32_t ob = tmem + ((uint32_t)qt << 21) + Geo::T_O + d0;
