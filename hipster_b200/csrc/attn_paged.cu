@@ -1,18 +1,22 @@
 // Attention of a ragged batch of rows over a cache of 8-bit pages (kv_pages.cu), with a window and first tokens that stay visible: calls of up to
-// 8 rows per sequence (decode steps, drafts, verify passes), the merge of the splits, and the plan. Prompts: attn_paged_tc.cu.
+// 16 rows per sequence (decode steps, drafts, verify passes), the merge of the splits, and the plan. Prompts: attn_paged_tc.cu.
 //
 // Row r at position p of its sequence: o = sum_j w_j v_j / sum_j w_j over the keys j <= p with j > p - window or j < n_sink (no window: all), w_j =
 // 2^(s_j - mu), s_j = (q . k_j) * scale * log2 e, times sigmoid(gate). No key: zeros.
 //
 // fp32 results from the f16 tensor pipe: codes of int8 and of e4m3 (times 2^-8) are exact in f16, a token's scale multiplies its score or its weight in
 // fp32, and q and the weights (times the scale of v) go in as two f16 each, the value and what is left of it: 22 bits. q is brought to [2^14, 2^15) by a
-// power of two per row, the weights by the reference mu, which is whole: every rescaling is by a power of two, exact (MU_TOP in paged.cuh). The tensor pipe adds up head_dim / 2 products for a score, in three sums, and 16
-// keys for an output; these are added to the running sums in fp32.
+// power of two per row, the weights by the reference mu, which is whole: every rescaling is by a power of two, exact (MU_TOP in paged.cuh). The tensor pipe adds up
+// head_dim / 2 products for a score, in three sums, and 16 keys for an output; these are added to the running sums in fp32.
 //
 // Keys, and dims, are the 16 rows of mma.sync, the pairs (row of the batch, query head) of a kv head its 8 columns: few pairs waste nothing. A warp has 16 keys at a
 // time, every fourth such slice of its CTA's split, in a ring of three slots of its own (k, v, k, ...), so that no warp waits for another; 16 keys of a head
 // lie in one page, one run of memory. The weights change from rows of keys to columns of pairs by movmatrix. Splits lie at fixed positions and a
 // slice's keys at fixed lanes and warps: a row's bits depend neither on the other rows of the call nor on the other sequences.
+//
+// Measured (captured, us): one token of 24 heads of 256 over 4 at 4097 12.6 (bytes alone 1.3): start, four slices per warp and merge one after the other. 48 such sequences of up to
+// 8192 117 (80; 4.5 TB/s): issue slots 58 %, a third of the instructions turning codes into f16, DRAM 0.66 of the copy rate. 8 x 3 rows over 2 kv heads at 2051 22 (2.0); 32 x 2
+// rows of 32 heads of 128, window 1000, 34 (11): half of the instructions are starts and ends of the CTAs. Pairs as the 16 rows of the products: 260 for the 48 sequences; eight warps per CTA: 128.
 #include "paged.cuh"
 #include <algorithm>
 #include <type_traits>
@@ -363,7 +367,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     }
 }
 
-// Splits of a row, gate, f32 and q8 outputs. A block per row and head: D / 4 threads hold four dims each, and 1024 / D sets of them take every such
+// Splits of a row, gate, f32 and q8 outputs; more than eight splits, or gates and outputs at odd addresses. A block per row and head: D / 4 threads hold four dims each, and 1024 / D sets of them take every such
 // split in order; the sets are added in order. Bound by latency: the row, its place and gate are read ahead of the dependency wait (the kernel of the splits
 // releases this one once its predecessors are complete), the partials of up to four splits of each set are in flight.
 struct MergeArgs {
@@ -484,7 +488,7 @@ __global__ void __launch_bounds__(256) k_paged_merge_few(const MergeArgs a) {
 
 struct Plan { int U, ns, nwin, MB; long long blocks; };
 // Splits lie at multiples of U, which the cache's capacity and the window alone decide (16 to 32 splits and more of a full sequence), so that a row's sums do not hang on what
-// else is in the call. Captured, us: 1 token of 24 heads at 4097, U = 128 13.3, 256 13.3, 512 17.4, 1024 27.7; 48 sequences of up to 8192, 197, 146, 124, 124.
+// else is in the call. Captured, us: 1 token of 24 heads at 4097, U = 128 12.8, 256 12.6, 512 16.9, 1024 26.6; 48 sequences of up to 8192, 187, 139, 118, 116.
 // Prompts have blocks of rows: their keys are split as the launch fills the GPU best, a split costing the start of a CTA, some six tiles. Sixteen splits at most (eight: 64 rows of 24 heads at 16000 104 us, now 91).
 Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink) {
     Plan p;

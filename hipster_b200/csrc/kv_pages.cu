@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(256) k_rope_table(const RopeArgs a) {
     }
 }
 // Large tables: position 32 h + k by the addition theorems from 32 h and k, in 64 bits: four products instead of some 80 operations per entry, which left
-// the 64-bit pipe the bound (262144 x 64 entries: 69 us; the bytes alone 20). A block holds the functions of k < 32 and of its `groups` values of h.
+// the 64-bit pipe the bound (262144 x 64 entries: 69 us, now 33; the bytes alone 20). A block holds the functions of k < 32 and of its `groups` values of h.
 constexpr int ROPE_GROUP = 32;
 __global__ void __launch_bounds__(256) k_rope_table_sums(const RopeArgs a, int groups) {
     extern __shared__ __align__(16) double2 rope_sm[];
@@ -79,8 +79,8 @@ template <int KIND> __device__ __forceinline__ uint32_t kv_code(float x) {
 }
 // D / 8 lanes take a head of a row, eight neighbouring elements each, so that a warp has 1, 2 or 4 heads side by side; it takes hpw such sets of neighbouring
 // heads (n_head query heads, then n_kv key heads, then n_kv value heads) in a loop that fetches a set ahead. The row's place and angles are found once. Instructions
-// bound it beyond a few thousand heads: 220 per head of 128 with a warp per head and the loop unrolled four times (which did not fit the
-// instruction cache), 171 in a loop.
+// bound it beyond a few thousand heads (issue 52 %): 220 per head of 128 with a warp per head and the loop unrolled four times (which did not fit the
+// instruction cache), 171 in a loop. Four prompts of up to 1000 rows of 48 heads of 128: 24.5 us, 73 MB; one row of 32 heads of 256 some 3 us, latency.
 template <int D, int KIND>
 __global__ void __launch_bounds__(256) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, int hpw, int* err) {
     constexpr int LPH = D / 8, HPS = 32 / LPH;   // lanes of a head, heads of a set
@@ -195,7 +195,8 @@ __global__ void __launch_bounds__(256) k_kv_append(PagedPool pool, PagedBatch b,
 }
 
 // RB rows per block, RB / 8 of them found by each warp; thread = 16 neighbouring codes of a row, a head and k or v, times the scale, rounded to f16 once. The e4m3
-// patterns 0x7f and 0xff, which the quantiser does not write, read as 480 and -480.
+// patterns 0x7f and 0xff, which the quantiser does not write, read as 480 and -480. Bound by memory: 16 caches of up to 5000 tokens of 8 x 128 68 us (322 MB, 4.7 TB/s; pages of 16
+// tokens are runs of 2 KB), with one piece in flight per thread 88; 4096 tokens of 4 x 256 7.4 us.
 template <int D, int KIND, int RB>
 __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, __half* __restrict__ ko, __half* __restrict__ vo, size_t row_stride, size_t head_stride, int* err) {
     constexpr int CPR = D / 16, PER = RB / 8;

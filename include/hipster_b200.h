@@ -164,7 +164,7 @@ int hp_kv_read(const int* table_dev, int table_ld, const int* row_start_dev, con
  * h / (n_head / n_kv). gate_dev (nullable): the output is multiplied by sigmoid(gate). out_dev f32 [R][n_head * head_dim] and / or its int8 quantisation (K = n_head * head_dim),
  * either may be NULL. max_rows, max_kv: bounds of a sequence's rows and tokens; they size the launch (R bounds max_rows too). Up to 16 rows per sequence (decode
  * steps, drafts, verify passes) a row's result depends neither on the other rows of its sequence nor on the other sequences, bit for bit (for one table_ld, window and
- * n_sink). Calls of more rows (prompts) turn the keys and values into f16 in the workspace, which then holds 4 * S * n_kv * max_kv * head_dim bytes besides the
+ * n_sink). Calls of more rows (prompts) turn the keys and values into f16 in the workspace, which then holds S * n_kv * max_kv * (4 * head_dim + 8) bytes besides the
  * partial outputs, and sum a row's keys in another order; a sequence of few rows and many tokens takes its time on few SMs there.
  * workspace_dev: hp_attn_paged_workspace_bytes of the same arguments, 16-byte aligned, of this call alone until it is done (captured calls that may run at once need one each). */
 size_t hp_attn_paged_workspace_bytes(int table_ld, int S, int R, int max_rows, int max_kv, int n_head, int window, int n_sink, const hp_kv_pages* pages);
