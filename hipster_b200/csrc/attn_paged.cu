@@ -543,7 +543,7 @@ size_t attn_paged_workspace_bytes(const PagedPool& pool, const PagedBatch& b, in
 
 int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams& p, cudaStream_t s) {
     const Plan pl = plan_of(pool, b, p.n_head, p.window, p.n_sink);
-    HP_REQUIRE(pl.blocks <= 65535 && (long long)b.R * p.n_head < (1ll << 31), "attn_paged: too many rows (%d) for one call", b.R);
+    HP_REQUIRE(pl.blocks <= 65535 && pool.n_kv <= 65535 && (long long)b.R * p.n_head < (1ll << 31), "attn_paged: too many rows (%d) or heads for one call", b.R);
     PagedArgs a; a.pool = pool; a.b = b; a.q = p.q; a.q_ld = p.q_ld; a.q_hs = p.q_hs; a.n_head = p.n_head; a.G = p.n_head / pool.n_kv;
     a.scale2 = (float)((double)p.scale * 1.4426950408889634074 * (pool.kind == KV_E4M3 ? 256.0 : 1.0)); a.window = p.window; a.n_sink = p.n_sink;
     a.U = pl.U; a.ns = pl.ns; a.nwin = pl.nwin;

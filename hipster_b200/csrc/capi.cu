@@ -255,6 +255,11 @@ int paged_ptrs(const char* who, const hp_kv_pages* c, const int* table, const in
     HP_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0 && (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale | (uintptr_t)table | (uintptr_t)row_start | (uintptr_t)kv_len) & 3) == 0, "%s: misaligned cache or batch", who);
     return HP_OK;
 }
+// rows and heads of an output that do not lie over each other: one of the strides spans all that the other one reaches
+bool apart(long long R, long long ld, long long heads, long long hs, long long dim) {
+    auto nested = [&](long long n, long long inner, long long m, long long outer) { return (n == 1 || inner >= dim) && (m == 1 || (outer >= dim && (outer - dim) / (n > 1 ? n - 1 : 1) >= (n > 1 ? inner : 0))); };
+    return nested(heads, hs, R, ld) || nested(R, ld, heads, hs);
+}
 bool rows_ok(const void* p, long long ld, long long hs) { return ((uintptr_t)p & 15) == 0 && ld % 4 == 0 && hs % 4 == 0 && ld >= 0 && hs >= 0; }
 }
 int hp_rope_table(float* table_dev, int n_pos, int n_rot, double base, int scaling, double factor, int orig_ctx, double beta_fast, double beta_slow, double attn_factor, void* stream) {
@@ -277,6 +282,7 @@ int hp_kv_append(const float* q_dev, long long q_ld, long long q_hs, float* q_ou
     HP_REQUIRE(k_dev && v_dev && n_head >= 0 && (n_head == 0 || (q_dev && q_out_dev)) && (n_rot == 0 || rope_dev), "hp_kv_append: null pointer");
     HP_REQUIRE(n_rot >= 0 && n_rot % 2 == 0 && n_rot <= pool.head_dim && (n_rot == 0 || n_pos >= 1) && ((uintptr_t)rope_dev & 7) == 0, "hp_kv_append: bad n_rot=%d n_pos=%d or rope table", n_rot, n_pos);
     HP_REQUIRE(rows_ok(k_dev, k_ld, k_hs) && rows_ok(v_dev, v_ld, v_hs) && (n_head == 0 || (rows_ok(q_dev, q_ld, q_hs) && rows_ok(q_out_dev, qo_ld, qo_hs))), "hp_kv_append: rows must be 16-byte aligned, with strides that are multiples of 4");
+    HP_REQUIRE(n_head == 0 || apart(R, qo_ld, n_head, qo_hs, pool.head_dim), "hp_kv_append: rows of q_out lie over each other");
     HP_REQUIRE((long long)R * (n_head + 2 * pool.n_kv) < (1ll << 33), "hp_kv_append: too many rows");
     hp::KvAppendParams p; p.q = q_dev; p.q_ld = q_ld; p.q_hs = q_hs; p.q_out = q_out_dev; p.qo_ld = qo_ld; p.qo_hs = qo_hs; p.n_head = n_head; p.k = k_dev; p.k_ld = k_ld; p.k_hs = k_hs;
     p.v = v_dev; p.v_ld = v_ld; p.v_hs = v_hs; p.q_norm = q_norm_bf16_dev; p.k_norm = k_norm_bf16_dev; p.rope = rope_dev; p.n_pos = n_rot ? n_pos : 1 << 30; p.n_rot = n_rot; p.interleaved = interleaved; p.eps = eps;
@@ -289,6 +295,7 @@ int hp_kv_read(const int* table_dev, int table_ld, const int* row_start_dev, con
     { int rc = paged_args("hp_kv_read", pages, table_dev, table_ld, row_start_dev, kv_len_dev, S, R, R, 1 << 30, &pool, &b); if (!rc) rc = paged_ptrs("hp_kv_read", pages, table_dev, row_start_dev, kv_len_dev); if (rc) return rc; }
     HP_REQUIRE(k_out_f16_dev && v_out_f16_dev, "hp_kv_read: null pointer");
     HP_REQUIRE((((uintptr_t)k_out_f16_dev | (uintptr_t)v_out_f16_dev) & 15) == 0 && row_stride >= 0 && head_stride >= 0 && row_stride % 8 == 0 && head_stride % 8 == 0, "hp_kv_read: outputs must be 16-byte aligned, with strides that are multiples of 8");
+    HP_REQUIRE(apart(R, row_stride, pool.n_kv, head_stride, pool.head_dim), "hp_kv_read: rows of the outputs lie over each other");
     return hp::kv_read(pool, b, k_out_f16_dev, v_out_f16_dev, (size_t)row_stride, (size_t)head_stride, (cudaStream_t)stream);
     HP_GUARD_END
 }

@@ -89,6 +89,7 @@ PyObject* py_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         else { if (!rows(a[9], (int)dev, R, n_head, c->head_dim, &qo)) Py_RETURN_NONE; out = *tensor(a[9]); }
     } else if (a[9] != Py_None) Py_RETURN_NONE;
     const int inter = PyObject_IsTrue(a[10]);
+    if (inter < 0) PyErr_Clear();
     void* s = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
     if (inter < 0 || outside([&] { return f_append(q.p, q.ld, q.hs, qo.p, qo.ld, qo.hs, n_head, k.p, k.ld, k.hs, v.p, v.ld, v.hs, qn, kn, rope, n_pos, n_rot, inter, b.table, b.ld, b.row_start, b.kv_len, b.S, (int)R, c, (float)eps, s); })) Py_RETURN_NONE;
     if (a[8] == Py_None) Py_RETURN_TRUE;

@@ -137,7 +137,8 @@ int hp_moe_layer(const float* xn_dev, const void* xq_q_dev, const void* xq_sc_de
  * not fit (rows outside of [0, R), a sequence with more rows than max_rows or more tokens than max_kv, table_ld * page_size or the rotary table, a
  * page number outside of [0, n_pages) of a token that is used) fault nothing: what does not fit is left out (append, read) or makes the outputs of its
  * sequence meaningless (attention), and hp_device_status returns HP_EINVAL. Rows of negative position are not appended, read back or
- * normalised (HP_EINVAL), and attend to nothing. Row strides (ld) and head strides (hs) are in elements. */
+ * normalised (HP_EINVAL), and attend to nothing. Row strides (ld) and head strides (hs) are in elements; those of outputs are nested, rows in heads or heads in
+ * rows (HP_EINVAL where they lie over each other). */
 enum { HP_KV_I8 = 0, HP_KV_E4M3 = 1 };
 typedef struct hp_kv_pages {
     void* k; void* v; float* k_scale; float* v_scale;

@@ -74,6 +74,9 @@ def test_bad_rows():
     refused(read(pages(), ko=0), "null")
     refused(read(pages(), vo=FAKE + 8), "aligned")
     refused(read(pages(), rs=132), "aligned")
+    for rs, hs in ((0, 64), (128, 0), (64, 64), (96, 64), (64, 248)):   # four rows of two heads of 64
+        refused(read(pages(), rs=rs, hs=hs), "over each other")
+        refused(append(pages(), qo=(FAKE, rs, hs), n_head=2), "over each other")
     refused(attn(pages(), q=(0, 256, 64)), "null")
     refused(attn(pages(), ws=0), "null")
     refused(attn(pages(), out=0), "null")
