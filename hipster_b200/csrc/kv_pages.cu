@@ -41,9 +41,10 @@ __global__ void __launch_bounds__(256) k_rope_table(const RopeArgs a) {
     }
 }
 // Large tables: position 32 h + k by the addition theorems from 32 h and k, in 64 bits: four products instead of some 80 operations per entry, which left
-// the 64-bit pipe the bound (262144 x 64 entries: 69 us, now 33; the bytes alone 20). A block holds the functions of k < 32 and of its `groups` values of h.
+// the 64-bit pipe the bound (262144 x 64 entries: 69 us, now 28; the bytes alone 20). A block holds the functions of k < 32 and of its `groups` values of h; two blocks of
+// 1024 threads per SM (of 256: 35).
 constexpr int ROPE_GROUP = 32;
-__global__ void __launch_bounds__(256) k_rope_table_sums(const RopeArgs a, int groups) {
+__global__ void __launch_bounds__(1024) k_rope_table_sums(const RopeArgs a, int groups) {
     extern __shared__ __align__(16) double2 rope_sm[];
     __shared__ double f[128];
     pdl_launch_dependents();
@@ -52,7 +53,7 @@ __global__ void __launch_bounds__(256) k_rope_table_sums(const RopeArgs a, int g
     __syncthreads();
     double2* const near = rope_sm; double2* const far = rope_sm + ROPE_GROUP * a.half;   // (cos, sin), far ones times mul
     const int h0 = blockIdx.x * groups;
-    for (int e = threadIdx.x; e < (ROPE_GROUP + groups) * a.half; e += 256) {
+    for (int e = threadIdx.x; e < (ROPE_GROUP + groups) * a.half; e += 1024) {
         const int k = e / a.half;
         double s, c;
         sincos((k < ROPE_GROUP ? (double)k : (double)(h0 + k - ROPE_GROUP) * ROPE_GROUP) * f[e % a.half], &s, &c);
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(256) k_rope_table_sums(const RopeArgs a, int g
     // a thread keeps k and i, and goes through the values of h: one read of shared memory per entry
     const int n = ROPE_GROUP * a.half;
     const size_t end = (size_t)a.n_pos * a.half;
-    for (int e = threadIdx.x; e < n; e += 256) {
+    for (int e = threadIdx.x; e < n; e += 1024) {
         const double2 v = near[e];
         const double2* u = far + e % a.half;
         size_t at = (size_t)h0 * n + e;
@@ -80,9 +81,9 @@ template <int KIND> __device__ __forceinline__ uint32_t kv_code(float x) {
 // D / 8 lanes take a head of a row, eight neighbouring elements each, so that a warp has 1, 2 or 4 heads side by side; it takes hpw such sets of neighbouring
 // heads (n_head query heads, then n_kv key heads, then n_kv value heads) in a loop that fetches a set ahead. The row's place and angles are found once. Instructions
 // bound it beyond a few thousand heads (issue 52 %): 220 per head of 128 with a warp per head and the loop unrolled four times (which did not fit the
-// instruction cache), 171 in a loop. Four prompts of up to 1000 rows of 48 heads of 128: 24.5 us, 73 MB; one row of 32 heads of 256 some 3 us, latency.
+// instruction cache), 171 in a loop. Four prompts of up to 1000 rows of 48 heads of 128: 24 us, 73 MB; one row of 32 heads of 256 some 3 us, latency.
 template <int D, int KIND>
-__global__ void __launch_bounds__(256) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, int hpw, int* err) {
+__global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, int hpw, int* err) {
     constexpr int LPH = D / 8, HPS = 32 / LPH;   // lanes of a head, heads of a set
     __shared__ __align__(16) float buf[8][32 * 8];
     pdl_launch_dependents();
@@ -282,7 +283,7 @@ int rope_table(float* table, int n_pos, int n_rot, double base, int scaling, dou
     static bool attr[MAX_DEVICES] = {};
     const int dev = current_device(); if (dev < 0) return HP_ECUDA;
     if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_rope_table_sums, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * ROPE_GROUP * 128 * 16)); attr[dev] = true; }
-    HP_CUDA(launch_pdl<4>(k_rope_table_sums, dim3((unsigned)((total + groups - 1) / groups)), dim3(256), (size_t)(ROPE_GROUP + groups) * a.half * 16, s, a, groups));
+    HP_CUDA(launch_pdl<4>(k_rope_table_sums, dim3((unsigned)((total + groups - 1) / groups)), dim3(1024), (size_t)(ROPE_GROUP + groups) * a.half * 16, s, a, groups));
     return HP_OK;
 }
 int kv_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, cudaStream_t s) {
