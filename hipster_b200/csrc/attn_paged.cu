@@ -425,10 +425,11 @@ __global__ void __launch_bounds__(256) k_paged_merge(const MergeArgs a) {
 }
 
 // The same sums, bit for bit, where a row has at most eight splits: a thread for four dims over all splits, 1024 dims of a row's heads per block. k_paged_merge's blocks, a head each,
-// are bound by their instructions and start-up once there are thousands of them. 509 rows of 24 heads in three splits (cold, us): 51 there, 27 here.
+// are bound by their instructions and start-up once there are thousands of them. 509 rows of 24 heads in three splits (cold, us): 51 there, 27 here. Five blocks per
+// SM at 256 dims (as many as registers allow: 151 us for the call, now 146); at 128 dims that spills (32 x 2 rows of 32 heads behind a window: 34 us, 41).
 constexpr int FEW = 8;
 template <int D>
-__global__ void __launch_bounds__(256) k_paged_merge_few(const MergeArgs a) {
+__global__ void __launch_bounds__(256, D == 256 ? 5 : 1) k_paged_merge_few(const MergeArgs a) {
     constexpr int HEADS = 1024 / D, SETS = 1024 / D < FEW ? 1024 / D : FEW;   // sums of k_paged_merge's sets
     const int per = (a.n_head + HEADS - 1) / HEADS, r = blockIdx.x / per, h = (blockIdx.x - r * per) * HEADS + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4, lane = threadIdx.x & 31;
     const PagedSeq q = paged_find(a.b, r, lane, a.err);
