@@ -50,6 +50,31 @@ template <int D, bool V> __device__ __forceinline__ int place(int r, int c) {
     else return r * D + ((c ^ (((V ? r >> 1 : r) & 3) << 1)) << 4);
 }
 
+// sums of a row to its output: quotient and gate
+template <typename A> __device__ __forceinline__ void finish(float4& o, float l, float4 g, const A& a) {
+    float x[4] = {0.f + o.x, 0.f + o.y, 0.f + o.z, 0.f + o.w}; const float y[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[e] = l == 0.f ? 0.f : x[e] * a.mul / l;
+        if (a.gate) x[e] = x[e] * sigmoid_det(y[e]);
+    }
+    o = make_float4(x[0], x[1], x[2], x[3]);
+}
+// warp_quant32_store for four dims at k per lane: groups of eight lanes, which are there together, have 32 dims each
+__device__ __forceinline__ void quant_four(float4 x, int r, int k, int K, int8_t* q, float* sc) {
+    const unsigned mask = 0xffu << (threadIdx.x & 24);
+    float amax = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, off));
+    const float dd = amax / 127.f, id = amax > 0.f ? 127.f / amax : 0.f;
+    const int q0 = __float2int_rn(x.x * id), q1 = __float2int_rn(x.y * id), q2 = __float2int_rn(x.z * id), q3 = __float2int_rn(x.w * id);
+    int sum = (q0 + q1) + (q2 + q3);
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(mask, sum, off);
+    q[xq_q_index(r, k, K)] = (int8_t)q0; q[xq_q_index(r, k + 1, K)] = (int8_t)q1; q[xq_q_index(r, k + 2, K)] = (int8_t)q2; q[xq_q_index(r, k + 3, K)] = (int8_t)q3;
+    if ((threadIdx.x & 7) == 0) { const size_t di = xq_d_index(r, k >> 5, K); sc[di] = dd; sc[di + 2] = dd * (float)sum; }
+}
+
 // grid (splits, n_kv, blocks), four warps; NT sets of 8 pairs
 template <int D, int KIND, int NT>
 __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : (D == 256 ? 3 : 4)) k_paged_split(const PagedArgs a) {
@@ -59,6 +84,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     __shared__ int s_pos[MB];   // position of a pair's row, -1: none
     __shared__ float s_mu[KW][MB], s_l[KW][MB];
     __shared__ float* s_out[MB];
+    __shared__ int s_row[MB];   // direct: row of a pair
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
     pdl_wait();
     pdl_launch_dependents();   // behind the wait: what was enqueued in front of this kernel is complete when the merge starts
@@ -67,7 +93,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     const PagedSeq& sq = blk.q;
     const Span sp = span_of(a, blk);
     const int kh = blockIdx.y;
-    if (sp.u0 >= sp.kend) return;
+    if (sp.u0 >= sp.kend && !a.direct) return;   // direct: rows without a key are zeros
     // slices of 16 keys [i * 16, i * 16 + 16): those of this warp leave remainder `warp`; first visible one at or behind i
     const int i_end = (int)((sp.u1 + KS - 1) / KS), i_lo = sp.lo / KS;
     auto first_from = [&](int i) {
@@ -76,7 +102,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     };
     {   // is any slice of the split visible?
         const int i0 = (int)(sp.u0 / KS);
-        if ((i0 * KS >= sp.sink && i0 < i_lo ? i_lo : i0) >= i_end) return;
+        if ((i0 * KS >= sp.sink && i0 < i_lo ? i_lo : i0) >= i_end && !a.direct) return;
     }
     // q: a warp per pair, 8 dims per lane; under way while the pages are looked up
     constexpr int QP = MB / KW;
@@ -348,10 +374,13 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         for (int k = 0; k < KW; ++k) m = fmaxf(m, s_mu[k][tid]);
 #pragma unroll
         for (int k = 0; k < KW; ++k) { const float w = pow2i(s_mu[k][tid] - m); s_mu[k][tid] = w; ls = fmaf(s_l[k][tid], w, ls); }
-        const bool live = s_pos[tid] >= 0;
-        const size_t at = ((size_t)(sq.row0 + t) * a.n_head + kh * a.G + p - t * a.G) * (a.ns + a.nwin) + blockIdx.x;
-        s_out[tid] = live ? a.pO + at * D : nullptr;
-        if (live) a.pml[at] = make_float2(m, ls);
+        if (a.direct) { s_l[0][tid] = ls; s_row[tid] = sq.row0 + t; s_pos[tid] = kh * a.G + p - t * a.G; }   // its head in place of its position
+        else {
+            const bool live = s_pos[tid] >= 0;
+            const size_t at = ((size_t)(sq.row0 + t) * a.n_head + kh * a.G + p - t * a.G) * (a.ns + a.nwin) + blockIdx.x;
+            s_out[tid] = live ? a.pO + at * D : nullptr;
+            if (live) a.pml[at] = make_float2(m, ls);
+        }
     }
     __syncthreads();
 #pragma unroll 4
@@ -363,7 +392,15 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             const float4 v = *reinterpret_cast<const float4*>(xo + (size_t)(k * MB + i) * XS + d); const float w = s_mu[k][i];
             o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
         }
-        if (s_out[i]) *reinterpret_cast<float4*>(s_out[i] + d) = o;
+        if (a.direct) {   // what the merge makes of one split, bit for bit; eight lanes hold 32 dims of a row and head
+            const int r = s_row[i], h = s_pos[i];
+            const float ls = s_l[0][i];
+            float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (a.gate) gate = *reinterpret_cast<const float4*>(a.gate + (size_t)r * a.g_ld + (size_t)h * a.g_hs + d);
+            finish(o, ls, gate, a);
+            if (a.out) *reinterpret_cast<float4*>(a.out + ((size_t)r * a.n_head + h) * D + d) = o;
+            if (a.oq) quant_four(o, r, h * D + d, a.n_head * D, a.oq, a.osc);
+        } else if (s_out[i]) *reinterpret_cast<float4*>(s_out[i] + d) = o;
     }
 }
 
@@ -469,22 +506,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 5 : 1) k_paged_merge_few(const
     float x[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
 #pragma unroll
     for (int i = 0; i < SETS; ++i) { x[0] = x[0] + o[i].x; x[1] = x[1] + o[i].y; x[2] = x[2] + o[i].z; x[3] = x[3] + o[i].w; ls = ls + l[i]; }
-    const float g[4] = {gate.x, gate.y, gate.z, gate.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        x[e] = ls == 0.f ? 0.f : x[e] * a.mul / ls;
-        if (a.gate) x[e] = x[e] * sigmoid_det(g[e]);
-    }
-    if (a.out && live) *reinterpret_cast<float4*>(a.out + ((size_t)r * a.n_head + h) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-    if (a.oq) {   // runs of 32 dims lie in eight lanes: a run at a time to all lanes
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int from = 8 * b + (lane >> 2), at = __shfl_sync(0xffffffffu, live ? h * D + d : -1, 8 * b);
-            if (at < 0) continue;
-            const float y0 = __shfl_sync(0xffffffffu, x[0], from), y1 = __shfl_sync(0xffffffffu, x[1], from), y2 = __shfl_sync(0xffffffffu, x[2], from), y3 = __shfl_sync(0xffffffffu, x[3], from);
-            warp_quant32_store((lane & 2) ? (lane & 1 ? y3 : y2) : (lane & 1 ? y1 : y0), r, at >> 5, a.n_head * D, a.oq, a.osc, lane);
-        }
-    }
+    float4 y = make_float4(x[0], x[1], x[2], x[3]);
+    finish(y, ls, gate, a);
+    if (!live) return;
+    if (a.out) *reinterpret_cast<float4*>(a.out + ((size_t)r * a.n_head + h) * D + d) = y;
+    if (a.oq) quant_four(y, r, h * D + d, a.n_head * D, a.oq, a.osc);
 }
 
 struct Plan { int U, ns, nwin, MB; long long blocks; };
@@ -550,12 +576,14 @@ int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams
     a.U = pl.U; a.ns = pl.ns; a.nwin = pl.nwin;
     a.pO = (float*)p.workspace; a.pml = (float2*)(a.pO + partials(pl, b, p.n_head) * pool.head_dim); a.err = device_err_flag(); a.arg_err = device_arg_flag();
     a.f16 = (uint8_t*)p.workspace + (partials(pl, b, p.n_head) * (pool.head_dim + 2) * sizeof(float) + 127) / 128 * 128; a.tiles = 0;
+    a.gate = p.gate; a.g_ld = p.g_ld; a.g_hs = p.g_hs; a.mul = pool.kind == KV_E4M3 ? 256.f : 1.f; a.out = p.out; a.oq = (int8_t*)p.xq.q; a.osc = (float*)p.xq.sc;
+    const bool wide = (((uintptr_t)p.gate | (uintptr_t)p.out) & 15) == 0 && (!p.gate || ((p.g_ld | p.g_hs) & 3) == 0);   // four dims of gate and output at a time
+    a.direct = wide && b.max_rows <= PAGED_DECODE_ROWS && pl.ns + pl.nwin == 1;
     const dim3 grid(pl.ns + pl.nwin, pool.n_kv, (unsigned)pl.blocks);
     const int rc = b.max_rows > PAGED_DECODE_ROWS ? attn_paged_tc(a, grid, s) : pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, pl.MB, s) : launch_split<KV_E4M3>(a, grid, pl.MB, s);
-    if (rc != HP_OK) return rc;
+    if (rc != HP_OK || a.direct) return rc;
     MergeArgs m; m.b = b; m.pO = a.pO; m.pml = a.pml; m.gate = p.gate; m.g_ld = p.g_ld; m.g_hs = p.g_hs; m.n_head = p.n_head; m.window = p.window; m.n_sink = p.n_sink;
-    m.U = pl.U; m.ns = pl.ns; m.nwin = pl.nwin; m.mul = pool.kind == KV_E4M3 ? 256.f : 1.f; m.out = p.out; m.oq = (int8_t*)p.xq.q; m.osc = (float*)p.xq.sc; m.err = a.arg_err;
-    const bool wide = (((uintptr_t)p.gate | (uintptr_t)p.out) & 15) == 0 && (!p.gate || ((p.g_ld | p.g_hs) & 3) == 0);   // four dims of gate and output at a time
+    m.U = pl.U; m.ns = pl.ns; m.nwin = pl.nwin; m.mul = a.mul; m.out = p.out; m.oq = (int8_t*)p.xq.q; m.osc = (float*)p.xq.sc; m.err = a.arg_err;
     auto merge = [&](auto dims) {
         constexpr int D = decltype(dims)::value, HPB = 1024 / D;
         if (pl.ns + pl.nwin <= FEW && wide) return launch_pdl<4>(k_paged_merge_few<D>, dim3((unsigned)(b.R * ((p.n_head + HPB - 1) / HPB))), dim3(256), 0, s, m);

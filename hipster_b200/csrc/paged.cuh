@@ -49,6 +49,8 @@ struct PagedArgs {
     int U, ns, nwin;            // keys of a split, splits of the first tokens, splits behind them
     float* pO; float2* pml;     // partials [row][head][ns + nwin] (x head_dim): sums, (mu, sum of weights)
     uint8_t* f16; int tiles;    // prompts: tiles of 64 tokens in f16, [sequence][kv head][tiles][k, v, scales]
+    // outputs of the rows: written by the merge, or by the only split there is (direct)
+    const float* gate; size_t g_ld, g_hs; float mul; float* out; int8_t* oq; float* osc; int direct;
     int* err; int* arg_err;
 };
 

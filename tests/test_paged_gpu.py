@@ -692,12 +692,14 @@ def test_a_sequence_from_prompt_to_rejected_drafts():
 
 
 @pytest.mark.parametrize("D,H,n_kv", [(64, 5, 1), (128, 3, 3), (256, 6, 2)])
-@pytest.mark.parametrize("rows,lens,window,n_sink", [([3, 0, 1, 2], [700, 10, 1, 300], 0, 0), ([3, 1, 2], [900, 40, 513], 300, 20), ([40, 3, 0], [600, 3, 9], 0, 0), ([40, 19], [600, 777], 200, 5)])
+@pytest.mark.parametrize("rows,lens,window,n_sink", [([3, 0, 1, 2], [700, 10, 1, 300], 0, 0), ([3, 1, 2], [900, 40, 513], 300, 20), ([40, 3, 0], [600, 3, 9], 0, 0), ([40, 19], [600, 777], 200, 5),
+                                                       ([3, 0, 1, 16], [256, 10, 1, 40], 0, 0), ([8, 2], [2, 33], 0, 0)])
 def test_gates_and_outputs_at_odd_places(D, H, n_kv, rows, lens, window, n_sink):
-    # the merge reads gates four at a time where they lie so, and one at a time elsewhere: the same bits, quantised rows too. The last row has no key.
+    # Gates are read four at a time where they lie so, and one at a time elsewhere; a single split writes the outputs itself where it can. The same bits, quantised rows too, and
+    # with more splits (max_kv). The last row has no key.
     lens = [*lens, 0]
     rows = [*rows, 1]
-    st = Setup(rows, lens, n_kv, D, 16, "e4m3", 3)
+    st = Setup(rows, lens, n_kv, D, 16, "e4m3", 3, cols=-(-4 * max(lens) // 16))
     g = gen(7)
     q = torch.randn((st.R, H, D), generator=g, device="cuda")
     gate = torch.randn((st.R, H, D), generator=g, device="cuda")
@@ -706,5 +708,8 @@ def test_gates_and_outputs_at_odd_places(D, H, n_kv, rows, lens, window, n_sink)
     run = lambda x: K_.attn_paged(q, st.pool, *st.batch, max_rows=max(rows), max_kv=max(lens), window=window, n_sink=n_sink, gate=x, want_q8=True)  # noqa: E731
     (a, xa), (b, xb) = run(gate), run(odd)
     assert torch.equal(a, b) and torch.equal(xa.q, xb.q) and torch.equal(xa.sc, xb.sc)
+    if max(rows) <= 16:
+        c, xc = K_.attn_paged(q, st.pool, *st.batch, max_rows=max(rows), max_kv=4 * max(lens), window=window, n_sink=n_sink, gate=gate, want_q8=True)
+        assert torch.equal(a, c) and torch.equal(xa.q, xc.q) and torch.equal(xa.sc, xc.sc)
     exact, tol = attn64(st, q, D ** -0.5, window, n_sink, gate)
     assert ((a.double() - exact).abs() <= tol).all() and (a[-1] == 0).all()
