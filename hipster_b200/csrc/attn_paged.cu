@@ -51,7 +51,7 @@ template <int D, bool V> __device__ __forceinline__ int place(int r, int c) {
 }
 
 // sums of a row to its output: quotient and gate
-template <typename A> __device__ __forceinline__ void finish(float4& o, float l, float4 g, const A& a) {
+__device__ __forceinline__ void finish(float4& o, float l, float4 g, const PagedArgs& a) {
     float x[4] = {0.f + o.x, 0.f + o.y, 0.f + o.z, 0.f + o.w}; const float y[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -71,12 +71,12 @@ __device__ __forceinline__ void quant_four(float4 x, int r, int k, int K, int8_t
     int sum = (q0 + q1) + (q2 + q3);
 #pragma unroll
     for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(mask, sum, off);
-    q[xq_q_index(r, k, K)] = (int8_t)q0; q[xq_q_index(r, k + 1, K)] = (int8_t)q1; q[xq_q_index(r, k + 2, K)] = (int8_t)q2; q[xq_q_index(r, k + 3, K)] = (int8_t)q3;
+    *reinterpret_cast<uint32_t*>(q + xq_q_index(r, k, K)) = (q0 & 0xff) | (q1 & 0xff) << 8 | (q2 & 0xff) << 16 | (uint32_t)q3 << 24;   // four bytes of one lane's eight
     if ((threadIdx.x & 7) == 0) { const size_t di = xq_d_index(r, k >> 5, K); sc[di] = dd; sc[di + 2] = dd * (float)sum; }
 }
 
-// grid (splits, n_kv, blocks), four warps; NT sets of 8 pairs
-template <int D, int KIND, int NT>
+// grid (splits, n_kv, blocks), four warps; NT sets of 8 pairs. DIRECT: the only split there is writes the outputs itself
+template <int D, int KIND, int NT, bool DIRECT>
 __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : (D == 256 ? 3 : 4)) k_paged_split(const PagedArgs a) {
     constexpr int CPR = D / 16, MB = 8 * NT, XS = out_stride(D);   // 16-byte pieces of a row
     extern __shared__ __align__(128) uint8_t sm[];
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     const PagedSeq& sq = blk.q;
     const Span sp = span_of(a, blk);
     const int kh = blockIdx.y;
-    if (sp.u0 >= sp.kend && !a.direct) return;   // direct: rows without a key are zeros
+    if (sp.u0 >= sp.kend && !DIRECT) return;   // direct: rows without a key are zeros
     // slices of 16 keys [i * 16, i * 16 + 16): those of this warp leave remainder `warp`; first visible one at or behind i
     const int i_end = (int)((sp.u1 + KS - 1) / KS), i_lo = sp.lo / KS;
     auto first_from = [&](int i) {
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     };
     {   // is any slice of the split visible?
         const int i0 = (int)(sp.u0 / KS);
-        if ((i0 * KS >= sp.sink && i0 < i_lo ? i_lo : i0) >= i_end && !a.direct) return;
+        if ((i0 * KS >= sp.sink && i0 < i_lo ? i_lo : i0) >= i_end && !DIRECT) return;
     }
     // q: a warp per pair, 8 dims per lane; under way while the pages are looked up
     constexpr int QP = MB / KW;
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         for (int k = 0; k < KW; ++k) m = fmaxf(m, s_mu[k][tid]);
 #pragma unroll
         for (int k = 0; k < KW; ++k) { const float w = pow2i(s_mu[k][tid] - m); s_mu[k][tid] = w; ls = fmaf(s_l[k][tid], w, ls); }
-        if (a.direct) { s_l[0][tid] = ls; s_row[tid] = sq.row0 + t; s_pos[tid] = kh * a.G + p - t * a.G; }   // its head in place of its position
+        if (DIRECT) { s_l[0][tid] = ls; s_row[tid] = sq.row0 + t; s_pos[tid] = kh * a.G + p - t * a.G; }   // its head in place of its position
         else {
             const bool live = s_pos[tid] >= 0;
             const size_t at = ((size_t)(sq.row0 + t) * a.n_head + kh * a.G + p - t * a.G) * (a.ns + a.nwin) + blockIdx.x;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             const float4 v = *reinterpret_cast<const float4*>(xo + (size_t)(k * MB + i) * XS + d); const float w = s_mu[k][i];
             o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
         }
-        if (a.direct) {   // what the merge makes of one split, bit for bit; eight lanes hold 32 dims of a row and head
+        if constexpr (DIRECT) {   // what the merge makes of one split, bit for bit; eight lanes hold 32 dims of a row and head
             const int r = s_row[i], h = s_pos[i];
             const float ls = s_l[0][i];
             float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -506,11 +506,22 @@ __global__ void __launch_bounds__(256, D == 256 ? 5 : 1) k_paged_merge_few(const
     float x[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
 #pragma unroll
     for (int i = 0; i < SETS; ++i) { x[0] = x[0] + o[i].x; x[1] = x[1] + o[i].y; x[2] = x[2] + o[i].z; x[3] = x[3] + o[i].w; ls = ls + l[i]; }
-    float4 y = make_float4(x[0], x[1], x[2], x[3]);
-    finish(y, ls, gate, a);
-    if (!live) return;
-    if (a.out) *reinterpret_cast<float4*>(a.out + ((size_t)r * a.n_head + h) * D + d) = y;
-    if (a.oq) quant_four(y, r, h * D + d, a.n_head * D, a.oq, a.osc);
+    const float g[4] = {gate.x, gate.y, gate.z, gate.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[e] = ls == 0.f ? 0.f : x[e] * a.mul / ls;
+        if (a.gate) x[e] = x[e] * sigmoid_det(g[e]);
+    }
+    if (a.out && live) *reinterpret_cast<float4*>(a.out + ((size_t)r * a.n_head + h) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+    if (a.oq) {   // runs of 32 dims lie in eight lanes: a run at a time to all lanes
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int from = 8 * b + (lane >> 2), at = __shfl_sync(0xffffffffu, live ? h * D + d : -1, 8 * b);
+            if (at < 0) continue;
+            const float y0 = __shfl_sync(0xffffffffu, x[0], from), y1 = __shfl_sync(0xffffffffu, x[1], from), y2 = __shfl_sync(0xffffffffu, x[2], from), y3 = __shfl_sync(0xffffffffu, x[3], from);
+            warp_quant32_store((lane & 2) ? (lane & 1 ? y3 : y2) : (lane & 1 ? y1 : y0), r, at >> 5, a.n_head * D, a.oq, a.osc, lane);
+        }
+    }
 }
 
 struct Plan { int U, ns, nwin, MB; long long blocks; };
@@ -548,15 +559,18 @@ Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window,
 }
 size_t partials(const Plan& p, const PagedBatch& b, int n_head) { return (size_t)b.R * n_head * (p.ns + p.nwin); }
 
-template <int D, int KIND, int NT> int launch_split(const PagedArgs& a, dim3 grid, cudaStream_t s) {
+template <int D, int KIND, int NT, bool DIRECT> int launch_split(const PagedArgs& a, dim3 grid, cudaStream_t s) {
     constexpr int smem = smem_bytes(D, NT);
     static bool attr[MAX_DEVICES] = {};   // per device: the opt-in belongs to the device's copy of the kernel
     const int dev = current_device(); if (dev < 0) return HP_ECUDA;
-    if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_split<D, KIND, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); attr[dev] = true; }
-    HP_CUDA(launch_pdl<4>(k_paged_split<D, KIND, NT>, grid, dim3(32 * KW), smem, s, a));
+    if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_split<D, KIND, NT, DIRECT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); attr[dev] = true; }
+    HP_CUDA(launch_pdl<4>(k_paged_split<D, KIND, NT, DIRECT>, grid, dim3(32 * KW), smem, s, a));
     return HP_OK;
 }
-template <int D, int KIND> int launch_split(const PagedArgs& a, dim3 grid, int MB, cudaStream_t s) { return MB == 8 ? launch_split<D, KIND, 1>(a, grid, s) : launch_split<D, KIND, 2>(a, grid, s); }
+template <int D, int KIND> int launch_split(const PagedArgs& a, dim3 grid, int MB, cudaStream_t s) {
+    if (a.direct) return MB == 8 ? launch_split<D, KIND, 1, true>(a, grid, s) : launch_split<D, KIND, 2, true>(a, grid, s);
+    return MB == 8 ? launch_split<D, KIND, 1, false>(a, grid, s) : launch_split<D, KIND, 2, false>(a, grid, s);
+}
 template <int KIND> int launch_split(const PagedArgs& a, dim3 grid, int MB, cudaStream_t s) {
     return a.pool.head_dim == 256 ? launch_split<256, KIND>(a, grid, MB, s) : a.pool.head_dim == 128 ? launch_split<128, KIND>(a, grid, MB, s) : launch_split<64, KIND>(a, grid, MB, s);
 }
@@ -578,6 +592,7 @@ int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams
     a.f16 = (uint8_t*)p.workspace + (partials(pl, b, p.n_head) * (pool.head_dim + 2) * sizeof(float) + 127) / 128 * 128; a.tiles = 0;
     a.gate = p.gate; a.g_ld = p.g_ld; a.g_hs = p.g_hs; a.mul = pool.kind == KV_E4M3 ? 256.f : 1.f; a.out = p.out; a.oq = (int8_t*)p.xq.q; a.osc = (float*)p.xq.sc;
     const bool wide = (((uintptr_t)p.gate | (uintptr_t)p.out) & 15) == 0 && (!p.gate || ((p.g_ld | p.g_hs) & 3) == 0);   // four dims of gate and output at a time
+    // One split: its kernel writes the outputs, for the price of a merge's launch (captured and host's time of 32 tokens of 32 heads over 8 at 256 tokens 14.6 and 9.9 us, now 8.6 and 7.3)
     a.direct = wide && b.max_rows <= PAGED_DECODE_ROWS && pl.ns + pl.nwin == 1;
     const dim3 grid(pl.ns + pl.nwin, pool.n_kv, (unsigned)pl.blocks);
     const int rc = b.max_rows > PAGED_DECODE_ROWS ? attn_paged_tc(a, grid, s) : pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, pl.MB, s) : launch_split<KV_E4M3>(a, grid, pl.MB, s);
