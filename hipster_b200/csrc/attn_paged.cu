@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         slot = slot + 1 == SLOTS ? 0 : slot + 1;
         // ---- weights
         const float k0 = __shfl_sync(0xffffffffu, sc, g), k1 = __shfl_sync(0xffffffffu, sc, g + 8), v0 = __shfl_sync(0xffffffffu, sc, g + 16), v1 = __shfl_sync(0xffffffffu, sc, g + 24);
-        const float lv0 = lg2(fmaxf(v0, 8.0779357e-28f)), lv1 = lg2(fmaxf(v1, 8.0779357e-28f));   // 2^-90: the weights' sum cannot overflow
+        const float lv0 = scale_lg2(v0), lv1 = scale_lg2(v1);
         const int j = i0 * KS + g;
         const bool whole = i0 * KS + KS - 1 <= all_hi && (i0 * KS > all_lo || i0 * KS + KS <= sp.sink);
         bool hide[NT][4];

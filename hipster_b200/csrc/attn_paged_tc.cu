@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
                 const int pos = x.pos[row];
                 see = below(pos + 1) & (a.window ? ~below(max(pos - a.window + 1, 0)) | below(sink) : ~0u);
             }
-            const float lv = lg2(fmaxf(warp_max(vs[lane]), 8.0779357e-28f));   // 2^-90: the weights' sum cannot overflow
+            const float lv = scale_lg2(warp_max(vs[lane]));
             float d[32];
             auto measure = [&] {   // distances of the logarithms from their reference
                 ld16(d, at); ld16(d + 16, at + 16);
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
                     ld16(y, at + i); ld_wait(); ld_there(y);
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float z = y[e] * (ks[i + e] * c) + lg2(fmaxf(vs[i + e], 8.0779357e-28f));
+                        const float z = y[e] * (ks[i + e] * c) + scale_lg2(vs[i + e]);
                         exact = fmaxf(exact, see >> (i + e) & 1 ? z : -INFINITY);
                     }
                 }

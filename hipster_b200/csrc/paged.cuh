@@ -64,6 +64,8 @@ int attn_paged_tc(PagedArgs& a, dim3 grid, cudaStream_t s);
 constexpr float MU_TOP = 8.f, MU_LIMIT = 15.f, MU_NONE = -1e30f;
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// logarithm of a scale of v, at least 2^-90: the weights' sum cannot overflow. NaN counts as that; infinity as the largest number, so that a reference stays finite and the rows that see it become NaN
+__device__ __forceinline__ float scale_lg2(float v) { return lg2(fminf(fmaxf(v, 8.0779357e-28f), 3.4028235e38f)); }
 __device__ __forceinline__ float pow2i(float d) { return d < -126.f ? 0.f : __uint_as_float((uint32_t)((int)d + 127) << 23); }   // 2^d, d whole and <= 0
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 // Two of four codes as two f16. int8: the code plus 128 becomes the low bits of 1024 + code + 128, and 1152 is subtracted, exactly. e4m3: its bits

@@ -1,5 +1,6 @@
 """The paged 8-bit cache on the GPU (hp_rope_table, hp_kv_append, hp_kv_read, hp_attn_paged) against plain implementations in 64 bits."""
 import ctypes
+import itertools
 import math
 import os
 import subprocess
@@ -422,10 +423,10 @@ def test_non_finite_tokens_reach_the_rows_that_see_them():
     st = Setup([4], [100], 1, 64, 16, "i8")
     q = torch.randn((4, 2, 64), generator=gen(1), device="cuda")
     clean, _ = K_.attn_paged(q, st.pool, *st.batch, max_rows=4, max_kv=100)
-    for scale in (st.pool.k_scale, st.pool.v_scale):
+    for scale, bad in ((st.pool.k_scale, math.nan), (st.pool.v_scale, math.nan), (st.pool.v_scale, math.inf)):
         pg, at = st.slot(0, 98)   # seen by the last two rows
         old = scale.clone()
-        scale[pg, 0, at] = math.nan
+        scale[pg, 0, at] = bad
         got, _ = K_.attn_paged(q, st.pool, *st.batch, max_rows=4, max_kv=100)
         assert torch.equal(got[:2], clean[:2]) and torch.isnan(got[2:]).all()
         scale.copy_(old)
@@ -713,3 +714,52 @@ def test_gates_and_outputs_at_odd_places(D, H, n_kv, rows, lens, window, n_sink)
         assert torch.equal(a, c) and torch.equal(xa.q, xc.q) and torch.equal(xa.sc, xc.sc)
     exact, tol = attn64(st, q, D ** -0.5, window, n_sink, gate)
     assert ((a.double() - exact).abs() <= tol).all() and (a[-1] == 0).all()
+
+
+@pytest.mark.parametrize("D,kind", [(64, "i8"), (128, "e4m3"), (256, "i8")])
+def test_non_finite_tokens_in_prompts(D, kind):
+    st = Setup([70], [300], 1, D, 16, kind)
+    q = torch.randn((70, 5, D), generator=gen(1), device="cuda")
+    run = lambda: K_.attn_paged(q, st.pool, *st.batch, max_rows=70, max_kv=300)[0]  # noqa: E731
+    clean = run()
+    for scale, bad in itertools.product((st.pool.k_scale, st.pool.v_scale), (math.nan, math.inf)):
+        pg, at = st.slot(0, 290)   # seen by the last ten rows
+        old = scale.clone()
+        scale[pg, 0, at] = bad
+        got = run()
+        assert torch.equal(got[:60], clean[:60]) and (scale is st.pool.k_scale and bad == math.inf or torch.isnan(got[60:]).all())
+        scale.copy_(old)
+    q[33, 2] = math.nan
+    got = run()
+    assert torch.isnan(got[33, 2]).all()
+    got[33, 2] = clean[33, 2]
+    assert torch.equal(got, clean) and status() == 0
+
+
+@pytest.mark.parametrize("k_up,v_up", [(1e-12, 1e-12), (1e10, 1e15), (1.0, 1e-25), (1e-30, 1.0)])
+@pytest.mark.parametrize("D", [64, 256])
+def test_magnitudes_in_prompts(D, k_up, v_up):
+    st = Setup([40, 17], [250, 90], 2, D, 16, "e4m3")
+    st.pool.k_scale.mul_(k_up)
+    st.pool.v_scale.mul_(v_up * torch.exp(3 * torch.randn(st.pool.v_scale.shape, generator=gen(8), device="cuda")))
+    st.pool.v_scale[:, :, 3] = 0
+    q = torch.randn((57, 8, D), generator=gen(5), device="cuda") / k_up
+    got, _ = K_.attn_paged(q, st.pool, *st.batch, max_rows=40, max_kv=250, scale=0.125)
+    want, tol = attn64(st, q, 0.125, 0, 0, None)
+    assert status() == 0 and ((got.double() - want).abs() <= tol).all()
+
+
+def test_prompts_and_steps_at_once():
+    # calls that hold all accumulator memory of an SM and calls that hold none, on four streams
+    st, few = Setup([150, 40], [1500, 700], 2, 256, 64, "i8"), Setup([2, 1], [900, 30], 2, 256, 16, "i8", 1)
+    q = torch.randn((190, 12, 256), generator=gen(1), device="cuda")
+    prompt = lambda: K_.attn_paged(q, st.pool, *st.batch, max_rows=150, max_kv=1500)[0]  # noqa: E731
+    step = lambda: K_.attn_paged(q[:3], few.pool, *few.batch, max_rows=2, max_kv=900)[0]  # noqa: E731
+    want = prompt(), step()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(4)], []
+    for i in range(24):
+        with torch.cuda.stream(streams[i % 4]):
+            got.append((prompt if i % 3 else step)())
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[0 if i % 3 else 1]) for i, g in enumerate(got)) and status() == 0
