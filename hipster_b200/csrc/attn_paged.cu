@@ -50,31 +50,6 @@ template <int D, bool V> __device__ __forceinline__ int place(int r, int c) {
     else return r * D + ((c ^ (((V ? r >> 1 : r) & 3) << 1)) << 4);
 }
 
-// sums of a row to its output: quotient and gate
-__device__ __forceinline__ void finish(float4& o, float l, float4 g, const PagedArgs& a) {
-    float x[4] = {0.f + o.x, 0.f + o.y, 0.f + o.z, 0.f + o.w}; const float y[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        x[e] = l == 0.f ? 0.f : x[e] * a.mul / l;
-        if (a.gate) x[e] = x[e] * sigmoid_det(y[e]);
-    }
-    o = make_float4(x[0], x[1], x[2], x[3]);
-}
-// warp_quant32_store for four dims at k per lane: groups of eight lanes, which are there together, have 32 dims each
-__device__ __forceinline__ void quant_four(float4 x, int r, int k, int K, int8_t* q, float* sc) {
-    const unsigned mask = 0xffu << (threadIdx.x & 24);
-    float amax = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-#pragma unroll
-    for (int off = 4; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, off));
-    const float dd = amax / 127.f, id = amax > 0.f ? 127.f / amax : 0.f;
-    const int q0 = __float2int_rn(x.x * id), q1 = __float2int_rn(x.y * id), q2 = __float2int_rn(x.z * id), q3 = __float2int_rn(x.w * id);
-    int sum = (q0 + q1) + (q2 + q3);
-#pragma unroll
-    for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(mask, sum, off);
-    *reinterpret_cast<uint32_t*>(q + xq_q_index(r, k, K)) = (q0 & 0xff) | (q1 & 0xff) << 8 | (q2 & 0xff) << 16 | (uint32_t)q3 << 24;   // four bytes of one lane's eight
-    if ((threadIdx.x & 7) == 0) { const size_t di = xq_d_index(r, k >> 5, K); sc[di] = dd; sc[di + 2] = dd * (float)sum; }
-}
-
 // grid (splits, n_kv, blocks), four warps; NT sets of 8 pairs. DIRECT: the only split there is writes the outputs itself
 template <int D, int KIND, int NT, bool DIRECT>
 __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : (D == 256 ? 3 : 4)) k_paged_split(const PagedArgs a) {
@@ -392,15 +367,8 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             const float4 v = *reinterpret_cast<const float4*>(xo + (size_t)(k * MB + i) * XS + d); const float w = s_mu[k][i];
             o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
         }
-        if constexpr (DIRECT) {   // what the merge makes of one split, bit for bit; eight lanes hold 32 dims of a row and head
-            const int r = s_row[i], h = s_pos[i];
-            const float ls = s_l[0][i];
-            float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (a.gate) gate = *reinterpret_cast<const float4*>(a.gate + (size_t)r * a.g_ld + (size_t)h * a.g_hs + d);
-            finish(o, ls, gate, a);
-            if (a.out) *reinterpret_cast<float4*>(a.out + ((size_t)r * a.n_head + h) * D + d) = o;
-            if (a.oq) quant_four(o, r, h * D + d, a.n_head * D, a.oq, a.osc);
-        } else if (s_out[i]) *reinterpret_cast<float4*>(s_out[i] + d) = o;
+        if constexpr (DIRECT) put(o, s_l[0][i], s_row[i], s_pos[i], d, D, a);
+        else if (s_out[i]) *reinterpret_cast<float4*>(s_out[i] + d) = o;
     }
 }
 
@@ -593,7 +561,7 @@ int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams
     a.gate = p.gate; a.g_ld = p.g_ld; a.g_hs = p.g_hs; a.mul = pool.kind == KV_E4M3 ? 256.f : 1.f; a.out = p.out; a.oq = (int8_t*)p.xq.q; a.osc = (float*)p.xq.sc;
     const bool wide = (((uintptr_t)p.gate | (uintptr_t)p.out) & 15) == 0 && (!p.gate || ((p.g_ld | p.g_hs) & 3) == 0);   // four dims of gate and output at a time
     // One split: its kernel writes the outputs, for the price of a merge's launch (captured and host's time of 32 tokens of 32 heads over 8 at 256 tokens 14.6 and 9.9 us, now 8.6 and 7.3)
-    a.direct = wide && b.max_rows <= PAGED_DECODE_ROWS && pl.ns + pl.nwin == 1;
+    a.direct = wide && pl.ns + pl.nwin == 1;
     const dim3 grid(pl.ns + pl.nwin, pool.n_kv, (unsigned)pl.blocks);
     const int rc = b.max_rows > PAGED_DECODE_ROWS ? attn_paged_tc(a, grid, s) : pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, pl.MB, s) : launch_split<KV_E4M3>(a, grid, pl.MB, s);
     if (rc != HP_OK || a.direct) return rc;

@@ -76,8 +76,8 @@ __device__ __forceinline__ void pair_sync(int qt) { asm volatile("bar.sync %0, 6
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) { return __all_sync(0xffffffffu, mbar_test(bar, parity) || tc_wait(bar, parity, err)); }
 __device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) { __syncwarp(); if (lane == 0) mbar_arrive(bar); }
 
-// grid (splits, n_kv, blocks)
-template <int D, int KIND>
+// grid (splits, n_kv, blocks). DIRECT: the only split there is writes the outputs itself
+template <int D, int KIND, bool DIRECT>
 __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(const PagedArgs a) {
     using Geo = PagedGeo<D>;
     extern __shared__ uint8_t sm_raw[];
@@ -85,12 +85,12 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
     uint8_t* const sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     struct Shared {
-        uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[4], s_full[2], p_full[2], pv_done, o_empty, fin;
+        uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[4], s_full[2], p_full[2], pv_done, o_empty, l_there[4], fin;
         float c[MB], alpha[4][MB];   // factor of a pair's scores; rescaling by tile
         float top[2][MB];            // by half of the keys: a pair's largest logarithm where a reference may move
-        float end[MB];               // sums of the weights of the second halves
+        float end[MB];               // sums of the weights of the second halves; direct: of all keys
         long long from[MB];          // a pair's row of q, -1: none
-        int pos[MB], at[MB];         // its position, -1: none; row * n_head + head, -1: nothing to write
+        int pos[MB], at[MB];         // its position, -1: none; row * n_head + head, -1: nothing to write (direct: rows without a key are zeros)
         int moved[4][4];             // by tile and warp: the tile's number + 1 where a reference moves, and alpha holds
     };
     static_assert(sizeof(Shared) <= Geo::X_BYTES, "");
@@ -103,7 +103,14 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
     const int kh = blockIdx.y, np = blk.np;
     const Span sp = span_of(a, blk);
     const int lo = sp.lo, sink = sp.sink;
-    if (sp.u0 >= sp.kend) return;
+    if (sp.u0 >= sp.kend) {   // no row of the block has a key
+        if constexpr (DIRECT)
+            for (int e = tid; e < np * (D / 4); e += Geo::WARPS * 32) {
+                const int p = blk.p0 + e / (D / 4), t = p / a.G;
+                put(make_float4(0.f, 0.f, 0.f, 0.f), 0.f, sq.row0 + t, kh * a.G + p - t * a.G, e % (D / 4) * 4, D, a);
+            }
+        return;
+    }
     const int t_end = (int)((sp.u1 + TK - 1) / TK);
     auto first_from = [&](int t) { return t * TK >= sink && t * TK + TK <= lo ? lo / TK : t; };   // first visible tile at or behind t
     const int t_first = first_from((int)(sp.u0 / TK));
@@ -112,6 +119,7 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.k_full[i]), 1); mbar_init(smem_u32(&x.k_empty[i]), 1); mbar_init(smem_u32(&x.v_full[i]), 1); mbar_init(smem_u32(&x.v_empty[i]), 1); }
         for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&x.sc_full[i]), 1);
+        for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&x.l_there[i]), 1);
         for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); mbar_init(smem_u32(&x.p_full[i]), 8); }
         mbar_init(smem_u32(&x.pv_done), 1); mbar_init(smem_u32(&x.o_empty), 8); mbar_init(smem_u32(&x.fin), 1);
         fence_barrier_init();
@@ -124,7 +132,7 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
     if (tid < MB) {
         const int p = blk.p0 + tid, t = p / a.G, head = kh * a.G + p - t * a.G, pos = tid < np ? max(-1, sq.len - sq.T + t) : -1;
         x.from[tid] = tid < np ? (long long)((size_t)(sq.row0 + t) * a.q_ld + (size_t)head * a.q_hs) : -1;
-        x.pos[tid] = pos; x.at[tid] = pos >= 0 ? (sq.row0 + t) * a.n_head + head : -1;
+        x.pos[tid] = pos; x.at[tid] = (DIRECT ? tid < np : pos >= 0) ? (sq.row0 + t) * a.n_head + head : -1;
     }
     __syncthreads();
     // q: a warp per pair, 8 dims per lane, a warp's pairs all in flight; rests to their place, values to that of k, on their way to accumulator memory
@@ -295,7 +303,8 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
             const float l = l2.x + l2.y;
             if (half) x.end[row] = l;
             pair_sync(qt);
-            if (ok && half == 0 && x.at[row] >= 0) a.pml[(size_t)x.at[row] * (a.ns + a.nwin) + blockIdx.x] = make_float2(mu, l + x.end[row]);
+            if (DIRECT && half == 0) { x.end[row] = l + x.end[row]; warp_arrive(smem_u32(&x.l_there[qt]), lane); }
+            else if (ok && half == 0 && x.at[row] >= 0) a.pml[(size_t)x.at[row] * (a.ns + a.nwin) + blockIdx.x] = make_float2(mu, l + x.end[row]);
         }
     } else if (warp < Geo::W_MMA) {   // ---- sums
         regs_more<152>();
@@ -337,11 +346,15 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
 #pragma unroll
             for (int i = 0; i < DW; i += 4) *reinterpret_cast<float4*>(w + lane * Geo::STRIDE + i) = make_float4(O[i], O[i + 1], O[i + 2], O[i + 3]);
             __syncwarp();
+            if constexpr (DIRECT) ok = warp_wait(smem_u32(&x.l_there[qt]), 0, a.err);
             constexpr int LPR = DW / 4, RPI = 32 / LPR;   // lanes of a row, rows at a time
 #pragma unroll 4
             for (int r = lane / LPR; r < 32; r += RPI) {
                 const int at = x.at[32 * qt + r], d = lane % LPR * 4;
-                if (at >= 0) *reinterpret_cast<float4*>(a.pO + ((size_t)at * (a.ns + a.nwin) + blockIdx.x) * D + d0 + d) = *reinterpret_cast<const float4*>(w + r * Geo::STRIDE + d);
+                if (at < 0) continue;
+                const float4 o = *reinterpret_cast<const float4*>(w + r * Geo::STRIDE + d);
+                if constexpr (DIRECT) put(o, x.end[32 * qt + r], at / a.n_head, at % a.n_head, d0 + d, D, a);
+                else *reinterpret_cast<float4*>(a.pO + ((size_t)at * (a.ns + a.nwin) + blockIdx.x) * D + d0 + d) = o;
             }
         }
     } else {
@@ -465,15 +478,16 @@ __global__ void __launch_bounds__(256) k_paged_f16(const PagedArgs a) {
     }
 }
 
-template <int D, int KIND> int launch_split(const PagedArgs& a, dim3 grid, cudaStream_t s) {
+template <int D, int KIND, bool DIRECT> int launch_split(const PagedArgs& a, dim3 grid, cudaStream_t s) {
     using Geo = PagedGeo<D>;
     static bool attr[MAX_DEVICES] = {};   // per device: the opt-in belongs to the device's copy of the kernel
     const int dev = current_device(); if (dev < 0) return HP_ECUDA;
-    if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_prompt<D, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo::SMEM)); attr[dev] = true; }
+    if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_prompt<D, KIND, DIRECT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo::SMEM)); attr[dev] = true; }
     HP_CUDA(launch_pdl<4>(k_paged_f16<KIND>, dim3(a.tiles, 2 * a.pool.n_kv, a.b.S), dim3(256), 0, s, a));
-    HP_CUDA(launch_pdl<4>(k_paged_prompt<D, KIND>, grid, dim3(Geo::WARPS * 32), Geo::SMEM, s, a));
+    HP_CUDA(launch_pdl<4>(k_paged_prompt<D, KIND, DIRECT>, grid, dim3(Geo::WARPS * 32), Geo::SMEM, s, a));
     return HP_OK;
 }
+template <int D, int KIND> int launch_split(const PagedArgs& a, dim3 grid, cudaStream_t s) { return a.direct ? launch_split<D, KIND, true>(a, grid, s) : launch_split<D, KIND, false>(a, grid, s); }
 template <int KIND> int launch_split(const PagedArgs& a, dim3 grid, cudaStream_t s) {
     return a.pool.head_dim == 256 ? launch_split<256, KIND>(a, grid, s) : a.pool.head_dim == 128 ? launch_split<128, KIND>(a, grid, s) : launch_split<64, KIND>(a, grid, s);
 }

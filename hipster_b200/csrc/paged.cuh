@@ -119,6 +119,38 @@ __device__ __forceinline__ Span span_of(const PagedArgs& a, const Block& blk) {
     v.u0 = (long long)split * a.U; v.u1 = min(v.u0 + a.U, (long long)v.kend);
     return v;
 }
+// sums of a row to its output: quotient and gate
+__device__ __forceinline__ void finish(float4& o, float l, float4 g, const PagedArgs& a) {
+    float x[4] = {0.f + o.x, 0.f + o.y, 0.f + o.z, 0.f + o.w}; const float y[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[e] = l == 0.f ? 0.f : x[e] * a.mul / l;
+        if (a.gate) x[e] = x[e] * sigmoid_det(y[e]);
+    }
+    o = make_float4(x[0], x[1], x[2], x[3]);
+}
+// warp_quant32_store for four dims at k per lane: groups of eight lanes, which are there together, have 32 dims each
+__device__ __forceinline__ void quant_four(float4 x, int r, int k, int K, int8_t* q, float* sc) {
+    const unsigned mask = 0xffu << (threadIdx.x & 24);
+    float amax = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, off));
+    const float dd = amax / 127.f, id = amax > 0.f ? 127.f / amax : 0.f;
+    const int q0 = __float2int_rn(x.x * id), q1 = __float2int_rn(x.y * id), q2 = __float2int_rn(x.z * id), q3 = __float2int_rn(x.w * id);
+    int sum = (q0 + q1) + (q2 + q3);
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(mask, sum, off);
+    *reinterpret_cast<uint32_t*>(q + xq_q_index(r, k, K)) = (q0 & 0xff) | (q1 & 0xff) << 8 | (q2 & 0xff) << 16 | (uint32_t)q3 << 24;   // four bytes of one lane's eight
+    if ((threadIdx.x & 7) == 0) { const size_t di = xq_d_index(r, k >> 5, K); sc[di] = dd; sc[di + 2] = dd * (float)sum; }
+}
+// four dims at d of a row and head, as the merge would write them from one split, bit for bit; eight neighbouring lanes hold 32 dims
+__device__ __forceinline__ void put(float4 o, float l, int r, int h, int d, int D, const PagedArgs& a) {
+    float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.gate) gate = *reinterpret_cast<const float4*>(a.gate + (size_t)r * a.g_ld + (size_t)h * a.g_hs + d);
+    finish(o, l, gate, a);
+    if (a.out) *reinterpret_cast<float4*>(a.out + ((size_t)r * a.n_head + h) * D + d) = o;
+    if (a.oq) quant_four(o, r, h * D + d, a.n_head * D, a.oq, a.osc);
+}
 // power of two that brings the largest magnitude (its bits) to [2^14, 2^15)
 __device__ __forceinline__ int q_exponent(uint32_t m) { return m == 0 || m >= 0x7f800000u ? 0 : min(100, 14 - ((int)(m >> 23) - 127)); }
 
