@@ -495,7 +495,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 5 : 1) k_paged_merge_few(const
 struct Plan { int U, ns, nwin, MB; long long blocks; };
 // Splits lie at multiples of U, which the cache's capacity and the window alone decide (16 to 32 splits and more of a full sequence), so that a row's sums do not hang on what
 // else is in the call. Captured, us: 1 token of 24 heads at 4097, U = 128 12.8, 256 12.6, 512 16.9, 1024 26.6; 48 sequences of up to 8192, 187, 139, 118, 116.
-// Prompts have blocks of rows: their keys are split as the launch fills the GPU best, a split costing the start of a CTA, some six tiles. Sixteen splits at most (eight: 64 rows of 24 heads at 16000 104 us, now 91).
+// Prompts have blocks of rows: their keys are split as the launch fills the GPU best, a split costing the start of a CTA, some six tiles, and several of them
+// the merge (without it in the sum 1000 rows of 24 heads 91 us, now 80). Sixteen splits at most (eight: 64 rows of 24 heads at 16000 104 us, now 91).
 Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink) {
     Plan p;
     const int G = n_head / pool.n_kv, cap = pool.table_ld << pool.lg_page;
@@ -509,7 +510,7 @@ Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window,
         const long long ctas = p.blocks * pool.n_kv, band = (b.max_kv + 1023) / 1024 * 16, tiles = (b.max_kv + 63) / 64;   // of 64 keys; as many splits for all max_kv up to the next 1024: the workspace grows with max_kv
         long long best = 0; int n = 1;
         for (int i = 1; i <= 16; ++i) {
-            const long long cost = (ctas * i + 147) / 148 * ((band + i - 1) / i + 6);
+            const long long cost = (ctas * i + 147) / 148 * ((band + i - 1) / i + 6) + (i == 1 ? 0 : 2 + ((long long)b.R * n_head * pool.head_dim * (i + 1) * 8 >> 20) / 12);   // and the merge, 12 MB in the time of a tile
             if (i == 1 || cost < best) { best = cost; n = i; }
         }
         if (n == 1 || window) { p.U = 1 << 30; p.ns = 0; p.nwin = 1; }
