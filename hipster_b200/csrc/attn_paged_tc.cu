@@ -68,7 +68,8 @@ __device__ __forceinline__ void ld_there(float* a) {   // orders the use of the 
 #pragma unroll
     for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(a[i]));
 }
-// Registers: 640 threads start with 96 each, 61440; eight warps with 152, eight with 72 and four with 32 take all of them (160 and 64: 157 us where this takes 151)
+// Registers: 640 threads start with 96 each, 61440; eight warps with 152, eight with 72 and four with 32 take all of them (160 and 64: 157 us where this took 151).
+// A share holds what is compiled here; a library function with registers of its own (printf) must not be called behind these
 template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void pair_sync(int qt) { asm volatile("bar.sync %0, 64;" ::"r"(qt + 1) : "memory"); }

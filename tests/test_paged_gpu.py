@@ -716,11 +716,12 @@ def test_gates_and_outputs_at_odd_places(D, H, n_kv, rows, lens, window, n_sink)
     assert ((a.double() - exact).abs() <= tol).all() and (a[-1] == 0).all()
 
 
+@pytest.mark.parametrize("window", [0, 5000])   # several splits; one, which writes the outputs itself
 @pytest.mark.parametrize("D,kind", [(64, "i8"), (128, "e4m3"), (256, "i8")])
-def test_non_finite_tokens_in_prompts(D, kind):
+def test_non_finite_tokens_in_prompts(D, kind, window):
     st = Setup([70], [300], 1, D, 16, kind)
     q = torch.randn((70, 5, D), generator=gen(1), device="cuda")
-    run = lambda: K_.attn_paged(q, st.pool, *st.batch, max_rows=70, max_kv=300)[0]  # noqa: E731
+    run = lambda: K_.attn_paged(q, st.pool, *st.batch, max_rows=70, max_kv=300, window=window)[0]  # noqa: E731
     clean = run()
     for scale, bad in itertools.product((st.pool.k_scale, st.pool.v_scale), (math.nan, math.inf)):
         pg, at = st.slot(0, 290)   # seen by the last ten rows
@@ -737,14 +738,14 @@ def test_non_finite_tokens_in_prompts(D, kind):
 
 
 @pytest.mark.parametrize("k_up,v_up", [(1e-12, 1e-12), (1e10, 1e15), (1.0, 1e-25), (1e-30, 1.0)])
-@pytest.mark.parametrize("D", [64, 256])
-def test_magnitudes_in_prompts(D, k_up, v_up):
+@pytest.mark.parametrize("D,window", [(64, 0), (256, 0), (128, 5000), (256, 5000)])
+def test_magnitudes_in_prompts(D, window, k_up, v_up):
     st = Setup([40, 17], [250, 90], 2, D, 16, "e4m3")
     st.pool.k_scale.mul_(k_up)
     st.pool.v_scale.mul_(v_up * torch.exp(3 * torch.randn(st.pool.v_scale.shape, generator=gen(8), device="cuda")))
     st.pool.v_scale[:, :, 3] = 0
     q = torch.randn((57, 8, D), generator=gen(5), device="cuda") / k_up
-    got, _ = K_.attn_paged(q, st.pool, *st.batch, max_rows=40, max_kv=250, scale=0.125)
+    got, _ = K_.attn_paged(q, st.pool, *st.batch, max_rows=40, max_kv=250, scale=0.125, window=window)
     want, tol = attn64(st, q, 0.125, 0, 0, None)
     assert status() == 0 and ((got.double() - want).abs() <= tol).all()
 
