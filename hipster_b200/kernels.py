@@ -308,7 +308,10 @@ def kv_read(pages, table, row_start, kv_len, R=None, k_out=None, v_out=None):
 
 @functools.lru_cache(maxsize=256, typed=True)
 def _attn_paged_workspace_bytes(cols, S, R, max_rows, max_kv, n_head, window, n_sink, kind, n_pages, n_kv, page_size, head_dim):
-    return lib().hp_attn_paged_workspace_bytes(cols, S, R, max_rows, max_kv, n_head, window, n_sink, ctypes.byref(_Pages(None, None, None, None, kind, n_pages, n_kv, page_size, head_dim)))
+    nb = lib().hp_attn_paged_workspace_bytes(cols, S, R, max_rows, max_kv, n_head, window, n_sink, ctypes.byref(_Pages(None, None, None, None, kind, n_pages, n_kv, page_size, head_dim)))
+    if nb == 0:   # refused: raised from here, so that no answer is kept
+        check(1)
+    return nb
 
 
 def attn_paged(q, pages, table, row_start, kv_len, max_rows, max_kv, scale=None, window=0, n_sink=0, gate=None, want_f32=True, want_q8=False):
@@ -324,7 +327,8 @@ def attn_paged(q, pages, table, row_start, kv_len, max_rows, max_kv, scale=None,
     qr = _rows(q, pages, R, n_head, "q")
     gr = (None, 0, 0) if gate is None else _rows(gate, pages, R, n_head, "gate")
     c = pages._c
-    nb = _attn_paged_workspace_bytes(at[1], S, R, max_rows, -(-max_kv // 1024) * 1024, n_head, window, n_sink, c.type, c.n_pages, c.n_kv, c.page_size, c.head_dim)   # grows with max_kv
+    cap = at[1] * pages.page_size   # as the library bounds max_kv; rounded up, INT_MAX would leave the ints
+    nb = _attn_paged_workspace_bytes(at[1], S, R, max_rows, min(-(-max_kv // 1024) * 1024, cap), n_head, window, n_sink, c.type, c.n_pages, c.n_kv, c.page_size, c.head_dim)   # grows with max_kv
     ws = q.new_empty(nb // 4 + 4)
     out = q.new_empty((R, n_head, D)) if want_f32 else None
     xq = XQ8(R, n_head * D, pages.device) if want_q8 else None
