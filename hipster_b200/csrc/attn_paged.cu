@@ -499,7 +499,7 @@ struct Plan { int U, ns, nwin, MB; long long blocks; };
 // the merge (without it in the sum 1000 rows of 24 heads 91 us, now 80). Sixteen splits at most (eight: 64 rows of 24 heads at 16000 104 us, now 91).
 Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink) {
     Plan p;
-    const int G = n_head / pool.n_kv, cap = pool.table_ld << pool.lg_page;
+    const int G = n_head / pool.n_kv, cap = pool.columns << pool.lg_page;
     const long long eff = window ? std::min<long long>(cap, (long long)window + n_sink) : cap;
     const long long pairs = (long long)b.max_rows * G;
     const bool prompt = b.max_rows > PAGED_DECODE_ROWS;

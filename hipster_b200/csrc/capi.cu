@@ -240,14 +240,15 @@ int paged_args(const char* who, const hp_kv_pages* c, const int* table, int tabl
     HP_REQUIRE(c->type == HP_KV_I8 || c->type == HP_KV_E4M3, "%s: unknown cache type %d", who, c->type);
     HP_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "%s: head_dim must be 64, 128 or 256, not %d", who, c->head_dim);
     HP_REQUIRE(c->page_size >= 16 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0, "%s: page_size must be a power of two from 16 to 1024, not %d", who, c->page_size);
-    HP_REQUIRE(c->n_pages >= 1 && c->n_kv >= 1 && table_ld >= 1 && (long long)c->n_pages * c->n_kv < (0xffffffffll / c->page_size) && (long long)table_ld * c->page_size < (1ll << 30),
-               "%s: bad cache n_pages=%d n_kv=%d table_ld=%d", who, c->n_pages, c->n_kv, table_ld);
+    const int columns = c->columns ? c->columns : table_ld;
+    HP_REQUIRE(c->n_pages >= 1 && c->n_kv >= 1 && columns >= 1 && columns <= table_ld && (long long)c->n_pages * c->n_kv < (0xffffffffll / c->page_size) && (long long)columns * c->page_size < (1ll << 30),
+               "%s: bad cache n_pages=%d n_kv=%d table_ld=%d columns=%d", who, c->n_pages, c->n_kv, table_ld, c->columns);
     HP_REQUIRE(S >= 1 && R >= 1 && max_rows >= 1 && max_kv >= 1, "%s: bad batch S=%d R=%d max_rows=%lld max_kv=%lld", who, S, R, max_rows, max_kv);
-    p->k = (uint8_t*)c->k; p->v = (uint8_t*)c->v; p->k_scale = c->k_scale; p->v_scale = c->v_scale; p->table = table; p->table_ld = table_ld;
+    p->k = (uint8_t*)c->k; p->v = (uint8_t*)c->v; p->k_scale = c->k_scale; p->v_scale = c->v_scale; p->table = table; p->table_ld = table_ld; p->columns = columns;
     p->kind = c->type; p->n_pages = c->n_pages; p->n_kv = c->n_kv; p->head_dim = c->head_dim; p->lg_page = 0;
     while ((1 << p->lg_page) < c->page_size) ++p->lg_page;
     b->row_start = row_start; b->kv_len = kv_len; b->S = S; b->R = R;
-    b->max_rows = (int)(max_rows < R ? max_rows : R); b->max_kv = (int)std::min<long long>(max_kv, (long long)table_ld * c->page_size);
+    b->max_rows = (int)(max_rows < R ? max_rows : R); b->max_kv = (int)std::min<long long>(max_kv, (long long)columns * c->page_size);
     return HP_OK;
 }
 int paged_ptrs(const char* who, const hp_kv_pages* c, const int* table, const int* row_start, const int* kv_len) {

@@ -185,7 +185,7 @@ int accept_greedy(const int* ids, const int* drafts, int n_draft, int* out, cuda
 enum : int { KV_I8 = 0, KV_E4M3 = 1 };
 struct PagedPool {
     uint8_t* k; uint8_t* v; float* k_scale; float* v_scale;   // codes [n_pages][n_kv][page][head_dim], scales [n_pages][n_kv][page]
-    const int* table; int table_ld;                           // [S][table_ld]
+    const int* table; int table_ld, columns;                  // [S][table_ld], of which `columns` are in use
     int kind, n_pages, n_kv, lg_page, head_dim;
 };
 struct PagedBatch { const int* row_start; const int* kv_len; int S, R, max_rows, max_kv; };   // max_rows, max_kv: bounds that the host knows

@@ -30,15 +30,15 @@ bool rows(PyObject* o, int dev, int64_t R, int64_t heads, int64_t D, Rows* out) 
     out->p = static_cast<float*>(t->data_ptr()); out->ld = t->stride(0); out->hs = t->stride(1);
     return true;
 }
-struct Batch { const int* table; int ld; const int* row_start; const int* kv_len; int S; };
+struct Batch { const int* table; int ld, cols; const int* row_start; const int* kv_len; int S; };
 bool batch(PyObject* table, PyObject* row_start, PyObject* kv_len, int dev, Batch* out) {
     const at::Tensor *t = tensor(table), *r = tensor(row_start), *k = tensor(kv_len);
     if (!on(t, dev, at::kInt) || !on(r, dev, at::kInt) || !on(k, dev, at::kInt) || t->dim() != 2) return false;
     const int64_t S = k->numel(), cols = t->size(1);
-    if (S < 1 || S > INT_MAX || t->size(0) != S || r->numel() != S + 1 || t->stride(1) != 1 || (S > 1 && t->stride(0) < cols) || !r->is_contiguous() || !k->is_contiguous()) return false;
-    const int64_t ld = S > 1 ? t->stride(0) : std::max<int64_t>(cols, 1);
+    if (S < 1 || S > INT_MAX || t->size(0) != S || r->numel() != S + 1 || t->stride(1) != 1 || cols < 1 || (S > 1 && t->stride(0) < cols) || !r->is_contiguous() || !k->is_contiguous()) return false;
+    const int64_t ld = S > 1 ? t->stride(0) : cols;
     if (ld > INT_MAX) return false;
-    *out = Batch{static_cast<const int*>(t->data_ptr()), (int)ld, static_cast<const int*>(r->data_ptr()), static_cast<const int*>(k->data_ptr()), (int)S};
+    *out = Batch{static_cast<const int*>(t->data_ptr()), (int)ld, (int)cols, static_cast<const int*>(r->data_ptr()), static_cast<const int*>(k->data_ptr()), (int)S};
     return true;
 }
 bool norm_weight(PyObject* o, int dev, int64_t D, const void** out) {
@@ -49,6 +49,8 @@ bool norm_weight(PyObject* o, int dev, int64_t D, const void** out) {
     return true;
 }
 const hp_kv_pages* pages(PyObject* o) { return reinterpret_cast<const hp_kv_pages*>(PyLong_AsSsize_t(o)); }
+// the cache as this call sees it: a table that is part of a wider one ends with its own columns
+hp_kv_pages with_columns(const hp_kv_pages* c, const Batch& b) { hp_kv_pages o = *c; o.columns = b.cols; return o; }
 bool whole(PyObject* o, int64_t* out) {   // an int that fits; floats and the like are for kernels.py to judge
     if (!PyLong_CheckExact(o)) return false;
     int over; *out = PyLong_AsLongLongAndOverflow(o, &over);
@@ -88,10 +90,11 @@ PyObject* py_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (a[9] == Py_None) { out = at::empty({R, n_head, c->head_dim}, options((int)dev, at::kFloat)); qo = Rows{static_cast<float*>(out.data_ptr()), (long long)n_head * c->head_dim, c->head_dim}; }
         else { if (!rows(a[9], (int)dev, R, n_head, c->head_dim, &qo)) Py_RETURN_NONE; out = *tensor(a[9]); }
     } else if (a[9] != Py_None) Py_RETURN_NONE;
+    const hp_kv_pages view = with_columns(c, b);
     const int inter = PyObject_IsTrue(a[10]);
     if (inter < 0) PyErr_Clear();
     void* s = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
-    if (inter < 0 || outside([&] { return f_append(q.p, q.ld, q.hs, qo.p, qo.ld, qo.hs, n_head, k.p, k.ld, k.hs, v.p, v.ld, v.hs, qn, kn, rope, n_pos, n_rot, inter, b.table, b.ld, b.row_start, b.kv_len, b.S, (int)R, c, (float)eps, s); })) Py_RETURN_NONE;
+    if (inter < 0 || outside([&] { return f_append(q.p, q.ld, q.hs, qo.p, qo.ld, qo.hs, n_head, k.p, k.ld, k.hs, v.p, v.ld, v.hs, qn, kn, rope, n_pos, n_rot, inter, b.table, b.ld, b.row_start, b.kv_len, b.S, (int)R, &view, (float)eps, s); })) Py_RETURN_NONE;
     if (a[8] == Py_None) Py_RETURN_TRUE;
     if (a[9] != Py_None) { Py_INCREF(a[9]); return a[9]; }
     return THPVariable_Wrap(std::move(out));
@@ -104,9 +107,10 @@ PyObject* py_kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TRY
     const hp_kv_pages* c = pages(a[0]);
     if (c10::cuda::current_device() != dev || !batch(a[2], a[3], a[4], (int)dev, &b)) Py_RETURN_NONE;
+    const hp_kv_pages view = with_columns(c, b);
     at::Tensor k = at::empty({R, c->n_kv, c->head_dim}, options((int)dev, at::kHalf)), v = at::empty({R, c->n_kv, c->head_dim}, options((int)dev, at::kHalf));
     void* s = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
-    if (outside([&] { return f_read(b.table, b.ld, b.row_start, b.kv_len, b.S, (int)R, c, k.data_ptr(), v.data_ptr(), (long long)c->n_kv * c->head_dim, c->head_dim, s); })) Py_RETURN_NONE;
+    if (outside([&] { return f_read(b.table, b.ld, b.row_start, b.kv_len, b.S, (int)R, &view, k.data_ptr(), v.data_ptr(), (long long)c->n_kv * c->head_dim, c->head_dim, s); })) Py_RETURN_NONE;
     PyObject *pk = THPVariable_Wrap(std::move(k)), *pv = THPVariable_Wrap(std::move(v)), *r = pk && pv ? PyTuple_Pack(2, pk, pv) : nullptr;
     Py_XDECREF(pk); Py_XDECREF(pv);
     return r;
@@ -123,11 +127,12 @@ PyObject* py_attn_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (c10::cuda::current_device() != dev || !t || t->dim() != 3 || t->size(0) < 1 || t->size(0) > INT_MAX || t->size(1) > INT_MAX || !batch(a[4], a[5], a[6], (int)dev, &b)) Py_RETURN_NONE;
     const int64_t R = t->size(0), H = t->size(1);
     if (!rows(a[2], (int)dev, R, H, c->head_dim, &q) || (a[3] != Py_None && !rows(a[3], (int)dev, R, H, c->head_dim, &g))) Py_RETURN_NONE;
-    const size_t bytes = f_bytes(b.ld, b.S, (int)R, (int)max_rows, (int)max_kv, (int)H, (int)window, (int)n_sink, c);
+    const hp_kv_pages view = with_columns(c, b);
+    const size_t bytes = f_bytes(b.ld, b.S, (int)R, (int)max_rows, (int)max_kv, (int)H, (int)window, (int)n_sink, &view);
     if (!bytes) Py_RETURN_NONE;
     at::Tensor out = at::empty({R, H, c->head_dim}, options((int)dev, at::kFloat)), ws = at::empty({(int64_t)bytes}, options((int)dev, at::kByte));
     void* s = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
-    if (outside([&] { return f_attn(q.p, q.ld, q.hs, g.p, g.ld, g.hs, (int)H, b.table, b.ld, b.row_start, b.kv_len, b.S, (int)R, (int)max_rows, (int)max_kv, c, (float)scale, (int)window, (int)n_sink,
+    if (outside([&] { return f_attn(q.p, q.ld, q.hs, g.p, g.ld, g.hs, (int)H, b.table, b.ld, b.row_start, b.kv_len, b.S, (int)R, (int)max_rows, (int)max_kv, &view, (float)scale, (int)window, (int)n_sink,
                                     static_cast<float*>(out.data_ptr()), nullptr, nullptr, ws.data_ptr(), s); })) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
     CATCH

@@ -169,7 +169,7 @@ _F32, _I32, _F16 = torch.float32, torch.int32, torch.float16
 
 
 class _Pages(ctypes.Structure):   # hp_kv_pages
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)] + [(n, ctypes.c_int) for n in ("type", "n_pages", "n_kv", "page_size", "head_dim")]
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)] + [(n, ctypes.c_int) for n in ("type", "n_pages", "n_kv", "page_size", "head_dim", "columns")]
 
 
 def _refuse(ok, what):
@@ -200,18 +200,25 @@ class KVPages:
 # Calls whose arguments are in order are taken by _lib.tensors(), in C++ (None: not taken). What follows takes the others, says what is wrong with them, and takes all calls
 # where that module was not built: it, too, reads each attribute once and makes no message before a test fails.
 def _batch(pages, table, row_start, kv_len):
-    """Checks what describes a ragged batch; -> number of sequences, and its addresses as the calls take them."""
+    """Checks what describes a ragged batch; -> number of sequences, the cache as the call sees it (hp_kv_pages: a table that is part of a wider one ends with its own
+    columns), and the batch's addresses as the calls take them."""
     dev, S = pages._dev, kv_len.numel()
     (rows, cols), (ld, one) = table.shape, table.stride()
     if dev != _device():
         raise HipsterError(1, f"the pages are on device {dev}, and device {_device()} is current")
     if not (table.dtype is _I32 and row_start.dtype is _I32 and kv_len.dtype is _I32):
         raise HipsterError(1, "table, row_start and kv_len must be int32")
-    if not (rows == S and row_start.numel() == S + 1 and one == 1 and (ld >= cols or S == 1) and row_start.is_contiguous() and kv_len.is_contiguous()):
-        raise HipsterError(1, "table [S][columns], row_start [S + 1] and kv_len [S] must be contiguous")
+    if not (rows == S and row_start.numel() == S + 1 and one == 1 and cols and (ld >= cols or S == 1) and row_start.is_contiguous() and kv_len.is_contiguous()):
+        raise HipsterError(1, "table must be [S][columns], in rows without gaps, row_start [S + 1] and kv_len [S] contiguous")
     if not (table.get_device() == dev and row_start.get_device() == dev and kv_len.get_device() == dev):
         raise HipsterError(1, "table, row_start and kv_len must be on the device of the pages")
-    return S, table.data_ptr(), ld if S > 1 else max(cols, 1), row_start.data_ptr(), kv_len.data_ptr()
+    if S == 1:
+        ld = cols
+    c = pages._c
+    if ld != cols:
+        c = _Pages.from_buffer_copy(c)
+        c.columns = cols
+    return S, c, table.data_ptr(), ld, row_start.data_ptr(), kv_len.data_ptr()
 
 
 def _rows(t, pages, R, heads, what):
@@ -261,7 +268,7 @@ def kv_append(pages, k, v, table, row_start, kv_len, rope=None, q=None, q_out=No
         out = fast.kv_append(pages._at, pages._dev, k, v, table, row_start, kv_len, rope, q, q_out, interleaved, q_norm, k_norm, eps)
         if out is not None:
             return None if out is True else out
-    S, *at = _batch(pages, table, row_start, kv_len)
+    S, c, *at = _batch(pages, table, row_start, kv_len)
     R, n_kv = k.shape[0], pages.n_kv
     qr = qo = (None, 0, 0)
     n_head = n_pos = n_rot = 0
@@ -278,7 +285,7 @@ def kv_append(pages, k, v, table, row_start, kv_len, rope=None, q=None, q_out=No
             raise HipsterError(1, "kv_append: rope must be f32 [n_pos][n_rot / 2][2]")
         rope = rope.data_ptr()
     check(hot().hp_kv_append(*qr, *qo, n_head, *_rows(k, pages, R, n_kv, "k"), *_rows(v, pages, R, n_kv, "v"), _norm_weight(q_norm, pages), _norm_weight(k_norm, pages), rope, n_pos, n_rot, int(interleaved),
-                             *at, S, R, pages._at, eps, _raw_stream(pages._dev)))
+                             *at, S, R, ctypes.addressof(c), eps, _raw_stream(pages._dev)))
     return q_out
 
 
@@ -290,7 +297,7 @@ def kv_read(pages, table, row_start, kv_len, R=None, k_out=None, v_out=None):
         out = fast.kv_read(pages._at, pages._dev, table, row_start, kv_len, R)
         if out is not None:
             return out
-    S, *at = _batch(pages, table, row_start, kv_len)
+    S, c, *at = _batch(pages, table, row_start, kv_len)
     n_kv, D = pages.n_kv, pages.head_dim
     if k_out is None and v_out is None and R is not None:
         k_out, v_out = pages._f16.new_empty((R, n_kv, D)), pages._f16.new_empty((R, n_kv, D))
@@ -302,7 +309,7 @@ def kv_read(pages, table, row_start, kv_len, R=None, k_out=None, v_out=None):
         if not (k_out.shape == (R, n_kv, D) and v_out.shape == k_out.shape and v_out.stride() == (ld, hs, 1) and one == 1 and k_out.dtype is _F16 and v_out.dtype is _F16 and
                 k_out.get_device() == pages._dev and v_out.get_device() == pages._dev):
             raise HipsterError(1, "kv_read: outputs are f16 [R][n_kv][head_dim] with the same strides")
-    check(hot().hp_kv_read(*at, S, R, pages._at, k_out.data_ptr(), v_out.data_ptr(), ld, hs, _raw_stream(pages._dev)))
+    check(hot().hp_kv_read(*at, S, R, ctypes.addressof(c), k_out.data_ptr(), v_out.data_ptr(), ld, hs, _raw_stream(pages._dev)))
     return k_out, v_out
 
 
@@ -323,15 +330,15 @@ def attn_paged(q, pages, table, row_start, kv_len, max_rows, max_kv, scale=None,
         out = fast.attn_paged(pages._at, pages._dev, q, gate, table, row_start, kv_len, max_rows, max_kv, scale, window, n_sink)
         if out is not None:
             return out, None
-    (S, *at), (R, n_head, D) = _batch(pages, table, row_start, kv_len), q.shape
+    (S, c, *at), (R, n_head, D) = _batch(pages, table, row_start, kv_len), q.shape
     qr = _rows(q, pages, R, n_head, "q")
     gr = (None, 0, 0) if gate is None else _rows(gate, pages, R, n_head, "gate")
-    c = pages._c
-    cap = at[1] * pages.page_size   # as the library bounds max_kv; rounded up, INT_MAX would leave the ints
-    nb = _attn_paged_workspace_bytes(at[1], S, R, max_rows, min(-(-max_kv // 1024) * 1024, cap), n_head, window, n_sink, c.type, c.n_pages, c.n_kv, c.page_size, c.head_dim)   # grows with max_kv
+    cols = table.shape[1]
+    cap = cols * pages.page_size   # as the library bounds max_kv; rounded up, INT_MAX would leave the ints
+    nb = _attn_paged_workspace_bytes(cols, S, R, max_rows, min(-(-max_kv // 1024) * 1024, cap), n_head, window, n_sink, c.type, c.n_pages, c.n_kv, c.page_size, c.head_dim)   # grows with max_kv
     ws = q.new_empty(nb // 4 + 4)
     out = q.new_empty((R, n_head, D)) if want_f32 else None
     xq = XQ8(R, n_head * D, pages.device) if want_q8 else None
-    check(hot().hp_attn_paged(*qr, *gr, n_head, *at, S, R, max_rows, max_kv, pages._at, D ** -0.5 if scale is None else scale, window, n_sink, None if out is None else out.data_ptr(),
+    check(hot().hp_attn_paged(*qr, *gr, n_head, *at, S, R, max_rows, max_kv, ctypes.addressof(c), D ** -0.5 if scale is None else scale, window, n_sink, None if out is None else out.data_ptr(),
                               xq.q.data_ptr() if xq else None, xq.sc.data_ptr() if xq else None, ws.data_ptr(), _raw_stream(pages._dev)))
     return out, xq

@@ -130,11 +130,11 @@ int hp_moe_layer(const float* xn_dev, const void* xq_q_dev, const void* xq_sc_de
  *
  * hp_kv_pages describes a cache (host struct, read during the call). k, v: [n_pages][n_kv][page_size][head_dim] bytes, 16-byte aligned; k_scale, v_scale: f32
  * [n_pages][n_kv][page_size]. page_size: a power of two, 16 to 1024; head_dim: 64, 128 or 256.
- * A batch: table_dev, int [S][table_ld], holds the page of positions [i * page_size, (i + 1) * page_size) of each sequence, which has at most table_ld * page_size
- * tokens. Sequences may share pages to read; the slots that one call appends to must be distinct. Rows [row_start[s], row_start[s + 1]) are the newest tokens of sequence s, which has kv_len[s] tokens with them, so that its row t is at
+ * A batch: table_dev, int [S][table_ld], holds the page of positions [i * page_size, (i + 1) * page_size) of each sequence, which has at most columns * page_size
+ * tokens: with `columns` of hp_kv_pages set, table_dev may be a part of a wider table, and what lies beside these columns is not read. Sequences may share pages to read; the slots that one call appends to must be distinct. Rows [row_start[s], row_start[s + 1]) are the newest tokens of sequence s, which has kv_len[s] tokens with them, so that its row t is at
  * position kv_len[s] - T + t. row_start (S + 1 ints) and kv_len (S ints) are device memory like the table, read when the kernels run: a captured call can be
  * replayed with other lengths. R is the number of rows that the buffers hold: rows behind row_start[S] are neither read nor written. Entries that do
- * not fit (rows outside of [0, R), a sequence with more rows than max_rows or more tokens than max_kv, table_ld * page_size or the rotary table, a
+ * not fit (rows outside of [0, R), a sequence with more rows than max_rows or more tokens than max_kv, columns * page_size or the rotary table, a
  * page number outside of [0, n_pages) of a token that is used) fault nothing: what does not fit is left out (append, read) or makes the outputs of its
  * sequence meaningless (attention), and hp_device_status returns HP_EINVAL. Rows of negative position are not appended, read back or
  * normalised (HP_EINVAL), and attend to nothing. Row strides (ld) and head strides (hs) are in elements; those of outputs are nested, rows in heads or heads in
@@ -143,6 +143,7 @@ enum { HP_KV_I8 = 0, HP_KV_E4M3 = 1 };
 typedef struct hp_kv_pages {
     void* k; void* v; float* k_scale; float* v_scale;
     int type, n_pages, n_kv, page_size, head_dim;
+    int columns;   /* of the batch's table that are in use, at most table_ld; 0: table_ld */
 } hp_kv_pages;
 /* table_dev f32 [n_pos][n_rot / 2][2] = (cos, sin) of pos * f_i, f_i = base^(-2 i / n_rot): the rope_dev of hp_attn_decode and hp_kv_append. Scaled for
  * contexts beyond the trained one: HP_ROPE_LINEAR f_i / factor; HP_ROPE_YARN (by parts; Peng et al. 2023) with r_i = orig_ctx * f_i / (2 pi) and
@@ -164,7 +165,7 @@ int hp_kv_read(const int* table_dev, int table_ld, const int* row_start_dev, con
  * j > pos - window or j < n_sink (first tokens that stay visible; pages without a visible token are not looked up). n_head a multiple of n_kv; head h reads kv head
  * h / (n_head / n_kv). gate_dev (nullable): the output is multiplied by sigmoid(gate). out_dev f32 [R][n_head * head_dim] and / or its int8 quantisation (K = n_head * head_dim),
  * either may be NULL. max_rows, max_kv: bounds of a sequence's rows and tokens; they size the launch (R bounds max_rows too). Up to 16 rows per sequence (decode
- * steps, drafts, verify passes) a row's result depends neither on the other rows of its sequence nor on the other sequences, bit for bit (for one table_ld, window and
+ * steps, drafts, verify passes) a row's result depends neither on the other rows of its sequence nor on the other sequences, bit for bit (for one number of columns, window and
  * n_sink). Calls of more rows (prompts) turn the keys and values into f16 in the workspace, which then holds S * n_kv * max_kv * (4 * head_dim + 8) bytes besides the
  * partial outputs, and sum a row's keys in another order; a sequence of few rows and many tokens takes its time on few SMs there.
  * workspace_dev: hp_attn_paged_workspace_bytes of the same arguments, 16-byte aligned, of this call alone until it is done (captured calls that may run at once need one each). */

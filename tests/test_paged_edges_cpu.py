@@ -66,3 +66,55 @@ def test_a_workspace_that_the_library_refuses_ends_the_call(recorded):
             with pytest.raises(hb.HipsterError, match="bad"):
                 K_.attn_paged(q, pages, torch.zeros((1, 64), dtype=torch.int32), i32([0, 1]), i32([1]), **kw)
     assert not recorded.calls
+
+
+def columns_seen(recorded, monkeypatch, call):
+    """(table, table_ld, columns) of the cache and batch that each call hands over."""
+    seen = []
+
+    class Reads:
+        def __getattr__(self, name):
+            at, table = {"hp_kv_append": (25, 19), "hp_kv_read": (6, 0), "hp_attn_paged": (15, 7)}[name]
+
+            def f(*a):
+                seen.append((a[table], a[table + 1], K_._Pages.from_address(a[at]).columns))
+                return 0
+            return f
+    monkeypatch.setattr(K_, "hot", lambda: Reads())
+    call()
+    return seen
+
+
+def test_a_table_that_is_part_of_a_wider_one_ends_with_its_columns(recorded, monkeypatch):
+    """What is handed to the library says where the columns of table[:, a:b] end: what lies beside them is not the caller's to use here."""
+    pages = K_.KVPages.empty(70, 2, 16, 64, device="cpu")
+    big = torch.zeros((2, 9), dtype=torch.int32)
+    x = torch.zeros((2, 2, 64))
+    for a, b in ((0, 4), (3, 9), (8, 9), (0, 9)):
+        t, rs, kl = big[:, a:b], i32([0, 1, 2]), i32([1, 1])
+
+        def call():
+            K_.kv_append(pages, x, x, t, rs, kl)
+            K_.kv_read(pages, t, rs, kl, R=2)
+            K_.attn_paged(x, pages, t, rs, kl, max_rows=1, max_kv=1000)
+        seen = columns_seen(recorded, monkeypatch, call)
+        assert len(seen) == 3 and all(at == t.data_ptr() and (cols or ld) == b - a and (cols == 0 or ld == 9) for at, ld, cols in seen)
+    one = columns_seen(recorded, monkeypatch, lambda: K_.kv_read(pages, big[1:, 2:5], i32([0, 1]), i32([1]), R=1))
+    assert [(cols or ld) for _, ld, cols in one] == [3] and pages._c.columns == 0
+    with pytest.raises(hb.HipsterError, match="table"):
+        K_.kv_read(pages, big[:, :0], i32([0, 1, 2]), i32([1, 1]), R=2)
+
+
+def test_columns_of_a_cache():
+    L, F = hb.lib(), 1 << 20
+    pages = lambda n: K_._Pages(F, F, F, F, 0, 8, 2, 16, 64, n)  # noqa: E731
+    v, z = ctypes.c_void_p, ctypes.c_longlong
+
+    def read(n, ld=4):
+        return L.hp_kv_read(v(F), ld, v(F), v(F), 2, 4, ctypes.byref(pages(n)), v(F), v(F), z(128), z(8), None)   # refused for its head stride, if not before
+    for n, ld in ((5, 4), (-1, 4), (1 << 26, 1 << 27)):
+        assert read(n, ld) == 1 and "columns" in L.hp_last_error().decode()
+    for n, ld in ((4, 4), (0, 4), (1, 4), (4, 1 << 27)):
+        assert read(n, ld) == 1 and "over each other" in L.hp_last_error().decode()
+    f = lambda n, ld, mk=10 ** 6: L.hp_attn_paged_workspace_bytes(ld, 4, 8, 2, mk, 4, 0, 0, ctypes.byref(pages(n)))  # noqa: E731
+    assert f(64, 5000) == f(0, 64) > 0   # the split of the keys, too, goes by the columns in use

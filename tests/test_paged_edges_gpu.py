@@ -38,3 +38,39 @@ def test_bounds_beyond_every_sequence(form, rows, max_kv):
         assert status() == 0 and ((got.double() - want).abs() <= tol).all()
         if q8:
             assert all(torch.equal(a, b) for a, b in zip(xq.unpack(), K_.quantize_x_q8(got.view(rows, -1)).unpack()))
+
+
+@pytest.mark.parametrize("a,b", [(0, 3), (2, 5), (5, 8)])
+def test_tables_that_are_part_of_wider_ones(form, a, b):
+    """table[:, a:b]: the same bits as with a table of its own; lengths beyond its columns are told, and the neighbouring columns' pages neither written nor read."""
+    page, D = 16, 64
+    st = Setup([2, 2], [20, 40], 1, D, page, "i8", cols=3, spare=12)
+    foreign = torch.tensor(st.spare[:12], dtype=torch.int32, device="cuda")
+    wide = foreign[torch.arange(16, device="cuda") % 12].view(2, 8).contiguous()
+    wide[:, a:b] = st.table
+    view = wide[:, a:b]
+    x = torch.randn((4, 2, D), generator=gen(1), device="cuda")
+    k = x[:, :1]
+    pool = lambda: [t.view(torch.uint8).clone() if t.dtype != torch.float32 else t.clone() for t in (st.pool.k, st.pool.v, st.pool.k_scale, st.pool.v_scale)]  # noqa: E731
+    outs = []
+    for t in (st.table, view):
+        K_.kv_append(st.pool, k, k, t, st.row_start, st.kv_len)
+        outs.append((*K_.kv_read(st.pool, t, st.row_start, st.kv_len, R=4), K_.attn_paged(x, st.pool, t, st.row_start, st.kv_len, max_rows=2, max_kv=100)[0],
+                     K_.attn_paged(x, st.pool, t, st.row_start, st.kv_len, max_rows=20, max_kv=100, want_q8=True)[0], *pool()))
+        assert status() == 0
+    assert all(torch.equal(u, w) for u, w in zip(*outs))
+    for n in (49, 60, 128, 129, 2 ** 31 - 1):   # beyond three pages; of each sequence in turn
+        for s in (0, 1):
+            kl = st.kv_len.clone()
+            kl[s] = n
+            st.pool.k_scale[foreign.long()] = math.nan   # what reads them shows
+            before = pool()
+            K_.kv_append(st.pool, k, k, view, st.row_start, kl)
+            assert status() == 1
+            for old, now in zip(before, pool()):
+                assert torch.equal(old[foreign.long()].view(torch.uint8), now[foreign.long()].view(torch.uint8))
+            back = K_.kv_read(st.pool, view, st.row_start, kl, R=4)[0]
+            assert status() == 1 and torch.isfinite(back[[2, 3] if s == 0 else [0, 1]]).all()
+            for mr in (2, 20):
+                got = K_.attn_paged(x, st.pool, view, st.row_start, kl, max_rows=mr, max_kv=2 ** 31 - 1)[0]
+                assert status() == 1 and torch.isfinite(got[2:] if s == 0 else got).all()   # the first one's third column is -1
