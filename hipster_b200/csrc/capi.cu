@@ -283,6 +283,7 @@ int hp_kv_append(const float* q_dev, long long q_ld, long long q_hs, float* q_ou
     HP_REQUIRE(k_dev && v_dev && n_head >= 0 && (n_head == 0 || (q_dev && q_out_dev)) && (n_rot == 0 || rope_dev), "hp_kv_append: null pointer");
     HP_REQUIRE(n_rot >= 0 && n_rot % 2 == 0 && n_rot <= pool.head_dim && (n_rot == 0 || n_pos >= 1) && ((uintptr_t)rope_dev & 7) == 0, "hp_kv_append: bad n_rot=%d n_pos=%d or rope table", n_rot, n_pos);
     HP_REQUIRE(rows_ok(k_dev, k_ld, k_hs) && rows_ok(v_dev, v_ld, v_hs) && (n_head == 0 || (rows_ok(q_dev, q_ld, q_hs) && rows_ok(q_out_dev, qo_ld, qo_hs))), "hp_kv_append: rows must be 16-byte aligned, with strides that are multiples of 4");
+    HP_REQUIRE((((uintptr_t)q_norm_bf16_dev | (uintptr_t)k_norm_bf16_dev) & 1) == 0, "hp_kv_append: norm weights must be 2-byte aligned");
     HP_REQUIRE(n_head == 0 || apart(R, qo_ld, n_head, qo_hs, pool.head_dim), "hp_kv_append: rows of q_out lie over each other");
     HP_REQUIRE((long long)R * (n_head + 2 * pool.n_kv) < (1ll << 33), "hp_kv_append: too many rows");
     hp::KvAppendParams p; p.q = q_dev; p.q_ld = q_ld; p.q_hs = q_hs; p.q_out = q_out_dev; p.qo_ld = qo_ld; p.qo_hs = qo_hs; p.n_head = n_head; p.k = k_dev; p.k_ld = k_ld; p.k_hs = k_hs;
@@ -318,6 +319,7 @@ int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const floa
       if (!rc) rc = attn_paged_check("hp_attn_paged", n_head, window, n_sink, pool); if (rc) return rc; }
     HP_REQUIRE(q_dev && workspace_dev && (out_dev || xq_q_dev), "hp_attn_paged: null pointer");
     HP_REQUIRE((xq_q_dev == nullptr) == (xq_sc_dev == nullptr), "hp_attn_paged: give both quantised-output buffers or neither");
+    HP_REQUIRE((((uintptr_t)xq_q_dev | (uintptr_t)xq_sc_dev) & 15) == 0, "hp_attn_paged: quantised outputs must be 16-byte aligned");
     HP_REQUIRE(rows_ok(q_dev, q_ld, q_hs) && (!gate_dev || (((uintptr_t)gate_dev & 3) == 0 && g_ld >= 0 && g_hs >= 0)) && ((uintptr_t)workspace_dev & 15) == 0 && ((uintptr_t)out_dev & 3) == 0,
                "hp_attn_paged: rows and workspace must be 16-byte aligned, with strides that are multiples of 4");
     HP_REQUIRE(scale > 0 && scale < 1e30f, "hp_attn_paged: bad scale");

@@ -163,8 +163,8 @@ int hp_kv_append(const float* q_dev, long long q_ld, long long q_hs, float* q_ou
 int hp_kv_read(const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, void* k_out_f16_dev, void* v_out_f16_dev, long long row_stride, long long head_stride, void* stream);
 /* Attention of the rows over their sequences' pages: softmax(scale * q k^T) v in fp32 over the keys j <= pos, with window > 0 only those with
  * j > pos - window or j < n_sink (first tokens that stay visible; pages without a visible token are not looked up). n_head a multiple of n_kv; head h reads kv head
- * h / (n_head / n_kv). gate_dev (nullable): the output is multiplied by sigmoid(gate). out_dev f32 [R][n_head * head_dim] and / or its int8 quantisation (K = n_head * head_dim),
- * either may be NULL. max_rows, max_kv: bounds of a sequence's rows and tokens; they size the launch (R bounds max_rows too). Up to 16 rows per sequence (decode
+ * h / (n_head / n_kv). gate_dev (nullable): the output is multiplied by sigmoid(gate). out_dev f32 [R][n_head * head_dim] and / or its int8 quantisation (K = n_head * head_dim; both
+ * buffers 16-byte aligned), either may be NULL. max_rows, max_kv: bounds of a sequence's rows and tokens; they size the launch (R bounds max_rows too). Up to 16 rows per sequence (decode
  * steps, drafts, verify passes) a row's result depends neither on the other rows of its sequence nor on the other sequences, bit for bit (for one number of columns, window and
  * n_sink). Calls of more rows (prompts) turn the keys and values into f16 in the workspace, which then holds S * n_kv * max_kv * (4 * head_dim + 8) bytes besides the
  * partial outputs, and sum a row's keys in another order; a sequence of few rows and many tokens takes its time on few SMs there.

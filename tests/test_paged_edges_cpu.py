@@ -118,3 +118,16 @@ def test_columns_of_a_cache():
         assert read(n, ld) == 1 and "over each other" in L.hp_last_error().decode()
     f = lambda n, ld, mk=10 ** 6: L.hp_attn_paged_workspace_bytes(ld, 4, 8, 2, mk, 4, 0, 0, ctypes.byref(pages(n)))  # noqa: E731
     assert f(64, 5000) == f(0, 64) > 0   # the split of the keys, too, goes by the columns in use
+
+
+def test_misaligned_outputs_and_weights_are_refused():
+    """Before anything reaches a device, where they would be written and read several bytes at a time."""
+    L, F = hb.lib(), 1 << 20
+    v, z, c = ctypes.c_void_p, ctypes.c_longlong, K_._Pages(F, F, F, F, 0, 8, 2, 16, 64)
+    for xq, sc in ((F + 1, F), (F + 4, F), (F + 8, F), (F, F + 2), (F, F + 4)):
+        for rows in (2, 20):
+            rc = L.hp_attn_paged(v(F), z(256), z(64), None, z(0), z(0), 4, v(F), 4, v(F), v(F), 2, 40, rows, 64, ctypes.byref(c), ctypes.c_float(0.125), 0, 0, v(F), v(xq), v(sc), v(F), None)
+            assert rc == 1 and "quantised outputs must be 16-byte aligned" in L.hp_last_error().decode()
+    for qn, kn in ((F + 1, F), (F, F + 3)):
+        rc = L.hp_kv_append(v(F), z(256), z(64), v(F), z(256), z(64), 4, v(F), z(128), z(64), v(F), z(128), z(64), v(qn), v(kn), None, 0, 0, 0, v(F), 4, v(F), v(F), 2, 4, ctypes.byref(c), ctypes.c_float(1e-6), None)
+        assert rc == 1 and "norm weights" in L.hp_last_error().decode()
