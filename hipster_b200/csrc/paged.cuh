@@ -14,8 +14,8 @@ __device__ __forceinline__ void paged_bad(int* err) { if (err) *err = HP_EINVAL;
 __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int s, int* err) {
     const int a = b.row_start[s], e = b.row_start[s + 1], n = b.kv_len[s];
     PagedSeq q; q.s = s;
-    q.row0 = min(max(a, 0), b.R); q.T = min(max(e - a, 0), min(b.max_rows, b.R - q.row0)); q.len = min(max(n, 0), b.max_kv);
-    if (q.row0 != a || q.T != e - a || q.len != n) paged_bad(err);
+    q.row0 = min(max(a, 0), b.R); q.T = min(max(min(max(e, 0), b.R) - q.row0, 0), b.max_rows); q.len = min(max(n, 0), b.max_kv);   // no row from e on, whatever a is: these belong to others
+    if (q.row0 != a || q.row0 + q.T != e || q.len != n) paged_bad(err);
     return q;
 }
 // The sequence of row r, by one warp: the number of sequences that end at or in front of it. Rows behind the last one: s = -1.

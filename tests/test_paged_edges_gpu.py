@@ -74,3 +74,18 @@ def test_tables_that_are_part_of_wider_ones(form, a, b):
             for mr in (2, 20):
                 got = K_.attn_paged(x, st.pool, view, st.row_start, kl, max_rows=mr, max_kv=2 ** 31 - 1)[0]
                 assert status() == 1 and torch.isfinite(got[2:] if s == 0 else got).all()   # the first one's third column is -1
+
+
+@pytest.mark.parametrize("rows", [2, 20])   # both kernels
+@pytest.mark.parametrize("first", [-4, -(2 ** 31)])
+def test_a_bad_first_row_leaves_the_other_sequences_alone(rows, first):
+    """A sequence that begins in front of row 0 owns no row of the others, and takes no block of theirs."""
+    st = Setup([rows] * 3, [60] * 3, 1, 64, 16, "i8")
+    q = torch.randn((3 * rows, 12, 64), generator=gen(1), device="cuda")
+    run = lambda: K_.attn_paged(q, st.pool, *st.batch, max_rows=3 * rows if rows < 4 else 60, max_kv=60)[0]  # noqa: E731
+    want = run()
+    assert status() == 0
+    st.row_start[0] = first
+    for _ in range(4):
+        got = run()
+        assert status() == 1 and torch.equal(got[rows:], want[rows:])
