@@ -135,7 +135,7 @@ int hp_moe_layer(const float* xn_dev, const void* xq_q_dev, const void* xq_sc_de
  * position kv_len[s] - T + t. row_start (S + 1 ints) and kv_len (S ints) are device memory like the table, read when the kernels run: a captured call can be
  * replayed with other lengths. R is the number of rows that the buffers hold: rows behind row_start[S] are neither read nor written. Entries that do
  * not fit (rows outside of [0, R), a sequence with more rows than max_rows or more tokens than max_kv, columns * page_size or the rotary table, a
- * page number outside of [0, n_pages) of a token that is used) fault nothing: what does not fit is left out (append, read) or makes the outputs of its
+ * page number outside of [0, n_pages) of a token that is used) fault nothing: what does not fit is left out (append, read; the other rows keep their positions) or makes the outputs of its
  * sequence meaningless (attention), and hp_device_status returns HP_EINVAL. Rows of negative position are not appended, read back or
  * normalised (HP_EINVAL), and attend to nothing. Row strides (ld) and head strides (hs) are in elements; those of outputs are nested, rows in heads or heads in
  * rows (HP_EINVAL where they lie over each other). */

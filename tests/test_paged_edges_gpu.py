@@ -89,3 +89,30 @@ def test_a_bad_first_row_leaves_the_other_sequences_alone(rows, first):
     for _ in range(4):
         got = run()
         assert status() == 1 and torch.equal(got[rows:], want[rows:])
+
+
+@pytest.mark.parametrize("what,at,value,places", [   # places: position of each row of the second and third sequence, None where it is left out
+    ("kv_len", 1, 33, (31, None, 18, 19)), ("kv_len", 1, 34, (None, None, 18, 19)), ("kv_len", 1, 1 << 30, (None, None, 18, 19)), ("kv_len", 1, 2 ** 31 - 1, (None, None, 18, 19)),
+    ("kv_len", 1, 1, (None, 0, 18, 19)), ("kv_len", 1, -5, (None, None, 18, 19)), ("kv_len", 1, -(2 ** 31), (None, None, 18, 19)),
+    ("row_start", 3, 9, (18, 19, 15, 16)), ("row_start", 3, 2 ** 31 - 1, (18, 19, None, None))])
+def test_rows_go_to_their_own_places_or_nowhere(what, at, value, places):
+    """Row t of T of a sequence of n tokens has position n - T + t, whatever else does not fit: no kept token is overwritten, and none is read back for another."""
+    st = Setup([2, 2, 2], [20, 20, 20], 1, 64, 16, "i8")
+    x = torch.randn((6, 1, 64), generator=gen(1), device="cuda")
+    getattr(st, what)[at] = value
+    before = st.pool.k.clone()
+    K_.kv_append(st.pool, x, 2 * x, *st.batch)
+    assert status() == 1
+    where = {2 + i: st.slot(1 + i // 2, p) for i, p in enumerate(places) if p is not None} | {0: st.slot(0, 18), 1: st.slot(0, 19)}
+    changed = {tuple(i) for i in (st.pool.k != before).any(-1).nonzero().tolist()}
+    assert changed == {(p, 0, i) for p, i in where.values()}
+    got_k, got_v = (torch.full((6, 1, 64), 5.0, device="cuda", dtype=torch.float16) for _ in range(2))
+    K_.kv_read(st.pool, *st.batch, k_out=got_k, v_out=got_v)
+    assert status() == 1
+    for r in range(6):
+        if r in where:
+            p, i = where[r]
+            k, v = ((codes[p, 0, i].float() * scale[p, 0, i]).half() for codes, scale in ((st.pool.k, st.pool.k_scale), (st.pool.v, st.pool.v_scale)))
+            assert torch.equal(got_k[r, 0], k) and torch.equal(got_v[r, 0], v) and (k.float() - x[r, 0]).abs().max() <= x[r].abs().max() / 250
+        else:
+            assert (got_k[r] == 5).all() and (got_v[r] == 5).all()
