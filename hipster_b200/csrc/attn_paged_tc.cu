@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
                 pair_sync(qt);
                 exact = fmaxf(exact, x.top[half ^ 1][row]);
                 float al = 1.f;
-                if (exact - mu > MU_LIMIT) { const float next = ceilf(exact) - MU_TOP; al = pow2i(mu - next); mu = next; l2 = mul2(l2, make_float2(al, al)); }
+                if (exact - mu > MU_LIMIT) { const float next = ceilf(exact) - MU_TOP; al = pow2i(mu - next); l2.x = scale_down(l2.x, mu - next); l2.y = scale_down(l2.y, mu - next); mu = next; }
                 if (half == 0) x.alpha[n & 3][row] = al;
                 measure();
             }

@@ -116,3 +116,18 @@ def test_rows_go_to_their_own_places_or_nowhere(what, at, value, places):
             assert torch.equal(got_k[r, 0], k) and torch.equal(got_v[r, 0], v) and (k.float() - x[r, 0]).abs().max() <= x[r].abs().max() / 250
         else:
             assert (got_k[r] == 5).all() and (got_v[r] == 5).all()
+
+
+@pytest.mark.parametrize("rows,n,window", [(2, 250, 0), (2, 600, 0), (1, 3000, 0), (2, 600, 400), (40, 300, 0), (40, 3000, 0), (40, 600, 400)])   # one split, few and many; decode and prompts
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("low,high", [(0.0, 1e15), (1e-25, 1e18), (0.0, 1e30)])
+def test_tokens_of_tiny_values_count_beside_huge_ones(D, rows, n, window, low, high):
+    """Scales of v as far apart as 32 bits allow: the first tokens' values are nothing beside the others', but their weights are as large."""
+    st = Setup([rows], [n], 2, D, 16, "i8")
+    up = torch.full(st.pool.v_scale.shape[:1], high, device="cuda")
+    up[st.table[0, :min(n // 2, 320) // 16].long()] = low   # whole slices, and where there are several splits a whole one
+    st.pool.v_scale.mul_(up[:, None, None])
+    q = torch.randn((rows, 4, D), generator=gen(1), device="cuda")
+    got, _ = K_.attn_paged(q, st.pool, *st.batch, max_rows=rows, max_kv=n, window=window)
+    want, tol = attn64(st, q, D ** -0.5, window, 0, None)
+    assert status() == 0 and ((got.double() - want).abs() <= tol).all(), float(((got.double() - want).abs() / tol).max())
