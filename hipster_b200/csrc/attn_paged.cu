@@ -497,9 +497,9 @@ struct Plan { int U, ns, nwin, MB; long long blocks; };
 // else is in the call. Captured, us: 1 token of 24 heads at 4097, U = 128 12.8, 256 12.6, 512 16.9, 1024 26.6; 48 sequences of up to 8192, 187, 139, 118, 116.
 // Prompts have blocks of rows: their keys are split as the launch fills the GPU best, a split costing the start of a CTA, some six tiles, and several of them
 // the merge (without it in the sum 1000 rows of 24 heads 91 us, now 80). Sixteen splits at most (eight: 64 rows of 24 heads at 16000 104 us, now 91).
-Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink) {
+Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink, int cap) {
     Plan p;
-    const int G = n_head / pool.n_kv, cap = pool.columns << pool.lg_page;
+    const int G = n_head / pool.n_kv;
     const long long eff = window ? std::min<long long>(cap, (long long)window + n_sink) : cap;
     const long long pairs = (long long)b.max_rows * G;
     const bool prompt = b.max_rows > PAGED_DECODE_ROWS;
@@ -546,13 +546,13 @@ template <int KIND> int launch_split(const PagedArgs& a, dim3 grid, int MB, cuda
 
 }  // namespace
 
-size_t attn_paged_workspace_bytes(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink) {
-    const Plan p = plan_of(pool, b, n_head, window, n_sink);
+size_t attn_paged_workspace_bytes(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink, int cap) {
+    const Plan p = plan_of(pool, b, n_head, window, n_sink, cap);
     return (partials(p, b, n_head) * (pool.head_dim + 2) * sizeof(float) + 127) / 128 * 128 + (b.max_rows > PAGED_DECODE_ROWS ? attn_paged_tc_bytes(pool, b) : 0);
 }
 
 int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams& p, cudaStream_t s) {
-    const Plan pl = plan_of(pool, b, p.n_head, p.window, p.n_sink);
+    const Plan pl = plan_of(pool, b, p.n_head, p.window, p.n_sink, p.cap);
     HP_REQUIRE(pl.blocks <= 65535 && pool.n_kv <= 65535 && (long long)b.R * p.n_head < (1ll << 31), "attn_paged: too many rows (%d) or heads for one call", b.R);
     PagedArgs a; a.pool = pool; a.b = b; a.q = p.q; a.q_ld = p.q_ld; a.q_hs = p.q_hs; a.n_head = p.n_head; a.G = p.n_head / pool.n_kv;
     a.scale2 = (float)((double)p.scale * 1.4426950408889634074 * (pool.kind == KV_E4M3 ? 256.0 : 1.0)); a.window = p.window; a.n_sink = p.n_sink;

@@ -235,20 +235,23 @@ int hp_moe_layer(const float* xn_dev, const void* xq_q_dev, const void* xq_sc_de
 
 // ------------------------------------------------------------------ paged 8-bit cache
 namespace {
+// columns of the table in use, and the tokens that they hold
+int columns_of(const hp_kv_pages* c, int table_ld) { return c->columns ? c->columns : table_ld; }
+int capacity(const hp_kv_pages* c, int table_ld) { return columns_of(c, table_ld) * c->page_size; }
 int paged_args(const char* who, const hp_kv_pages* c, const int* table, int table_ld, const int* row_start, const int* kv_len, int S, int R, long long max_rows, long long max_kv, hp::PagedPool* p, hp::PagedBatch* b) {
     HP_REQUIRE(c, "%s: null cache", who);
     HP_REQUIRE(c->type == HP_KV_I8 || c->type == HP_KV_E4M3, "%s: unknown cache type %d", who, c->type);
     HP_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "%s: head_dim must be 64, 128 or 256, not %d", who, c->head_dim);
     HP_REQUIRE(c->page_size >= 16 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0, "%s: page_size must be a power of two from 16 to 1024, not %d", who, c->page_size);
-    const int columns = c->columns ? c->columns : table_ld;
+    const int columns = columns_of(c, table_ld);
     HP_REQUIRE(c->n_pages >= 1 && c->n_kv >= 1 && columns >= 1 && columns <= table_ld && (long long)c->n_pages * c->n_kv < (0xffffffffll / c->page_size) && (long long)columns * c->page_size < (1ll << 30),
                "%s: bad cache n_pages=%d n_kv=%d table_ld=%d columns=%d", who, c->n_pages, c->n_kv, table_ld, c->columns);
     HP_REQUIRE(S >= 1 && R >= 1 && max_rows >= 1 && max_kv >= 1, "%s: bad batch S=%d R=%d max_rows=%lld max_kv=%lld", who, S, R, max_rows, max_kv);
-    p->k = (uint8_t*)c->k; p->v = (uint8_t*)c->v; p->k_scale = c->k_scale; p->v_scale = c->v_scale; p->table = table; p->table_ld = table_ld; p->columns = columns;
+    p->k = (uint8_t*)c->k; p->v = (uint8_t*)c->v; p->k_scale = c->k_scale; p->v_scale = c->v_scale; p->table = table; p->table_ld = table_ld;
     p->kind = c->type; p->n_pages = c->n_pages; p->n_kv = c->n_kv; p->head_dim = c->head_dim; p->lg_page = 0;
     while ((1 << p->lg_page) < c->page_size) ++p->lg_page;
     b->row_start = row_start; b->kv_len = kv_len; b->S = S; b->R = R;
-    b->max_rows = (int)(max_rows < R ? max_rows : R); b->max_kv = (int)std::min<long long>(max_kv, (long long)columns * c->page_size);
+    b->max_rows = (int)(max_rows < R ? max_rows : R); b->max_kv = (int)std::min<long long>(max_kv, capacity(c, table_ld));
     return HP_OK;
 }
 int paged_ptrs(const char* who, const hp_kv_pages* c, const int* table, const int* row_start, const int* kv_len) {
@@ -309,7 +312,7 @@ static int attn_paged_check(const char* who, int n_head, int window, int n_sink,
 size_t hp_attn_paged_workspace_bytes(int table_ld, int S, int R, int max_rows, int max_kv, int n_head, int window, int n_sink, const hp_kv_pages* pages) {
     hp::PagedPool pool; hp::PagedBatch b;
     if (paged_args("hp_attn_paged_workspace_bytes", pages, nullptr, table_ld, nullptr, nullptr, S, R, max_rows, max_kv, &pool, &b) || attn_paged_check("hp_attn_paged_workspace_bytes", n_head, window, n_sink, pool)) return 0;
-    return hp::attn_paged_workspace_bytes(pool, b, n_head, window > 1 << 30 ? 1 << 30 : window, n_sink > 1 << 30 ? 1 << 30 : n_sink);
+    return hp::attn_paged_workspace_bytes(pool, b, n_head, window > 1 << 30 ? 1 << 30 : window, n_sink > 1 << 30 ? 1 << 30 : n_sink, capacity(pages, table_ld));
 }
 int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const float* gate_dev, long long g_ld, long long g_hs, int n_head, const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev,
                   int S, int R, int max_rows, int max_kv, const hp_kv_pages* pages, float scale, int window, int n_sink, float* out_dev, void* xq_q_dev, void* xq_sc_dev, void* workspace_dev, void* stream) {
@@ -325,7 +328,7 @@ int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const floa
     HP_REQUIRE(scale > 0 && scale < 1e30f, "hp_attn_paged: bad scale");
     if (window > 1 << 30) window = 1 << 30;   // longer than any sequence
     if (n_sink > 1 << 30) n_sink = 1 << 30;
-    hp::AttnPagedParams p; p.q = q_dev; p.q_ld = q_ld; p.q_hs = q_hs; p.gate = gate_dev; p.g_ld = g_ld; p.g_hs = g_hs; p.n_head = n_head; p.scale = scale; p.window = window; p.n_sink = n_sink;
+    hp::AttnPagedParams p; p.q = q_dev; p.q_ld = q_ld; p.q_hs = q_hs; p.gate = gate_dev; p.g_ld = g_ld; p.g_hs = g_hs; p.n_head = n_head; p.scale = scale; p.window = window; p.n_sink = n_sink; p.cap = capacity(pages, table_ld);
     p.out = out_dev; p.xq = hp::XQ8F{xq_q_dev, xq_sc_dev}; p.workspace = workspace_dev;
     return hp::attn_paged(pool, b, p, (cudaStream_t)stream);
     HP_GUARD_END

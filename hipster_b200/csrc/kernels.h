@@ -185,10 +185,10 @@ int accept_greedy(const int* ids, const int* drafts, int n_draft, int* out, cuda
 enum : int { KV_I8 = 0, KV_E4M3 = 1 };
 struct PagedPool {
     uint8_t* k; uint8_t* v; float* k_scale; float* v_scale;   // codes [n_pages][n_kv][page][head_dim], scales [n_pages][n_kv][page]
-    const int* table; int table_ld, columns;                  // [S][table_ld], of which `columns` are in use
+    const int* table; int table_ld;                           // [S][table_ld]
     int kind, n_pages, n_kv, lg_page, head_dim;
 };
-struct PagedBatch { const int* row_start; const int* kv_len; int S, R, max_rows, max_kv; };   // max_rows, max_kv: bounds that the host knows
+struct PagedBatch { const int* row_start; const int* kv_len; int S, R, max_rows, max_kv; };   // max_rows, max_kv: bounds that the host knows; max_kv at most what the table's columns in use hold
 int rope_table(float* table, int n_pos, int n_rot, double base, int scaling, double factor, int orig_ctx, double beta_fast, double beta_slow, double attn_factor, cudaStream_t s);
 struct KvAppendParams {
     const float* q; size_t q_ld, q_hs; float* q_out; size_t qo_ld, qo_hs; int n_head;   // n_head = 0: keys and values alone
@@ -198,10 +198,10 @@ struct KvAppendParams {
 int kv_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, cudaStream_t s);
 int kv_read(const PagedPool& pool, const PagedBatch& b, void* k_out, void* v_out, size_t row_stride, size_t head_stride, cudaStream_t s);
 struct AttnPagedParams {
-    const float* q; const float* gate; size_t q_ld, q_hs, g_ld, g_hs; int n_head; float scale; int window, n_sink;
+    const float* q; const float* gate; size_t q_ld, q_hs, g_ld, g_hs; int n_head; float scale; int window, n_sink; int cap;   // cap: tokens that the table's columns in use hold
     float* out; XQ8F xq; void* workspace;
 };
-size_t attn_paged_workspace_bytes(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink);
+size_t attn_paged_workspace_bytes(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink, int cap);
 int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams& p, cudaStream_t s);
 
 }  // namespace hp
