@@ -102,8 +102,8 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
     if (h0 < h1) fetch(h0);
     const PagedSeq q = paged_find(b, r, lane, err);
     if (q.s < 0) return;
-    const int pos = paged_place(b, q, r);
-    if (pos < 0 || pos >= p.n_pos) { paged_bad(err); return; }
+    const int pos = paged_place(q, r);
+    if ((unsigned)pos >= (unsigned)min(b.max_kv, p.n_pos)) { paged_bad(err); return; }
     const uint32_t page = h1 > p.n_head ? paged_row(pool, q.s, pos >> pool.lg_page, 0, err) : 0u;
     const int half = p.n_rot / 2;
     // angles of the lane's elements; interleaved: of its four pairs
@@ -207,17 +207,18 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.x * RB;
     {
         int s = -1, pos = -1;   // of row `lane` of the warp's
-        PagedSeq q{-1, 0, 0, 0, 0, 0};
+        PagedSeq q{-1, 0, 0, 0, 0};
 #pragma unroll 1
         for (int i = 0; i < PER; ++i) {
             const int r = r0 + warp * PER + i;
             if (r >= b.R) break;
             if (q.s < 0 || r >= q.row0 + q.T) q = paged_find(b, r, lane, err);   // neighbours mostly belong to one sequence
-            if (q.s >= 0 && lane == i) { s = q.s; pos = paged_place(b, q, r); }
+            if (q.s >= 0 && lane == i) { s = q.s; pos = paged_place(q, r); }
         }
         uint32_t at = 0xffffffffu;
-        if (s >= 0 && pos < 0) paged_bad(err);
-        if (s >= 0 && pos >= 0) { at = paged_row(pool, s, pos >> pool.lg_page, 0, err); if (at != 0xffffffffu) at += pos & ((1 << pool.lg_page) - 1); }
+        const bool fits = (unsigned)pos < (unsigned)b.max_kv;
+        if (s >= 0 && !fits) paged_bad(err);
+        if (s >= 0 && fits) { at = paged_row(pool, s, pos >> pool.lg_page, 0, err); if (at != 0xffffffffu) at += pos & ((1 << pool.lg_page) - 1); }
         if (lane < PER) base[warp * PER + lane] = at;
     }
     __syncthreads();

@@ -2,27 +2,25 @@
 #pragma once
 #include "hp_common.cuh"
 #include "kernels.h"
+#include <climits>
 
 namespace hp {
 
 // Rows of a batch as the kernels see them. Lengths come from device memory, so nothing they hold is trusted: rows stay inside [0, R), a
 // sequence's tokens inside its columns of the table, page numbers inside the pool; what does not is left out and told by the status word.
-struct PagedSeq { int s, row0, T, len, end, n; };   // sequence, its first row, rows, tokens with these rows (s < 0: none); end of its rows and number of its tokens as given
+struct PagedSeq { int s, row0, T, len, base; };   // sequence, its first row, rows, tokens with these rows (s < 0: none); what a row's number lacks to its position
 
 __device__ __forceinline__ void paged_bad(int* err) { if (err) *err = HP_EINVAL; }
 // rows and tokens of sequence s
 __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int s, int* err) {
     const int a = b.row_start[s], e = b.row_start[s + 1], n = b.kv_len[s];
-    PagedSeq q; q.s = s; q.end = e; q.n = n;
+    PagedSeq q; q.s = s; q.base = n < 0 ? INT_MIN : (int)((unsigned)n - (unsigned)e);   // of the numbers as given: what does not fit shifts no other row
     q.row0 = min(max(a, 0), b.R); q.T = min(max(min(max(e, 0), b.R) - q.row0, 0), b.max_rows); q.len = min(max(n, 0), b.max_kv);   // no row from e on, whatever a is: these belong to others
     if (q.row0 != a || q.row0 + q.T != e || q.len != n) paged_bad(err);
     return q;
 }
-// Position of one of its rows, from the numbers as given: what does not fit shifts no other row. -1: none in the table
-__device__ __forceinline__ int paged_place(const PagedBatch& b, const PagedSeq& q, int r) {
-    const long long p = (long long)q.n - q.end + r;
-    return p >= 0 && p < b.max_kv ? (int)p : -1;
-}
+// Position of one of its rows; beyond max_kv (as an unsigned number) where it has no place
+__device__ __forceinline__ int paged_place(const PagedSeq& q, int r) { return (int)((unsigned)q.base + (unsigned)r); }
 // The sequence of row r, by one warp: the number of sequences that end at or in front of it. Rows behind the last one: s = -1.
 __device__ __forceinline__ PagedSeq paged_find(const PagedBatch& b, int r, int lane, int* err) {
     int s = 0;
@@ -32,7 +30,7 @@ __device__ __forceinline__ PagedSeq paged_find(const PagedBatch& b, int r, int l
         s += n;
         if (n < 32) break;
     }
-    if (s >= b.S) return PagedSeq{-1, 0, 0, 0, 0, 0};
+    if (s >= b.S) return PagedSeq{-1, 0, 0, 0, 0};
     PagedSeq q = paged_seq(b, s, err);
     if (r < q.row0 || r >= q.row0 + q.T) q.s = -1;
     return q;
@@ -94,7 +92,7 @@ __device__ __forceinline__ Block find_block(const PagedBatch& b, int G, int MB, 
     Block o; o.q.s = -1; o.p0 = o.np = 0;
     int acc = 0;
     for (int s0 = 0; s0 < b.S; s0 += 32) {
-        PagedSeq q{-1, 0, 0, 0, 0, 0};
+        PagedSeq q{-1, 0, 0, 0, 0};
         if (s0 + lane < b.S) q = paged_seq(b, s0 + lane, err);
         const int n = (q.T * G + MB - 1) / MB;
         int incl = n;
