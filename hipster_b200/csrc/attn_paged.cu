@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
                     t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
                     if (t - mu[n][c] > MU_LIMIT) {
                         const float next = ceilf(t) - MU_TOP, al = pow2i(mu[n][c] - next);
-                        l[n][c] = scale_down(l[n][c], mu[n][c] - next); mu[n][c] = next;
+                        l[n][c] = add_scaled(0.f, l[n][c], al, mu[n][c] - next); mu[n][c] = next;
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i) { O[i][n][c] = O[i][n][c] * al; O[i][n][c + 2] = O[i][n][c + 2] * al; }
                     }
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
 #pragma unroll
         for (int k = 0; k < KW; ++k) m = fmaxf(m, s_mu[k][tid]);
 #pragma unroll
-        for (int k = 0; k < KW; ++k) { const float d = s_mu[k][tid] - m; s_mu[k][tid] = pow2i(d); ls = ls + scale_down(s_l[k][tid], d); }
+        for (int k = 0; k < KW; ++k) { const float d = s_mu[k][tid] - m, w = pow2i(d); s_mu[k][tid] = w; ls = add_scaled(ls, s_l[k][tid], w, d); }
         if (DIRECT) { s_l[0][tid] = ls; s_row[tid] = sq.row0 + t; s_pos[tid] = kh * a.G + p - t * a.G; }   // its head in place of its position
         else {
             const bool live = s_pos[tid] >= 0;
@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(256) k_paged_merge(const MergeArgs a) {
     const size_t base = ((size_t)r * a.n_head + head) * (a.ns + a.nwin);
     auto slot = [&](int i) { return base + (i < s1 ? i : a.ns + (w0 + i - s1 - a.ns) % a.nwin); };
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f); float l = 0.f, mu = -INFINITY;
+    bool far = false;
     float4 v[PF];
 #pragma unroll
     for (int i = 0; i < PF; ++i) if (set + i * SETS < n) v[i] = reinterpret_cast<const float4*>(a.pO + slot(set + i * SETS) * D)[d4];
@@ -410,10 +411,14 @@ __global__ void __launch_bounds__(256) k_paged_merge(const MergeArgs a) {
             if (i < n) {
                 const float2 ml = a.pml[slot(i)];
                 const float w = pow2i(ml.x - mu);
-                o.x = fmaf(w, v[j].x, o.x); o.y = fmaf(w, v[j].y, o.y); o.z = fmaf(w, v[j].z, o.z); o.w = fmaf(w, v[j].w, o.w); l = l + scale_down(ml.y, ml.x - mu);
+                o.x = fmaf(w, v[j].x, o.x); o.y = fmaf(w, v[j].y, o.y); o.z = fmaf(w, v[j].z, o.z); o.w = fmaf(w, v[j].w, o.w); l = fmaf(w, ml.y, l); far |= ml.x - mu < -126.f;
                 if (i + PF * SETS < n) v[j] = reinterpret_cast<const float4*>(a.pO + slot(i + PF * SETS) * D)[d4];
             }
         }
+    }
+    if (far) {   // rare, so apart from the loop (8 x 3 rows over 2 kv heads at 2051: 22.3 us with it inside, 21.8)
+        l = 0.f;
+        for (int i = set; i < n; i += SETS) { const float2 ml = a.pml[slot(i)]; const float d = ml.x - mu; l = add_scaled(l, ml.y, pow2i(d), d); }
     }
     s_o[set][d4] = o;
     if (d4 == 0) s_l[set] = l;
@@ -468,7 +473,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 5 : 1) k_paged_merge_few(const
             if (i0 + j < n) {
                 const float w = pow2i(ml[i0 + j].x - mu);
                 float4& t = o[(i0 + j) % SETS];
-                t.x = fmaf(w, v[j].x, t.x); t.y = fmaf(w, v[j].y, t.y); t.z = fmaf(w, v[j].z, t.z); t.w = fmaf(w, v[j].w, t.w); l[(i0 + j) % SETS] = l[(i0 + j) % SETS] + scale_down(ml[i0 + j].y, ml[i0 + j].x - mu);
+                t.x = fmaf(w, v[j].x, t.x); t.y = fmaf(w, v[j].y, t.y); t.z = fmaf(w, v[j].z, t.z); t.w = fmaf(w, v[j].w, t.w); l[(i0 + j) % SETS] = add_scaled(l[(i0 + j) % SETS], ml[i0 + j].y, w, ml[i0 + j].x - mu);
             }
     }
     float x[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;

@@ -70,9 +70,9 @@ __device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32
 // logarithm of a scale of v, at least 2^-90: the weights' sum cannot overflow. NaN counts as that; infinity as the largest number, so that a reference stays finite and the rows that see it become NaN
 __device__ __forceinline__ float scale_lg2(float v) { return lg2(fminf(fmaxf(v, 8.0779357e-28f), 3.4028235e38f)); }
 __device__ __forceinline__ float pow2i(float d) { return d < -126.f ? 0.f : __uint_as_float((uint32_t)((int)d + 127) << 23); }   // 2^d, d whole and <= 0
-// l * 2^d in two factors. Sums of outputs scaled down by more than 2^-126 are nothing beside what they are added to; sums of weights are not: logarithms of scales span 218, so weights of
-// tokens with tiny values may be as large as 2^105 and count in full behind a reference that moved by twice as much
-__device__ __forceinline__ float scale_down(float l, float d) { const float h = fmaxf(d, -126.f); return l * pow2i(h) * pow2i(d - h); }
+// l + y * 2^d, w = pow2i(d), for sums of weights. Sums of outputs scaled down by more than 2^-126 are nothing beside what they are added to; sums of weights are not: logarithms of scales
+// span 218, so the weights of tokens with tiny values may be as large as 2^105, and count in full behind a reference that has moved by twice as much. Hence two factors, the second mostly 1
+__device__ __forceinline__ float add_scaled(float l, float y, float w, float d) { return fmaf(y * pow2i(fminf(d + 126.f, 0.f)), d < -126.f ? 1.17549435e-38f : w, l); }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 // Two of four codes as two f16. int8: the code plus 128 becomes the low bits of 1024 + code + 128, and 1152 is subtracted, exactly. e4m3: its bits
 // are those of the f16 2^-8 times as large, subnormals included (so 0x7f, which the quantiser does not write, reads as 480 and not as NaN: what lies in
