@@ -247,14 +247,14 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 4; ++c) { d[n][c] = distance(n, c); top = fmaxf(top, d[n][c] + (c < 2 ? lv0 : lv1)); }
-        if (__any_sync(0xffffffffu, top > MU_LIMIT)) {   // rare behind the first slices. A pair moves by its own keys alone
+        if (__any_sync(0xffffffffu, top > MU_LIMIT)) {   // rare behind the first slices. A pair moves by its own keys alone, and by the very sums that brought the warp here: others, rounded elsewhere, would move it only beside a pair that moves
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float t = fmaxf(hide[n][c] ? -INFINITY : s[n][c] * (k0 * cf[n][c]) + lv0, hide[n][c + 2] ? -INFINITY : s[n][c + 2] * (k1 * cf[n][c]) + lv1);
+                    float t = fmaxf(d[n][c] + lv0 > MU_LIMIT ? s[n][c] * (k0 * cf[n][c]) + lv0 : -INFINITY, d[n][c + 2] + lv1 > MU_LIMIT ? s[n][c + 2] * (k1 * cf[n][c]) + lv1 : -INFINITY);
                     t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-                    if (t - mu[n][c] > MU_LIMIT) {
+                    if (t > -INFINITY) {
                         const float next = ceilf(t) - MU_TOP, al = pow2i(mu[n][c] - next);
                         l[n][c] = add_scaled(0.f, l[n][c], al, mu[n][c] - next); mu[n][c] = next;
 #pragma unroll

@@ -131,3 +131,37 @@ def test_tokens_of_tiny_values_count_beside_huge_ones(D, rows, n, window, low, h
     got, _ = K_.attn_paged(q, st.pool, *st.batch, max_rows=rows, max_kv=n, window=window)
     want, tol = attn64(st, q, D ** -0.5, window, 0, None)
     assert status() == 0 and ((got.double() - want).abs() <= tol).all(), float(((got.double() - want).abs() / tol).max())
+
+
+def near_the_limit(S, T, seed):
+    """S sequences of 200 tokens whose last row has one factor x, such that the logarithm of the key at 64 lies within 4e-6 of the place where the reference of the row's weights, which the key
+    at 0 set, moves: 15 above it. The last row's distances from the reference and its logarithms round in different steps there.
+    -> q [S][T][64] (the other rows are zeros), pool, table."""
+    g, f = torch.Generator(), torch.float32
+    g.manual_seed(seed)
+    rand = lambda lo, hi: lo + (hi - lo) * torch.rand(S, generator=g, dtype=torch.float64)  # noqa: E731
+    x, v = rand(1, 1.9).to(f), torch.exp2(rand(-40, -20)).to(f)
+    per = x.double() * 100 * 0.125 * math.log2(math.e)   # logarithm per unit of the key's scale, codes of 100
+    z0, lv = rand(10, 40), torch.log2(v.double())
+    z1 = torch.ceil(z0 + lv) - 8 + 15 - lv + rand(-4e-6, 4e-6)
+    pool = K_.KVPages.empty(S, 1, 256, 64)
+    pool.v_scale[:] = v.cuda()[:, None, None]
+    pool.k_scale.fill_(1.0)
+    pool.k[:, 0, 0, 0] = pool.k[:, 0, 64:200, 0] = 100
+    pool.k_scale[:, 0, 0], pool.k_scale[:, 0, 64] = (z0 / per).to(f).cuda(), (z1 / per).to(f).cuda()
+    # the tokens behind these alone have values; their distances round in other steps from another reference
+    pool.k_scale[:, 0, 65:200] = pool.k_scale[:, 0, 64, None] * (0.3 + 0.25 * torch.rand((S, 135), generator=g)).cuda()
+    pool.v[:, 0, 65:200] = torch.randint(-127, 128, (S, 135, 64), generator=g, dtype=torch.int8).cuda()
+    q = torch.zeros((S, T, 64), device="cuda")
+    q[:, -1, 0] = x.cuda()
+    return q, pool, torch.arange(S, dtype=torch.int32, device="cuda")[:, None]
+
+
+def test_a_references_move_hangs_on_its_own_row():
+    """Rows whose reference is about to move, alone and beside a head whose reference does move: the same bits."""
+    S = 2048
+    q, pool, table = near_the_limit(S, 1, 1)
+    rs, kl = i32(list(range(S + 1))), i32([200] * S)
+    run = lambda q: K_.attn_paged(q, pool, table, rs, kl, max_rows=1, max_kv=200, scale=0.125)[0]  # noqa: E731
+    both, alone = run(torch.cat([q, 10 * q], 1)), run(q)
+    assert status() == 0 and torch.equal(both[:, :1], alone), int((both[:, :1] != alone).any(-1).sum())
