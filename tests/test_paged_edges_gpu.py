@@ -165,3 +165,15 @@ def test_a_references_move_hangs_on_its_own_row():
     run = lambda q: K_.attn_paged(q, pool, table, rs, kl, max_rows=1, max_kv=200, scale=0.125)[0]  # noqa: E731
     both, alone = run(torch.cat([q, 10 * q], 1)), run(q)
     assert status() == 0 and torch.equal(both[:, :1], alone), int((both[:, :1] != alone).any(-1).sum())
+
+
+def test_a_references_move_hangs_on_its_own_row_in_prompts():
+    """The same in a prompt, beside rows whose references move."""
+    S, T = 1024, 24
+    q, pool, table = near_the_limit(S, T, 2)
+    rs, kl = i32([T * s for s in range(S + 1)]), i32([200] * S)
+    run = lambda: K_.attn_paged(q.view(S * T, 1, 64), pool, table, rs, kl, max_rows=T, max_kv=200, scale=0.125)[0].view(S, T, 64)[:, -1]  # noqa: E731
+    alone = run()
+    q[:, :-1, 0] = 10 * q[:, -1:, 0]
+    beside = run()
+    assert status() == 0 and torch.equal(beside, alone), int((beside != alone).any(-1).sum())
