@@ -99,9 +99,9 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
                                                                                             : p.v + (size_t)r * p.v_ld + (size_t)(h - p.n_head - pool.n_kv) * p.v_hs;
         next[0] = reinterpret_cast<const float4*>(from + d0)[0]; next[1] = reinterpret_cast<const float4*>(from + d0)[1];
     };
-    if (h0 < h1) fetch(h0);
     const PagedSeq q = paged_find(b, r, lane, err);
     if (q.s < 0) return;
+    if (h0 < h1) fetch(h0);   // a row of a sequence, and no other, is read
     const int pos = paged_place(q, r);
     if ((unsigned)pos >= (unsigned)min(b.max_kv, p.n_pos)) { paged_bad(err); return; }
     const uint32_t page = h1 > p.n_head ? paged_row(pool, q.s, pos >> pool.lg_page, 0, err) : 0u;
