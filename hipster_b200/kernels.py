@@ -229,6 +229,12 @@ def _rows(t, pages, R, heads, what):
     return t.data_ptr(), ld, hs
 
 
+def _ints(what, *numbers):
+    """The library takes them as 32 bits; what does not fit would arrive as another number."""
+    if not -2 ** 31 <= min(numbers) <= max(numbers) < 2 ** 31:
+        raise HipsterError(1, f"{what} must fit 32 bits")
+
+
 _SCALING = {None: 0, "none": 0, "linear": 1, "yarn": 2}
 
 
@@ -242,6 +248,7 @@ def rope_table(n_pos, n_rot, base, scaling=None, factor=1.0, orig_ctx=0, beta_fa
         out = fast.rope_table(n_pos, n_rot, base, _SCALING[scaling], factor, orig_ctx, beta_fast, beta_slow, attn_factor)
         if out is not None:
             return out
+    _ints("rope_table: n_pos, n_rot and orig_ctx", n_pos, n_rot, orig_ctx)
     if n_pos < 1 or n_rot < 2:
         raise HipsterError(1, f"rope_table: bad shape n_pos={n_pos} n_rot={n_rot}")
     out = torch.empty((n_pos, n_rot // 2, 2), dtype=_F32, device=device)
@@ -330,6 +337,7 @@ def attn_paged(q, pages, table, row_start, kv_len, max_rows, max_kv, scale=None,
         out = fast.attn_paged(pages._at, pages._dev, q, gate, table, row_start, kv_len, max_rows, max_kv, scale, window, n_sink)
         if out is not None:
             return out, None
+    _ints("attn_paged: max_rows, max_kv, window and n_sink", max_rows, max_kv, window, n_sink)
     (S, c, *at), (R, n_head, D) = _batch(pages, table, row_start, kv_len), q.shape
     qr = _rows(q, pages, R, n_head, "q")
     gr = (None, 0, 0) if gate is None else _rows(gate, pages, R, n_head, "gate")

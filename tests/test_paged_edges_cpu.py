@@ -131,3 +131,19 @@ def test_misaligned_outputs_and_weights_are_refused():
     for qn, kn in ((F + 1, F), (F, F + 3)):
         rc = L.hp_kv_append(v(F), z(256), z(64), v(F), z(256), z(64), 4, v(F), z(128), z(64), v(F), z(128), z(64), v(qn), v(kn), None, 0, 0, 0, v(F), 4, v(F), v(F), 2, 4, ctypes.byref(c), ctypes.c_float(1e-6), None)
         assert rc == 1 and "norm weights" in L.hp_last_error().decode()
+
+
+def test_integers_beyond_32_bits_are_refused(recorded, monkeypatch):
+    """They do not arrive as what is left of them in 32 bits: a window of 2^32 + 5 is not one of 5."""
+    pages = K_.KVPages.empty(70, 2, 16, 64, device="cpu")
+    q = torch.zeros((1, 4, 64))
+    good = dict(max_rows=1, max_kv=64, window=5, n_sink=1)
+    for name in good:
+        for n in (2 ** 31, 2 ** 32 + 5, -2 ** 31 - 1, 2 ** 64 + 5):
+            with pytest.raises(hb.HipsterError, match="32 bits"):
+                K_.attn_paged(q, pages, torch.zeros((1, 64), dtype=torch.int32), i32([0, 1]), i32([1]), **{**good, name: n})
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: pytest.fail("allocated"))
+    for a, kw in (((2 ** 32 + 8, 64), {}), ((8, 2 ** 32 + 2), {}), ((8, 64), dict(scaling="yarn", factor=2.0, orig_ctx=2 ** 32 + 64))):
+        with pytest.raises(hb.HipsterError, match="32 bits"):
+            K_.rope_table(*a, 1e4, **kw)
+    assert not recorded.calls
