@@ -70,7 +70,7 @@ int hp_device_status(void* stream) {
     int h[2] = {0, 0};
     HP_CUDA(cudaMemcpyAsync(h, f, sizeof h, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
     HP_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
-    if (h[0] || h[1]) HP_CUDA(cudaMemsetAsync(f, 0, sizeof h, (cudaStream_t)stream));
+    if (h[0] || h[1]) HP_CUDA(cudaMemsetAsync(h[0] ? f : f + 1, 0, sizeof(int), (cudaStream_t)stream));   // the one that is reported; the other one by the next call
     if (h[0]) { hp::set_error("a kernel gave up a bounded wait (device status %d)", h[0]); return h[0]; }
     if (h[1]) { hp::set_error("a kernel met a length or an index in device memory that does not fit (device status %d)", h[1]); return h[1]; }
     return HP_OK;

@@ -26,7 +26,7 @@ enum { HP_OK = 0, HP_EINVAL = 1, HP_ECUDA = 2, HP_ENOMEM = 3, HP_ETIMEOUT = 4, H
 const char* hp_last_error(void);
 int hp_version(void);
 /* Reads (and clears) the device-side status word that kernels set when a bounded wait gave up (HP_ETIMEOUT), or when lengths or page numbers in
- * device memory did not fit (HP_EINVAL). */
+ * device memory did not fit (HP_EINVAL). Where both happened, one call reports the first and the next call the other. */
 int hp_device_status(void* stream);
 
 /* ------------------------------------------------------------------ kernel level (engine/kernels/gemv.h, ops.h) */

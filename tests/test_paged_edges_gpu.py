@@ -177,3 +177,15 @@ def test_a_references_move_hangs_on_its_own_row_in_prompts():
     q[:, :-1, 0] = 10 * q[:, -1:, 0]
     beside = run()
     assert status() == 0 and torch.equal(beside, alone), int((beside != alone).any(-1).sum())
+
+
+def test_both_kinds_of_status_are_reported():
+    """A wait that gave up and an index that does not fit, before anyone asks: one after the other."""
+    st = Setup([1], [20], 1, 64, 16, "i8")
+    x = torch.randn((1, 1, 64), generator=gen(1), device="cuda")
+    assert status() == 0
+    flags = torch.zeros(8, dtype=torch.int32, device="cuda")
+    hb.check(_lib.lib().hp_ep_wait_probe(_lib.ptr(flags), 2, 0, ctypes.c_uint(5), K_._stream()))   # a wait for a flag that nothing sets: ends by itself
+    st.kv_len[0] = 40
+    K_.kv_append(st.pool, x, x, *st.batch)
+    assert [status() for _ in range(3)] == [4, 1, 0]
