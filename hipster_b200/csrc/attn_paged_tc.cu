@@ -248,8 +248,8 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
             float top = d[0];
 #pragma unroll
             for (int e = 1; e < 32; ++e) top = fmaxf(top, d[e]);
-            // Looked at from 1/4 below the limit: this sum and the logarithms below are rounded apart by less than that (up to logarithms of 2^21), so a pair that would move is always looked at, whatever its neighbours do
-            if (__any_sync(0xffffffffu, top + lv > MU_LIMIT - 0.25f) && lane == 0) x.moved[n & 3][qt] = n + 1;
+            // Looked at from 2^-6 below the limit: this sum and the logarithms below are rounded apart by less than that (up to logarithms of 2^17), so a pair that would move is always looked at, whatever its neighbours do
+            if (__any_sync(0xffffffffu, top + lv > MU_LIMIT - 0.015625f) && lane == 0) x.moved[n & 3][qt] = n + 1;
             pair_sync(qt);
             if (x.moved[n & 3][qt] == n + 1) {   // rare behind the first tiles. A pair moves by its own keys alone
                 float exact = -INFINITY;
