@@ -14,9 +14,10 @@
 // lie in one page, one run of memory. The weights change from rows of keys to columns of pairs by movmatrix. Splits lie at fixed positions and a
 // slice's keys at fixed lanes and warps: a row's bits depend neither on the other rows of the call nor on the other sequences.
 //
-// Measured (captured, us): one token of 24 heads of 256 over 4 at 4097 12.6 (bytes alone 1.3): start, four slices per warp and merge one after the other. 48 such sequences of up to
-// 8192 117 (80; 4.5 TB/s): issue slots 58 %, a third of the instructions turning codes into f16, DRAM 0.66 of the copy rate. 8 x 3 rows over 2 kv heads at 2051 22 (2.0); 32 x 2
+// Measured (captured, us): one token of 24 heads of 256 over 4 at 4097 12.8 (bytes alone 1.3): start, four slices per warp and merge one after the other. 48 such sequences of up to
+// 8192 117 (80; 4.4 TB/s): issue slots 58 %, a third of the instructions turning codes into f16, DRAM 0.66 of the copy rate. 8 x 3 rows over 2 kv heads at 2051 21.8 (2.0); 32 x 2
 // rows of 32 heads of 128, window 1000, 34 (11): half of the instructions are starts and ends of the CTAs. Pairs as the 16 rows of the products: 260 for the 48 sequences; eight warps per CTA: 128.
+// Two sets of pairs spill up to 28 bytes a thread, one set of 256 dims 12.
 #include "paged.cuh"
 #include <algorithm>
 #include <type_traits>
@@ -435,8 +436,9 @@ __global__ void __launch_bounds__(256) k_paged_merge(const MergeArgs a) {
 }
 
 // The same sums, bit for bit, where a row has at most eight splits: a thread for four dims over all splits, 1024 dims of a row's heads per block. k_paged_merge's blocks, a head each,
-// are bound by their instructions and start-up once there are thousands of them. 509 rows of 24 heads in three splits (cold, us): 51 there, 27 here. Five blocks per
-// SM at 256 dims (as many as registers allow: 151 us for the call, now 146); at 128 dims that spills (32 x 2 rows of 32 heads behind a window: 34 us, 41).
+// are bound by their instructions and start-up once there are thousands of them. 509 rows of 24 heads in three splits (cold, us): 51 there, 27 here. At 256 dims five
+// blocks per SM, with 48 registers a thread and 140 bytes spilled, take less than two with the 95 that 64 and 128 dims have (the call 146 us, 151); squeezed like that, 128 dims take more (32 x 2 rows of 32 heads
+// behind a window: 41 us, 34).
 constexpr int FEW = 8;
 template <int D>
 __global__ void __launch_bounds__(256, D == 256 ? 5 : 1) k_paged_merge_few(const MergeArgs a) {
@@ -502,6 +504,8 @@ struct Plan { int U, ns, nwin, MB; long long blocks; };
 // else is in the call. Captured, us: 1 token of 24 heads at 4097, U = 128 12.8, 256 12.6, 512 16.9, 1024 26.6; 48 sequences of up to 8192, 187, 139, 118, 116.
 // Prompts have blocks of rows: their keys are split as the launch fills the GPU best, a split costing the start of a CTA, some six tiles, and several of them
 // the merge (without it in the sum 1000 rows of 24 heads 91 us, now 80). Sixteen splits at most (eight: 64 rows of 24 heads at 16000 104 us, now 91).
+// Behind a window a block has all its keys in one split, however few the blocks: 17 rows of 24 heads over 4 at 8000 take 174 us with a window of 4000, 83 of 1000, 46 without one.
+// A table for 131072 tokens has splits of 1024: one token at 4097 27.8 us there, 12.8 with a table of its own length; at 131072 both 79.
 Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink, int cap) {
     Plan p;
     const int G = n_head / pool.n_kv;

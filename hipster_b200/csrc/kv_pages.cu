@@ -41,8 +41,8 @@ __global__ void __launch_bounds__(256) k_rope_table(const RopeArgs a) {
     }
 }
 // Large tables: position 32 h + k by the addition theorems from 32 h and k, in 64 bits: four products instead of some 80 operations per entry, which left
-// the 64-bit pipe the bound (262144 x 64 entries: 69 us, now 28; the bytes alone 20). A block holds the functions of k < 32 and of its `groups` values of h; two blocks of
-// 1024 threads per SM (of 256: 35).
+// the 64-bit pipe the bound (262144 x 64 entries: 69 us, now 28; the bytes alone 20). A block holds the functions of k < 32 and of its `groups` values of h; blocks of
+// 1024 threads (of 256: 35), one per SM at a time by registers and shared memory, in two waves. Issue slots 72 %, the 64-bit pipe 26 %: instructions, and the functions at a block's start, during which nothing is written.
 constexpr int ROPE_GROUP = 32;
 __global__ void __launch_bounds__(1024) k_rope_table_sums(const RopeArgs a, int groups) {
     extern __shared__ __align__(16) double2 rope_sm[];
@@ -79,9 +79,9 @@ template <int KIND> __device__ __forceinline__ uint32_t kv_code(float x) {
     else return (uint32_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
 }
 // D / 8 lanes take a head of a row, eight neighbouring elements each, so that a warp has 1, 2 or 4 heads side by side; it takes hpw such sets of neighbouring
-// heads (n_head query heads, then n_kv key heads, then n_kv value heads) in a loop that fetches a set ahead. The row's place and angles are found once. Instructions
-// bound it beyond a few thousand heads (issue 52 %): 220 per head of 128 with a warp per head and the loop unrolled four times (which did not fit the
-// instruction cache), 171 in a loop. Four prompts of up to 1000 rows of 48 heads of 128: 24 us, 73 MB; one row of 32 heads of 256 some 3 us, latency.
+// heads (n_head query heads, then n_kv key heads, then n_kv value heads) in a loop that fetches a set ahead. The row's place and angles are found once. Four prompts of
+// up to 1000 rows of 48 heads of 128: 22.5 us, 73 MB, 95 instructions per head (with a warp per head and the loop unrolled four times 220, which did not fit the instruction cache). Neither issue
+// slots (56 %) nor memory (3.3 TB/s) are used up: the warps, 43 % of what an SM holds, wait for their next set of heads (4.6 of them at a time). One row of 32 heads of 256 3.3 us, latency.
 template <int D, int KIND>
 __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, int hpw, int* err) {
     constexpr int LPH = D / 8, HPS = 32 / LPH;   // lanes of a head, heads of a set
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
 }
 
 // RB rows per block, RB / 8 of them found by each warp; thread = 16 neighbouring codes of a row, a head and k or v, times the scale, rounded to f16 once. The e4m3
-// patterns 0x7f and 0xff, which the quantiser does not write, read as 480 and -480. Bound by memory: 16 caches of up to 5000 tokens of 8 x 128 68 us (322 MB, 4.7 TB/s; pages of 16
+// patterns 0x7f and 0xff, which the quantiser does not write, read as 480 and -480. Bound by memory: 16 caches of up to 5000 tokens of 8 x 128 67 us (322 MB, 4.8 TB/s; pages of 16
 // tokens are runs of 2 KB), with one piece in flight per thread 88; 4096 tokens of 4 x 256 7.4 us.
 template <int D, int KIND, int RB>
 __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, __half* __restrict__ ko, __half* __restrict__ vo, size_t row_stride, size_t head_stride, int* err) {
@@ -257,7 +257,8 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
 template <int D, int KIND> int launch_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, cudaStream_t s) {
     const int heads = p.n_head + 2 * pool.n_kv;
     int* err = device_arg_flag();
-    // one set of heads per warp while all of them fit on the GPU at once; several beyond
+    // One set of heads per warp while all of them fit on the GPU at once; six beyond. One and six, us: 256 rows of 48 heads of 128 6.7 and 7.9, 512 10.3 and 10.5, 1024 17.5 and 12.0, 4096 63 and 40; of 32
+    // heads of 256 512 rows 12.5 and 13.0, 1024 21.9 and 20.8; of 24 heads of 64 1024 rows 6.7 and 8.0, 4096 17.5 and 13.0
     constexpr int HPS = 32 / (D / 8);
     const int hpw = (long long)b.R * heads <= 148 * 64 * HPS ? 1 : 6;
     const long long items = (long long)b.R * ((heads + hpw * HPS - 1) / (hpw * HPS));
@@ -291,7 +292,8 @@ int kv_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& 
     return pool.kind == KV_I8 ? launch_append<KV_I8>(pool, b, p, s) : launch_append<KV_E4M3>(pool, b, p, s);
 }
 int kv_read(const PagedPool& pool, const PagedBatch& b, void* k_out, void* v_out, size_t row_stride, size_t head_stride, cudaStream_t s) {
-    // 8 rows per block until there are several blocks for every SM; 32 beyond, where finding the rows bounds a block of 8
+    // 8 rows per block until there are several blocks for every SM; 32 beyond, where finding the rows bounds a block of 8. Eight and 32, us, 16 caches in pages of 16: 250 tokens each of 1 x 64 2.9 and 3.1, of 4 x 256 7.5
+    // and 9.4; 5000 tokens of 1 x 64 24 and 12, of 1 x 256 43 and 28, of 4 x 64 44 and 29, of 8 x 128 98 and 100. Between, wide rows would do better with 8: 1000 tokens of 8 x 128 21 and 30, of 1 x 64 6.7 and 4.2
     const bool many = b.R > 148 * 32;
     int* err = device_arg_flag();
     auto go = [&](auto kernel, int rb) { return launch_pdl<4>(kernel, dim3((b.R + rb - 1) / rb), dim3(256), 0, s, pool, b, (__half*)k_out, (__half*)v_out, row_stride, head_stride, err); };

@@ -148,7 +148,8 @@ typedef struct hp_kv_pages {
 /* table_dev f32 [n_pos][n_rot / 2][2] = (cos, sin) of pos * f_i, f_i = base^(-2 i / n_rot): the rope_dev of hp_attn_decode and hp_kv_append. Scaled for
  * contexts beyond the trained one: HP_ROPE_LINEAR f_i / factor; HP_ROPE_YARN (by parts; Peng et al. 2023) with r_i = orig_ctx * f_i / (2 pi) and
  * g_i = clamp((r_i - beta_slow) / (beta_fast - beta_slow), 0, 1): f_i * (g_i + (1 - g_i) / factor). attn_factor multiplies cos and sin; 0 takes
- * 0.1 ln(factor) + 1 with HP_ROPE_YARN and 1 otherwise. Computed in 64 bits. n_rot even, 2 to 256; factor >= 1. */
+ * 0.1 ln(factor) + 1 with HP_ROPE_YARN and 1 otherwise. Computed in 64 bits. n_rot even, 2 to 256; factor >= 1. (Where a model's
+ * tables come from another rule, a ramp over the dimension's index with rounded borders for instance, the caller fills the table: the calls below take any.) */
 enum { HP_ROPE_NONE = 0, HP_ROPE_LINEAR = 1, HP_ROPE_YARN = 2 };
 int hp_rope_table(float* table_dev, int n_pos, int n_rot, double base, int scaling, double factor, int orig_ctx, double beta_fast, double beta_slow, double attn_factor, void* stream);
 /* Appends the rows of a batch: per head RMSNorm (q_norm / k_norm: bf16 [head_dim], NULL: none; eps), rotation of the first n_rot dims (rope_dev
@@ -167,7 +168,8 @@ int hp_kv_read(const int* table_dev, int table_ld, const int* row_start_dev, con
  * buffers 16-byte aligned), either may be NULL. max_rows, max_kv: bounds of a sequence's rows and tokens; they size the launch (R bounds max_rows too). Up to 16 rows per sequence (decode
  * steps, drafts, verify passes) a row's result depends neither on the other rows of its sequence nor on the other sequences, bit for bit (for one number of columns, window and
  * n_sink). Calls of more rows (prompts) turn the keys and values into f16 in the workspace, which then holds S * n_kv * max_kv * (4 * head_dim + 8) bytes besides the
- * partial outputs, and sum a row's keys in another order; a sequence of few rows and many tokens takes its time on few SMs there.
+ * partial outputs, and sum a row's keys in another order; a sequence of few rows and many tokens takes its time on few SMs there, and costs less in a call of its own. Behind
+ * a window they have one split of the keys per block of rows.
  * workspace_dev: hp_attn_paged_workspace_bytes of the same arguments, 16-byte aligned, of this call alone until it is done (captured calls that may run at once need one each). */
 size_t hp_attn_paged_workspace_bytes(int table_ld, int S, int R, int max_rows, int max_kv, int n_head, int window, int n_sink, const hp_kv_pages* pages);
 int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const float* gate_dev, long long g_ld, long long g_hs, int n_head, const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev,
