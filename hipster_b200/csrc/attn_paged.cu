@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
                     float t = fmaxf(d[n][c] + lv0 > MU_LIMIT ? s[n][c] * (k0 * cf[n][c]) + lv0 : -INFINITY, d[n][c + 2] + lv1 > MU_LIMIT ? s[n][c + 2] * (k1 * cf[n][c]) + lv1 : -INFINITY);
                     t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
                     if (t > -INFINITY) {
-                        const float next = ceilf(t) - MU_TOP, al = pow2i(mu[n][c] - next);
+                        const float next = mu_next(mu[n][c], t), al = pow2i(mu[n][c] - next);
                         l[n][c] = add_scaled(0.f, l[n][c], al, mu[n][c] - next); mu[n][c] = next;
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i) { O[i][n][c] = O[i][n][c] * al; O[i][n][c + 2] = O[i][n][c + 2] * al; }
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) d[n][c] = distance(n, c);
+                for (int c = 0; c < 4; ++c) d[n][c] = cut_off(distance(n, c), c < 2 ? lv0 : lv1);
         }
         uint32_t bh[NT][2], br[NT][2];   // weights times scales of v as columns of pairs: values and rests
 #pragma unroll

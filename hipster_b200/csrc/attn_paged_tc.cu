@@ -268,9 +268,13 @@ __global__ void __launch_bounds__(PagedGeo<D>::WARPS * 32, 1) k_paged_prompt(con
                 pair_sync(qt);
                 exact = fmaxf(exact, x.top[half ^ 1][row]);
                 float al = 1.f;
-                if (exact - mu > MU_LIMIT) { const float next = ceilf(exact) - MU_TOP; al = pow2i(mu - next); l2 = make_float2(add_scaled(0.f, l2.x, al, mu - next), add_scaled(0.f, l2.y, al, mu - next)); mu = next; }
+                if (exact - mu > MU_LIMIT) { const float next = mu_next(mu, exact); al = pow2i(mu - next); l2 = make_float2(add_scaled(0.f, l2.x, al, mu - next), add_scaled(0.f, l2.y, al, mu - next)); mu = next; }
                 if (half == 0) x.alpha[n & 3][row] = al;
                 measure();
+                if (fabsf(mu) >= 67108864.f) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) d[e] = cut_off(d[e], lv);
+                }
             }
 #pragma unroll
             for (int i = 0; i < 32; i += 16) {

@@ -70,6 +70,13 @@ __device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32
 // logarithm of a scale of v, at least 2^-90: the weights' sum cannot overflow. NaN counts as that; infinity as the largest number, so that a reference stays finite and the rows that see it become NaN
 __device__ __forceinline__ float scale_lg2(float v) { return lg2(fminf(fmaxf(v, 8.0779357e-28f), 3.4028235e38f)); }
 __device__ __forceinline__ float pow2i(float d) { return d < -126.f ? 0.f : __uint_as_float((uint32_t)((int)d + 127) << 23); }   // 2^d, d whole and <= 0
+// The reference for a largest logarithm t, never below the one there is. Logarithms from 2^26 on lie in steps of 8 and more: these take a reference some steps lower, and what passes the
+// limit behind a move all the same, a distance being rounded less than t, is cut off there (cut_off), so that finite scores of any size have finite weights. NaN stays, and an infinite t becomes one.
+__device__ __forceinline__ float mu_next(float mu, float t) {
+    const float a = fabsf(t), next = ceilf(a >= 67108864.f ? fmaf(a, -2.3841858e-7f, t) : t) - MU_TOP;
+    float o; asm("max.NaN.f32 %0, %1, %2;" : "=f"(o) : "f"(mu), "f"(next)); return o;
+}
+__device__ __forceinline__ float cut_off(float d, float lv) { float o; asm("min.NaN.f32 %0, %1, %2;" : "=f"(o) : "f"(d), "f"(MU_LIMIT + 0.5f - lv)); return o; }   // half a power beyond: what the limit let pass stays as it is
 // l + y * 2^d, w = pow2i(d), for sums of weights. Sums of outputs scaled down by more than 2^-126 are nothing beside what they are added to; sums of weights are not: logarithms of scales
 // span 218, so the weights of tokens with tiny values may be as large as 2^105, and count in full behind a reference that has moved by twice as much. Hence two factors, the second mostly 1
 __device__ __forceinline__ float add_scaled(float l, float y, float w, float d) { return fmaf(y * pow2i(fminf(d + 126.f, 0.f)), d < -126.f ? 1.17549435e-38f : w, l); }

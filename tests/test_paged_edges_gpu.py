@@ -189,3 +189,31 @@ def test_both_kinds_of_status_are_reported():
     st.kv_len[0] = 40
     K_.kv_append(st.pool, x, x, *st.batch)
     assert [status() for _ in range(3)] == [4, 1, 0]
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("D,n,window", [(64, 300, 0), (256, 3000, 0), (128, 700, 500)])
+@pytest.mark.parametrize("up", [1e6, 1e7, 1e8, 1e9, 1e12, 1e20, 1e30])
+def test_scores_of_any_size(rows, D, n, window, up):
+    """Finite scores have finite outputs: those of the largest one alone where it stands out of what 32 bits resolve, and never beyond the values there are."""
+    st = Setup([rows] * 3, [n] * 3, 2, D, 16, "i8")
+    q = torch.randn((3 * rows, 8, D), generator=gen(1), device="cuda") * up
+    got = K_.attn_paged(q, st.pool, *st.batch, max_rows=rows, max_kv=n, window=window)[0].double()
+    assert status() == 0
+    stands_out = 0
+    for s in range(3):
+        k, v = st.tokens(s, "k").repeat_interleave(4, 0), st.tokens(s, "v").repeat_interleave(4, 0)
+        for t in range(rows):
+            pos = n - rows + t
+            j = slice(max(0, pos - window + 1) if window else 0, pos + 1)
+            x, o = q[s * rows + t].double(), got[s * rows + t]
+            z = torch.einsum("hd,hjd->hj", x, k[:, j]) * (D ** -0.5 * math.log2(math.e))
+            A = (torch.einsum("hd,hjd->hj", x.abs(), k[:, j].abs()) * (D ** -0.5 * math.log2(math.e))).amax(-1)
+            top = z.topk(2, -1)
+            # twice a score's error (the tensor pipe's additions, roundings), the steps by which a reference is lowered, and weights that are nothing beside the first
+            clear = top.values[:, 0] - top.values[:, 1] > 2 * (D / 16 + 8) * 2.0 ** -23 * A + 8 * 2.0 ** -23 * top.values[:, 0].abs() + 60
+            want = v[torch.arange(8, device="cuda"), top.indices[:, 0] + j.start]
+            assert ((o - want).abs() <= 1e-5 * want.abs().amax(-1, keepdim=True))[clear].all()
+            assert (o.abs() <= v[:, j].abs().amax((1, 2), keepdim=True)[:, 0] * (1 + 1e-5)).all()   # not for NaN
+            stands_out += int(clear.sum())
+    assert stands_out > 12 * rows
