@@ -64,7 +64,7 @@ int attn_paged_tc(PagedArgs& a, dim3 grid, cudaStream_t s);
 
 // The reference mu of a pair's weights is whole. It moves when a logarithm passes mu + MU_LIMIT, to MU_TOP below the largest of the keys at hand: weights times scales stay
 // below 2^15 (f16 ends at 65504), the largest is above 2^7 (f16 ends in steps of 2^-24), and almost all keys take no maximum at all.
-constexpr float MU_TOP = 8.f, MU_LIMIT = 15.f, MU_NONE = -1e30f;
+constexpr float MU_TOP = 8.f, MU_LIMIT = 15.f, MU_NONE = -3.4028235e38f;
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // logarithm of a scale of v, at least 2^-90: the weights' sum cannot overflow. NaN counts as that; infinity as the largest number, so that a reference stays finite and the rows that see it become NaN

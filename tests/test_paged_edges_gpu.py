@@ -217,3 +217,17 @@ def test_scores_of_any_size(rows, D, n, window, up):
             assert (o.abs() <= v[:, j].abs().amax((1, 2), keepdim=True)[:, 0] * (1 + 1e-5)).all()   # not for NaN
             stands_out += int(clear.sum())
     assert stands_out > 12 * rows
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("up", [1.0, 1e10, 1e28, 1e32, 1e35])
+def test_a_single_key_takes_all_whatever_its_score(rows, up):
+    """Rows that see themselves alone, with scores as far below zero as 32 bits go: the value is their own."""
+    st = Setup([rows] * 2, [rows + 70] * 2, 2, 64, 16, "e4m3")
+    at = torch.arange(70, 70 + rows, device="cuda")
+    k, v = (torch.cat([st.tokens(s, w)[:, at].transpose(0, 1) for s in range(2)]) for w in "kv")   # [row][kv head][dim]
+    q = (-up * k.repeat_interleave(2, 1)).float()
+    got = K_.attn_paged(q, st.pool, *st.batch, max_rows=rows, max_kv=rows + 70, window=1)[0].double()
+    want = v.repeat_interleave(2, 1)
+    # a weight as two f16 is off by 2^-22 of itself; its product with the scale, the sum, the quotient and the factor of e4m3 are rounded, by 2^-24 each
+    assert status() == 0 and ((got - want).abs() <= 8 * 2.0 ** -24 * want.abs().amax(-1, keepdim=True) + 2.0 ** -22 * want.abs()).all()
