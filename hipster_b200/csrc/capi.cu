@@ -288,6 +288,7 @@ int hp_kv_append(const float* q_dev, long long q_ld, long long q_hs, float* q_ou
     HP_REQUIRE(rows_ok(k_dev, k_ld, k_hs) && rows_ok(v_dev, v_ld, v_hs) && (n_head == 0 || (rows_ok(q_dev, q_ld, q_hs) && rows_ok(q_out_dev, qo_ld, qo_hs))), "hp_kv_append: rows must be 16-byte aligned, with strides that are multiples of 4");
     HP_REQUIRE((((uintptr_t)q_norm_bf16_dev | (uintptr_t)k_norm_bf16_dev) & 1) == 0, "hp_kv_append: norm weights must be 2-byte aligned");
     HP_REQUIRE(n_head == 0 || apart(R, qo_ld, n_head, qo_hs, pool.head_dim), "hp_kv_append: rows of q_out lie over each other");
+    HP_REQUIRE(n_head == 0 || q_dev != q_out_dev || ((R == 1 || q_ld == qo_ld) && (n_head == 1 || q_hs == qo_hs)), "hp_kv_append: q_out in place of q must have its strides");
     HP_REQUIRE((long long)R * (n_head + 2 * pool.n_kv) < (1ll << 33), "hp_kv_append: too many rows");
     hp::KvAppendParams p; p.q = q_dev; p.q_ld = q_ld; p.q_hs = q_hs; p.q_out = q_out_dev; p.qo_ld = qo_ld; p.qo_hs = qo_hs; p.n_head = n_head; p.k = k_dev; p.k_ld = k_ld; p.k_hs = k_hs;
     p.v = v_dev; p.v_ld = v_ld; p.v_hs = v_hs; p.q_norm = q_norm_bf16_dev; p.k_norm = k_norm_bf16_dev; p.rope = rope_dev; p.n_pos = n_rot ? n_pos : 1 << 30; p.n_rot = n_rot; p.interleaved = interleaved; p.eps = eps;
@@ -301,6 +302,7 @@ int hp_kv_read(const int* table_dev, int table_ld, const int* row_start_dev, con
     HP_REQUIRE(k_out_f16_dev && v_out_f16_dev, "hp_kv_read: null pointer");
     HP_REQUIRE((((uintptr_t)k_out_f16_dev | (uintptr_t)v_out_f16_dev) & 15) == 0 && row_stride >= 0 && head_stride >= 0 && row_stride % 8 == 0 && head_stride % 8 == 0, "hp_kv_read: outputs must be 16-byte aligned, with strides that are multiples of 8");
     HP_REQUIRE(apart(R, row_stride, pool.n_kv, head_stride, pool.head_dim), "hp_kv_read: rows of the outputs lie over each other");
+    HP_REQUIRE(k_out_f16_dev != v_out_f16_dev, "hp_kv_read: k_out and v_out are the same");
     return hp::kv_read(pool, b, k_out_f16_dev, v_out_f16_dev, (size_t)row_stride, (size_t)head_stride, (cudaStream_t)stream);
     HP_GUARD_END
 }

@@ -147,3 +147,12 @@ def test_integers_beyond_32_bits_are_refused(recorded, monkeypatch):
         with pytest.raises(hb.HipsterError, match="32 bits"):
             K_.rope_table(*a, 1e4, **kw)
     assert not recorded.calls
+
+
+def test_outputs_that_would_be_written_twice_are_refused():
+    L, F = hb.lib(), 1 << 20
+    v, z, c = ctypes.c_void_p, ctypes.c_longlong, K_._Pages(F, F, F, F, 0, 8, 2, 16, 64)
+    for ld, hs in ((512, 64), (256, 1024), (512, 128)):
+        rc = L.hp_kv_append(v(F), z(256), z(64), v(F), z(ld), z(hs), 4, v(F), z(128), z(64), v(F), z(128), z(64), None, None, None, 0, 0, 0, v(F), 4, v(F), v(F), 2, 4, ctypes.byref(c), ctypes.c_float(1e-6), None)
+        assert rc == 1 and "in place" in L.hp_last_error().decode()
+    assert L.hp_kv_read(v(F), 4, v(F), v(F), 2, 4, ctypes.byref(c), v(F), v(F), z(128), z(64), None) == 1 and "the same" in L.hp_last_error().decode()
