@@ -14,8 +14,8 @@
 // lie in one page, one run of memory. The weights change from rows of keys to columns of pairs by movmatrix. Splits lie at fixed positions and a
 // slice's keys at fixed lanes and warps: a row's bits depend neither on the other rows of the call nor on the other sequences.
 //
-// Measured (captured, us): one token of 24 heads of 256 over 4 at 4097 12.8 (bytes alone 1.3): start, four slices per warp and merge one after the other. 48 such sequences of up to
-// 8192 117 (80; 4.4 TB/s): issue slots 58 %, a third of the instructions turning codes into f16, DRAM 0.66 of the copy rate. 8 x 3 rows over 2 kv heads at 2051 21.8 (2.0); 32 x 2
+// Measured (captured, us): one token of 24 heads of 256 over 4 at 4097 12.85 (bytes alone 1.3): start, four slices per warp and merge one after the other. 48 such sequences of up to
+// 8192 118 (80; 4.4 TB/s): issue slots 58 %, a third of the instructions turning codes into f16, DRAM 0.66 of the copy rate. 8 x 3 rows over 2 kv heads at 2051 21.8 (2.0); 32 x 2
 // rows of 32 heads of 128, window 1000, 34 (11): half of the instructions are starts and ends of the CTAs. Pairs as the 16 rows of the products: 260 for the 48 sequences; eight warps per CTA: 128.
 // Two sets of pairs spill up to 28 bytes a thread, one set of 256 dims 12.
 #include "paged.cuh"

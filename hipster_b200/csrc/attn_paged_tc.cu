@@ -13,7 +13,7 @@
 //   products (one thread; issuing them takes as long as they take): scores of a tile in front of the outputs of the one before
 //   weights (eight warps, a thread per pair and half of the keys): S -> w, in its place. The mask, the sum and the rescaling are a thread's own; two warps tell each other whether a reference moves
 //   sums (eight warps, a thread per pair and half of the dims): O of the tile into registers, while the scores of the next but one are formed
-// Measured: 509 rows of 24 heads of 256 over 4 behind 4096 tokens 147 us, of these the pictures 8, the merge 15; operations alone 33, and 65 as they are done, q and weights as two f16 each. A tile takes
+// Measured: 509 rows of 24 heads of 256 over 4 behind 4096 tokens 148 us, of these the pictures 8, the merge 15; operations alone 33, and 65 as they are done, q and weights as two f16 each. A tile takes
 // 3200 clocks, 2400 of them products: an output waits for its weights (700 clocks to read the scores and see whether a reference moves, 300 for the other half's
 // answer, 1200 for the weights), and each hand-over between products and warps for some 200. A CTA starts in 11000 clocks, 6500 of them q, and writes its sums in 5500. Keys and dims as the 128
 // rows, with pairs as columns (48 a block) and tiles of 128 keys: 225 us, since a thread then needs all other warps to know whether a reference moves, and the
