@@ -210,7 +210,8 @@ def prepare(c, seed):
     S, R, kv, D, H = c["seqs"], sum(rows), c["kv"], c["dim"], c.get("heads", 0)
     st = {"c": c, "R": R, "max_rows": max(rows), "max_kv": max(lens)}
     st["row_start"] = torch.tensor([sum(rows[:s]) for s in range(S + 1)], dtype=torch.int32, device=dev)
-    sigma = 1 + 2 * (torch.rand(D, generator=g, device=dev) > 0.95).float()   # rows as projections give them: normal, a few dims larger than the others
+    sigma = torch.rand(D, generator=g, device=dev)   # rows as projections give them: normal, a few dims larger than the others; what is quantised on its way comes from a projection whose heads are even
+    sigma = 1 + 0.2 * sigma if c["op"] == "append" else 1 + 2 * (sigma > 0.95).float()
     if c["op"] == "prompt":
         kind = TYPES[c["type"]]
         x = (torch.randn((R, H + 2 * kv, D), generator=g, device=dev) * sigma).to(kind)
