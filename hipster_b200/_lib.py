@@ -7,12 +7,14 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("HIPSTER_B200_LIB") or os.path.join(HERE, "libhipster_b200.so")
 HEADER = os.path.join(HERE, "..", "include", "hipster_b200.h")
 
-_lib = _hot = _tensor_calls = None
+_lib = _hot = _more = _tensor_calls = None
 # the calls whose latency counts, with their argument types (p pointer, i int, l long long, f float, d double), so that integers pass without a wrapper object
 _TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float, "d": ctypes.c_double}
 _HOT = {"hp_quantize_x_q8": "piiippp", "hp_gemv_q4k_q8": "ppppiiiip", "hp_argmax": "piiipppp", "hp_accept_greedy": "ppipp", "hp_attn_decode": "piiiiiipppppipppfpp",
         "hp_kv_append": "pllpllipllpllpppiiipippiipfp", "hp_kv_read": "pippiipppllp", "hp_attn_paged": "pllpllipippiiiipfiippppp",
         "hp_rope_table": "piidididddp"}
+# calls that go through ctypes alone
+_MORE = {"hp_kv_append_axes": "pllpllipllpllpppiiiplpipippiipfp", "hp_rope_rows": "pllpllipllpllpllplliiipppiiiplpiifp", "hp_attn_prompt": "pllpllplliplliiipiiifpppp"}
 
 
 class HipsterError(RuntimeError):
@@ -62,6 +64,18 @@ def hot():
     return _hot
 
 
+def more():
+    """The calls of _MORE with integers (None: absent) for every argument, through ctypes, on function objects of this package's own."""
+    global _more
+    if _more is None:
+        lib()
+        calls = ctypes.CDLL(LIB_PATH)
+        for name, types in _MORE.items():
+            getattr(calls, name).argtypes = [_TYPES[t] for t in types]
+        _more = calls
+    return _more
+
+
 def tensors():
     """The paged-cache calls on torch tensors (csrc/pytensors.cpp), bound to the library that is loaded here; None where the module was not built, or for another torch."""
     global _tensor_calls
@@ -73,7 +87,7 @@ def tensors():
         except ImportError:
             calls = None
         if calls is not None and torch.__version__.split("+")[0] == calls.torch:
-            for name in ("hp_kv_append", "hp_kv_read", "hp_attn_paged", "hp_attn_paged_workspace_bytes", "hp_rope_table"):
+            for name in ("hp_kv_append", "hp_kv_read", "hp_attn_paged", "hp_attn_paged_workspace_bytes", "hp_rope_table", "hp_kv_append_axes", "hp_rope_rows", "hp_attn_prompt"):
                 calls.bind(name, ctypes.cast(getattr(L, name), ctypes.c_void_p).value)
             _tensor_calls = calls
         else:

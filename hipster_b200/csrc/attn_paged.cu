@@ -27,8 +27,10 @@ namespace {
 
 constexpr int KW = 4, KS = 16, SLOTS = 3;   // warps that share a split, keys of a slice, slots of a warp's ring
 __host__ __device__ constexpr int out_stride(int D) { return D + 4; }
-__host__ __device__ constexpr int smem_bytes(int D, int NT) {   // fragments of q | rings; the outputs of the warps pass through the same memory at the end
-    const int run = NT * D * 32 + KW * SLOTS * KS * D, end = KW * NT * 8 * out_stride(D) * 4;
+__host__ __device__ constexpr int row_bytes(int D, int KIND) { return KIND == KV_I4 ? D / 2 : D; }                       // codes of a row
+__host__ __device__ constexpr int slot_bytes(int D, int KIND) { return KS * (row_bytes(D, KIND) + (KIND == KV_I4 ? D / 32 : 0)); }   // 4 bits: codes, then the bytes of the groups
+__host__ __device__ constexpr int smem_bytes(int D, int KIND, int NT) {   // fragments of q | rings; the outputs of the warps pass through the same memory at the end
+    const int run = NT * D * 32 + KW * SLOTS * slot_bytes(D, KIND), end = KW * NT * 8 * out_stride(D) * 4;
     return run > end ? run : end;
 }
 
@@ -50,11 +52,19 @@ template <int D, bool V> __device__ __forceinline__ int place(int r, int c) {
     if constexpr (D == 64) return (r >> 1) * 128 + (((r & 1) ^ ((r >> 2) & 1)) << 6) + ((c ^ (((r >> 1) & 1) << 1)) << 4);
     else return r * D + ((c ^ (((V ? r >> 1 : r) & 3) << 1)) << 4);
 }
+// The same for 4 bits, rows of D / 2 bytes. A lane reads a group of k (16 bytes) of rows g, and of v D / 8 dims (16, 8 or 4 bytes) of every second row. 256 dims: rows are 128 bytes, and neighbours (v: every
+// second) shift. 128 dims: v as above for rows of 64 bytes; k, and 64 dims' k, hit distinct banks as they lie. 64 dims, v: four rows share 128 bytes, rows 4 to 7 swap neighbours.
+template <int D, bool V> __device__ __forceinline__ int place4(int r, int c) {
+    if constexpr (D == 256) return r * 128 + ((c ^ (V ? ((r >> 1) & 3) << 1 : (r & 1) << 2)) << 4);
+    else if constexpr (D == 128) return V ? place<64, true>(r, c) : r * 64 + (c << 4);
+    else return V ? (r >> 2) * 128 + ((r & 3) ^ ((r >> 2) & 1)) * 32 + (c << 4) : r * 32 + (c << 4);
+}
+template <int D, int KIND, bool V> __device__ __forceinline__ int place_of(int r, int c) { if constexpr (KIND == KV_I4) return place4<D, V>(r, c); else return place<D, V>(r, c); }
 
 // grid (splits, n_kv, blocks), four warps; NT sets of 8 pairs. DIRECT: the only split there is writes the outputs itself
 template <int D, int KIND, int NT, bool DIRECT>
 __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : (D == 256 ? 3 : 4)) k_paged_split(const PagedArgs a) {
-    constexpr int CPR = D / 16, MB = 8 * NT, XS = out_stride(D);   // 16-byte pieces of a row
+    constexpr int RB = row_bytes(D, KIND), SLOT = slot_bytes(D, KIND), CPR = RB / 16, MB = 8 * NT, XS = out_stride(D);   // 16-byte pieces of a row
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ float s_c[MB];   // factor of a pair's scores
     __shared__ int s_pos[MB];   // position of a pair's row, -1: none
@@ -100,21 +110,26 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         const uint32_t r = paged_row_of(a.pool, id, kh, a.arg_err);
         return r == 0xffffffffu ? 0u : r + (uint32_t)((i * KS) & pmask);
     };
-    uint8_t* const ring = sm + NT * D * 32 + warp * (SLOTS * KS * D);
+    uint8_t* const ring = sm + NT * D * 32 + warp * (SLOTS * SLOT);
     const uint32_t ring_u = smem_u32(ring);
     // A slot's 16 rows are one run of memory; piece e = 32 i + lane of it goes to place(e / CPR, e % CPR), which is 512 i and a part that repeats after two (k) or four (v) i
     int kput[2], vput[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int e = 32 * i + lane;
-        if (i < 2) kput[i] = place<D, false>(e / CPR, e % CPR) - 512 * i;
-        vput[i] = place<D, true>(e / CPR, e % CPR) - 512 * i;
+        if (i < 2) kput[i] = place_of<D, KIND, false>(e / CPR, e % CPR) - 512 * i;
+        vput[i] = place_of<D, KIND, true>(e / CPR, e % CPR) - 512 * i;
     }
     const uint8_t* const kbase = a.pool.k + lane * 16; const uint8_t* const vbase = a.pool.v + lane * 16;
     auto fetch_k = [&](int slot, uint32_t row, bool live) {
         if (live) {
-            const uint8_t* src = kbase + (size_t)row * D;
-            const uint32_t d0 = ring_u + slot * (KS * D) + kput[0], d1 = ring_u + slot * (KS * D) + kput[1];
+            const uint8_t* src;
+            if constexpr (KIND == KV_I4) {
+                const I4Row at = i4_row(row, lg, D);
+                src = kbase + at.codes;
+                if (lane < D / 32) cp_async16(ring_u + slot * SLOT + KS * RB + lane * 16, kbase + at.groups);
+            } else src = kbase + (size_t)row * D;
+            const uint32_t d0 = ring_u + slot * SLOT + kput[0], d1 = ring_u + slot * SLOT + kput[1];
 #pragma unroll
             for (int i = 0; i < KS * CPR / 32; ++i) cp_async16((i & 1 ? d1 : d0) + 512 * i, src + 512 * i);
         }
@@ -122,8 +137,13 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     };
     auto fetch_v = [&](int slot, uint32_t row, bool live) {
         if (live) {
-            const uint8_t* src = vbase + (size_t)row * D;
-            const uint32_t at = ring_u + slot * (KS * D), d[4] = {at + vput[0], at + vput[1], at + vput[2], at + vput[3]};
+            const uint32_t at = ring_u + slot * SLOT, d[4] = {at + vput[0], at + vput[1], at + vput[2], at + vput[3]};
+            const uint8_t* src;
+            if constexpr (KIND == KV_I4) {
+                const I4Row from = i4_row(row, lg, D);
+                src = vbase + from.codes;
+                if (lane < D / 32) cp_async16(at + KS * RB + lane * 16, vbase + from.groups);
+            } else src = vbase + (size_t)row * D;
 #pragma unroll
             for (int i = 0; i < KS * CPR / 32; ++i) cp_async16(d[i & 3] + 512 * i, src + 512 * i);
         }
@@ -139,7 +159,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     auto scales = [&](uint32_t r) { return sbase[r]; };
     float sc = i0 < i_end ? scales(r0) : 0.f;
 
-    // the 8 dims of a lane are its words of two steps of 16 dims, values and rests
+    // the 8 dims of a lane are its words of two steps of 16 dims, values and rests; 4 bits: dims i and i + 4 side by side, at the step and the four lanes that the word of codes falls to
 #pragma unroll
     for (int u = 0; u < QP; ++u) {
         const int i = warp + KW * u, t = (blk.p0 + i) / a.G;
@@ -155,12 +175,13 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             uint32_t h[4], r[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float y0 = x[2 * j] * up, y1 = x[2 * j + 1] * up;
+                const float y0 = x[KIND == KV_I4 ? j : 2 * j] * up, y1 = x[KIND == KV_I4 ? j + 4 : 2 * j + 1] * up;
                 const __half2 hh = __floats2half2_rn(y0, y1);
                 const float2 f = __half22float2(hh);
                 h[j] = h2_bits(hh); r[j] = h2_bits(__floats2half2_rn(y0 - f.x, y1 - f.y));
             }
-            uint4* dst = reinterpret_cast<uint4*>(sm + (i >> 3) * D * 32 + (lane >> 2) * 1024) + (i & 7) * 4 + (lane & 3);
+            const int step = KIND != KV_I4 ? lane >> 2 : D == 64 ? lane & 1 : (lane >> 4) * 4 + (lane & 3), four = KIND != KV_I4 ? lane & 3 : D == 64 ? lane >> 1 : (lane >> 2) & 3;
+            uint4* dst = reinterpret_cast<uint4*>(sm + (i >> 3) * D * 32 + step * 1024) + (i & 7) * 4 + four;
             dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
             dst[32] = make_uint4(r[0], r[1], r[2], r[3]);
         }
@@ -178,7 +199,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     const int all_hi = sp.pos_lo, all_lo = a.window ? sp.pos_hi - a.window : -1;
     const uint8_t* const qf = sm + lane * 16;
 
-    float O[D / 16][NT][4];   // dims (tile m of 64 y: 64 y + 8 g + 2 m, and the next one) x pairs (2 q4, 2 q4 + 1)
+    float O[D / 16][NT][4];   // dims (tile m of 64 y: 64 y + 8 g + 2 m, and the next one; 4 bits: D / 8 * g + 8 y + 2 m) x pairs (2 q4, 2 q4 + 1)
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -187,9 +208,9 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     // where a lane's 8 bytes lie: rows g and g + 8 of k (these shift alike), the 32 dims x; rows 2 q4 and 2 q4 + 1 (+ 8) of v, the 64 dims y
     int kofs[4], vofs[2][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) kofs[i] = i < D / 32 ? place<D, false>(g, 2 * i + (q4 >> 1)) + (q4 & 1) * 8 : 0;
+    for (int i = 0; i < 4; ++i) kofs[i] = KIND == KV_I4 ? (i < D / 128 ? place4<D, false>(g, q4 + 4 * i) : place4<D, false>(g, q4 >> 1) + (q4 & 1) * 8) : i < D / 32 ? place<D, false>(g, 2 * i + (q4 >> 1)) + (q4 & 1) * 8 : 0;   // 4 bits: groups q4 and q4 + 4; 64 dims: half of one
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vofs[i >> 1][i & 1] = (i & 1) < D / 64 ? place<D, true>(2 * q4 + (i >> 1), 4 * (i & 1) + (g >> 1)) + (g & 1) * 8 : 0;
+    for (int i = 0; i < 4; ++i) vofs[i >> 1][i & 1] = KIND == KV_I4 ? place4<D, true>(2 * q4 + (i >> 1), g / (256 / D)) + g % (256 / D) * (D / 16) : (i & 1) < D / 64 ? place<D, true>(2 * q4 + (i >> 1), 4 * (i & 1) + (g >> 1)) + (g & 1) * 8 : 0;   // 4 bits: D / 8 dims from D / 8 * g on
     int slot = 0;
     for (; i0 < i_end; ) {
         const float sc1 = i1 < i_end ? scales(r1) : 0.f;
@@ -202,19 +223,45 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         float s[NT][4];
         {
             float sh[NT][2][4], sl[NT][4];
-            const uint8_t* kr = ring + slot * (KS * D);
-#pragma unroll
-            for (int x = 0; x < D / 32; ++x) {
-                const uint8_t* kx = kr + kofs[x & 3] + (x >> 2) * 128;
-                const uint2 ka = at_smem<uint2>(kx), kb = at_smem<uint2>(kx + 8 * D);
-                const uint32_t a0[4] = {code_pair<KIND, 0>(ka.x), code_pair<KIND, 0>(kb.x), code_pair<KIND, 2>(ka.x), code_pair<KIND, 2>(kb.x)};
-                const uint32_t a1[4] = {code_pair<KIND, 0>(ka.y), code_pair<KIND, 0>(kb.y), code_pair<KIND, 2>(ka.y), code_pair<KIND, 2>(kb.y)};
+            const uint8_t* kr = ring + slot * SLOT;
+            auto products = [&](int x, const uint32_t (&a0)[4], const uint32_t (&a1)[4]) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const uint4 h = at_smem<uint4>(qf + n * D * 32 + x * 1024), r = at_smem<uint4>(qf + n * D * 32 + x * 1024 + 512);
                     if (x == 0) { mma_f16_first(sh[n][0], a0, h.x, h.y); mma_f16_first(sl[n], a0, r.x, r.y); mma_f16_first(sh[n][1], a1, h.z, h.w); }
                     else { mma_f16(sh[n][0], a0, h.x, h.y); mma_f16(sl[n], a0, r.x, r.y); mma_f16(sh[n][1], a1, h.z, h.w); }
                     mma_f16(sl[n], a1, r.z, r.w);
+                }
+            };
+            if constexpr (KIND == KV_I4) {
+                constexpr int PER = D == 64 ? 2 : 4;   // words of a lane that lie together, in one group
+#pragma unroll
+                for (int y = 0; y < D / 32 / PER; ++y) {
+                    const uint8_t *kx = kr + kofs[y], *gx = kr + KS * RB + g * (D / 32) + (D == 64 ? q4 >> 1 : q4 + 4 * y);
+                    const I4Group ga = i4_group(__byte_perm(gx[0], 0x64u, 0x4040)), gb = i4_group(__byte_perm(gx[8 * (D / 32)], 0x64u, 0x4040));
+                    uint32_t ka[PER], kb[PER];
+                    if constexpr (PER == 4) {
+                        const uint4 u = at_smem<uint4>(kx), v = at_smem<uint4>(kx + 8 * RB);
+                        ka[0] = u.x; ka[1] = u.y; ka[2] = u.z; ka[3] = u.w; kb[0] = v.x; kb[1] = v.y; kb[2] = v.z; kb[3] = v.w;
+                    } else {
+                        const uint2 u = at_smem<uint2>(kx), v = at_smem<uint2>(kx + 8 * RB);
+                        ka[0] = u.x; ka[1] = u.y; kb[0] = v.x; kb[1] = v.y;
+                    }
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) {
+                        const uint32_t a0[4] = {i4_low(ka[i], ga), i4_low(kb[i], gb), i4_high(ka[i], ga), i4_high(kb[i], gb)};
+                        const uint32_t a1[4] = {i4_low(ka[i] >> 8, ga), i4_low(kb[i] >> 8, gb), i4_high(ka[i] >> 8, ga), i4_high(kb[i] >> 8, gb)};
+                        products(y * PER + i, a0, a1);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x) {
+                    const uint8_t* kx = kr + kofs[x & 3] + (x >> 2) * 128;
+                    const uint2 ka = at_smem<uint2>(kx), kb = at_smem<uint2>(kx + 8 * D);
+                    const uint32_t a0[4] = {code_pair<KIND, 0>(ka.x), code_pair<KIND, 0>(kb.x), code_pair<KIND, 2>(ka.x), code_pair<KIND, 2>(kb.x)};
+                    const uint32_t a1[4] = {code_pair<KIND, 0>(ka.y), code_pair<KIND, 0>(kb.y), code_pair<KIND, 2>(ka.y), code_pair<KIND, 2>(kb.y)};
+                    products(x, a0, a1);
                 }
             }
 #pragma unroll
@@ -288,27 +335,54 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         __syncwarp();
         // ---- outputs: 64 dims at a time; the 8 dims of a lane group are four tiles of 16 rows
         {
-            const uint8_t* vr = ring + slot * (KS * D);
+            const uint8_t* vr = ring + slot * SLOT;
+            auto products = [&](float (&o)[NT][4], const uint32_t (&af)[4]) {
 #pragma unroll
-            for (int y = 0; y < D / 64; ++y) {
-                uint2 v[4];   // keys 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
+                for (int n = 0; n < NT; ++n) {
+                    float f[4];
+                    mma_f16_first(f, af, br[n][0], br[n][1]);
+                    mma_f16(f, af, bh[n][0], bh[n][1]);
+                    const float2 u = add2(make_float2(o[n][0], o[n][1]), make_float2(f[0], f[1])), t = add2(make_float2(o[n][2], o[n][3]), make_float2(f[2], f[3]));
+                    o[n][0] = u.x; o[n][1] = u.y; o[n][2] = t.x; o[n][3] = t.y;
+                }
+            };
+            if constexpr (KIND == KV_I4) {   // D / 64 words of a lane group, of one group of 32 dims; a word is four tiles
+                constexpr int W = D / 64;
+                uint32_t v[4][W];   // keys 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = at_smem<uint2>(vr + vofs[i & 1][y & 1] + (y >> 1) * 128 + (i >> 1) * 8 * D);
+                for (int i = 0; i < 4; ++i) {
+                    const uint8_t* vx = vr + vofs[i & 1][0] + (i >> 1) * 8 * RB;
+                    if constexpr (W == 4) { const uint4 u = at_smem<uint4>(vx); v[i][0] = u.x; v[i][1] = u.y; v[i][2] = u.z; v[i][3] = u.w; }
+                    else if constexpr (W == 2) { const uint2 u = at_smem<uint2>(vx); v[i][0] = u.x; v[i][1] = u.y; }
+                    else v[i][0] = at_smem<uint32_t>(vx);
+                }
+                const uint8_t* gx = vr + KS * RB + 2 * q4 * (D / 32) + g / (256 / D);
+                const I4Group ga = i4_group(gx[0] | (uint32_t)gx[D / 32] << 16 | 0x64006400u), gb = i4_group(gx[8 * (D / 32)] | (uint32_t)gx[9 * (D / 32)] << 16 | 0x64006400u);
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const uint32_t x0 = w ? v[0].y : v[0].x, x1 = w ? v[1].y : v[1].x, x2 = w ? v[2].y : v[2].x, x3 = w ? v[3].y : v[3].x;
+                for (int w = 0; w < W; ++w)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t lo2 = __byte_perm(x0, x1, h ? 0x7362 : 0x5140), hi2 = __byte_perm(x2, x3, h ? 0x7362 : 0x5140);
-                        const uint32_t af[4] = {code_pair<KIND, 0>(lo2), code_pair<KIND, 2>(lo2), code_pair<KIND, 0>(hi2), code_pair<KIND, 2>(hi2)};
+                        const uint32_t lo = __byte_perm(v[0][w], v[1][w], h ? 0x7632 : 0x5410), hi = __byte_perm(v[2][w], v[3][w], h ? 0x7632 : 0x5410);   // four dims of two keys
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            float f[4];
-                            mma_f16_first(f, af, br[n][0], br[n][1]);
-                            mma_f16(f, af, bh[n][0], bh[n][1]);
-                            float (&o)[4] = O[y * 4 + w * 2 + h][n];
-                            const float2 u = add2(make_float2(o[0], o[1]), make_float2(f[0], f[1])), t = add2(make_float2(o[2], o[3]), make_float2(f[2], f[3]));
-                            o[0] = u.x; o[1] = u.y; o[2] = t.x; o[3] = t.y;
+                        for (int k = 0; k < 2; ++k) {
+                            const uint32_t af[4] = {i4_low(lo >> (8 * k), ga), i4_high(lo >> (8 * k), ga), i4_low(hi >> (8 * k), gb), i4_high(hi >> (8 * k), gb)};
+                            products(O[w * 4 + h * 2 + k], af);
+                        }
+                    }
+            } else {
+#pragma unroll
+                for (int y = 0; y < D / 64; ++y) {
+                    uint2 v[4];   // keys 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = at_smem<uint2>(vr + vofs[i & 1][y & 1] + (y >> 1) * 128 + (i >> 1) * 8 * D);
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const uint32_t x0 = w ? v[0].y : v[0].x, x1 = w ? v[1].y : v[1].x, x2 = w ? v[2].y : v[2].x, x3 = w ? v[3].y : v[3].x;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t lo2 = __byte_perm(x0, x1, h ? 0x7362 : 0x5140), hi2 = __byte_perm(x2, x3, h ? 0x7362 : 0x5140);
+                            const uint32_t af[4] = {code_pair<KIND, 0>(lo2), code_pair<KIND, 2>(lo2), code_pair<KIND, 0>(hi2), code_pair<KIND, 2>(hi2)};
+                            products(O[y * 4 + w * 2 + h], af);
                         }
                     }
                 }
@@ -334,12 +408,12 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            float* dst = xo + (size_t)(warp * MB + 8 * n + 2 * q4 + c) * XS + 8 * g;
+            float* dst = xo + (size_t)(warp * MB + 8 * n + 2 * q4 + c) * XS + (KIND == KV_I4 ? D / 8 : 8) * g;
 #pragma unroll
             for (int y = 0; y < D / 64; ++y)
 #pragma unroll
                 for (int m = 0; m < 4; m += 2)
-                    *reinterpret_cast<float4*>(dst + 64 * y + 2 * m) = make_float4(O[y * 4 + m][n][c], O[y * 4 + m][n][c + 2], O[y * 4 + m + 1][n][c], O[y * 4 + m + 1][n][c + 2]);
+                    *reinterpret_cast<float4*>(dst + (KIND == KV_I4 ? 8 : 64) * y + 2 * m) = make_float4(O[y * 4 + m][n][c], O[y * 4 + m][n][c + 2], O[y * 4 + m + 1][n][c], O[y * 4 + m + 1][n][c + 2]);
             if (g == 0) { s_mu[warp][8 * n + 2 * q4 + c] = mu[n][c]; s_l[warp][8 * n + 2 * q4 + c] = l[n][c]; }
         }
     __syncthreads();
@@ -538,7 +612,7 @@ Plan plan_of(const PagedPool& pool, const PagedBatch& b, int n_head, int window,
 size_t partials(const Plan& p, const PagedBatch& b, int n_head) { return (size_t)b.R * n_head * (p.ns + p.nwin); }
 
 template <int D, int KIND, int NT, bool DIRECT> int launch_split(const PagedArgs& a, dim3 grid, cudaStream_t s) {
-    constexpr int smem = smem_bytes(D, NT);
+    constexpr int smem = smem_bytes(D, KIND, NT);
     static bool attr[MAX_DEVICES] = {};   // per device: the opt-in belongs to the device's copy of the kernel
     const int dev = current_device(); if (dev < 0) return HP_ECUDA;
     if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_split<D, KIND, NT, DIRECT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); attr[dev] = true; }
@@ -573,7 +647,7 @@ int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams
     // One split: its kernel writes the outputs, for the price of a merge's launch (captured and host's time of 32 tokens of 32 heads over 8 at 256 tokens 14.6 and 9.9 us, now 8.6 and 7.3)
     a.direct = wide && pl.ns + pl.nwin == 1;
     const dim3 grid(pl.ns + pl.nwin, pool.n_kv, (unsigned)pl.blocks);
-    const int rc = b.max_rows > PAGED_DECODE_ROWS ? attn_paged_tc(a, grid, s) : pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, pl.MB, s) : launch_split<KV_E4M3>(a, grid, pl.MB, s);
+    const int rc = b.max_rows > PAGED_DECODE_ROWS ? attn_paged_tc(a, grid, s) : pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, pl.MB, s) : pool.kind == KV_E4M3 ? launch_split<KV_E4M3>(a, grid, pl.MB, s) : launch_split<KV_I4>(a, grid, pl.MB, s);
     if (rc != HP_OK || a.direct) return rc;
     MergeArgs m; m.b = b; m.pO = a.pO; m.pml = a.pml; m.gate = p.gate; m.g_ld = p.g_ld; m.g_hs = p.g_hs; m.n_head = p.n_head; m.window = p.window; m.n_sink = p.n_sink;
     m.U = pl.U; m.ns = pl.ns; m.nwin = pl.nwin; m.mul = a.mul; m.out = p.out; m.oq = (int8_t*)p.xq.q; m.osc = (float*)p.xq.sc; m.err = a.arg_err;

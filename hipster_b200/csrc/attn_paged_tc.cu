@@ -470,8 +470,14 @@ __global__ void __launch_bounds__(256) k_paged_f16(const PagedArgs a) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int e = e0 + u * 256, row = e / cpr, part = e % cpr;
-            w[u] = make_uint4(0, 0, 0, 0);   // codes of zero
-            if (e < TK * cpr && rows[row >> 4] != 0xffffffffu && t * TK + row < q.len) w[u] = *reinterpret_cast<const uint4*>(src + ((size_t)rows[row >> 4] + (row & 15)) * D + part * 16);
+            w[u] = make_uint4(0, 0, 0, 0);   // codes of zero; 4 bits: two words of codes, and a factor of zero
+            if (e < TK * cpr && rows[row >> 4] != 0xffffffffu && t * TK + row < q.len) {
+                if constexpr (KIND == KV_I4) {
+                    const I4Row at = i4_row(rows[row >> 4] + (row & 15), lg, D);
+                    const uint2 c = *reinterpret_cast<const uint2*>(src + at.codes + part * 8);
+                    w[u] = make_uint4(c.x, c.y, src[at.groups + (part >> 1)], 0u);
+                } else w[u] = *reinterpret_cast<const uint4*>(src + ((size_t)rows[row >> 4] + (row & 15)) * D + part * 16);
+            }
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -479,8 +485,14 @@ __global__ void __launch_bounds__(256) k_paged_f16(const PagedArgs a) {
             if (e >= TK * cpr) break;
             uint8_t* o = dst + (part >> 2) * (TK * 128) + row * 128;
             const int ch = (part & 3) * 2;
-            *reinterpret_cast<uint4*>(o + ((ch ^ (row & 7)) << 4)) = make_uint4(code_pair<KIND, 0>(w[u].x), code_pair<KIND, 2>(w[u].x), code_pair<KIND, 0>(w[u].y), code_pair<KIND, 2>(w[u].y));
-            *reinterpret_cast<uint4*>(o + (((ch + 1) ^ (row & 7)) << 4)) = make_uint4(code_pair<KIND, 0>(w[u].z), code_pair<KIND, 2>(w[u].z), code_pair<KIND, 0>(w[u].w), code_pair<KIND, 2>(w[u].w));
+            if constexpr (KIND == KV_I4) {
+                const I4Group g = i4_group(__byte_perm(w[u].z, 0x64u, 0x4040));
+                *reinterpret_cast<uint4*>(o + ((ch ^ (row & 7)) << 4)) = i4_word(w[u].x, g);
+                *reinterpret_cast<uint4*>(o + (((ch + 1) ^ (row & 7)) << 4)) = i4_word(w[u].y, g);
+            } else {
+                *reinterpret_cast<uint4*>(o + ((ch ^ (row & 7)) << 4)) = make_uint4(code_pair<KIND, 0>(w[u].x), code_pair<KIND, 2>(w[u].x), code_pair<KIND, 0>(w[u].y), code_pair<KIND, 2>(w[u].y));
+                *reinterpret_cast<uint4*>(o + (((ch + 1) ^ (row & 7)) << 4)) = make_uint4(code_pair<KIND, 0>(w[u].z), code_pair<KIND, 2>(w[u].z), code_pair<KIND, 0>(w[u].w), code_pair<KIND, 2>(w[u].w));
+            }
         }
     }
 }
@@ -490,7 +502,7 @@ template <int D, int KIND, bool DIRECT> int launch_split(const PagedArgs& a, dim
     static bool attr[MAX_DEVICES] = {};   // per device: the opt-in belongs to the device's copy of the kernel
     const int dev = current_device(); if (dev < 0) return HP_ECUDA;
     if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_paged_prompt<D, KIND, DIRECT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo::SMEM)); attr[dev] = true; }
-    HP_CUDA(launch_pdl<4>(k_paged_f16<KIND>, dim3(a.tiles, 2 * a.pool.n_kv, a.b.S), dim3(256), 0, s, a));
+    HP_CUDA(launch_pdl<4>(a.pool.kind == KV_I4 ? k_paged_f16<KV_I4> : k_paged_f16<KIND>, dim3(a.tiles, 2 * a.pool.n_kv, a.b.S), dim3(256), 0, s, a));
     HP_CUDA(launch_pdl<4>(k_paged_prompt<D, KIND, DIRECT>, grid, dim3(Geo::WARPS * 32), Geo::SMEM, s, a));
     return HP_OK;
 }
@@ -505,7 +517,7 @@ size_t attn_paged_tc_bytes(const PagedPool& pool, const PagedBatch& b) { return 
 int attn_paged_tc(PagedArgs& a, dim3 grid, cudaStream_t s) {
     a.tiles = (a.b.max_kv + TK - 1) / TK;
     HP_REQUIRE(a.b.S <= 65535 && 2 * a.pool.n_kv <= 65535, "attn_paged: too many sequences (%d) or heads for a prompt", a.b.S);
-    return a.pool.kind == KV_I8 ? launch_split<KV_I8>(a, grid, s) : launch_split<KV_E4M3>(a, grid, s);
+    return a.pool.kind == KV_E4M3 ? launch_split<KV_E4M3>(a, grid, s) : launch_split<KV_I8>(a, grid, s);   // behind the pictures 4 bits are whole numbers as int8 is
 }
 
 }  // namespace hp

@@ -233,14 +233,14 @@ int hp_moe_layer(const float* xn_dev, const void* xq_q_dev, const void* xq_sc_de
     HP_GUARD_END
 }
 
-// ------------------------------------------------------------------ paged 8-bit cache
+// ------------------------------------------------------------------ paged cache in 8 or 4 bits, prompts
 namespace {
 // columns of the table in use, and the tokens that they hold
 int columns_of(const hp_kv_pages* c, int table_ld) { return c->columns ? c->columns : table_ld; }
 int capacity(const hp_kv_pages* c, int table_ld) { return columns_of(c, table_ld) * c->page_size; }
 int paged_args(const char* who, const hp_kv_pages* c, const int* table, int table_ld, const int* row_start, const int* kv_len, int S, int R, long long max_rows, long long max_kv, hp::PagedPool* p, hp::PagedBatch* b) {
     HP_REQUIRE(c, "%s: null cache", who);
-    HP_REQUIRE(c->type == HP_KV_I8 || c->type == HP_KV_E4M3, "%s: unknown cache type %d", who, c->type);
+    HP_REQUIRE(c->type == HP_KV_I8 || c->type == HP_KV_E4M3 || c->type == HP_KV_I4, "%s: unknown cache type %d", who, c->type);
     HP_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "%s: head_dim must be 64, 128 or 256, not %d", who, c->head_dim);
     HP_REQUIRE(c->page_size >= 16 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0, "%s: page_size must be a power of two from 16 to 1024, not %d", who, c->page_size);
     const int columns = columns_of(c, table_ld);
@@ -264,6 +264,19 @@ bool apart(long long R, long long ld, long long heads, long long hs, long long d
     auto nested = [&](long long n, long long inner, long long m, long long outer) { return (n == 1 || inner >= dim) && (m == 1 || (outer >= dim && (outer - dim) / (n > 1 ? n - 1 : 1) >= (n > 1 ? inner : 0))); };
     return nested(heads, hs, R, ld) || nested(R, ld, heads, hs);
 }
+// positions of several axes: the host's bytes as two bits per pair
+int axes_args(const char* who, const int* pos, long long pos_ld, const unsigned char* axes, int n_axes, int n_rot, int R, hp::RopeAxes* o) {
+    HP_REQUIRE(pos && axes, "%s: null positions or axes", who);
+    HP_REQUIRE(n_axes >= 1 && n_axes <= 4 && ((uintptr_t)pos & 3) == 0 && (n_axes == 1 || pos_ld >= 0), "%s: bad positions n_axes=%d pos_ld=%lld", who, n_axes, pos_ld);
+    HP_REQUIRE(n_rot >= 2 && n_rot <= 256, "%s: bad n_rot=%d for positions", who, n_rot);
+    o->pos = pos; o->pos_ld = (size_t)pos_ld; o->n_axes = n_axes;
+    for (int i = 0; i < 8; ++i) o->axes[i] = 0;
+    for (int i = 0; i < n_rot / 2; ++i) {
+        HP_REQUIRE(axes[i] < n_axes, "%s: pair %d has axis %d of %d", who, i, (int)axes[i], n_axes);
+        o->axes[i >> 4] |= (uint32_t)axes[i] << (2 * (i & 15));
+    }
+    return HP_OK;
+}
 bool rows_ok(const void* p, long long ld, long long hs) { return ((uintptr_t)p & 15) == 0 && ld % 4 == 0 && hs % 4 == 0 && ld >= 0 && hs >= 0; }
 }
 int hp_rope_table(float* table_dev, int n_pos, int n_rot, double base, int scaling, double factor, int orig_ctx, double beta_fast, double beta_slow, double attn_factor, void* stream) {
@@ -277,22 +290,72 @@ int hp_rope_table(float* table_dev, int n_pos, int n_rot, double base, int scali
     return hp::rope_table(table_dev, n_pos, n_rot, base, scaling, factor, orig_ctx, beta_fast, beta_slow, attn_factor, (cudaStream_t)stream);
     HP_GUARD_END
 }
+static int append(const char* who, const hp::RopeAxes& axes, const float* q_dev, long long q_ld, long long q_hs, float* q_out_dev, long long qo_ld, long long qo_hs, int n_head, const float* k_dev, long long k_ld, long long k_hs,
+                  const float* v_dev, long long v_ld, long long v_hs, const void* q_norm_bf16_dev, const void* k_norm_bf16_dev, const float* rope_dev, int n_pos, int n_rot, int interleaved,
+                  const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, float eps, void* stream) {
+    hp::PagedPool pool; hp::PagedBatch b;
+    { int rc = paged_args(who, pages, table_dev, table_ld, row_start_dev, kv_len_dev, S, R, R, 1 << 30, &pool, &b); if (!rc) rc = paged_ptrs(who, pages, table_dev, row_start_dev, kv_len_dev); if (rc) return rc; }
+    HP_REQUIRE(k_dev && v_dev && n_head >= 0 && (n_head == 0 || (q_dev && q_out_dev)) && (n_rot == 0 || rope_dev), "%s: null pointer", who);
+    HP_REQUIRE(n_rot >= 0 && n_rot % 2 == 0 && n_rot <= pool.head_dim && (n_rot == 0 || n_pos >= 1) && ((uintptr_t)rope_dev & 7) == 0, "%s: bad n_rot=%d n_pos=%d or rope table", who, n_rot, n_pos);
+    HP_REQUIRE(rows_ok(k_dev, k_ld, k_hs) && rows_ok(v_dev, v_ld, v_hs) && (n_head == 0 || (rows_ok(q_dev, q_ld, q_hs) && rows_ok(q_out_dev, qo_ld, qo_hs))), "%s: rows must be 16-byte aligned, with strides that are multiples of 4", who);
+    HP_REQUIRE((((uintptr_t)q_norm_bf16_dev | (uintptr_t)k_norm_bf16_dev) & 1) == 0, "%s: norm weights must be 2-byte aligned", who);
+    HP_REQUIRE(n_head == 0 || apart(R, qo_ld, n_head, qo_hs, pool.head_dim), "%s: rows of q_out lie over each other", who);
+    HP_REQUIRE(n_head == 0 || q_dev != q_out_dev || ((R == 1 || q_ld == qo_ld) && (n_head == 1 || q_hs == qo_hs)), "%s: q_out in place of q must have its strides", who);
+    HP_REQUIRE((long long)R * (n_head + 2 * pool.n_kv) < (1ll << 33), "%s: too many rows", who);
+    hp::KvAppendParams p; p.q = q_dev; p.q_ld = q_ld; p.q_hs = q_hs; p.q_out = q_out_dev; p.qo_ld = qo_ld; p.qo_hs = qo_hs; p.n_head = n_head; p.k = k_dev; p.k_ld = k_ld; p.k_hs = k_hs;
+    p.v = v_dev; p.v_ld = v_ld; p.v_hs = v_hs; p.q_norm = q_norm_bf16_dev; p.k_norm = k_norm_bf16_dev; p.rope = rope_dev; p.n_pos = n_rot ? n_pos : 1 << 30; p.n_rot = n_rot; p.interleaved = interleaved; p.eps = eps;
+    return hp::kv_append(pool, b, p, axes, (cudaStream_t)stream);
+}
 int hp_kv_append(const float* q_dev, long long q_ld, long long q_hs, float* q_out_dev, long long qo_ld, long long qo_hs, int n_head, const float* k_dev, long long k_ld, long long k_hs,
                  const float* v_dev, long long v_ld, long long v_hs, const void* q_norm_bf16_dev, const void* k_norm_bf16_dev, const float* rope_dev, int n_pos, int n_rot, int interleaved,
                  const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, float eps, void* stream) {
     HP_GUARD_BEGIN
-    hp::PagedPool pool; hp::PagedBatch b;
-    { int rc = paged_args("hp_kv_append", pages, table_dev, table_ld, row_start_dev, kv_len_dev, S, R, R, 1 << 30, &pool, &b); if (!rc) rc = paged_ptrs("hp_kv_append", pages, table_dev, row_start_dev, kv_len_dev); if (rc) return rc; }
-    HP_REQUIRE(k_dev && v_dev && n_head >= 0 && (n_head == 0 || (q_dev && q_out_dev)) && (n_rot == 0 || rope_dev), "hp_kv_append: null pointer");
-    HP_REQUIRE(n_rot >= 0 && n_rot % 2 == 0 && n_rot <= pool.head_dim && (n_rot == 0 || n_pos >= 1) && ((uintptr_t)rope_dev & 7) == 0, "hp_kv_append: bad n_rot=%d n_pos=%d or rope table", n_rot, n_pos);
-    HP_REQUIRE(rows_ok(k_dev, k_ld, k_hs) && rows_ok(v_dev, v_ld, v_hs) && (n_head == 0 || (rows_ok(q_dev, q_ld, q_hs) && rows_ok(q_out_dev, qo_ld, qo_hs))), "hp_kv_append: rows must be 16-byte aligned, with strides that are multiples of 4");
-    HP_REQUIRE((((uintptr_t)q_norm_bf16_dev | (uintptr_t)k_norm_bf16_dev) & 1) == 0, "hp_kv_append: norm weights must be 2-byte aligned");
-    HP_REQUIRE(n_head == 0 || apart(R, qo_ld, n_head, qo_hs, pool.head_dim), "hp_kv_append: rows of q_out lie over each other");
-    HP_REQUIRE(n_head == 0 || q_dev != q_out_dev || ((R == 1 || q_ld == qo_ld) && (n_head == 1 || q_hs == qo_hs)), "hp_kv_append: q_out in place of q must have its strides");
-    HP_REQUIRE((long long)R * (n_head + 2 * pool.n_kv) < (1ll << 33), "hp_kv_append: too many rows");
-    hp::KvAppendParams p; p.q = q_dev; p.q_ld = q_ld; p.q_hs = q_hs; p.q_out = q_out_dev; p.qo_ld = qo_ld; p.qo_hs = qo_hs; p.n_head = n_head; p.k = k_dev; p.k_ld = k_ld; p.k_hs = k_hs;
-    p.v = v_dev; p.v_ld = v_ld; p.v_hs = v_hs; p.q_norm = q_norm_bf16_dev; p.k_norm = k_norm_bf16_dev; p.rope = rope_dev; p.n_pos = n_rot ? n_pos : 1 << 30; p.n_rot = n_rot; p.interleaved = interleaved; p.eps = eps;
-    return hp::kv_append(pool, b, p, (cudaStream_t)stream);
+    return append("hp_kv_append", hp::RopeAxes{}, q_dev, q_ld, q_hs, q_out_dev, qo_ld, qo_hs, n_head, k_dev, k_ld, k_hs, v_dev, v_ld, v_hs, q_norm_bf16_dev, k_norm_bf16_dev, rope_dev, n_pos, n_rot, interleaved, table_dev, table_ld,
+                  row_start_dev, kv_len_dev, S, R, pages, eps, stream);
+    HP_GUARD_END
+}
+int hp_kv_append_axes(const float* q_dev, long long q_ld, long long q_hs, float* q_out_dev, long long qo_ld, long long qo_hs, int n_head, const float* k_dev, long long k_ld, long long k_hs,
+                      const float* v_dev, long long v_ld, long long v_hs, const void* q_norm_bf16_dev, const void* k_norm_bf16_dev, const float* rope_dev, int n_pos, int n_rot, int interleaved,
+                      const int* pos_dev, long long pos_ld, const unsigned char* axes_host, int n_axes,
+                      const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, float eps, void* stream) {
+    HP_GUARD_BEGIN
+    hp::RopeAxes axes;
+    { const int rc = axes_args("hp_kv_append_axes", pos_dev, pos_ld, axes_host, n_axes, n_rot, R, &axes); if (rc) return rc; }
+    return append("hp_kv_append_axes", axes, q_dev, q_ld, q_hs, q_out_dev, qo_ld, qo_hs, n_head, k_dev, k_ld, k_hs, v_dev, v_ld, v_hs, q_norm_bf16_dev, k_norm_bf16_dev, rope_dev, n_pos, n_rot, interleaved, table_dev, table_ld,
+                  row_start_dev, kv_len_dev, S, R, pages, eps, stream);
+    HP_GUARD_END
+}
+int hp_rope_rows(const float* q_dev, long long q_ld, long long q_hs, void* q_out_dev, long long qo_ld, long long qo_hs, int n_head, const float* k_dev, long long k_ld, long long k_hs, void* k_out_dev, long long ko_ld, long long ko_hs,
+                 const float* v_dev, long long v_ld, long long v_hs, void* v_out_dev, long long vo_ld, long long vo_hs, int n_kv, int head_dim, int out_type, const void* q_norm_bf16_dev, const void* k_norm_bf16_dev,
+                 const float* rope_dev, int n_pos, int n_rot, int interleaved, const int* pos_dev, long long pos_ld, const unsigned char* axes_host, int n_axes, int R, float eps, void* stream) {
+    HP_GUARD_BEGIN
+    HP_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "hp_rope_rows: head_dim must be 64, 128 or 256, not %d", head_dim);
+    HP_REQUIRE(out_type == HP_F32 || out_type == HP_F16 || out_type == HP_BF16, "hp_rope_rows: unknown output type %d", out_type);
+    HP_REQUIRE(R >= 1 && n_head >= 0 && n_kv >= 0, "hp_rope_rows: bad shape R=%d n_head=%d n_kv=%d", R, n_head, n_kv);
+    HP_REQUIRE(n_rot >= 0 && n_rot % 2 == 0 && n_rot <= head_dim && (n_rot == 0 || (n_pos >= 1 && rope_dev)) && ((uintptr_t)rope_dev & 7) == 0, "hp_rope_rows: bad n_rot=%d n_pos=%d or rope table", n_rot, n_pos);
+    HP_REQUIRE((((uintptr_t)q_norm_bf16_dev | (uintptr_t)k_norm_bf16_dev) & 1) == 0, "hp_rope_rows: norm weights must be 2-byte aligned");
+    hp::RopeAxes axes{};
+    if (n_rot) { const int rc = axes_args("hp_rope_rows", pos_dev, pos_ld, axes_host, n_axes, n_rot, R, &axes); if (rc) return rc; }
+    hp::RopeRowsParams p;
+    const float* in[3] = {q_dev, k_dev, v_dev}; void* out[3] = {q_out_dev, k_out_dev, v_out_dev};
+    const long long ld[3] = {q_ld, k_ld, v_ld}, hs[3] = {q_hs, k_hs, v_hs}, old[3] = {qo_ld, ko_ld, vo_ld}, ohs[3] = {qo_hs, ko_hs, vo_hs};
+    int heads = 0;
+    for (int i = 0; i < 3; ++i) {
+        HP_REQUIRE((in[i] == nullptr) == (out[i] == nullptr), "hp_rope_rows: null pointer");
+        const int n = in[i] ? (i ? n_kv : n_head) : 0;
+        if (n) {
+            HP_REQUIRE(rows_ok(in[i], ld[i], hs[i]) && rows_ok(out[i], old[i], ohs[i]) && (out_type == HP_F32 || ((old[i] | ohs[i]) & 7) == 0), "hp_rope_rows: rows must be 16-byte aligned, with strides that are multiples of 16 bytes");
+            HP_REQUIRE(apart(R, old[i], n, ohs[i], head_dim), "hp_rope_rows: rows of an output lie over each other");
+            HP_REQUIRE((const void*)in[i] != out[i] || (out_type == HP_F32 && (R == 1 || ld[i] == old[i]) && (n == 1 || hs[i] == ohs[i])), "hp_rope_rows: an output in place of its input must be f32 with its strides");
+            for (int j = 0; j < i; ++j) HP_REQUIRE(!p.heads[j] || out[i] != out[j], "hp_rope_rows: two outputs are the same");
+        }
+        p.in[i] = in[i]; p.out[i] = out[i]; p.in_ld[i] = (size_t)ld[i]; p.in_hs[i] = (size_t)hs[i]; p.out_ld[i] = (size_t)old[i]; p.out_hs[i] = (size_t)ohs[i]; p.heads[i] = n;
+        heads += n;
+    }
+    HP_REQUIRE(heads >= 1, "hp_rope_rows: no rows");
+    HP_REQUIRE((long long)R * heads < (1ll << 33), "hp_rope_rows: too many rows");
+    p.norm[0] = q_norm_bf16_dev; p.norm[1] = k_norm_bf16_dev; p.rope = rope_dev; p.n_pos = n_pos; p.n_rot = n_rot; p.interleaved = interleaved; p.eps = eps; p.R = R; p.head_dim = head_dim; p.type = out_type;
+    return hp::rope_rows(p, axes, (cudaStream_t)stream);
     HP_GUARD_END
 }
 int hp_kv_read(const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, void* k_out_f16_dev, void* v_out_f16_dev, long long row_stride, long long head_stride, void* stream) {
@@ -333,6 +396,27 @@ int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const floa
     hp::AttnPagedParams p; p.q = q_dev; p.q_ld = q_ld; p.q_hs = q_hs; p.gate = gate_dev; p.g_ld = g_ld; p.g_hs = g_hs; p.n_head = n_head; p.scale = scale; p.window = window; p.n_sink = n_sink; p.cap = capacity(pages, table_ld);
     p.out = out_dev; p.xq = hp::XQ8F{xq_q_dev, xq_sc_dev}; p.workspace = workspace_dev;
     return hp::attn_paged(pool, b, p, (cudaStream_t)stream);
+    HP_GUARD_END
+}
+
+int hp_attn_prompt(const void* q_dev, long long q_ld, long long q_hs, const void* k_dev, long long k_ld, long long k_hs, const void* v_dev, long long v_ld, long long v_hs, int type, const float* gate_dev, long long g_ld, long long g_hs,
+                   int n_head, int n_kv, int head_dim, const int* row_start_dev, int S, int R, int max_rows, float scale, void* out_dev, void* xq_q_dev, void* xq_sc_dev, void* stream) {
+    HP_GUARD_BEGIN
+    HP_REQUIRE(type == HP_F16 || type == HP_BF16, "hp_attn_prompt: type must be HP_F16 or HP_BF16, not %d", type);
+    HP_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "hp_attn_prompt: head_dim must be 64, 128 or 256, not %d", head_dim);
+    HP_REQUIRE(n_kv >= 1 && n_head >= 1 && n_head % n_kv == 0, "hp_attn_prompt: n_head=%d must be a multiple of n_kv=%d", n_head, n_kv);
+    HP_REQUIRE(S >= 1 && R >= 1 && max_rows >= 1, "hp_attn_prompt: bad batch S=%d R=%d max_rows=%d", S, R, max_rows);
+    HP_REQUIRE(q_dev && k_dev && v_dev && row_start_dev && (out_dev || xq_q_dev), "hp_attn_prompt: null pointer");
+    HP_REQUIRE((xq_q_dev == nullptr) == (xq_sc_dev == nullptr), "hp_attn_prompt: give both quantised-output buffers or neither");
+    HP_REQUIRE((((uintptr_t)out_dev | (uintptr_t)xq_q_dev | (uintptr_t)xq_sc_dev) & 15) == 0 && ((uintptr_t)row_start_dev & 3) == 0, "hp_attn_prompt: outputs must be 16-byte aligned");
+    auto fits = [&](const void* p, long long ld, long long hs, int heads) { return rows_ok(p, ld, hs) && ((ld | hs) & 7) == 0 && (R == 1 || (ld > 0 && ld < (1ll << 38))) && (heads == 1 || (hs > 0 && hs < (1ll << 38))); };
+    HP_REQUIRE(fits(q_dev, q_ld, q_hs, n_head) && fits(k_dev, k_ld, k_hs, n_kv) && fits(v_dev, v_ld, v_hs, n_kv), "hp_attn_prompt: rows must be 16-byte aligned, with positive strides that are multiples of 8");
+    HP_REQUIRE(!gate_dev || rows_ok(gate_dev, g_ld, g_hs), "hp_attn_prompt: the gate must be 16-byte aligned, with strides that are multiples of 4");
+    HP_REQUIRE(scale > 0 && scale < 1e30f, "hp_attn_prompt: bad scale");
+    hp::AttnPromptParams p; p.q = q_dev; p.q_ld = (size_t)q_ld; p.q_hs = (size_t)q_hs; p.k = k_dev; p.k_ld = (size_t)k_ld; p.k_hs = (size_t)k_hs; p.v = v_dev; p.v_ld = (size_t)v_ld; p.v_hs = (size_t)v_hs; p.type = type;
+    p.n_head = n_head; p.n_kv = n_kv; p.head_dim = head_dim; p.gate = gate_dev; p.g_ld = (size_t)g_ld; p.g_hs = (size_t)g_hs; p.row_start = row_start_dev; p.S = S; p.R = R; p.max_rows = max_rows < R ? max_rows : R; p.scale = scale;
+    p.out = out_dev; p.xq = hp::XQ8F{xq_q_dev, xq_sc_dev};
+    return hp::attn_prompt(p, (cudaStream_t)stream);
     HP_GUARD_END
 }
 

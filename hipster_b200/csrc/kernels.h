@@ -181,10 +181,10 @@ int argmax_static_max_n();
 // greedy prefix acceptance on device: out[0] = accepted drafts mm, out[1] = bonus id ids[mm]
 int accept_greedy(const int* ids, const int* drafts, int n_draft, int* out, cudaStream_t s);
 
-// ---- kv_pages.cu, attn_paged.cu: a cache of 8-bit pages for ragged batches (no counterpart in the reference) ----
-enum : int { KV_I8 = 0, KV_E4M3 = 1 };
+// ---- kv_pages.cu, attn_paged.cu: a cache of pages in 8 or 4 bits for ragged batches (no counterpart in the reference) ----
+enum : int { KV_I8 = 0, KV_E4M3 = 1, KV_I4 = 4 };
 struct PagedPool {
-    uint8_t* k; uint8_t* v; float* k_scale; float* v_scale;   // codes [n_pages][n_kv][page][head_dim], scales [n_pages][n_kv][page]
+    uint8_t* k; uint8_t* v; float* k_scale; float* v_scale;   // codes [n_pages][n_kv][page][head_dim] (4 bits: see I4Row in paged.cuh), scales [n_pages][n_kv][page]
     const int* table; int table_ld;                           // [S][table_ld]
     int kind, n_pages, n_kv, lg_page, head_dim;
 };
@@ -195,7 +195,16 @@ struct KvAppendParams {
     const float* k; size_t k_ld, k_hs; const float* v; size_t v_ld, v_hs;
     const void* q_norm; const void* k_norm; const float* rope; int n_pos, n_rot, interleaved; float eps;
 };
-int kv_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, cudaStream_t s);
+// Positions of several axes: pos[axis * pos_ld + row]; two bits per pair of dims tell its axis. pos = nullptr: the row's position in its cache
+struct RopeAxes { const int* pos; size_t pos_ld; int n_axes; uint32_t axes[8]; };
+int kv_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, const RopeAxes& axes, cudaStream_t s);
+// rows of q, k and v to outputs of a type (head counts of 0: none)
+enum : int { OUT_F32 = 0, OUT_F16 = 1, OUT_BF16 = 2 };
+struct RopeRowsParams {
+    const float* in[3]; size_t in_ld[3], in_hs[3]; void* out[3]; size_t out_ld[3], out_hs[3]; int heads[3];   // q, k, v
+    const void* norm[2]; const float* rope; int n_pos, n_rot, interleaved; float eps; int R, head_dim, type;
+};
+int rope_rows(const RopeRowsParams& p, const RopeAxes& axes, cudaStream_t s);
 int kv_read(const PagedPool& pool, const PagedBatch& b, void* k_out, void* v_out, size_t row_stride, size_t head_stride, cudaStream_t s);
 struct AttnPagedParams {
     const float* q; const float* gate; size_t q_ld, q_hs, g_ld, g_hs; int n_head; float scale; int window, n_sink; int cap;   // cap: tokens that the table's columns in use hold
@@ -203,5 +212,12 @@ struct AttnPagedParams {
 };
 size_t attn_paged_workspace_bytes(const PagedPool& pool, const PagedBatch& b, int n_head, int window, int n_sink, int cap);
 int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams& p, cudaStream_t s);
+
+// ---- attn_prompt.cu: causal attention of packed prompts in 16 bits (no counterpart in the reference) ----
+struct AttnPromptParams {
+    const void* q; const void* k; const void* v; size_t q_ld, q_hs, k_ld, k_hs, v_ld, v_hs; int type, n_head, n_kv, head_dim;   // type: OUT_F16, OUT_BF16
+    const float* gate; size_t g_ld, g_hs; const int* row_start; int S, R, max_rows; float scale; void* out; XQ8F xq;
+};
+int attn_prompt(const AttnPromptParams& p, cudaStream_t s);
 
 }  // namespace hp

@@ -6,6 +6,7 @@
 // plain store: the same token appended again leaves the same bytes.
 #include "paged.cuh"
 #include <algorithm>
+#include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <type_traits>
 
@@ -78,12 +79,100 @@ template <int KIND> __device__ __forceinline__ uint32_t kv_code(float x) {
     if constexpr (KIND == KV_I8) return (uint32_t)min(127, max(-127, __float2int_rn(x))) & 0xffu;
     else return (uint32_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
 }
+// A head's norm (nw = nullptr: none) and rotation (n_rot = 0: none) where D / 8 lanes hold 8 neighbouring dims each; cs: angles of the lane's elements, interleaved of its four pairs; row: D floats of
+// shared memory of these lanes
+template <int D>
+__device__ __forceinline__ void turn_head(float (&x)[8], const uint16_t* nw, int n_rot, int interleaved, float eps, const float2 (&cs)[8], int d0, unsigned mask, float* row) {
+    constexpr int LPH = D / 8;
+    const int half = n_rot / 2;
+    const bool turns = d0 < n_rot;
+    if (nw) {
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+#pragma unroll
+        for (int off = LPH / 2; off > 0; off >>= 1) ss = ss + __shfl_xor_sync(mask, ss, off);
+        const float inv = 1.0f / sqrtf(ss / (float)D + eps);
+        const uint16_t* w = nw + d0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (x[j] * inv) * bf2f(w[j]);
+    }
+    if (!n_rot) return;
+    if (interleaved) {   // the other one of a pair is the lane's own
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+            if (d0 + j < n_rot) {
+                const float x0 = x[j], x1 = x[j + 1];
+                x[j] = fmaf(-x1, cs[j].y, x0 * cs[j].x); x[j + 1] = fmaf(x1, cs[j].x, x0 * cs[j].y);
+            }
+        return;
+    }
+    __syncwarp(mask);
+    reinterpret_cast<float4*>(row + d0)[0] = make_float4(x[0], x[1], x[2], x[3]); reinterpret_cast<float4*>(row + d0)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    __syncwarp(mask);
+    if (!turns) return;
+    if (half % 8 == 0) {   // the lane's elements are all first or all second ones
+        const float* t = row + (d0 < half ? d0 + half : d0 - half);
+        const float4 u = reinterpret_cast<const float4*>(t)[0], v = reinterpret_cast<const float4*>(t)[1];
+        const float o[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w}, sign = d0 < half ? -1.f : 1.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = d0 < half ? fmaf(sign * o[j], cs[j].y, x[j] * cs[j].x) : fmaf(x[j], cs[j].x, o[j] * cs[j].y);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int d = d0 + j;
+            if (d < half) x[j] = fmaf(-row[d + half], cs[j].y, x[j] * cs[j].x); else if (d < n_rot) x[j] = fmaf(x[j], cs[j].x, row[d - half] * cs[j].y);
+        }
+    }
+}
+// angles of the lane's elements (interleaved: of its four pairs) at one position
+__device__ __forceinline__ void angles(float2 (&cs)[8], const float* rope, int pos, int n_rot, int interleaved, int d0) {
+    const int half = n_rot / 2;
+    const float2* t = reinterpret_cast<const float2*>(rope) + (size_t)pos * half;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int d = d0 + j;
+        if (d < n_rot && (!interleaved || !(j & 1))) cs[j] = t[interleaved ? d >> 1 : d < half ? d : d - half];
+    }
+}
+// Positions of a row, one per axis; false where one lies outside of the table
+struct RowPos { int at[4]; };
+__device__ __forceinline__ bool row_pos(RowPos& p, const RopeAxes& a, int r, int n_pos) {
+    bool ok = true;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { p.at[k] = k < a.n_axes ? a.pos[(size_t)k * a.pos_ld + r] : 0; ok &= (unsigned)p.at[k] < (unsigned)n_pos; }
+    return ok;
+}
+__device__ __forceinline__ uint32_t axis_word(const RopeAxes& a, int w) {   // selected, not indexed: the words are kernel arguments
+    uint32_t v = a.axes[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v = w == i ? a.axes[i] : v;
+    return v;
+}
+// the same angles where each pair has an axis of its own
+__device__ __forceinline__ void angles(float2 (&cs)[8], const float* rope, const RowPos& p, const RopeAxes& a, int n_rot, int interleaved, int d0) {
+    const int half = n_rot / 2;
+    const float2* t = reinterpret_cast<const float2*>(rope);
+    auto pair_of = [&](int d) { return interleaved ? d >> 1 : d < half ? d : d - half; };
+    const bool run = interleaved || half % 8 == 0;   // the lane's pairs are 4 or 8 neighbours in one word
+    uint32_t w = run ? axis_word(a, pair_of(d0) >> 4) : 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int d = d0 + j, i = pair_of(d);
+        if (d >= n_rot || (interleaved && (j & 1))) continue;
+        if (!run) w = axis_word(a, i >> 4);
+        const uint32_t k = w >> (2 * (i & 15)) & 3u;
+        const int at = k == 0 ? p.at[0] : k == 1 ? p.at[1] : k == 2 ? p.at[2] : p.at[3];
+        cs[j] = t[(size_t)at * half + i];
+    }
+}
 // D / 8 lanes take a head of a row, eight neighbouring elements each, so that a warp has 1, 2 or 4 heads side by side; it takes hpw such sets of neighbouring
 // heads (n_head query heads, then n_kv key heads, then n_kv value heads) in a loop that fetches a set ahead. The row's place and angles are found once. Four prompts of
 // up to 1000 rows of 48 heads of 128: 22.5 us, 73 MB, 95 instructions per head (with a warp per head and the loop unrolled four times 220, which did not fit the instruction cache). Neither issue
 // slots (56 %) nor memory (3.3 TB/s) are used up: the warps, 43 % of what an SM holds, wait for their next set of heads (4.6 of them at a time). One row of 32 heads of 256 3.3 us, latency.
-template <int D, int KIND>
-__global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, int hpw, int* err) {
+// AXES: positions of several axes. 4 bits: four lanes share a group; its range takes four exchanges, the largest range of the head the others.
+template <int D, int KIND, bool AXES>
+__global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, RopeAxes axes, int hpw, int* err) {
     constexpr int LPH = D / 8, HPS = 32 / LPH;   // lanes of a head, heads of a set
     __shared__ __align__(16) float buf[8][32 * 8];
     pdl_launch_dependents();
@@ -103,67 +192,22 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
     if (q.s < 0) return;
     if (h0 < h1) fetch(h0);   // a row of a sequence, and no other, is read
     const int pos = paged_place(q, r);
-    if ((unsigned)pos >= (unsigned)min(b.max_kv, p.n_pos)) { paged_bad(err); return; }
+    RowPos at;
+    if constexpr (AXES) {
+        if (!row_pos(at, axes, r, p.n_pos) || (unsigned)pos >= (unsigned)b.max_kv) { paged_bad(err); return; }
+    } else if ((unsigned)pos >= (unsigned)min(b.max_kv, p.n_pos)) { paged_bad(err); return; }
     const uint32_t page = h1 > p.n_head ? paged_row(pool, q.s, pos >> pool.lg_page, 0, err) : 0u;
-    const int half = p.n_rot / 2;
-    // angles of the lane's elements; interleaved: of its four pairs
     float2 cs[8];
-    const bool turns = d0 < p.n_rot;
-    if (turns) {
-        const float2* t = reinterpret_cast<const float2*>(p.rope) + (size_t)pos * half;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int d = d0 + j;
-            if (d < p.n_rot && (!p.interleaved || !(j & 1))) cs[j] = t[p.interleaved ? d >> 1 : d < half ? d : d - half];
-        }
+    if (d0 < p.n_rot) {
+        if constexpr (AXES) angles(cs, p.rope, at, axes, p.n_rot, p.interleaved, d0);
+        else angles(cs, p.rope, pos, p.n_rot, p.interleaved, d0);
     }
 #pragma unroll 1
     for (int h = h0; h < h1; h += HPS) {
         float x[8] = {next[0].x, next[0].y, next[0].z, next[0].w, next[1].x, next[1].y, next[1].z, next[1].w};
         if (h + HPS < h1) fetch(h + HPS);
         const int kind = h < p.n_head ? 0 : h < p.n_head + pool.n_kv ? 1 : 2, hh = kind == 0 ? h : kind == 1 ? h - p.n_head : h - p.n_head - pool.n_kv;
-        const uint16_t* nw = (const uint16_t*)(kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr);
-        if (nw) {
-            float ss = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
-#pragma unroll
-            for (int off = LPH / 2; off > 0; off >>= 1) ss = ss + __shfl_xor_sync(mask, ss, off);
-            const float inv = 1.0f / sqrtf(ss / (float)D + p.eps);
-            const uint16_t* w = nw + d0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = (x[j] * inv) * bf2f(w[j]);
-        }
-        if (kind < 2 && p.n_rot) {
-            if (p.interleaved) {   // the other one of a pair is the lane's own
-#pragma unroll
-                for (int j = 0; j < 8; j += 2)
-                    if (d0 + j < p.n_rot) {
-                        const float x0 = x[j], x1 = x[j + 1];
-                        x[j] = fmaf(-x1, cs[j].y, x0 * cs[j].x); x[j + 1] = fmaf(x1, cs[j].x, x0 * cs[j].y);
-                    }
-            } else {
-                float* row = buf[warp] + sub * D;
-                __syncwarp(mask);
-                reinterpret_cast<float4*>(row + d0)[0] = make_float4(x[0], x[1], x[2], x[3]); reinterpret_cast<float4*>(row + d0)[1] = make_float4(x[4], x[5], x[6], x[7]);
-                __syncwarp(mask);
-                if (turns) {
-                    if (half % 8 == 0) {   // the lane's elements are all first or all second ones
-                        const float* t = row + (d0 < half ? d0 + half : d0 - half);
-                        const float4 u = reinterpret_cast<const float4*>(t)[0], v = reinterpret_cast<const float4*>(t)[1];
-                        const float o[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w}, sign = d0 < half ? -1.f : 1.f;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x[j] = d0 < half ? fmaf(sign * o[j], cs[j].y, x[j] * cs[j].x) : fmaf(x[j], cs[j].x, o[j] * cs[j].y);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const int d = d0 + j;
-                            if (d < half) x[j] = fmaf(-row[d + half], cs[j].y, x[j] * cs[j].x); else if (d < p.n_rot) x[j] = fmaf(x[j], cs[j].x, row[d - half] * cs[j].y);
-                        }
-                    }
-                }
-            }
-        }
+        turn_head<D>(x, (const uint16_t*)(kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr), kind < 2 ? p.n_rot : 0, p.interleaved, p.eps, cs, d0, mask, buf[warp] + sub * D);
         if (kind == 0) {
             float4* o = reinterpret_cast<float4*>(p.q_out + (size_t)r * p.qo_ld + (size_t)hh * p.qo_hs + d0);
             o[0] = make_float4(x[0], x[1], x[2], x[3]); o[1] = make_float4(x[4], x[5], x[6], x[7]);
@@ -177,21 +221,53 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
         for (int off = LPH / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(mask, m, off));
         if (page == 0xffffffffu) continue;
         const bool finite = m < 0x7f800000u;
-        const float scale = finite ? __fdiv_rn(__uint_as_float(m), KIND == KV_I8 ? 127.f : 448.f) : __uint_as_float(0x7fc00000u);
-        const bool live = finite && scale > 0.f;
-        const float inv = live ? __fdiv_rn(1.f, scale) : 0.f;
-        const size_t at = (size_t)page + ((size_t)hh << pool.lg_page) + (pos & ((1 << pool.lg_page) - 1));
-        uint32_t w[2] = {0u, 0u};
-        if (live) {
-            if (inv < INFINITY) {
+        const size_t at_row = (size_t)page + ((size_t)hh << pool.lg_page) + (pos & ((1 << pool.lg_page) - 1));
+        if constexpr (KIND == KV_I4) {
+            // A group spans lo to hi, zero among them, in 15 steps of scale * u; halves, since hi - lo may pass the largest number. The largest span of the head has u = 15
+            float lo = 0.f, hi = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[j >> 2] |= kv_code<KIND>(x[j] * inv) << (8 * (j & 3));
-            } else {   // a scale below 2^-128 has no reciprocal in 32 bits
-                for (int j = 0; j < 8; ++j) w[j >> 2] |= kv_code<KIND>(__fdiv_rn(x[j], scale)) << (8 * (j & 3));
+            for (int j = 0; j < 8; ++j) { lo = fminf(lo, x[j]); hi = fmaxf(hi, x[j]); }
+#pragma unroll
+            for (int off = 1; off < 4; off <<= 1) { lo = fminf(lo, __shfl_xor_sync(mask, lo, off)); hi = fmaxf(hi, __shfl_xor_sync(mask, hi, off)); }
+            const float span = 0.5f * hi - 0.5f * lo;
+            float most = span;
+#pragma unroll
+            for (int off = LPH / 2; off >= 4; off >>= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, off));
+            const float scale = finite ? __fdiv_rn(most, 112.5f) : __uint_as_float(0x7fc00000u);
+            uint32_t w = 0, group = 0;
+            if (finite && scale > 0.f) {
+                const float f = most > 1e37f ? 0.0625f : 1.f, ratio = fminf(ceilf(__fdiv_rn(15.f * (span * f), most * f)), 15.f);   // u
+                const float step = scale * ratio;
+                if (step > 0.f) {
+                    const float inv = __fdiv_rn(1.f, step);
+                    const bool near = inv < INFINITY;   // a step below 2^-128 has no reciprocal in 32 bits
+                    const float z = fminf(rintf(near ? -lo * inv : __fdiv_rn(-lo, step)), 15.f);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w |= (uint32_t)fminf(fmaxf(rintf(near ? x[j] * inv : __fdiv_rn(x[j], step)) + z, 0.f), 15.f) << (4 * j);
+                    group = (uint32_t)z | (uint32_t)ratio << 4;
+                }
             }
+            const I4Row to = i4_row((uint32_t)at_row, pool.lg_page, D);
+            uint8_t* const base = kind == 1 ? pool.k : pool.v;
+            *reinterpret_cast<uint32_t*>(base + to.codes + d0 / 2) = w;
+            if (d0 % 32 == 0) base[to.groups + d0 / 32] = (uint8_t)group;
+            if (d0 == 0) (kind == 1 ? pool.k_scale : pool.v_scale)[at_row] = scale;
+        } else {
+            const float scale = finite ? __fdiv_rn(__uint_as_float(m), KIND == KV_I8 ? 127.f : 448.f) : __uint_as_float(0x7fc00000u);
+            const bool live = finite && scale > 0.f;
+            const float inv = live ? __fdiv_rn(1.f, scale) : 0.f;
+            uint32_t w[2] = {0u, 0u};
+            if (live) {
+                if (inv < INFINITY) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j >> 2] |= kv_code<KIND>(x[j] * inv) << (8 * (j & 3));
+                } else {   // a scale below 2^-128 has no reciprocal in 32 bits
+                    for (int j = 0; j < 8; ++j) w[j >> 2] |= kv_code<KIND>(__fdiv_rn(x[j], scale)) << (8 * (j & 3));
+                }
+            }
+            *reinterpret_cast<uint2*>((kind == 1 ? pool.k : pool.v) + at_row * D + d0) = make_uint2(w[0], w[1]);
+            if (d0 == 0) (kind == 1 ? pool.k_scale : pool.v_scale)[at_row] = scale;
         }
-        *reinterpret_cast<uint2*>((kind == 1 ? pool.k : pool.v) + at * D + d0) = make_uint2(w[0], w[1]);
-        if (d0 == 0) (kind == 1 ? pool.k_scale : pool.v_scale)[at] = scale;
     }
 }
 
@@ -200,7 +276,7 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
 // tokens are runs of 2 KB), with one piece in flight per thread 88; 4096 tokens of 4 x 256 7.4 us.
 template <int D, int KIND, int RB>
 __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, __half* __restrict__ ko, __half* __restrict__ vo, size_t row_stride, size_t head_stride, int* err) {
-    constexpr int CPR = D / 16, PER = RB / 8;
+    constexpr int PIECE = KIND == KV_I4 ? 32 : 16, CPR = D / PIECE, PER = RB / 8;   // 16 bytes of codes: 4 bits, a group
     __shared__ uint32_t base[RB];   // of head 0
     pdl_launch_dependents();
     pdl_wait();
@@ -224,14 +300,19 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
     __syncthreads();
     const int n = 2 * pool.n_kv * RB * CPR;
     for (int i0 = threadIdx.x; i0 < n; i0 += 4 * 256) {   // four pieces of a thread in flight
-        uint4 w[4]; float sc[4]; uint32_t row[4];
+        uint4 w[4]; float sc[4]; uint32_t row[4], group[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int i = i0 + u * 256, hv = i / (RB * CPR), c = i % CPR;
             row[u] = i < n ? base[i / CPR % RB] : 0xffffffffu;
             if (row[u] != 0xffffffffu) {
                 const size_t at = (size_t)row[u] + ((size_t)(hv >> 1) << pool.lg_page);
-                w[u] = *reinterpret_cast<const uint4*>((hv & 1 ? pool.v : pool.k) + at * D + c * 16);
+                const uint8_t* const from = hv & 1 ? pool.v : pool.k;
+                if constexpr (KIND == KV_I4) {
+                    const I4Row at4 = i4_row((uint32_t)at, pool.lg_page, D);
+                    w[u] = *reinterpret_cast<const uint4*>(from + at4.codes + c * 16);
+                    group[u] = from[at4.groups + c];
+                } else w[u] = *reinterpret_cast<const uint4*>(from + at * D + c * 16);
                 sc[u] = (hv & 1 ? pool.v_scale : pool.k_scale)[at];
             }
         }
@@ -239,34 +320,97 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
         for (int u = 0; u < 4; ++u) {
             if (row[u] == 0xffffffffu) continue;
             const int i = i0 + u * 256, hv = i / (RB * CPR), c = i % CPR;
-            const float s = KIND == KV_I8 ? sc[u] : sc[u] * 256.f;   // code_pair gives e4m3 codes times 2^-8
             const uint32_t ws[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
-            uint32_t o[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t pr = j & 1 ? code_pair<KIND, 2>(ws[j / 2]) : code_pair<KIND, 0>(ws[j / 2]);
+            uint4* dst = reinterpret_cast<uint4*>((hv & 1 ? vo : ko) + (size_t)(r0 + i / CPR % RB) * row_stride + (size_t)(hv >> 1) * head_stride + c * PIECE);
+            auto scaled = [](uint32_t pr, float s) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pr));
-                o[j] = h2_bits(__floats2half2_rn(f.x * s, f.y * s));
+                return h2_bits(__floats2half2_rn(f.x * s, f.y * s));
+            };
+            if constexpr (KIND == KV_I4) {
+                const I4Group g = i4_group(__byte_perm(group[u], 0x64u, 0x4040));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { const uint4 o = i4_word(ws[j], g); dst[j] = make_uint4(scaled(o.x, sc[u]), scaled(o.y, sc[u]), scaled(o.z, sc[u]), scaled(o.w, sc[u])); }
+            } else {
+                const float s = KIND == KV_I8 ? sc[u] : sc[u] * 256.f;   // code_pair gives e4m3 codes times 2^-8
+                uint32_t o[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = scaled(j & 1 ? code_pair<KIND, 2>(ws[j / 2]) : code_pair<KIND, 0>(ws[j / 2]), s);
+                dst[0] = make_uint4(o[0], o[1], o[2], o[3]); dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
             }
-            uint4* dst = reinterpret_cast<uint4*>((hv & 1 ? vo : ko) + (size_t)(r0 + i / CPR % RB) * row_stride + (size_t)(hv >> 1) * head_stride + c * 16);
-            dst[0] = make_uint4(o[0], o[1], o[2], o[3]); dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
         }
     }
 }
 
-template <int D, int KIND> int launch_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, cudaStream_t s) {
-    const int heads = p.n_head + 2 * pool.n_kv;
+// Rows of q, k and v, each head's norm and rotation, to outputs of another type: what k_kv_append does for rows that stay rows. The same lanes, sets of heads and loop.
+template <int D, typename T>
+__global__ void __launch_bounds__(256, 4) k_rope_rows(RopeRowsParams p, RopeAxes axes, int hpw, int* err) {
+    constexpr int LPH = D / 8, HPS = 32 / LPH;
+    __shared__ __align__(16) float buf[8][32 * 8];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPH, d0 = (lane % LPH) * 8, heads = p.heads[0] + p.heads[1] + p.heads[2], parts = (heads + hpw * HPS - 1) / (hpw * HPS);
+    const unsigned mask = LPH == 32 ? 0xffffffffu : ((1u << (LPH & 31)) - 1u) << (sub * LPH);
+    const long long item = (long long)blockIdx.x * 8 + warp;
+    const int r = (int)(item / parts), h0 = (int)(item % parts) * hpw * HPS + sub, h1 = min(heads, h0 - sub + hpw * HPS);
+    if (r >= p.R) return;
+    // which of q, k and v a head belongs to, and its number there
+    auto which = [&](int& h) { int w = 0; if (h >= p.heads[0]) { h -= p.heads[0]; w = 1; if (h >= p.heads[1]) { h -= p.heads[1]; w = 2; } } return w; };
+    float4 next[2];
+    auto fetch = [&](int h) {
+        const int w = which(h);
+        const float* from = (w == 0 ? p.in[0] : w == 1 ? p.in[1] : p.in[2]) + (size_t)r * (w == 0 ? p.in_ld[0] : w == 1 ? p.in_ld[1] : p.in_ld[2]) + (size_t)h * (w == 0 ? p.in_hs[0] : w == 1 ? p.in_hs[1] : p.in_hs[2]) + d0;
+        next[0] = reinterpret_cast<const float4*>(from)[0]; next[1] = reinterpret_cast<const float4*>(from)[1];
+    };
+    if (h0 < h1) fetch(h0);
+    RowPos at;
+    float2 cs[8];
+    if (p.n_rot) {
+        if (!row_pos(at, axes, r, p.n_pos)) { paged_bad(err); return; }   // a row without a place stays as it was
+        if (d0 < p.n_rot) angles(cs, p.rope, at, axes, p.n_rot, p.interleaved, d0);
+    }
+#pragma unroll 1
+    for (int h = h0; h < h1; h += HPS) {
+        float x[8] = {next[0].x, next[0].y, next[0].z, next[0].w, next[1].x, next[1].y, next[1].z, next[1].w};
+        if (h + HPS < h1) fetch(h + HPS);
+        int hh = h;
+        const int w = which(hh);
+        turn_head<D>(x, (const uint16_t*)(w == 0 ? p.norm[0] : w == 1 ? p.norm[1] : nullptr), w < 2 ? p.n_rot : 0, p.interleaved, p.eps, cs, d0, mask, buf[warp] + sub * D);
+        T* to = (T*)(w == 0 ? p.out[0] : w == 1 ? p.out[1] : p.out[2]) + (size_t)r * (w == 0 ? p.out_ld[0] : w == 1 ? p.out_ld[1] : p.out_ld[2]) + (size_t)hh * (w == 0 ? p.out_hs[0] : w == 1 ? p.out_hs[1] : p.out_hs[2]) + d0;
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]); reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (std::is_same<T, __half>::value) o[j] = h2_bits(__floats2half2_rn(x[2 * j], x[2 * j + 1]));
+                else { const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]); o[j] = *reinterpret_cast<const uint32_t*>(&b); }
+            }
+            *reinterpret_cast<uint4*>(to) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+}
+
+// One set of heads per warp while all of them fit on the GPU at once; six beyond. One and six, us: 256 rows of 48 heads of 128 6.7 and 7.9, 512 10.3 and 10.5, 1024 17.5 and 12.0, 4096 63 and 40; of 32
+// heads of 256 512 rows 12.5 and 13.0, 1024 21.9 and 20.8; of 24 heads of 64 1024 rows 6.7 and 8.0, 4096 17.5 and 13.0
+struct Cut { int hpw; unsigned blocks; };
+Cut cut_heads(long long R, int heads, int D) {
+    const int HPS = 32 / (D / 8), hpw = R * heads <= 148 * 64 * HPS ? 1 : 6;
+    return Cut{hpw, (unsigned)((R * ((heads + hpw * HPS - 1) / (hpw * HPS)) + 7) / 8)};
+}
+template <int D, int KIND> int launch_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, const RopeAxes& axes, cudaStream_t s) {
     int* err = device_arg_flag();
-    // One set of heads per warp while all of them fit on the GPU at once; six beyond. One and six, us: 256 rows of 48 heads of 128 6.7 and 7.9, 512 10.3 and 10.5, 1024 17.5 and 12.0, 4096 63 and 40; of 32
-    // heads of 256 512 rows 12.5 and 13.0, 1024 21.9 and 20.8; of 24 heads of 64 1024 rows 6.7 and 8.0, 4096 17.5 and 13.0
-    constexpr int HPS = 32 / (D / 8);
-    const int hpw = (long long)b.R * heads <= 148 * 64 * HPS ? 1 : 6;
-    const long long items = (long long)b.R * ((heads + hpw * HPS - 1) / (hpw * HPS));
-    HP_CUDA(launch_pdl<4>(k_kv_append<D, KIND>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, s, pool, b, p, hpw, err));
+    const Cut c = cut_heads(b.R, p.n_head + 2 * pool.n_kv, D);
+    HP_CUDA(launch_pdl<4>(axes.pos ? k_kv_append<D, KIND, true> : k_kv_append<D, KIND, false>, dim3(c.blocks), dim3(256), 0, s, pool, b, p, axes, c.hpw, err));
     return HP_OK;
 }
-template <int KIND> int launch_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, cudaStream_t s) {
-    return pool.head_dim == 256 ? launch_append<256, KIND>(pool, b, p, s) : pool.head_dim == 128 ? launch_append<128, KIND>(pool, b, p, s) : launch_append<64, KIND>(pool, b, p, s);
+template <int KIND> int launch_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, const RopeAxes& axes, cudaStream_t s) {
+    return pool.head_dim == 256 ? launch_append<256, KIND>(pool, b, p, axes, s) : pool.head_dim == 128 ? launch_append<128, KIND>(pool, b, p, axes, s) : launch_append<64, KIND>(pool, b, p, axes, s);
+}
+template <typename T> int launch_rows(const RopeRowsParams& p, const RopeAxes& axes, cudaStream_t s) {
+    int* err = device_arg_flag();
+    const Cut c = cut_heads(p.R, p.heads[0] + p.heads[1] + p.heads[2], p.head_dim);
+    HP_CUDA(launch_pdl<4>(p.head_dim == 256 ? k_rope_rows<256, T> : p.head_dim == 128 ? k_rope_rows<128, T> : k_rope_rows<64, T>, dim3(c.blocks), dim3(256), 0, s, p, axes, c.hpw, err));
+    return HP_OK;
 }
 
 }  // namespace
@@ -288,8 +432,11 @@ int rope_table(float* table, int n_pos, int n_rot, double base, int scaling, dou
     HP_CUDA(launch_pdl<4>(k_rope_table_sums, dim3((unsigned)((total + groups - 1) / groups)), dim3(1024), (size_t)(ROPE_GROUP + groups) * a.half * 16, s, a, groups));
     return HP_OK;
 }
-int kv_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, cudaStream_t s) {
-    return pool.kind == KV_I8 ? launch_append<KV_I8>(pool, b, p, s) : launch_append<KV_E4M3>(pool, b, p, s);
+int kv_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, const RopeAxes& axes, cudaStream_t s) {
+    return pool.kind == KV_I8 ? launch_append<KV_I8>(pool, b, p, axes, s) : pool.kind == KV_E4M3 ? launch_append<KV_E4M3>(pool, b, p, axes, s) : launch_append<KV_I4>(pool, b, p, axes, s);
+}
+int rope_rows(const RopeRowsParams& p, const RopeAxes& axes, cudaStream_t s) {
+    return p.type == OUT_F32 ? launch_rows<float>(p, axes, s) : p.type == OUT_F16 ? launch_rows<__half>(p, axes, s) : launch_rows<__nv_bfloat16>(p, axes, s);
 }
 int kv_read(const PagedPool& pool, const PagedBatch& b, void* k_out, void* v_out, size_t row_stride, size_t head_stride, cudaStream_t s) {
     // 8 rows per block until there are several blocks for every SM; 32 beyond, where finding the rows bounds a block of 8. Eight and 32, us, 16 caches in pages of 16: 250 tokens each of 1 x 64 2.9 and 3.1, of 4 x 256 7.5
@@ -302,7 +449,7 @@ int kv_read(const PagedPool& pool, const PagedBatch& b, void* k_out, void* v_out
         return pool.head_dim == 256 ? (many ? go(k_kv_read<256, KIND, 32>, 32) : go(k_kv_read<256, KIND, 8>, 8)) : pool.head_dim == 128 ? (many ? go(k_kv_read<128, KIND, 32>, 32) : go(k_kv_read<128, KIND, 8>, 8))
                                                                                                                           : (many ? go(k_kv_read<64, KIND, 32>, 32) : go(k_kv_read<64, KIND, 8>, 8));
     };
-    HP_CUDA(pool.kind == KV_I8 ? type(std::integral_constant<int, KV_I8>()) : type(std::integral_constant<int, KV_E4M3>()));
+    HP_CUDA(pool.kind == KV_I8 ? type(std::integral_constant<int, KV_I8>()) : pool.kind == KV_E4M3 ? type(std::integral_constant<int, KV_E4M3>()) : type(std::integral_constant<int, KV_I4>()));
     return HP_OK;
 }
 

@@ -1,4 +1,4 @@
-// What the operators of the paged 8-bit cache share: the description of a cache and of a ragged batch, and where a row belongs.
+// What the operators of the paged cache share: the description of a cache and of a ragged batch, and where a row belongs.
 #pragma once
 #include "hp_common.cuh"
 #include "kernels.h"
@@ -92,6 +92,33 @@ template <int KIND, int LO> __device__ __forceinline__ uint32_t code_pair(uint32
         const uint32_t h = __byte_perm(w, 0u, LO == 0 ? 0x1404 : 0x3424);
         return (h & 0x80008000u) | ((h >> 1) & 0x3f803f80u);
     }
+}
+// ---- 4 bits. A head of a token in groups of 32 dims: codes c of 4 bits, and a byte of a group: the code z of zero in its low half, a factor u of 0 to 15 in the high
+// one. A value is the token's scale times u * (c - z), a whole number of at most 225, exact in f16. A page of a head holds the codes of its tokens, head_dim / 2 bytes
+// each (the even dim in the low half of a byte), then the bytes of the groups, head_dim / 32 each.
+struct I4Row { size_t codes, groups; };   // where a row of the pool (paged_row and its place in the page) lies
+__device__ __forceinline__ I4Row i4_row(uint32_t row, int lg, int D) {
+    const uint32_t in = row & ((1u << lg) - 1);
+    const size_t page = (size_t)(row - in) * (size_t)(17 * D / 32);
+    return I4Row{page + in * (uint32_t)(D / 2), page + ((size_t)(D / 2) << lg) + in * (uint32_t)(D / 32)};
+}
+// A group's byte, or those of two tokens, as two f16: 1024 + z, u, -(64 + z) u; all exact. `two`: 0x6400 + byte in both halves
+struct I4Group { __half2 z, u, n; };
+__device__ __forceinline__ __half2 bits_h2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
+__device__ __forceinline__ I4Group i4_group(uint32_t two) {
+    I4Group g;
+    g.z = bits_h2((two & 0x000f000fu) | 0x64006400u);
+    g.u = __hsub2(bits_h2((two & 0x00f000f0u) | 0x54005400u), __floats2half2_rn(64.f, 64.f));
+    g.n = __hmul2(__hsub2(__floats2half2_rn(960.f, 960.f), g.z), g.u);
+    return g;
+}
+// Codes at bits 0 to 3 of both halves of w, at bits 4 to 7: as low bits of 1024 + c the difference and the product are exact, as bits 4 to 7 of 64 + c a single fma is: (64 + c) u is below 2048
+__device__ __forceinline__ uint32_t i4_low(uint32_t w, const I4Group& g) { return h2_bits(__hmul2(__hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), g.z), g.u)); }
+__device__ __forceinline__ uint32_t i4_high(uint32_t w, const I4Group& g) { return h2_bits(__hfma2(bits_h2((w & 0x00f000f0u) | 0x54005400u), g.u, g.n)); }
+// the 8 dims of a word in order
+__device__ __forceinline__ uint4 i4_word(uint32_t w, const I4Group& g) {
+    const uint32_t a = i4_low(w, g), b = i4_high(w, g), c = i4_low(w >> 8, g), d = i4_high(w >> 8, g);   // dims (0, 4), (1, 5), (2, 6), (3, 7)
+    return make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632));
 }
 // The block of pairs that blockIdx.z stands for: sequences in order, each with ceil(T * G / MB) blocks.
 struct Block { PagedSeq q; int p0, np; };

@@ -5,7 +5,7 @@ import functools
 
 import torch
 
-from ._lib import HipsterError, lib, hot, tensors, check, ptr
+from ._lib import HipsterError, lib, hot, more, tensors, check, ptr
 
 # The calls below are a few microseconds of device work, so what they spend in Python counts: the handle of the current stream
 # comes without a Stream object around it, the short calls go through native entry points that take addresses as integers (_lib.hot; to
@@ -178,22 +178,38 @@ def _refuse(ok, what):
 
 
 class KVPages:
-    """A pool of pages: k, v [n_pages][n_kv][page_size][head_dim] in int8 or float8_e4m3fn, k_scale, v_scale f32 [n_pages][n_kv][page_size] (one scale per
+    """A pool of pages: k, v [n_pages][n_kv][page_size][head_dim] in int8 or float8_e4m3fn, or 4 bits as uint8 [n_pages][n_kv][page_size * 17 * head_dim / 32] (of a page and head the
+    codes of its tokens, head_dim / 2 bytes each, then their groups' bytes, head_dim / 32 each: hipster_b200.h), with k_scale, v_scale f32 [n_pages][n_kv][page_size] (one scale per
     token and head). The tensors are kept, not copied; KVPages.empty() allocates them."""
 
     def __init__(self, k, v, k_scale, v_scale):
-        _refuse(k.dim() == 4 and k.dtype in (torch.int8, torch.float8_e4m3fn), "KVPages: k must be [n_pages][n_kv][page_size][head_dim] in int8 or float8_e4m3fn")
+        four = k.dim() == 3 and k.dtype == torch.uint8
+        _refuse(four or k.dim() == 4 and k.dtype in (torch.int8, torch.float8_e4m3fn),
+                "KVPages: k must be [n_pages][n_kv][page_size][head_dim] in int8 or float8_e4m3fn, or uint8 [n_pages][n_kv][page_size * 17 * head_dim / 32]")
         _refuse(v.dtype == k.dtype and v.shape == k.shape, "KVPages: k and v must be alike")
-        _refuse(all(t.dtype == torch.float32 and t.shape == k.shape[:3] for t in (k_scale, v_scale)), "KVPages: scales must be f32 [n_pages][n_kv][page_size]")
+        _refuse(all(t.dtype == torch.float32 and t.dim() == 3 and t.shape[:2] == k.shape[:2] and (four or t.shape == k.shape[:3]) for t in (k_scale, v_scale)) and k_scale.shape == v_scale.shape,
+                "KVPages: scales must be f32 [n_pages][n_kv][page_size]")
         _refuse(all(t.is_contiguous() and t.device == k.device for t in (k, v, k_scale, v_scale)), "KVPages: contiguous tensors of one device")
+        if four:
+            page = k_scale.shape[2]
+            head_dim, rest = divmod(32 * k.shape[2], 17 * page) if page else (0, 1)
+            _refuse(rest == 0 and head_dim in (64, 128, 256), "KVPages: 4 bits take page_size * 17 * head_dim / 32 bytes per page and head, with a head_dim of 64, 128 or 256")
+            shape = (*k_scale.shape, head_dim)
+        else:
+            shape = tuple(k.shape)
         self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
-        self.n_pages, self.n_kv, self.page_size, self.head_dim = k.shape
-        self._c = _Pages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), int(k.dtype != torch.int8), *k.shape)
+        self.n_pages, self.n_kv, self.page_size, self.head_dim = shape
+        self._c = _Pages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), 4 if four else int(k.dtype != torch.int8), *shape)
         self._at, self._dev, self._f16 = ctypes.addressof(self._c), k.get_device(), torch.empty(0, dtype=_F16, device=k.device)
 
     @classmethod
     def empty(cls, n_pages, n_kv, page_size, head_dim, dtype=torch.int8, device="cuda"):
-        codes = [torch.zeros((n_pages, n_kv, page_size, head_dim), dtype=torch.uint8, device=device).view(dtype) for _ in range(2)]
+        """dtype: torch.int8, torch.float8_e4m3fn, or "i4" for 4 bits."""
+        if dtype == "i4":
+            _refuse(head_dim in (64, 128, 256), "KVPages: 4 bits go with a head_dim of 64, 128 or 256")
+            codes = [torch.zeros((n_pages, n_kv, page_size * 17 * head_dim // 32), dtype=torch.uint8, device=device) for _ in range(2)]
+        else:
+            codes = [torch.zeros((n_pages, n_kv, page_size, head_dim), dtype=torch.uint8, device=device).view(dtype) for _ in range(2)]
         return cls(*codes, *(torch.zeros((n_pages, n_kv, page_size), dtype=torch.float32, device=device) for _ in range(2)))
 
 
@@ -259,20 +275,104 @@ def rope_table(n_pos, n_rot, base, scaling=None, factor=1.0, orig_ctx=0, beta_fa
 
 
 def _norm_weight(w, pages):
+    return _norm_weight_on(w, pages.head_dim, pages._dev)
+
+
+def _norm_weight_on(w, head_dim, dev):
     if w is None:
         return None
-    if not (w.dtype in (torch.bfloat16, torch.int16) and w.shape == (pages.head_dim,) and w.is_contiguous() and w.get_device() == pages._dev):
+    if not (w.dtype in (torch.bfloat16, torch.int16) and w.shape == (head_dim,) and w.is_contiguous() and w.get_device() == dev):
         raise HipsterError(1, "norm weights are bf16 [head_dim]")
     return w.data_ptr()
 
 
-def kv_append(pages, k, v, table, row_start, kv_len, rope=None, q=None, q_out=None, interleaved=False, q_norm=None, k_norm=None, eps=1e-6):
-    """Appends rows k, v f32 [R][n_kv][head_dim] of a ragged batch to their sequences' pages, k normalised (k_norm bf16 [head_dim]) and rotated by rope
-    f32 [n_pos][n_rot / 2][2]. q [R][n_head][head_dim] is normalised and rotated alike. -> q_out (f32 [R][n_head][head_dim]; None without q).
-    Rows row_start[s] .. row_start[s + 1] - 1 are the newest of the kv_len[s] tokens of sequence s."""
+def rope_axes(sections, n_rot=None, interleaved=False):
+    """The axis of each rotated pair of dims, as kv_append and rope_rows take it: sections[a] pairs for axis a, one axis after the other; interleaved: the axes in turn (pair i to axis i mod n)
+    until an axis has its pairs, and what is left over to axis 0. n_rot: the dims that are rotated (2 * sum(sections))."""
+    n, half = len(sections), sum(sections)
+    if not (1 <= n <= 4 and min(sections) >= 0 and half and (n_rot is None or n_rot == 2 * half)):
+        raise HipsterError(1, "rope_axes: 1 to 4 sections, which add up to half of the rotated dims")
+    if not interleaved:
+        return bytes(a for a, m in enumerate(sections) for _ in range(m))
+    return bytes(i % n if i < n * sections[i % n] else 0 for i in range(half))
+
+
+def _rope_args(who, rope, positions, axes, R, dev):
+    """-> table, n_pos, n_rot, and after `interleaved`: positions, their row stride, axes, number of axes."""
+    if rope is None:
+        if positions is not None or axes is not None:
+            raise HipsterError(1, f"{who}: positions and axes go with a rope table")
+        return (None, 0, 0), (None, 0, None, 0)
+    n_pos, half, two = rope.shape
+    if not (rope.dtype is _F32 and two == 2 and rope.is_contiguous() and rope.get_device() == dev):
+        raise HipsterError(1, f"{who}: rope must be f32 [n_pos][n_rot / 2][2]")
+    if positions.dim() == 1:
+        positions = positions[None]
+    (n_axes, cols), (ld, one) = positions.shape, positions.stride()
+    if not (positions.dtype is _I32 and cols == R and (one == 1 or R == 1) and (n_axes == 1 or ld >= 0) and positions.get_device() == dev):
+        raise HipsterError(1, f"{who}: positions must be int32 [axes][{R}], rows without gaps, on the device of the rows")
+    if axes is None:
+        if n_axes != 1:
+            raise HipsterError(1, f"{who}: positions of several axes go with the axis of each pair (rope_axes)")
+        axes = bytes(half)
+    try:
+        if type(axes) is not bytes:
+            axes = bytes(axes)
+    except (ValueError, TypeError):
+        raise HipsterError(1, f"{who}: axes are whole numbers below the number of axes, one per rotated pair of dims") from None
+    if len(axes) != half:
+        raise HipsterError(1, f"{who}: {half} rotated pairs of dims, and {len(axes)} axes")
+    return (rope.data_ptr(), n_pos, 2 * half), (positions.data_ptr(), ld if n_axes > 1 else 0, axes, n_axes)
+
+
+_OUT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def rope_rows(q=None, k=None, v=None, rope=None, positions=None, axes=None, interleaved=False, q_norm=None, k_norm=None, eps=1e-6, dtype=torch.float16):
+    """Rows of a prompt, f32 q [R][n_head][head_dim], k and v [R][n_kv][head_dim] (each may be None), as attn_prompt takes them: per head RMSNorm of q and k (q_norm, k_norm bf16 [head_dim], or None),
+    rotation by rope f32 [n_pos][n_rot / 2][2] at positions int32 [axes][R] (or [R]), the axis of each pair in axes (rope_axes), rounded to dtype (float16, bfloat16, float32). -> q, k, v"""
+    given = [t for t in (q, k, v) if t is not None]
+    if not given or dtype not in _OUT or any(t.dim() != 3 for t in given):
+        raise HipsterError(1, "rope_rows: q, k and v are [R][heads][head_dim]; outputs are float16, bfloat16 or float32")
     fast = tensors()
     if fast:
-        out = fast.kv_append(pages._at, pages._dev, k, v, table, row_start, kv_len, rope, q, q_out, interleaved, q_norm, k_norm, eps)
+        out = fast.rope_rows(q, k, v, rope, positions, axes, interleaved, q_norm, k_norm, eps, _OUT[dtype])
+        if out is not None:
+            return out
+    R, _, D = given[0].shape
+    dev = given[0].get_device()
+    if dev != _device():
+        raise HipsterError(1, f"rope_rows: the rows are on device {dev}, and device {_device()} is current")
+    if k is not None and v is not None and k.shape[1] != v.shape[1]:
+        raise HipsterError(1, "rope_rows: k and v have as many heads")
+    if rope is not None and positions is None:
+        raise HipsterError(1, "rope_rows: a rope table goes with positions")
+    rows, out = [], []
+    for t in (q, k, v):
+        if t is None:
+            rows.append((None, 0, 0, None, 0, 0))
+            out.append(None)
+            continue
+        ld, hs, one = t.stride()
+        if not (t.dtype is _F32 and t.shape[0] == R and t.shape[2] == D and one == 1 and t.get_device() == dev):
+            raise HipsterError(1, f"rope_rows: rows are f32 [{R}][heads][{D}] on one device")
+        o = t.new_empty(t.shape, dtype=dtype)
+        rows.append((t.data_ptr(), ld, hs, o.data_ptr(), t.shape[1] * D, D))
+        out.append(o)
+    table, pos = _rope_args("rope_rows", rope, positions, axes, R, dev)
+    n_head, n_kv = 0 if q is None else q.shape[1], k.shape[1] if k is not None else 0 if v is None else v.shape[1]
+    check(more().hp_rope_rows(*rows[0], n_head, *rows[1], *rows[2], n_kv, D, _OUT[dtype], _norm_weight_on(q_norm, D, dev), _norm_weight_on(k_norm, D, dev), *table, int(interleaved), *pos, R, eps, _raw_stream(dev)))
+    return tuple(out)
+
+
+def kv_append(pages, k, v, table, row_start, kv_len, rope=None, q=None, q_out=None, interleaved=False, q_norm=None, k_norm=None, eps=1e-6, positions=None, axes=None):
+    """Appends rows k, v f32 [R][n_kv][head_dim] of a ragged batch to their sequences' pages, k normalised (k_norm bf16 [head_dim]) and rotated by rope
+    f32 [n_pos][n_rot / 2][2]. q [R][n_head][head_dim] is normalised and rotated alike. -> q_out (f32 [R][n_head][head_dim]; None without q).
+    Rows row_start[s] .. row_start[s + 1] - 1 are the newest of the kv_len[s] tokens of sequence s. They are rotated by their places in the cache, or by positions int32 [axes][R] (or [R])
+    with the axis of each pair in axes (rope_axes)."""
+    fast = tensors()
+    if fast:
+        out = fast.kv_append(pages._at, pages._dev, k, v, table, row_start, kv_len, rope, q, q_out, interleaved, q_norm, k_norm, eps, positions, axes)
         if out is not None:
             return None if out is True else out
     S, c, *at = _batch(pages, table, row_start, kv_len)
@@ -285,14 +385,20 @@ def kv_append(pages, k, v, table, row_start, kv_len, rope=None, q=None, q_out=No
         if q_out is None:
             q_out = q.new_empty((R, n_head, pages.head_dim))
         qo = _rows(q_out, pages, R, n_head, "q_out")
+    rows = (*qr, *qo, n_head, *_rows(k, pages, R, n_kv, "k"), *_rows(v, pages, R, n_kv, "v"), _norm_weight(q_norm, pages), _norm_weight(k_norm, pages))
+    if positions is not None or axes is not None:
+        if rope is None or positions is None:
+            raise HipsterError(1, "kv_append: positions and axes go with a rope table")
+        turn, pos = _rope_args("kv_append", rope, positions, axes, R, pages._dev)
+        check(more().hp_kv_append_axes(*rows, *turn, int(interleaved), *pos, *at, S, R, ctypes.addressof(c), eps, _raw_stream(pages._dev)))
+        return q_out
     if rope is not None:
         n_pos, n_rot, two = rope.shape
         n_rot *= 2
         if not (rope.dtype is _F32 and two == 2 and rope.is_contiguous() and rope.get_device() == pages._dev):
             raise HipsterError(1, "kv_append: rope must be f32 [n_pos][n_rot / 2][2]")
         rope = rope.data_ptr()
-    check(hot().hp_kv_append(*qr, *qo, n_head, *_rows(k, pages, R, n_kv, "k"), *_rows(v, pages, R, n_kv, "v"), _norm_weight(q_norm, pages), _norm_weight(k_norm, pages), rope, n_pos, n_rot, int(interleaved),
-                             *at, S, R, ctypes.addressof(c), eps, _raw_stream(pages._dev)))
+    check(hot().hp_kv_append(*rows, rope, n_pos, n_rot, int(interleaved), *at, S, R, ctypes.addressof(c), eps, _raw_stream(pages._dev)))
     return q_out
 
 
@@ -349,4 +455,36 @@ def attn_paged(q, pages, table, row_start, kv_len, max_rows, max_kv, scale=None,
     xq = XQ8(R, n_head * D, pages.device) if want_q8 else None
     check(hot().hp_attn_paged(*qr, *gr, n_head, *at, S, R, max_rows, max_kv, ctypes.addressof(c), D ** -0.5 if scale is None else scale, window, n_sink, None if out is None else out.data_ptr(),
                               xq.q.data_ptr() if xq else None, xq.sc.data_ptr() if xq else None, ws.data_ptr(), _raw_stream(pages._dev)))
+    return out, xq
+
+
+def attn_prompt(q, k, v, row_start, max_rows, scale=None, gate=None, want_out=True, want_q8=False):
+    """Causal attention of whole prompts, packed: rows row_start[s] .. row_start[s + 1] - 1 of q [R][n_head][head_dim], k and v [R][n_kv][head_dim] (all float16, or all bfloat16; any strides of rows and
+    heads) are prompt s. Times sigmoid(gate) where a gate f32 [R][n_head][head_dim] is given. scale: 1 / sqrt(head_dim). max_rows bounds a prompt's rows.
+    -> (out [R][n_head][head_dim] of q's type or None, XQ8 of its rows or None)"""
+    fast = want_out and not want_q8 and tensors()
+    if fast:
+        out = fast.attn_prompt(q, k, v, row_start, max_rows, scale, gate)
+        if out is not None:
+            return out, None
+    if q.dim() != 3 or k.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16):
+        raise HipsterError(1, "attn_prompt: q, k and v are [R][heads][head_dim] in float16 or bfloat16")
+    (R, n_head, D), n_kv, dev = q.shape, k.shape[1], q.get_device()
+    _ints("attn_prompt: max_rows", max_rows)
+    if dev != _device():
+        raise HipsterError(1, f"attn_prompt: the rows are on device {dev}, and device {_device()} is current")
+    for t, heads, what in ((q, n_head, "q"), (k, n_kv, "k"), (v, n_kv, "v")):
+        if not (t.dtype is q.dtype and t.shape == (R, heads, D) and t.stride(2) == 1 and t.get_device() == dev):
+            raise HipsterError(1, f"attn_prompt: {what} must be {q.dtype} [{R}][{heads}][{D}] on the device of q")
+    if not (row_start.dtype is _I32 and row_start.dim() == 1 and row_start.is_contiguous() and row_start.get_device() == dev):
+        raise HipsterError(1, "attn_prompt: row_start must be int32 [S + 1], contiguous, on the device of the rows")
+    gr = (None, 0, 0)
+    if gate is not None:
+        if not (gate.dtype is _F32 and gate.shape == q.shape and gate.stride(2) == 1 and gate.get_device() == dev):
+            raise HipsterError(1, f"attn_prompt: gate must be f32 [{R}][{n_head}][{D}] on the device of q")
+        gr = (gate.data_ptr(), *gate.stride()[:2])
+    out = q.new_empty((R, n_head, D)) if want_out else None
+    xq = XQ8(R, n_head * D, q.device) if want_q8 else None
+    check(more().hp_attn_prompt(q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], _OUT[q.dtype], *gr, n_head, n_kv, D, row_start.data_ptr(), row_start.numel() - 1, R, max_rows,
+                                D ** -0.5 if scale is None else scale, None if out is None else out.data_ptr(), xq.q.data_ptr() if xq else None, xq.sc.data_ptr() if xq else None, _raw_stream(dev)))
     return out, xq

@@ -122,11 +122,15 @@ int hp_moe_layer(const float* xn_dev, const void* xq_q_dev, const void* xq_sc_de
                  const void* sh_gate_up_tiled_dev, const void* sh_down_tiled_dev, int T, int E, int F, int n_expert, int k, int* ids_dev, float* weights_dev, float* y_dev,
                  void* workspace_dev, void* stream);
 
-/* ------------------------------------------------------------------ a paged cache in 8 bits, for ragged batches
+/* ------------------------------------------------------------------ a paged cache in 8 or 4 bits, for ragged batches
  * No counterpart in the reference, whose caches are f16 and contiguous. Tokens of many sequences share a pool of pages; k and v are held as
  * int8 or e4m3 codes with one f32 scale per token and head (int8: largest magnitude / 127, e4m3: / 448), so that a token that a verify pass wrote
  * and that is overwritten later leaves no trace in its neighbours. A token with an infinite or NaN element gets a NaN scale over codes of
  * zero: rows that see it become NaN, others do not. e4m3 codes 0x7f and 0xff are never written and read as 480 and -480.
+ * HP_KV_I4 holds 4 bits: per group of 32 dims a code z of zero and a factor u, per token and head a scale; the value of a code c is scale * (u * (c - z)). With lo = min(0, x) and hi =
+ * max(0, x) over a group, scale = (largest hi - lo of the head) / 225, u = ceil(15 (hi - lo) / largest) (0: all of the group is zero), z = round(-lo / (scale u)), c = round(x / (scale u)) + z in 0 .. 15: zero is
+ * always held exactly, other elements to a step scale * u, half of it but at the ends of a group's range. k, v: [n_pages][n_kv][page_size * 17 * head_dim / 32] bytes: of a page and head first the codes of its tokens,
+ * head_dim / 2 bytes each with the even dim in the low half, then their groups' bytes z + 16 u, head_dim / 32 each. 4.5 bits per element at 64 dims, 4.375 at 128, 4.3125 at 256, scales included (4.75, 4.5, 4.375).
  *
  * hp_kv_pages describes a cache (host struct, read during the call). k, v: [n_pages][n_kv][page_size][head_dim] bytes, 16-byte aligned; k_scale, v_scale: f32
  * [n_pages][n_kv][page_size]. page_size: a power of two, 16 to 1024; head_dim: 64, 128 or 256.
@@ -139,7 +143,7 @@ int hp_moe_layer(const float* xn_dev, const void* xq_q_dev, const void* xq_sc_de
  * sequence meaningless (attention), and hp_device_status returns HP_EINVAL. Rows of negative position are not appended, read back or
  * normalised (HP_EINVAL), and attend to nothing. Row strides (ld) and head strides (hs) are in elements; those of outputs are nested, rows in heads or heads in
  * rows (HP_EINVAL where they lie over each other). */
-enum { HP_KV_I8 = 0, HP_KV_E4M3 = 1 };
+enum { HP_KV_I8 = 0, HP_KV_E4M3 = 1, HP_KV_I4 = 4 };
 typedef struct hp_kv_pages {
     void* k; void* v; float* k_scale; float* v_scale;
     int type, n_pages, n_kv, page_size, head_dim;
@@ -159,6 +163,20 @@ int hp_rope_table(float* table_dev, int n_pos, int n_rot, double base, int scali
 int hp_kv_append(const float* q_dev, long long q_ld, long long q_hs, float* q_out_dev, long long qo_ld, long long qo_hs, int n_head, const float* k_dev, long long k_ld, long long k_hs,
                  const float* v_dev, long long v_ld, long long v_hs, const void* q_norm_bf16_dev, const void* k_norm_bf16_dev, const float* rope_dev, int n_pos, int n_rot, int interleaved,
                  const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, float eps, void* stream);
+/* hp_kv_append with rotary positions of their own, of 1 to 4 axes (time, height and width of an image's patches, say): pos_dev int [n_axes][R], rows pos_ld apart, holds each row's position on each
+ * axis; axes_host [n_rot / 2] (read during the call) tells the axis whose position turns each pair of dims. Positions lie in [0, n_pos), all n_axes of a row: a row with another one is left out, and
+ * hp_device_status returns HP_EINVAL. Where a token is kept goes by kv_len as before. n_rot at least 2; R here counts the columns of pos_dev. */
+int hp_kv_append_axes(const float* q_dev, long long q_ld, long long q_hs, float* q_out_dev, long long qo_ld, long long qo_hs, int n_head, const float* k_dev, long long k_ld, long long k_hs,
+                      const float* v_dev, long long v_ld, long long v_hs, const void* q_norm_bf16_dev, const void* k_norm_bf16_dev, const float* rope_dev, int n_pos, int n_rot, int interleaved,
+                      const int* pos_dev, long long pos_ld, const unsigned char* axes_host, int n_axes,
+                      const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, float eps, void* stream);
+/* The same norm and rotation for rows that stay rows, of q [R][n_head][head_dim], k and v [R][n_kv][head_dim] f32, v as it is, rounded to out_type: what hp_attn_prompt takes. q_dev, or k_dev, or v_dev may be NULL
+ * with its output: none. n_rot = 0: no rotation (rope_dev, pos_dev, axes_host NULL, n_axes 0). A row with a position outside of the table is not written (HP_EINVAL from hp_device_status). An output may be
+ * its input with the same strides where both are f32. Pointers 16-byte aligned, strides multiples of 16 bytes; outputs' rows do not lie over each other. */
+enum { HP_F32 = 0, HP_F16 = 1, HP_BF16 = 2 };
+int hp_rope_rows(const float* q_dev, long long q_ld, long long q_hs, void* q_out_dev, long long qo_ld, long long qo_hs, int n_head, const float* k_dev, long long k_ld, long long k_hs, void* k_out_dev, long long ko_ld, long long ko_hs,
+                 const float* v_dev, long long v_ld, long long v_hs, void* v_out_dev, long long vo_ld, long long vo_hs, int n_kv, int head_dim, int out_type, const void* q_norm_bf16_dev, const void* k_norm_bf16_dev,
+                 const float* rope_dev, int n_pos, int n_rot, int interleaved, const int* pos_dev, long long pos_ld, const unsigned char* axes_host, int n_axes, int R, float eps, void* stream);
 /* The tokens of the rows back as f16 (code * scale, rounded once): k_out / v_out + r * row_stride + head * head_stride hold head_dim values each. With kv_len[s] rows a
  * whole sequence; row_stride = head_dim and head_stride = max_ctx * head_dim give the cache of hp_attn_decode. Strides multiples of 8. */
 int hp_kv_read(const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, void* k_out_f16_dev, void* v_out_f16_dev, long long row_stride, long long head_stride, void* stream);
@@ -174,6 +192,15 @@ int hp_kv_read(const int* table_dev, int table_ld, const int* row_start_dev, con
 size_t hp_attn_paged_workspace_bytes(int table_ld, int S, int R, int max_rows, int max_kv, int n_head, int window, int n_sink, const hp_kv_pages* pages);
 int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const float* gate_dev, long long g_ld, long long g_hs, int n_head, const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev,
                   int S, int R, int max_rows, int max_kv, const hp_kv_pages* pages, float scale, int window, int n_sink, float* out_dev, void* xq_q_dev, void* xq_sc_dev, void* workspace_dev, void* stream);
+
+/* Causal attention of whole prompts, packed: rows [row_start[s], row_start[s + 1]) of q [R][n_head][head_dim], k and v [R][n_kv][head_dim] are prompt s, whose row i sees the keys of its rows 0 .. i: softmax(scale * q k^T) v,
+ * sums in fp32, weights rounded to the inputs' type, times sigmoid(gate) (gate_dev f32 [R][n_head][head_dim], nullable). type: HP_F16 or HP_BF16, of q, k, v and out [R][n_head * head_dim]; and / or the int8 quantisation of the
+ * outputs before they are rounded (K = n_head * head_dim, buffers as hp_attn_paged has them); either may be NULL. head_dim 64, 128 or 256; n_head a multiple of n_kv. max_rows bounds a prompt's rows and sizes the launch. row_start
+ * (S + 1 ints, rising) is device memory, read when the kernel runs; rows behind row_start[S] are not written. What does not fit is left out and told by hp_device_status, as for the paged calls.
+ * A row is not touched by infinite or NaN keys and values that it does not see; of a value that it sees, an infinite element makes the output's infinite or NaN.
+ * q, k, v: 16-byte aligned, strides positive multiples of 8; gate 16-byte aligned, strides multiples of 4; out and quantised outputs 16-byte aligned. No workspace. A row's result depends on its own prompt alone. */
+int hp_attn_prompt(const void* q_dev, long long q_ld, long long q_hs, const void* k_dev, long long k_ld, long long k_hs, const void* v_dev, long long v_ld, long long v_hs, int type, const float* gate_dev, long long g_ld, long long g_hs,
+                   int n_head, int n_kv, int head_dim, const int* row_start_dev, int S, int R, int max_rows, float scale, void* out_dev, void* xq_q_dev, void* xq_sc_dev, void* stream);
 
 /* ------------------------------------------------------------------ engine level (engine/src/qwen35.h, qwen4exp.h) */
 
