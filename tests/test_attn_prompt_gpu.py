@@ -1,0 +1,382 @@
+"""Causal attention of packed prompts in 16 bits (hp_attn_prompt) on the GPU against a plain implementation in 64 bits, and a run of the prompt's and the cache's calls together."""
+import math
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+import hipster_b200 as hb
+from hipster_b200 import kernels as K_
+import test_paged_gpu as P
+
+pytestmark = pytest.mark.gpu
+
+gen, status, form = P.gen, P.status, P.form
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def starts(rows):
+    return i32([sum(rows[:s]) for s in range(len(rows) + 1)])
+
+
+def prompt64(q, k, v, rows, scale, gate=None):
+    """-> values and tolerances of every output, in 64 bits.
+
+    h: half a step of the inputs' type. The output is rounded once (h of it, at most h sum p |v|), each weight once (h of it: together h sum p |v|), below f16's smallest normal to steps of 2^-24, where the largest
+    weight is 1 or more, as is their sum (2^-25 sum |v|; bf16 has no such steps). A score is the sum of D products, formed 16 at a time: D / 16 additions and a rounding of each 16, each a step 2^-23 of at most A = scale sum |q k|,
+    and the factor's three roundings: ds <= (D / 8 + 4) 2^-23 A, and moves the result by at most 2 ds sum p |v|. Reference, exponential (2^-22) and the sums (keys / 16 steps on the tensor pipe; 2^-24 times 64 + keys / 128 for the
+    weights), the rescaling of a row at most once per tile on both sides of the quotient, and 8 for quotient and gate."""
+    R, H, D = q.shape
+    G = H // k.shape[1]
+    h = torch.finfo(q.dtype).eps / 2
+    out, tol = (torch.zeros((R, H, D), dtype=torch.float64, device="cuda") for _ in range(2))
+    r0 = 0
+    for T in filter(None, rows):
+        hidden = torch.ones((T, T), dtype=torch.bool, device="cuda").triu(1)
+        for i in range(H):
+            x, y, z = q[r0:r0 + T, i].double(), k[r0:r0 + T, i // G].double(), v[r0:r0 + T, i // G].double()
+            p = torch.softmax((x @ y.T * scale).masked_fill(hidden, -math.inf), -1)
+            A = (x.abs() @ y.abs().T * scale).masked_fill(hidden, 0).amax(-1, keepdim=True)
+            mag = p @ z.abs()
+            n = torch.arange(1, T + 1, device="cuda", dtype=torch.float64)[:, None]
+            out[r0:r0 + T, i] = p @ z
+            tol[r0:r0 + T, i] = mag * (2 * h + (2 * (D / 8 + 4) * A + n / 16 + 2 * n / 128 + 64 + 16) * 2.0 ** -23) + (2.0 ** -25 * (z.abs().cumsum(0) + 1) if q.dtype == torch.float16 else 0)
+        r0 += T
+    if gate is not None:
+        g = torch.sigmoid(gate.double())
+        out, tol = out * g, tol * g
+        if q.dtype == torch.float16:
+            tol += 2.0 ** -25
+    return out, tol
+
+
+def make(rows, H, n_kv, D, kind, seed=0, tail=0, packed=True, up=1.0):
+    R = sum(rows) + tail
+    x = torch.randn((R, H + 2 * n_kv, D), generator=gen(seed), device="cuda") * torch.exp(0.5 * torch.randn((R, H + 2 * n_kv, 1), generator=gen(seed + 1), device="cuda"))
+    x[:, :H] *= up
+    x = x.to(TYPES[kind])
+    q, k, v = x.split([H, n_kv, n_kv], 1)
+    return (q, k, v) if packed else (q.contiguous(), k.contiguous(), v.contiguous())
+
+
+def check(rows, H, n_kv, D, kind, gate=False, seed=0, tail=0, packed=True, up=1.0, scale=None, max_rows=None):
+    q, k, v = make(rows, H, n_kv, D, kind, seed, tail, packed, up)
+    R = sum(rows)
+    g = torch.randn((R + tail, H, D + 4), generator=gen(seed + 2), device="cuda")[..., :D] if gate else None
+    got, none = K_.attn_prompt(q, k, v, starts(rows), max_rows=max_rows or max(max(rows), 1), gate=g, scale=scale)
+    assert status() == 0 and none is None and got.dtype == q.dtype
+    want, tol = prompt64(q[:R], k[:R], v[:R], rows, D ** -0.5 if scale is None else scale, None if g is None else g[:R])
+    bad = ~((got[:R].double() - want).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), float(((got[:R].double() - want).abs() / tol).max()))
+    return q, k, v, got
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows", [[1], [2], [127], [128], [129], [255, 1, 0, 257], [300, 64, 33], [1] * 40, [700]])
+def test_shapes(kind, D, rows):
+    check(rows, 6, 2, D, kind, gate=len(rows) == 1)
+
+
+@pytest.mark.parametrize("H,n_kv", [(1, 1), (5, 5), (17, 1), (24, 4), (32, 8), (70, 2)])
+@pytest.mark.parametrize("D", [64, 256])
+def test_heads(H, n_kv, D):
+    check([140, 3], H, n_kv, D, "bf16")
+    check([5], H, n_kv, D, "f16", packed=False)
+
+
+@pytest.mark.parametrize("D,kind", [(64, "f16"), (128, "bf16"), (256, "f16"), (256, "bf16")])
+def test_long_prompts(D, kind):
+    check([2500, 1111], 2, 1, D, kind)
+    check([5001], 1, 1, D, kind, gate=True, packed=False)
+
+
+def test_many_prompts_in_any_order():
+    rows = [(37 * i) % 300 for i in range(150)]   # more than a warp has lanes; empty ones
+    check(rows, 2, 1, 64, "f16")
+    check(sorted(rows), 1, 1, 128, "bf16", max_rows=5000)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_references_that_move(D, kind):
+    """Scores that grow along the keys, so that the reference of a row moves tile by tile, and large ones: nearly all of the weight on one key."""
+    rows, H = [700, 300], 2
+    q, k, v = make(rows, H, 1, D, kind, 3, packed=False)
+    k *= torch.linspace(0.1, 6, 1000, device="cuda")[:, None, None].to(k.dtype)
+    for up in (1.0, 8.0):
+        y = q * up
+        got, _ = K_.attn_prompt(y, k, v, starts(rows), max_rows=700)
+        want, tol = prompt64(y, k, v, rows, D ** -0.5)
+        assert ((got.double() - want).abs() <= tol).all() and status() == 0
+
+
+def test_rows_behind_the_last_and_between_are_left_as_they_were():
+    rows, H, D = [130, 0, 5], 3, 64
+    q, k, v = make(rows, H, 1, D, "f16", tail=60)
+    for extra in (0, 60):
+        out = torch.full((195, H, D), 3.0, device="cuda", dtype=torch.float16)
+        rs = starts(rows)
+        from hipster_b200 import _lib
+        hb.check(_lib.more().hp_attn_prompt(q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], 1, None, 0, 0, H, 1, D, rs.data_ptr(), 3, 135 + extra, 130, D ** -0.5, out.data_ptr(), None, None,
+                                            torch.cuda.current_stream().cuda_stream))
+        want, tol = prompt64(q[:135], k[:135], v[:135], rows, D ** -0.5)
+        assert status() == 0 and (out[135:] == 3).all() and ((out[:135].double() - want).abs() <= tol).all()
+
+
+def test_a_prompts_result_depends_on_itself_alone():
+    rows = [400, 77, 128, 1]
+    q, k, v, got = check(rows, 4, 2, 128, "bf16")
+    r = 0
+    for t in rows:
+        alone, _ = K_.attn_prompt(q[r:r + t], k[r:r + t], v[r:r + t], i32([0, t]), max_rows=t)
+        assert torch.equal(alone, got[r:r + t])
+        r += t
+    head, _ = K_.attn_prompt(q[:200], k[:200], v[:200], i32([0, 200]), max_rows=200)   # causal: the first rows know nothing of the others
+    assert torch.equal(head, got[:200])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("at", [0, 1, 127, 128, 200, 383, 391])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(kind, D, at, bad):
+    rows, H = [392, 150], 2
+    q, k, v = make(rows, H, 1, D, kind, 7, packed=False)
+    clean, _ = K_.attn_prompt(q, k, v, starts(rows), max_rows=392)
+    v[at, 0, 5] = bad
+    v[at, 0, D - 1] = bad
+    got, _ = K_.attn_prompt(q, k, v, starts(rows), max_rows=392)
+    hit = torch.zeros((542, H, D), dtype=torch.bool, device="cuda")
+    hit[at:392, :, [5, D - 1]] = True
+    assert torch.equal(got[~hit], clean[~hit]) and not torch.isfinite(got[hit]).any() and status() == 0
+    if bad == math.inf:   # the key's own row: its weight is not zero
+        assert (got[at, :, 5] == math.inf).all()
+
+
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("at", [0, 130, 391])
+def test_keys_and_queries_that_are_not_finite(D, at):
+    rows, H = [392, 150], 2
+    q, k, v = make(rows, H, 1, D, "bf16", 7, packed=False)
+    clean, _ = K_.attn_prompt(q, k, v, starts(rows), max_rows=392)
+    old = k[at].clone()
+    k[at, 0, 3] = math.nan
+    got, _ = K_.attn_prompt(q, k, v, starts(rows), max_rows=392)
+    assert torch.equal(got[:at], clean[:at]) and torch.isnan(got[at:392]).all() and torch.equal(got[392:], clean[392:])
+    k[at] = old
+    q[at, 1, 0] = math.inf
+    got, _ = K_.attn_prompt(q, k, v, starts(rows), max_rows=392)
+    keep = torch.ones((542, H), dtype=torch.bool, device="cuda")
+    keep[at, 1] = False
+    assert torch.equal(got[keep], clean[keep]) and status() == 0
+
+
+def test_another_prompts_non_finite_rows_do_not_count():
+    """Tiles reach over a prompt's end into the next one's rows, and past the last row of the buffers."""
+    rows = [50, 200, 10]
+    q, k, v = make(rows, 2, 1, 128, "f16", 5, packed=False)
+    clean, _ = K_.attn_prompt(q, k, v, starts(rows), max_rows=200)
+    for t in (q, k, v):
+        t[50:250] = math.nan
+    got, _ = K_.attn_prompt(q, k, v, starts(rows), max_rows=200)
+    keep = [*range(50), *range(250, 260)]
+    assert torch.equal(got[keep], clean[keep]) and torch.isnan(got[50:250]).all() and status() == 0
+
+
+@pytest.mark.parametrize("up", [1e15, 1e18])
+def test_scores_of_any_size(up):
+    """Scores up to 1e36: the largest one takes it all, and outputs are finite."""
+    T, D = 300, 64
+    q, k, v = make([T], 2, 1, D, "bf16", 9, packed=False)
+    q, k = (q.float() * up).bfloat16(), (k.float() * up).bfloat16()
+    got, _ = K_.attn_prompt(q, k, v, i32([0, T]), max_rows=T)
+    s = torch.einsum("ihd,jd->hij", q.double(), k[:, 0].double()).masked_fill(torch.ones((T, T), dtype=torch.bool, device="cuda").triu(1), -math.inf)
+    want = v[:, 0][s.argmax(-1)].permute(1, 0, 2)
+    assert status() == 0 and ((got.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs()).all()
+
+
+def test_no_weight_at_all():
+    """Scores that are all minus infinity: zeros, as elsewhere."""
+    q, k, v = make([3], 1, 1, 64, "bf16", packed=False)
+    q.fill_(1)
+    k.fill_(-math.inf)
+    got, _ = K_.attn_prompt(q, k, v, i32([0, 3]), max_rows=3)
+    assert (got == 0).all() and status() == 0
+
+
+def test_strides():
+    T, H, n_kv, D = 200, 4, 2, 128
+    q, k, v = make([T], H, n_kv, D, "f16", packed=False)
+    want, _ = K_.attn_prompt(q, k, v, i32([0, T]), max_rows=T)
+    heads_first = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    padded = lambda t: torch.nn.functional.pad(t, (0, 8, 0, 1))[:, :-1, :D]  # noqa: E731
+    for f in (heads_first, padded):
+        got, _ = K_.attn_prompt(f(q), f(k), f(v), i32([0, T]), max_rows=T, gate=None)
+        assert torch.equal(got, want)
+    one = k[:, :1]
+    got, _ = K_.attn_prompt(q[:1], one[:1], v[:1, :1], i32([0, 1]), max_rows=7)
+    assert torch.equal(got[:1, 0], v[:1, 0]) and status() == 0
+
+
+def test_quantised_output_is_the_quantised_output():
+    """Rows of the next projection: int8 of the outputs in 32 bits, which lie half a step of f16 from those in 16 bits."""
+    rows, H, D = [150, 3], 6, 64
+    q, k, v = make(rows, H, 2, D, "f16")
+    gate = torch.randn((153, H, D), generator=gen(1), device="cuda")
+    out, xq = K_.attn_prompt(q, k, v, starts(rows), max_rows=150, gate=gate, want_q8=True)
+    none, only = K_.attn_prompt(q, k, v, starts(rows), max_rows=150, gate=gate, want_out=False, want_q8=True)
+    assert none is None and torch.equal(xq.q, only.q) and torch.equal(xq.sc, only.sc)
+    c, d, s = xq.unpack()
+    x = out.view(153, -1).float()
+    amax = x.unflatten(1, (-1, 32)).abs().amax(-1)
+    assert ((d * 127 - amax).abs() <= 2.0 ** -10 * amax).all() and torch.equal(s, d * c.float().unflatten(1, (-1, 32)).sum(-1))
+    assert ((c.float().unflatten(1, (-1, 32)) * d[..., None] - x.unflatten(1, (-1, 32))).abs() <= (0.5 + 127 * 2.0 ** -10) * d[..., None]).all() and status() == 0
+
+
+def test_bad_row_starts_are_told():
+    q, k, v = make([40], 2, 1, 64, "f16", packed=False)
+    want, _ = K_.attn_prompt(q, k, v, i32([0, 30, 40]), max_rows=30)
+    assert status() == 0
+    for rs, kept in (([0, 30, 41], 40), ([-1, 30, 40], 0), ([0, 30, 1 << 30], 40), ([0, 30, 20], 30), ([0, -5, 40], 0)):
+        got, _ = K_.attn_prompt(q, k, v, i32(rs), max_rows=30)
+        assert status() == 1, rs
+        assert torch.equal(got[:kept], want[:kept])
+    K_.attn_prompt(q, k, v, i32([0, 30, 40]), max_rows=29)
+    assert status() == 1
+
+
+def test_streams_and_captures():
+    rows = [300, 90]
+    q, k, v = make(rows, 4, 2, 256, "f16", packed=False)
+    rs = starts(rows)
+    run = lambda: K_.attn_prompt(q, k, v, rs, max_rows=300)[0]  # noqa: E731
+    want = run()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for i in range(9):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append(run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = run()
+    for r in ([300, 90], [10, 300], [0, 390], [128, 128]):   # other lengths in a captured call: 390 rows are more than it was told
+        rs.copy_(starts(r))
+        q.normal_(generator=gen(r[0]))
+        g.replay()
+        torch.cuda.synchronize()
+        n = sum(r)
+        if max(r) <= 300:
+            assert torch.equal(y[:n], run()[:n]) and status() == 0
+        else:
+            assert status() == 1
+
+
+def test_prompts_beside_calls_that_hold_all_accumulator_memory():
+    st = P.Setup([150, 40], [1500, 700], 2, 256, 64, "i8")
+    x = torch.randn((190, 12, 256), generator=gen(1), device="cuda")
+    q, k, v = make([500, 100], 8, 2, 128, "bf16")
+    paged = lambda: K_.attn_paged(x, st.pool, *st.batch, max_rows=150, max_kv=1500)[0]  # noqa: E731
+    prompt = lambda: K_.attn_prompt(q, k, v, starts([500, 100]), max_rows=500)[0]  # noqa: E731
+    want = paged(), prompt()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(4)], []
+    for i in range(24):
+        with torch.cuda.stream(streams[i % 4]):
+            got.append((prompt if i % 3 else paged)())
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[1 if i % 3 else 0]) for i, g in enumerate(got)) and status() == 0
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    code = ("import torch\n"
+            "from hipster_b200 import kernels as K\n"
+            "x = torch.randn((30, 4, 64), device='cuda')\n"
+            "rs = torch.tensor([0, 30], dtype=torch.int32, device='cuda')\n"
+            "pos = torch.arange(30, dtype=torch.int32, device='cuda')\n"
+            "torch.cuda.synchronize()\n"
+            "g = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(g):\n"
+            "    rope = K.rope_table(32, 64, 1e4)\n"
+            "    q, k, v = K.rope_rows(x[:, :2], x[:, 2:3], x[:, 3:], rope, pos)\n"
+            "    y, _ = K.attn_prompt(q, k, v, rs, max_rows=30)\n"
+            "g.replay()\n"
+            "torch.cuda.synchronize()\n"
+            "K.device_status()\n"
+            "z, _ = K.attn_prompt(q, k, v, rs, max_rows=30)\n"
+            "assert torch.equal(y, z)\n"
+            "print('fine')\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+def test_refusals_of_the_python_call(form):
+    q, k, v = make([10], 4, 2, 64, "f16", packed=False)
+    rs = i32([0, 10])
+    f = lambda q=q, k=k, v=v, rs=rs, max_rows=10, **kw: K_.attn_prompt(q, k, v, rs, max_rows, **kw)  # noqa: E731
+    f()
+    odd = torch.zeros(10 * 4 * 64 + 8, device="cuda", dtype=torch.float16)[1:2561].view(10, 4, 64)
+    bad = [lambda: f(q=q.float(), k=k.float(), v=v.float()), lambda: f(k=k.bfloat16()), lambda: f(q=q[:, :3]), lambda: f(k=k[:9]), lambda: f(v=v[:, :1]), lambda: f(v=v[..., :32]), lambda: f(q=q[0]), lambda: f(q=q.cpu()), lambda: f(rs=rs.long()),
+           lambda: f(rs=rs.cpu()), lambda: f(rs=rs[:1]), lambda: f(max_rows=0), lambda: f(max_rows=1 << 40), lambda: f(scale=0.0), lambda: f(scale=math.nan), lambda: f(gate=q), lambda: f(gate=q.float()[:, :2]), lambda: f(want_out=False),
+           lambda: f(q=odd), lambda: f(q=q[:1].expand(10, -1, -1)), lambda: f(q=q.transpose(1, 2).contiguous().transpose(1, 2)), lambda: f(q=q[:0], k=k[:0], v=v[:0]), lambda: f(q=q[..., :48], k=k[..., :48], v=v[..., :48])]
+    for i, g in enumerate(bad):
+        with pytest.raises(hb.HipsterError):
+            g()
+            pytest.fail(f"call {i} was not refused")
+    assert status() == 0
+
+
+def test_a_chat_about_an_image():
+    """A prompt with an image and the steps behind it, as a server runs them: the prompt's rows are rotated by time, height and width, attended at full precision and written to a cache in 4 bits; drafts are appended at
+    positions that run on behind the image's, verified over the cache, and partly rejected."""
+    H, n_kv, D, page, T, steps = 6, 2, 256, 16, 150, 8
+    g = gen(11)
+    n = T + 3 * steps
+    stream = torch.randn((n, H + 2 * n_kv, D), generator=g, device="cuda")
+    gates = torch.randn((n, H, D), generator=g, device="cuda")
+    qn, kn = ((1 + 0.1 * torch.randn(D, generator=g, device="cuda")).bfloat16() for _ in range(2))
+    rope, axes = K_.rope_table(n, 64, 1e7), K_.rope_axes((11, 11, 10), interleaved=True)
+    pos = [[], [], []]   # 20 tokens, an image of 10 x 12 patches, text
+    for i in range(n):
+        j = i - 20
+        for a in range(3):
+            pos[a].append(i if j < 0 else 20 + (0, j // 12, j % 12)[a] if j < 120 else 32 + j - 120)
+    pos = i32(pos)
+    table = i32([[3, 0, 5, 1, 4, 9, 10, 11, 2, 6, 7, 8]])
+    pool = K_.KVPages.empty(12, n_kv, page, D, dtype="i4")
+    rs, ln = i32([0, T]), i32([T])
+    x = stream[:T]
+    q, k, v = K_.rope_rows(x[:, :H], x[:, H:H + n_kv], x[:, H + n_kv:], rope, pos[:, :T].contiguous(), axes, q_norm=qn, k_norm=kn)
+    out, xq = K_.attn_prompt(q, k, v, rs, max_rows=T, gate=gates[:T], want_q8=True)
+    K_.kv_append(pool, x[:, H:H + n_kv], x[:, H + n_kv:], table, rs, ln, rope, k_norm=kn, positions=pos[:, :T].contiguous(), axes=axes)
+    want, tol = prompt64(q, k, v, [T], D ** -0.5, gates[:T])
+    assert ((out.double() - want).abs() <= tol).all() and xq.unpack()[0].shape == (T, H * D) and status() == 0
+    # the cache holds the keys that the prompt saw, to a step of 4 bits: S u / 2 and a full one at the ends of a group's range, at most 2 |max - min| / 15
+    kb, vb = K_.kv_read(pool, table, rs, ln, R=T)
+    for a, b in ((kb, k), (vb, v)):
+        lo, hi = b.float().unflatten(-1, (-1, 32)).amin(-1).clamp(max=0), b.float().unflatten(-1, (-1, 32)).amax(-1).clamp(min=0)
+        step = (hi - lo).amax(-1, keepdim=True) / 15   # the factor of a group at most one too large: a fifteenth of the largest
+        assert ((a.float() - b.float()).unflatten(-1, (-1, 32)).abs() <= ((hi - lo) / 15 + step / 15)[..., None] * 1.01 + 0.01).all()
+
+    import test_four_bits_gpu as F
+    at = T
+    for i in range(steps):   # three rows, of which one to three are kept
+        keep = 1 + i % 3
+        x = stream[at:at + 3].clone()
+        x[keep:] *= 30
+        rs, ln = i32([0, 3]), i32([at + 3])
+        q = K_.kv_append(pool, x[:, H:H + n_kv], x[:, H + n_kv:], table, rs, ln, rope, q=x[:, :H], q_norm=qn, k_norm=kn, positions=pos[:, at:at + 3].contiguous(), axes=axes)
+        got, _ = K_.attn_paged(q, pool, table, rs, ln, max_rows=3, max_kv=n, gate=gates[at:at + 3])
+        st = F.Setup.__new__(F.Setup)
+        st.rows, st.lens, st.R, st.D, st.page, st.pool, st.table = [3], [at + 3], 3, D, page, pool, table
+        want, tol = P.attn64(st, q, 1 / 16, 0, 0, gates[at:at + 3])
+        assert ((got.double() - want).abs() <= tol).all() and status() == 0
+        at += keep
