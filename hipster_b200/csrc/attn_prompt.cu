@@ -21,8 +21,9 @@
 namespace hp {
 namespace {
 
-constexpr int TQ = 128, TK = 128;   // rows of a CTA, keys of a tile
+constexpr int TQ = 128;   // rows of a CTA
 constexpr float MU_STEP = 8.f;
+constexpr int PASS = 68;            // floats of a row of 64 outputs on their way out: 16-byte pieces of 8 rows hit distinct banks
 
 struct PromptArgs {
     const int* row_start; int S, R, max_rows, n_head, n_kv, G; float scale2;   // scale * log2 e
@@ -30,25 +31,30 @@ struct PromptArgs {
     const float* gate; size_t g_ld, g_hs; void* out; int8_t* oq; float* osc; int* err; int* arg_err;
 };
 
+// Tiles of TK keys in ST stages; a stage's K comes in KP parts of 64 dims or as one, its V in VP parts of 32 keys or as one. Two tiles of scores: one is formed while the other is weighed.
 template <int D> struct Geo {
-    static constexpr int PARTS = D / 64, VP = 4, VROWS = TK / VP;              // parts of K (64 dims), of V (32 keys)
-    static constexpr int K_PART = TK * 128, V_PART = VROWS * D * 2;
-    static constexpr int OFF_Q = 0, OFF_K = TQ * D * 2, OFF_V = OFF_K + TK * D * 2, SMEM = OFF_V + TK * D * 2 + 1024;   // 1024 for the alignment
-    static constexpr int NS = D == 256 ? 2 : 1;                                // tiles of scores
+    static constexpr int TK = D == 256 ? 128 : 64, ST = D == 256 ? 1 : 2, PARTS = D / 64, KP = D == 256 ? PARTS : 1, VP = D == 256 ? 4 : 1, VROWS = TK / VP;
+    static constexpr int HAND = 2;                                             // hand-overs of a tile's weights
+    static constexpr int K_GROUP = TK * 128, K_PART = PARTS / KP * K_GROUP, V_PART = VROWS * D * 2, TILE = TK * D * 2;
+    static constexpr int OFF_Q = 0, OFF_K = TQ * D * 2, OFF_V = OFF_K + ST * TILE, SMEM = OFF_V + ST * TILE + 1024;   // 1024 for the alignment
     static constexpr int T_O = 0, T_S = D, TMEM = D == 256 ? 512 : 256;
-    static constexpr int CTAS = D == 256 ? 1 : 2, THREADS = 192;
-    static_assert(T_S + NS * TK <= TMEM && CTAS * SMEM <= 227 * 1024, "");
+    static constexpr int CTAS = D == 256 ? 1 : 2;
+    // 256 dims: a warp of its own fetches whichever part is free next (copies by the products' warps: 1.76 -> 1.95 ms for 16384 rows of 16 heads). Two CTAs per SM: 224 threads would leave 128 registers each, with spills (1.04 -> 1.08 ms)
+    static constexpr bool COPIER = D == 256;
+    static constexpr int THREADS = COPIER ? 224 : 192;
+    static_assert(T_S + 2 * TK <= TMEM && CTAS * SMEM <= 227 * 1024 && 4 * 32 * PASS * 4 <= SMEM - 1024, "");
 };
 
-// 128-byte swizzle, groups of 8 rows 1024 bytes apart; N-major: the next 64 elements lie `next` bytes behind
-__device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t next) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(next >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+// Operands in shared memory: 128-byte swizzle, groups of 8 rows 1024 bytes apart; N-major: the next 64 elements lie `next` bytes behind. The lower half of a descriptor, to which offsets / 16 are added; the upper one is
+// the same for all. Few instructions per product: the products' warp shares its instruction cache with the weights' long loops
+constexpr uint32_t DESC_HIGH = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t next) { return (addr >> 4) | ((next >> 4) << 16); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int add) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 a, {%1, %5};\nmov.b64 b, {%2, %5};\ntcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(DESC_HIGH) : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int add) {   // A in accumulator memory
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int add) {   // A in accumulator memory
+    asm volatile("{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 b, {%2, %5};\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(DESC_HIGH) : "memory");
 }
 __device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -75,12 +81,23 @@ template <int N> __device__ __forceinline__ void ld_wait(float* a) {   // orders
 #pragma unroll
     for (int i = 0; i < N; ++i) asm volatile("" : "+f"(a[i]));
 }
-__device__ __forceinline__ bool one_wait(uint32_t bar, uint32_t parity, int* err) { return mbar_test(bar, parity) || tc_wait(bar, parity, err); }
+// Bounded waits that keep asking, some half a second: a wait that may park its warp sees a hand-over some 300 clocks later, and a tile has four in a row
+__device__ __forceinline__ bool one_wait(uint32_t bar, uint32_t parity, int* err) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < (1u << 24); ++i) if (mbar_test(bar, parity)) return true;
+    if (err) atomicExch(err, HP_ETIMEOUT);
+    return false;
+}
+// of the products' warps: where two CTAs share an SM, one's wait costs less than its questions
+template <int D> __device__ __forceinline__ bool mma_wait(uint32_t bar, uint32_t parity, int* err) { return D == 256 ? one_wait(bar, parity, err) : mbar_test(bar, parity) || tc_wait(bar, parity, err); }
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) { return __all_sync(0xffffffffu, one_wait(bar, parity, err)); }
+__device__ __forceinline__ float max3(float a, float b, float c) { float y; asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c)); return y; }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y) {
     if constexpr (std::is_same<T, __half>::value) return h2_bits(__floats2half2_rn(x, y));
     else { const __nv_bfloat162 b = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&b); }
 }
+// to 2^-21: outputs have 16 bits or 8
+__device__ __forceinline__ float sigmoid16(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.f + ex2(x * -1.4426950408889634f))); return y; }
 template <typename T> __device__ __forceinline__ float to_f32(uint16_t b) { if constexpr (std::is_same<T, __half>::value) return h2f(b); else return bf2f(b); }
 template <typename T> __device__ __forceinline__ bool odd16(uint32_t b) { constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u; return (b & E) == E; }   // infinite or NaN
 // the top bits of both halves: set where the half is infinite or NaN, its exponent plus one
@@ -99,9 +116,12 @@ __device__ __forceinline__ QBlock find_rows(const PromptArgs& a, int blk, int la
     };
     QBlock o{-1, 0, 0, 0};
     if (a.S == 1) { o.T = seq(0, o.row0); o.i = (o.T + TQ - 1) / TQ - 1 - blk; o.s = o.i < 0 ? -1 : 0; return o; }
+    int row0 = 0, T = 0;   // of sequence `lane`; calls of more look the others up again
+    if (lane < a.S) T = seq(lane, row0);
+    const int n0 = (T + TQ - 1) / TQ;
     auto from = [&](int i) {   // F(i)
-        int n = 0, r;
-        for (int s = lane; s < a.S; s += 32) n += max(0, (seq(s, r) + TQ - 1) / TQ - i);
+        int n = max(0, n0 - i), r;
+        for (int s = lane + 32; s < a.S; s += 32) n += max(0, (seq(s, r) + TQ - 1) / TQ - i);
         return __reduce_add_sync(0xffffffffu, n);
     };
     int lo = 0, hi = (a.max_rows + TQ - 1) / TQ;   // F(lo) > blk >= F(hi)
@@ -109,8 +129,7 @@ __device__ __forceinline__ QBlock find_rows(const PromptArgs& a, int blk, int la
     while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (from(mid) > blk) lo = mid; else hi = mid; }
     int k = blk - from(lo + 1);
     for (int s0 = 0; s0 < a.S; s0 += 32) {
-        int row0 = 0, T = 0;
-        if (s0 + lane < a.S) T = seq(s0 + lane, row0);
+        if (s0) { row0 = T = 0; if (s0 + lane < a.S) T = seq(s0 + lane, row0); }
         const unsigned has = __ballot_sync(0xffffffffu, (T + TQ - 1) / TQ > lo);
         const int n = __popc(has);
         if (k < n) {
@@ -123,33 +142,95 @@ __device__ __forceinline__ QBlock find_rows(const PromptArgs& a, int blk, int la
     return o;
 }
 
+// Infinite and NaN values of a tile that has hidden keys: noted in odd[] (a bit per key of the block's rows) and taken out of the tile in shared memory, before its products. A thread has a key, or half of its dims
+template <int D, typename T>
+__device__ bool take_out(uint8_t* v, uint64_t* v_full, uint32_t* odd, uint32_t parity, int tid, int* err) {
+    using G = Geo<D>;
+    constexpr int SHARE = 128 / G::TK, N = D / 8 / SHARE;   // 16-byte pieces of a thread
+    const int key = tid % G::TK, lane = tid & 31, i0 = tid / G::TK * N, part = key / G::VROWS, in = key % G::VROWS;
+    const bool ok = warp_wait(smem_u32(&v_full[part]), parity, err);
+    if (!ok) return false;
+    uint8_t* const vr = v + part * G::V_PART + in * 128;
+    uint32_t any = 0;
+#pragma unroll 8
+    for (int i = i0; i < i0 + N; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(vr + (i >> 3) * (G::VROWS * 128) + (((i & 7) ^ (in & 7)) << 4));
+        any |= odd_pair<T>(u.x) | odd_pair<T>(u.y) | odd_pair<T>(u.z) | odd_pair<T>(u.w);
+    }
+    any &= 0x80008000u;
+    if (any) {
+#pragma unroll 1
+        for (int i = i0 * 8; i < (i0 + N) * 8; ++i) {
+            uint16_t* const e = reinterpret_cast<uint16_t*>(vr + (i >> 6) * (G::VROWS * 128) + (((i >> 3 & 7) ^ (in & 7)) << 4)) + (i & 7);
+            if (odd16<T>(*e)) *e = 0;
+        }
+        fence_proxy_async();
+    }
+    const unsigned bad = __ballot_sync(0xffffffffu, any != 0);
+    if (lane == 0 && bad) atomicOr(&odd[key >> 5], bad);
+    return true;
+}
+// and their share of the sums of the rows that see them, in accumulator memory. Keys are those of the block's own rows, first row r0
+template <int D, typename T>
+__device__ __noinline__ void put_in(const PromptArgs& a, const uint32_t* odd, int r0, int row, bool live, int head, int kh, float c, float mu, uint32_t at) {
+#pragma unroll 1
+    for (int j = 0; j < TQ; ++j) {
+        if (!(odd[j >> 5] >> (j & 31) & 1) || r0 + j >= a.R) continue;
+        const uint16_t* const kr = (const uint16_t*)a.k + (size_t)(r0 + j) * a.k_ld + (size_t)kh * a.k_hs;
+        const uint16_t* const vr = (const uint16_t*)a.v + (size_t)(r0 + j) * a.v_ld + (size_t)kh * a.v_hs;
+        const bool sees = live && j <= row;
+        float w = 0.f;
+        if (sees) {
+            const uint16_t* const qr = (const uint16_t*)a.q + (size_t)(r0 + row) * a.q_ld + (size_t)head * a.q_hs;
+#pragma unroll 1
+            for (int d = 0; d < D; ++d) w = fmaf(to_f32<T>(qr[d]), to_f32<T>(kr[d]), w);
+            w = w * c - mu;
+            w = w > 2.f * MU_STEP ? ex2(2.f * MU_STEP) : ex2(w);   // summed in another order than S: not beyond what a weight can be; NaN stays
+        }
+#pragma unroll 1
+        for (int d = 0; d < D; ++d) {
+            const uint16_t e = vr[d];
+            if (!odd16<T>(e)) continue;   // the same for all lanes
+            uint32_t o;
+            asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(at + d) : "memory");
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            asm volatile("" : "+r"(o));
+            if (sees) o = __float_as_uint(__uint_as_float(o) + w * to_f32<T>(e));
+            __syncwarp();
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(at + d), "r"(o) : "memory");
+            st_wait();
+        }
+        __syncwarp();
+    }
+}
+
 template <int D, typename T>
 __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const PromptArgs a) {
     using G = Geo<D>;
     extern __shared__ uint8_t sm_raw[];
     struct Shared {
-        uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2], pv_done, fin;
-        uint32_t tmem, odd[TK / 32];   // keys of the last tile with an infinite or NaN value
+        uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2][4], pv_done, fin[2];   // parts: stage * (KP or VP) + part
+        uint32_t tmem, odd[TQ / 32];   // keys of the block's own rows with an infinite or NaN value
     };
     __shared__ Shared x;
     uint8_t* const sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t base = smem_u32(sm);
+    if (tid == 0) {
+        mbar_init(smem_u32(&x.q_full), 1);
+        for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&x.k_full[i]), 1); mbar_init(smem_u32(&x.k_empty[i]), 1); mbar_init(smem_u32(&x.v_full[i]), 1); mbar_init(smem_u32(&x.v_empty[i]), 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); for (int p = 0; p < G::HAND; ++p) mbar_init(smem_u32(&x.p_full[i][p]), 4); }
+        mbar_init(smem_u32(&x.pv_done), 1); mbar_init(smem_u32(&x.fin[0]), 1); mbar_init(smem_u32(&x.fin[1]), 1);
+        for (int i = 0; i < TQ / 32; ++i) x.odd[i] = 0;
+        fence_barrier_init();
+    }
     pdl_wait();
     pdl_launch_dependents();
     const int head = blockIdx.x % a.n_head;
     const QBlock b = find_rows(a, blockIdx.x / a.n_head, lane);
     if (b.s < 0) return;
-    const int kh = head / a.G, tiles = b.i + 1, q0 = b.i * TQ;   // first row of the block in its sequence
-    const uint32_t base = smem_u32(sm);
-    if (tid == 0) {
-        mbar_init(smem_u32(&x.q_full), 1);
-        for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&x.k_full[i]), 1); mbar_init(smem_u32(&x.k_empty[i]), 1); mbar_init(smem_u32(&x.v_full[i]), 1); mbar_init(smem_u32(&x.v_empty[i]), 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); mbar_init(smem_u32(&x.p_full[i]), 4); }
-        mbar_init(smem_u32(&x.pv_done), 1); mbar_init(smem_u32(&x.fin), 1);
-        for (int i = 0; i < TK / 32; ++i) x.odd[i] = 0;
-        fence_barrier_init();
-    }
-    if (warp == 4) {
+    const int kh = head / a.G, q0 = b.i * TQ, tiles = (min(q0 + TQ, b.T) + G::TK - 1) / G::TK;   // q0: first row of the block in its sequence
+    if (warp == 4) {   // behind the wait: a CTA that waits holds no accumulator memory
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&x.tmem)), "n"(G::TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -160,32 +241,45 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
     bool ok = true;
 
     if (warp < 4) {   // ---- weights
+        constexpr int TK = G::TK;
         const int row = tid;                              // of the block
         const uint32_t at = tmem + ((uint32_t)warp << 21);
         const float c = a.scale2;
         float mu = MU_NONE, l = 0.f;
+        bool there = false, far = false;   // scores of the next tile; a row of the warp has a reference from 2^26 on
+        if (a.gate && q0 + row < b.T) {   // this row's gates on their way to L2, lines of 128 bytes
+            const float* const g = a.gate + (size_t)(b.row0 + q0 + row) * a.g_ld + (size_t)head * a.g_hs;
+#pragma unroll
+            for (int i = 0; i < D; i += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(g + i));
+        }
 #pragma unroll 1
         for (int n = 0; n < tiles; ++n) {
-            const uint32_t sc = at + G::T_S + n % G::NS * TK;
-            ok = ok && warp_wait(smem_u32(&x.s_full[n % G::NS]), n / G::NS & 1, a.err);
+            const uint32_t sc = at + G::T_S + (n & 1) * TK;
+            if (!__all_sync(0xffffffffu, there)) ok = ok && warp_wait(smem_u32(&x.s_full[n & 1]), n >> 1 & 1, a.err);
             if (!ok) break;
             tc_fence_after();
             float s[TK];
 #pragma unroll
             for (int i = 0; i < TK; i += 32) ld32(s + i, sc + i);
             ld_wait<TK>(s);
-            const bool last = n == tiles - 1;
-            if (last) {
+            const int lim = q0 + row - n * TK;   // last key of the tile that the row sees
+            const bool hides = n * TK + TK - 1 > q0;
+            if (hides) {
 #pragma unroll
-                for (int i = 0; i < TK; ++i) if (i > row) s[i] = -INFINITY;
+                for (int i = 0; i < TK; ++i) if (i > lim) s[i] = -INFINITY;
             }
             float t[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 4; i < TK; i += 4) { t[0] = fmaxf(t[0], s[i]); t[1] = fmaxf(t[1], s[i + 1]); t[2] = fmaxf(t[2], s[i + 2]); t[3] = fmaxf(t[3], s[i + 3]); }
-            const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * c;
+            for (int i = 4; i + 7 < TK; i += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[e] = max3(t[e], s[i + e], s[i + 4 + e]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = fmaxf(t[e], s[TK - 4 + e]);
+            const float top = fmaxf(max3(t[0], t[1], t[2]), t[3]) * c;
             if (__any_sync(0xffffffffu, top > mu + MU_STEP)) {   // a row moves by its own scores alone
                 float al = 1.f;
                 if (top > mu + MU_STEP) { al = ex2(mu - top); mu = top; l = l * al; }   // the first reference: 0
+                far = __any_sync(0xffffffffu, fabsf(mu) >= 67108864.f && mu != MU_NONE);
                 if (n) {
                     ok = warp_wait(smem_u32(&x.pv_done), (n - 1) & 1, a.err);
                     if (!ok) break;
@@ -203,185 +297,204 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
                 }
             }
             // distances from the reference. Logarithms from 2^26 on lie in steps of 8: there the product is rounded as it was for the reference
-            if (__any_sync(0xffffffffu, fabsf(mu) >= 67108864.f && mu != MU_NONE)) {
+            if (far) {
 #pragma unroll
                 for (int i = 0; i < TK; ++i) s[i] = s[i] * c - mu;
             } else {
 #pragma unroll
                 for (int i = 0; i < TK; i += 2) { float2 d = make_float2(-mu, -mu); fma2(d, make_float2(s[i], s[i + 1]), make_float2(c, c)); s[i] = d.x; s[i + 1] = d.y; }
             }
+            if (hides) ok = take_out<D, T>(sm + G::OFF_V + n % G::ST * G::TILE, x.v_full + n % G::ST * G::VP, x.odd + (n * TK - q0) / 32, n / G::ST & 1, tid, a.err) && ok;
+            // weights of 32 keys are handed over as soon as they are there: their products run under the next ones' exponentials
             float2 l2 = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < TK; i += 16) {
-                uint32_t w[8];
+            for (int p = 0; p < G::HAND; ++p) {
+                constexpr int KEYS = TK / G::HAND;
+                if (p == G::HAND - 1) there = n + 1 < tiles && mbar_test(smem_u32(&x.s_full[(n + 1) & 1]), (n + 1) >> 1 & 1);   // an answer takes some 200 clocks
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const float2 y = make_float2(ex2(s[i + e]), ex2(s[i + e + 1]));
-                    l2 = add2(l2, y);
-                    w[e / 2] = pack2<T>(y.x, y.y);
+                for (int i = p * KEYS; i < p * KEYS + KEYS; i += 16) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float2 y = make_float2(ex2(s[i + e]), ex2(s[i + e + 1]));
+                        l2 = add2(l2, y);
+                        w[e / 2] = pack2<T>(y.x, y.y);
+                    }
+                    st8(sc + i, w);   // 16 keys in the first half of their scores' columns
                 }
-                st8(sc + i, w);   // 16 keys in the first half of their scores' columns
+                st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0 && ok) mbar_arrive(smem_u32(&x.p_full[n & 1][p]));
             }
             l = l + (l2.x + l2.y);
-            if (last) {   // a key per thread: its values
-                const int part = warp;   // 32 keys
-                ok = warp_wait(smem_u32(&x.v_full[part]), n & 1, a.err);
-                if (!ok) break;
-                uint8_t* const vr = sm + G::OFF_V + part * G::V_PART + lane * 128;
-                uint32_t any = 0;
-#pragma unroll 4
-                for (int i = 0; i < D / 8; ++i) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(vr + (i >> 3) * (G::VROWS * 128) + (((i & 7) ^ (lane & 7)) << 4));
-                    any |= odd_pair<T>(u.x) | odd_pair<T>(u.y) | odd_pair<T>(u.z) | odd_pair<T>(u.w);
-                }
-                any &= 0x80008000u;
-                if (any) {
-                    for (int i = 0; i < D; ++i) {
-                        uint16_t* const e = reinterpret_cast<uint16_t*>(vr + (i >> 6) * (G::VROWS * 128) + (((i >> 3 & 7) ^ (lane & 7)) << 4)) + (i & 7);
-                        if (odd16<T>(*e)) *e = 0;
-                    }
-                    fence_proxy_async();
-                }
-                const unsigned bad = __ballot_sync(0xffffffffu, any != 0);
-                if (lane == 0) x.odd[part] = bad;
-            }
-            st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&x.p_full[n % G::NS]));
+            if (!ok) break;
         }
         // ---- outputs
         ok = ok && warp_wait(smem_u32(&x.pv_done), (tiles - 1) & 1, a.err);
         tc_fence_after();
         asm volatile("bar.sync 1, 128;" ::: "memory");   // odd[] of all four warps, which all come here
-        const int r = b.row0 + q0 + row;
-        const bool mine = ok && q0 + row < b.T;
+        // 64 dims at a time through shared memory, which nothing else uses any more: a thread has a row, and 16 lanes write one
         if (ok) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            const bool odd = (x.odd[0] | x.odd[1] | x.odd[2] | x.odd[3]) != 0;
+            const int there = min(32, b.T - q0 - 32 * warp);   // rows of this warp
+            if (x.odd[0] | x.odd[1] | x.odd[2] | x.odd[3]) put_in<D, T>(a, x.odd, b.row0 + q0, row, lane < there, head, kh, c, mu, at + G::T_O);
+            float* const pass = reinterpret_cast<float*>(sm) + warp * (32 * PASS);
 #pragma unroll 1
-            for (int i = 0; i < D; i += 32) {
-                float o[32];
-                ld32(o, at + G::T_O + i); ld_wait<32>(o);
-                if (!mine) continue;
-                if (odd) {
-                    const uint16_t* const qr = (const uint16_t*)a.q + (size_t)r * a.q_ld + (size_t)head * a.q_hs;
-                    for (int j = 0; j <= row; ++j) {
-                        if (!(x.odd[j >> 5] >> (j & 31) & 1)) continue;
-                        const uint16_t* const kr = (const uint16_t*)a.k + (size_t)(b.row0 + q0 + j) * a.k_ld + (size_t)kh * a.k_hs;
-                        const uint16_t* const vr = (const uint16_t*)a.v + (size_t)(b.row0 + q0 + j) * a.v_ld + (size_t)kh * a.v_hs + i;
-                        float dot = 0.f;
-                        for (int d = 0; d < D; ++d) dot = fmaf(to_f32<T>(qr[d]), to_f32<T>(kr[d]), dot);
-                        const float w = ex2(fminf(dot * c - mu, 2.f * MU_STEP));   // summed in another order than S: not beyond what a weight can be
+            for (int i = 0; i < D; i += 64) {
+                float o[64];
+                ld32(o, at + G::T_O + i); ld32(o + 32, at + G::T_O + i + 32); ld_wait<64>(o);
+                __syncwarp();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) if (odd16<T>(vr[e])) o[e] = o[e] + w * to_f32<T>(vr[e]);
-                    }
-                }
+                for (int e = 0; e < 64; e += 4) *reinterpret_cast<float4*>(pass + lane * PASS + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+                __syncwarp();
+                // 16 lanes write a row, every second one theirs. Short loops: this runs once per block, from a cold instruction cache
+                const int d = i + lane % 16 * 4, r = b.row0 + q0 + 32 * warp, j0 = lane / 16;
+                float* const mine = pass + d - i;
+                if (a.gate) {   // all of a chunk's gates are under way before the first is used
+                    const float* const gate = a.gate + (size_t)(r + j0) * a.g_ld + (size_t)head * a.g_hs + d;
+                    float4 g[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = o[e] * inv;
-                if (a.gate) {
-                    const float4* const g = reinterpret_cast<const float4*>(a.gate + (size_t)r * a.g_ld + (size_t)head * a.g_hs + i);
+                    for (int j = 0; j < 16; ++j) if (2 * j + j0 < there) g[j] = *reinterpret_cast<const float4*>(gate + (size_t)(2 * j) * a.g_ld);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float4 y = g[e];
-                        o[4 * e] = o[4 * e] * sigmoid_det(y.x); o[4 * e + 1] = o[4 * e + 1] * sigmoid_det(y.y); o[4 * e + 2] = o[4 * e + 2] * sigmoid_det(y.z); o[4 * e + 3] = o[4 * e + 3] * sigmoid_det(y.w);
-                    }
+                    for (int j = 0; j < 16; ++j)
+                        if (2 * j + j0 < there) {
+                            float4* const y = reinterpret_cast<float4*>(mine + (2 * j + j0) * PASS);
+                            *y = make_float4(y->x * sigmoid16(g[j].x), y->y * sigmoid16(g[j].y), y->z * sigmoid16(g[j].z), y->w * sigmoid16(g[j].w));
+                        }
                 }
                 if (a.out) {
-                    uint4* const to = reinterpret_cast<uint4*>((T*)a.out + ((size_t)r * a.n_head + head) * D + i);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) to[e] = make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]), pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
-                }
-                if (a.oq) {   // as warp_quant32_store has it, 32 dims in one thread
-                    const int K = a.n_head * D, k = head * D + i;
-                    float amax = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) amax = fmaxf(amax, fabsf(o[e]));
-                    const float dd = amax / 127.f, id = amax > 0.f ? 127.f / amax : 0.f;
-                    int sum = 0;
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint32_t w[2] = {0u, 0u};
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) { const int qi = __float2int_rn(o[e + j] * id); sum += qi; w[j >> 2] |= (uint32_t)(qi & 0xff) << (8 * (j & 3)); }
-                        *reinterpret_cast<uint2*>(a.oq + xq_q_index(r, k + e, K)) = make_uint2(w[0], w[1]);
+                    T* to = (T*)a.out + ((size_t)(r + j0) * a.n_head + head) * D + d;
+#pragma unroll 4
+                    for (int j = j0; j < there; j += 2, to += 2 * (size_t)a.n_head * D) {
+                        const float4 y = *reinterpret_cast<const float4*>(mine + j * PASS);
+                        *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
                     }
-                    const size_t di = xq_d_index(r, k >> 5, K);
-                    a.osc[di] = dd; a.osc[di + 2] = dd * (float)sum;
                 }
+                if (a.oq)
+#pragma unroll 1
+                    for (int j = j0; j < there; j += 2) quant_four(*reinterpret_cast<const float4*>(mine + j * PASS), r + j, head * D + d, a.n_head * D, a.oq, a.osc);
             }
         }
-    } else if (warp == 4) {
-        if (tc_elect()) {   // ---- products
+    } else {   // ---- products and copies: K and scores in one warp, V and outputs in another, so that neither waits for what the other one waits for
+        auto fetch_q = [&] {
+            mbar_expect_tx(smem_u32(&x.q_full), TQ * D * 2);
+#pragma unroll
+            for (int i = 0; i < G::PARTS; ++i) tma3(base + G::OFF_Q + i * (TQ * 128), &mq, i * 64, head, b.row0 + q0, smem_u32(&x.q_full));
+        };
+        auto fetch_k = [&](int n, int p) {
+            const int bar = n % G::ST * G::KP + p;
+            const uint32_t full = smem_u32(&x.k_full[bar]), dst = base + G::OFF_K + n % G::ST * G::TILE + p * G::K_PART;
+            mbar_expect_tx(full, G::K_PART);
+#pragma unroll
+            for (int i = 0; i < G::PARTS / G::KP; ++i) tma3(dst + i * G::K_GROUP, &mk, (p * (G::PARTS / G::KP) + i) * 64, kh, b.row0 + n * G::TK, full);
+        };
+        auto fetch_v = [&](int n, int p) {
+            const int bar = n % G::ST * G::VP + p;
+            const uint32_t full = smem_u32(&x.v_full[bar]), dst = base + G::OFF_V + n % G::ST * G::TILE + p * G::V_PART;
+            mbar_expect_tx(full, G::V_PART);
+#pragma unroll
+            for (int i = 0; i < G::PARTS; ++i) tma3(dst + i * (G::VROWS * 128), &mv, i * 64, kh, b.row0 + n * G::TK + p * G::VROWS, full);
+        };
+        if (warp < 6 && tc_elect()) {
             constexpr uint32_t TYPE = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
-            constexpr uint32_t ID = (1u << 4) | TYPE | ((uint32_t)(TQ >> 4) << 24), ID_S = ID | ((uint32_t)(TK >> 3) << 17), ID_O = ID | ((uint32_t)(D >> 3) << 17) | (1u << 16);   // O: V is N-major
+            constexpr uint32_t ID = (1u << 4) | TYPE | ((uint32_t)(TQ >> 4) << 24), ID_S = ID | ((uint32_t)(G::TK >> 3) << 17), ID_O = ID | ((uint32_t)(D >> 3) << 17) | (1u << 16);   // O: V is N-major
+            const uint32_t q_desc = desc_low(base + G::OFF_Q, 16), k_desc = desc_low(base + G::OFF_K, 16), v_desc = desc_low(base + G::OFF_V, G::VROWS * 128);
             auto scores = [&](int n) {
-                if (n >= G::NS && !one_wait(smem_u32(&x.pv_done), (n - G::NS) & 1, a.err)) return false;   // the weights in its place are read
-                const uint32_t st = tmem + G::T_S + n % G::NS * TK;
+                if (n >= 2 && !mma_wait<D>(smem_u32(&x.pv_done), n & 1, a.err)) return false;   // the weights of n - 2, in its place, are read
+                const uint32_t st = tmem + G::T_S + (n & 1) * G::TK;
+                uint32_t qd = q_desc, kd = k_desc + n % G::ST * (G::TILE / 16);
 #pragma unroll
-                for (int p = 0; p < G::PARTS; ++p) {
-                    if (!one_wait(smem_u32(&x.k_full[p]), n & 1, a.err)) return false;
-                    tc_fence_after();
+                for (int p = 0; p < G::PARTS; ++p, qd += TQ * 8, kd += G::K_GROUP / 16) {
+                    const int bar = n % G::ST * G::KP + p * G::KP / G::PARTS;
+                    if (p % (G::PARTS / G::KP) == 0) {
+                        if (!mma_wait<D>(smem_u32(&x.k_full[bar]), n / G::ST & 1, a.err)) return false;
+                        tc_fence_after();
+                    }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mma_ss(st, desc128(base + G::OFF_Q + p * (TQ * 128) + i * 32, 16), desc128(base + G::OFF_K + p * G::K_PART + i * 32, 16), ID_S, p | i);
-                    tc_commit(smem_u32(&x.k_empty[p]));
+                    for (int i = 0; i < 4; ++i) mma_ss(st, qd + 2 * i, kd + 2 * i, ID_S, i ? 1 : p);
+                    if ((p + 1) % (G::PARTS / G::KP) == 0) tc_commit(smem_u32(&x.k_empty[bar]));
                 }
-                tc_commit(smem_u32(&x.s_full[n % G::NS]));
+                tc_commit(smem_u32(&x.s_full[n & 1]));
                 return true;
             };
             auto outputs = [&](int n) {
-                const uint32_t wt = tmem + G::T_S + n % G::NS * TK;
-                if (!one_wait(smem_u32(&x.p_full[n % G::NS]), n / G::NS & 1, a.err)) return false;
+                constexpr int SLICES = G::TK / 32, PER = G::VROWS / 32, GIVEN = SLICES / G::HAND;   // slices of 32 keys: all, of a part of V, of a hand-over
+                uint32_t wt = tmem + G::T_S + (n & 1) * G::TK, vd = v_desc + n % G::ST * (G::TILE / 16);
 #pragma unroll
-                for (int p = 0; p < G::VP; ++p) {
-                    if (!one_wait(smem_u32(&x.v_full[p]), n & 1, a.err)) return false;
+                for (int p = 0; p < SLICES; ++p, wt += 32, vd += (G::VP > 1 ? G::V_PART : 4096) / 16) {
+                    const int bar = n % G::ST * G::VP + p / PER;
+                    if (p % PER == 0 && !mma_wait<D>(smem_u32(&x.v_full[bar]), n / G::ST & 1, a.err)) return false;
+                    if (p % GIVEN == 0) {
+                        if (!mma_wait<D>(smem_u32(&x.p_full[n & 1][p / GIVEN]), n >> 1 & 1, a.err)) return false;
+                    }
                     tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < G::VROWS / 16; ++i) mma_ts(tmem + G::T_O, wt + (p * (G::VROWS / 16) + i) * 16, desc128(base + G::OFF_V + p * G::V_PART + i * 2048, G::VROWS * 128), ID_O, n | p | i);
-                    tc_commit(smem_u32(&x.v_empty[p]));
+                    for (int i = 0; i < 2; ++i) mma_ts(tmem + G::T_O, wt + 16 * i, vd + 128 * i, ID_O, i ? 1 : n | p);
+                    if ((p + 1) % PER == 0) tc_commit(smem_u32(&x.v_empty[bar]));
                 }
                 tc_commit(smem_u32(&x.pv_done));
                 return true;
             };
-            ok = one_wait(smem_u32(&x.q_full), 0, a.err) && scores(0);
-            for (int n = 0; n < tiles && ok; ++n) {
-                if (G::NS == 2 && n + 1 < tiles) ok = scores(n + 1);
-                ok = ok && outputs(n);
-                if (G::NS == 1 && n + 1 < tiles && ok) ok = scores(n + 1);
+            const bool first = warp == 4;
+            if (G::COPIER) {
+                if (first) ok = mma_wait<D>(smem_u32(&x.q_full), 0, a.err);
+                for (int n = 0; n < tiles && ok; ++n) ok = first ? scores(n) : outputs(n);
+            } else {   // a stage is fetched again when the products of the tile that it held are through
+                uint64_t *const full = first ? x.k_full : x.v_full, *const empty = first ? x.k_empty : x.v_empty;
+                const int parts = first ? G::KP : G::VP;
+                int fetched = 0;   // tiles whose copies have been issued
+                if (first) fetch_q();
+                for (; fetched < min(G::ST, tiles); ++fetched)
+                    for (int p = 0; p < parts; ++p) { if (first) fetch_k(fetched, p); else fetch_v(fetched, p); }
+                if (first) ok = mma_wait<D>(smem_u32(&x.q_full), 0, a.err);
+                for (int n = 0; n < tiles && ok; ++n) {
+                    if (n && fetched < tiles) {
+                        for (int p = 0; p < parts && ok; ++p) {
+                            ok = tc_wait(smem_u32(&empty[(n - 1) % G::ST * parts + p]), (n - 1) / G::ST & 1, a.err);
+                            if (ok) { if (first) fetch_k(fetched, p); else fetch_v(fetched, p); }
+                        }
+                        if (!ok) break;
+                        ++fetched;
+                    }
+                    ok = first ? scores(n) : outputs(n);
+                }
+                if (!ok) {   // gave up: no copy outlives the CTA
+                    for (int n = max(0, fetched - G::ST); n < fetched; ++n)
+                        for (int p = 0; p < parts; ++p) tc_wait(smem_u32(&full[n % G::ST * parts + p]), n / G::ST & 1, a.err);
+                    if (first) tc_wait(smem_u32(&x.q_full), 0, a.err);
+                }
             }
-            tc_commit(smem_u32(&x.fin));
-            tc_wait(smem_u32(&x.fin), 0, a.err);   // nothing in flight when the accumulator memory is given back
+            uint64_t& fin = x.fin[warp - 4];
+            tc_commit(smem_u32(&fin));
+            tc_wait(smem_u32(&fin), 0, a.err);   // nothing in flight when the accumulator memory is given back
         }
-    } else if (tc_elect()) {   // ---- copies: whichever part is free next
-        mbar_expect_tx(smem_u32(&x.q_full), TQ * D * 2);
-#pragma unroll
-        for (int i = 0; i < G::PARTS; ++i) tma3(base + G::OFF_Q + i * (TQ * 128), &mq, i * 64, head, b.row0 + q0, smem_u32(&x.q_full));
-        int nk = 0, nv = 0, pk = 0, pv = 0;   // tile and part next to be fetched
-        uint32_t idle = 0;
-        while ((nk < tiles || nv < tiles) && idle < (1u << 24)) {
-            ++idle;
-            if (nk < tiles && mbar_test(smem_u32(&x.k_empty[pk]), (nk & 1) ^ 1)) {
-                const uint32_t bar = smem_u32(&x.k_full[pk]);
-                mbar_expect_tx(bar, G::K_PART);
-                tma3(base + G::OFF_K + pk * G::K_PART, &mk, pk * 64, kh, b.row0 + nk * TK, bar);
-                if (++pk == G::PARTS) { pk = 0; ++nk; }
-                idle = 0;
+        if (G::COPIER && warp == 6 && tc_elect()) {
+            fetch_q();
+            int nk = 0, nv = 0, pk = 0, pv = 0;   // tile and part next to be fetched
+            uint32_t idle = 0;
+            while ((nk < tiles || nv < tiles) && idle < (1u << 23)) {
+                ++idle;
+                if (nk < tiles && mbar_test(smem_u32(&x.k_empty[nk % G::ST * G::KP + pk]), (nk / G::ST & 1) ^ 1)) {
+                    fetch_k(nk, pk);
+                    if (++pk == G::KP) { pk = 0; ++nk; }
+                    idle = 0;
+                }
+                if (nv < tiles && mbar_test(smem_u32(&x.v_empty[nv % G::ST * G::VP + pv]), (nv / G::ST & 1) ^ 1)) {
+                    fetch_v(nv, pv);
+                    if (++pv == G::VP) { pv = 0; ++nv; }
+                    idle = 0;
+                }
+                if (idle) __nanosleep(40);   // its questions take the weights' warps' time
             }
-            if (nv < tiles && mbar_test(smem_u32(&x.v_empty[pv]), (nv & 1) ^ 1)) {
-                const uint32_t bar = smem_u32(&x.v_full[pv]);
-                mbar_expect_tx(bar, G::V_PART);
-#pragma unroll
-                for (int i = 0; i < G::PARTS; ++i) tma3(base + G::OFF_V + pv * G::V_PART + i * (G::VROWS * 128), &mv, i * 64, kh, b.row0 + nv * TK + pv * G::VROWS, bar);
-                if (++pv == G::VP) { pv = 0; ++nv; }
-                idle = 0;
+            if (nk < tiles || nv < tiles) {   // gave up: no copy outlives the CTA
+                if (a.err) atomicExch(a.err, HP_ETIMEOUT);
+                for (int back = 0; back < G::ST; ++back) {
+                    for (int i = 0; i < G::KP; ++i) { const int n = (i < pk ? nk : nk - 1) - back; if (n >= 0) tc_wait(smem_u32(&x.k_full[n % G::ST * G::KP + i]), n / G::ST & 1, a.err); }
+                    for (int i = 0; i < G::VP; ++i) { const int n = (i < pv ? nv : nv - 1) - back; if (n >= 0) tc_wait(smem_u32(&x.v_full[n % G::ST * G::VP + i]), n / G::ST & 1, a.err); }
+                }
+                tc_wait(smem_u32(&x.q_full), 0, a.err);
             }
-            if (idle > 16) __nanosleep(20);
-        }
-        if (nk < tiles || nv < tiles) {   // gave up: no copy outlives the CTA
-            if (a.err) atomicExch(a.err, HP_ETIMEOUT);
-            for (int i = 0; i < G::PARTS; ++i) { const int n = i < pk ? nk : nk - 1; if (n >= 0) tc_wait(smem_u32(&x.k_full[i]), n & 1, a.err); }
-            for (int i = 0; i < G::VP; ++i) { const int n = i < pv ? nv : nv - 1; if (n >= 0) tc_wait(smem_u32(&x.v_full[i]), n & 1, a.err); }
-            tc_wait(smem_u32(&x.q_full), 0, a.err);
         }
     }
     __syncwarp();
@@ -423,8 +536,8 @@ int attn_prompt(const AttnPromptParams& p, cudaStream_t s) {
     HP_REQUIRE(blocks * p.n_head < (1ll << 31), "attn_prompt: too many rows (%d) or heads for one call", p.R);
     CUtensorMap m[3];
     int rc = encode(f, &m[0], p.q, p.q_ld, p.q_hs, p.R, p.n_head, p.head_dim, TQ, p.type);
-    if (!rc) rc = encode(f, &m[1], p.k, p.k_ld, p.k_hs, p.R, p.n_kv, p.head_dim, TK, p.type);
-    if (!rc) rc = encode(f, &m[2], p.v, p.v_ld, p.v_hs, p.R, p.n_kv, p.head_dim, TK / 4, p.type);
+    if (!rc) rc = encode(f, &m[1], p.k, p.k_ld, p.k_hs, p.R, p.n_kv, p.head_dim, p.head_dim == 256 ? Geo<256>::TK : Geo<128>::TK, p.type);
+    if (!rc) rc = encode(f, &m[2], p.v, p.v_ld, p.v_hs, p.R, p.n_kv, p.head_dim, p.head_dim == 256 ? Geo<256>::VROWS : Geo<128>::VROWS, p.type);
     if (rc) return rc;
     PromptArgs a; a.row_start = p.row_start; a.S = p.S; a.R = p.R; a.max_rows = p.max_rows; a.n_head = p.n_head; a.n_kv = p.n_kv; a.G = p.n_head / p.n_kv; a.scale2 = (float)((double)p.scale * 1.4426950408889634074);
     a.q = p.q; a.k = p.k; a.v = p.v; a.q_ld = p.q_ld; a.q_hs = p.q_hs; a.k_ld = p.k_ld; a.k_hs = p.k_hs; a.v_ld = p.v_ld; a.v_hs = p.v_hs;
