@@ -28,7 +28,8 @@ namespace {
 constexpr int KW = 4, KS = 16, SLOTS = 3;   // warps that share a split, keys of a slice, slots of a warp's ring
 __host__ __device__ constexpr int out_stride(int D) { return D + 4; }
 __host__ __device__ constexpr int row_bytes(int D, int KIND) { return KIND == KV_I4 ? D / 2 : D; }                       // codes of a row
-__host__ __device__ constexpr int slot_bytes(int D, int KIND) { return KS * (row_bytes(D, KIND) + (KIND == KV_I4 ? D / 32 : 0)); }   // 4 bits: codes, then the bytes of the groups
+__host__ __device__ constexpr int code_bytes(int D, int KIND) { return KS * (row_bytes(D, KIND) + (KIND == KV_I4 ? D / 32 : 0)); }   // of a slice; 4 bits: codes, then the bytes of the groups
+__host__ __device__ constexpr int slot_bytes(int D, int KIND) { return code_bytes(D, KIND) + 2 * KS * 4; }                            // and, beside a slice's k, its scales of k and of v
 __host__ __device__ constexpr int smem_bytes(int D, int KIND, int NT) {   // fragments of q | rings; the outputs of the warps pass through the same memory at the end
     const int run = NT * D * 32 + KW * SLOTS * slot_bytes(D, KIND), end = KW * NT * 8 * out_stride(D) * 4;
     return run > end ? run : end;
@@ -64,7 +65,7 @@ template <int D, int KIND, bool V> __device__ __forceinline__ int place_of(int r
 // grid (splits, n_kv, blocks), four warps; NT sets of 8 pairs. DIRECT: the only split there is writes the outputs itself
 template <int D, int KIND, int NT, bool DIRECT>
 __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : (D == 256 ? 3 : 4)) k_paged_split(const PagedArgs a) {
-    constexpr int RB = row_bytes(D, KIND), SLOT = slot_bytes(D, KIND), CPR = RB / 16, MB = 8 * NT, XS = out_stride(D);   // 16-byte pieces of a row
+    constexpr int RB = row_bytes(D, KIND), SLOT = slot_bytes(D, KIND), SCALES = code_bytes(D, KIND), CPR = RB / 16, MB = 8 * NT, XS = out_stride(D);   // 16-byte pieces of a row
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ float s_c[MB];   // factor of a pair's scores
     __shared__ int s_pos[MB];   // position of a pair's row, -1: none
@@ -80,16 +81,17 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     const Span sp = span_of(a, blk);
     const int kh = blockIdx.y;
     if (sp.u0 >= sp.kend && !DIRECT) return;   // direct: rows without a key are zeros
-    // slices of 16 keys [i * 16, i * 16 + 16): those of this warp leave remainder `warp`; first visible one at or behind i
-    const int i_end = (int)((sp.u1 + KS - 1) / KS), i_lo = sp.lo / KS;
-    auto first_from = [&](int i) {
-        if (i * KS >= sp.sink && i < i_lo) i += (i_lo - i + KW - 1) / KW * KW;
-        return i;
-    };
+    // slices of 16 keys [i * 16, i * 16 + 16): those of this warp leave remainder `warp`. Visible are those in front of the end of the first tokens and those from the window's first key on: two runs, na
+    // slices from ia and the others from ib. A split has 1024 keys at most: 16 slices per warp
+    const int i_end = (int)((sp.u1 + KS - 1) / KS), i_lo = sp.lo / KS, i_first = (int)(sp.u0 / KS);
     {   // is any slice of the split visible?
-        const int i0 = (int)(sp.u0 / KS);
-        if ((i0 * KS >= sp.sink && i0 < i_lo ? i_lo : i0) >= i_end && !DIRECT) return;
+        if ((i_first * KS >= sp.sink && i_first < i_lo ? i_lo : i_first) >= i_end && !DIRECT) return;
     }
+    const int ia = i_first + ((warp - i_first) & (KW - 1)), a_end = min(i_end, sp.sink / KS + (sp.sink % KS != 0)), na = max(0, (a_end - ia + KW - 1) / KW);
+    int ib = max(ia + na * KW, i_lo);
+    ib += (warp - ib) & (KW - 1);
+    const int n_slices = na + max(0, (i_end - ib + KW - 1) / KW);
+    auto slice = [&](int t) { return t < na ? ia + t * KW : ib + (t - na) * KW; };
     // q: a warp per pair, 8 dims per lane; under way while the pages are looked up
     constexpr int QP = MB / KW;
     float4 qv[QP][2];
@@ -103,13 +105,13 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         }
     }
     const int lg = a.pool.lg_page, pmask = (1 << lg) - 1;
-    // the pool's row of a slice's first key; 0 behind the end, and for a page number out of range (told by the status word). The number is fetched a slice ahead
-    auto id_of = [&](int i) -> int { return i < i_end ? paged_id(a.pool, sq.s, (i * KS) >> lg) : 0; };
-    auto row_of = [&](int i, int id) -> uint32_t {
-        if (i >= i_end) return 0u;
-        const uint32_t r = paged_row_of(a.pool, id, kh, a.arg_err);
-        return r == 0xffffffffu ? 0u : r + (uint32_t)((i * KS) & pmask);
-    };
+    // the pool's rows of the warp's slices' first keys, a slice per lane; 0 for a page number out of range (told by the status word)
+    uint32_t where = 0;
+    if (lane < n_slices) {
+        const int i = slice(lane);
+        const uint32_t r = paged_row(a.pool, sq.s, (i * KS) >> lg, kh, a.arg_err);
+        where = r == 0xffffffffu ? 0u : r + (uint32_t)((i * KS) & pmask);
+    }
     uint8_t* const ring = sm + NT * D * 32 + warp * (SLOTS * SLOT);
     const uint32_t ring_u = smem_u32(ring);
     // A slot's 16 rows are one run of memory; piece e = 32 i + lane of it goes to place(e / CPR, e % CPR), which is 512 i and a part that repeats after two (k) or four (v) i
@@ -121,9 +123,13 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         vput[i] = place_of<D, KIND, true>(e / CPR, e % CPR) - 512 * i;
     }
     const uint8_t* const kbase = a.pool.k + lane * 16; const uint8_t* const vbase = a.pool.v + lane * 16;
-    auto fetch_k = [&](int slot, uint32_t row, bool live) {
-        if (live) {
+    // slice t's k and scales, its v
+    const float* const sbase = (lane < 16 ? a.pool.k_scale : a.pool.v_scale) + (lane & 15);   // scales of k in lanes 0 to 15, of v in the others
+    auto fetch_k = [&](int slot, int t) {
+        const uint32_t row = __shfl_sync(0xffffffffu, where, t & 31);
+        if (t < n_slices) {
             const uint8_t* src;
+            cp_async4(ring + slot * SLOT + SCALES + lane * 4, sbase + row);
             if constexpr (KIND == KV_I4) {
                 const I4Row at = i4_row(row, lg, D);
                 src = kbase + at.codes;
@@ -135,8 +141,9 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto fetch_v = [&](int slot, uint32_t row, bool live) {
-        if (live) {
+    auto fetch_v = [&](int slot, int t) {
+        const uint32_t row = __shfl_sync(0xffffffffu, where, t & 31);
+        if (t < n_slices) {
             const uint32_t at = ring_u + slot * SLOT, d[4] = {at + vput[0], at + vput[1], at + vput[2], at + vput[3]};
             const uint8_t* src;
             if constexpr (KIND == KV_I4) {
@@ -149,15 +156,8 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    int i0 = first_from((int)(sp.u0 / KS) + ((warp - (int)(sp.u0 / KS)) & (KW - 1)));   // this slice, the next ones and where they lie
-    int i1 = first_from(i0 + KW), i2 = first_from(i1 + KW);
-    const int id0 = id_of(i0), id1 = id_of(i1);
-    int id2 = id_of(i2);
-    uint32_t r0 = row_of(i0, id0), r1 = row_of(i1, id1);
-    fetch_k(0, r0, i0 < i_end); fetch_v(1, r0, i0 < i_end); fetch_k(2, r1, i1 < i_end);
-    const float* const sbase = (lane < 16 ? a.pool.k_scale : a.pool.v_scale) + (lane & 15);   // scales of k in lanes 0 to 15, of v in the others
-    auto scales = [&](uint32_t r) { return sbase[r]; };
-    float sc = i0 < i_end ? scales(r0) : 0.f;
+#pragma unroll
+    for (int m = 0; m < SLOTS; ++m) { if (m & 1) fetch_v(m, m / 2); else fetch_k(m, m / 2); }   // k and v in turn
 
     // the 8 dims of a lane are its words of two steps of 16 dims, values and rests; 4 bits: dims i and i + 4 side by side, at the step and the four lanes that the word of codes falls to
 #pragma unroll
@@ -212,13 +212,14 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
 #pragma unroll
     for (int i = 0; i < 4; ++i) vofs[i >> 1][i & 1] = KIND == KV_I4 ? place4<D, true>(2 * q4 + (i >> 1), g / (256 / D)) + g % (256 / D) * (D / 16) : (i & 1) < D / 64 ? place<D, true>(2 * q4 + (i >> 1), 4 * (i & 1) + (g >> 1)) + (g & 1) * 8 : 0;   // 4 bits: D / 8 dims from D / 8 * g on
     int slot = 0;
-    for (; i0 < i_end; ) {
-        const float sc1 = i1 < i_end ? scales(r1) : 0.f;
-        const uint32_t r2 = row_of(i2, id2);
-        const int i3 = first_from(i2 + KW);
-        id2 = id_of(i3);
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
+    constexpr int AHEAD = SLOTS / 2;   // slices of v; k is fetched one further
+#pragma unroll 1
+    for (int t = 0; t < n_slices; ++t) {
+        const int i0 = slice(t);
+        asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 1) : "memory");
         __syncwarp();
+        const float* const sc = reinterpret_cast<const float*>(ring + slot * SLOT + SCALES);
+        const float k0 = sc[g], k1 = sc[g + 8], v0 = sc[g + 16], v1 = sc[g + 24];
         // ---- scores of 16 keys
         float s[NT][4];
         {
@@ -270,31 +271,36 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
                 for (int c = 0; c < 4; ++c) s[n][c] = (sh[n][0][c] + sh[n][1][c]) + sl[n][c];
         }
         __syncwarp();
-        fetch_v(slot, r1, i1 < i_end);
+        fetch_v(slot, t + AHEAD);
         slot = slot + 1 == SLOTS ? 0 : slot + 1;
         // ---- weights
-        const float k0 = __shfl_sync(0xffffffffu, sc, g), k1 = __shfl_sync(0xffffffffu, sc, g + 8), v0 = __shfl_sync(0xffffffffu, sc, g + 16), v1 = __shfl_sync(0xffffffffu, sc, g + 24);
         const float lv0 = scale_lg2(v0), lv1 = scale_lg2(v1);
         const int j = i0 * KS + g;
         const bool whole = i0 * KS + KS - 1 <= all_hi && (i0 * KS > all_lo || i0 * KS + KS <= sp.sink);
-        bool hide[NT][4];
-        float d[NT][4], top = -INFINITY;
-        if (whole) {
+        uint32_t hidden = 0;   // a bit per score; most slices have none
+        if (!whole) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) hide[n][c] = false;
-        } else {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) { const int key = c < 2 ? j : j + 8, p = pos[n][c & 1]; hide[n][c] = !(key <= p && (key > p - win || key < sp.sink)); }
+                for (int c = 0; c < 4; ++c) { const int key = c < 2 ? j : j + 8, p = pos[n][c & 1]; hidden |= (uint32_t)!(key <= p && (key > p - win || key < sp.sink)) << (4 * n + c); }
         }
-        auto distance = [&](int n, int c) { return hide[n][c] ? -INFINITY : fmaf(s[n][c], (c < 2 ? k0 : k1) * cf[n][c & 1], -mu[n][c & 1]); };
+        float d[NT][4], top = -INFINITY;
+        auto distance = [&](int n, int c) { return fmaf(s[n][c], (c < 2 ? k0 : k1) * cf[n][c & 1], -mu[n][c & 1]); };
+        auto hide = [&](float none) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) if (hidden >> (4 * n + c) & 1) d[n][c] = none;
+        };
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) { d[n][c] = distance(n, c); top = fmaxf(top, d[n][c] + (c < 2 ? lv0 : lv1)); }
+            for (int c = 0; c < 4; ++c) d[n][c] = distance(n, c);
+        if (!whole) hide(-INFINITY);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) top = fmaxf(top, d[n][c] + (c < 2 ? lv0 : lv1));
         if (__any_sync(0xffffffffu, top > MU_LIMIT)) {   // rare behind the first slices. A pair moves by its own keys alone, and by the very sums that brought the warp here: others, rounded elsewhere, would move it only beside a pair that moves
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -313,25 +319,27 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) d[n][c] = cut_off(distance(n, c), c < 2 ? lv0 : lv1);
+            if (!whole) hide(-INFINITY);
         }
         uint32_t bh[NT][2], br[NT][2];   // weights times scales of v as columns of pairs: values and rests
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float y[4];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const float e0 = ex2(d[n][c]), e1 = ex2(d[n][c + 2]);
                 l[n][c] = l[n][c] + (e0 + e1);
-                y[c] = hide[n][c] ? 0.f : e0 * v0; y[c + 2] = hide[n][c + 2] ? 0.f : e1 * v1;   // a masked key's scale may be anything
+                d[n][c] = e0 * v0; d[n][c + 2] = e1 * v1;
             }
+        if (!whole) hide(0.f);   // a masked key's scale may be anything
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const __half2 hh = __floats2half2_rn(y[2 * c], y[2 * c + 1]);
+                const __half2 hh = __floats2half2_rn(d[n][2 * c], d[n][2 * c + 1]);
                 const float2 f = __half22float2(hh);
-                bh[n][c] = transpose8(h2_bits(hh)); br[n][c] = transpose8(h2_bits(__floats2half2_rn(y[2 * c] - f.x, y[2 * c + 1] - f.y)));
+                bh[n][c] = transpose8(h2_bits(hh)); br[n][c] = transpose8(h2_bits(__floats2half2_rn(d[n][2 * c] - f.x, d[n][2 * c + 1] - f.y)));
             }
-        }
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 1) : "memory");
         __syncwarp();
         // ---- outputs: 64 dims at a time; the 8 dims of a lane group are four tiles of 16 rows
         {
@@ -339,6 +347,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             auto products = [&](float (&o)[NT][4], const uint32_t (&af)[4]) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
+if constexpr (KIND == KV_I4) { mma_f16(o[n], af, br[n][0], br[n][1]); mma_f16(o[n], af, bh[n][0], bh[n][1]); continue; }   // a step 2^-23 of the sums per slice at most, 16 slices of a warp: b256 below 114 us, 107 so
                     float f[4];
                     mma_f16_first(f, af, br[n][0], br[n][1]);
                     mma_f16(f, af, bh[n][0], bh[n][1]);
@@ -389,9 +398,8 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             }
         }
         __syncwarp();
-        fetch_k(slot, r2, i2 < i_end);
+        fetch_k(slot, t + AHEAD + 1);
         slot = slot + 1 == SLOTS ? 0 : slot + 1;
-        i0 = i1; i1 = i2; i2 = i3; r1 = r2; sc = sc1;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -638,11 +646,11 @@ int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams
     const Plan pl = plan_of(pool, b, p.n_head, p.window, p.n_sink, p.cap);
     HP_REQUIRE(pl.blocks <= 65535 && pool.n_kv <= 65535 && (long long)b.R * p.n_head < (1ll << 31), "attn_paged: too many rows (%d) or heads for one call", b.R);
     PagedArgs a; a.pool = pool; a.b = b; a.q = p.q; a.q_ld = p.q_ld; a.q_hs = p.q_hs; a.n_head = p.n_head; a.G = p.n_head / pool.n_kv;
-    a.scale2 = (float)((double)p.scale * 1.4426950408889634074 * (pool.kind == KV_E4M3 ? 256.0 : 1.0)); a.window = p.window; a.n_sink = p.n_sink;
+    a.scale2 = (float)((double)p.scale * 1.4426950408889634074 * (pool.kind == KV_E4M3 ? 256.0 : pool.kind == KV_I4 ? (double)I4_UNIT : 1.0)); a.window = p.window; a.n_sink = p.n_sink;
     a.U = pl.U; a.ns = pl.ns; a.nwin = pl.nwin;
     a.pO = (float*)p.workspace; a.pml = (float2*)(a.pO + partials(pl, b, p.n_head) * pool.head_dim); a.err = device_err_flag(); a.arg_err = device_arg_flag();
     a.f16 = (uint8_t*)p.workspace + (partials(pl, b, p.n_head) * (pool.head_dim + 2) * sizeof(float) + 127) / 128 * 128; a.tiles = 0;
-    a.gate = p.gate; a.g_ld = p.g_ld; a.g_hs = p.g_hs; a.mul = pool.kind == KV_E4M3 ? 256.f : 1.f; a.out = p.out; a.oq = (int8_t*)p.xq.q; a.osc = (float*)p.xq.sc;
+    a.gate = p.gate; a.g_ld = p.g_ld; a.g_hs = p.g_hs; a.mul = pool.kind == KV_E4M3 ? 256.f : pool.kind == KV_I4 ? I4_UNIT : 1.f; a.out = p.out; a.oq = (int8_t*)p.xq.q; a.osc = (float*)p.xq.sc;
     const bool wide = (((uintptr_t)p.gate | (uintptr_t)p.out) & 15) == 0 && (!p.gate || ((p.g_ld | p.g_hs) & 3) == 0);   // four dims of gate and output at a time
     // One split: its kernel writes the outputs, for the price of a merge's launch (captured and host's time of 32 tokens of 32 heads over 8 at 256 tokens 14.6 and 9.9 us, now 8.6 and 7.3)
     a.direct = wide && pl.ns + pl.nwin == 1;

@@ -322,16 +322,17 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
             const int i = i0 + u * 256, hv = i / (RB * CPR), c = i % CPR;
             const uint32_t ws[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
             uint4* dst = reinterpret_cast<uint4*>((hv & 1 ? vo : ko) + (size_t)(r0 + i / CPR % RB) * row_stride + (size_t)(hv >> 1) * head_stride + c * PIECE);
+            const float s = KIND == KV_E4M3 ? sc[u] * 256.f : sc[u];   // code_pair gives e4m3 codes times 2^-8; 4 bits: I4_UNIT times the number first, since the scale may be too large for it
             auto scaled = [](uint32_t pr, float s) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pr));
+                float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pr));
+                if constexpr (KIND == KV_I4) { f.x = f.x * I4_UNIT; f.y = f.y * I4_UNIT; }
                 return h2_bits(__floats2half2_rn(f.x * s, f.y * s));
             };
             if constexpr (KIND == KV_I4) {
                 const I4Group g = i4_group(__byte_perm(group[u], 0x64u, 0x4040));
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { const uint4 o = i4_word(ws[j], g); dst[j] = make_uint4(scaled(o.x, sc[u]), scaled(o.y, sc[u]), scaled(o.z, sc[u]), scaled(o.w, sc[u])); }
+                for (int j = 0; j < 4; ++j) { const uint4 o = i4_word(ws[j], g); dst[j] = make_uint4(scaled(o.x, s), scaled(o.y, s), scaled(o.z, s), scaled(o.w, s)); }
             } else {
-                const float s = KIND == KV_I8 ? sc[u] : sc[u] * 256.f;   // code_pair gives e4m3 codes times 2^-8
                 uint32_t o[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = scaled(j & 1 ? code_pair<KIND, 2>(ws[j / 2]) : code_pair<KIND, 0>(ws[j / 2]), s);

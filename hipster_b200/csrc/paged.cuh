@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t paged_row(const PagedPool& p, int s, int col
 // ---- attention: what its two kernels (attn_paged.cu, attn_paged_tc.cu) share
 struct PagedArgs {
     PagedPool pool; PagedBatch b;
-    const float* q; size_t q_ld, q_hs; int n_head, G; float scale2;   // scale2 = scale * log2 e (times 256 for e4m3)
+    const float* q; size_t q_ld, q_hs; int n_head, G; float scale2;   // scale2 = scale * log2 e (times 256 for e4m3, 4096 for 4 bits)
     int window, n_sink;
     int U, ns, nwin;            // keys of a split, splits of the first tokens, splits behind them
     float* pO; float2* pml;     // partials [row][head][ns + nwin] (x head_dim): sums, (mu, sum of weights)
@@ -102,19 +102,20 @@ __device__ __forceinline__ I4Row i4_row(uint32_t row, int lg, int D) {
     const size_t page = (size_t)(row - in) * (size_t)(17 * D / 32);
     return I4Row{page + in * (uint32_t)(D / 2), page + ((size_t)(D / 2) << lg) + in * (uint32_t)(D / 32)};
 }
-// A group's byte, or those of two tokens, as two f16: 1024 + z, u, -(64 + z) u; all exact. `two`: 0x6400 + byte in both halves
-struct I4Group { __half2 z, u, n; };
+// Codes become f16 by one mask and one fma each: at bits 0 to 3 of a half c is the subnormal c 2^-24, at bits 4 to 7 c 2^-20, and times u 2^12, or u 2^8, minus z u 2^-12 that is u (c - z) 2^-12, exactly. The
+// factor 2^12 is made up for where the scales are (I4_UNIT). Of a group's byte, or of those of two tokens: both factors and the subtrahend. `two`: 0x6400 + byte in both halves
+constexpr float I4_UNIT = 4096.f;
+struct I4Group { __half2 low, high, n; };
 __device__ __forceinline__ __half2 bits_h2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 __device__ __forceinline__ I4Group i4_group(uint32_t two) {
+    const __half2 z = __hsub2(bits_h2((two & 0x000f000fu) | 0x64006400u), __floats2half2_rn(1024.f, 1024.f)), u = __hsub2(bits_h2((two & 0x00f000f0u) | 0x54005400u), __floats2half2_rn(64.f, 64.f));
     I4Group g;
-    g.z = bits_h2((two & 0x000f000fu) | 0x64006400u);
-    g.u = __hsub2(bits_h2((two & 0x00f000f0u) | 0x54005400u), __floats2half2_rn(64.f, 64.f));
-    g.n = __hmul2(__hsub2(__floats2half2_rn(960.f, 960.f), g.z), g.u);
+    g.low = __hmul2(u, __floats2half2_rn(4096.f, 4096.f)); g.high = __hmul2(u, __floats2half2_rn(256.f, 256.f));
+    g.n = __hmul2(__hmul2(z, __floats2half2_rn(-1.f / 4096.f, -1.f / 4096.f)), u);
     return g;
 }
-// Codes at bits 0 to 3 of both halves of w, at bits 4 to 7: as low bits of 1024 + c the difference and the product are exact, as bits 4 to 7 of 64 + c a single fma is: (64 + c) u is below 2048
-__device__ __forceinline__ uint32_t i4_low(uint32_t w, const I4Group& g) { return h2_bits(__hmul2(__hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), g.z), g.u)); }
-__device__ __forceinline__ uint32_t i4_high(uint32_t w, const I4Group& g) { return h2_bits(__hfma2(bits_h2((w & 0x00f000f0u) | 0x54005400u), g.u, g.n)); }
+__device__ __forceinline__ uint32_t i4_low(uint32_t w, const I4Group& g) { return h2_bits(__hfma2(bits_h2(w & 0x000f000fu), g.low, g.n)); }
+__device__ __forceinline__ uint32_t i4_high(uint32_t w, const I4Group& g) { return h2_bits(__hfma2(bits_h2(w & 0x00f000f0u), g.high, g.n)); }
 // the 8 dims of a word in order
 __device__ __forceinline__ uint4 i4_word(uint32_t w, const I4Group& g) {
     const uint32_t a = i4_low(w, g), b = i4_high(w, g), c = i4_low(w >> 8, g), d = i4_high(w >> 8, g);   // dims (0, 4), (1, 5), (2, 6), (3, 7)
