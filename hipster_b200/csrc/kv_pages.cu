@@ -79,6 +79,8 @@ template <int KIND> __device__ __forceinline__ uint32_t kv_code(float x) {
     if constexpr (KIND == KV_I8) return (uint32_t)min(127, max(-127, __float2int_rn(x))) & 0xffu;
     else return (uint32_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
 }
+__device__ __forceinline__ float max_nan(float a, float b) { float y; asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }
+__device__ __forceinline__ float min_nan(float a, float b) { float y; asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }
 // A head's norm (nw = nullptr: none) and rotation (n_rot = 0: none) where D / 8 lanes hold 8 neighbouring dims each; cs: angles of the lane's elements, interleaved of its four pairs; row: D floats of
 // shared memory of these lanes
 template <int D>
@@ -188,20 +190,20 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
                                                                                             : p.v + (size_t)r * p.v_ld + (size_t)(h - p.n_head - pool.n_kv) * p.v_hs;
         next[0] = reinterpret_cast<const float4*>(from + d0)[0]; next[1] = reinterpret_cast<const float4*>(from + d0)[1];
     };
+    RowPos at;
+    float2 cs[8];
+    bool placed = true;
+    if constexpr (AXES) {   // under way while the sequence is looked up
+        placed = row_pos(at, axes, r, p.n_pos);
+        if (placed && d0 < p.n_rot) angles(cs, p.rope, at, axes, p.n_rot, p.interleaved, d0);
+    }
     const PagedSeq q = paged_find(b, r, lane, err);
     if (q.s < 0) return;
     if (h0 < h1) fetch(h0);   // a row of a sequence, and no other, is read
     const int pos = paged_place(q, r);
-    RowPos at;
-    if constexpr (AXES) {
-        if (!row_pos(at, axes, r, p.n_pos) || (unsigned)pos >= (unsigned)b.max_kv) { paged_bad(err); return; }
-    } else if ((unsigned)pos >= (unsigned)min(b.max_kv, p.n_pos)) { paged_bad(err); return; }
+    if (!placed || (unsigned)pos >= (unsigned)(AXES ? b.max_kv : min(b.max_kv, p.n_pos))) { paged_bad(err); return; }
     const uint32_t page = h1 > p.n_head ? paged_row(pool, q.s, pos >> pool.lg_page, 0, err) : 0u;
-    float2 cs[8];
-    if (d0 < p.n_rot) {
-        if constexpr (AXES) angles(cs, p.rope, at, axes, p.n_rot, p.interleaved, d0);
-        else angles(cs, p.rope, pos, p.n_rot, p.interleaved, d0);
-    }
+    if (!AXES && d0 < p.n_rot) angles(cs, p.rope, pos, p.n_rot, p.interleaved, d0);
 #pragma unroll 1
     for (int h = h0; h < h1; h += HPS) {
         float x[8] = {next[0].x, next[0].y, next[0].z, next[0].w, next[1].x, next[1].y, next[1].z, next[1].w};
@@ -213,26 +215,20 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
             o[0] = make_float4(x[0], x[1], x[2], x[3]); o[1] = make_float4(x[4], x[5], x[6], x[7]);
             continue;
         }
-        // largest magnitude, over the bit patterns: an infinity or a NaN wins, and the token is then marked by a NaN scale over codes of zero
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
-#pragma unroll
-        for (int off = LPH / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(mask, m, off));
-        if (page == 0xffffffffu) continue;
-        const bool finite = m < 0x7f800000u;
-        const size_t at_row = (size_t)page + ((size_t)hh << pool.lg_page) + (pos & ((1 << pool.lg_page) - 1));
         if constexpr (KIND == KV_I4) {
-            // A group spans lo to hi, zero among them, in 15 steps of scale * u; halves, since hi - lo may pass the largest number. The largest span of the head has u = 15
+            // A group spans lo to hi, zero among them, in 15 steps of scale * u; halves, since hi - lo may pass the largest number. The largest span of the head has u = 15. Infinities and NaN stay in spans, and
+            // the token is then marked by a NaN scale over codes of zero
             float lo = 0.f, hi = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { lo = fminf(lo, x[j]); hi = fmaxf(hi, x[j]); }
+            for (int j = 0; j < 8; ++j) { lo = min_nan(lo, x[j]); hi = max_nan(hi, x[j]); }
 #pragma unroll
-            for (int off = 1; off < 4; off <<= 1) { lo = fminf(lo, __shfl_xor_sync(mask, lo, off)); hi = fmaxf(hi, __shfl_xor_sync(mask, hi, off)); }
+            for (int off = 1; off < 4; off <<= 1) { lo = min_nan(lo, __shfl_xor_sync(mask, lo, off)); hi = max_nan(hi, __shfl_xor_sync(mask, hi, off)); }
             const float span = 0.5f * hi - 0.5f * lo;
             float most = span;
 #pragma unroll
-            for (int off = LPH / 2; off >= 4; off >>= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, off));
+            for (int off = LPH / 2; off >= 4; off >>= 1) most = max_nan(most, __shfl_xor_sync(mask, most, off));
+            if (page == 0xffffffffu) continue;
+            const bool finite = most < INFINITY;
             const float scale = finite ? __fdiv_rn(most, 112.5f) : __uint_as_float(0x7fc00000u);
             uint32_t w = 0, group = 0;
             if (finite && scale > 0.f) {
@@ -240,19 +236,42 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
                 const float step = scale * ratio;
                 if (step > 0.f) {
                     const float inv = __fdiv_rn(1.f, step);
-                    const bool near = inv < INFINITY;   // a step below 2^-128 has no reciprocal in 32 bits
-                    const float z = fminf(rintf(near ? -lo * inv : __fdiv_rn(-lo, step)), 15.f);
+                    int z;
+                    if (inv < INFINITY) {   // rounded by adding 1.5 * 2^23: the whole number is in the low bits, as a difference of bit patterns
+                        constexpr float BIG = 12582912.f;
+                        const int unit = __float_as_int(BIG);
+                        z = min(15, __float_as_int(-lo * inv + BIG) - unit);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) w |= (uint32_t)fminf(fmaxf(rintf(near ? x[j] * inv : __fdiv_rn(x[j], step)) + z, 0.f), 15.f) << (4 * j);
+                        for (int j = 0; j < 8; ++j) w += (uint32_t)max(0, min(15, __float_as_int(x[j] * inv + BIG) + (z - unit))) << (4 * j);
+                    } else {   // a step below 2^-128 has no reciprocal in 32 bits
+                        z = (int)fminf(rintf(__fdiv_rn(-lo, step)), 15.f);
+#pragma unroll 1
+                        for (int j = 0; j < 8; ++j) {
+                            float y = 0.f;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) if (e == j) y = x[e];
+                            w |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(y, step)) + (float)z, 0.f), 15.f) << (4 * j);
+                        }
+                    }
                     group = (uint32_t)z | (uint32_t)ratio << 4;
                 }
             }
+            const size_t at_row = (size_t)page + ((size_t)hh << pool.lg_page) + (pos & ((1 << pool.lg_page) - 1));
             const I4Row to = i4_row((uint32_t)at_row, pool.lg_page, D);
             uint8_t* const base = kind == 1 ? pool.k : pool.v;
             *reinterpret_cast<uint32_t*>(base + to.codes + d0 / 2) = w;
             if (d0 % 32 == 0) base[to.groups + d0 / 32] = (uint8_t)group;
             if (d0 == 0) (kind == 1 ? pool.k_scale : pool.v_scale)[at_row] = scale;
         } else {
+            // largest magnitude, over the bit patterns: an infinity or a NaN wins, and the token is then marked by a NaN scale over codes of zero
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+#pragma unroll
+            for (int off = LPH / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(mask, m, off));
+            if (page == 0xffffffffu) continue;
+            const bool finite = m < 0x7f800000u;
+            const size_t at_row = (size_t)page + ((size_t)hh << pool.lg_page) + (pos & ((1 << pool.lg_page) - 1));
             const float scale = finite ? __fdiv_rn(__uint_as_float(m), KIND == KV_I8 ? 127.f : 448.f) : __uint_as_float(0x7fc00000u);
             const bool live = finite && scale > 0.f;
             const float inv = live ? __fdiv_rn(1.f, scale) : 0.f;
@@ -276,7 +295,7 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
 // tokens are runs of 2 KB), with one piece in flight per thread 88; 4096 tokens of 4 x 256 7.4 us.
 template <int D, int KIND, int RB>
 __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, __half* __restrict__ ko, __half* __restrict__ vo, size_t row_stride, size_t head_stride, int* err) {
-    constexpr int PIECE = KIND == KV_I4 ? 32 : 16, CPR = D / PIECE, PER = RB / 8;   // 16 bytes of codes: 4 bits, a group
+    constexpr int PIECE = KIND == KV_I4 ? 8 : 16, CPR = D / PIECE, PER = RB / 8;   // codes of a thread's piece
     __shared__ uint32_t base[RB];   // of head 0
     pdl_launch_dependents();
     pdl_wait();
@@ -299,28 +318,28 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
     }
     __syncthreads();
     const int n = 2 * pool.n_kv * RB * CPR;
-    for (int i0 = threadIdx.x; i0 < n; i0 += 4 * 256) {   // four pieces of a thread in flight
-        uint4 w[4]; float sc[4]; uint32_t row[4], group[4];
+    constexpr int FLY = KIND == KV_I4 ? 8 : 4;   // pieces of a thread in flight
+    for (int i0 = threadIdx.x; i0 < n; i0 += FLY * 256) {
+        uint4 w[FLY]; float sc[FLY]; uint32_t row[FLY], group[FLY];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < FLY; ++u) {
             const int i = i0 + u * 256, hv = i / (RB * CPR), c = i % CPR;
             row[u] = i < n ? base[i / CPR % RB] : 0xffffffffu;
             if (row[u] != 0xffffffffu) {
                 const size_t at = (size_t)row[u] + ((size_t)(hv >> 1) << pool.lg_page);
                 const uint8_t* const from = hv & 1 ? pool.v : pool.k;
-                if constexpr (KIND == KV_I4) {
+                if constexpr (KIND == KV_I4) {   // a word of codes: 16 bytes of the output per lane
                     const I4Row at4 = i4_row((uint32_t)at, pool.lg_page, D);
-                    w[u] = *reinterpret_cast<const uint4*>(from + at4.codes + c * 16);
-                    group[u] = from[at4.groups + c];
+                    w[u].x = *reinterpret_cast<const uint32_t*>(from + at4.codes + c * 4);
+                    group[u] = from[at4.groups + c / 4];
                 } else w[u] = *reinterpret_cast<const uint4*>(from + at * D + c * 16);
                 sc[u] = (hv & 1 ? pool.v_scale : pool.k_scale)[at];
             }
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < FLY; ++u) {
             if (row[u] == 0xffffffffu) continue;
             const int i = i0 + u * 256, hv = i / (RB * CPR), c = i % CPR;
-            const uint32_t ws[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
             uint4* dst = reinterpret_cast<uint4*>((hv & 1 ? vo : ko) + (size_t)(r0 + i / CPR % RB) * row_stride + (size_t)(hv >> 1) * head_stride + c * PIECE);
             const float s = KIND == KV_E4M3 ? sc[u] * 256.f : sc[u];   // code_pair gives e4m3 codes times 2^-8; 4 bits: I4_UNIT times the number first, since the scale may be too large for it
             auto scaled = [](uint32_t pr, float s) {
@@ -329,10 +348,10 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
                 return h2_bits(__floats2half2_rn(f.x * s, f.y * s));
             };
             if constexpr (KIND == KV_I4) {
-                const I4Group g = i4_group(__byte_perm(group[u], 0x64u, 0x4040));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { const uint4 o = i4_word(ws[j], g); dst[j] = make_uint4(scaled(o.x, s), scaled(o.y, s), scaled(o.z, s), scaled(o.w, s)); }
+                const uint4 o = i4_word(w[u].x, i4_group(__byte_perm(group[u], 0x64u, 0x4040)));
+                dst[0] = make_uint4(scaled(o.x, s), scaled(o.y, s), scaled(o.z, s), scaled(o.w, s));
             } else {
+                const uint32_t ws[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
                 uint32_t o[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = scaled(j & 1 ? code_pair<KIND, 2>(ws[j / 2]) : code_pair<KIND, 0>(ws[j / 2]), s);
@@ -391,16 +410,17 @@ __global__ void __launch_bounds__(256, 4) k_rope_rows(RopeRowsParams p, RopeAxes
     }
 }
 
-// One set of heads per warp while all of them fit on the GPU at once; six beyond. One and six, us: 256 rows of 48 heads of 128 6.7 and 7.9, 512 10.3 and 10.5, 1024 17.5 and 12.0, 4096 63 and 40; of 32
-// heads of 256 512 rows 12.5 and 13.0, 1024 21.9 and 20.8; of 24 heads of 64 1024 rows 6.7 and 8.0, 4096 17.5 and 13.0
+// One set of heads per warp while all of them fit on the GPU at once; eight beyond: what a warp does once per row (its sequence, its place, its angles) takes as long as some three sets. One, six and eight, us: 8 bits, 256
+// rows of 48 heads of 128 6.7, 7.9 and -, 512 10.3, 10.5, -, four prompts of up to 1000 -, 32.1, 30.6; 4 bits with three axes, 2503 rows 62, 37, 34.5. Rows that stay rows, enough of them for a warp each: all of a row, up to 24 sets
+// (8403 rows of 48 heads of 128: 64.7 with eight, 59.9)
 struct Cut { int hpw; unsigned blocks; };
-Cut cut_heads(long long R, int heads, int D) {
-    const int HPS = 32 / (D / 8), hpw = R * heads <= 148 * 64 * HPS ? 1 : 6;
+Cut cut_heads(long long R, int heads, int D, bool stay) {
+    const int HPS = 32 / (D / 8), sets = (heads + HPS - 1) / HPS, hpw = R * heads <= 148 * 64 * HPS ? 1 : stay && R >= 148 * 32 ? std::min(sets, 24) : 8;
     return Cut{hpw, (unsigned)((R * ((heads + hpw * HPS - 1) / (hpw * HPS)) + 7) / 8)};
 }
 template <int D, int KIND> int launch_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, const RopeAxes& axes, cudaStream_t s) {
     int* err = device_arg_flag();
-    const Cut c = cut_heads(b.R, p.n_head + 2 * pool.n_kv, D);
+    const Cut c = cut_heads(b.R, p.n_head + 2 * pool.n_kv, D, false);
     HP_CUDA(launch_pdl<4>(axes.pos ? k_kv_append<D, KIND, true> : k_kv_append<D, KIND, false>, dim3(c.blocks), dim3(256), 0, s, pool, b, p, axes, c.hpw, err));
     return HP_OK;
 }
@@ -409,7 +429,7 @@ template <int KIND> int launch_append(const PagedPool& pool, const PagedBatch& b
 }
 template <typename T> int launch_rows(const RopeRowsParams& p, const RopeAxes& axes, cudaStream_t s) {
     int* err = device_arg_flag();
-    const Cut c = cut_heads(p.R, p.heads[0] + p.heads[1] + p.heads[2], p.head_dim);
+    const Cut c = cut_heads(p.R, p.heads[0] + p.heads[1] + p.heads[2], p.head_dim, true);
     HP_CUDA(launch_pdl<4>(p.head_dim == 256 ? k_rope_rows<256, T> : p.head_dim == 128 ? k_rope_rows<128, T> : k_rope_rows<64, T>, dim3(c.blocks), dim3(256), 0, s, p, axes, c.hpw, err));
     return HP_OK;
 }

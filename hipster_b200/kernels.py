@@ -331,14 +331,14 @@ _OUT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 def rope_rows(q=None, k=None, v=None, rope=None, positions=None, axes=None, interleaved=False, q_norm=None, k_norm=None, eps=1e-6, dtype=torch.float16):
     """Rows of a prompt, f32 q [R][n_head][head_dim], k and v [R][n_kv][head_dim] (each may be None), as attn_prompt takes them: per head RMSNorm of q and k (q_norm, k_norm bf16 [head_dim], or None),
     rotation by rope f32 [n_pos][n_rot / 2][2] at positions int32 [axes][R] (or [R]), the axis of each pair in axes (rope_axes), rounded to dtype (float16, bfloat16, float32). -> q, k, v"""
+    fast = tensors()
+    if fast:
+        out = fast.rope_rows(q, k, v, rope, positions, axes, interleaved, q_norm, k_norm, eps, _OUT.get(dtype, -1))
+        if out is not None:
+            return out
     given = [t for t in (q, k, v) if t is not None]
     if not given or dtype not in _OUT or any(t.dim() != 3 for t in given):
         raise HipsterError(1, "rope_rows: q, k and v are [R][heads][head_dim]; outputs are float16, bfloat16 or float32")
-    fast = tensors()
-    if fast:
-        out = fast.rope_rows(q, k, v, rope, positions, axes, interleaved, q_norm, k_norm, eps, _OUT[dtype])
-        if out is not None:
-            return out
     R, _, D = given[0].shape
     dev = given[0].get_device()
     if dev != _device():
