@@ -224,13 +224,40 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
         for (int i = 0; i < TQ / 32; ++i) x.odd[i] = 0;
         fence_barrier_init();
     }
+    __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
     const int head = blockIdx.x % a.n_head;
     const QBlock b = find_rows(a, blockIdx.x / a.n_head, lane);
     if (b.s < 0) return;
     const int kh = head / a.G, q0 = b.i * TQ, tiles = (min(q0 + TQ, b.T) + G::TK - 1) / G::TK;   // q0: first row of the block in its sequence
-    if (warp == 4) {   // behind the wait: a CTA that waits holds no accumulator memory
+    auto fetch_q = [&] {
+        mbar_expect_tx(smem_u32(&x.q_full), TQ * D * 2);
+#pragma unroll
+        for (int i = 0; i < G::PARTS; ++i) tma3(base + G::OFF_Q + i * (TQ * 128), &mq, i * 64, head, b.row0 + q0, smem_u32(&x.q_full));
+    };
+    auto fetch_k = [&](int n, int p) {
+        const int bar = n % G::ST * G::KP + p;
+        const uint32_t full = smem_u32(&x.k_full[bar]), dst = base + G::OFF_K + n % G::ST * G::TILE + p * G::K_PART;
+        mbar_expect_tx(full, G::K_PART);
+#pragma unroll
+        for (int i = 0; i < G::PARTS / G::KP; ++i) tma3(dst + i * G::K_GROUP, &mk, (p * (G::PARTS / G::KP) + i) * 64, kh, b.row0 + n * G::TK, full);
+    };
+    auto fetch_v = [&](int n, int p) {
+        const int bar = n % G::ST * G::VP + p;
+        const uint32_t full = smem_u32(&x.v_full[bar]), dst = base + G::OFF_V + n % G::ST * G::TILE + p * G::V_PART;
+        mbar_expect_tx(full, G::V_PART);
+#pragma unroll
+        for (int i = 0; i < G::PARTS; ++i) tma3(dst + i * (G::VROWS * 128), &mv, i * 64, kh, b.row0 + n * G::TK + p * G::VROWS, full);
+    };
+    // the first copies are under way while accumulator memory is taken (behind the dependency wait: a CTA that waits holds none)
+    constexpr int W_FETCH = G::COPIER ? 6 : 4;
+    if (warp == W_FETCH && tc_elect()) {
+        fetch_q();
+        for (int p = 0; p < G::KP; ++p) fetch_k(0, p);
+    }
+    __syncwarp();
+    if (warp == 5) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&x.tmem)), "n"(G::TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -246,7 +273,8 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
         const uint32_t at = tmem + ((uint32_t)warp << 21);
         const float c = a.scale2;
         float mu = MU_NONE, l = 0.f;
-        bool there = false, far = false;   // scores of the next tile; a row of the warp has a reference from 2^26 on
+        auto take = [&](int n) { return take_out<D, T>(sm + G::OFF_V + n % G::ST * G::TILE, x.v_full + n % G::ST * G::VP, x.odd + (n * TK - q0) / 32, n / G::ST & 1, tid, a.err); };
+        bool ready = false, far = false;   // scores of the next tile; a row of the warp has a reference from 2^26 on
         if (a.gate && q0 + row < b.T) {   // this row's gates on their way to L2, lines of 128 bytes
             const float* const g = a.gate + (size_t)(b.row0 + q0 + row) * a.g_ld + (size_t)head * a.g_hs;
 #pragma unroll
@@ -255,7 +283,8 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
 #pragma unroll 1
         for (int n = 0; n < tiles; ++n) {
             const uint32_t sc = at + G::T_S + (n & 1) * TK;
-            if (!__all_sync(0xffffffffu, there)) ok = ok && warp_wait(smem_u32(&x.s_full[n & 1]), n >> 1 & 1, a.err);
+            if (!n && TK - 1 > q0) ok = take(0) && ok;   // of the first tile while its scores are formed
+            if (!__all_sync(0xffffffffu, ready)) ok = ok && warp_wait(smem_u32(&x.s_full[n & 1]), n >> 1 & 1, a.err);
             if (!ok) break;
             tc_fence_after();
             float s[TK];
@@ -304,13 +333,13 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
 #pragma unroll
                 for (int i = 0; i < TK; i += 2) { float2 d = make_float2(-mu, -mu); fma2(d, make_float2(s[i], s[i + 1]), make_float2(c, c)); s[i] = d.x; s[i + 1] = d.y; }
             }
-            if (hides) ok = take_out<D, T>(sm + G::OFF_V + n % G::ST * G::TILE, x.v_full + n % G::ST * G::VP, x.odd + (n * TK - q0) / 32, n / G::ST & 1, tid, a.err) && ok;
+            if (hides && n) ok = take(n) && ok;
             // weights of 32 keys are handed over as soon as they are there: their products run under the next ones' exponentials
             float2 l2 = make_float2(0.f, 0.f);
 #pragma unroll
             for (int p = 0; p < G::HAND; ++p) {
                 constexpr int KEYS = TK / G::HAND;
-                if (p == G::HAND - 1) there = n + 1 < tiles && mbar_test(smem_u32(&x.s_full[(n + 1) & 1]), (n + 1) >> 1 & 1);   // an answer takes some 200 clocks
+                if (p == G::HAND - 1) ready = n + 1 < tiles && mbar_test(smem_u32(&x.s_full[(n + 1) & 1]), (n + 1) >> 1 & 1);   // an answer takes some 200 clocks
 #pragma unroll
                 for (int i = p * KEYS; i < p * KEYS + KEYS; i += 16) {
                     uint32_t w[8];
@@ -331,71 +360,83 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
             if (!ok) break;
         }
         // ---- outputs
+        const int there = min(32, b.T - q0 - 32 * warp);   // rows of this warp
+        float4 g[16];   // gates of 64 dims of every second row, under way before they are needed
+        auto gates = [&](int i) {
+            const float* const from = a.gate + (size_t)(b.row0 + q0 + 32 * warp + lane / 16) * a.g_ld + (size_t)head * a.g_hs + i + lane % 16 * 4;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) g[j] = 2 * j + lane / 16 < there ? *reinterpret_cast<const float4*>(from + (size_t)(2 * j) * a.g_ld) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        if (a.gate) gates(0);
         ok = ok && warp_wait(smem_u32(&x.pv_done), (tiles - 1) & 1, a.err);
         tc_fence_after();
         asm volatile("bar.sync 1, 128;" ::: "memory");   // odd[] of all four warps, which all come here
         // 64 dims at a time through shared memory, which nothing else uses any more: a thread has a row, and 16 lanes write one
         if (ok) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            const int there = min(32, b.T - q0 - 32 * warp);   // rows of this warp
             if (x.odd[0] | x.odd[1] | x.odd[2] | x.odd[3]) put_in<D, T>(a, x.odd, b.row0 + q0, row, lane < there, head, kh, c, mu, at + G::T_O);
             float* const pass = reinterpret_cast<float*>(sm) + warp * (32 * PASS);
+            // Short loops: this runs once per block, from a cold instruction cache
+            if (!a.gate && !a.oq) {   // 16 bits through shared memory, rows of 144 bytes; 8 lanes write a row
+                const int r = b.row0 + q0 + 32 * warp + lane / 8;
+                T* to = (T*)a.out + ((size_t)r * a.n_head + head) * D + lane % 8 * 8;
 #pragma unroll 1
-            for (int i = 0; i < D; i += 64) {
-                float o[64];
-                ld32(o, at + G::T_O + i); ld32(o + 32, at + G::T_O + i + 32); ld_wait<64>(o);
-                __syncwarp();
+                for (int i = 0; i < D; i += 64, to += 64) {
+                    float o[64];
+                    ld32(o, at + G::T_O + i); ld32(o + 32, at + G::T_O + i + 32); ld_wait<64>(o);
+                    __syncwarp();
 #pragma unroll
-                for (int e = 0; e < 64; e += 4) *reinterpret_cast<float4*>(pass + lane * PASS + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
-                __syncwarp();
-                // 16 lanes write a row, every second one theirs. Short loops: this runs once per block, from a cold instruction cache
-                const int d = i + lane % 16 * 4, r = b.row0 + q0 + 32 * warp, j0 = lane / 16;
-                float* const mine = pass + d - i;
-                if (a.gate) {   // all of a chunk's gates are under way before the first is used
-                    const float* const gate = a.gate + (size_t)(r + j0) * a.g_ld + (size_t)head * a.g_hs + d;
-                    float4 g[16];
+                    for (int e = 0; e < 64; e += 8)
+                        *reinterpret_cast<uint4*>(pass + lane * 36 + e / 2) = make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv), pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
+                    __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) if (2 * j + j0 < there) g[j] = *reinterpret_cast<const float4*>(gate + (size_t)(2 * j) * a.g_ld);
+                    for (int j = 0; j < 8; ++j)
+                        if (4 * j + lane / 8 < there) *reinterpret_cast<uint4*>(to + (size_t)(4 * j) * a.n_head * D) = *reinterpret_cast<const uint4*>(pass + (4 * j + lane / 8) * 36 + lane % 8 * 4);
+                }
+            } else {
+                // 16 lanes have a row, every second one theirs
+                const int d0 = lane % 16 * 4, r = b.row0 + q0 + 32 * warp, j0 = lane / 16;
+                float* const mine = pass + d0;
+#pragma unroll 1
+                for (int i = 0; i < D; i += 64) {
+                    const int d = i + d0;
+                    float o[64];
+                    ld32(o, at + G::T_O + i); ld32(o + 32, at + G::T_O + i + 32); ld_wait<64>(o);
+                    __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (2 * j + j0 < there) {
-                            float4* const y = reinterpret_cast<float4*>(mine + (2 * j + j0) * PASS);
-                            *y = make_float4(y->x * sigmoid16(g[j].x), y->y * sigmoid16(g[j].y), y->z * sigmoid16(g[j].z), y->w * sigmoid16(g[j].w));
+                    for (int e = 0; e < 64; e += 4) *reinterpret_cast<float4*>(pass + lane * PASS + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+                    __syncwarp();
+                    if (a.gate) {   // all rows at once, those that are not there too: a row after the other would wait for each
+                        float4 y[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) y[j] = *reinterpret_cast<const float4*>(mine + (2 * j + j0) * PASS);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) y[j] = make_float4(y[j].x * sigmoid16(g[j].x), y[j].y * sigmoid16(g[j].y), y[j].z * sigmoid16(g[j].z), y[j].w * sigmoid16(g[j].w));
+                        if (i + 64 < D) gates(i + 64);
+                        if (a.out) {
+                            T* const to = (T*)a.out + ((size_t)(r + j0) * a.n_head + head) * D + d;
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) if (2 * j + j0 < there) *reinterpret_cast<uint2*>(to + (size_t)(2 * j) * a.n_head * D) = make_uint2(pack2<T>(y[j].x, y[j].y), pack2<T>(y[j].z, y[j].w));
                         }
-                }
-                if (a.out) {
-                    T* to = (T*)a.out + ((size_t)(r + j0) * a.n_head + head) * D + d;
+                        if (a.oq) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) *reinterpret_cast<float4*>(mine + (2 * j + j0) * PASS) = y[j];
+                        }
+                    } else if (a.out) {
+                        T* to = (T*)a.out + ((size_t)(r + j0) * a.n_head + head) * D + d;
 #pragma unroll 4
-                    for (int j = j0; j < there; j += 2, to += 2 * (size_t)a.n_head * D) {
-                        const float4 y = *reinterpret_cast<const float4*>(mine + j * PASS);
-                        *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+                        for (int j = j0; j < there; j += 2, to += 2 * (size_t)a.n_head * D) {
+                            const float4 y = *reinterpret_cast<const float4*>(mine + j * PASS);
+                            *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+                        }
                     }
-                }
-                if (a.oq)
+                    if (a.oq)
 #pragma unroll 1
-                    for (int j = j0; j < there; j += 2) quant_four(*reinterpret_cast<const float4*>(mine + j * PASS), r + j, head * D + d, a.n_head * D, a.oq, a.osc);
+                        for (int j = j0; j < there; j += 2) quant_four(*reinterpret_cast<const float4*>(mine + j * PASS), r + j, head * D + d, a.n_head * D, a.oq, a.osc);
+                }
             }
         }
     } else {   // ---- products and copies: K and scores in one warp, V and outputs in another, so that neither waits for what the other one waits for
-        auto fetch_q = [&] {
-            mbar_expect_tx(smem_u32(&x.q_full), TQ * D * 2);
-#pragma unroll
-            for (int i = 0; i < G::PARTS; ++i) tma3(base + G::OFF_Q + i * (TQ * 128), &mq, i * 64, head, b.row0 + q0, smem_u32(&x.q_full));
-        };
-        auto fetch_k = [&](int n, int p) {
-            const int bar = n % G::ST * G::KP + p;
-            const uint32_t full = smem_u32(&x.k_full[bar]), dst = base + G::OFF_K + n % G::ST * G::TILE + p * G::K_PART;
-            mbar_expect_tx(full, G::K_PART);
-#pragma unroll
-            for (int i = 0; i < G::PARTS / G::KP; ++i) tma3(dst + i * G::K_GROUP, &mk, (p * (G::PARTS / G::KP) + i) * 64, kh, b.row0 + n * G::TK, full);
-        };
-        auto fetch_v = [&](int n, int p) {
-            const int bar = n % G::ST * G::VP + p;
-            const uint32_t full = smem_u32(&x.v_full[bar]), dst = base + G::OFF_V + n % G::ST * G::TILE + p * G::V_PART;
-            mbar_expect_tx(full, G::V_PART);
-#pragma unroll
-            for (int i = 0; i < G::PARTS; ++i) tma3(dst + i * (G::VROWS * 128), &mv, i * 64, kh, b.row0 + n * G::TK + p * G::VROWS, full);
-        };
         if (warp < 6 && tc_elect()) {
             constexpr uint32_t TYPE = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
             constexpr uint32_t ID = (1u << 4) | TYPE | ((uint32_t)(TQ >> 4) << 24), ID_S = ID | ((uint32_t)(G::TK >> 3) << 17), ID_O = ID | ((uint32_t)(D >> 3) << 17) | (1u << 16);   // O: V is N-major
@@ -443,8 +484,7 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
             } else {   // a stage is fetched again when the products of the tile that it held are through
                 uint64_t *const full = first ? x.k_full : x.v_full, *const empty = first ? x.k_empty : x.v_empty;
                 const int parts = first ? G::KP : G::VP;
-                int fetched = 0;   // tiles whose copies have been issued
-                if (first) fetch_q();
+                int fetched = first;   // tiles whose copies have been issued
                 for (; fetched < min(G::ST, tiles); ++fetched)
                     for (int p = 0; p < parts; ++p) { if (first) fetch_k(fetched, p); else fetch_v(fetched, p); }
                 if (first) ok = mma_wait<D>(smem_u32(&x.q_full), 0, a.err);
@@ -470,8 +510,7 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
             tc_wait(smem_u32(&fin), 0, a.err);   // nothing in flight when the accumulator memory is given back
         }
         if (G::COPIER && warp == 6 && tc_elect()) {
-            fetch_q();
-            int nk = 0, nv = 0, pk = 0, pv = 0;   // tile and part next to be fetched
+            int nk = 1, nv = 0, pk = 0, pv = 0;   // tile and part next to be fetched
             uint32_t idle = 0;
             while ((nk < tiles || nv < tiles) && idle < (1u << 23)) {
                 ++idle;
@@ -500,7 +539,7 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(G::TMEM) : "memory");
+    if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(G::TMEM) : "memory");
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
