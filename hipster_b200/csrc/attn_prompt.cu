@@ -1,16 +1,24 @@
 // Causal attention of whole prompts, packed one behind the other, with grouped heads, in f16 or bf16: o_i = sum_{j <= i} w_ij v_j / sum_{j <= i} w_ij, w_ij =
 // 2^(q_i . k_j * scale * log2 e - mu_i), times sigmoid(gate). No cache: a prompt sees its own keys and values as they are, not what a cache of few bits makes of them.
 //
-// A CTA has 128 rows of one sequence and query head, and goes through its keys in tiles of 128, the tile of its own rows last: the only one with hidden keys. Warps:
+// A CTA has 128 rows of one sequence and query head and goes through their keys in tiles of 64 (256 dims: 128), its own rows' last: hidden keys lie in these alone. Warps:
 //   weights (four warps, a thread per row): S of a tile into registers, the row's largest score, weights in 16 bits in place of the scores, the outputs at the end
-//   products (one thread): S[128 rows][128 keys] = Q K^T with both from shared memory, O[128 rows][dims] += W V with W from accumulator memory
-//   copies (one thread): K in parts of 64 dims, V in parts of 32 keys, each of them fetched again as soon as its products are through
-// Up to 128 dims take half of the accumulator memory and of shared memory: two CTAs per SM, one's weights under the other's products. 256 dims take an SM, with two tiles of scores.
+//   scores (one thread): S[128 rows][keys] = Q K^T from shared memory, a tile ahead of the weights; K's copies (tensor maps; 64 dims of 128 bytes to a row, 128-byte swizzle)
+//   outputs (one thread): O[128 rows][dims] += W V with W from accumulator memory; V's copies
+// Up to 128 dims take half of the accumulator memory and of shared memory: two CTAs per SM. 256 dims take an SM; K is fetched in parts of 64 dims and V in parts of 32 keys, each again as soon as its products are through.
 // A row's reference mu moves when a logarithm passes it by more than MU_STEP, so the sums are rescaled rarely (by the row's own thread); weights reach 2^MU_STEP at most. Sums of weights are fp32 of the
 // weights before they are rounded to 16 bits: that rounding is at most half a step of the outputs' own type per weight.
 //
-// A value that is infinite or NaN must not reach the rows in front of it through a weight of zero. Hidden keys lie in the last tile alone: its values are looked at there, such elements are taken out
-// (and noted), and the rows that see them get their weight times that element at the end.
+// A value that is infinite or NaN must not reach the rows in front of it through a weight of zero: in the tiles with hidden keys such elements are taken out of shared memory (and noted) before the products, and the rows that see them
+// get their weight times that element at the end.
+//
+// Measured (captured, back to back; cuBLAS' sustained rate is 1402 TFLOP/s): 8190 rows of 24 heads of 256 690 us, 1.19 PFLOP/s, at 1.44 GHz under the power limit (1560 us of 16384 rows of 16 heads after a pause, 1.41 PFLOP/s; 1790 back to
+// back). 16384 rows of 16 heads of 128 1060 us, 1.04 PFLOP/s at 1.6 GHz, of 64 800 us, 0.69 at 1.93. Bounds: 256 dims shared memory (320 KB per tile of 128 keys of 2048 clocks of products) and power; 128 and 64 the weights' warps, two
+// per scheduler, some 1300 clocks per 64 keys each. Seven prompts of up to 3001 rows of 32 heads of 128 264 to 295 us (by card): of a CTA's 37000 clocks 6000 pass before its first scores are there, 2700 with its outputs. Five gated
+// prompts of up to 77 rows of 24 heads of 256 14.9 us: latency, the gates' sigmoids last.
+// Tried: one warp for both products 1119 us at 128 dims where two take 1080 (a wait that is over still takes 250 clocks, and an output waited behind the next scores'); waits that ask without a pause in those warps: they take the
+// issue slots of the weights' warp beside them (2360 -> 3440 clocks per tile); a quarter, a half of the exponentials as polynomials on the fp32 pipe: 1732 -> 1762, 1802 us at 256 dims, 819 -> 827, 892 at 64 (instructions, not the
+// special functions, bound them); outputs unrolled over a row: 14800 clocks instead of 5800, cold instructions.
 #include "paged.cuh"
 #include "tc.cuh"
 #include <algorithm>
@@ -325,10 +333,11 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
                     st_wait();
                 }
             }
-            // distances from the reference. Logarithms from 2^26 on lie in steps of 8: there the product is rounded as it was for the reference
+            // distances from the reference. Logarithms from 2^26 on lie in steps of 8: there the product is rounded as it was for the reference, in the rows that have such a one
             if (far) {
+                const bool own = fabsf(mu) >= 67108864.f;
 #pragma unroll
-                for (int i = 0; i < TK; ++i) s[i] = s[i] * c - mu;
+                for (int i = 0; i < TK; ++i) s[i] = own ? s[i] * c - mu : fmaf(s[i], c, -mu);
             } else {
 #pragma unroll
                 for (int i = 0; i < TK; i += 2) { float2 d = make_float2(-mu, -mu); fma2(d, make_float2(s[i], s[i + 1]), make_float2(c, c)); s[i] = d.x; s[i + 1] = d.y; }

@@ -178,6 +178,19 @@ def test_keys_and_queries_that_are_not_finite(D, at):
     assert torch.equal(got[keep], clean[keep]) and status() == 0
 
 
+@pytest.mark.parametrize("kind,up", [("f16", 200.0), ("bf16", 1e12)])
+@pytest.mark.parametrize("D", [64, 256])
+def test_a_row_with_scores_of_another_size_leaves_its_neighbours_as_they_were(D, kind, up):
+    """Queries so large that a row's scores pass 2^26, where the kernel rounds otherwise: rows beside it, and their bits in 32-bit sums, know nothing of it."""
+    q, k, v = make([150], 2, 1, D, kind, 8, packed=False)
+    k[:, 0, 0] = 300
+    clean, xc = K_.attn_prompt(q, k, v, i32([0, 150]), max_rows=150, want_q8=True)
+    q[77, 0, 0] = 300 * up
+    got, xq = K_.attn_prompt(q, k, v, i32([0, 150]), max_rows=150, want_q8=True)
+    keep = [i for i in range(150) if i != 77]
+    assert torch.equal(got[keep], clean[keep]) and all(torch.equal(a[keep], b[keep]) for a, b in zip(xq.unpack(), xc.unpack())) and torch.isfinite(got[77]).all() and status() == 0
+
+
 def test_another_prompts_non_finite_rows_do_not_count():
     """Tiles reach over a prompt's end into the next one's rows, and past the last row of the buffers."""
     rows = [50, 200, 10]

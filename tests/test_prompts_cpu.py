@@ -90,6 +90,7 @@ def test_bad_prompts():
     refused(prompt(n_kv=0), "n_head")
     for kw in (dict(S=0), dict(R=0), dict(max_rows=0)):
         refused(prompt(**kw), "bad batch")
+    refused(prompt(S=65536), "bad batch")
     for kw in (dict(q=(None, 256, 64)), dict(k=(None, 128, 64)), dict(v=(None, 128, 64)), dict(rs=None), dict(out=None)):
         refused(prompt(**kw), "null")
     refused(prompt(xq=FAKE), "both")
