@@ -34,7 +34,7 @@ constexpr float MU_STEP = 8.f;
 constexpr int PASS = 68;            // floats of a row of 64 outputs on their way out: 16-byte pieces of 8 rows hit distinct banks
 
 struct PromptArgs {
-    const int* row_start; int S, R, max_rows, n_head, n_kv, G; float scale2;   // scale * log2 e
+    const int* row_start; int S, R, max_rows, order, n_head, n_kv, G; float scale2;   // scale * log2 e
     const void *q, *k, *v; size_t q_ld, q_hs, k_ld, k_hs, v_ld, v_hs;          // as the tensor maps have them
     const float* gate; size_t g_ld, g_hs; void* out; int8_t* oq; float* osc; int* err; int* arg_err;
 };
@@ -111,8 +111,11 @@ template <typename T> __device__ __forceinline__ bool odd16(uint32_t b) { conste
 // the top bits of both halves: set where the half is infinite or NaN, its exponent plus one
 template <typename T> __device__ __forceinline__ uint32_t odd_pair(uint32_t w) { constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u, ONE = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u; return (w & E) + ONE; }
 
-// The block of 128 rows that number `blk` stands for: those with most keys first, whatever sequence they belong to. Blocks i of a sequence (rows from 128 i on): F(i) = sum_s max(0, n_s - i) blocks have number
-// i or more in a sequence of n_s; the largest i with F(i) > blk is the block's, and blk - F(i + 1) counts the sequences that have an i-th one.
+// The block of 128 rows that number `blk` stands for, in one of three ways (the rule stands at the launch):
+//   GRID: i-th blocks of all sequences (rows from 128 i on) behind the later ones of all. Nothing to look for, and a number per sequence and i, most of them for nothing where lengths differ
+//   SORTED: the same order without gaps. F(i) = sum_s max(0, n_s - i) blocks have number i or more in a sequence of n_s; the largest i with F(i) > blk is the block's, and blk - F(i + 1) counts the sequences that have an i-th one
+//   ALONG: one sequence behind the other. Sequence s has the numbers from row_start[s] / 128 + s on, which is room enough for its blocks; s by 32 questions at a time. The first CTA sees whether all sequences are as they should be
+enum : int { GRID, SORTED, ALONG };
 struct QBlock { int s, row0, T, i; };
 __device__ __forceinline__ QBlock find_rows(const PromptArgs& a, int blk, int lane) {
     auto seq = [&](int s, int& row0) {   // rows of sequence s, within what the call says
@@ -123,30 +126,36 @@ __device__ __forceinline__ QBlock find_rows(const PromptArgs& a, int blk, int la
         return T;
     };
     QBlock o{-1, 0, 0, 0};
-    if (a.S == 1) { o.T = seq(0, o.row0); o.i = (o.T + TQ - 1) / TQ - 1 - blk; o.s = o.i < 0 ? -1 : 0; return o; }
-    int row0 = 0, T = 0;   // of sequence `lane`; calls of more look the others up again
+    if (a.order == GRID) {
+        const int per = (a.max_rows + TQ - 1) / TQ, s = blk % a.S;
+        o.T = seq(s, o.row0); o.i = per - 1 - blk / a.S;
+        if (o.i * TQ < o.T) o.s = s;
+        return o;
+    }
+    if (a.order == ALONG) {
+        auto first = [&](int s) { return min(max(a.row_start[s], 0), a.R) / TQ + s; };
+        int s = 0, n = a.S;   // the last one of s .. s + n - 1 with first(s) <= blk
+        while (n > 1) {
+            const int step = (n + 31) / 32, at = s + lane * step;
+            const int k = __popc(__ballot_sync(0xffffffffu, lane * step < n && first(at) <= blk)) - 1;
+            if (k < 0) return o;
+            s += k * step; n = min(step, n - k * step);
+        }
+        if (blockIdx.x == 0) for (int i = lane, r; i < a.S; i += 32) seq(i, r);
+        o.T = seq(s, o.row0); o.i = (o.T + TQ - 1) / TQ - 1 - (blk - first(s));
+        if (o.i >= 0 && blk >= first(s)) o.s = s;
+        return o;
+    }
+    int row0 = 0, T = 0;   // of sequence `lane`: 32 at most
     if (lane < a.S) T = seq(lane, row0);
-    const int n0 = (T + TQ - 1) / TQ;
-    auto from = [&](int i) {   // F(i)
-        int n = max(0, n0 - i), r;
-        for (int s = lane + 32; s < a.S; s += 32) n += max(0, (seq(s, r) + TQ - 1) / TQ - i);
-        return __reduce_add_sync(0xffffffffu, n);
-    };
+    const int n = (T + TQ - 1) / TQ;
+    auto from = [&](int i) { return __reduce_add_sync(0xffffffffu, max(0, n - i)); };   // F(i)
     int lo = 0, hi = (a.max_rows + TQ - 1) / TQ;   // F(lo) > blk >= F(hi)
     if (from(0) <= blk) return o;
     while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (from(mid) > blk) lo = mid; else hi = mid; }
-    int k = blk - from(lo + 1);
-    for (int s0 = 0; s0 < a.S; s0 += 32) {
-        if (s0) { row0 = T = 0; if (s0 + lane < a.S) T = seq(s0 + lane, row0); }
-        const unsigned has = __ballot_sync(0xffffffffu, (T + TQ - 1) / TQ > lo);
-        const int n = __popc(has);
-        if (k < n) {
-            const int l = __ffs(__ballot_sync(0xffffffffu, (has >> lane & 1) && __popc(has & ((1u << lane) - 1)) == k)) - 1;
-            o.s = s0 + l; o.row0 = __shfl_sync(0xffffffffu, row0, l); o.T = __shfl_sync(0xffffffffu, T, l); o.i = lo;
-            return o;
-        }
-        k -= n;
-    }
+    const unsigned has = __ballot_sync(0xffffffffu, n > lo);
+    const int k = blk - from(lo + 1), l = __ffs(__ballot_sync(0xffffffffu, (has >> lane & 1) && __popc(has & ((1u << lane) - 1)) == k)) - 1;
+    o.s = l; o.row0 = __shfl_sync(0xffffffffu, row0, l); o.T = __shfl_sync(0xffffffffu, T, l); o.i = lo;
     return o;
 }
 
@@ -580,14 +589,17 @@ int attn_prompt(const AttnPromptParams& p, cudaStream_t s) {
         return cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &at, 12000, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess ? (EncodeFn)at : nullptr;
     }();
     if (!f) { set_error("attn_prompt: the driver has no tensor maps"); return HP_ECUDA; }
-    const long long per = (p.max_rows + TQ - 1) / TQ, blocks = std::min<long long>((long long)p.S * per, (long long)p.R / TQ + p.S);
+    // Numbers for blocks: a CTA without one costs some 2 us of its SM, a search among 32 lengths 1000 clocks. GRID and SORTED or ALONG, us, heads of 128, 16 over 4: 24 prompts of 500 rows 66 and 71, 40 of 100 23.6 and 26.9, one
+    // of 8000 beside 39 of 100 788 and 265 (SORTED by pieces of 32 sequences 275, but 46000 for one of 4000 beside 4095 of 5, where ALONG takes 1530)
+    const long long per = (p.max_rows + TQ - 1) / TQ, most = p.S * per, least = (long long)p.R / TQ + p.S, blocks = std::min(most, least);
+    const int order = most <= least ? GRID : p.S <= 32 ? SORTED : ALONG;
     HP_REQUIRE(blocks * p.n_head < (1ll << 31), "attn_prompt: too many rows (%d) or heads for one call", p.R);
     CUtensorMap m[3];
     int rc = encode(f, &m[0], p.q, p.q_ld, p.q_hs, p.R, p.n_head, p.head_dim, TQ, p.type);
     if (!rc) rc = encode(f, &m[1], p.k, p.k_ld, p.k_hs, p.R, p.n_kv, p.head_dim, p.head_dim == 256 ? Geo<256>::TK : Geo<128>::TK, p.type);
     if (!rc) rc = encode(f, &m[2], p.v, p.v_ld, p.v_hs, p.R, p.n_kv, p.head_dim, p.head_dim == 256 ? Geo<256>::VROWS : Geo<128>::VROWS, p.type);
     if (rc) return rc;
-    PromptArgs a; a.row_start = p.row_start; a.S = p.S; a.R = p.R; a.max_rows = p.max_rows; a.n_head = p.n_head; a.n_kv = p.n_kv; a.G = p.n_head / p.n_kv; a.scale2 = (float)((double)p.scale * 1.4426950408889634074);
+    PromptArgs a; a.row_start = p.row_start; a.S = p.S; a.R = p.R; a.max_rows = p.max_rows; a.order = order; a.n_head = p.n_head; a.n_kv = p.n_kv; a.G = p.n_head / p.n_kv; a.scale2 = (float)((double)p.scale * 1.4426950408889634074);
     a.q = p.q; a.k = p.k; a.v = p.v; a.q_ld = p.q_ld; a.q_hs = p.q_hs; a.k_ld = p.k_ld; a.k_hs = p.k_hs; a.v_ld = p.v_ld; a.v_hs = p.v_hs;
     a.gate = p.gate; a.g_ld = p.g_ld; a.g_hs = p.g_hs; a.out = p.out; a.oq = (int8_t*)p.xq.q; a.osc = (float*)p.xq.sc; a.err = device_err_flag(); a.arg_err = device_arg_flag();
     return p.type == OUT_F16 ? launch<__half>(m, a, blocks, p.head_dim, s) : launch<__nv_bfloat16>(m, a, blocks, p.head_dim, s);

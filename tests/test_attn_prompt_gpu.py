@@ -265,6 +265,39 @@ def test_bad_row_starts_are_told():
     assert status() == 1
 
 
+# same lengths (a number for every block), few of very different ones, and many: blocks are counted in three ways
+@pytest.mark.parametrize("rows", [[100] * 50, [128] * 33, [130] * 20, [0, 1, 900, 3, 0, 129], [700] + [5] * 40, [5] * 40 + [700], [1, 0, 127, 128, 129, 0, 256, 257] * 9 + [1500], [0] * 100 + [300] + [0] * 100 + [2]])
+@pytest.mark.parametrize("D", [64, 256])
+def test_blocks_of_many_prompts(rows, D):
+    q, k, v = make(rows, 2, 1, D, "f16", 11, tail=3)
+    got, _ = K_.attn_prompt(q, k, v, starts(rows), max_rows=max(rows))
+    at = 0
+    for T in rows:
+        if T:
+            part = slice(at, at + T)
+            assert torch.equal(got[part], K_.attn_prompt(q[part], k[part], v[part], i32([0, T]), max_rows=T)[0]), (at, T)
+        at += T
+    assert status() == 0
+
+
+def test_bad_row_starts_among_many_prompts_are_told():
+    rows = [5] * 60 + [400]
+    q, k, v = make(rows, 2, 1, 64, "f16", packed=False)
+    good = starts(rows)
+    want, _ = K_.attn_prompt(q, k, v, good, max_rows=400)
+    assert status() == 0
+    for at, to in ((61, 701), (61, 1 << 30), (0, -1), (30, -5), (30, 1 << 30), (59, 100), (61, 1)):
+        rs = good.clone()
+        rs[at] = to
+        got, _ = K_.attn_prompt(q, k, v, rs, max_rows=400)
+        assert status() == 1, (at, to)
+        if at == 61 and to > 1:
+            assert torch.equal(got, want)
+    K_.attn_prompt(q, k, v, good, max_rows=399)
+    assert status() == 1
+    assert torch.equal(K_.attn_prompt(q, k, v, good, max_rows=400)[0], want) and status() == 0
+
+
 def test_streams_and_captures():
     rows = [300, 90]
     q, k, v = make(rows, 4, 2, 256, "f16", packed=False)
