@@ -353,6 +353,8 @@ int hp_rope_rows(const float* q_dev, long long q_ld, long long q_hs, void* q_out
         heads += n;
     }
     HP_REQUIRE(heads >= 1, "hp_rope_rows: no rows");
+    for (int i = 0; i < 3; ++i)
+        for (int j = 0; j < 3; ++j) HP_REQUIRE(i == j || !p.heads[i] || !p.heads[j] || out[i] != (const void*)in[j], "hp_rope_rows: an output in place of another one's input");
     HP_REQUIRE((long long)R * heads < (1ll << 33), "hp_rope_rows: too many rows");
     p.norm[0] = q_norm_bf16_dev; p.norm[1] = k_norm_bf16_dev; p.rope = rope_dev; p.n_pos = n_pos; p.n_rot = n_rot; p.interleaved = interleaved; p.eps = eps; p.R = R; p.head_dim = head_dim; p.type = out_type;
     return hp::rope_rows(p, axes, (cudaStream_t)stream);
@@ -413,6 +415,9 @@ int hp_attn_prompt(const void* q_dev, long long q_ld, long long q_hs, const void
     HP_REQUIRE(fits(q_dev, q_ld, q_hs, n_head) && fits(k_dev, k_ld, k_hs, n_kv) && fits(v_dev, v_ld, v_hs, n_kv), "hp_attn_prompt: rows must be 16-byte aligned, with positive strides that are multiples of 8");
     HP_REQUIRE(!gate_dev || rows_ok(gate_dev, g_ld, g_hs), "hp_attn_prompt: the gate must be 16-byte aligned, with strides that are multiples of 4");
     HP_REQUIRE(scale > 0 && scale < 1e30f, "hp_attn_prompt: bad scale");
+    for (const void* o : {(const void*)out_dev, (const void*)xq_q_dev, (const void*)xq_sc_dev})
+        HP_REQUIRE(!o || (o != q_dev && o != k_dev && o != v_dev && o != gate_dev), "hp_attn_prompt: an output in place of an input, which other rows still read");
+    HP_REQUIRE(!xq_q_dev || (xq_q_dev != xq_sc_dev && out_dev != xq_q_dev && out_dev != xq_sc_dev), "hp_attn_prompt: two outputs are the same");
     hp::AttnPromptParams p; p.q = q_dev; p.q_ld = (size_t)q_ld; p.q_hs = (size_t)q_hs; p.k = k_dev; p.k_ld = (size_t)k_ld; p.k_hs = (size_t)k_hs; p.v = v_dev; p.v_ld = (size_t)v_ld; p.v_hs = (size_t)v_hs; p.type = type;
     p.n_head = n_head; p.n_kv = n_kv; p.head_dim = head_dim; p.gate = gate_dev; p.g_ld = (size_t)g_ld; p.g_hs = (size_t)g_hs; p.row_start = row_start_dev; p.S = S; p.R = R; p.max_rows = max_rows < R ? max_rows : R; p.scale = scale;
     p.out = out_dev; p.xq = hp::XQ8F{xq_q_dev, xq_sc_dev};

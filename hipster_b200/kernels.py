@@ -303,11 +303,13 @@ def _rope_args(who, rope, positions, axes, R, dev):
         if positions is not None or axes is not None:
             raise HipsterError(1, f"{who}: positions and axes go with a rope table")
         return (None, 0, 0), (None, 0, None, 0)
-    n_pos, half, two = rope.shape
-    if not (rope.dtype is _F32 and two == 2 and rope.is_contiguous() and rope.get_device() == dev):
+    if not (rope.dtype is _F32 and rope.dim() == 3 and rope.shape[2] == 2 and rope.is_contiguous() and rope.get_device() == dev):
         raise HipsterError(1, f"{who}: rope must be f32 [n_pos][n_rot / 2][2]")
+    n_pos, half, _ = rope.shape
     if positions.dim() == 1:
         positions = positions[None]
+    if positions.dim() != 2:
+        raise HipsterError(1, f"{who}: positions must be int32 [axes][{R}] or [{R}]")
     (n_axes, cols), (ld, one) = positions.shape, positions.stride()
     if not (positions.dtype is _I32 and cols == R and (one == 1 or R == 1) and (n_axes == 1 or ld >= 0) and positions.get_device() == dev):
         raise HipsterError(1, f"{who}: positions must be int32 [axes][{R}], rows without gaps, on the device of the rows")

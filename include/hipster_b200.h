@@ -130,7 +130,7 @@ int hp_moe_layer(const float* xn_dev, const void* xq_q_dev, const void* xq_sc_de
  * HP_KV_I4 holds 4 bits: per group of 32 dims a code z of zero and a factor u, per token and head a scale; the value of a code c is scale * (u * (c - z)). With lo = min(0, x) and hi =
  * max(0, x) over a group, scale = (largest hi - lo of the head) / 225, u = ceil(15 (hi - lo) / largest) (0: all of the group is zero), z = round(-lo / (scale u)), c = round(x / (scale u)) + z in 0 .. 15: zero is
  * always held exactly, other elements to a step scale * u, half of it but at the ends of a group's range. k, v: [n_pages][n_kv][page_size * 17 * head_dim / 32] bytes: of a page and head first the codes of its tokens,
- * head_dim / 2 bytes each with the even dim in the low half, then their groups' bytes z + 16 u, head_dim / 32 each. 4.5 bits per element at 64 dims, 4.375 at 128, 4.3125 at 256, scales included (4.75, 4.5, 4.375).
+ * head_dim / 2 bytes each with the even dim in the low half, then their groups' bytes z + 16 u, head_dim / 32 each. 4.25 bits per element; with the scales 4.75 at 64 dims, 4.5 at 128, 4.375 at 256.
  *
  * hp_kv_pages describes a cache (host struct, read during the call). k, v: [n_pages][n_kv][page_size][head_dim] bytes, 16-byte aligned; k_scale, v_scale: f32
  * [n_pages][n_kv][page_size]. page_size: a power of two, 16 to 1024; head_dim: 64, 128 or 256.
@@ -172,7 +172,7 @@ int hp_kv_append_axes(const float* q_dev, long long q_ld, long long q_hs, float*
                       const int* table_dev, int table_ld, const int* row_start_dev, const int* kv_len_dev, int S, int R, const hp_kv_pages* pages, float eps, void* stream);
 /* The same norm and rotation for rows that stay rows, of q [R][n_head][head_dim], k and v [R][n_kv][head_dim] f32, v as it is, rounded to out_type: what hp_attn_prompt takes. q_dev, or k_dev, or v_dev may be NULL
  * with its output: none. n_rot = 0: no rotation (rope_dev, pos_dev, axes_host NULL, n_axes 0). A row with a position outside of the table is not written (HP_EINVAL from hp_device_status). An output may be
- * its input with the same strides where both are f32. Pointers 16-byte aligned, strides multiples of 16 bytes; outputs' rows do not lie over each other. */
+ * its input with the same strides where both are f32; otherwise outputs overlap neither inputs nor each other. Pointers 16-byte aligned, strides multiples of 16 bytes; outputs' rows do not lie over each other. */
 enum { HP_F32 = 0, HP_F16 = 1, HP_BF16 = 2 };
 int hp_rope_rows(const float* q_dev, long long q_ld, long long q_hs, void* q_out_dev, long long qo_ld, long long qo_hs, int n_head, const float* k_dev, long long k_ld, long long k_hs, void* k_out_dev, long long ko_ld, long long ko_hs,
                  const float* v_dev, long long v_ld, long long v_hs, void* v_out_dev, long long vo_ld, long long vo_hs, int n_kv, int head_dim, int out_type, const void* q_norm_bf16_dev, const void* k_norm_bf16_dev,
@@ -198,7 +198,8 @@ int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const floa
  * outputs before they are rounded (K = n_head * head_dim, buffers as hp_attn_paged has them); either may be NULL. head_dim 64, 128 or 256; n_head a multiple of n_kv. max_rows bounds a prompt's rows and sizes the launch. row_start
  * (S + 1 ints, rising; S at most 65535) is device memory, read when the kernel runs; rows behind row_start[S] are not written. What does not fit is left out and told by hp_device_status, as for the paged calls.
  * A row is not touched by infinite or NaN keys and values that it does not see; of a value that it sees, an infinite element makes the output's infinite or NaN.
- * q, k, v: 16-byte aligned, strides positive multiples of 8; gate 16-byte aligned, strides multiples of 4; out and quantised outputs 16-byte aligned. No workspace. A row's result depends on its own prompt alone. */
+ * q, k, v: 16-byte aligned, strides positive multiples of 8; gate 16-byte aligned, strides multiples of 4; out and quantised outputs 16-byte aligned. Outputs overlap neither inputs nor each other. No
+ * workspace. A row's result depends on its own prompt alone. */
 int hp_attn_prompt(const void* q_dev, long long q_ld, long long q_hs, const void* k_dev, long long k_ld, long long k_hs, const void* v_dev, long long v_ld, long long v_hs, int type, const float* gate_dev, long long g_ld, long long g_hs,
                    int n_head, int n_kv, int head_dim, const int* row_start_dev, int S, int R, int max_rows, float scale, void* out_dev, void* xq_q_dev, void* xq_sc_dev, void* stream);
 

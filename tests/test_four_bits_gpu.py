@@ -469,6 +469,7 @@ def test_refusals_of_the_python_calls(form):
     bad += [lambda: row(dtype=torch.float64), lambda: K_.rope_rows(), lambda: K_.rope_rows(x.half()), lambda: K_.rope_rows(x[0]), lambda: K_.rope_rows(x, k=x[:1]), lambda: K_.rope_rows(x, k=x[:, :2], v=x[:, :1]), lambda: K_.rope_rows(x[..., :32]),
             lambda: K_.rope_rows(x, k=x.cpu()), lambda: K_.rope_rows(x, q_norm=x[0, 0]), lambda: K_.rope_rows(x.transpose(1, 2).contiguous().transpose(1, 2)), lambda: K_.rope_rows(x[..., 1:], None, None),
             lambda: K_.rope_rows(torch.zeros((2, 4, 65), device="cuda")[..., 1:])]
+    bad += [lambda f=f, kw=kw: f(**kw) for f in (app, row) for kw in (dict(positions=pos[None]), dict(positions=pos[0, 0]), dict(rope=rope[0]), dict(rope=rope[None]))]
     for i, f in enumerate(bad):
         with pytest.raises(hb.HipsterError):
             f()

@@ -79,6 +79,8 @@ def test_bad_rows():
     refused(rows(q=(FAKE, 256, 64), qo=(FAKE, 256, 64)), "in place")
     refused(rows(kind=0, qo=(FAKE, 320, 64)), "in place")
     refused(rows(qo=(5 * FAKE, 256, 64), ko=(3 * FAKE, 128, 64)), "same")
+    refused(rows(kind=0, q=(6 * FAKE, 256, 64), ko=(6 * FAKE, 128, 64)), "another one's input")
+    refused(rows(kind=0, qo=(FAKE, 256, 64)), "another one's input")   # q, k and v in one place
 
 
 def test_bad_prompts():
@@ -102,6 +104,13 @@ def test_bad_prompts():
     refused(prompt(gate=(FAKE, 254, 64)), "gate")
     refused(prompt(scale=0.0), "scale")
     refused(prompt(scale=float("nan")), "scale")
+    there = dict(q=(2 * FAKE, 256, 64), k=(3 * FAKE, 128, 64), v=(4 * FAKE, 128, 64), gate=(5 * FAKE, 256, 64))
+    for i in (2, 3, 4, 5):
+        refused(prompt(**there, out=i * FAKE), "in place of an input")
+        refused(prompt(**there, xq=i * FAKE, sc=6 * FAKE), "in place of an input")
+        refused(prompt(**there, xq=6 * FAKE, sc=i * FAKE), "in place of an input")
+    for out, xq, sc in ((FAKE, FAKE, 6 * FAKE), (FAKE, 6 * FAKE, FAKE), (None, FAKE, FAKE)):
+        refused(prompt(**there, out=out, xq=xq, sc=sc), "same")
 
 
 def test_axes_of_pairs():
