@@ -1,22 +1,27 @@
-// Attention of a ragged batch of rows over a cache of 8-bit pages (kv_pages.cu), with a window and first tokens that stay visible: calls of up to
+// Attention of a ragged batch of rows over a cache of pages in 8 or 4 bits (kv_pages.cu), with a window and first tokens that stay visible: calls of up to
 // 16 rows per sequence (decode steps, drafts, verify passes), the merge of the splits, and the plan. Prompts: attn_paged_tc.cu.
 //
 // Row r at position p of its sequence: o = sum_j w_j v_j / sum_j w_j over the keys j <= p with j > p - window or j < n_sink (no window: all), w_j =
 // 2^(s_j - mu), s_j = (q . k_j) * scale * log2 e, times sigmoid(gate). No key: zeros.
 //
-// fp32 results from the f16 tensor pipe: codes of int8 and of e4m3 (times 2^-8) are exact in f16, a token's scale multiplies its score or its weight in
+// fp32 results from the f16 tensor pipe: codes of int8, of e4m3 (times 2^-8) and of 4 bits (u (c - z), times 2^-12) are exact in f16, a token's scale multiplies its score or its weight in
 // fp32, and q and the weights (times the scale of v) go in as two f16 each, the value and what is left of it: 22 bits. q is brought to [2^14, 2^15) by a
 // power of two per row, the weights by the reference mu, which is whole: every rescaling is by a power of two, exact (MU_TOP in paged.cuh). The tensor pipe adds up
-// head_dim / 2 products for a score, in three sums, and 16 keys for an output; these are added to the running sums in fp32.
+// head_dim / 2 products for a score, in three sums, and 16 keys for an output; these are added to the running sums in fp32 (4 bits: by the tensor pipe itself).
 //
 // Keys, and dims, are the 16 rows of mma.sync, the pairs (row of the batch, query head) of a kv head its 8 columns: few pairs waste nothing. A warp has 16 keys at a
 // time, every fourth such slice of its CTA's split, in a ring of three slots of its own (k, v, k, ...), so that no warp waits for another; 16 keys of a head
 // lie in one page, one run of memory. The weights change from rows of keys to columns of pairs by movmatrix. Splits lie at fixed positions and a
 // slice's keys at fixed lanes and warps: a row's bits depend neither on the other rows of the call nor on the other sequences.
 //
-// Measured (captured, us): one token of 24 heads of 256 over 4 at 4097 12.85 (bytes alone 1.3): start, four slices per warp and merge one after the other. 48 such sequences of up to
-// 8192 118 (80; 4.4 TB/s): issue slots 58 %, a third of the instructions turning codes into f16, DRAM 0.66 of the copy rate. 8 x 3 rows over 2 kv heads at 2051 21.8 (2.0); 32 x 2
-// rows of 32 heads of 128, window 1000, 34 (11): half of the instructions are starts and ends of the CTAs. Pairs as the 16 rows of the products: 260 for the 48 sequences; eight warps per CTA: 128.
+// A warp looks up the pages of all its slices at once, a lane each, and fetches a slice's scales with its keys; hidden keys are masked in the slices that have some.
+//
+// Measured (captured, us): one token of 24 heads of 256 over 4 at 4097 12.6 (bytes alone 1.3): start, four slices per warp and merge one after the other. 48 such sequences of up to
+// 8192 111 to 116 by card (80), 118 to 121 with the page looked up per slice and every slice masked: issue slots 58 %, a third of the instructions turning codes into f16. 8 x 3 rows over 2 kv heads at 2051 22.0 (2.0); 32 x 2
+// rows of 32 heads of 128, window 1000, 34.6 (11): half of the instructions are starts and ends of the CTAs. Pairs as the 16 rows of the products: 260 for the 48 sequences; eight warps per CTA: 128.
+// 4 bits: one token at 4097 11.8 (0.7), the 48 sequences 103 (43), 256 sequences of 32 heads of 128 over 8 at up to 4096 222 (86): issue slots 57 to 66 %, 840 instructions per slice of 256 dims, of which 192 are products
+// and their operands' rests as many again. Two dims become f16 by one mask and one fma; by two masks and conversions 129 for the 48. Products of tcgen05 with the pictures of attn_paged_tc.cu: 15.9 for one token, 180 for the 48;
+// a head's dims split over the warps, 64 keys shared by them: 13.1, 110.
 // Two sets of pairs spill up to 28 bytes a thread, one set of 256 dims 12.
 #include "paged.cuh"
 #include <algorithm>
@@ -347,7 +352,11 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             auto products = [&](float (&o)[NT][4], const uint32_t (&af)[4]) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-if constexpr (KIND == KV_I4) { mma_f16(o[n], af, br[n][0], br[n][1]); mma_f16(o[n], af, bh[n][0], bh[n][1]); continue; }   // a step 2^-23 of the sums per slice at most, 16 slices of a warp: b256 below 114 us, 107 so
+                    if constexpr (KIND == KV_I4) {   // into the running sums: a step of 2^-23 of them per slice at most, 2^-19 in a split; the 48 sequences of the head of this file 107 us so, 114 with adds of their own
+                        mma_f16(o[n], af, br[n][0], br[n][1]);
+                        mma_f16(o[n], af, bh[n][0], bh[n][1]);
+                        continue;
+                    }
                     float f[4];
                     mma_f16_first(f, af, br[n][0], br[n][1]);
                     mma_f16(f, af, bh[n][0], bh[n][1]);
