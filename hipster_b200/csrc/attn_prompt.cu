@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
     using G = Geo<D>;
     extern __shared__ uint8_t sm_raw[];
     struct Shared {
-        uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2][4], pv_done, fin[2];   // parts: stage * (KP or VP) + part
+        uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2][4], pv_done[2], fin[2];   // parts: stage * (KP or VP) + part. pv_done: of even and of odd tiles. Who waits for a tile's may be a tile ahead or behind, and a phase's bit tells only neighbours apart
         uint32_t tmem, odd[TQ / 32];   // keys of the block's own rows with an infinite or NaN value
     };
     __shared__ Shared x;
@@ -236,8 +236,7 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
     if (tid == 0) {
         mbar_init(smem_u32(&x.q_full), 1);
         for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&x.k_full[i]), 1); mbar_init(smem_u32(&x.k_empty[i]), 1); mbar_init(smem_u32(&x.v_full[i]), 1); mbar_init(smem_u32(&x.v_empty[i]), 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); for (int p = 0; p < G::HAND; ++p) mbar_init(smem_u32(&x.p_full[i][p]), 4); }
-        mbar_init(smem_u32(&x.pv_done), 1); mbar_init(smem_u32(&x.fin[0]), 1); mbar_init(smem_u32(&x.fin[1]), 1);
+        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); mbar_init(smem_u32(&x.pv_done[i]), 1); mbar_init(smem_u32(&x.fin[i]), 1); for (int p = 0; p < G::HAND; ++p) mbar_init(smem_u32(&x.p_full[i][p]), 4); }
         for (int i = 0; i < TQ / 32; ++i) x.odd[i] = 0;
         fence_barrier_init();
     }
@@ -327,7 +326,7 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
                 if (top > mu + MU_STEP) { al = ex2(mu - top); mu = top; l = l * al; }   // the first reference: 0
                 far = __any_sync(0xffffffffu, fabsf(mu) >= 67108864.f && mu != MU_NONE);
                 if (n) {
-                    ok = warp_wait(smem_u32(&x.pv_done), (n - 1) & 1, a.err);
+                    ok = warp_wait(smem_u32(&x.pv_done[(n - 1) & 1]), (n - 1) >> 1 & 1, a.err);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -386,7 +385,7 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
             for (int j = 0; j < 16; ++j) g[j] = 2 * j + lane / 16 < there ? *reinterpret_cast<const float4*>(from + (size_t)(2 * j) * a.g_ld) : make_float4(0.f, 0.f, 0.f, 0.f);
         };
         if (a.gate) gates(0);
-        ok = ok && warp_wait(smem_u32(&x.pv_done), (tiles - 1) & 1, a.err);
+        ok = ok && warp_wait(smem_u32(&x.pv_done[(tiles - 1) & 1]), (tiles - 1) >> 1 & 1, a.err);
         tc_fence_after();
         asm volatile("bar.sync 1, 128;" ::: "memory");   // odd[] of all four warps, which all come here
         // 64 dims at a time through shared memory, which nothing else uses any more: a thread has a row, and 16 lanes write one
@@ -460,7 +459,7 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
             constexpr uint32_t ID = (1u << 4) | TYPE | ((uint32_t)(TQ >> 4) << 24), ID_S = ID | ((uint32_t)(G::TK >> 3) << 17), ID_O = ID | ((uint32_t)(D >> 3) << 17) | (1u << 16);   // O: V is N-major
             const uint32_t q_desc = desc_low(base + G::OFF_Q, 16), k_desc = desc_low(base + G::OFF_K, 16), v_desc = desc_low(base + G::OFF_V, G::VROWS * 128);
             auto scores = [&](int n) {
-                if (n >= 2 && !mma_wait<D>(smem_u32(&x.pv_done), n & 1, a.err)) return false;   // the weights of n - 2, in its place, are read
+                if (n >= 2 && !mma_wait<D>(smem_u32(&x.pv_done[n & 1]), (n >> 1 & 1) ^ 1, a.err)) return false;   // the weights of n - 2, in its place, are read
                 const uint32_t st = tmem + G::T_S + (n & 1) * G::TK;
                 uint32_t qd = q_desc, kd = k_desc + n % G::ST * (G::TILE / 16);
 #pragma unroll
@@ -492,7 +491,7 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
                     for (int i = 0; i < 2; ++i) mma_ts(tmem + G::T_O, wt + 16 * i, vd + 128 * i, ID_O, i ? 1 : n | p);
                     if ((p + 1) % PER == 0) tc_commit(smem_u32(&x.v_empty[bar]));
                 }
-                tc_commit(smem_u32(&x.pv_done));
+                tc_commit(smem_u32(&x.pv_done[n & 1]));
                 return true;
             };
             const bool first = warp == 4;

@@ -298,6 +298,22 @@ def test_bad_row_starts_among_many_prompts_are_told():
     assert torch.equal(K_.attn_prompt(q, k, v, good, max_rows=400)[0], want) and status() == 0
 
 
+@pytest.mark.parametrize("D,kind", [(64, "f16"), (128, "bf16"), (256, "bf16")])
+@pytest.mark.parametrize("gated", [False, True])
+def test_many_calls_in_a_row_have_the_same_bits(D, kind, gated):
+    """Some 700 blocks a call, two to an SM where they fit, one call behind the other: products of one block wait for those of another, and no wait may take one tile's products for another's."""
+    rows = [1000, 251, 501, 751]
+    q, k, v = make(rows, 32, 8, D, kind, 31, packed=False)
+    g = torch.randn(q.shape, generator=gen(7), device="cuda") if gated else None
+    rs = starts(rows)
+    got = [K_.attn_prompt(q, k, v, rs, max_rows=1000, gate=g)[0] for _ in range(40)]
+    assert status() == 0
+    for t in got[1:]:
+        assert torch.equal(t, got[0])
+    want, tol = prompt64(q, k, v, rows, D ** -0.5, g)
+    assert ((got[0].double() - want).abs() <= tol).all()
+
+
 def test_streams_and_captures():
     rows = [300, 90]
     q, k, v = make(rows, 4, 2, 256, "f16", packed=False)
