@@ -4,7 +4,7 @@
 // A CTA has 128 rows of one sequence and query head and goes through their keys in tiles of 64 (256 dims: 128), its own rows' last: hidden keys lie in these alone. Warps:
 //   weights (four warps, a thread per row): S of a tile into registers, the row's largest score, weights in 16 bits in place of the scores, the outputs at the end
 //   scores (one thread): S[128 rows][keys] = Q K^T from shared memory, a tile ahead of the weights; K's copies (tensor maps; 64 dims of 128 bytes to a row, 128-byte swizzle)
-//   outputs (one thread): O[128 rows][dims] += W V with W from accumulator memory; V's copies
+//   outputs (one thread): O[128 rows][dims] += W V with W from accumulator memory; V's copies (256 dims: a warp of their own has all copies)
 // Up to 128 dims take half of the accumulator memory and of shared memory: two CTAs per SM. 256 dims take an SM; K is fetched in parts of 64 dims and V in parts of 32 keys, each again as soon as its products are through.
 // A row's reference mu moves when a logarithm passes it by more than MU_STEP, so the sums are rescaled rarely (by the row's own thread); weights reach 2^MU_STEP at most. Sums of weights are fp32 of the
 // weights before they are rounded to 16 bits: that rounding is at most half a step of the outputs' own type per weight.
@@ -15,7 +15,8 @@
 // Measured (captured, back to back; cuBLAS' sustained rate is 1402 TFLOP/s): 8190 rows of 24 heads of 256 690 us, 1.19 PFLOP/s, at 1.44 GHz under the power limit (1560 us of 16384 rows of 16 heads after a pause, 1.41 PFLOP/s; 1790 back to
 // back). 16384 rows of 16 heads of 128 1060 us, 1.04 PFLOP/s at 1.6 GHz, of 64 800 us, 0.69 at 1.93. Bounds: 256 dims shared memory (320 KB per tile of 128 keys of 2048 clocks of products) and power; 128 and 64 the weights' warps, two
 // per scheduler, some 1300 clocks per 64 keys each. Seven prompts of up to 3001 rows of 32 heads of 128 264 to 295 us (by card): of a CTA's 37000 clocks 6000 pass before its first scores are there, 2700 with its outputs. Five gated
-// prompts of up to 77 rows of 24 heads of 256 14.9 us: latency, the gates' sigmoids last.
+// prompts of up to 77 rows of 24 heads of 256 10.3 us: 400 KB of a CTA at some 64 bytes a clock, and latency. Gates come in place of q and k while the last weights are formed, and at 256 dims all eight warps write outputs: with gates fetched
+// into registers by the four weights' warps, a step ahead, 13.3, and 8 x 600 rows of 16 heads 92.7 instead of 78.2; without gates four warps, or eight, take the same.
 // Tried: one warp for both products 1119 us at 128 dims where two take 1080 (a wait that is over still takes 250 clocks, and an output waited behind the next scores'); waits that ask without a pause in those warps: they take the
 // issue slots of the weights' warp beside them (2360 -> 3440 clocks per tile); a quarter, a half of the exponentials as polynomials on the fp32 pipe: 1732 -> 1762, 1802 us at 256 dims, 819 -> 827, 892 at 64 (instructions, not the
 // special functions, bound them); outputs unrolled over a row: 14800 clocks instead of 5800, cold instructions.
@@ -40,17 +41,19 @@ struct PromptArgs {
 };
 
 // Tiles of TK keys in ST stages; a stage's K comes in KP parts of 64 dims or as one, its V in VP parts of 32 keys or as one. Two tiles of scores: one is formed while the other is weighed.
-template <int D> struct Geo {
+template <int D, bool GATE = false> struct Geo {
     static constexpr int TK = D == 256 ? 128 : 64, ST = D == 256 ? 1 : 2, PARTS = D / 64, KP = D == 256 ? PARTS : 1, VP = D == 256 ? 4 : 1, VROWS = TK / VP;
     static constexpr int HAND = 2;                                             // hand-overs of a tile's weights
     static constexpr int K_GROUP = TK * 128, K_PART = PARTS / KP * K_GROUP, V_PART = VROWS * D * 2, TILE = TK * D * 2;
-    static constexpr int OFF_Q = 0, OFF_K = TQ * D * 2, OFF_V = OFF_K + ST * TILE, SMEM = OFF_V + ST * TILE + 1024;   // 1024 for the alignment
+    static constexpr int OFF_Q = 0, OFF_K = TQ * D * 2, OFF_V = OFF_K + ST * TILE;
+    static constexpr int OUT_WARPS = D == 256 && GATE ? 8 : 4;   // warps that write outputs: two per quarter of the accumulator memory's lanes, or the weights' warps alone
+    static constexpr int PASSES = OUT_WARPS * 32 * PASS * 4, SMEM = OFF_V + (ST * TILE > PASSES ? ST * TILE : PASSES) + 1024;   // 1024 for the alignment. At the end gates in place of q and k, outputs on their way in place of v
     static constexpr int T_O = 0, T_S = D, TMEM = D == 256 ? 512 : 256;
     static constexpr int CTAS = D == 256 ? 1 : 2;
     // 256 dims: a warp of its own fetches whichever part is free next (copies by the products' warps: 1.76 -> 1.95 ms for 16384 rows of 16 heads). Two CTAs per SM: 224 threads would leave 128 registers each, with spills (1.04 -> 1.08 ms)
     static constexpr bool COPIER = D == 256;
-    static constexpr int THREADS = COPIER ? 224 : 192;
-    static_assert(T_S + 2 * TK <= TMEM && CTAS * SMEM <= 227 * 1024 && 4 * 32 * PASS * 4 <= SMEM - 1024, "");
+    static constexpr int THREADS = !COPIER ? 192 : GATE ? 256 : 224;
+    static_assert(T_S + 2 * TK <= TMEM && CTAS * SMEM <= 227 * 1024 && OFF_V == TQ * D * 4, "");
 };
 
 // Operands in shared memory: 128-byte swizzle, groups of 8 rows 1024 bytes apart; N-major: the next 64 elements lie `next` bytes behind. The lower half of a descriptor, to which offsets / 16 are added; the upper one is
@@ -221,12 +224,14 @@ __device__ __noinline__ void put_in(const PromptArgs& a, const uint32_t* odd, in
     }
 }
 
-template <int D, typename T>
-__global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const PromptArgs a) {
-    using G = Geo<D>;
+template <int D, typename T, bool GATE>
+__global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mg, const PromptArgs a) {
+    using G = Geo<D, GATE>;
     extern __shared__ uint8_t sm_raw[];
     struct Shared {
-        uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2][4], pv_done[2], fin[2];   // parts: stage * (KP or VP) + part. pv_done: of even and of odd tiles. Who waits for a tile's may be a tile ahead or behind, and a phase's bit tells only neighbours apart
+        uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2][4], pv_done[2], fin[2], gates;   // parts: stage * (KP or VP) + part. pv_done: of even and of odd tiles. Who waits for a tile's may be a tile ahead or behind, and a phase's bit tells only neighbours apart
+        float inv[TQ];   // of a row's sum of weights
+        int failed;
         uint32_t tmem, odd[TQ / 32];   // keys of the block's own rows with an infinite or NaN value
     };
     __shared__ Shared x;
@@ -237,6 +242,8 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
         mbar_init(smem_u32(&x.q_full), 1);
         for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&x.k_full[i]), 1); mbar_init(smem_u32(&x.k_empty[i]), 1); mbar_init(smem_u32(&x.v_full[i]), 1); mbar_init(smem_u32(&x.v_empty[i]), 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); mbar_init(smem_u32(&x.pv_done[i]), 1); mbar_init(smem_u32(&x.fin[i]), 1); for (int p = 0; p < G::HAND; ++p) mbar_init(smem_u32(&x.p_full[i][p]), 4); }
+        mbar_init(smem_u32(&x.gates), 1);
+        x.failed = 0;
         for (int i = 0; i < TQ / 32; ++i) x.odd[i] = 0;
         fence_barrier_init();
     }
@@ -281,17 +288,85 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = x.tmem;
-    bool ok = true;
+    bool ok = true, gated = false;   // gated: this warp has fetched gates
+    constexpr bool SHARED = G::OUT_WARPS == 8;
+    const int there = min(32, b.T - q0 - 32 * (warp & 3));   // rows of this warp's outputs
+    const uint32_t at = tmem + ((uint32_t)(warp & 3) << 21);
+    // Outputs, 64 dims at a time through shared memory, which nothing else uses any more: a thread has a row, and 16 lanes write one
+    auto write_outputs = [&](float inv) {
+        if (GATE && !warp_wait(smem_u32(&x.gates), 0, a.err)) return;
+        if (there <= 0) return;
+        const int from = (warp >> 2) * (D / 2), end = from + D * 4 / G::OUT_WARPS, r = b.row0 + q0 + 32 * (warp & 3);
+        float* const pass = reinterpret_cast<float*>(sm + (GATE ? G::OFF_V : 0)) + warp * (32 * PASS);
+        // Short loops: this runs once per block, from a cold instruction cache
+        if (!GATE && !a.oq) {   // 16 bits through shared memory, rows of 144 bytes; 8 lanes write a row
+            T* to = (T*)a.out + ((size_t)(r + lane / 8) * a.n_head + head) * D + from + lane % 8 * 8;
+#pragma unroll 1
+            for (int i = from; i < end; i += 64, to += 64) {
+                float o[64];
+                ld32(o, at + G::T_O + i); ld32(o + 32, at + G::T_O + i + 32); ld_wait<64>(o);
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < 64; e += 8)
+                    *reinterpret_cast<uint4*>(pass + lane * 36 + e / 2) = make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv), pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (4 * j + lane / 8 < there) *reinterpret_cast<uint4*>(to + (size_t)(4 * j) * a.n_head * D) = *reinterpret_cast<const uint4*>(pass + (4 * j + lane / 8) * 36 + lane % 8 * 4);
+            }
+        } else {
+            // 16 lanes have a row, every second one theirs
+            const int d0 = lane % 16 * 4, j0 = lane / 16;
+            float* const mine = pass + d0;
+#pragma unroll 1
+            for (int i = from; i < end; i += 64) {
+                const int d = i + d0;
+                float o[64];
+                ld32(o, at + G::T_O + i); ld32(o + 32, at + G::T_O + i + 32); ld_wait<64>(o);
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < 64; e += 4) *reinterpret_cast<float4*>(pass + lane * PASS + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+                __syncwarp();
+                if (GATE) {   // all rows at once, those that are not there too: a row after the other would wait for each
+                    const float* const g = reinterpret_cast<const float*>(sm) + (32 * (warp & 3) + j0) * D + d;
+                    float4 y[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float4 o4 = *reinterpret_cast<const float4*>(mine + (2 * j + j0) * PASS), g4 = *reinterpret_cast<const float4*>(g + 2 * j * D);
+                        y[j] = make_float4(o4.x * sigmoid16(g4.x), o4.y * sigmoid16(g4.y), o4.z * sigmoid16(g4.z), o4.w * sigmoid16(g4.w));
+                    }
+                    if (a.out) {
+                        T* const to = (T*)a.out + ((size_t)(r + j0) * a.n_head + head) * D + d;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) if (2 * j + j0 < there) *reinterpret_cast<uint2*>(to + (size_t)(2 * j) * a.n_head * D) = make_uint2(pack2<T>(y[j].x, y[j].y), pack2<T>(y[j].z, y[j].w));
+                    }
+                    if (a.oq) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) *reinterpret_cast<float4*>(mine + (2 * j + j0) * PASS) = y[j];
+                    }
+                } else if (a.out) {
+                    T* to = (T*)a.out + ((size_t)(r + j0) * a.n_head + head) * D + d;
+#pragma unroll 4
+                    for (int j = j0; j < there; j += 2, to += 2 * (size_t)a.n_head * D) {
+                        const float4 y = *reinterpret_cast<const float4*>(mine + j * PASS);
+                        *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+                    }
+                }
+                if (a.oq)
+#pragma unroll 1
+                    for (int j = j0; j < there; j += 2) quant_four(*reinterpret_cast<const float4*>(mine + j * PASS), r + j, head * D + d, a.n_head * D, a.oq, a.osc);
+            }
+        }
+    };
 
     if (warp < 4) {   // ---- weights
         constexpr int TK = G::TK;
         const int row = tid;                              // of the block
-        const uint32_t at = tmem + ((uint32_t)warp << 21);
         const float c = a.scale2;
         float mu = MU_NONE, l = 0.f;
         auto take = [&](int n) { return take_out<D, T>(sm + G::OFF_V + n % G::ST * G::TILE, x.v_full + n % G::ST * G::VP, x.odd + (n * TK - q0) / 32, n / G::ST & 1, tid, a.err); };
         bool ready = false, far = false;   // scores of the next tile; a row of the warp has a reference from 2^26 on
-        if (a.gate && q0 + row < b.T) {   // this row's gates on their way to L2, lines of 128 bytes
+        if (GATE && q0 + row < b.T) {   // this row's gates on their way to L2, lines of 128 bytes
             const float* const g = a.gate + (size_t)(b.row0 + q0 + row) * a.g_ld + (size_t)head * a.g_hs;
 #pragma unroll
             for (int i = 0; i < D; i += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(g + i));
@@ -376,83 +451,13 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
             l = l + (l2.x + l2.y);
             if (!ok) break;
         }
-        // ---- outputs
-        const int there = min(32, b.T - q0 - 32 * warp);   // rows of this warp
-        float4 g[16];   // gates of 64 dims of every second row, under way before they are needed
-        auto gates = [&](int i) {
-            const float* const from = a.gate + (size_t)(b.row0 + q0 + 32 * warp + lane / 16) * a.g_ld + (size_t)head * a.g_hs + i + lane % 16 * 4;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) g[j] = 2 * j + lane / 16 < there ? *reinterpret_cast<const float4*>(from + (size_t)(2 * j) * a.g_ld) : make_float4(0.f, 0.f, 0.f, 0.f);
-        };
-        if (a.gate) gates(0);
         ok = ok && warp_wait(smem_u32(&x.pv_done[(tiles - 1) & 1]), (tiles - 1) >> 1 & 1, a.err);
         tc_fence_after();
         asm volatile("bar.sync 1, 128;" ::: "memory");   // odd[] of all four warps, which all come here
-        // 64 dims at a time through shared memory, which nothing else uses any more: a thread has a row, and 16 lanes write one
-        if (ok) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            if (x.odd[0] | x.odd[1] | x.odd[2] | x.odd[3]) put_in<D, T>(a, x.odd, b.row0 + q0, row, lane < there, head, kh, c, mu, at + G::T_O);
-            float* const pass = reinterpret_cast<float*>(sm) + warp * (32 * PASS);
-            // Short loops: this runs once per block, from a cold instruction cache
-            if (!a.gate && !a.oq) {   // 16 bits through shared memory, rows of 144 bytes; 8 lanes write a row
-                const int r = b.row0 + q0 + 32 * warp + lane / 8;
-                T* to = (T*)a.out + ((size_t)r * a.n_head + head) * D + lane % 8 * 8;
-#pragma unroll 1
-                for (int i = 0; i < D; i += 64, to += 64) {
-                    float o[64];
-                    ld32(o, at + G::T_O + i); ld32(o + 32, at + G::T_O + i + 32); ld_wait<64>(o);
-                    __syncwarp();
-#pragma unroll
-                    for (int e = 0; e < 64; e += 8)
-                        *reinterpret_cast<uint4*>(pass + lane * 36 + e / 2) = make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv), pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
-                    __syncwarp();
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (4 * j + lane / 8 < there) *reinterpret_cast<uint4*>(to + (size_t)(4 * j) * a.n_head * D) = *reinterpret_cast<const uint4*>(pass + (4 * j + lane / 8) * 36 + lane % 8 * 4);
-                }
-            } else {
-                // 16 lanes have a row, every second one theirs
-                const int d0 = lane % 16 * 4, r = b.row0 + q0 + 32 * warp, j0 = lane / 16;
-                float* const mine = pass + d0;
-#pragma unroll 1
-                for (int i = 0; i < D; i += 64) {
-                    const int d = i + d0;
-                    float o[64];
-                    ld32(o, at + G::T_O + i); ld32(o + 32, at + G::T_O + i + 32); ld_wait<64>(o);
-                    __syncwarp();
-#pragma unroll
-                    for (int e = 0; e < 64; e += 4) *reinterpret_cast<float4*>(pass + lane * PASS + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
-                    __syncwarp();
-                    if (a.gate) {   // all rows at once, those that are not there too: a row after the other would wait for each
-                        float4 y[16];
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) y[j] = *reinterpret_cast<const float4*>(mine + (2 * j + j0) * PASS);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) y[j] = make_float4(y[j].x * sigmoid16(g[j].x), y[j].y * sigmoid16(g[j].y), y[j].z * sigmoid16(g[j].z), y[j].w * sigmoid16(g[j].w));
-                        if (i + 64 < D) gates(i + 64);
-                        if (a.out) {
-                            T* const to = (T*)a.out + ((size_t)(r + j0) * a.n_head + head) * D + d;
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) if (2 * j + j0 < there) *reinterpret_cast<uint2*>(to + (size_t)(2 * j) * a.n_head * D) = make_uint2(pack2<T>(y[j].x, y[j].y), pack2<T>(y[j].z, y[j].w));
-                        }
-                        if (a.oq) {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) *reinterpret_cast<float4*>(mine + (2 * j + j0) * PASS) = y[j];
-                        }
-                    } else if (a.out) {
-                        T* to = (T*)a.out + ((size_t)(r + j0) * a.n_head + head) * D + d;
-#pragma unroll 4
-                        for (int j = j0; j < there; j += 2, to += 2 * (size_t)a.n_head * D) {
-                            const float4 y = *reinterpret_cast<const float4*>(mine + j * PASS);
-                            *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
-                        }
-                    }
-                    if (a.oq)
-#pragma unroll 1
-                        for (int j = j0; j < there; j += 2) quant_four(*reinterpret_cast<const float4*>(mine + j * PASS), r + j, head * D + d, a.n_head * D, a.oq, a.osc);
-                }
-            }
-        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (ok && (x.odd[0] | x.odd[1] | x.odd[2] | x.odd[3])) put_in<D, T>(a, x.odd, b.row0 + q0, row, lane < there, head, kh, c, mu, at + G::T_O);
+        if constexpr (SHARED) x.inv[row] = inv;
+        else if (ok) write_outputs(inv);
     } else {   // ---- products and copies: K and scores in one warp, V and outputs in another, so that neither waits for what the other one waits for
         if (warp < 6 && tc_elect()) {
             constexpr uint32_t TYPE = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
@@ -522,9 +527,18 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
                     if (first) tc_wait(smem_u32(&x.q_full), 0, a.err);
                 }
             }
-            uint64_t& fin = x.fin[warp - 4];
-            tc_commit(smem_u32(&fin));
-            tc_wait(smem_u32(&fin), 0, a.err);   // nothing in flight when the accumulator memory is given back
+            tc_commit(smem_u32(&x.fin[warp - 4]));
+            ok = tc_wait(smem_u32(&x.fin[warp - 4]), 0, a.err) && ok;   // nothing in flight when the accumulator memory is given back
+        }
+        if (GATE && warp == 4) {   // the gates of the block's rows in place of q and k
+            ok = __all_sync(0xffffffffu, ok);
+            gated = ok;
+            if (ok && tc_elect()) {
+                const int boxes = (min(TQ, b.T - q0) + 31) / 32;
+                mbar_expect_tx(smem_u32(&x.gates), boxes * 32 * D * 4);
+                for (int i = 0; i < boxes; ++i) tma3(base + i * (32 * D * 4), &mg, 0, head, b.row0 + q0 + 32 * i, smem_u32(&x.gates));
+            }
+            __syncwarp();
         }
         if (G::COPIER && warp == 6 && tc_elect()) {
             int nk = 1, nv = 0, pk = 0, pv = 0;   // tile and part next to be fetched
@@ -553,6 +567,14 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
             }
         }
     }
+    if constexpr (SHARED) {   // all warps write
+        if (!ok) x.failed = 1;
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        if (!x.failed) write_outputs(x.inv[32 * (warp & 3) + lane]);
+    }
+    if (gated) tc_wait(smem_u32(&x.gates), 0, a.err);   // no copy outlives the CTA
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -560,24 +582,24 @@ __global__ void __launch_bounds__(Geo<D>::THREADS, Geo<D>::CTAS) k_attn_prompt(c
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-// [R][heads][D] in boxes of `rows` x 64 dims of one head. Rows behind the tensor read as zeros
+// [R][heads][D] in boxes of `rows` x 64 dims of one head (gates, f32: all dims). Rows behind the tensor read as zeros
 int encode(EncodeFn f, CUtensorMap* m, const void* p, size_t ld, size_t hs, int R, int heads, int D, int rows, int type) {
-    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)R}, strides[2] = {heads == 1 ? (cuuint64_t)D * 2 : hs * 2, R == 1 ? (cuuint64_t)D * 2 : ld * 2};
-    const cuuint32_t box[3] = {64, 1, (cuuint32_t)rows}, step[3] = {1, 1, 1};
-    const CUresult r = f(m, type == OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint64_t size = type == OUT_F32 ? 4 : 2, dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)R}, strides[2] = {(heads == 1 ? D : hs) * size, (R == 1 ? D : ld) * size};
+    const cuuint32_t box[3] = {type == OUT_F32 ? (cuuint32_t)D : 64, 1, (cuuint32_t)rows}, step[3] = {1, 1, 1};
+    const CUresult r = f(m, type == OUT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, step,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, type == OUT_F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     HP_REQUIRE(r == CUDA_SUCCESS, "attn_prompt: rows that a tensor map cannot describe (%d): ld=%zu hs=%zu", (int)r, ld, hs);
     return HP_OK;
 }
-template <int D, typename T> int launch(const CUtensorMap (&m)[3], const PromptArgs& a, long long blocks, cudaStream_t s) {
+template <int D, typename T, bool GATE> int launch(const CUtensorMap (&m)[4], const PromptArgs& a, long long blocks, cudaStream_t s) {
     static bool attr[MAX_DEVICES] = {};   // per device: the opt-in belongs to the device's copy of the kernel
     const int dev = current_device(); if (dev < 0) return HP_ECUDA;
-    if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_attn_prompt<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<D>::SMEM)); attr[dev] = true; }
-    HP_CUDA(launch_pdl<4>(k_attn_prompt<D, T>, dim3((unsigned)(blocks * a.n_head)), dim3(Geo<D>::THREADS), Geo<D>::SMEM, s, m[0], m[1], m[2], a));
+    if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_attn_prompt<D, T, GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<D, GATE>::SMEM)); attr[dev] = true; }
+    HP_CUDA(launch_pdl<4>(k_attn_prompt<D, T, GATE>, dim3((unsigned)(blocks * a.n_head)), dim3(Geo<D, GATE>::THREADS), Geo<D, GATE>::SMEM, s, m[0], m[1], m[2], m[3], a));
     return HP_OK;
 }
-template <typename T> int launch(const CUtensorMap (&m)[3], const PromptArgs& a, long long blocks, int D, cudaStream_t s) {
-    return D == 256 ? launch<256, T>(m, a, blocks, s) : D == 128 ? launch<128, T>(m, a, blocks, s) : launch<64, T>(m, a, blocks, s);
+template <typename T, bool GATE> int launch(const CUtensorMap (&m)[4], const PromptArgs& a, long long blocks, int D, cudaStream_t s) {
+    return D == 256 ? launch<256, T, GATE>(m, a, blocks, s) : D == 128 ? launch<128, T, GATE>(m, a, blocks, s) : launch<64, T, GATE>(m, a, blocks, s);
 }
 
 }  // namespace
@@ -593,15 +615,17 @@ int attn_prompt(const AttnPromptParams& p, cudaStream_t s) {
     const long long per = (p.max_rows + TQ - 1) / TQ, most = p.S * per, least = (long long)p.R / TQ + p.S, blocks = std::min(most, least);
     const int order = most <= least ? GRID : p.S <= 32 ? SORTED : ALONG;
     HP_REQUIRE(blocks * p.n_head < (1ll << 31), "attn_prompt: too many rows (%d) or heads for one call", p.R);
-    CUtensorMap m[3];
+    CUtensorMap m[4] = {};
     int rc = encode(f, &m[0], p.q, p.q_ld, p.q_hs, p.R, p.n_head, p.head_dim, TQ, p.type);
     if (!rc) rc = encode(f, &m[1], p.k, p.k_ld, p.k_hs, p.R, p.n_kv, p.head_dim, p.head_dim == 256 ? Geo<256>::TK : Geo<128>::TK, p.type);
     if (!rc) rc = encode(f, &m[2], p.v, p.v_ld, p.v_hs, p.R, p.n_kv, p.head_dim, p.head_dim == 256 ? Geo<256>::VROWS : Geo<128>::VROWS, p.type);
+    if (!rc && p.gate) rc = encode(f, &m[3], p.gate, p.g_ld, p.g_hs, p.R, p.n_head, p.head_dim, 32, OUT_F32);
     if (rc) return rc;
     PromptArgs a; a.row_start = p.row_start; a.S = p.S; a.R = p.R; a.max_rows = p.max_rows; a.order = order; a.n_head = p.n_head; a.n_kv = p.n_kv; a.G = p.n_head / p.n_kv; a.scale2 = (float)((double)p.scale * 1.4426950408889634074);
     a.q = p.q; a.k = p.k; a.v = p.v; a.q_ld = p.q_ld; a.q_hs = p.q_hs; a.k_ld = p.k_ld; a.k_hs = p.k_hs; a.v_ld = p.v_ld; a.v_hs = p.v_hs;
     a.gate = p.gate; a.g_ld = p.g_ld; a.g_hs = p.g_hs; a.out = p.out; a.oq = (int8_t*)p.xq.q; a.osc = (float*)p.xq.sc; a.err = device_err_flag(); a.arg_err = device_arg_flag();
-    return p.type == OUT_F16 ? launch<__half>(m, a, blocks, p.head_dim, s) : launch<__nv_bfloat16>(m, a, blocks, p.head_dim, s);
+    auto type = [&](auto gate) { constexpr bool GATE = decltype(gate)::value; return p.type == OUT_F16 ? launch<__half, GATE>(m, a, blocks, p.head_dim, s) : launch<__nv_bfloat16, GATE>(m, a, blocks, p.head_dim, s); };
+    return p.gate ? type(std::true_type()) : type(std::false_type());
 }
 
 }  // namespace hp

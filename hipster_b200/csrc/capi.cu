@@ -413,7 +413,7 @@ int hp_attn_prompt(const void* q_dev, long long q_ld, long long q_hs, const void
     HP_REQUIRE((((uintptr_t)out_dev | (uintptr_t)xq_q_dev | (uintptr_t)xq_sc_dev) & 15) == 0 && ((uintptr_t)row_start_dev & 3) == 0, "hp_attn_prompt: outputs must be 16-byte aligned");
     auto fits = [&](const void* p, long long ld, long long hs, int heads) { return rows_ok(p, ld, hs) && ((ld | hs) & 7) == 0 && (R == 1 || (ld > 0 && ld < (1ll << 38))) && (heads == 1 || (hs > 0 && hs < (1ll << 38))); };
     HP_REQUIRE(fits(q_dev, q_ld, q_hs, n_head) && fits(k_dev, k_ld, k_hs, n_kv) && fits(v_dev, v_ld, v_hs, n_kv), "hp_attn_prompt: rows must be 16-byte aligned, with positive strides that are multiples of 8");
-    HP_REQUIRE(!gate_dev || rows_ok(gate_dev, g_ld, g_hs), "hp_attn_prompt: the gate must be 16-byte aligned, with strides that are multiples of 4");
+    HP_REQUIRE(!gate_dev || (rows_ok(gate_dev, g_ld, g_hs) && (R == 1 || (g_ld > 0 && g_ld < (1ll << 37))) && (n_head == 1 || (g_hs > 0 && g_hs < (1ll << 37)))), "hp_attn_prompt: the gate must be 16-byte aligned, with positive strides that are multiples of 4");
     HP_REQUIRE(scale > 0 && scale < 1e30f, "hp_attn_prompt: bad scale");
     for (const void* o : {(const void*)out_dev, (const void*)xq_q_dev, (const void*)xq_sc_dev})
         HP_REQUIRE(!o || (o != q_dev && o != k_dev && o != v_dev && o != gate_dev), "hp_attn_prompt: an output in place of an input, which other rows still read");

@@ -265,6 +265,32 @@ def test_bad_row_starts_are_told():
     assert status() == 1
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("heads", [1, 6])
+def test_gates_of_any_strides(D, heads):
+    rows = [130, 0, 33, 1, 257]
+    q, k, v = make(rows, heads, 1, D, "bf16", 21, tail=2)
+    n = sum(rows) + 2
+    wide = torch.randn((heads, n, 3 * D), generator=gen(3), device="cuda")
+    got = []
+    for gate in (wide[..., D:2 * D].transpose(0, 1), wide[..., D:2 * D].transpose(0, 1).contiguous(), torch.cat([wide[..., D:2 * D].transpose(0, 1), torch.full((n, heads, 8), math.nan, device="cuda")], 2)[..., :D]):
+        got.append(K_.attn_prompt(q, k, v, starts(rows), max_rows=257, gate=gate)[0][:n - 2])
+    want, tol = prompt64(q[:n - 2], k[:n - 2], v[:n - 2], rows, D ** -0.5, wide[:, :n - 2, D:2 * D].transpose(0, 1))
+    assert ((got[0].double() - want).abs() <= tol).all() and torch.equal(got[0], got[1]) and torch.equal(got[0], got[2]) and status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_gates_at_their_ends(D):
+    """Infinite gates and NaN of one row: 0, the ungated result, NaN, and nothing of it in other rows or behind the last."""
+    q, k, v = make([140], 2, 1, D, "f16", 5, tail=1)
+    plain, _ = K_.attn_prompt(q, k, v, i32([0, 140]), max_rows=140)
+    gate = torch.full((141, 2, D), math.inf, device="cuda")
+    gate[3], gate[4, 1], gate[140] = -math.inf, math.nan, math.nan
+    got, _ = K_.attn_prompt(q, k, v, i32([0, 140]), max_rows=140, gate=gate)
+    keep = [i for i in range(140) if i not in (3, 4)]
+    assert torch.equal(got[keep], plain[keep]) and (got[3] == 0).all() and torch.equal(got[4, 0], plain[4, 0]) and got[4, 1].isnan().all() and status() == 0
+
+
 # same lengths (a number for every block), few of very different ones, and many: blocks are counted in three ways
 @pytest.mark.parametrize("rows", [[100] * 50, [128] * 33, [130] * 20, [0, 1, 900, 3, 0, 129], [700] + [5] * 40, [5] * 40 + [700], [1, 0, 127, 128, 129, 0, 256, 257] * 9 + [1500], [0] * 100 + [300] + [0] * 100 + [2]])
 @pytest.mark.parametrize("D", [64, 256])

@@ -102,6 +102,9 @@ def test_bad_prompts():
         refused(prompt(q=t), "aligned")
     refused(prompt(gate=(FAKE + 4, 256, 64)), "gate")
     refused(prompt(gate=(FAKE, 254, 64)), "gate")
+    refused(prompt(gate=(FAKE, 0, 64)), "gate")
+    refused(prompt(gate=(FAKE, 256, 0)), "gate")
+    refused(prompt(gate=(FAKE, 1 << 38, 64)), "gate")
     refused(prompt(scale=0.0), "scale")
     refused(prompt(scale=float("nan")), "scale")
     there = dict(q=(2 * FAKE, 256, 64), k=(3 * FAKE, 128, 64), v=(4 * FAKE, 128, 64), gate=(5 * FAKE, 256, 64))
