@@ -1,4 +1,4 @@
-// Attention over 8-bit pages for prompts: calls of many rows per sequence. The formulas, the exact splits of q and of the weights, and the merge are those of
+// Attention over pages in 8 or 4 bits for prompts: calls of many rows per sequence. The formulas, the exact splits of q and of the weights, and the merge are those of
 // attn_paged.cu; here the products run on tcgen05, and the codes are turned into f16 once per call instead of once per block of rows.
 //
 // k_paged_f16 writes each visible tile of 64 tokens of a kv head as the picture that shared memory holds: rows of 64 dims (128 bytes) per token, 128-byte

@@ -1,9 +1,10 @@
-// A cache of 8-bit pages: rotary tables, appending rows with their rotation on the way, and reading tokens back as f16.
+// A cache of pages in 8 or 4 bits: rotary tables, appending rows with their rotation on the way (at the row's place, or at positions of several axes), reading tokens back as f16; and the same norm and
+// rotation for rows that stay rows.
 //
 // k, v: codes [n_pages][n_kv][page][head_dim] in int8 or e4m3, k_scale, v_scale: f32 [n_pages][n_kv][page]: one scale per token and head. A
 // scale shared by several tokens would grow with a row that a verify pass writes and then rejects, and kept tokens would be requantised for
 // it: the speculative stream would no longer be the plain one. A scale per token costs 4 bytes beside head_dim codes and makes appending a
-// plain store: the same token appended again leaves the same bytes.
+// plain store: the same token appended again leaves the same bytes. 4 bits (i4_row in paged.cuh) hold to that: the scale, the factors and the zeros of a head's groups are a token's own.
 #include "paged.cuh"
 #include <algorithm>
 #include <cuda_bf16.h>
@@ -170,9 +171,10 @@ __device__ __forceinline__ void angles(float2 (&cs)[8], const float* rope, const
 }
 // D / 8 lanes take a head of a row, eight neighbouring elements each, so that a warp has 1, 2 or 4 heads side by side; it takes hpw such sets of neighbouring
 // heads (n_head query heads, then n_kv key heads, then n_kv value heads) in a loop that fetches a set ahead. The row's place and angles are found once. Four prompts of
-// up to 1000 rows of 48 heads of 128: 22.5 us, 73 MB, 95 instructions per head (with a warp per head and the loop unrolled four times 220, which did not fit the instruction cache). Neither issue
+// up to 1000 rows of 48 heads of 128, normalised: 26 us, 73 MB of DRAM traffic, 95 instructions per head (with a warp per head and the loop unrolled four times 220, which did not fit the instruction cache). Neither issue
 // slots (56 %) nor memory (3.3 TB/s) are used up: the warps, 43 % of what an SM holds, wait for their next set of heads (4.6 of them at a time). One row of 32 heads of 256 3.3 us, latency.
-// AXES: positions of several axes. 4 bits: four lanes share a group; its range takes four exchanges, the largest range of the head the others.
+// AXES: positions of several axes. 4 bits: four lanes share a group; its range takes four exchanges, the largest range of the head the others. The same four prompts of 48 heads of 128 with three axes, 30 us, to 4 bits 32;
+// 165 instructions per head, issue slots 58 %, otherwise waiting for exchanges and rows, in 1.6 waves of blocks. 8 x 3 rows of 24 + 4 heads of 256 4.6, latency.
 template <int D, int KIND, bool AXES>
 __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, RopeAxes axes, int hpw, int* err) {
     constexpr int LPH = D / 8, HPS = 32 / LPH;   // lanes of a head, heads of a set
@@ -292,7 +294,8 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
 
 // RB rows per block, RB / 8 of them found by each warp; thread = 16 neighbouring codes of a row, a head and k or v, times the scale, rounded to f16 once. The e4m3
 // patterns 0x7f and 0xff, which the quantiser does not write, read as 480 and -480. Bound by memory: 16 caches of up to 5000 tokens of 8 x 128 67 us (322 MB, 4.8 TB/s; pages of 16
-// tokens are runs of 2 KB), with one piece in flight per thread 88; 4096 tokens of 4 x 256 7.4 us.
+// tokens are runs of 2 KB), with one piece in flight per thread 88; 4096 tokens of 4 x 256 7.4 us. 4 bits: a word of 8 codes per piece, eight pieces in flight; bound by instructions (issue slots 76 %, 214 MB of it written or read):
+// the same caches 61 us, 4096 tokens 7.2. Where a row's codes lie, looked up once per row in shared memory: 63.8.
 template <int D, int KIND, int RB>
 __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, __half* __restrict__ ko, __half* __restrict__ vo, size_t row_stride, size_t head_stride, int* err) {
     constexpr int PIECE = KIND == KV_I4 ? 8 : 16, CPR = D / PIECE, PER = RB / 8;   // codes of a thread's piece
@@ -341,10 +344,10 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
             if (row[u] == 0xffffffffu) continue;
             const int i = i0 + u * 256, hv = i / (RB * CPR), c = i % CPR;
             uint4* dst = reinterpret_cast<uint4*>((hv & 1 ? vo : ko) + (size_t)(r0 + i / CPR % RB) * row_stride + (size_t)(hv >> 1) * head_stride + c * PIECE);
-            const float s = KIND == KV_E4M3 ? sc[u] * 256.f : sc[u];   // code_pair gives e4m3 codes times 2^-8; 4 bits: I4_UNIT times the number first, since the scale may be too large for it
+            // code_pair gives e4m3 codes times 2^-8, i4_word 4 bits times 1 / I4_UNIT. A scale that is too large for that factor: what is not zero becomes infinite in f16 with a smaller one too
+            const float s = KIND == KV_E4M3 ? sc[u] * 256.f : KIND == KV_I4 ? (sc[u] > 8e34f && sc[u] < INFINITY ? 8e34f : sc[u]) * I4_UNIT : sc[u];
             auto scaled = [](uint32_t pr, float s) {
-                float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pr));
-                if constexpr (KIND == KV_I4) { f.x = f.x * I4_UNIT; f.y = f.y * I4_UNIT; }
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pr));
                 return h2_bits(__floats2half2_rn(f.x * s, f.y * s));
             };
             if constexpr (KIND == KV_I4) {
@@ -361,7 +364,8 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
     }
 }
 
-// Rows of q, k and v, each head's norm and rotation, to outputs of another type: what k_kv_append does for rows that stay rows. The same lanes, sets of heads and loop.
+// Rows of q, k and v, each head's norm and rotation, to outputs of another type: what k_kv_append does for rows that stay rows. The same lanes, sets of heads and loop. Bound by memory: 8403 rows of 48 heads of 128 with
+// three axes to bf16 59.7 us, 310 MB (5.2 TB/s; copies 6.5), of which the rows' own start, behind their positions, hides under other warps' heads; 48 rows of 32 heads of 256 4.9 us, latency.
 template <int D, typename T>
 __global__ void __launch_bounds__(256, 4) k_rope_rows(RopeRowsParams p, RopeAxes axes, int hpw, int* err) {
     constexpr int LPH = D / 8, HPS = 32 / LPH;
