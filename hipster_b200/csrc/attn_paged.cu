@@ -17,10 +17,10 @@
 // A warp looks up the pages of all its slices at once, a lane each, and fetches a slice's scales with its keys; hidden keys are masked in the slices that have some.
 //
 // Measured (captured, us): one token of 24 heads of 256 over 4 at 4097 12.6 (bytes alone 1.3): start, four slices per warp and merge one after the other. 48 such sequences of up to
-// 8192 111 to 116 by card (80), 118 to 121 with the page looked up per slice and every slice masked: issue slots 58 %, a third of the instructions turning codes into f16. 8 x 3 rows over 2 kv heads at 2051 22.0 (2.0); 32 x 2
+// 8192 109 to 114 by card (80), 118 to 121 with the page looked up per slice, every slice masked, and blocks looked for where each sequence has one: issue slots 58 %, a third of the instructions turning codes into f16. 8 x 3 rows over 2 kv heads at 2051 22.0 (2.0); 32 x 2
 // rows of 32 heads of 128, window 1000, 34.6 (11): half of the instructions are starts and ends of the CTAs. Pairs as the 16 rows of the products: 260 for the 48 sequences; eight warps per CTA: 128.
-// 4 bits: one token at 4097 11.8 (0.7), the 48 sequences 103 (43), 256 sequences of 32 heads of 128 over 8 at up to 4096 222 (86): issue slots 57 to 66 %, 840 instructions per slice of 256 dims, of which 192 are products
-// and their operands' rests as many again. Two dims become f16 by one mask and one fma; by two masks and conversions 129 for the 48. Products of tcgen05 with the pictures of attn_paged_tc.cu: 15.9 for one token, 180 for the 48;
+// 4 bits: one token at 4097 11.8 (0.7), the 48 sequences 100 (43), 64 of 32 heads of 128 over 8 at up to 12001 212 (86): issue slots 57 to 66 %; a slice takes 464 instructions at 128 dims, 675 at 256,
+// a warp and split some 850 and 1050 around them. Two dims become f16 by one mask and one fma; by two masks and conversions 129 for the 48. Products of tcgen05 with the pictures of attn_paged_tc.cu: 15.9 for one token, 180 for the 48;
 // a head's dims split over the warps, 64 keys shared by them: 13.1, 110.
 // Two sets of pairs spill up to 28 bytes a thread, one set of 256 dims 12.
 #include "paged.cuh"
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
     pdl_wait();
     pdl_launch_dependents();   // behind the wait: what was enqueued in front of this kernel is complete when the merge starts
-    const Block blk = find_block(a.b, a.G, MB, blockIdx.z, lane, a.arg_err);
+    const Block blk = a.single ? only_block(a.b, a.G, blockIdx.z, a.arg_err) : find_block(a.b, a.G, MB, blockIdx.z, lane, a.arg_err);
     if (blk.q.s < 0) return;
     const PagedSeq& sq = blk.q;
     const Span sp = span_of(a, blk);
@@ -170,6 +170,13 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
         const int i = warp + KW * u, t = (blk.p0 + i) / a.G;
         const float x[8] = {qv[u][0].x, qv[u][0].y, qv[u][0].z, qv[u][0].w, qv[u][1].x, qv[u][1].y, qv[u][1].z, qv[u][1].w};
         const bool live = i < blk.np;
+        const int step = KIND != KV_I4 ? lane >> 2 : D == 64 ? lane & 1 : (lane >> 4) * 4 + (lane & 3), four = KIND != KV_I4 ? lane & 3 : D == 64 ? lane >> 1 : (lane >> 2) & 3;
+        uint4* const dst = reinterpret_cast<uint4*>(sm + (i >> 3) * D * 32 + step * 1024) + (i & 7) * 4 + four;
+        if (!live) {   // the warp's: zeros
+            if (lane < D / 8) dst[0] = dst[32] = make_uint4(0u, 0u, 0u, 0u);
+            if (lane == 0) { s_c[i] = a.scale2; s_pos[i] = -1; }
+            continue;
+        }
         uint32_t m = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
@@ -185,12 +192,10 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
                 const float2 f = __half22float2(hh);
                 h[j] = h2_bits(hh); r[j] = h2_bits(__floats2half2_rn(y0 - f.x, y1 - f.y));
             }
-            const int step = KIND != KV_I4 ? lane >> 2 : D == 64 ? lane & 1 : (lane >> 4) * 4 + (lane & 3), four = KIND != KV_I4 ? lane & 3 : D == 64 ? lane >> 1 : (lane >> 2) & 3;
-            uint4* dst = reinterpret_cast<uint4*>(sm + (i >> 3) * D * 32 + step * 1024) + (i & 7) * 4 + four;
             dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
             dst[32] = make_uint4(r[0], r[1], r[2], r[3]);
         }
-        if (lane == 0) { s_c[i] = a.scale2 * __uint_as_float((uint32_t)(127 - e) << 23); s_pos[i] = live ? max(-1, sq.len - sq.T + t) : -1; }
+        if (lane == 0) { s_c[i] = a.scale2 * __uint_as_float((uint32_t)(127 - e) << 23); s_pos[i] = max(-1, sq.len - sq.T + t); }
     }
     __syncthreads();
     float cf[NT][2], mu[NT][2], l[NT][2];
@@ -656,7 +661,7 @@ int attn_paged(const PagedPool& pool, const PagedBatch& b, const AttnPagedParams
     HP_REQUIRE(pl.blocks <= 65535 && pool.n_kv <= 65535 && (long long)b.R * p.n_head < (1ll << 31), "attn_paged: too many rows (%d) or heads for one call", b.R);
     PagedArgs a; a.pool = pool; a.b = b; a.q = p.q; a.q_ld = p.q_ld; a.q_hs = p.q_hs; a.n_head = p.n_head; a.G = p.n_head / pool.n_kv;
     a.scale2 = (float)((double)p.scale * 1.4426950408889634074 * (pool.kind == KV_E4M3 ? 256.0 : pool.kind == KV_I4 ? (double)I4_UNIT : 1.0)); a.window = p.window; a.n_sink = p.n_sink;
-    a.U = pl.U; a.ns = pl.ns; a.nwin = pl.nwin;
+    a.U = pl.U; a.ns = pl.ns; a.nwin = pl.nwin; a.single = (long long)b.max_rows * a.G <= pl.MB;
     a.pO = (float*)p.workspace; a.pml = (float2*)(a.pO + partials(pl, b, p.n_head) * pool.head_dim); a.err = device_err_flag(); a.arg_err = device_arg_flag();
     a.f16 = (uint8_t*)p.workspace + (partials(pl, b, p.n_head) * (pool.head_dim + 2) * sizeof(float) + 127) / 128 * 128; a.tiles = 0;
     a.gate = p.gate; a.g_ld = p.g_ld; a.g_hs = p.g_hs; a.mul = pool.kind == KV_E4M3 ? 256.f : pool.kind == KV_I4 ? I4_UNIT : 1.f; a.out = p.out; a.oq = (int8_t*)p.xq.q; a.osc = (float*)p.xq.sc;

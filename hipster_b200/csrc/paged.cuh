@@ -50,6 +50,7 @@ struct PagedArgs {
     const float* q; size_t q_ld, q_hs; int n_head, G; float scale2;   // scale2 = scale * log2 e (times 256 for e4m3, 4096 for 4 bits)
     int window, n_sink;
     int U, ns, nwin;            // keys of a split, splits of the first tokens, splits behind them
+    int single;                 // decode steps: no sequence has more pairs than a block takes
     float* pO; float2* pml;     // partials [row][head][ns + nwin] (x head_dim): sums, (mu, sum of weights)
     uint8_t* f16; int tiles;    // prompts: tiles of 64 tokens in f16, [sequence][kv head][tiles][k, v, scales]
     // outputs of the rows: written by the merge, or by the only split there is (direct)
@@ -147,6 +148,12 @@ __device__ __forceinline__ Block find_block(const PagedBatch& b, int G, int MB, 
 }
 
 // What a CTA of a block has to look at: keys [0, sink) and [lo, kend), of these its split's.
+// the same where no sequence can have more than one block: that of sequence blk
+__device__ __forceinline__ Block only_block(const PagedBatch& b, int G, int blk, int* err) {
+    Block o; o.q = paged_seq(b, blk, err); o.p0 = 0; o.np = o.q.T * G;
+    if (!o.np) o.q.s = -1;
+    return o;
+}
 struct Span { int kend, lo, sink, pos_lo, pos_hi; long long u0, u1; };
 __device__ __forceinline__ Span span_of(const PagedArgs& a, const Block& blk) {
     Span v;
