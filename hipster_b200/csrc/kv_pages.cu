@@ -82,23 +82,30 @@ template <int KIND> __device__ __forceinline__ uint32_t kv_code(float x) {
 }
 __device__ __forceinline__ float max_nan(float a, float b) { float y; asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }
 __device__ __forceinline__ float min_nan(float a, float b) { float y; asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }
-// A head's norm (nw = nullptr: none) and rotation (n_rot = 0: none) where D / 8 lanes hold 8 neighbouring dims each; cs: angles of the lane's elements, interleaved of its four pairs; row: D floats of
+// A lane's 8 norm weights, in bf16: one load where they are aligned
+__device__ __forceinline__ uint4 norm_words(const void* norm, int d0) {
+    const uint16_t* const w = (const uint16_t*)norm + d0;
+    if (((uintptr_t)w & 15) == 0) return *reinterpret_cast<const uint4*>(w);
+    return make_uint4(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16, w[4] | (uint32_t)w[5] << 16, w[6] | (uint32_t)w[7] << 16);
+}
+// A head's norm (weights `norm`, nullptr: none; HELD: fetched before) and rotation (n_rot = 0: none) where D / 8 lanes hold 8 neighbouring dims each; cs: angles of the lane's elements, interleaved of its four pairs; row: D floats of
 // shared memory of these lanes
-template <int D>
-__device__ __forceinline__ void turn_head(float (&x)[8], const uint16_t* nw, int n_rot, int interleaved, float eps, const float2 (&cs)[8], int d0, unsigned mask, float* row) {
+template <int D, bool HELD>
+__device__ __forceinline__ void turn_head(float (&x)[8], const void* norm, uint4 held, int n_rot, int interleaved, float eps, const float2 (&cs)[8], int d0, unsigned mask, float* row) {
     constexpr int LPH = D / 8;
     const int half = n_rot / 2;
     const bool turns = d0 < n_rot;
-    if (nw) {
+    if (norm) {
+        const uint4 nw = HELD ? held : norm_words(norm, d0);
         float ss = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
 #pragma unroll
         for (int off = LPH / 2; off > 0; off >>= 1) ss = ss + __shfl_xor_sync(mask, ss, off);
         const float inv = 1.0f / sqrtf(ss / (float)D + eps);
-        const uint16_t* w = nw + d0;
+        const uint32_t w[4] = {nw.x, nw.y, nw.z, nw.w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (x[j] * inv) * bf2f(w[j]);
+        for (int j = 0; j < 8; ++j) x[j] = (x[j] * inv) * __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
     }
     if (!n_rot) return;
     if (interleaved) {   // the other one of a pair is the lane's own
@@ -171,10 +178,10 @@ __device__ __forceinline__ void angles(float2 (&cs)[8], const float* rope, const
 }
 // D / 8 lanes take a head of a row, eight neighbouring elements each, so that a warp has 1, 2 or 4 heads side by side; it takes hpw such sets of neighbouring
 // heads (n_head query heads, then n_kv key heads, then n_kv value heads) in a loop that fetches a set ahead. The row's place and angles are found once. Four prompts of
-// up to 1000 rows of 48 heads of 128, normalised: 26 us, 73 MB of DRAM traffic, 95 instructions per head (with a warp per head and the loop unrolled four times 220, which did not fit the instruction cache). Neither issue
+// up to 1000 rows of 48 heads of 128, normalised: 22.7 us, 73 MB of DRAM traffic, 95 instructions per head (with a warp per head and the loop unrolled four times 220, which did not fit the instruction cache). Neither issue
 // slots (56 %) nor memory (3.3 TB/s) are used up: the warps, 43 % of what an SM holds, wait for their next set of heads (4.6 of them at a time). One row of 32 heads of 256 3.3 us, latency.
-// AXES: positions of several axes. 4 bits: four lanes share a group; its range takes four exchanges, the largest range of the head the others. The same four prompts of 48 heads of 128 with three axes, 30 us, to 4 bits 32;
-// 165 instructions per head, issue slots 58 %, otherwise waiting for exchanges and rows, in 1.6 waves of blocks. 8 x 3 rows of 24 + 4 heads of 256 4.6, latency.
+// AXES: positions of several axes. 4 bits: four lanes share a group; its range takes four exchanges, the largest range of the head the others. The same four prompts of 48 heads of 128 with three axes, 29 us, to 4 bits 31.6;
+// 165 instructions per head, issue slots 58 %, otherwise waiting for exchanges and rows, in 1.6 waves of blocks. 8 x 3 rows of 24 + 4 heads of 256 4.4, latency.
 template <int D, int KIND, bool AXES>
 __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, RopeAxes axes, int hpw, int* err) {
     constexpr int LPH = D / 8, HPS = 32 / LPH;   // lanes of a head, heads of a set
@@ -206,12 +213,18 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
     if (!placed || (unsigned)pos >= (unsigned)(AXES ? b.max_kv : min(b.max_kv, p.n_pos))) { paged_bad(err); return; }
     const uint32_t page = h1 > p.n_head ? paged_row(pool, q.s, pos >> pool.lg_page, 0, err) : 0u;
     if (!AXES && d0 < p.n_rot) angles(cs, p.rope, pos, p.n_rot, p.interleaved, d0);
+    // Norm weights are kept from head to head, and fetched again where k's follow q's: four prompts of up to 1000 rows in 8 bits 24.5 -> 22.7 us. With axes they would spill others (4 bits 31.6 -> 33.1)
+    constexpr bool HELD = !AXES;
+    int held = -1;
+    uint4 nw = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
     for (int h = h0; h < h1; h += HPS) {
         float x[8] = {next[0].x, next[0].y, next[0].z, next[0].w, next[1].x, next[1].y, next[1].z, next[1].w};
         if (h + HPS < h1) fetch(h + HPS);
         const int kind = h < p.n_head ? 0 : h < p.n_head + pool.n_kv ? 1 : 2, hh = kind == 0 ? h : kind == 1 ? h - p.n_head : h - p.n_head - pool.n_kv;
-        turn_head<D>(x, (const uint16_t*)(kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr), kind < 2 ? p.n_rot : 0, p.interleaved, p.eps, cs, d0, mask, buf[warp] + sub * D);
+        const void* const norm = kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr;
+        if constexpr (HELD) if (norm && held != kind) { held = kind; nw = norm_words(norm, d0); }
+        turn_head<D, HELD>(x, norm, nw, kind < 2 ? p.n_rot : 0, p.interleaved, p.eps, cs, d0, mask, buf[warp] + sub * D);
         if (kind == 0) {
             float4* o = reinterpret_cast<float4*>(p.q_out + (size_t)r * p.qo_ld + (size_t)hh * p.qo_hs + d0);
             o[0] = make_float4(x[0], x[1], x[2], x[3]); o[1] = make_float4(x[4], x[5], x[6], x[7]);
@@ -398,7 +411,8 @@ __global__ void __launch_bounds__(256, 4) k_rope_rows(RopeRowsParams p, RopeAxes
         if (h + HPS < h1) fetch(h + HPS);
         int hh = h;
         const int w = which(hh);
-        turn_head<D>(x, (const uint16_t*)(w == 0 ? p.norm[0] : w == 1 ? p.norm[1] : nullptr), w < 2 ? p.n_rot : 0, p.interleaved, p.eps, cs, d0, mask, buf[warp] + sub * D);
+        const void* const norm = w == 0 ? p.norm[0] : w == 1 ? p.norm[1] : nullptr;
+        turn_head<D, false>(x, norm, make_uint4(0u, 0u, 0u, 0u), w < 2 ? p.n_rot : 0, p.interleaved, p.eps, cs, d0, mask, buf[warp] + sub * D);
         T* to = (T*)(w == 0 ? p.out[0] : w == 1 ? p.out[1] : p.out[2]) + (size_t)r * (w == 0 ? p.out_ld[0] : w == 1 ? p.out_ld[1] : p.out_ld[2]) + (size_t)hh * (w == 0 ? p.out_hs[0] : w == 1 ? p.out_hs[1] : p.out_hs[2]) + d0;
         if constexpr (sizeof(T) == 4) {
             reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]); reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
