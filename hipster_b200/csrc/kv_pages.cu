@@ -153,6 +153,13 @@ __device__ __forceinline__ bool row_pos(RowPos& p, const RopeAxes& a, int r, int
     for (int k = 0; k < 4; ++k) { p.at[k] = k < a.n_axes ? a.pos[(size_t)k * a.pos_ld + r] : 0; ok &= (unsigned)p.at[k] < (unsigned)n_pos; }
     return ok;
 }
+// position on axis k, chosen without a branch: lanes have different axes (four prompts of up to 1000 rows in 4 bits 31.6 -> 30.5 us, 8 x 3 rows 4.4 -> 3.75)
+__device__ __forceinline__ int pick(const RowPos& p, uint32_t k) {
+    int o;
+    asm("{\n.reg .pred a, b;\n.reg .b32 t, u, v;\nand.b32 t, %5, 1;\nsetp.ne.u32 a, t, 0;\nand.b32 t, %5, 2;\nsetp.ne.u32 b, t, 0;\nselp.b32 u, %2, %1, a;\nselp.b32 v, %4, %3, a;\nselp.b32 %0, v, u, b;\n}"
+        : "=r"(o) : "r"(p.at[0]), "r"(p.at[1]), "r"(p.at[2]), "r"(p.at[3]), "r"(k));
+    return o;
+}
 __device__ __forceinline__ uint32_t axis_word(const RopeAxes& a, int w) {   // selected, not indexed: the words are kernel arguments
     uint32_t v = a.axes[0];
 #pragma unroll
@@ -172,16 +179,15 @@ __device__ __forceinline__ void angles(float2 (&cs)[8], const float* rope, const
         if (d >= n_rot || (interleaved && (j & 1))) continue;
         if (!run) w = axis_word(a, i >> 4);
         const uint32_t k = w >> (2 * (i & 15)) & 3u;
-        const int at = k == 0 ? p.at[0] : k == 1 ? p.at[1] : k == 2 ? p.at[2] : p.at[3];
-        cs[j] = t[(size_t)at * half + i];
+        cs[j] = t[(size_t)pick(p, k) * half + i];
     }
 }
 // D / 8 lanes take a head of a row, eight neighbouring elements each, so that a warp has 1, 2 or 4 heads side by side; it takes hpw such sets of neighbouring
 // heads (n_head query heads, then n_kv key heads, then n_kv value heads) in a loop that fetches a set ahead. The row's place and angles are found once. Four prompts of
-// up to 1000 rows of 48 heads of 128, normalised: 22.7 us, 73 MB of DRAM traffic, 95 instructions per head (with a warp per head and the loop unrolled four times 220, which did not fit the instruction cache). Neither issue
+// up to 1000 rows of 48 heads of 128, normalised: 26 us, 73 MB of DRAM traffic, 95 instructions per head (with a warp per head and the loop unrolled four times 220, which did not fit the instruction cache). Neither issue
 // slots (56 %) nor memory (3.3 TB/s) are used up: the warps, 43 % of what an SM holds, wait for their next set of heads (4.6 of them at a time). One row of 32 heads of 256 3.3 us, latency.
-// AXES: positions of several axes. 4 bits: four lanes share a group; its range takes four exchanges, the largest range of the head the others. The same four prompts of 48 heads of 128 with three axes, 29 us, to 4 bits 31.6;
-// 165 instructions per head, issue slots 58 %, otherwise waiting for exchanges and rows, in 1.6 waves of blocks. 8 x 3 rows of 24 + 4 heads of 256 4.4, latency.
+// AXES: positions of several axes. 4 bits: four lanes share a group; its range takes four exchanges, the largest range of the head the others. The same four prompts of 48 heads of 128 with three axes 28.2 us, to 4 bits 30.5;
+// 160 instructions per head, issue slots 58 %, otherwise waiting for exchanges and rows, in 1.6 waves of blocks. 8 x 3 rows of 24 + 4 heads of 256 3.75, latency.
 template <int D, int KIND, bool AXES>
 __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, RopeAxes axes, int hpw, int* err) {
     constexpr int LPH = D / 8, HPS = 32 / LPH;   // lanes of a head, heads of a set
@@ -213,7 +219,7 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
     if (!placed || (unsigned)pos >= (unsigned)(AXES ? b.max_kv : min(b.max_kv, p.n_pos))) { paged_bad(err); return; }
     const uint32_t page = h1 > p.n_head ? paged_row(pool, q.s, pos >> pool.lg_page, 0, err) : 0u;
     if (!AXES && d0 < p.n_rot) angles(cs, p.rope, pos, p.n_rot, p.interleaved, d0);
-    // Norm weights are kept from head to head, and fetched again where k's follow q's: four prompts of up to 1000 rows in 8 bits 24.5 -> 22.7 us. With axes they would spill others (4 bits 31.6 -> 33.1)
+    // Norm weights are kept from head to head, and fetched again where k's follow q's: four prompts of up to 1000 rows in 8 bits 27.6 -> 26.0 us. With axes they would spill others (4 bits 31.6 -> 33.1)
     constexpr bool HELD = !AXES;
     int held = -1;
     uint4 nw = make_uint4(0u, 0u, 0u, 0u);
@@ -378,7 +384,7 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
 }
 
 // Rows of q, k and v, each head's norm and rotation, to outputs of another type: what k_kv_append does for rows that stay rows. The same lanes, sets of heads and loop. Bound by memory: 8403 rows of 48 heads of 128 with
-// three axes to bf16 59.7 us, 310 MB (5.2 TB/s; copies 6.5), of which the rows' own start, behind their positions, hides under other warps' heads; 48 rows of 32 heads of 256 4.9 us, latency.
+// three axes to bf16 59.7 us, 310 MB (5.2 TB/s; copies 6.5), of which the rows' own start, behind their positions, hides under other warps' heads; 48 rows of 32 heads of 256 3.6 us, latency.
 template <int D, typename T>
 __global__ void __launch_bounds__(256, 4) k_rope_rows(RopeRowsParams p, RopeAxes axes, int hpw, int* err) {
     constexpr int LPH = D / 8, HPS = 32 / LPH;
