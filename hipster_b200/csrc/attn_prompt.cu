@@ -425,7 +425,11 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
 #pragma unroll
                 for (int i = 0; i < TK; i += 2) { float2 d = make_float2(-mu, -mu); fma2(d, make_float2(s[i], s[i + 1]), make_float2(c, c)); s[i] = d.x; s[i + 1] = d.y; }
             }
-            if (hides && n) ok = take(n) && ok;
+            if (hides && n) {
+                // One stage: V(n) comes behind the products of n - 1, and until V(n - 1) is there its barrier has the bit of n. With two stages the scores of n come behind the products of n - 2
+                if (G::ST == 1) ok = warp_wait(smem_u32(&x.pv_done[(n - 1) & 1]), (n - 1) >> 1 & 1, a.err);
+                ok = ok && take(n);
+            }
             // weights of 32 keys are handed over as soon as they are there: their products run under the next ones' exponentials
             float2 l2 = make_float2(0.f, 0.f);
 #pragma unroll

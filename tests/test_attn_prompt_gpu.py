@@ -468,3 +468,44 @@ def test_a_chat_about_an_image():
         want, tol = P.attn64(st, q, 1 / 16, 0, 0, gates[at:at + 3])
         assert ((got.double() - want).abs() <= tol).all() and status() == 0
         at += keep
+
+
+def hidden_values(kind, D, gated):
+    """Infinite and NaN values of later rows, of the next prompt and behind the last one, in some hundred blocks of three to nine tiles whose references do not move (scores are almost alike), while copies of as much memory as there is keep theirs late: the
+    last tile's values may be looked at only when they have come. Bits as without such values, in each of 40 calls."""
+    rows, H, n_kv = [500, 384, 640, 300, 513], 24, 4
+    R = sum(rows)
+    q, k, v = make(rows, H, n_kv, D, kind, 41, tail=100, packed=False)
+    q *= 0.01
+    rs = starts(rows)
+    g = torch.randn(q.shape, generator=gen(9), device="cuda") if gated else None
+    run = lambda: K_.attn_prompt(q, k, v, rs, max_rows=640, gate=g)[0]  # noqa: E731
+    clean = run()[:R]
+    keep = torch.ones(R, dtype=torch.bool, device="cuda")
+    at = 0
+    for i, T in enumerate(rows):   # the last rows of every other prompt, and what lies behind the last prompt's last row: hidden from the rows in front of them
+        if i % 2 == 0:
+            bad = at + T - 20
+            v[bad:at + T:3] = math.nan
+            v[bad + 1:at + T:3] = math.inf
+            keep[bad:at + T] = False
+        at += T
+    v[R:] = math.nan
+    big = torch.empty((2, 1 << 28), dtype=torch.uint8, device="cuda")
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(40):
+        with torch.cuda.stream(other):
+            big[0].copy_(big[1])
+        got.append(run()[:R])
+    torch.cuda.synchronize()
+    assert status() == 0
+    for y in got:
+        assert torch.equal(y[keep], clean[keep]) and not torch.isfinite(y[~keep]).any()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [128, 256])
+def test_hidden_values_of_many_blocks_beside_late_copies(kind, D):
+    hidden_values(kind, D, False)
