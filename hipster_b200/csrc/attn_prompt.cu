@@ -9,8 +9,8 @@
 // A row's reference mu moves when a logarithm passes it by more than MU_STEP, so the sums are rescaled rarely (by the row's own thread); weights reach 2^MU_STEP at most. Sums of weights are fp32 of the
 // weights before they are rounded to 16 bits: that rounding is at most half a step of the outputs' own type per weight.
 //
-// A value that is infinite or NaN must not reach the rows in front of it through a weight of zero: in the tiles with hidden keys such elements are taken out of shared memory (and noted) before the products, and the rows that see them
-// get their weight times that element at the end.
+// A value that is infinite or NaN must not reach the rows in front of it through a weight of zero: in the tiles with hidden keys such elements are taken out of shared memory before the products. A weight being positive, a row has
+// NaN, infinity or minus infinity of all that it sees, so the first key of each kind is noted per dim, and outputs from that row on get it added on their way out.
 //
 // Measured (captured, back to back; cuBLAS' sustained rate is 1402 TFLOP/s): 8190 rows of 24 heads of 256 690 us, 1.19 PFLOP/s, at 1.44 GHz under the power limit (1560 us of 16384 rows of 16 heads after a pause, 1.41 PFLOP/s; 1790 back to
 // back). 16384 rows of 16 heads of 128 1060 us, 1.04 PFLOP/s at 1.6 GHz, of 64 800 us, 0.69 at 1.93. Bounds: 256 dims shared memory (320 KB per tile of 128 keys of 2048 clocks of products) and power; 128 and 64 the weights' warps, two
@@ -35,8 +35,7 @@ constexpr float MU_STEP = 8.f;
 constexpr int PASS = 68;            // floats of a row of 64 outputs on their way out: 16-byte pieces of 8 rows hit distinct banks
 
 struct PromptArgs {
-    const int* row_start; int S, R, max_rows, order, n_head, n_kv, G; float scale2;   // scale * log2 e
-    const void *q, *k, *v; size_t q_ld, q_hs, k_ld, k_hs, v_ld, v_hs;          // as the tensor maps have them
+    const int* row_start; int S, R, max_rows, order, n_head, G; float scale2;   // scale * log2 e
     const float* gate; size_t g_ld, g_hs; void* out; int8_t* oq; float* osc; int* err; int* arg_err;
 };
 
@@ -162,12 +161,14 @@ __device__ __forceinline__ QBlock find_rows(const PromptArgs& a, int blk, int la
     return o;
 }
 
-// Infinite and NaN values of a tile that has hidden keys: noted in odd[] (a bit per key of the block's rows) and taken out of the tile in shared memory, before its products. A thread has a key, or half of its dims
+// Infinite and NaN values of a tile that has hidden keys are taken out of the tile in shared memory, before its products, and noted in `first`: the first key with NaN, infinity, minus infinity at a dim, counted in the block's rows
+// (k0: the tile's first). A thread has a key, or half of its dims
+template <int D> struct Odd { int any, first[3 * D]; };
 template <int D, typename T>
-__device__ bool take_out(uint8_t* v, uint64_t* v_full, uint32_t* odd, uint32_t parity, int tid, int* err) {
+__device__ bool take_out(uint8_t* v, uint64_t* v_full, Odd<D>& odd, int k0, uint32_t parity, int tid, int* err) {
     using G = Geo<D>;
     constexpr int SHARE = 128 / G::TK, N = D / 8 / SHARE;   // 16-byte pieces of a thread
-    const int key = tid % G::TK, lane = tid & 31, i0 = tid / G::TK * N, part = key / G::VROWS, in = key % G::VROWS;
+    const int key = tid % G::TK, i0 = tid / G::TK * N, part = key / G::VROWS, in = key % G::VROWS;
     const bool ok = warp_wait(smem_u32(&v_full[part]), parity, err);
     if (!ok) return false;
     uint8_t* const vr = v + part * G::V_PART + in * 128;
@@ -177,51 +178,25 @@ __device__ bool take_out(uint8_t* v, uint64_t* v_full, uint32_t* odd, uint32_t p
         const uint4 u = *reinterpret_cast<const uint4*>(vr + (i >> 3) * (G::VROWS * 128) + (((i & 7) ^ (in & 7)) << 4));
         any |= odd_pair<T>(u.x) | odd_pair<T>(u.y) | odd_pair<T>(u.z) | odd_pair<T>(u.w);
     }
-    any &= 0x80008000u;
-    if (any) {
+    if (any & 0x80008000u) {
 #pragma unroll 1
         for (int i = i0 * 8; i < (i0 + N) * 8; ++i) {
             uint16_t* const e = reinterpret_cast<uint16_t*>(vr + (i >> 6) * (G::VROWS * 128) + (((i >> 3 & 7) ^ (in & 7)) << 4)) + (i & 7);
-            if (odd16<T>(*e)) *e = 0;
+            if (!odd16<T>(*e)) continue;
+            const float x = to_f32<T>(*e);
+            atomicMin(&odd.first[(x != x ? 0 : x > 0.f ? 1 : 2) * D + i], k0 + key);
+            *e = 0;
         }
+        odd.any = 1;
         fence_proxy_async();
     }
-    const unsigned bad = __ballot_sync(0xffffffffu, any != 0);
-    if (lane == 0 && bad) atomicOr(&odd[key >> 5], bad);
+    __syncwarp();
     return true;
 }
-// and their share of the sums of the rows that see them, in accumulator memory. Keys are those of the block's own rows, first row r0
-template <int D, typename T>
-__device__ __noinline__ void put_in(const PromptArgs& a, const uint32_t* odd, int r0, int row, bool live, int head, int kh, float c, float mu, uint32_t at) {
-#pragma unroll 1
-    for (int j = 0; j < TQ; ++j) {
-        if (!(odd[j >> 5] >> (j & 31) & 1) || r0 + j >= a.R) continue;
-        const uint16_t* const kr = (const uint16_t*)a.k + (size_t)(r0 + j) * a.k_ld + (size_t)kh * a.k_hs;
-        const uint16_t* const vr = (const uint16_t*)a.v + (size_t)(r0 + j) * a.v_ld + (size_t)kh * a.v_hs;
-        const bool sees = live && j <= row;
-        float w = 0.f;
-        if (sees) {
-            const uint16_t* const qr = (const uint16_t*)a.q + (size_t)(r0 + row) * a.q_ld + (size_t)head * a.q_hs;
-#pragma unroll 1
-            for (int d = 0; d < D; ++d) w = fmaf(to_f32<T>(qr[d]), to_f32<T>(kr[d]), w);
-            w = w * c - mu;
-            w = w > 2.f * MU_STEP ? ex2(2.f * MU_STEP) : ex2(w);   // summed in another order than S: not beyond what a weight can be; NaN stays
-        }
-#pragma unroll 1
-        for (int d = 0; d < D; ++d) {
-            const uint16_t e = vr[d];
-            if (!odd16<T>(e)) continue;   // the same for all lanes
-            uint32_t o;
-            asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(at + d) : "memory");
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            asm volatile("" : "+r"(o));
-            if (sees) o = __float_as_uint(__uint_as_float(o) + w * to_f32<T>(e));
-            __syncwarp();
-            asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(at + d), "r"(o) : "memory");
-            st_wait();
-        }
-        __syncwarp();
-    }
+// and what a row of the block has of them at dim d; 0: it sees none
+template <int D> __device__ __forceinline__ float put_in(const Odd<D>& odd, int row, int d) {
+    const bool nan = row >= odd.first[d], up = row >= odd.first[D + d], down = row >= odd.first[2 * D + d];
+    return nan || (up && down) ? __uint_as_float(0x7fc00000u) : up ? INFINITY : down ? -INFINITY : 0.f;
 }
 
 template <int D, typename T, bool GATE>
@@ -232,19 +207,21 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
         uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2][4], pv_done[2], fin[2], gates;   // parts: stage * (KP or VP) + part. pv_done: of even and of odd tiles. Who waits for a tile's may be a tile ahead or behind, and a phase's bit tells only neighbours apart
         float inv[TQ];   // of a row's sum of weights
         int failed;
-        uint32_t tmem, odd[TQ / 32];   // keys of the block's own rows with an infinite or NaN value
+        uint32_t tmem;
+        Odd<D> odd;   // infinite and NaN values of the block's own rows
     };
     __shared__ Shared x;
     uint8_t* const sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = smem_u32(sm);
+    for (int i = tid; i < 3 * D; i += G::THREADS) x.odd.first[i] = TQ;
     if (tid == 0) {
         mbar_init(smem_u32(&x.q_full), 1);
         for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&x.k_full[i]), 1); mbar_init(smem_u32(&x.k_empty[i]), 1); mbar_init(smem_u32(&x.v_full[i]), 1); mbar_init(smem_u32(&x.v_empty[i]), 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); mbar_init(smem_u32(&x.pv_done[i]), 1); mbar_init(smem_u32(&x.fin[i]), 1); for (int p = 0; p < G::HAND; ++p) mbar_init(smem_u32(&x.p_full[i][p]), 4); }
         mbar_init(smem_u32(&x.gates), 1);
         x.failed = 0;
-        for (int i = 0; i < TQ / 32; ++i) x.odd[i] = 0;
+        x.odd.any = 0;
         fence_barrier_init();
     }
     __syncthreads();
@@ -296,7 +273,8 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
     auto write_outputs = [&](float inv) {
         if (GATE && !warp_wait(smem_u32(&x.gates), 0, a.err)) return;
         if (there <= 0) return;
-        const int from = (warp >> 2) * (D / 2), end = from + D * 4 / G::OUT_WARPS, r = b.row0 + q0 + 32 * (warp & 3);
+        const int from = (warp >> 2) * (D / 2), end = from + D * 4 / G::OUT_WARPS, r = b.row0 + q0 + 32 * (warp & 3), own = 32 * (warp & 3) + lane;
+        const bool odd = x.odd.any;
         float* const pass = reinterpret_cast<float*>(sm + (GATE ? G::OFF_V : 0)) + warp * (32 * PASS);
         // Short loops: this runs once per block, from a cold instruction cache
         if (!GATE && !a.oq) {   // 16 bits through shared memory, rows of 144 bytes; 8 lanes write a row
@@ -309,6 +287,11 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
 #pragma unroll
                 for (int e = 0; e < 64; e += 8)
                     *reinterpret_cast<uint4*>(pass + lane * 36 + e / 2) = make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv), pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
+                if (odd) {   // a row each
+                    uint16_t* const y = reinterpret_cast<uint16_t*>(pass + lane * 36);
+#pragma unroll 1
+                    for (int e = 0; e < 64; ++e) { const float add = put_in(x.odd, own, i + e); if (add != 0.f) y[e] = (uint16_t)pack2<T>(to_f32<T>(y[e]) + add, 0.f); }
+                }
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -326,6 +309,10 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
                 __syncwarp();
 #pragma unroll
                 for (int e = 0; e < 64; e += 4) *reinterpret_cast<float4*>(pass + lane * PASS + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+                if (odd) {
+#pragma unroll 1
+                    for (int e = 0; e < 64; ++e) { const float add = put_in(x.odd, own, i + e); if (add != 0.f) pass[lane * PASS + e] += add; }
+                }
                 __syncwarp();
                 if (GATE) {   // all rows at once, those that are not there too: a row after the other would wait for each
                     const float* const g = reinterpret_cast<const float*>(sm) + (32 * (warp & 3) + j0) * D + d;
@@ -364,7 +351,7 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
         const int row = tid;                              // of the block
         const float c = a.scale2;
         float mu = MU_NONE, l = 0.f;
-        auto take = [&](int n) { return take_out<D, T>(sm + G::OFF_V + n % G::ST * G::TILE, x.v_full + n % G::ST * G::VP, x.odd + (n * TK - q0) / 32, n / G::ST & 1, tid, a.err); };
+        auto take = [&](int n) { return take_out<D, T>(sm + G::OFF_V + n % G::ST * G::TILE, x.v_full + n % G::ST * G::VP, x.odd, n * TK - q0, n / G::ST & 1, tid, a.err); };
         bool ready = false, far = false;   // scores of the next tile; a row of the warp has a reference from 2^26 on
         if (GATE && q0 + row < b.T) {   // this row's gates on their way to L2, lines of 128 bytes
             const float* const g = a.gate + (size_t)(b.row0 + q0 + row) * a.g_ld + (size_t)head * a.g_hs;
@@ -457,9 +444,8 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
         }
         ok = ok && warp_wait(smem_u32(&x.pv_done[(tiles - 1) & 1]), (tiles - 1) >> 1 & 1, a.err);
         tc_fence_after();
-        asm volatile("bar.sync 1, 128;" ::: "memory");   // odd[] of all four warps, which all come here
+        asm volatile("bar.sync 1, 128;" ::: "memory");   // what all four warps took out; they all come here
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (ok && (x.odd[0] | x.odd[1] | x.odd[2] | x.odd[3])) put_in<D, T>(a, x.odd, b.row0 + q0, row, lane < there, head, kh, c, mu, at + G::T_O);
         if constexpr (SHARED) x.inv[row] = inv;
         else if (ok) write_outputs(inv);
     } else {   // ---- products and copies: K and scores in one warp, V and outputs in another, so that neither waits for what the other one waits for
@@ -625,8 +611,7 @@ int attn_prompt(const AttnPromptParams& p, cudaStream_t s) {
     if (!rc) rc = encode(f, &m[2], p.v, p.v_ld, p.v_hs, p.R, p.n_kv, p.head_dim, p.head_dim == 256 ? Geo<256>::VROWS : Geo<128>::VROWS, p.type);
     if (!rc && p.gate) rc = encode(f, &m[3], p.gate, p.g_ld, p.g_hs, p.R, p.n_head, p.head_dim, 32, OUT_F32);
     if (rc) return rc;
-    PromptArgs a; a.row_start = p.row_start; a.S = p.S; a.R = p.R; a.max_rows = p.max_rows; a.order = order; a.n_head = p.n_head; a.n_kv = p.n_kv; a.G = p.n_head / p.n_kv; a.scale2 = (float)((double)p.scale * 1.4426950408889634074);
-    a.q = p.q; a.k = p.k; a.v = p.v; a.q_ld = p.q_ld; a.q_hs = p.q_hs; a.k_ld = p.k_ld; a.k_hs = p.k_hs; a.v_ld = p.v_ld; a.v_hs = p.v_hs;
+    PromptArgs a; a.row_start = p.row_start; a.S = p.S; a.R = p.R; a.max_rows = p.max_rows; a.order = order; a.n_head = p.n_head; a.G = p.n_head / p.n_kv; a.scale2 = (float)((double)p.scale * 1.4426950408889634074);
     a.gate = p.gate; a.g_ld = p.g_ld; a.g_hs = p.g_hs; a.out = p.out; a.oq = (int8_t*)p.xq.q; a.osc = (float*)p.xq.sc; a.err = device_err_flag(); a.arg_err = device_arg_flag();
     auto type = [&](auto gate) { constexpr bool GATE = decltype(gate)::value; return p.type == OUT_F16 ? launch<__half, GATE>(m, a, blocks, p.head_dim, s) : launch<__nv_bfloat16, GATE>(m, a, blocks, p.head_dim, s); };
     return p.gate ? type(std::true_type()) : type(std::false_type());

@@ -509,3 +509,39 @@ def hidden_values(kind, D, gated):
 @pytest.mark.parametrize("D", [128, 256])
 def test_hidden_values_of_many_blocks_beside_late_copies(kind, D):
     hidden_values(kind, D, False)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("gated", [False, True])
+def test_what_rows_have_of_values_that_are_not_finite(kind, D, gated):
+    """Of NaN, or of infinities of both signs, NaN; of infinities of one sign these; by dim, in the block of the key's own row and in later ones, with gates and without, and nothing anywhere else. In int8: the run of 32 dims around it alone."""
+    rows, H = [300, 70], 4
+    q, k, v = make(rows, H, 2, D, kind, 51, packed=False)
+    q *= 0.1   # no weight so small that it is zero in 16 bits
+    gate = torch.randn(q.shape, generator=gen(3), device="cuda") if gated else None
+    run = lambda **kw: K_.attn_prompt(q, k, v, starts(rows), max_rows=300, gate=gate, **kw)  # noqa: E731
+    clean, xc = run(want_q8=True)
+    inf, nan = math.inf, math.nan
+    put = [(10, 0, inf), (200, 0, -inf), (130, 1, nan), (299, 2, inf), (128, 5, inf), (127, 6, -inf), (250, D - 1, -inf), (369, 3, -inf), (300, 4, nan), (300, 5, inf), (301, 5, -inf)]
+    want = torch.zeros((370, D), dtype=torch.float64, device="cuda")   # what is added to the finite part
+    for row, d, x in put:
+        v[row, 1, d] = x
+        want[row:300 if row < 300 else 370, d] += x
+    got, _ = run()
+    both, xq = run(want_q8=True)
+    assert status() == 0 and torch.equal(got.view(torch.int16), both.view(torch.int16)) and torch.equal(got[:, :2], clean[:, :2])
+    for h in (2, 3):
+        y, w = got[:, h].double(), want
+        hit = ~torch.isfinite(w)
+        assert torch.equal(y[~hit], clean[:, h].double()[~hit])
+        assert torch.equal(torch.isnan(y[hit]), torch.isnan(w[hit])) and torch.equal(y[hit].nan_to_num(7.0, posinf=8.0, neginf=9.0), w[hit].nan_to_num(7.0, posinf=8.0, neginf=9.0))
+    runs = torch.cat([torch.zeros_like(want), torch.zeros_like(want), want, want], 1).isfinite().unflatten(1, (-1, 32)).all(-1)
+    (c, d, s), (c0, d0, s0) = xq.unpack(), xc.unpack()
+    assert torch.equal(d[runs], d0[runs]) and torch.equal(s[runs], s0[runs]) and torch.equal(c.unflatten(1, (-1, 32))[runs], c0.unflatten(1, (-1, 32))[runs])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_hidden_values_of_many_gated_blocks_beside_late_copies(kind, D):
+    hidden_values(kind, D, True)
