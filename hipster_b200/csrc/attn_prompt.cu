@@ -383,9 +383,10 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[e] = fmaxf(t[e], s[TK - 4 + e]);
             const float top = fmaxf(max3(t[0], t[1], t[2]), t[3]) * c;
-            if (__any_sync(0xffffffffu, top > mu + MU_STEP)) {   // a row moves by its own scores alone
+            const bool moves = top - mu > MU_STEP;   // the difference of neighbours is exact, a sum beyond 2^26 is not: there mu + 8 may be mu + 16, and weights of 2^16 are more than f16 holds
+            if (__any_sync(0xffffffffu, moves)) {   // a row moves by its own scores alone
                 float al = 1.f;
-                if (top > mu + MU_STEP) { al = ex2(mu - top); mu = top; l = l * al; }   // the first reference: 0
+                if (moves) { al = ex2(mu - top); mu = top; l = l * al; }   // the first reference: 0
                 far = __any_sync(0xffffffffu, fabsf(mu) >= 67108864.f && mu != MU_NONE);
                 if (n) {
                     ok = warp_wait(smem_u32(&x.pv_done[(n - 1) & 1]), (n - 1) >> 1 & 1, a.err);

@@ -545,3 +545,27 @@ def test_what_rows_have_of_values_that_are_not_finite(kind, D, gated):
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_hidden_values_of_many_gated_blocks_beside_late_copies(kind, D):
     hidden_values(kind, D, True)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("low", [0, 1, 2])
+@pytest.mark.parametrize("e", [24, 25, 26, 27, 28])
+def test_references_next_to_larger_scores(kind, D, e, low):
+    """Logarithms at 2^e + low steps of 32-bit numbers there (2^(e - 23)), and from the third tile on one step more: the reference moves or the weights reach 2 to that step, which may be more than f16 holds.
+
+    Scores are whole and exact, the factor is 1 (scale = ln 2 in 32 bits, times log2 e, is 1 to 2^-28). Weights are powers of two, so an output has the half step of its type, h, and sums of some 300 weights and products in fp32, together less than 2^-14 of the largest value."""
+    step, T = 2.0 ** (e - 23), 300
+    q = torch.zeros((T, 1, D), dtype=TYPES[kind], device="cuda")
+    k, v = q.clone(), torch.randn((T, 1, D), generator=gen(5), device="cuda").to(TYPES[kind])
+    a = 2.0 ** (e // 2)
+    q[:, 0, 0], q[:, 0, 1] = a, step
+    k[:, 0, 0], k[:, 0, 1] = 2.0 ** e / a, low
+    k[128:, 0, 1] = low + 1
+    got, _ = K_.attn_prompt(q, k, v, i32([0, T]), max_rows=T, scale=math.log(2))
+    w = torch.ones(T, dtype=torch.float64, device="cuda")
+    w[128:] = 2.0 ** step
+    x = v[:, 0].double() * w[:, None]
+    want = x.cumsum(0) / w.cumsum(0)[:, None]
+    h = torch.finfo(q.dtype).eps / 2
+    assert ((got[:, 0].double() - want).abs() <= h * want.abs() + (2.0 ** -14 + 2.0 ** -24) * v.double().abs().max()).all() and status() == 0
