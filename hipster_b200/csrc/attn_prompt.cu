@@ -6,8 +6,9 @@
 //   scores (one thread): S[128 rows][keys] = Q K^T from shared memory, a tile ahead of the weights; K's copies (tensor maps; 64 dims of 128 bytes to a row, 128-byte swizzle)
 //   outputs (one thread): O[128 rows][dims] += W V with W from accumulator memory; V's copies (256 dims: a warp of their own has all copies)
 // Up to 128 dims take half of the accumulator memory and of shared memory: two CTAs per SM. 256 dims take an SM; K is fetched in parts of 64 dims and V in parts of 32 keys, each again as soon as its products are through.
-// A row's reference mu moves when a logarithm passes it by more than MU_STEP, so the sums are rescaled rarely (by the row's own thread); weights reach 2^MU_STEP at most. Sums of weights are fp32 of the
-// weights before they are rounded to 16 bits: that rounding is at most half a step of the outputs' own type per weight.
+// A row's reference mu moves to TOP below a logarithm that passes it by more than LIMIT, so the sums are rescaled rarely (by the row's own thread). Sums of weights are fp32 of the weights before they are rounded to 16 bits: that
+// rounding is half a step of the outputs' own type per weight. f16 has steps of 2^-24 below 2^-14 as well: the largest weight is at least 2^6 there, so that a key loses 2^-31 of it at most, and 2^18 weak keys beside a strong
+// one lose less than half a step together; none is above 2^15 (f16 ends at 65504).
 //
 // A value that is infinite or NaN must not reach the rows in front of it through a weight of zero: in the tiles with hidden keys such elements are taken out of shared memory before the products. A weight being positive, a row has
 // NaN, infinity or minus infinity of all that it sees, so the first key of each kind is noted per dim, and outputs from that row on get it added on their way out.
@@ -31,7 +32,9 @@ namespace hp {
 namespace {
 
 constexpr int TQ = 128;   // rows of a CTA
-constexpr float MU_STEP = 8.f;
+template <typename T> struct Ref { static constexpr float TOP = 0.f, LIMIT = 8.f; };
+template <> struct Ref<__half> { static constexpr float TOP = 6.f, LIMIT = 14.f; };
+constexpr float FAR = 16777216.f;   // 2^24: references from here on
 constexpr int PASS = 68;            // floats of a row of 64 outputs on their way out: 16-byte pieces of 8 rows hit distinct banks
 
 struct PromptArgs {
@@ -352,7 +355,7 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
         const float c = a.scale2;
         float mu = MU_NONE, l = 0.f;
         auto take = [&](int n) { return take_out<D, T>(sm + G::OFF_V + n % G::ST * G::TILE, x.v_full + n % G::ST * G::VP, x.odd, n * TK - q0, n / G::ST & 1, tid, a.err); };
-        bool ready = false, far = false;   // scores of the next tile; a row of the warp has a reference from 2^26 on
+        bool ready = false, far = false;   // scores of the next tile; a row of the warp has a reference from 2^24 on
         if (GATE && q0 + row < b.T) {   // this row's gates on their way to L2, lines of 128 bytes
             const float* const g = a.gate + (size_t)(b.row0 + q0 + row) * a.g_ld + (size_t)head * a.g_hs;
 #pragma unroll
@@ -383,11 +386,11 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[e] = fmaxf(t[e], s[TK - 4 + e]);
             const float top = fmaxf(max3(t[0], t[1], t[2]), t[3]) * c;
-            const bool moves = top - mu > MU_STEP;   // the difference of neighbours is exact, a sum beyond 2^26 is not: there mu + 8 may be mu + 16, and weights of 2^16 are more than f16 holds
+            const bool moves = top - mu > Ref<T>::LIMIT;   // the difference of neighbours is exact, a sum of large numbers is not: mu + 8 may be mu + 16, and weights of 2^16 are more than f16 holds
             if (__any_sync(0xffffffffu, moves)) {   // a row moves by its own scores alone
                 float al = 1.f;
-                if (moves) { al = ex2(mu - top); mu = top; l = l * al; }   // the first reference: 0
-                far = __any_sync(0xffffffffu, fabsf(mu) >= 67108864.f && mu != MU_NONE);
+                if (moves) { const float next = top - Ref<T>::TOP; al = ex2(mu - next); mu = next; l = l * al; }   // the first reference: 0
+                far = __any_sync(0xffffffffu, fabsf(mu) >= FAR && mu != MU_NONE);
                 if (n) {
                     ok = warp_wait(smem_u32(&x.pv_done[(n - 1) & 1]), (n - 1) >> 1 & 1, a.err);
                     if (!ok) break;
@@ -404,9 +407,10 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
                     st_wait();
                 }
             }
-            // distances from the reference. Logarithms from 2^26 on lie in steps of 8: there the product is rounded as it was for the reference, in the rows that have such a one
+            // distances from the reference. Logarithms from 2^24 on lie in steps of 2 and more: there the product is rounded as it was for the reference, in the rows that have such a one, so that a distance is LIMIT at most (LIMIT and a
+            // half step of the logarithm, 1 next to 2^24, else)
             if (far) {
-                const bool own = fabsf(mu) >= 67108864.f;
+                const bool own = fabsf(mu) >= FAR;
 #pragma unroll
                 for (int i = 0; i < TK; ++i) s[i] = own ? s[i] * c - mu : fmaf(s[i], c, -mu);
             } else {

@@ -569,3 +569,21 @@ def test_references_next_to_larger_scores(kind, D, e, low):
     want = x.cumsum(0) / w.cumsum(0)[:, None]
     h = torch.finfo(q.dtype).eps / 2
     assert ((got[:, 0].double() - want).abs() <= h * want.abs() + (2.0 ** -14 + 2.0 ** -24) * v.double().abs().max()).all() and status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("far", [24.25, 25.25, 27.0])
+def test_many_weak_keys_beside_a_strong_one(D, far):
+    """The first key 2^far times as heavy as each of the 20000 behind it, whose values alone are not zero: what they have together is not lost, although a weight of one of them is next to nothing.
+
+    In f16 a weight is off by half a step of it, or of 2^-24 where it is subnormal, and the largest weight is at least 2^6: 2^-31 of the largest one per key. The output is rounded to half a step of f16 or of 2^-24."""
+    T = 20001
+    q = torch.zeros((T, 1, D), dtype=torch.float16, device="cuda")
+    k, v = q.clone(), (torch.rand((T, 1, D), generator=gen(5), device="cuda") + 0.5).half()
+    q[:, 0, 0], k[0, 0, 0], v[0] = 1, far, 0
+    got, _ = K_.attn_prompt(q, k, v, i32([0, T]), max_rows=T, scale=math.log(2))
+    n = torch.arange(T, device="cuda", dtype=torch.float64)[:, None]
+    total = v[:, 0].double().cumsum(0)
+    want = total * 2.0 ** -far / (1 + n * 2.0 ** -far)
+    tol = want * (2 * 2.0 ** -11 + 2.0 ** -15) + 2.0 ** -31 * total + 2.0 ** -25
+    assert ((got[:, 0].double() - want).abs() <= tol).all() and status() == 0
