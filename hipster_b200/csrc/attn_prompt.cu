@@ -8,7 +8,8 @@
 // Up to 128 dims take half of the accumulator memory and of shared memory: two CTAs per SM. 256 dims take an SM; K is fetched in parts of 64 dims and V in parts of 32 keys, each again as soon as its products are through.
 // A row's reference mu moves to TOP below a logarithm that passes it by more than LIMIT, so the sums are rescaled rarely (by the row's own thread). Sums of weights are fp32 of the weights before they are rounded to 16 bits: that
 // rounding is half a step of the outputs' own type per weight. f16 has steps of 2^-24 below 2^-14 as well: the largest weight is at least 2^6 there, so that a key loses 2^-31 of it at most, and 2^18 weak keys beside a strong
-// one lose less than half a step together; none is above 2^15 (f16 ends at 65504).
+// one lose less than half a step together; none is above 2^15 (f16 ends at 65504). bf16 has weights of 2^-10 at most: sums of 1000 of the largest values, or of 2^18 where scores do not rise, stay finite, and products of
+// values down to 2^-108 are normal numbers (subnormal ones keep the bits that an output has down to 2^-121).
 //
 // A value that is infinite or NaN must not reach the rows in front of it through a weight of zero: in the tiles with hidden keys such elements are taken out of shared memory before the products. A weight being positive, a row has
 // NaN, infinity or minus infinity of all that it sees, so the first key of each kind is noted per dim, and outputs from that row on get it added on their way out.
@@ -32,7 +33,7 @@ namespace hp {
 namespace {
 
 constexpr int TQ = 128;   // rows of a CTA
-template <typename T> struct Ref { static constexpr float TOP = 0.f, LIMIT = 8.f; };
+template <typename T> struct Ref { static constexpr float TOP = -18.f, LIMIT = -10.f; };
 template <> struct Ref<__half> { static constexpr float TOP = 6.f, LIMIT = 14.f; };
 constexpr float FAR = 16777216.f;   // 2^24: references from here on
 constexpr int PASS = 68;            // floats of a row of 64 outputs on their way out: 16-byte pieces of 8 rows hit distinct banks

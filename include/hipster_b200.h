@@ -197,7 +197,8 @@ int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const floa
  * sums in fp32, weights rounded to the inputs' type, times sigmoid(gate) (gate_dev f32 [R][n_head][head_dim], nullable). type: HP_F16 or HP_BF16, of q, k, v and out [R][n_head * head_dim]; and / or the int8 quantisation of the
  * outputs before they are rounded (K = n_head * head_dim, buffers as hp_attn_paged has them); either may be NULL. head_dim 64, 128 or 256; n_head a multiple of n_kv. max_rows bounds a prompt's rows and sizes the launch. row_start
  * (S + 1 ints, rising; S at most 65535) is device memory, read when the kernel runs; rows behind row_start[S] are not written. What does not fit is left out and told by hp_device_status, as for the paged calls.
- * A row is not touched by infinite or NaN keys and values that it does not see; of a value that it sees, an infinite element makes the output's infinite or NaN.
+ * A row is not touched by infinite or NaN keys and values that it does not see; of a value that it sees, an infinite element makes the output's infinite or NaN. Finite values have
+ * finite outputs, in bf16 where the rows of the prompt times the largest magnitude stay below 3.4e38 * 512; of values within a step of the type's largest number, the weights' rounding may make an infinite output.
  * q, k, v: 16-byte aligned, strides positive multiples of 8; gate 16-byte aligned, strides positive multiples of 4; out and quantised outputs 16-byte aligned. Outputs overlap neither inputs nor each other. No
  * workspace. A row's result depends on its own prompt alone. */
 int hp_attn_prompt(const void* q_dev, long long q_ld, long long q_hs, const void* k_dev, long long k_ld, long long k_hs, const void* v_dev, long long v_ld, long long v_hs, int type, const float* gate_dev, long long g_ld, long long g_hs,

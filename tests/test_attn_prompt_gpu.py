@@ -587,3 +587,18 @@ def test_many_weak_keys_beside_a_strong_one(D, far):
     want = total * 2.0 ** -far / (1 + n * 2.0 ** -far)
     tol = want * (2 * 2.0 ** -11 + 2.0 ** -15) + 2.0 ** -31 * total + 2.0 ** -25
     assert ((got[:, 0].double() - want).abs() <= tol).all() and status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("size", [2.5e38, 1e30, 1e-33])
+def test_values_of_any_size(D, size):
+    """Values in bf16 next to the largest number and to the smallest normal one: outputs are means of them, whatever the sums of weights and values on the way."""
+    rows = [700, 90]
+    q, k, v = make(rows, 4, 2, D, "bf16", 61, packed=False)
+    v = (v.float().clamp(-1, 1) * size).bfloat16()
+    v[300:420] = size   # of one sign
+    gate = torch.randn(q.shape, generator=gen(3), device="cuda")
+    for g in (None, gate):
+        got, _ = K_.attn_prompt(q, k, v, starts(rows), max_rows=700, gate=g)
+        want, tol = prompt64(q, k, v, rows, D ** -0.5, g)
+        assert ((got.double() - want).abs() <= tol).all() and status() == 0
