@@ -288,13 +288,16 @@ def _norm_weight_on(w, head_dim, dev):
 
 def rope_axes(sections, n_rot=None, interleaved=False):
     """The axis of each rotated pair of dims, as kv_append and rope_rows take it: sections[a] pairs for axis a, one axis after the other; interleaved: the axes in turn (pair i to axis i mod n)
-    until an axis has its pairs, and what is left over to axis 0. n_rot: the dims that are rotated (2 * sum(sections))."""
+    until an axis has its pairs, and what is left over to axis 0; sections that do not come out so are refused. n_rot: the dims that are rotated (2 * sum(sections))."""
     n, half = len(sections), sum(sections)
     if not (1 <= n <= 4 and min(sections) >= 0 and half and (n_rot is None or n_rot == 2 * half)):
         raise HipsterError(1, "rope_axes: 1 to 4 sections, which add up to half of the rotated dims")
     if not interleaved:
         return bytes(a for a, m in enumerate(sections) for _ in range(m))
-    return bytes(i % n if i < n * sections[i % n] else 0 for i in range(half))
+    axes = bytes(i % n if i < n * sections[i % n] else 0 for i in range(half))
+    if any(axes.count(a) != m for a, m in enumerate(sections)):
+        raise HipsterError(1, f"rope_axes: in turn, {half} pairs cannot be {', '.join(map(str, sections))} of the axes")
+    return axes
 
 
 def _rope_args(who, rope, positions, axes, R, dev):

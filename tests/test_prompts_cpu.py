@@ -161,3 +161,15 @@ def test_what_reaches_the_library(recorded, monkeypatch):  # noqa: F811
     assert n1 == "hp_kv_append_axes" and a1[6] == 0 and a1[16:23] == (9, 32, 0, pos.data_ptr(), 5, bytes([0, 1, 2, 0] * 4), 3)
     assert n2 == "hp_rope_rows" and a2[6] == 4 and a2[7] is None and a2[19:22] == (2, 64, 2) and a2[28:32] == (pos.data_ptr(), 0, bytes(16), 1)
     assert n3 == "hp_rope_rows" and a3[24] is None and a3[28] is None and a3[31] == 0
+
+
+def test_sections_that_turns_do_not_give_are_refused():
+    """In turn, an axis has every n-th pair until it has its own; axis 0 has what is left. Sections that come out otherwise are refused, those that fit have all their pairs, axis 0 included."""
+    for sections in ((24, 20, 20), (11, 11, 10), (8, 2, 2, 4), (4, 1, 1), (1, 1), (2, 1), (5,), (6, 0, 0), (3, 0, 1)):
+        a = K_.rope_axes(sections, interleaved=True)
+        assert [a.count(i) for i in range(len(sections))] == list(sections)
+    for sections in ((1, 4, 4), (0, 4, 4), (8, 12, 12), (1, 2), (0, 1), (2, 2, 3), (4, 4, 4, 5)):
+        with pytest.raises(hb.HipsterError, match="in turn"):
+            K_.rope_axes(sections, interleaved=True)
+        a = K_.rope_axes(sections)
+        assert [a.count(i) for i in range(len(sections))] == list(sections)
