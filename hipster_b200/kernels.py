@@ -2,6 +2,7 @@
 (engine/kernels/gemv.h, ops.h). Arguments are torch CUDA tensors; every call goes through the C ABI."""
 import ctypes
 import functools
+import operator
 
 import torch
 
@@ -322,7 +323,7 @@ def _rope_args(who, rope, positions, axes, R, dev):
         axes = bytes(half)
     try:
         if type(axes) is not bytes:
-            axes = bytes(axes)
+            axes = bytes([operator.index(a) for a in axes])   # bytes() of a number is that many zeros, of an array the bytes of its numbers
     except (ValueError, TypeError):
         raise HipsterError(1, f"{who}: axes are whole numbers below the number of axes, one per rotated pair of dims") from None
     if len(axes) != half:

@@ -173,3 +173,22 @@ def test_sections_that_turns_do_not_give_are_refused():
             K_.rope_axes(sections, interleaved=True)
         a = K_.rope_axes(sections)
         assert [a.count(i) for i in range(len(sections))] == list(sections)
+
+
+def test_axes_that_are_not_a_number_per_pair_are_refused(recorded, monkeypatch):  # noqa: F811
+    """A number is not a list of that many zeros, and the bytes of wider integers are not axes. Lists, tuples, bytes and arrays of any integers are taken by value."""
+    import numpy as np
+    monkeypatch.setattr(K_, "more", lambda: recorded)
+    x, rope, pos = torch.zeros((3, 4, 64)), torch.zeros((9, 16, 2)), torch.zeros((3, 3), dtype=torch.int32)
+    pool = K_.KVPages.empty(4, 2, 16, 64, dtype="i4", device="cpu")
+    i = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    good = [0, 1, 2, 0] * 4
+    calls = (lambda axes: K_.rope_rows(x, None, None, rope, pos, axes), lambda axes: K_.kv_append(pool, x[:, :2], x[:, 2:], i([[0, 1]]), i([0, 3]), i([20]), rope, positions=pos, axes=axes))
+    for call in calls:
+        for axes in (16, np.int64(16), np.zeros(2, dtype=np.int64), np.zeros(4, dtype=np.float32), np.zeros((2, 8), dtype=np.uint8), [0.0] * 16, [0, -1] * 8, [0, 256] * 8, "0" * 16, [True] * 15, torch.zeros(15), None):
+            with pytest.raises(hb.HipsterError):
+                call(axes)
+                pytest.fail(f"{axes!r} was not refused")
+        for axes in (good, tuple(good), bytes(good), bytearray(good), np.array(good), np.array(good, dtype=np.uint8), torch.tensor(good), torch.tensor(good, dtype=torch.uint8)):
+            call(axes)
+            assert recorded.calls[-1][1][30 if recorded.calls[-1][0] == "hp_rope_rows" else 21] == bytes(good)
