@@ -602,3 +602,17 @@ def test_values_of_any_size(D, size):
         got, _ = K_.attn_prompt(q, k, v, starts(rows), max_rows=700, gate=g)
         want, tol = prompt64(q, k, v, rows, D ** -0.5, g)
         assert ((got.double() - want).abs() <= tol).all() and status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("rs,there", [([-1, 30, 40, 90], [(1, 30, 40), (2, 40, 90)]), ([0, -5, 40, 90], [(2, 40, 90)]), ([0, 30, 20, 90], [(0, 0, 30)]), ([0, 30, 40, 91], [(0, 0, 30), (1, 30, 40)]), ([0, 30, 1 << 30, 90], [(0, 0, 30)]),
+                                      ([-2 ** 31, 30, 40, 2 ** 31 - 1], [(1, 30, 40)])])
+def test_prompts_beside_bad_row_starts_are_served(D, rs, there):
+    """Rows of a prompt whose two ends fit, as without the others. Of 0, 30, 20, 90 rows 20 to 29 are claimed by two prompts (0 to 29, and 20 on), and are no one's to be compared."""
+    q, k, v = make([90], 2, 1, D, "bf16", 3, packed=False)
+    got, _ = K_.attn_prompt(q, k, v, i32(rs), max_rows=60)
+    assert status() == 1
+    for _, a, b in there:
+        n = 20 if rs[1:3] == [30, 20] else b - a
+        assert torch.equal(got[a:a + n], K_.attn_prompt(q[a:b], k[a:b], v[a:b], i32([0, b - a]), max_rows=60)[0][:n]), (a, b)
+    assert status() == 0

@@ -517,3 +517,24 @@ def test_rope_rows_into_views_and_in_place():
     f32 = K_.rope_rows(x[:, :3], x[:, 3:4], x[:, 4:], rope, pos, axes, dtype=torch.float32)
     call((y[:, :3], y[:, 3:4], y[:, 4:]), (y[:, :3], y[:, 3:4], y[:, 4:]), 0)
     assert torch.equal(y, torch.cat(f32, 1)) and status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("mr", [2, 16, 17, 40])
+@pytest.mark.parametrize("kind", ["i4", "i8", "e4m3"])
+def test_sequences_beside_one_with_a_bad_page_are_served(D, mr, kind):
+    """The same bits as without the bad page, in decode steps and in prompts (more than 16 rows)."""
+    n = min(mr, 20)
+    st = Setup([n, n, n], [100, 300, 50], 2, D, 16) if kind == "i4" else P.Setup([n, n, n], [100, 300, 50], 2, D, 16, kind)
+    x = torch.randn((3 * n, 4, D), generator=gen(1), device="cuda")
+    run = lambda: K_.attn_paged(x, st.pool, *st.batch, max_rows=mr, max_kv=300)[0]  # noqa: E731
+    want = run()
+    assert status() == 0
+    keep = [*range(n), *range(2 * n, 3 * n)]
+    for column, bad in ((0, -1), (7, st.pool.n_pages), (18, 1 << 30), (3, -2 ** 31)):
+        old = int(st.table[1, column])
+        st.table[1, column] = bad
+        got = run()
+        assert status() == 1 and torch.equal(got[keep], want[keep])
+        st.table[1, column] = old
+    assert torch.equal(run(), want) and status() == 0
