@@ -438,17 +438,28 @@ __global__ void __launch_bounds__(256, 4) k_rope_rows(RopeRowsParams p, RopeAxes
     }
 }
 
-// One set of heads per warp while all of them fit on the GPU at once; eight beyond: what a warp does once per row (its sequence, its place, its angles) takes as long as some three sets. One, six and eight, us: 8 bits, 256
-// rows of 48 heads of 128 6.7, 7.9 and -, 512 10.3, 10.5, -, four prompts of up to 1000 -, 32.1, 30.6; 4 bits with three axes, 2503 rows 62, 37, 34.5. Rows that stay rows, enough of them for a warp each: all of a row, up to 24 sets
-// (8403 rows of 48 heads of 128: 64.7 with eight, 59.9)
+// Sets of heads per warp. What a warp does once per row (its sequence, its place, its angles) takes as long as one or two sets; 4736 warps run at once. So a number of sets costs the warps' mean length for each full wave of them, and the longest one
+// (two fifths of it, however few) for what is left; least wins. Us with one set, with six, with eight (rows that stay rows: all) and so: int8, 2000 rows of 32 heads of 64 11.1, 7.7, 12.0 and 8.0, 1500 rows of 32 heads of
+// 128 17.2, 10.6, 14.7 and 10.4, four prompts of up to 1000 rows of 48 40.6, 28.3, 25.7 and 25.7; the same to 4 bits with axes 54.5, 33.9, 31.1 and 31.1; 8403 rows of 48 heads of 128 that stay rows, at positions as they come, 144, 77, 72.4 and 72.5. Over 696 shapes of 300 to 12000 rows the best of all numbers is 1 % faster on average, where it was 13 %.
 struct Cut { int hpw; unsigned blocks; };
-Cut cut_heads(long long R, int heads, int D, bool stay) {
-    const int HPS = 32 / (D / 8), sets = (heads + HPS - 1) / HPS, hpw = R * heads <= 148 * 64 * HPS ? 1 : stay && R >= 148 * 32 ? std::min(sets, 24) : 8;
+Cut cut_heads(long long R, int heads, int D) {
+    constexpr long long WARPS = 148 * 32;
+    const int HPS = 32 / (D / 8), sets = (heads + HPS - 1) / HPS;
+    int hpw = 1;
+    if (R * sets > WARPS) {
+        double least = 0;
+        for (int h = 1; h <= std::min(sets, 24); ++h) {
+            const int parts = (sets + h - 1) / h;
+            const long long n = R * parts, full = n / WARPS, left = n % WARPS;
+            const double cost = full * (1.5 + (double)sets / parts) + (left ? (1.5 + h) * (full ? 0.4 + 0.6 * left / WARPS : 1.0) : 0.0);
+            if (h == 1 || cost < least) { least = cost; hpw = h; }
+        }
+    }
     return Cut{hpw, (unsigned)((R * ((heads + hpw * HPS - 1) / (hpw * HPS)) + 7) / 8)};
 }
 template <int D, int KIND> int launch_append(const PagedPool& pool, const PagedBatch& b, const KvAppendParams& p, const RopeAxes& axes, cudaStream_t s) {
     int* err = device_arg_flag();
-    const Cut c = cut_heads(b.R, p.n_head + 2 * pool.n_kv, D, false);
+    const Cut c = cut_heads(b.R, p.n_head + 2 * pool.n_kv, D);
     HP_CUDA(launch_pdl<4>(axes.pos ? k_kv_append<D, KIND, true> : k_kv_append<D, KIND, false>, dim3(c.blocks), dim3(256), 0, s, pool, b, p, axes, c.hpw, err));
     return HP_OK;
 }
@@ -457,7 +468,7 @@ template <int KIND> int launch_append(const PagedPool& pool, const PagedBatch& b
 }
 template <typename T> int launch_rows(const RopeRowsParams& p, const RopeAxes& axes, cudaStream_t s) {
     int* err = device_arg_flag();
-    const Cut c = cut_heads(p.R, p.heads[0] + p.heads[1] + p.heads[2], p.head_dim, true);
+    const Cut c = cut_heads(p.R, p.heads[0] + p.heads[1] + p.heads[2], p.head_dim);
     HP_CUDA(launch_pdl<4>(p.head_dim == 256 ? k_rope_rows<256, T> : p.head_dim == 128 ? k_rope_rows<128, T> : k_rope_rows<64, T>, dim3(c.blocks), dim3(256), 0, s, p, axes, c.hpw, err));
     return HP_OK;
 }
