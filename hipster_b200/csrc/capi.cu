@@ -9,6 +9,7 @@
 #include <cstdlib>
 #include <string>
 #include <algorithm>
+#include <climits>
 #include <exception>
 
 namespace hp {
@@ -408,6 +409,7 @@ int hp_attn_prompt(const void* q_dev, long long q_ld, long long q_hs, const void
     HP_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "hp_attn_prompt: head_dim must be 64, 128 or 256, not %d", head_dim);
     HP_REQUIRE(n_kv >= 1 && n_head >= 1 && n_head % n_kv == 0, "hp_attn_prompt: n_head=%d must be a multiple of n_kv=%d", n_head, n_kv);
     HP_REQUIRE(S >= 1 && S <= 65535 && R >= 1 && max_rows >= 1, "hp_attn_prompt: bad batch S=%d R=%d max_rows=%d", S, R, max_rows);
+    HP_REQUIRE(R < INT_MAX - 256, "hp_attn_prompt: too many rows (%d)", R);   // tiles and blocks end up to 127 rows behind the last
     HP_REQUIRE(q_dev && k_dev && v_dev && row_start_dev && (out_dev || xq_q_dev), "hp_attn_prompt: null pointer");
     HP_REQUIRE((xq_q_dev == nullptr) == (xq_sc_dev == nullptr), "hp_attn_prompt: give both quantised-output buffers or neither");
     HP_REQUIRE((((uintptr_t)out_dev | (uintptr_t)xq_q_dev | (uintptr_t)xq_sc_dev) & 15) == 0 && ((uintptr_t)row_start_dev & 3) == 0, "hp_attn_prompt: outputs must be 16-byte aligned");

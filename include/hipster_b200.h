@@ -196,7 +196,7 @@ int hp_attn_paged(const float* q_dev, long long q_ld, long long q_hs, const floa
 /* Causal attention of whole prompts, packed: rows [row_start[s], row_start[s + 1]) of q [R][n_head][head_dim], k and v [R][n_kv][head_dim] are prompt s, whose row i sees the keys of its rows 0 .. i: softmax(scale * q k^T) v,
  * sums in fp32, weights rounded to the inputs' type, times sigmoid(gate) (gate_dev f32 [R][n_head][head_dim], nullable). type: HP_F16 or HP_BF16, of q, k, v and out [R][n_head * head_dim]; and / or the int8 quantisation of the
  * outputs before they are rounded (K = n_head * head_dim, buffers as hp_attn_paged has them); either may be NULL. head_dim 64, 128 or 256; n_head a multiple of n_kv. max_rows bounds a prompt's rows and sizes the launch. row_start
- * (S + 1 ints, rising; S at most 65535) is device memory, read when the kernel runs; rows behind row_start[S] are not written. What does not fit is left out and told by hp_device_status, as for the paged calls.
+ * (S + 1 ints, rising; S at most 65535, R below 2^31 - 257) is device memory, read when the kernel runs; rows behind row_start[S] are not written. What does not fit is left out and told by hp_device_status, as for the paged calls.
  * A row is not touched by infinite or NaN keys and values that it does not see; of a value that it sees, an infinite element makes the output's infinite or NaN. Finite values have
  * finite outputs, in bf16 where the rows of the prompt times the largest magnitude stay below 3.4e38 * 512; of values within a step of the type's largest number, the weights' rounding may make an infinite output.
  * q, k, v: 16-byte aligned, strides positive multiples of 8; gate 16-byte aligned, strides positive multiples of 4; out and quantised outputs 16-byte aligned. Outputs overlap neither inputs nor each other. No

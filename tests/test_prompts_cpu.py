@@ -192,3 +192,10 @@ def test_axes_that_are_not_a_number_per_pair_are_refused(recorded, monkeypatch):
         for axes in (good, tuple(good), bytes(good), bytearray(good), np.array(good), np.array(good, dtype=np.uint8), torch.tensor(good), torch.tensor(good, dtype=torch.uint8)):
             call(axes)
             assert recorded.calls[-1][1][30 if recorded.calls[-1][0] == "hp_rope_rows" else 21] == bytes(good)
+
+
+@pytest.mark.parametrize("R", [2 ** 31 - 1, 2 ** 31 - 128, 2 ** 31 - 256])
+def test_rows_whose_tiles_end_beyond_32_bits_are_refused(R):
+    """Tiles and blocks reach up to 127 rows beyond the last one, and their numbers are 32-bit."""
+    refused(prompt(R=R, max_rows=R, S=1, q=(FAKE, 8, 64), k=(FAKE, 8, 64), v=(FAKE, 8, 64), n_head=1, n_kv=1), "too many rows")
+    refused(prompt(R=R, max_rows=1, S=1), "too many rows")
