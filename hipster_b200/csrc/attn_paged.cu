@@ -22,7 +22,7 @@
 // 4 bits: one token at 4097 11.8 (0.7), the 48 sequences 100 (43), 64 of 32 heads of 128 over 8 at up to 12001 212 (86): issue slots 57 to 66 %; a slice takes 464 instructions at 128 dims, 675 at 256,
 // a warp and split some 850 and 1050 around them. Two dims become f16 by one mask and one fma; by two masks and conversions 129 for the 48. Products of tcgen05 with the pictures of attn_paged_tc.cu: 15.9 for one token, 180 for the 48;
 // a head's dims split over the warps, 64 keys shared by them: 13.1, 110.
-// Two sets of pairs spill up to 28 bytes a thread, one set of 256 dims 12.
+// Two sets of pairs spill up to 56 bytes a thread (4 bits, 64 dims; 8 bits 40), 256 dims and one set none.
 #include "paged.cuh"
 #include <algorithm>
 #include <type_traits>
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(32 * KW, NT == 2 ? (D == 256 ? 2 : D == 128 ? 
             auto products = [&](float (&o)[NT][4], const uint32_t (&af)[4]) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    if constexpr (KIND == KV_I4) {   // into the running sums: a step of 2^-23 of them per slice at most, 2^-19 in a split; the 48 sequences of the head of this file 107 us so, 114 with adds of their own
+                    if constexpr (KIND == KV_I4) {   // into the running sums: two products, a step of 2^-23 of them each, 2^-22 per slice at most, 2^-18 in a split (16 slices of a warp); the 48 sequences of the head of this file 107 us so, 114 with adds of their own
                         mma_f16(o[n], af, br[n][0], br[n][1]);
                         mma_f16(o[n], af, bh[n][0], bh[n][1]);
                         continue;

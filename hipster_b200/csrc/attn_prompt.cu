@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
     using G = Geo<D, GATE>;
     extern __shared__ uint8_t sm_raw[];
     struct Shared {
-        uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2][4], pv_done[2], fin[2], gates;   // parts: stage * (KP or VP) + part. pv_done: of even and of odd tiles. Who waits for a tile's may be a tile ahead or behind, and a phase's bit tells only neighbours apart
+        uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2][G::HAND], pv_done[2], fin[2], gates;   // parts: stage * (KP or VP) + part. pv_done: of even and of odd tiles. Who waits for a tile's may be a tile ahead or behind, and a phase's bit tells only neighbours apart
         float inv[TQ];   // of a row's sum of weights
         int failed;
         uint32_t tmem;

@@ -147,13 +147,13 @@ __device__ __forceinline__ Block find_block(const PagedBatch& b, int G, int MB, 
     return o;
 }
 
-// What a CTA of a block has to look at: keys [0, sink) and [lo, kend), of these its split's.
-// the same where no sequence can have more than one block: that of sequence blk
+// find_block where no sequence can have more than one block: that of sequence blk
 __device__ __forceinline__ Block only_block(const PagedBatch& b, int G, int blk, int* err) {
     Block o; o.q = paged_seq(b, blk, err); o.p0 = 0; o.np = o.q.T * G;
     if (!o.np) o.q.s = -1;
     return o;
 }
+// What a CTA of a block has to look at: keys [0, sink) and [lo, kend), of these its split's.
 struct Span { int kend, lo, sink, pos_lo, pos_hi; long long u0, u1; };
 __device__ __forceinline__ Span span_of(const PagedArgs& a, const Block& blk) {
     Span v;
