@@ -70,6 +70,7 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint3
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int add) {   // A in accumulator memory
     asm volatile("{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 b, {%2, %5};\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(DESC_HIGH) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
@@ -204,11 +205,11 @@ template <int D> __device__ __forceinline__ float put_in(const Odd<D>& odd, int 
 }
 
 template <int D, typename T, bool GATE>
-__global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mg, const PromptArgs a) {
+__global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const PromptArgs a) {
     using G = Geo<D, GATE>;
     extern __shared__ uint8_t sm_raw[];
     struct Shared {
-        uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2][G::HAND], pv_done[2], fin[2], gates;   // parts: stage * (KP or VP) + part. pv_done: of even and of odd tiles. Who waits for a tile's may be a tile ahead or behind, and a phase's bit tells only neighbours apart
+        uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2][G::HAND], pv_done[2], fin[2];   // parts: stage * (KP or VP) + part. pv_done: of even and of odd tiles. Who waits for a tile's may be a tile ahead or behind, and a phase's bit tells only neighbours apart
         float inv[TQ];   // of a row's sum of weights
         int failed;
         uint32_t tmem;
@@ -223,7 +224,6 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
         mbar_init(smem_u32(&x.q_full), 1);
         for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&x.k_full[i]), 1); mbar_init(smem_u32(&x.k_empty[i]), 1); mbar_init(smem_u32(&x.v_full[i]), 1); mbar_init(smem_u32(&x.v_empty[i]), 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&x.s_full[i]), 1); mbar_init(smem_u32(&x.pv_done[i]), 1); mbar_init(smem_u32(&x.fin[i]), 1); for (int p = 0; p < G::HAND; ++p) mbar_init(smem_u32(&x.p_full[i][p]), 4); }
-        mbar_init(smem_u32(&x.gates), 1);
         x.failed = 0;
         x.odd.any = 0;
         fence_barrier_init();
@@ -269,13 +269,12 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = x.tmem;
-    bool ok = true, gated = false;   // gated: this warp has fetched gates
+    bool ok = true;
     constexpr bool SHARED = G::OUT_WARPS == 8;
     const int there = min(32, b.T - q0 - 32 * (warp & 3));   // rows of this warp's outputs
     const uint32_t at = tmem + ((uint32_t)(warp & 3) << 21);
     // Outputs, 64 dims at a time through shared memory, which nothing else uses any more: a thread has a row, and 16 lanes write one
     auto write_outputs = [&](float inv) {
-        if (GATE && !warp_wait(smem_u32(&x.gates), 0, a.err)) return;
         if (there <= 0) return;
         const int from = (warp >> 2) * (D / 2), end = from + D * 4 / G::OUT_WARPS, r = b.row0 + q0 + 32 * (warp & 3), own = 32 * (warp & 3) + lane;
         const bool odd = x.odd.any;
@@ -357,11 +356,6 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
         float mu = MU_NONE, l = 0.f;
         auto take = [&](int n) { return take_out<D, T>(sm + G::OFF_V + n % G::ST * G::TILE, x.v_full + n % G::ST * G::VP, x.odd, n * TK - q0, n / G::ST & 1, tid, a.err); };
         bool ready = false, far = false;   // scores of the next tile; a row of the warp has a reference from 2^24 on
-        if (GATE && q0 + row < b.T) {   // this row's gates on their way to L2, lines of 128 bytes
-            const float* const g = a.gate + (size_t)(b.row0 + q0 + row) * a.g_ld + (size_t)head * a.g_hs;
-#pragma unroll
-            for (int i = 0; i < D; i += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(g + i));
-        }
 #pragma unroll 1
         for (int n = 0; n < tiles; ++n) {
             const uint32_t sc = at + G::T_S + (n & 1) * TK;
@@ -373,6 +367,13 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
 #pragma unroll
             for (int i = 0; i < TK; i += 32) ld32(s + i, sc + i);
             ld_wait<TK>(s);
+            if (GATE && n == tiles - 1) {   // the last scores are there, so nothing reads q and k any more: the gates of this warp's rows in their place, each thread its own copies
+                const float* const from = a.gate + (size_t)(b.row0 + q0 + 32 * warp) * a.g_ld + (size_t)head * a.g_hs;
+                const uint32_t to = base + 32 * warp * (D * 4);
+#pragma unroll 4
+                for (int e = lane; e < there * (D / 4); e += 32) cp_async16(to + e * 16, from + (size_t)(e / (D / 4)) * a.g_ld + e % (D / 4) * 4);
+                __syncwarp();
+            }
             const int lim = q0 + row - n * TK;   // last key of the tile that the row sees
             const bool hides = n * TK + TK - 1 > q0;
             if (hides) {
@@ -450,6 +451,8 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
         }
         ok = ok && warp_wait(smem_u32(&x.pv_done[(tiles - 1) & 1]), (tiles - 1) >> 1 & 1, a.err);
         tc_fence_after();
+        if (GATE) cp_async_wait_all();   // no copy outlives its thread
+        __syncwarp();
         asm volatile("bar.sync 1, 128;" ::: "memory");   // what all four warps took out; they all come here
         const float inv = l == 0.f ? 0.f : 1.f / l;
         if constexpr (SHARED) x.inv[row] = inv;
@@ -526,16 +529,7 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
             tc_commit(smem_u32(&x.fin[warp - 4]));
             ok = tc_wait(smem_u32(&x.fin[warp - 4]), 0, a.err) && ok;   // nothing in flight when the accumulator memory is given back
         }
-        if (GATE && warp == 4) {   // the gates of the block's rows in place of q and k
-            ok = __all_sync(0xffffffffu, ok);
-            gated = ok;
-            if (ok && tc_elect()) {
-                const int boxes = (min(TQ, b.T - q0) + 31) / 32;
-                mbar_expect_tx(smem_u32(&x.gates), boxes * 32 * D * 4);
-                for (int i = 0; i < boxes; ++i) tma3(base + i * (32 * D * 4), &mg, 0, head, b.row0 + q0 + 32 * i, smem_u32(&x.gates));
-            }
-            __syncwarp();
-        }
+        __syncwarp();   // the other lanes wait here: what follows takes whole warps
         if (G::COPIER && warp == 6 && tc_elect()) {
             int nk = 1, nv = 0, pk = 0, pv = 0;   // tile and part next to be fetched
             uint32_t idle = 0;
@@ -563,6 +557,7 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
             }
         }
     }
+    __syncwarp();
     if constexpr (SHARED) {   // all warps write
         if (!ok) x.failed = 1;
         tc_fence_before();
@@ -570,31 +565,31 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
         tc_fence_after();
         if (!x.failed) write_outputs(x.inv[32 * (warp & 3) + lane]);
     }
-    if (gated) tc_wait(smem_u32(&x.gates), 0, a.err);   // no copy outlives the CTA
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    tc_fence_after();
     if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(G::TMEM) : "memory");
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-// [R][heads][D] in boxes of `rows` x 64 dims of one head (gates, f32: all dims). Rows behind the tensor read as zeros
+// [R][heads][D] in boxes of `rows` x 64 dims of one head. Rows behind the tensor read as zeros
 int encode(EncodeFn f, CUtensorMap* m, const void* p, size_t ld, size_t hs, int R, int heads, int D, int rows, int type) {
-    const cuuint64_t size = type == OUT_F32 ? 4 : 2, dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)R}, strides[2] = {(heads == 1 ? D : hs) * size, (R == 1 ? D : ld) * size};
-    const cuuint32_t box[3] = {type == OUT_F32 ? (cuuint32_t)D : 64, 1, (cuuint32_t)rows}, step[3] = {1, 1, 1};
-    const CUresult r = f(m, type == OUT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, step,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, type == OUT_F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)R}, strides[2] = {(heads == 1 ? D : hs) * 2, (R == 1 ? D : ld) * 2};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)rows}, step[3] = {1, 1, 1};
+    const CUresult r = f(m, type == OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, step,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     HP_REQUIRE(r == CUDA_SUCCESS, "attn_prompt: rows that a tensor map cannot describe (%d): ld=%zu hs=%zu", (int)r, ld, hs);
     return HP_OK;
 }
-template <int D, typename T, bool GATE> int launch(const CUtensorMap (&m)[4], const PromptArgs& a, long long blocks, cudaStream_t s) {
+template <int D, typename T, bool GATE> int launch(const CUtensorMap (&m)[3], const PromptArgs& a, long long blocks, cudaStream_t s) {
     static bool attr[MAX_DEVICES] = {};   // per device: the opt-in belongs to the device's copy of the kernel
     const int dev = current_device(); if (dev < 0) return HP_ECUDA;
     if (!attr[dev]) { HP_CUDA(cudaFuncSetAttribute(k_attn_prompt<D, T, GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<D, GATE>::SMEM)); attr[dev] = true; }
-    HP_CUDA(launch_pdl<4>(k_attn_prompt<D, T, GATE>, dim3((unsigned)(blocks * a.n_head)), dim3(Geo<D, GATE>::THREADS), Geo<D, GATE>::SMEM, s, m[0], m[1], m[2], m[3], a));
+    HP_CUDA(launch_pdl<4>(k_attn_prompt<D, T, GATE>, dim3((unsigned)(blocks * a.n_head)), dim3(Geo<D, GATE>::THREADS), Geo<D, GATE>::SMEM, s, m[0], m[1], m[2], a));
     return HP_OK;
 }
-template <typename T, bool GATE> int launch(const CUtensorMap (&m)[4], const PromptArgs& a, long long blocks, int D, cudaStream_t s) {
+template <typename T, bool GATE> int launch(const CUtensorMap (&m)[3], const PromptArgs& a, long long blocks, int D, cudaStream_t s) {
     return D == 256 ? launch<256, T, GATE>(m, a, blocks, s) : D == 128 ? launch<128, T, GATE>(m, a, blocks, s) : launch<64, T, GATE>(m, a, blocks, s);
 }
 
@@ -611,11 +606,10 @@ int attn_prompt(const AttnPromptParams& p, cudaStream_t s) {
     const long long per = (p.max_rows + TQ - 1) / TQ, most = p.S * per, least = (long long)p.R / TQ + p.S, blocks = std::min(most, least);
     const int order = most <= least ? GRID : p.S <= 32 ? SORTED : ALONG;
     HP_REQUIRE(blocks * p.n_head < (1ll << 31), "attn_prompt: too many rows (%d) or heads for one call", p.R);
-    CUtensorMap m[4] = {};
+    CUtensorMap m[3] = {};
     int rc = encode(f, &m[0], p.q, p.q_ld, p.q_hs, p.R, p.n_head, p.head_dim, TQ, p.type);
     if (!rc) rc = encode(f, &m[1], p.k, p.k_ld, p.k_hs, p.R, p.n_kv, p.head_dim, p.head_dim == 256 ? Geo<256>::TK : Geo<128>::TK, p.type);
     if (!rc) rc = encode(f, &m[2], p.v, p.v_ld, p.v_hs, p.R, p.n_kv, p.head_dim, p.head_dim == 256 ? Geo<256>::VROWS : Geo<128>::VROWS, p.type);
-    if (!rc && p.gate) rc = encode(f, &m[3], p.gate, p.g_ld, p.g_hs, p.R, p.n_head, p.head_dim, 32, OUT_F32);
     if (rc) return rc;
     PromptArgs a; a.row_start = p.row_start; a.S = p.S; a.R = p.R; a.max_rows = p.max_rows; a.order = order; a.n_head = p.n_head; a.G = p.n_head / p.n_kv; a.scale2 = (float)((double)p.scale * 1.4426950408889634074);
     a.gate = p.gate; a.g_ld = p.g_ld; a.g_hs = p.g_hs; a.out = p.out; a.oq = (int8_t*)p.xq.q; a.osc = (float*)p.xq.sc; a.err = device_err_flag(); a.arg_err = device_arg_flag();

@@ -616,3 +616,25 @@ def test_prompts_beside_bad_row_starts_are_served(D, rs, there):
         n = 20 if rs[1:3] == [30, 20] else b - a
         assert torch.equal(got[a:a + n], K_.attn_prompt(q[a:b], k[a:b], v[a:b], i32([0, b - a]), max_rows=60)[0][:n]), (a, b)
     assert status() == 0
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_gated_prompts_over_and_over(kind, D):
+    """One wave of blocks whose last ones have few and odd rows, a sync behind each call, outputs in 16 bits and in int8, finite values and others in turn: the same bits every time."""
+    rows, H = [1234, 225, 1161, 984, 1135], 6
+    q, k, v = make(rows, H, 1, D, kind, 71, packed=False, up=0.2)
+    gate = torch.randn(q.shape, generator=gen(3), device="cuda")
+    rs, odd = starts(rows), v.clone()
+    for i in range(0, sum(rows), 371):
+        odd[i, 0, i % D] = (math.nan, math.inf, -math.inf)[i % 3]
+    first = {}
+    for i in range(200):
+        x = (v, odd)[i % 2]
+        out, xq = K_.attn_prompt(q, k, x, rs, max_rows=5000, gate=gate, want_q8=True)
+        assert status() == 0
+        bits = out.view(torch.int16)
+        want = first.setdefault(i % 2, (bits, *xq.unpack()))
+        assert torch.equal(bits, want[0]) and torch.equal(xq.unpack()[0], want[1])
+    hit = torch.cat([torch.where(torch.isfinite(t), 0, t).double().cumsum(0) for t in odd.split(rows)]).isfinite().expand(-1, H, -1)
+    assert torch.equal(first[0][0][hit], first[1][0][hit])
