@@ -368,10 +368,14 @@ __global__ void __launch_bounds__(Geo<D, GATE>::THREADS, Geo<D, GATE>::CTAS) k_a
             for (int i = 0; i < TK; i += 32) ld32(s + i, sc + i);
             ld_wait<TK>(s);
             if (GATE && n == tiles - 1) {   // the last scores are there, so nothing reads q and k any more: the gates of this warp's rows in their place, each thread its own copies
-                const float* const from = a.gate + (size_t)(b.row0 + q0 + 32 * warp) * a.g_ld + (size_t)head * a.g_hs;
-                const uint32_t to = base + 32 * warp * (D * 4);
+                constexpr int LPR = D / 4 < 32 ? D / 4 : 32, RPI = 32 / LPR;   // lanes of a row, rows of an instruction
+                const int j0 = lane / LPR, c0 = lane % LPR * 4;
+                const float* from = a.gate + (size_t)(b.row0 + q0 + 32 * warp + j0) * a.g_ld + (size_t)head * a.g_hs + c0;
+                uint32_t to = base + (32 * warp + j0) * (D * 4) + c0 * 4;
 #pragma unroll 4
-                for (int e = lane; e < there * (D / 4); e += 32) cp_async16(to + e * 16, from + (size_t)(e / (D / 4)) * a.g_ld + e % (D / 4) * 4);
+                for (int j = j0; j < there; j += RPI, from += RPI * a.g_ld, to += RPI * D * 4)
+#pragma unroll
+                    for (int c = 0; c < D; c += 128) cp_async16(to + c * 4, from + c);
                 __syncwarp();
             }
             const int lim = q0 + row - n * TK;   // last key of the tile that the row sees
