@@ -16,10 +16,10 @@
 //
 // A warp looks up the pages of all its slices at once, a lane each, and fetches a slice's scales with its keys; hidden keys are masked in the slices that have some.
 //
-// Measured (captured, us): one token of 24 heads of 256 over 4 at 4097 12.6 (bytes alone 1.3): start, four slices per warp and merge one after the other. 48 such sequences of up to
-// 8192 109 to 114 by card (80), 118 to 121 with the page looked up per slice, every slice masked, and blocks looked for where each sequence has one: issue slots 58 %, a third of the instructions turning codes into f16. 8 x 3 rows over 2 kv heads at 2051 22.0 (2.0); 32 x 2
-// rows of 32 heads of 128, window 1000, 34.6 (11): half of the instructions are starts and ends of the CTAs. Pairs as the 16 rows of the products: 260 for the 48 sequences; eight warps per CTA: 128.
-// 4 bits: one token at 4097 11.8 (0.7), the 48 sequences 100 (43), 64 of 32 heads of 128 over 8 at up to 12001 212 (86): issue slots 57 to 66 %; a slice takes 464 instructions at 128 dims, 675 at 256,
+// Measured (captured, us): one token of 24 heads of 256 over 4 at 4097 11.9 (bytes alone 1.3): start, four slices per warp and merge one after the other. 48 such sequences of up to
+// 8192 108 to 114 by card (80), 118 to 121 with the page looked up per slice, every slice masked, and blocks looked for where each sequence has one: issue slots 58 %, a third of the instructions turning codes into f16. 8 x 3 rows over 2 kv heads at 2051 21.3 (2.0); 32 x 2
+// rows of 32 heads of 128, window 1000, 32.5 (11): half of the instructions are starts and ends of the CTAs. Pairs as the 16 rows of the products: 260 for the 48 sequences; eight warps per CTA: 128.
+// 4 bits: one token at 4097 11.5 (0.7), the 48 sequences 100 (43), 64 of 32 heads of 128 over 8 at up to 12001 211 (86): issue slots 57 to 66 %; a slice takes 464 instructions at 128 dims, 675 at 256,
 // a warp and split some 850 and 1050 around them. Two dims become f16 by one mask and one fma; by two masks and conversions 129 for the 48. Products of tcgen05 with the pictures of attn_paged_tc.cu: 15.9 for one token, 180 for the 48;
 // a head's dims split over the warps, 64 keys shared by them: 13.1, 110.
 // Two sets of pairs spill up to 56 bytes a thread (4 bits, 64 dims; 8 bits 40), 256 dims and one set none.

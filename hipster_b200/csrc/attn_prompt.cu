@@ -14,11 +14,12 @@
 // A value that is infinite or NaN must not reach the rows in front of it through a weight of zero: in the tiles with hidden keys such elements are taken out of shared memory before the products. A weight being positive, a row has
 // NaN, infinity or minus infinity of all that it sees, so the first key of each kind is noted per dim, and outputs from that row on get it added on their way out.
 //
-// Measured (captured, back to back; cuBLAS' sustained rate is 1402 TFLOP/s): 8190 rows of 24 heads of 256 690 us, 1.19 PFLOP/s, at 1.44 GHz under the power limit (1560 us of 16384 rows of 16 heads after a pause, 1.41 PFLOP/s; 1790 back to
-// back). 16384 rows of 16 heads of 128 1060 us, 1.04 PFLOP/s at 1.6 GHz, of 64 800 us, 0.69 at 1.93. Bounds: 256 dims shared memory (320 KB per tile of 128 keys of 2048 clocks of products) and power; 128 and 64 the weights' warps, two
-// per scheduler, some 1300 clocks per 64 keys each. Seven prompts of up to 3001 rows of 32 heads of 128 264 to 295 us (by card): of a CTA's 37000 clocks 6000 pass before its first scores are there, 2700 with its outputs. Five gated
-// prompts of up to 77 rows of 24 heads of 256 10.3 us: 400 KB of a CTA at some 64 bytes a clock, and latency. Gates come in place of q and k while the last weights are formed, and at 256 dims all eight warps write outputs: with gates fetched
-// into registers by the four weights' warps, a step ahead, 13.3, and 8 x 600 rows of 16 heads 92.7 instead of 78.2; without gates four warps, or eight, take the same.
+// Measured (captured; cuBLAS' burst rate is 1655 TFLOP/s, its sustained one 1402): 8190 rows of 24 heads of 256 605 to 630 us in threes, 1.31 to 1.36 PFLOP/s; 715 to 740 one behind the other for longer, 1.12 to 1.16, at some
+// 1.44 GHz under the power limit. 16384 rows of 16 heads of 256 1526 us (1.44 PFLOP/s), of 128 946 (1.16), of 64 803 (0.68). Bounds: 256 dims shared memory (320 KB per tile of 128 keys of 2048 clocks of products) and power; 128
+// and 64 the weights' warps, two per scheduler, some 1300 clocks per 64 keys each. Seven prompts of up to 3001 rows of 32 heads of 128 250 to 300 us (by card and power): of a CTA's 37000 clocks 6000 pass before its first scores are
+// there, 2700 with its outputs. Five gated prompts of up to 77 rows of 24 heads of 256 11.1 us: 400 KB of a CTA at some 64 bytes a clock, and latency. Gates come in place of q and k while the last weights are formed, each warp's by its own threads,
+// and at 256 dims all eight warps write outputs: with gates fetched into registers by the four weights' warps, a step ahead, 13.3, and 8 x 600 rows of 16 heads 92.7 instead of 74; without gates four warps, or eight, take the same.
+// Int8 outputs go 32 dims at a time through exchanges of eight lanes, row by row: 8 x 600 rows of 16 heads of 256 159 us, in 16 bits 55.
 // Tried: one warp for both products 1119 us at 128 dims where two take 1080 (a wait that is over still takes 250 clocks, and an output waited behind the next scores'); waits that ask without a pause in those warps: they take the
 // issue slots of the weights' warp beside them (2360 -> 3440 clocks per tile); a quarter, a half of the exponentials as polynomials on the fp32 pipe: 1732 -> 1762, 1802 us at 256 dims, 819 -> 827, 892 at 64 (instructions, not the
 // special functions, bound them); outputs unrolled over a row: 14800 clocks instead of 5800, cold instructions.

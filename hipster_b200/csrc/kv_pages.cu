@@ -186,7 +186,7 @@ __device__ __forceinline__ void angles(float2 (&cs)[8], const float* rope, const
 // heads (n_head query heads, then n_kv key heads, then n_kv value heads) in a loop that fetches a set ahead. The row's place and angles are found once. Four prompts of
 // up to 1000 rows of 48 heads of 128, normalised: 26 us, 73 MB of DRAM traffic, 95 instructions per head (with a warp per head and the loop unrolled four times 220, which did not fit the instruction cache). Neither issue
 // slots (56 %) nor memory (3.3 TB/s) are used up: the warps, 43 % of what an SM holds, wait for their next set of heads (4.6 of them at a time). One row of 32 heads of 256 3.3 us, latency.
-// AXES: positions of several axes. 4 bits: four lanes share a group; its range takes four exchanges, the largest range of the head the others. The same four prompts of 48 heads of 128 with three axes 28.2 us, to 4 bits 30.5;
+// AXES: positions of several axes. 4 bits: four lanes share a group; its range takes four exchanges, the largest range of the head the others. The same four prompts of 48 heads of 128 with three axes 28.3 us, to 4 bits 30.5 to 31, at the rows' places 29.2;
 // 160 instructions per head, issue slots 58 %, otherwise waiting for exchanges and rows, in 1.6 waves of blocks. 8 x 3 rows of 24 + 4 heads of 256 3.75, latency.
 template <int D, int KIND, bool AXES>
 __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch b, KvAppendParams p, RopeAxes axes, int hpw, int* err) {
@@ -312,8 +312,8 @@ __global__ void __launch_bounds__(256, 4) k_kv_append(PagedPool pool, PagedBatch
 }
 
 // RB rows per block, RB / 8 of them found by each warp; thread = 16 neighbouring codes of a row, a head and k or v, times the scale, rounded to f16 once. The e4m3
-// patterns 0x7f and 0xff, which the quantiser does not write, read as 480 and -480. Bound by memory: 16 caches of up to 5000 tokens of 8 x 128 67 us (322 MB, 4.8 TB/s; pages of 16
-// tokens are runs of 2 KB), with one piece in flight per thread 88; 4096 tokens of 4 x 256 7.4 us. 4 bits: a word of 8 codes per piece, eight pieces in flight; bound by instructions (issue slots 76 %, 214 MB of it written or read):
+// patterns 0x7f and 0xff, which the quantiser does not write, read as 480 and -480. Bound by memory: 16 caches of up to 5000 tokens of 8 x 128 66 us (322 MB, 4.9 TB/s; pages of 16
+// tokens are runs of 2 KB), with one piece in flight per thread 88; 4096 tokens of 4 x 256 7.4 us. 4 bits: a word of 8 codes per piece, eight pieces in flight; bound by instructions (issue slots 78 %, 214 MB of it written or read):
 // the same caches 61 us, 4096 tokens 7.2. Where a row's codes lie, looked up once per row in shared memory: 63.8.
 template <int D, int KIND, int RB>
 __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, __half* __restrict__ ko, __half* __restrict__ vo, size_t row_stride, size_t head_stride, int* err) {
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(256) k_kv_read(PagedPool pool, PagedBatch b, _
 }
 
 // Rows of q, k and v, each head's norm and rotation, to outputs of another type: what k_kv_append does for rows that stay rows. The same lanes, sets of heads and loop. Bound by memory: 8403 rows of 48 heads of 128 with
-// three axes to bf16 59.7 us, 310 MB (5.2 TB/s; copies 6.5), of which the rows' own start, behind their positions, hides under other warps' heads; 48 rows of 32 heads of 256 3.6 us, latency.
+// three axes to bf16 58.7 us, 310 MB (5.3 TB/s; copies 6.5); the rows' own start, behind their positions, hides under other warps' heads. To f32 11 % more. 48 rows of 32 heads of 256 3.6 us, latency.
 template <int D, typename T>
 __global__ void __launch_bounds__(256, 4) k_rope_rows(RopeRowsParams p, RopeAxes axes, int hpw, int* err) {
     constexpr int LPH = D / 8, HPS = 32 / LPH;
